@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define TATTN_ABI_VERSION 3
+#define TATTN_ABI_VERSION 4
 
 #if defined(__GNUC__)
 #define TATTN_API __attribute__((visibility("default")))
@@ -107,6 +107,29 @@ TATTN_API int tattn_bwd_fused(const void* q, const void* k, const void* v, const
 /* Bytes of the workspace tattn_bwd_fused needs for a [Z, H, N, D] call (a multiple of 16), or -1 for
  * invalid dimensions. */
 TATTN_API int64_t tattn_bwd_fused_workspace_bytes(int Z, int H, int N, int D);
+
+/* Sliding-window attention with sinks (no reference counterpart). Query i of Nq stands at position p = Nk - Nq
+ * + i of a sequence of Nk >= Nq tokens and sees the keys j <= p that are among the last `window` ones (j >
+ * p - window, window >= 1) or the first `sinks` (j < sinks, sinks >= 0); every query sees its own key. K and V
+ * have Hk heads, each shared by H / Hk consecutive query heads (Hk divides H).
+ * strides: 16 int64 = q, k, v, o each (z, h, n, d). m: dense fp32 [Z, H, Nq]. */
+TATTN_API int tattn_window_fwd(const void* q, const void* k, const void* v, void* o, float* m, const int64_t* strides,
+                     int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window, int sinks, float sm_scale,
+                     void* stream);
+
+/* Its backward: delta = rowsum(dO * O), dq [Z, H, Nq, D], and dk, dv [Z, Hk, Nk, D], summed over the query heads
+ * that share a head; all dense. strides: 20 int64 = q, k, v, o, dout each (z, h, n, d). delta: fp32 [Z, H,
+ * Nq]. workspace: tattn_window_bwd_workspace_bytes bytes, 16-byte aligned (fp32: 0 bytes, may be null). fp16
+ * sums dq by fp32 additions in the workspace in an order that varies from run to run, as tattn_bwd_fused;
+ * dk and dv, and everything in fp32, are bitwise reproducible. */
+TATTN_API int tattn_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, void* dq,
+                     void* dk, void* dv, const float* m, float* delta, void* workspace, const int64_t* strides,
+                     int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window, int sinks, float sm_scale,
+                     void* stream);
+
+/* Bytes of the workspace that tattn_window_bwd needs, or -1 for invalid arguments. */
+TATTN_API int64_t tattn_window_bwd_workspace_bytes(int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window,
+                                         int sinks);
 
 /* Largest Z*H*N accepted by tattn_bwd_noalloc (its fixed fp32 row buffer: 16 MiB per GPU). */
 #define TATTN_BWD_NOALLOC_MAX_ROWS 4194304

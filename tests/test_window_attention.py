@@ -1,0 +1,273 @@
+"""``tattn.window_attention``: refusals and host arithmetic without a GPU; outputs and gradients on a B200
+against the definition in 64 bits, against differences, and against ``tattn.attention`` where both apply."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import tattn
+from tattn import _lib, attention, window_attention
+from tattn.window import _backward, _forward
+from tests.plain64 import assert_within, window_attention64
+
+
+def _qkv(b, h, hk, nq, nk, d, dtype, seed, layout="bhnd", device="cuda"):
+    g = torch.Generator().manual_seed(seed)
+
+    def make(heads, n):
+        if layout == "bnhd":
+            return torch.randn((b, n, heads, d), generator=g).to(dtype).to(device).transpose(1, 2)
+        return torch.randn((b, heads, n, d), generator=g).to(dtype).to(device)
+
+    return make(h, nq), make(hk, nk), make(hk, nk), make(h, nq)
+
+
+# ------------------------------------------------------------------------------------ without a GPU
+def _cpu(*shape, dtype=torch.float16):
+    return torch.zeros(shape, dtype=dtype)
+
+
+@pytest.mark.parametrize(
+    "q, k, v, window, sinks, message",
+    [
+        (_cpu(1, 4, 8), _cpu(1, 2, 8, 16), _cpu(1, 2, 8, 16), 4, 0, "expected q"),
+        (_cpu(1, 4, 8, 16), _cpu(1, 2, 8, 16), _cpu(1, 2, 9, 16), 4, 0, "expected q"),
+        (_cpu(2, 4, 8, 16), _cpu(1, 2, 8, 16), _cpu(1, 2, 8, 16), 4, 0, "agree in batch"),
+        (_cpu(1, 4, 8, 16), _cpu(1, 2, 8, 32), _cpu(1, 2, 8, 32), 4, 0, "agree in batch"),
+        (_cpu(1, 4, 8, 16), _cpu(1, 3, 8, 16), _cpu(1, 3, 8, 16), 4, 0, "multiple"),
+        (_cpu(1, 4, 8, 16), _cpu(1, 0, 8, 16), _cpu(1, 0, 8, 16), 4, 0, "multiple"),
+        (_cpu(1, 4, 8, 48), _cpu(1, 2, 8, 48), _cpu(1, 2, 8, 48), 4, 0, "head dim"),
+        (_cpu(1, 4, 8, 16), _cpu(1, 2, 8, 16), _cpu(1, 2, 8, 16, dtype=torch.float32), 4, 0, "dtype"),
+        (*[_cpu(1, 2, 8, 16, dtype=torch.bfloat16)] * 3, 4, 0, "dtype"),
+        (_cpu(1, 4, 8, 16), _cpu(1, 2, 8, 16), _cpu(1, 2, 8, 16), 0, 0, "window"),
+        (_cpu(1, 4, 8, 16), _cpu(1, 2, 8, 16), _cpu(1, 2, 8, 16), 4, -1, "sinks"),
+        (_cpu(1, 4, 8, 16), _cpu(1, 2, 7, 16), _cpu(1, 2, 7, 16), 4, 0, "last of the keys"),
+    ],
+)
+def test_refusals(q, k, v, window, sinks, message) -> None:
+    with pytest.raises(ValueError, match=message):
+        window_attention(q, k, v, window, sinks)
+
+
+def test_no_cpu_path() -> None:
+    x = _cpu(1, 2, 8, 16)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        window_attention(x, x, x, 4)
+
+
+def test_abi_refuses_before_any_device_call() -> None:
+    lib = _lib.load()
+    s = _lib.strides_array(*[(8 * 16, 8 * 16, 16, 1)] * 5)
+    dims = dict(z=1, h=2, hk=2, nq=8, nk=8, d=16, dtype=0, window=4, sinks=0)
+    for bad in (dict(d=24), dict(hk=0), dict(hk=3), dict(nk=7), dict(window=0), dict(sinks=-1), dict(dtype=2), dict(z=-1)):
+        a = (dims | bad).values()
+        assert lib.tattn_window_fwd(16, 16, 16, 16, 16, s, *a, 0.1, None) == _lib.ERR_INVALID_ARGUMENT
+        assert lib.tattn_window_bwd(*[16] * 11, s, *a, 0.1, None) == _lib.ERR_INVALID_ARGUMENT
+        assert lib.tattn_window_bwd_workspace_bytes(*a) == -1
+    # No queries of no batch: nothing to do.
+    assert lib.tattn_window_fwd(None, None, None, None, None, s, *(dims | dict(z=0)).values(), 0.1, None) == 0
+
+
+def test_workspace_size() -> None:
+    """The fp32 dQ rows and 16 bytes, and partial dV and dK of the sink tiles where they are cut."""
+    size = _lib.load().tattn_window_bwd_workspace_bytes
+    assert size(2, 4, 2, 1000, 1000, 64, 0, 100, 0) == 2 * 4 * 1000 * 64 * 4 + 16
+    # 1000 queries are 8 blocks of 128; a window of 100 spans at most ceil(227 / 128) + 1 = 3: 3 chunks.
+    assert size(2, 4, 2, 1000, 1000, 64, 0, 100, 4) == 2 * 4 * 1000 * 64 * 4 + 16 + 2 * 2 * 1 * 3 * 2 * 128 * 64 * 4
+    assert size(2, 4, 2, 1000, 1000, 64, 0, 1000, 4) == 2 * 4 * 1000 * 64 * 4 + 16  # one chunk: no partials
+    assert size(2, 4, 2, 1000, 1000, 64, 1, 100, 4) == 0  # fp32 needs none
+
+
+# -------------------------------------------------------------------------------------- on a B200
+@pytest.fixture
+def gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    yield
+    assert _lib.device_status() == 0  # no bounded wait ran out
+
+
+def _check(b, h, hk, nq, nk, d, window, sinks, dtype, seed=0, layout="bhnd", scale=None):
+    q, k, v, do = _qkv(b, h, hk, nq, nk, d, dtype, seed, layout)
+    for t in (q, k, v):
+        t.requires_grad_()
+    o = window_attention(q, k, v, window, sinks, scale)
+    got = (o, *torch.autograd.grad(o, (q, k, v), do))
+    want, bounds = window_attention64(q, k, v, do, window, sinks, 1 / math.sqrt(d) if scale is None else scale)
+    for g, w, e, name in zip(got, want, bounds, ("o", "dq", "dk", "dv"), strict=True):
+        assert g.dtype == dtype
+        assert_within(g, w, e, name)
+
+
+SHAPES = [
+    # b, h, hk, nq, nk, window, sinks
+    (1, 1, 1, 1, 1, 1, 0),
+    (2, 2, 1, 1, 40, 7, 3),
+    (1, 2, 2, 17, 17, 1, 0),  # every query sees itself alone
+    (1, 2, 2, 33, 33, 1, 1),
+    (2, 6, 2, 70, 70, 16, 4),
+    (1, 3, 3, 128, 128, 128, 0),
+    (1, 2, 1, 129, 129, 128, 1),
+    (1, 4, 2, 300, 300, 64, 4),
+    (1, 2, 2, 300, 300, 129, 128),
+    (1, 2, 2, 700, 700, 100, 130),  # sinks end in the second tile, cut into chunks
+    (1, 2, 2, 700, 700, 100, 600),  # sinks past most windows
+    (2, 5, 1, 260, 515, 127, 2),  # queries begin inside a block
+    (1, 2, 1, 40, 700, 50, 4),  # keys that no query sees
+    (1, 2, 1, 100, 1000, 300, 200),
+    (1, 2, 2, 200, 200, 10**9, 10**9),  # longer than the keys
+    (3, 5, 5, 1000, 1000, 200, 4),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["f16", "f32"])
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_against_the_definition(gpu, shape, d, dtype) -> None:
+    b, h, hk, nq, nk, window, sinks = shape
+    _check(b, h, hk, nq, nk, d, window, sinks, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("window, sinks", [(512, 4), (777, 130), (1500, 0), (64, 33)])
+def test_longer_sequences(gpu, window, sinks, d) -> None:
+    _check(1, 4, 2, 2500, 2500, d, window, sinks, torch.float16)
+    _check(1, 4, 2, 1100, 2500, d, window, sinks, torch.float16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["f16", "f32"])
+@pytest.mark.parametrize("scale", [0.3, -0.2, 0.0])
+def test_scales(gpu, scale, dtype) -> None:
+    _check(1, 4, 2, 300, 333, 64, 90, 4, dtype, scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["f16", "f32"])
+def test_transposed_layout_is_read_in_place(gpu, dtype) -> None:
+    _check(2, 6, 3, 200, 290, 64, 70, 5, dtype, layout="bnhd")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["f16", "f32"])
+def test_layouts_that_need_a_copy(gpu, dtype) -> None:
+    """Odd strides, a base that no 16-byte load reaches and a broadcast dO give the dense tensors' results."""
+    b, h, hk, n, d = 1, 4, 2, 150, 64
+    q, k, v, _ = _qkv(b, h, hk, n, n, d, dtype, 3)
+    odd = torch.empty((b, h, n, d + 1), device="cuda", dtype=dtype)[..., 1:].copy_(q)
+    do = torch.randn((b, h, 1, d), device="cuda").to(dtype).expand(b, h, n, d)
+    args = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+    want = window_attention(*args, 40, 4)
+    want_g = torch.autograd.grad(want, args, do.contiguous())
+    odd.requires_grad_()
+    got = window_attention(odd, args[1], args[2], 40, 4)
+    assert torch.equal(got, want)
+    got_g = torch.autograd.grad(got, (odd, args[1], args[2]), do)
+    assert torch.equal(got_g[1], want_g[1]) and torch.equal(got_g[2], want_g[2])
+    torch.testing.assert_close(got_g[0], want_g[0], atol=2e-3, rtol=2e-3)  # fp16 dQ sums in varying order
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_window_of_everything_is_causal_attention(gpu, d) -> None:
+    q, k, v, do = _qkv(1, 3, 3, 400, 400, d, torch.float16, 5)
+    ref = [t.clone().requires_grad_() for t in (q, k, v)]
+    own = [t.clone().requires_grad_() for t in (q, k, v)]
+    a, b = attention(*ref, causal=True), window_attention(*own, 400)
+    torch.testing.assert_close(a, b, atol=2e-3, rtol=2e-3)
+    for x, y in zip(torch.autograd.grad(a, ref, do), torch.autograd.grad(b, own, do), strict=True):
+        torch.testing.assert_close(x, y, atol=2e-3, rtol=2e-3)
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences(gpu) -> None:
+    """fp32: d/de of sum(O * dO) along random directions by central differences. With e = 2e-3 the third
+    derivative's part is of the order e^2 and the rounding of O about 2^-24 / e, both below 1e-3 of the
+    slope's scale (the root of the number of summed products)."""
+    q, k, v, do = _qkv(1, 4, 2, 90, 120, 32, torch.float32, 9)
+    args = [t.clone().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(window_attention(*args, 30, 3), args, do)
+    e = 2e-3
+    for i, t in enumerate((q, k, v)):
+        direction = torch.randn(t.shape, generator=torch.Generator().manual_seed(i)).cuda()
+        values = []
+        for sign in (1, -1):
+            moved = [x + sign * e * direction if j == i else x for j, x in enumerate((q, k, v))]
+            values.append((window_attention(*moved, 30, 3).double() * do.double()).sum())
+        slope = float((values[0] - values[1]) / (2 * e))
+        want = float((grads[i].double() * direction.double()).sum())
+        size = float(grads[i].double().norm())
+        assert abs(slope - want) <= 1e-3 * max(size, abs(want)), (i, slope, want, size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_dk_and_dv_do_not_vary(gpu, d) -> None:
+    """Cut sink tiles are summed in a fixed order: dK and dV are bitwise the same each time."""
+    q, k, v, do = _qkv(2, 4, 2, 900, 900, d, torch.float16, 11)
+    o, m = _forward(q, k, v, 100, 130, 0.125)
+    first = _backward(q, k, v, o, m, do, 100, 130, 0.125)
+    for _ in range(3):
+        again = _backward(q, k, v, o, m, do, 100, 130, 0.125)
+        assert torch.equal(first[1], again[1]) and torch.equal(first[2], again[2])
+
+
+@pytest.mark.gpu
+def test_log_sum_exp(gpu) -> None:
+    q, k, v, _ = _qkv(1, 2, 1, 200, 330, 64, torch.float16, 12)
+    _, m = _forward(q, k, v, 50, 3, 0.125)
+    x = q.double() @ k.repeat_interleave(2, 1).double().transpose(-1, -2) * 0.125
+    from tests.plain64 import visible
+
+    x = x.masked_fill(~visible(200, 330, 50, 3, "cuda"), -math.inf)
+    want = torch.logsumexp(x, -1) / math.log(2)
+    torch.testing.assert_close(m.double(), want, atol=1e-3, rtol=0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["f16", "f32"])
+def test_large_scores(gpu, dtype) -> None:
+    """Scores of some hundreds: one key takes nearly all the weight, and the first block that a row sees may
+    hold none of its keys. The output is a convex combination of rows of V."""
+    q, k, v, _ = _qkv(1, 2, 1, 300, 300, 64, dtype, 13)
+    o = window_attention(20 * q, k, v, 30, 2)
+    assert bool(torch.isfinite(o).all())
+    want, _ = window_attention64(20 * q, k, v, torch.zeros_like(q), 30, 2, 0.125)
+    # 20 q doubles the exponent's size about 20 times over: its error, 2^-21 of some 300, is below 2e-4.
+    torch.testing.assert_close(o.double(), want[0], atol=4e-3, rtol=4e-3)
+
+
+@pytest.mark.gpu
+def test_no_queries(gpu) -> None:
+    q, k, v, do = _qkv(2, 2, 1, 0, 50, 64, torch.float16, 14)
+    for t in (q, k, v):
+        t.requires_grad_()
+    o = window_attention(q, k, v, 8, 2)
+    assert o.shape == q.shape
+    dq, dk, dv = torch.autograd.grad(o, (q, k, v), do)
+    assert dq.shape == q.shape and not bool(dk.any()) and not bool(dv.any())
+
+
+@pytest.mark.gpu
+def test_side_stream_and_once_differentiable(gpu) -> None:
+    q, k, v, do = _qkv(1, 4, 2, 500, 500, 64, torch.float16, 15)
+    want = window_attention(q, k, v, 100, 4)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = window_attention(q, k, v, 100, 4)
+    side.synchronize()
+    assert torch.equal(got, want)
+    args = [t.clone().requires_grad_() for t in (q, k, v)]
+    (g,) = torch.autograd.grad(window_attention(*args, 100, 4), args[:1], do.requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_public_name() -> None:
+    assert tattn.window_attention is window_attention and "window_attention" in tattn.__all__

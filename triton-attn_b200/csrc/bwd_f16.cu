@@ -1757,6 +1757,10 @@ cudaError_t dkdv_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
 //     accumulated in TMEM by its own MMAs; the compute warps read it one block later, right after
 //     handing over the next block's P^T/dS^T (the dQ MMAs of that block wait for the read: dq_read),
 //     and add it into a dense fp32 workspace through TMA tensor reduce-adds (one 32 x 32 box per warp).
+//   * kMaskWindow: a unit is a key tile of one key/value head with the query blocks that see it, once for
+//     every query head that shares the head, so dK and dV are summed over those heads in TMEM. The tiles
+//     with sinks, which all later queries see, are cut into units of about a window's length (WindowSplit);
+//     each writes fp32 partial dV and dK, which the last phase sums in a fixed order.
 //   * After its last tile every CTA (a cooperative launch of at most one CTA per SM) waits at a grid
 //     barrier for all reduce-adds, then its compute warps scale a share of the workspace by sm_scale
 //     into the fp16 dQ.
@@ -1930,7 +1934,55 @@ __device__ __forceinline__ void fused_dq_epilogue(const BwdArgs& a, int nthreads
   }
 }
 
-template <int D, bool CAUSAL>
+// Last phase of a window backward whose sink tiles were cut: dV and dK of those tiles, 8 elements a
+// thread, as the sum of the chunks' partials in their order (dK times sm_scale).
+template <int D>
+__device__ __forceinline__ void fused_part_epilogue(const BwdArgs& a, int nthreads) {
+  unsigned t, cta;
+  asm volatile("mov.u32 %0, %%tid.x;" : "=r"(t));
+  asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(cta));
+  constexpr int kRow = D / 8, kTile = 128 * kRow;  // groups of 8 elements
+  const int64_t n8 = int64_t(a.Z) * a.win.Hk * a.split.tiles * 2 * kTile;
+  for (int64_t i = int64_t(cta) * nthreads + t; i < n8; i += int64_t(gridDim.x) * nthreads) {
+    const int e = int(i % kTile), which = int(i / kTile % 2);  // 0: dV, 1: dK
+    const int64_t tile = i / (2 * kTile);                      // head-major
+    const int key = int(tile % a.split.tiles) * 128 + e / kRow;
+    if (key >= a.win.Nk) continue;
+    const float4* p = reinterpret_cast<const float4*>(a.part) + 2 * ((tile * a.split.chunks * 2 + which) * kTile + e);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+    for (int c = 0; c < a.split.chunks; ++c, p += 4 * kTile) {
+      const float4 u = __ldcg(p), v = __ldcg(p + 1);
+      x = make_float4(x.x + u.x, x.y + u.y, x.z + u.z, x.w + u.w);
+      y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
+    }
+    const float sc = which ? a.sm_scale : 1.f;
+    uint4* out = static_cast<uint4*>(which ? a.dk : a.dv) + ((tile / a.split.tiles) * a.win.Nk + key) * kRow + e % kRow;
+    *out = make_uint4(pack_half2(x.x * sc, x.y * sc), pack_half2(x.z * sc, x.w * sc), pack_half2(y.x * sc, y.y * sc),
+                      pack_half2(y.z * sc, y.w * sc));
+  }
+}
+
+// One unit of a CTA's work in the fused backward: key tile kt of key/value head hk, and the query blocks
+// [lo, lo + nb) of each of the query heads h0, h0 + 1, ... : n blocks in all, head by head.
+struct Unit {
+  int zi, hk, h0, kt, lo, nb, n;
+  int chunk;  // kMaskWindow: of a cut sink tile, else -1
+};
+// The (query head, query block) pairs of a unit in order. Not kMaskWindow: one head, blocks ascending.
+template <bool WINDOW>
+struct UnitWalk {
+  int h, blk;
+  __device__ __forceinline__ explicit UnitWalk(const Unit& u) : h(u.h0), blk(u.lo) {}
+  __device__ __forceinline__ void next(const Unit& u) {
+    ++blk;
+    if (WINDOW && blk == u.lo + u.nb) {
+      blk = u.lo;
+      ++h;
+    }
+  }
+};
+
+template <int D, int MASK>
 __global__ void __launch_bounds__(kThreads, 1)
     bwd_fused_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
@@ -1939,6 +1991,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = FusedCfg<D>;
   using G = Geo<D>;
   constexpr int H = C::H, BQ = C::BQ, NS = C::NS;
+  constexpr bool CAUSAL = MASK == kMaskCausal, WINDOW = MASK == kMaskWindow;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
   const uint32_t base_u32 = (raw_u32 + 1023u) & ~1023u;
@@ -1966,8 +2019,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int N = args.N;
-  const int zh = args.Z * args.H;
-  const int nct = (N + 127) / 128;
+  const int Nk = WINDOW ? args.win.Nk : N;
+  const int zh = args.Z * (WINDOW ? args.win.Hk : args.H);  // key/value heads
+  const int nct = (Nk + 127) / 128;
   const int ntiles = nct * zh;
   const int NBq = (N + BQ - 1) / BQ;
   // Query blocks of key tile kt: [lo, NBq) (causal: from the diagonal block on).
@@ -1979,7 +2033,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // unit first. Equal units balance the CTAs, and the tiles running at any time belong to a few
   // neighbouring heads, so their fp32 dQ workspace rows and Q/dO blocks are shared in L2 (ordering the
   // tiles longest-first across all heads instead spreads 148 CTAs over ~148 heads, whose workspaces miss
-  // L2: ~10x the algorithmic DRAM traffic at N = 8192 with 1,024 heads).
+  // L2: ~10x the algorithmic DRAM traffic at N = 8192 with 1,024 heads). kMaskWindow: window_unit below.
   const int n_units = CAUSAL ? zh * ((nct + 1) / 2) : ntiles;
   auto next_tile = [&](int2& seq, int* bh, int* kt) -> bool {  // seq = (unit, second tile of the unit)
     if (seq.x >= n_units) return false;
@@ -1997,6 +2051,47 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
       seq.y = 1;
     }
+    return true;
+  };
+
+  // kMaskWindow: of each key/value head, the chunks of the sink tiles, then the other tiles; these units
+  // cost about the same and are taken round-robin. A tile may have no query blocks (n = 0) where the
+  // queries begin after its window, and a chunk none where its tile's queries begin later.
+  auto window_unit = [&](int2& seq, Unit* u) -> bool {
+    const int cut = args.split.tiles * args.split.chunks, per_head = cut + nct - args.split.tiles;
+    if (seq.x >= zh * per_head) return false;
+    const int bh = seq.x / per_head, p = seq.x % per_head;
+    seq.x += int(gridDim.x);
+    u->zi = bh / args.win.Hk;
+    u->hk = bh % args.win.Hk;
+    u->h0 = u->hk * args.win.group;
+    const bool sink = p < cut;
+    u->kt = sink ? p / args.split.chunks : p - cut + args.split.tiles;
+    const int k0 = 128 * u->kt, first = max(0, k0 - args.win.off) / BQ;  // first block with a query at k0 or later
+    // The last query that sees key k0 + 127 is at position k0 + 127 + window - 1.
+    const int last = k0 + 126 + args.win.window - args.win.off;
+    int end = sink ? NBq : last < 0 ? 0 : min(NBq, last / BQ + 1);
+    u->lo = first;
+    u->chunk = -1;
+    if (sink && args.split.chunks > 1) {
+      u->chunk = p % args.split.chunks;
+      u->lo = first + u->chunk * args.split.blocks;
+      end = min(NBq, u->lo + args.split.blocks);
+    }
+    u->nb = max(0, end - u->lo);
+    u->n = u->nb * args.win.group;
+    return true;
+  };
+  auto next_unit = [&](int2& seq, Unit* u) -> bool {
+    if (WINDOW) return window_unit(seq, u);
+    int bh, kt;
+    if (!next_tile(seq, &bh, &kt)) return false;
+    u->zi = bh / args.H;
+    u->hk = u->h0 = bh % args.H;
+    u->kt = kt;
+    u->lo = tile_lo(kt);
+    u->n = u->nb = NBq - u->lo;
+    u->chunk = -1;
     return true;
   };
 
@@ -2058,23 +2153,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       int g = 0, it = 0, kv_issued = 0;
       bool ok = true;
       int2 seq = make_int2(int(blockIdx.x), 0);
-      for (int bh, kt; ok && next_tile(seq, &bh, &kt); ++it) {
-        const int zi = bh / args.H, hi = bh % args.H, k0 = 128 * kt, lo = tile_lo(kt), n = NBq - lo;
+      for (Unit u; ok && next_unit(seq, &u); ++it) {
+        const int zi = u.zi, k0 = 128 * u.kt, n = u.n;
         const int kb = it & 1;
         if (it >= 2 && !warp_wait(&bar_kv_empty[kb], ((it >> 1) - 1) & 1, ab)) { ok = false; break; }
         if (lane == 0) {
           mbar_arrive_expect_tx(&bar_kv_full[kb], C::T_KEY);
           for (int ch = 0; ch < G::NCH; ++ch)
-            tma_load_4d(sK + kb * C::T_KEY + ch * G::chunk(128), &tm_k, ch * G::CW, k0, hi, zi, &bar_kv_full[kb]);
+            tma_load_4d(sK + kb * C::T_KEY + ch * G::chunk(128), &tm_k, ch * G::CW, k0, u.hk, zi, &bar_kv_full[kb]);
         }
         ++kv_issued;
-        const float* mrow = args.m + int64_t(bh) * N;
-        const float* drow = args.delta + int64_t(bh) * N;
         const float inv_scale = 1.f / fold_scale(args.qk_scale);
-        for (int c = 0; c < n; ++c, ++g) {
+        UnitWalk<WINDOW> at(u);
+        for (int c = 0; c < n; ++c, ++g, at.next(u)) {
           const int st = g % NS;
           if (g >= NS && !warp_wait(&bar_q_empty[st], ((g / NS) - 1) & 1, ab)) { ok = false; break; }
-          const int qr = (lo + c) * BQ;
+          const int qr = at.blk * BQ, hi = at.h;
+          const float* mrow = args.m + (int64_t(zi) * args.H + hi) * N;
+          const float* drow = args.delta + (int64_t(zi) * args.H + hi) * N;
           if (lane == 0) {
             mbar_arrive_expect_tx(&bar_q_full[st], 2 * C::T_Q);
             for (int ch = 0; ch < G::NCH; ++ch) {
@@ -2118,8 +2214,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       int g = 0, it = 0;
       bool ok = true;
       int2 seq = make_int2(int(blockIdx.x), 0);
-      for (int bh, kt; ok && next_tile(seq, &bh, &kt); ++it) {
-        const int n = NBq - tile_lo(kt);
+      for (Unit u; ok && next_unit(seq, &u); ++it) {
+        const int n = u.n;
         const int kb = it & 1;
         if (!warp_wait(&bar_kv_full[kb], (it >> 1) & 1, ab) || !warp_wait(bar_v_full, it & 1, ab)) {
           ok = false;
@@ -2158,8 +2254,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       int g = 0, it = 0;
       bool ok = true;
       int2 seq = make_int2(int(blockIdx.x), 0);
-      for (int bh, kt; ok && next_tile(seq, &bh, &kt); ++it) {
-        const int n = NBq - tile_lo(kt);
+      for (Unit u; ok && next_unit(seq, &u); ++it) {
+        const int n = u.n;
         const int kb = it & 1;
         const uint64_t ko = uint64_t((kb * C::T_KEY) >> 4);
         // The accumulators are overwritten by this tile's first MMAs: the previous tile's epilogue
@@ -2215,12 +2311,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       int it = 0, v_issued = 0;
       bool ok = true;
       int2 seq = make_int2(int(blockIdx.x), 0);
-      for (int bh, kt; ok && next_tile(seq, &bh, &kt); ++it) {
+      for (Unit u; ok && next_unit(seq, &u); ++it) {
         if (it >= 1 && !warp_wait(bar_v_empty, (it - 1) & 1, ab)) { ok = false; break; }
         if (lane == 0) {
           mbar_arrive_expect_tx(bar_v_full, C::T_KEY);
           for (int ch = 0; ch < G::NCH; ++ch)
-            tma_load_4d(sV + ch * G::chunk(128), &tm_v, ch * G::CW, 128 * kt, bh % args.H, bh / args.H, bar_v_full);
+            tma_load_4d(sV + ch * G::chunk(128), &tm_v, ch * G::CW, 128 * u.kt, u.hk, u.zi, bar_v_full);
         }
         ++v_issued;
       }
@@ -2245,10 +2341,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     int g = 0, it = 0;
     bool ok = true;
     int2 seq = make_int2(int(blockIdx.x), 0);
-    for (int bh, kt; ok && next_tile(seq, &bh, &kt); ++it) {
-      const int zi = bh / args.H, hi = bh % args.H, k0 = 128 * kt, lo = tile_lo(kt), n = NBq - lo;
+    for (Unit u; ok && next_unit(seq, &u); ++it) {
+      const int zi = u.zi, k0 = 128 * u.kt, n = u.n;
       const int key = k0 + r;
-      for (int c = 0; c < n; ++c, ++g) {
+      UnitWalk<WINDOW> at(u);
+      int prev_h = at.h, prev_blk = at.blk;  // the block whose dQ part is in TMEM
+      for (int c = 0; c < n; ++c, ++g, at.next(u)) {
         if (!warp_wait(bar_s_full, g & 1, ab)) { ok = false; break; }
         tc_fence_after();
         uint32_t s[H], dp[H];
@@ -2259,10 +2357,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         reg_fence<H>(dp);
         tc_fence_before();
         mbar_arrive(bar_s_free);  // the tensor core may now write S^T/dP^T of the next block
-        const int q0 = (lo + c) * BQ + w * H;  // first query column of this warpgroup's half
-        const bool masked = (q0 + H > N) || (k0 + 128 > N) || (CAUSAL && q0 < k0 + 127);
-        const int c_lo = CAUSAL ? max(0, key - q0) : 0;  // valid query columns: c_lo <= c < c_hi
-        const int c_hi = key < N ? N - q0 : 0;
+        const int q0 = at.blk * BQ + w * H;  // first query column of this warpgroup's half
+        bool masked = (q0 + H > N) || (k0 + 128 > Nk) || (CAUSAL && q0 < k0 + 127);
+        int c_lo = CAUSAL ? max(0, key - q0) : 0;  // valid query columns: c_lo <= c < c_hi
+        int c_hi = key < Nk ? N - q0 : 0;
+        if (WINDOW) {  // a key is seen from its own position on, for one window unless it is a sink
+          const int p0 = q0 + args.win.off;
+          masked = masked || p0 < k0 + 127 || (p0 + H - 1 >= k0 + args.win.window && k0 + 128 > args.win.sinks);
+          c_lo = max(0, key - p0);
+          if (key >= args.win.sinks) c_hi = min(c_hi, key + args.win.window - p0);
+        }
         uint32_t pt[H / 2], dst[H / 2];
         if (masked)
           pds_row_folded<H, true>(s, dp, pt, dst, scale2, c_lo, c_hi);
@@ -2294,12 +2398,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_before();
           mbar_arrive(bar_dq_read);
           if constexpr (C::DQT)
-            fused_dqt_out(oq, stg, &tm_dqacc, 32 * q4, (lo + c - 1) * BQ + 32 * w, hi, zi, lane);
+            fused_dqt_out(oq, stg, &tm_dqacc, 32 * q4, prev_blk * BQ + 32 * w, prev_h, zi, lane);
           else
-            fused_dq_out<D>(oq, stg, &tm_dqacc, w * C::HW, (lo + c - 1) * BQ + 32 * q4, hi, zi, lane);
+            fused_dq_out<D>(oq, stg, &tm_dqacc, w * C::HW, prev_blk * BQ + 32 * q4, prev_h, zi, lane);
         } else {
           mbar_arrive(bar_dq_read);
         }
+        prev_h = at.h;
+        prev_blk = at.blk;
       }
       if (!ok || !warp_wait(bar_acc_done, it & 1, ab)) { ok = false; break; }
       // ---- epilogue: the last block's dQ part, then dV (warpgroup 0) or dK * sm_scale (warpgroup 1)
@@ -2314,12 +2420,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_wait_ld();
       reg_fence<OR>(o);
       reg_fence<C::QW>(oq);
+      const bool any = !WINDOW || n > 0;  // no query block: the accumulators hold nothing of this tile
       if constexpr (!C::DQT) {
         tc_fence_before();
         mbar_arrive(bar_acc_read);  // the next tile's first MMAs may overwrite the accumulators
-        fused_dq_out<D>(oq, stg, &tm_dqacc, w * C::HW, (lo + n - 1) * BQ + 32 * q4, hi, zi, lane);
+        if (any) fused_dq_out<D>(oq, stg, &tm_dqacc, w * C::HW, prev_blk * BQ + 32 * q4, prev_h, zi, lane);
       } else {
-        fused_dqt_out(oq, stg, &tm_dqacc, 32 * q4, (lo + n - 1) * BQ + 32 * w, hi, zi, lane);
+        if (any) fused_dqt_out(oq, stg, &tm_dqacc, 32 * q4, prev_blk * BQ + 32 * w, prev_h, zi, lane);
+      }
+      float* part = nullptr;  // kMaskWindow: this thread's row of the chunk's partial
+      if (WINDOW && u.chunk >= 0) {
+        const int64_t slot = ((int64_t(zi) * args.win.Hk + u.hk) * args.split.tiles + u.kt) * args.split.chunks + u.chunk;
+        part = args.part + ((slot * 2 + w) * 128 + r) * D;
       }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {  // columns [half * HW, half * HW + HW)
@@ -2331,6 +2443,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_before();
             mbar_arrive(bar_acc_read);
           }
+        }
+        if (WINDOW && !any) {
+#pragma unroll
+          for (int c = 0; c < OR; ++c) o[c] = 0u;
+        }
+        if (WINDOW && part != nullptr) {
+#pragma unroll
+          for (int c = 0; c < C::HW; c += 4)
+            *reinterpret_cast<uint4*>(part + half * C::HW + c) =
+                make_uint4(o[(C::DQT ? 0 : half * C::HW) + c], o[(C::DQT ? 0 : half * C::HW) + c + 1],
+                           o[(C::DQT ? 0 : half * C::HW) + c + 2], o[(C::DQT ? 0 : half * C::HW) + c + 3]);
+          continue;
         }
         if (lane == 0) tma_store_wait_read_all();  // this warp's previous store has left the staging area
         __syncwarp();
@@ -2348,7 +2472,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {  // rows past N are clipped by the tensor map
-          tma_store_4d(tm_out, stg, half * C::HW, k0 + 32 * q4, hi, zi);
+          tma_store_4d(tm_out, stg, half * C::HW, k0 + 32 * q4, u.hk, zi);
           tma_store_commit();
         }
       }
@@ -2360,8 +2484,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     // Last phase, once every CTA's dQ additions have completed: dq = sm_scale * dq_acc, by the compute
     // warps of all CTAs (named barrier 1 over their 256 threads).
-    if (grid_barrier(args.grid_sync, gridDim.x, ab, 1, 256, threadIdx.x == 0))
+    if (grid_barrier(args.grid_sync, gridDim.x, ab, 1, 256, threadIdx.x == 0)) {
       fused_dq_epilogue<D>(args, 256);
+      if (WINDOW && args.part != nullptr) fused_part_epilogue<D>(args, 256);
+    }
   }
 
   tc_fence_before();
@@ -2372,19 +2498,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int D, bool CAUSAL>
+template <int D, int MASK>
 cudaError_t fused_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
                        const CUtensorMap& tdk, const CUtensorMap& tdv, const CUtensorMap& tdqacc, const BwdArgs& a,
                        cudaStream_t s) {
-  auto kern = bwd_fused_kernel<D, CAUSAL>;
+  auto kern = bwd_fused_kernel<D, MASK>;
   constexpr int smem = FusedCfg<D>::SMEM_BYTES;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const long long nct = (a.N + 127) / 128;
-  const long long tiles = nct * a.Z * a.H;
+  constexpr bool WINDOW = MASK == kMaskWindow;
+  const long long nct = ((WINDOW ? a.win.Nk : a.N) + 127) / 128;
+  const long long tiles = nct * a.Z * (WINDOW ? a.win.Hk : a.H);
   if (tiles <= 0) return cudaSuccess;
-  if (tiles > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  const long long units = CAUSAL ? (nct + 1) / 2 * a.Z * a.H : tiles;  // the kernel's next_tile units
+  // The kernel's units (next_unit).
+  const long long units = WINDOW ? (nct + (long long)a.split.tiles * (a.split.chunks - 1)) * a.Z * a.win.Hk
+                          : MASK == kMaskCausal ? (nct + 1) / 2 * a.Z * a.H
+                                                : tiles;
+  if (tiles > 0x7fffffffLL || units > 0x7fffffffLL - 1024) return cudaErrorInvalidConfiguration;
   // One CTA per SM at most (shared memory), so a cooperative launch keeps every CTA resident: the grid
   // barrier before the kernel's last phase needs that (its counter is zeroed by the preprocess).
   const unsigned grid = unsigned(units < sm_count() ? units : sm_count());
@@ -2460,18 +2590,20 @@ cudaError_t launch_bwd_dkdv_f16(int D, bool causal, int variant, const CUtensorM
 static_assert(FusedCfg<64>::BQ == bwd_fused_query_rows(64) && FusedCfg<128>::BQ == bwd_fused_query_rows(128),
               "fused backward query blocks");
 
-cudaError_t launch_bwd_fused_f16(int D, bool causal, const CUtensorMap& tq, const CUtensorMap& tk,
+cudaError_t launch_bwd_fused_f16(int D, Mask mask, const CUtensorMap& tq, const CUtensorMap& tk,
                                  const CUtensorMap& tv, const CUtensorMap& tdo, const CUtensorMap& tdk,
                                  const CUtensorMap& tdv, const CUtensorMap& tdqacc, const BwdArgs& a, cudaStream_t s) {
   switch (D) {
-    case 16: return causal ? fused_impl<16, true>(tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s)
-                           : fused_impl<16, false>(tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s);
-    case 32: return causal ? fused_impl<32, true>(tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s)
-                           : fused_impl<32, false>(tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s);
-    case 64: return causal ? fused_impl<64, true>(tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s)
-                           : fused_impl<64, false>(tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s);
-    case 128: return causal ? fused_impl<128, true>(tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s)
-                            : fused_impl<128, false>(tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s);
+#define TATTN_FUSED_CASE(DD)                                                                              \
+  case DD:                                                                                                \
+    return mask == kMaskWindow   ? fused_impl<DD, kMaskWindow>(tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s)   \
+           : mask == kMaskCausal ? fused_impl<DD, kMaskCausal>(tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s)   \
+                                 : fused_impl<DD, kMaskNone>(tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s);
+    TATTN_FUSED_CASE(16)
+    TATTN_FUSED_CASE(32)
+    TATTN_FUSED_CASE(64)
+    TATTN_FUSED_CASE(128)
+#undef TATTN_FUSED_CASE
     default: return cudaErrorNotSupported;
   }
 }

@@ -177,7 +177,7 @@ extern "C" int tattn_fwd(const void* q, const void* k, const void* v, void* o, f
   a.wait_limit_ns = g_wait_limit_ns.load();
   if (dtype == TATTN_F32) {
     a.qk_scale = sm_scale * kLog2e;
-    return cuda_rc(launch_fwd_f32(D, causal != 0, q, k, v, sq, sk, sv, a, sm_scale, s));
+    return cuda_rc(launch_fwd_f32(D, causal ? kMaskCausal : kMaskNone, q, k, v, sq, sk, sv, a, sm_scale, s));
   }
   if (!layout_ok(q, sq, Z, H, N, D) || !layout_ok(k, sk, Z, H, N, D) || !layout_ok(v, sv, Z, H, N, D) ||
       !layout_ok(o, so, Z, H, N, D))
@@ -190,7 +190,7 @@ extern "C" int tattn_fwd(const void* q, const void* k, const void* v, void* o, f
   if ((rc = encode_f16(&tq, q, sq, Z, H, N, D, 128)) != TATTN_OK) return rc;
   if ((rc = encode_f16(&tk, k, sk, Z, H, N, D, kv_rows)) != TATTN_OK) return rc;
   if ((rc = encode_f16(&tv, v, sv, Z, H, N, D, kv_rows)) != TATTN_OK) return rc;
-  return cuda_rc(launch_fwd_f16(D, causal != 0, variant, tq, tk, tv, a, s));
+  return cuda_rc(launch_fwd_f16(D, causal ? kMaskCausal : kMaskNone, variant, tq, tk, tv, a, s));
 }
 
 extern "C" int tattn_bwd_preprocess(const void* o, const void* dout, float* delta, const int64_t* strides, int Z,
@@ -266,7 +266,8 @@ int bwd_common(bool dq_pass, const void* q, const void* k, const void* v, const 
   a.wait_limit_ns = g_wait_limit_ns.load();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == TATTN_F32)
-    return cuda_rc(dq_pass ? launch_bwd_dq_f32(D, causal != 0, a, s) : launch_bwd_dkdv_f32(D, causal != 0, a, s));
+    return cuda_rc(dq_pass ? launch_bwd_dq_f32(D, causal ? kMaskCausal : kMaskNone, a, s)
+                           : launch_bwd_dkdv_f32(D, causal ? kMaskCausal : kMaskNone, a, s));
   if (!layout_ok(q, a.sq, Z, H, N, D) || !layout_ok(k, a.sk, Z, H, N, D) || !layout_ok(v, a.sv, Z, H, N, D) ||
       !layout_ok(dout, a.sdo, Z, H, N, D))
     return TATTN_ERR_LAYOUT;
@@ -371,7 +372,147 @@ extern "C" int tattn_bwd_fused(const void* q, const void* k, const void* v, cons
   if ((rc = encode_f32_dense(&tdqacc, dq_acc, Z, H, N, D, kBwdStoreRows, acc_cols)) != TATTN_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if ((rc = cuda_rc(launch_bwd_preprocess(D, true, a, s))) != TATTN_OK) return rc;  // delta, zeroed workspace
-  return cuda_rc(launch_bwd_fused_f16(D, causal != 0, tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s));
+  return cuda_rc(launch_bwd_fused_f16(D, causal ? kMaskCausal : kMaskNone, tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s));
+}
+
+namespace {
+
+bool valid_window(int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window, int sinks) {
+  return valid_dims(Z, H, Nq, D) && Hk >= 1 && H % Hk == 0 && Nk >= Nq && window >= 1 && sinks >= 0 &&
+         (dtype == TATTN_F16 || dtype == TATTN_F32);
+}
+
+// Windows and sinks longer than the keys say no more than the keys themselves.
+WindowArgs window_args(int H, int Hk, int Nq, int Nk, int window, int sinks) {
+  return WindowArgs{Hk, H / Hk, Nk, Nk - Nq, window < Nk ? window : Nk, sinks < Nk ? sinks : Nk};
+}
+
+}  // namespace
+
+extern "C" int tattn_window_fwd(const void* q, const void* k, const void* v, void* o, float* m, const int64_t* strides,
+                                int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window, int sinks,
+                                float sm_scale, void* stream) {
+  if (!strides || !valid_window(Z, H, Hk, Nq, Nk, D, dtype, window, sinks)) return TATTN_ERR_INVALID_ARGUMENT;
+  if (int64_t(Z) * H * Nq == 0) return TATTN_OK;
+  if (!q || !k || !v || !o || !m) return TATTN_ERR_INVALID_ARGUMENT;
+  DeviceState* st;
+  int rc = device_setup(&st);
+  if (rc != TATTN_OK) return rc;
+  const Strides4 sq = load_strides(strides), sk = load_strides(strides + 4), sv = load_strides(strides + 8),
+                 so = load_strides(strides + 12);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  FwdArgs a{};
+  a.o = o;
+  a.m = m;
+  a.so = so;
+  a.Z = Z;
+  a.H = H;
+  a.N = Nq;
+  a.status = st->status;
+  a.wait_limit_ns = g_wait_limit_ns.load();
+  a.win = window_args(H, Hk, Nq, Nk, window, sinks);
+  if (dtype == TATTN_F32) {
+    a.qk_scale = sm_scale * kLog2e;
+    return cuda_rc(launch_fwd_f32(D, kMaskWindow, q, k, v, sq, sk, sv, a, sm_scale, s));
+  }
+  if (!layout_ok(q, sq, Z, H, Nq, D) || !layout_ok(k, sk, Z, Hk, Nk, D) || !layout_ok(v, sv, Z, Hk, Nk, D) ||
+      !layout_ok(o, so, Z, H, Nq, D))
+    return TATTN_ERR_LAYOUT;
+  a.so = normalize(so, Z, H, Nq, D);
+  a.qk_scale = (sm_scale < 0.f ? -sm_scale : sm_scale) * kLog2e;
+  a.negate_s = sm_scale < 0.f ? 1 : 0;
+  const int variant = tile_default(0, D, true), kv_rows = fwd_f16_kv_rows(D, variant);
+  CUtensorMap tq, tk, tv;
+  if ((rc = encode_f16(&tq, q, sq, Z, H, Nq, D, 128)) != TATTN_OK) return rc;
+  if ((rc = encode_f16(&tk, k, sk, Z, Hk, Nk, D, kv_rows)) != TATTN_OK) return rc;
+  if ((rc = encode_f16(&tv, v, sv, Z, Hk, Nk, D, kv_rows)) != TATTN_OK) return rc;
+  return cuda_rc(launch_fwd_f16(D, kMaskWindow, variant, tq, tk, tv, a, s));
+}
+
+extern "C" int tattn_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
+                                void* dq, void* dk, void* dv, const float* m, float* delta, void* workspace,
+                                const int64_t* strides, int Z, int H, int Hk, int Nq, int Nk, int D, int dtype,
+                                int window, int sinks, float sm_scale, void* stream) {
+  if (!strides || !valid_window(Z, H, Hk, Nq, Nk, D, dtype, window, sinks)) return TATTN_ERR_INVALID_ARGUMENT;
+  if (int64_t(Z) * H * Nk == 0) return TATTN_OK;
+  if (!dk || !dv) return TATTN_ERR_INVALID_ARGUMENT;
+  DeviceState* st;
+  int rc = device_setup(&st);
+  if (rc != TATTN_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (Nq == 0) {  // keys that no query sees
+    const size_t bytes = size_t(Z) * Hk * Nk * D * (dtype == TATTN_F16 ? 2 : 4);
+    for (void* p : {dk, dv})
+      if (cudaMemsetAsync(p, 0, bytes, s) != cudaSuccess) return TATTN_ERR_CUDA;
+    return TATTN_OK;
+  }
+  if (!q || !k || !v || !o || !dout || !dq || !m || !delta || (dtype == TATTN_F16 && !workspace))
+    return TATTN_ERR_INVALID_ARGUMENT;
+  BwdArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.o = o;
+  a.dout = dout;
+  a.sq = load_strides(strides);
+  a.sk = load_strides(strides + 4);
+  a.sv = load_strides(strides + 8);
+  a.so = load_strides(strides + 12);
+  a.sdo = load_strides(strides + 16);
+  a.m = m;
+  a.delta = delta;
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  a.Z = Z;
+  a.H = H;
+  a.N = Nq;
+  a.sm_scale = sm_scale;
+  a.qk_scale = (sm_scale < 0.f ? -sm_scale : sm_scale) * kLog2e;
+  a.negate_s = sm_scale < 0.f ? 1 : 0;
+  a.status = st->status;
+  a.wait_limit_ns = g_wait_limit_ns.load();
+  a.win = window_args(H, Hk, Nq, Nk, window, sinks);
+  if (dtype == TATTN_F32) {
+    rc = tattn_bwd_preprocess(o, dout, delta, strides + 12, Z, H, Nq, D, dtype, stream);
+    if (rc == TATTN_OK) rc = cuda_rc(launch_bwd_dkdv_f32(D, kMaskWindow, a, s));
+    if (rc == TATTN_OK) rc = cuda_rc(launch_bwd_dq_f32(D, kMaskWindow, a, s));
+    return rc;
+  }
+  if (!layout_ok(q, a.sq, Z, H, Nq, D) || !layout_ok(k, a.sk, Z, Hk, Nk, D) || !layout_ok(v, a.sv, Z, Hk, Nk, D) ||
+      !layout_ok(o, a.so, Z, H, Nq, D) || !layout_ok(dout, a.sdo, Z, H, Nq, D))
+    return TATTN_ERR_LAYOUT;
+  for (const void* p : {static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv),
+                        static_cast<const void*>(workspace)})
+    if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0) return TATTN_ERR_LAYOUT;
+  a.dq_acc = static_cast<float*>(workspace);
+  char* after = static_cast<char*>(workspace) + int64_t(Z) * H * Nq * D * 4;
+  a.grid_sync = reinterpret_cast<unsigned*>(after);
+  a.split = window_split(D, Nq, a.win.window, a.win.sinks);
+  a.part = a.split.chunks > 1 ? reinterpret_cast<float*>(after + 16) : nullptr;
+  CUtensorMap tq, tk, tv, tdo, tdk, tdv, tdqacc;
+  const int q_rows = bwd_fused_query_rows(D), acc_cols = D == 128 ? 32 : D / 2;  // as tattn_bwd_fused
+  if ((rc = encode_f16(&tq, q, a.sq, Z, H, Nq, D, q_rows)) != TATTN_OK) return rc;
+  if ((rc = encode_f16(&tk, k, a.sk, Z, Hk, Nk, D, 128)) != TATTN_OK) return rc;
+  if ((rc = encode_f16(&tv, v, a.sv, Z, Hk, Nk, D, 128)) != TATTN_OK) return rc;
+  if ((rc = encode_f16(&tdo, dout, a.sdo, Z, H, Nq, D, q_rows)) != TATTN_OK) return rc;
+  const Strides4 dense{int64_t(Hk) * Nk * D, int64_t(Nk) * D, D, 1};
+  if ((rc = encode_f16(&tdk, dk, dense, Z, Hk, Nk, D, kBwdStoreRows, D / 2)) != TATTN_OK) return rc;
+  if ((rc = encode_f16(&tdv, dv, dense, Z, Hk, Nk, D, kBwdStoreRows, D / 2)) != TATTN_OK) return rc;
+  if ((rc = encode_f32_dense(&tdqacc, a.dq_acc, Z, H, Nq, D, kBwdStoreRows, acc_cols)) != TATTN_OK) return rc;
+  a.so = normalize(a.so, Z, H, Nq, D);
+  a.sdo = normalize(a.sdo, Z, H, Nq, D);
+  if ((rc = cuda_rc(launch_bwd_preprocess(D, true, a, s))) != TATTN_OK) return rc;  // delta, zeroed workspace
+  return cuda_rc(launch_bwd_fused_f16(D, kMaskWindow, tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s));
+}
+
+extern "C" int64_t tattn_window_bwd_workspace_bytes(int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window,
+                                                    int sinks) {
+  if (!valid_window(Z, H, Hk, Nq, Nk, D, dtype, window, sinks) || double(Z) * H * Nk * (4.0 * D + 4.0) > 4e17)
+    return -1;
+  if (dtype == TATTN_F32 || Nq == 0) return 0;
+  const WindowArgs w = window_args(H, Hk, Nq, Nk, window, sinks);
+  return window_bwd_workspace_bytes(Z, H, Hk, Nq, D, window_split(D, Nq, w.window, w.sinks));
 }
 
 extern "C" int64_t tattn_bwd_fused_workspace_bytes(int Z, int H, int N, int D) {

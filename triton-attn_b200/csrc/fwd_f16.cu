@@ -19,6 +19,7 @@
 // its tile's issuer starts the next QK^T. P then feeds the PV MMA as the A operand straight from
 // TMEM. The two warpgroups ping-pong on the exponent pass (the MUFU-bound part) through a token pair
 // of mbarriers; a warpgroup hands the turn over before its last quarter of columns.
+// A sliding window with sinks (kMaskWindow) is the same kernel on a shorter list of key blocks (Blocks).
 // The running max is rescaled lazily: O (in TMEM) and l are only corrected when a row's max grows by
 // more than kRescaleThreshold (log2 units); P values stay below 2^kRescaleThreshold, exact in fp16.
 #include "common.cuh"
@@ -125,16 +126,60 @@ __device__ __forceinline__ void issue_pv_stage(int st, uint32_t d_tmem, uint32_t
   issue_pv_st<C, D, ST>(d_tmem, p_tmem, dV, accumulate);
 }
 
-// Max of one row of raw scores; MASK ignores columns >= lim.
-template <int BN, bool MASK>
-__device__ __forceinline__ float row_max(const uint32_t* s, int lim) {
+// The key blocks that a CTA's two query tiles go through. Both walk one list, j = 0 .. n1 - 1, through the
+// ring; tile 0 takes its first n0 entries. kMaskWindow: the list is the blocks that hold sinks, then those
+// from the first one in tile 0's window up to the diagonal; tile 1 leaves out the `skip` entries from
+// `from` on, which only tile 0's window reaches.
+struct Blocks {
+  int n0, n1;        // list entries up to the end of tile 0 / 1 (0: the tile has no rows)
+  int sink, jump;    // entry j >= sink is block j + jump
+  int from, skip;
+
+  __device__ __forceinline__ int block(int j) const { return j < sink ? j : j + jump; }
+  // List entry of tile i's u-th block.
+  __device__ __forceinline__ int entry(int i, int u) const { return i == 1 && u >= from ? u + skip : u; }
+  // Blocks that tile i takes.
+  __device__ __forceinline__ int count(int i) const { return i == 0 ? n0 : n1 > 0 ? n1 - skip : 0; }
+};
+
+// With a ring of 2 (D = 128) tile 1 leaves nothing out: it would run one entry ahead of tile 0, and the
+// entry after that could only be loaded once tile 0 is done with its own.
+template <int BM, int BN, int NS>
+__device__ __forceinline__ Blocks window_blocks(int row0, int N, const WindowArgs& w) {
+  const int p0 = row0 + w.off, p1 = p0 + BM;  // positions of the tiles' first rows
+  const int end0 = min(p1 - 1, w.Nk - 1) / BN + 1, end1 = min(p1 + BM - 1, w.Nk - 1) / BN + 1;
+  const int first0 = max(0, p0 - w.window + 1) / BN, first1 = max(0, p1 - w.window + 1) / BN;
+  const int ns = (w.sinks + BN - 1) / BN;
+  Blocks b;
+  b.sink = min(ns, first0);
+  b.jump = first0 - b.sink;
+  b.n0 = end0 - b.jump;
+  b.n1 = row0 + BM < N ? end1 - b.jump : 0;
+  const int keep = max(first0, ns);  // tile 1 needs no block of [keep, first1)
+  b.from = keep - b.jump;
+  b.skip = NS > 2 && b.n1 > 0 ? max(0, first1 - keep) : 0;
+  return b;
+}
+
+// Columns of a key block that a row sees: c < lim and, kMaskWindow, c >= first or c < sink as well.
+struct Columns {
+  int lim, first, sink;
+  template <int MASK>
+  __device__ __forceinline__ bool see(int c) const {
+    return MASK == kMaskWindow ? c < lim && (c >= first || c < sink) : c < lim;
+  }
+};
+
+// Max of one row of raw scores; MASKED ignores the columns that the row does not see.
+template <int BN, bool MASKED, int MASK>
+__device__ __forceinline__ float row_max(const uint32_t* s, const Columns& cols) {
   float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int c = 0; c < BN; c += 2) {
     float a = __uint_as_float(s[c]), b = __uint_as_float(s[c + 1]);
-    if (MASK) {
-      a = c < lim ? a : -INFINITY;
-      b = c + 1 < lim ? b : -INFINITY;
+    if (MASKED) {
+      a = cols.see<MASK>(c) ? a : -INFINITY;
+      b = cols.see<MASK>(c + 1) ? b : -INFINITY;
     }
     m[(c / 2) & 3] = fmax3(m[(c / 2) & 3], a, b);
   }
@@ -142,10 +187,11 @@ __device__ __forceinline__ float row_max(const uint32_t* s, int lim) {
 }
 
 // One row of P = exp2(S * scale - m) for columns [C0, C1) as fp16 pairs (p[c/2] = columns c, c+1) and
-// its fp32 sum. kEmuPairs of every 8 column pairs use the FMA-pipe exp2, the rest MUFU. MASK zeroes
-// columns >= lim.
-template <int C0, int C1, bool MASK>
-__device__ __forceinline__ float exp_cols(const uint32_t* s, uint32_t* p, uint64_t scale2, uint64_t negm2, int lim) {
+// its fp32 sum. kEmuPairs of every 8 column pairs use the FMA-pipe exp2, the rest MUFU. MASKED zeroes
+// the columns that the row does not see.
+template <int C0, int C1, bool MASKED, int MASK>
+__device__ __forceinline__ float exp_cols(const uint32_t* s, uint32_t* p, uint64_t scale2, uint64_t negm2,
+                                          const Columns& cols) {
   uint64_t acc0 = 0, acc1 = 0;
 #pragma unroll
   for (int c = C0; c < C1; c += 2) {
@@ -157,9 +203,9 @@ __device__ __forceinline__ float exp_cols(const uint32_t* s, uint32_t* p, uint64
       const float2 xv = f2_unpack(x);
       e = make_float2(ex2_approx(xv.x), ex2_approx(xv.y));
     }
-    if (MASK) {
-      e.x = c < lim ? e.x : 0.f;
-      e.y = c + 1 < lim ? e.y : 0.f;
+    if (MASKED) {
+      e.x = cols.see<MASK>(c) ? e.x : 0.f;
+      e.y = cols.see<MASK>(c + 1) ? e.y : 0.f;
     }
     if ((c / 2) & 1)
       acc1 = fadd2(acc1, f2(e.x, e.y));
@@ -171,12 +217,13 @@ __device__ __forceinline__ float exp_cols(const uint32_t* s, uint32_t* p, uint64
   return t.x + t.y;
 }
 
-template <int D, bool CAUSAL, int BN_, int NS_>
+template <int D, int MASK, int BN_, int NS_>
 __global__ void __launch_bounds__(384, 1)
     fwd_f16_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const FwdArgs args) {
   using C = FwdCfg<D, BN_, NS_>;
   constexpr int BN = C::BN;
+  constexpr bool CAUSAL = MASK == kMaskCausal, WINDOW = MASK == kMaskWindow;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
   const uint32_t base_u32 = (raw_u32 + 1023u) & ~1023u;
@@ -208,12 +255,16 @@ __global__ void __launch_bounds__(384, 1)
     cta = blockIdx.x % nct;
   }
   const int zi = bh / args.H, hi = bh % args.H;
+  const int hk = WINDOW ? hi / args.win.group : hi;  // key/value head
   const int NB = (N + BN - 1) / BN;
-  // Query tile i of this CTA: rows [row0_i, row0_i + 128), key blocks [0, n_i).
+  // Query tile i of this CTA: rows [row0_i, row0_i + 128), n_i key blocks: [0, n_i) or, kMaskWindow,
+  // those of the list.
   const int row0_0 = 2 * cta * C::BM, row0_1 = row0_0 + C::BM;
-  const int n_0 = row0_0 >= N ? 0 : (CAUSAL ? min((row0_0 + C::BM + BN - 1) / BN, NB) : NB);
-  const int n_1 = row0_1 >= N ? 0 : (CAUSAL ? min((row0_1 + C::BM + BN - 1) / BN, NB) : NB);
-  const int nmax = max(n_0, n_1);
+  Blocks list{};
+  if (WINDOW) list = window_blocks<C::BM, BN, C::NS>(row0_0, N, args.win);
+  const int n_0 = WINDOW ? list.count(0) : row0_0 >= N ? 0 : (CAUSAL ? min((row0_0 + C::BM + BN - 1) / BN, NB) : NB);
+  const int n_1 = WINDOW ? list.count(1) : row0_1 >= N ? 0 : (CAUSAL ? min((row0_1 + C::BM + BN - 1) / BN, NB) : NB);
+  const int nmax = WINDOW ? max(list.n0, list.n1) : max(n_0, n_1);
 
   if (threadIdx.x == 0) {
     mbar_init(bar_q, 1);
@@ -269,16 +320,17 @@ __global__ void __launch_bounds__(384, 1)
         if (j >= C::NS) {  // both tiles that used the stage's previous block must be done with it
           const int old = j - C::NS;
           for (int i = 0; i < 2 && ok; ++i)
-            if (old < (i ? n_1 : n_0) && !mbar_wait(&bar_kv_empty[i * C::NS + st], ((j / C::NS) - 1) & 1, ab))
+            if (old < (WINDOW ? (i ? list.n1 : list.n0) : (i ? n_1 : n_0)) && !mbar_wait(&bar_kv_empty[i * C::NS + st], ((j / C::NS) - 1) & 1, ab))
               ok = false;
           if (!ok) break;
         }
+        const int key0 = (WINDOW ? list.block(j) : j) * BN;
         mbar_arrive_expect_tx(&bar_k_full[st], C::KTILE);
         for (int ch = 0; ch < C::NCH; ++ch)
-          tma_load_4d(sK + st * C::KTILE + ch * C::KCHUNK, &tm_k, ch * C::CW, j * BN, hi, zi, &bar_k_full[st]);
+          tma_load_4d(sK + st * C::KTILE + ch * C::KCHUNK, &tm_k, ch * C::CW, key0, hk, zi, &bar_k_full[st]);
         mbar_arrive_expect_tx(&bar_v_full[st], C::KTILE);
         for (int ch = 0; ch < C::NCH; ++ch)
-          tma_load_4d(sV + st * C::KTILE + ch * C::KCHUNK, &tm_v, ch * C::CW, j * BN, hi, zi, &bar_v_full[st]);
+          tma_load_4d(sV + st * C::KTILE + ch * C::KCHUNK, &tm_v, ch * C::CW, key0, hk, zi, &bar_v_full[st]);
       }
       // Every copy this CTA issued must land before the CTA exits (instant on the normal path).
       const unsigned long long lim = 100ull * 1000ull * 1000ull;
@@ -300,26 +352,38 @@ __global__ void __launch_bounds__(384, 1)
       const uint64_t dK = smem_desc(sK, 16, 8 * C::SWB, C::LAYOUT);
       const uint64_t dV = smem_desc(sV, C::KCHUNK, 8 * C::SWB, C::LAYOUT);
       const uint32_t tS = tmem + C::TM_S + i * BN, tP = tmem + C::TM_P + i * C::P_STRIDE, tO = tmem + C::TM_O + i * D;
-      bool ok = n > 0 && warp_wait(bar_q, 0, ab) && warp_wait(&bar_k_full[0], 0, ab);
+      // kMaskWindow: releases the list entries [a, b) that this tile leaves out, each once it has landed
+      // (a phase of kv_empty may only complete after the producer has waited for the one before).
+      auto leave_out = [&](int a, int b) -> bool {
+        for (; a < b; ++a) {
+          if (!warp_wait(&bar_k_full[a % C::NS], (a / C::NS) & 1, ab)) return false;
+          mma_commit_elect(&bar_kv_empty[i * C::NS + a % C::NS]);
+        }
+        return true;
+      };
+      int e = WINDOW ? list.entry(i, 0) : 0;  // list entry of block j
+      bool ok = n > 0 && warp_wait(bar_q, 0, ab) && (!WINDOW || leave_out(0, e)) &&
+                warp_wait(&bar_k_full[e % C::NS], (e / C::NS) & 1, ab);
       if (ok) {
         tc_fence_after();
-        issue_qk_stage<C, D>(0, i, tS, dQ, dK, idesc_s);
+        issue_qk_stage<C, D>(e % C::NS, i, tS, dQ, dK, idesc_s);
         mma_commit_elect(&bar_s_full[i]);
       }
       for (int j = 0; ok && j < n; ++j) {
+        e = WINDOW ? list.entry(i, j) : j;
+        const int b = WINDOW ? list.entry(i, j + 1) : j + 1;  // list entry of the next block
         if (C::ALIAS_P) {
           // PV(j) reads P(j) where S(j) was, then S(j + 1) overwrites both (in issue order).
-          if (!warp_wait(&bar_p_full[i], j & 1, ab) || !warp_wait(&bar_v_full[j % C::NS], (j / C::NS) & 1, ab)) {
+          if (!warp_wait(&bar_p_full[i], j & 1, ab) || !warp_wait(&bar_v_full[e % C::NS], (e / C::NS) & 1, ab)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          issue_pv_stage<C, D>(j % C::NS, tO, tP, dV, j > 0 ? 1u : 0u);
+          issue_pv_stage<C, D>(e % C::NS, tO, tP, dV, j > 0 ? 1u : 0u);
           mma_commit_elect(&bar_o_done[i]);
-          mma_commit_elect(&bar_kv_empty[i * C::NS + j % C::NS]);
+          mma_commit_elect(&bar_kv_empty[i * C::NS + e % C::NS]);
           if (j + 1 < n) {
-            const int b = j + 1;
-            if (!warp_wait(&bar_k_full[b % C::NS], (b / C::NS) & 1, ab)) {
+            if ((WINDOW && !leave_out(e + 1, b)) || !warp_wait(&bar_k_full[b % C::NS], (b / C::NS) & 1, ab)) {
               ok = false;
               break;
             }
@@ -330,8 +394,8 @@ __global__ void __launch_bounds__(384, 1)
           continue;
         }
         if (j + 1 < n) {
-          const int b = j + 1;
-          if (!warp_wait(&bar_s_free[i], j & 1, ab) || !warp_wait(&bar_k_full[b % C::NS], (b / C::NS) & 1, ab)) {
+          if (!warp_wait(&bar_s_free[i], j & 1, ab) || (WINDOW && !leave_out(e + 1, b)) ||
+              !warp_wait(&bar_k_full[b % C::NS], (b / C::NS) & 1, ab)) {
             ok = false;
             break;
           }
@@ -339,14 +403,14 @@ __global__ void __launch_bounds__(384, 1)
           issue_qk_stage<C, D>(b % C::NS, i, tS, dQ, dK, idesc_s);
           mma_commit_elect(&bar_s_full[i]);
         }
-        if (!warp_wait(&bar_p_full[i], j & 1, ab) || !warp_wait(&bar_v_full[j % C::NS], (j / C::NS) & 1, ab)) {
+        if (!warp_wait(&bar_p_full[i], j & 1, ab) || !warp_wait(&bar_v_full[e % C::NS], (e / C::NS) & 1, ab)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        issue_pv_stage<C, D>(j % C::NS, tO, tP, dV, j > 0 ? 1u : 0u);
+        issue_pv_stage<C, D>(e % C::NS, tO, tP, dV, j > 0 ? 1u : 0u);
         mma_commit_elect(&bar_o_done[i]);
-        mma_commit_elect(&bar_kv_empty[i * C::NS + j % C::NS]);
+        mma_commit_elect(&bar_kv_empty[i * C::NS + e % C::NS]);
       }
       // Every MMA of this tile must retire before TMEM is released.
       mma_commit_elect(&bar_fin[i]);
@@ -379,11 +443,21 @@ __global__ void __launch_bounds__(384, 1)
 
       // Columns past N (ragged tail) only occur in the last block; columns above the diagonal
       // (causal) in every block that reaches past the tile's first row (the last BM / BN blocks).
-      const int col0 = j * BN;
-      const bool last = (col0 + BN > N) || (CAUSAL && col0 + BN - 1 > row - t);
-      int lim = N - col0;
-      if (CAUSAL) lim = min(lim, row - col0 + 1);
-      const float m_cand = (last ? row_max<BN, true>(s, lim) : row_max<BN, false>(s, lim)) * scale;
+      // kMaskWindow: in every block that the diagonal or the lower edge of some row's window cuts.
+      const int col0 = (WINDOW ? list.block(list.entry(i, j)) : j) * BN;
+      bool last;
+      Columns cols{};
+      if (WINDOW) {
+        const int pos = row + args.win.off, tile = pos - t;  // positions of this row and of the tile's first
+        last = col0 + BN - 1 > tile || (col0 <= tile + C::BM - 1 - args.win.window && col0 + BN > args.win.sinks);
+        cols = Columns{min(args.win.Nk, pos + 1) - col0, pos + 1 - args.win.window - col0, args.win.sinks - col0};
+      } else {
+        last = (col0 + BN > N) || (CAUSAL && col0 + BN - 1 > row - t);
+        cols.lim = N - col0;
+        if (CAUSAL) cols.lim = min(cols.lim, row - col0 + 1);
+      }
+      float m_cand = last ? row_max<BN, true, MASK>(s, cols) : row_max<BN, false, MASK>(s, cols);
+      if (!WINDOW || m_cand != -INFINITY) m_cand *= scale;  // (-inf: the row sees none of this block; scale may be 0)
       float alpha = 1.f;
       bool need = false;
       if (j == 0) {
@@ -409,12 +483,14 @@ __global__ void __launch_bounds__(384, 1)
       // hand-off (measured at BN = 128: 7/8 best, 3/4 within 1%, 1/2 8% slower; slower at BN = 64).
       constexpr int kSplit = BN == 128 ? BN * 7 / 8 : BN;
       uint32_t p[BN / 2];
-      const uint64_t negm2 = f2(-m_run, -m_run);
-      l_run += last ? exp_cols<0, kSplit, true>(s, p, scale2, negm2, lim) : exp_cols<0, kSplit, false>(s, p, scale2, negm2, lim);
+      const float m_use = WINDOW && m_run == -INFINITY ? 0.f : m_run;  // nothing seen yet: every p is masked to 0
+      const uint64_t negm2 = f2(-m_use, -m_use);
+      l_run += last ? exp_cols<0, kSplit, true, MASK>(s, p, scale2, negm2, cols)
+                    : exp_cols<0, kSplit, false, MASK>(s, p, scale2, negm2, cols);
       mbar_arrive(&bar_exp_done[i]);
       if constexpr (kSplit < BN)
-        l_run += last ? exp_cols<kSplit, BN, true>(s, p, scale2, negm2, lim)
-                      : exp_cols<kSplit, BN, false>(s, p, scale2, negm2, lim);
+        l_run += last ? exp_cols<kSplit, BN, true, MASK>(s, p, scale2, negm2, cols)
+                      : exp_cols<kSplit, BN, false, MASK>(s, p, scale2, negm2, cols);
 
       // PV(j-1) must have landed before P and O of this tile are touched again (ALIAS_P: it has, since
       // S(j) was issued after it and has completed).
@@ -478,11 +554,11 @@ __global__ void __launch_bounds__(384, 1)
   }
 }
 
-template <int D, bool CAUSAL, int BN, int NS>
+template <int D, int MASK, int BN, int NS>
 cudaError_t launch_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FwdArgs& a,
                         cudaStream_t s) {
   using C = FwdCfg<D, BN, NS>;
-  auto kern = fwd_f16_kernel<D, CAUSAL, BN, NS>;
+  auto kern = fwd_f16_kernel<D, MASK, BN, NS>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
   if (e != cudaSuccess) return e;
   const int nct = (a.N + 2 * C::BM - 1) / (2 * C::BM);
@@ -494,23 +570,30 @@ cudaError_t launch_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUte
 }
 
 // Variant v (tiles.h, kFwdTiles) for head dim D; variants whose blocks do not fit D's TMEM budget are
-// not instantiated.
-template <int D, bool CAUSAL>
+// not instantiated. kMaskWindow has the default variant only.
+template <int D, int MASK>
 cudaError_t launch_variant(int v, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                            const FwdArgs& a, cudaStream_t s) {
   static_assert(kNumFwdTiles == 3, "variant dispatch");
-  switch (v) {
-    case 0:
-      if constexpr (D <= 64) return launch_impl<D, CAUSAL, kFwdTiles[0].block_n, kFwdTiles[0].stages>(tq, tk, tv, a, s);
-      break;
-    case 1:
-      return launch_impl<D, CAUSAL, kFwdTiles[1].block_n, kFwdTiles[1].stages>(tq, tk, tv, a, s);
-    case 2:
-      return launch_impl<D, CAUSAL, kFwdTiles[2].block_n, kFwdTiles[2].stages>(tq, tk, tv, a, s);
-    default:
-      break;
+  if constexpr (MASK == kMaskWindow) {
+    constexpr TileVariant tile = kFwdTiles[tile_default(0, D, true)];
+    static_assert(tile.block_n == 128, "window_blocks: tile 1 starts at most one block after tile 0");
+    return v == tile_default(0, D, true) ? launch_impl<D, MASK, tile.block_n, tile.stages>(tq, tk, tv, a, s)
+                                         : cudaErrorNotSupported;
+  } else {
+    switch (v) {
+      case 0:
+        if constexpr (D <= 64) return launch_impl<D, MASK, kFwdTiles[0].block_n, kFwdTiles[0].stages>(tq, tk, tv, a, s);
+        break;
+      case 1:
+        return launch_impl<D, MASK, kFwdTiles[1].block_n, kFwdTiles[1].stages>(tq, tk, tv, a, s);
+      case 2:
+        return launch_impl<D, MASK, kFwdTiles[2].block_n, kFwdTiles[2].stages>(tq, tk, tv, a, s);
+      default:
+        break;
+    }
+    return cudaErrorNotSupported;
   }
-  return cudaErrorNotSupported;
 }
 
 }  // namespace
@@ -519,13 +602,14 @@ int fwd_f16_kv_rows(int D, int variant) {
   return tile_supported(0, variant, D) ? kFwdTiles[variant].block_n : 0;
 }
 
-cudaError_t launch_fwd_f16(int D, bool causal, int variant, const CUtensorMap& tq, const CUtensorMap& tk,
+cudaError_t launch_fwd_f16(int D, Mask mask, int variant, const CUtensorMap& tq, const CUtensorMap& tk,
                            const CUtensorMap& tv, const FwdArgs& a, cudaStream_t s) {
   if (!tile_supported(0, variant, D)) return cudaErrorNotSupported;
 #define TATTN_FWD_CASE(DD)                                                                     \
   case DD:                                                                                     \
-    return causal ? launch_variant<DD, true>(variant, tq, tk, tv, a, s)                        \
-                  : launch_variant<DD, false>(variant, tq, tk, tv, a, s);
+    return mask == kMaskWindow   ? launch_variant<DD, kMaskWindow>(variant, tq, tk, tv, a, s)  \
+           : mask == kMaskCausal ? launch_variant<DD, kMaskCausal>(variant, tq, tk, tv, a, s)  \
+                                 : launch_variant<DD, kMaskNone>(variant, tq, tk, tv, a, s);
   switch (D) {
     TATTN_FWD_CASE(16)
     TATTN_FWD_CASE(32)

@@ -13,6 +13,23 @@ struct Strides4 {
   int64_t z, h, n, d;
 };
 
+// Which keys a query sees (template parameter of the attention kernels).
+enum Mask : int {
+  kMaskNone = 0,    // all
+  kMaskCausal = 1,  // key <= query
+  kMaskWindow = 2,  // a sliding window and the first tokens (WindowArgs)
+};
+
+// kMaskWindow: query row i stands at position i + off of its sequence and sees the keys j <= i + off with
+// j > i + off - window or j < sinks. K and V have H / group heads of Nk tokens, shared by `group`
+// consecutive query heads each.
+struct WindowArgs {
+  int Hk, group;  // key/value heads, query heads per key/value head
+  int Nk, off;    // tokens of K and V; off = Nk - N >= 0
+  int window;     // 1 <= window <= Nk
+  int sinks;      // 0 <= sinks <= Nk
+};
+
 struct FwdArgs {
   void* o;           // [Z, H, N, D], strides `so`
   float* m;          // [Z, H, N] dense fp32: rowmax + log2(rowsum), base-2 units
@@ -22,6 +39,14 @@ struct FwdArgs {
   int negate_s;      // 1 when sm_scale < 0 (fp16 path)
   int* status;       // device status word
   unsigned long long wait_limit_ns;  // bound of every mbarrier wait (tattn_set_wait_limit_ns)
+  WindowArgs win;    // kMaskWindow only
+};
+
+// Fused window backward: the `tiles` first key tiles hold sinks and are seen by every later query, the
+// others by one window of queries only. Each sink tile's query blocks are cut into `chunks` units of at
+// most `blocks` blocks (tiles = 0, or chunks = 1: no cut).
+struct WindowSplit {
+  int tiles, chunks, blocks;
 };
 
 struct BwdArgs {
@@ -40,6 +65,9 @@ struct BwdArgs {
   int negate_s;
   int* status;
   unsigned long long wait_limit_ns;  // bound of every mbarrier wait (tattn_set_wait_limit_ns)
+  WindowArgs win;    // kMaskWindow only: dk and dv are then dense [Z, win.Hk, win.Nk, D]
+  WindowSplit split; // kMaskWindow, fused backward only
+  float* part;       // kMaskWindow, fused backward: partial dV and dK of the split key tiles, or null
 };
 
 // `variant` below is a 0-based tile variant of tiles.h (kFwdTiles / kBwdTiles); launchers return
@@ -52,7 +80,7 @@ int fwd_f16_kv_rows(int D, int variant);
 void bwd_f16_box_rows(int D, bool dq_pass, int variant, int* q_rows, int* kv_rows);
 
 // fp16 tcgen05 kernels (tensor maps describe [Z, H, N, D] tensors as 4-D {D, N, H, Z}).
-cudaError_t launch_fwd_f16(int D, bool causal, int variant, const CUtensorMap& tq, const CUtensorMap& tk,
+cudaError_t launch_fwd_f16(int D, Mask mask, int variant, const CUtensorMap& tq, const CUtensorMap& tk,
                            const CUtensorMap& tv, const FwdArgs& a, cudaStream_t s);
 // tdq: store map of the dense dQ output, kBwdStoreRows-row boxes of D/2 columns (D <= 64).
 cudaError_t launch_bwd_dq_f16(int D, bool causal, int variant, const CUtensorMap& tq, const CUtensorMap& tk,
@@ -68,7 +96,7 @@ cudaError_t launch_bwd_dkdv_f16(int D, bool causal, int variant, const CUtensorM
 // tq/tdo with boxes of bwd_fused_query_rows(D) rows, tk/tv 128-row boxes, tdk/tdv store maps of
 // kBwdStoreRows-row boxes of D/2 columns, tdqacc a reduce map over a.dq_acc (kBwdStoreRows-row boxes
 // of D/2 columns; 32 columns at D = 128).
-cudaError_t launch_bwd_fused_f16(int D, bool causal, const CUtensorMap& tq, const CUtensorMap& tk,
+cudaError_t launch_bwd_fused_f16(int D, Mask mask, const CUtensorMap& tq, const CUtensorMap& tk,
                                  const CUtensorMap& tv, const CUtensorMap& tdo, const CUtensorMap& tdk,
                                  const CUtensorMap& tdv, const CUtensorMap& tdqacc, const BwdArgs& a, cudaStream_t s);
 // Box height of the backward's output store maps (one warp's 32 TMEM lanes).
@@ -77,12 +105,28 @@ constexpr int kBwdStoreRows = 32;
 __host__ __device__ constexpr int bwd_fused_query_rows(int D) { return D == 128 ? 64 : 128; }
 // Workspace of tattn_bwd_fused: the fp32 dQ rows [Z, H, N, D], then 16 bytes for the grid-barrier counter.
 inline int64_t bwd_fused_workspace_bytes(int Z, int H, int N, int D) { return int64_t(Z) * H * N * D * 4 + 16; }
+// The cut of the sink tiles, so that a unit costs about what a tile with one window of queries does: such
+// a tile sees ceil((window + 127) / BQ) + 1 query blocks at most. At most 32 chunks bound the partials.
+inline WindowSplit window_split(int D, int N, int window, int sinks) {
+  const int bq = bwd_fused_query_rows(D), all = (N + bq - 1) / bq;
+  const int tiles = (sinks + 127) / 128;
+  if (tiles == 0 || all == 0) return WindowSplit{0, 1, 0};
+  const int one = int((int64_t(window) + 127 + bq - 1) / bq + 1), least = (all + 31) / 32;
+  const int blocks = one > least ? one : least;
+  return WindowSplit{tiles, (all + blocks - 1) / blocks, blocks};
+}
+// Workspace of the fused window backward: the fp32 dQ rows and the barrier counter as above, then, if the
+// sink tiles are cut, fp32 [Z * Hk, tiles, chunks, 2 (dV, dK), 128, D] partials.
+inline int64_t window_bwd_workspace_bytes(int Z, int H, int Hk, int N, int D, const WindowSplit& w) {
+  const int64_t part = w.chunks > 1 ? int64_t(Z) * Hk * w.tiles * w.chunks * 2 * 128 * D * 4 : 0;
+  return bwd_fused_workspace_bytes(Z, H, N, D) + part;
+}
 
 // SIMT kernels (fp32 inputs; any strides).
-cudaError_t launch_fwd_f32(int D, bool causal, const void* q, const void* k, const void* v, Strides4 sq,
+cudaError_t launch_fwd_f32(int D, Mask mask, const void* q, const void* k, const void* v, Strides4 sq,
                            Strides4 sk, Strides4 sv, const FwdArgs& a, float sm_scale, cudaStream_t s);
-cudaError_t launch_bwd_dq_f32(int D, bool causal, const BwdArgs& a, cudaStream_t s);
-cudaError_t launch_bwd_dkdv_f32(int D, bool causal, const BwdArgs& a, cudaStream_t s);
+cudaError_t launch_bwd_dq_f32(int D, Mask mask, const BwdArgs& a, cudaStream_t s);
+cudaError_t launch_bwd_dkdv_f32(int D, Mask mask, const BwdArgs& a, cudaStream_t s);
 
 // delta = rowsum(dO * O) in fp32 (fp16 or fp32 inputs); also zeroes the rows of a.dq_acc and the
 // counter a.grid_sync when they are set (the fused backward's workspace).

@@ -2,5 +2,6 @@
 ``tattn`` package (src/tattn/__init__.py:3-5)."""
 
 from tattn.api import attention, cuda_available, triton_available
+from tattn.window import window_attention
 
-__all__ = ["attention", "cuda_available", "triton_available"]
+__all__ = ["attention", "cuda_available", "triton_available", "window_attention"]

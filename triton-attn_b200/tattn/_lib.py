@@ -30,6 +30,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tattn_bwd_noalloc": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64P, _I, _I, _I, _I, _I, _I, _F, _P]),
     "tattn_bwd_fused": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64P, _I, _I, _I, _I, _I, _I, _F, _P]),
     "tattn_bwd_fused_workspace_bytes": (ctypes.c_int64, [_I, _I, _I, _I]),
+    "tattn_window_fwd": (_I, [_P, _P, _P, _P, _P, _I64P, *[_I] * 9, _F, _P]),
+    "tattn_window_bwd": (_I, [*[_P] * 11, _I64P, *[_I] * 9, _F, _P]),
+    "tattn_window_bwd_workspace_bytes": (ctypes.c_int64, [_I] * 9),
     "tattn_layout_ok": (_I, [_P, _I64P, _I, _I, _I, _I]),
     "tattn_selftest_exp2": (_I, [_P, _P, _P, _P, _I, _P]),
     "tattn_selftest_exp2_poly4": (_I, [_P, _P, _I, _P]),
@@ -44,7 +47,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tattn_status_string": (ctypes.c_char_p, [_I]),
     "tattn_abi_version": (_I, []),
 }
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
