@@ -58,6 +58,7 @@ enum tattn_status {
 /* Device status word bits (tattn_device_status). */
 #define TATTN_DEV_WAIT_TIMEOUT 1 /* an mbarrier wait exceeded the wait limit (tattn_set_wait_limit_ns); the CTA unwound */
 #define TATTN_DEV_ABORTED 2
+#define TATTN_DEV_INDEX_RANGE 4 /* a position or a length read by a kernel lies outside its table or cache */
 
 /* Forward: O = softmax(Q K^T * sm_scale) V and M, for one attention call.
  * Replaces the launch of _fwd_kernel (src/tattn/kernels.py:57-148) made by _forward
@@ -130,6 +131,31 @@ TATTN_API int tattn_window_bwd(const void* q, const void* k, const void* v, cons
 /* Bytes of the workspace that tattn_window_bwd needs, or -1 for invalid arguments. */
 TATTN_API int64_t tattn_window_bwd_workspace_bytes(int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window,
                                          int sinks);
+
+/* Norms of query and key heads and the position rotation, in one pass (no reference counterpart). A row x of D
+ * values (one head of one token) becomes R(p) (x / sqrt(mean(x^2) + eps) * w): w = wq or wk [D], and R(p)
+ * rotates pair j by the angle whose cosine and sine are cos[p, j] and sin[p, j]; the pairs are (j, j + D / 2)
+ * or, interleaved nonzero, (2 j, 2 j + 1). cos, sin: dense fp32 [P, D / 2], 16-byte aligned. positions:
+ * int32 [Z, N] or null (p = n); a p outside [0, P) makes its rows NaN and sets TATTN_DEV_INDEX_RANGE.
+ * q [Z, H, N, D], k [Z, Hk, N, D] of `dtype`; weights (16-byte aligned) of `w_dtype`, which is `dtype` or
+ * TATTN_F32. strides: 18 int64 = q, k, q_out, k_out each (z, h, n, d), then the positions' (z, n). Rows need
+ * unit D stride and 16-byte alignment (TATTN_ERR_LAYOUT). Z * N * max(H, Hk) < 2^30 (TATTN_ERR_TOO_LARGE). */
+TATTN_API int tattn_qk_norm_rope(const void* q, const void* k, const void* wq, const void* wk, void* q_out, void* k_out,
+                       const float* cos, const float* sin, const int32_t* positions, const int64_t* strides,
+                       int Z, int H, int Hk, int N, int D, int P, int dtype, int w_dtype, float eps,
+                       int interleaved, void* stream);
+
+/* Its gradients: dq, dk from q_grad, k_grad (the gradients of q_out, k_out), and dwq, dwk [D] of w_dtype, summed
+ * over rows in a fixed order. strides: 26 int64 = q, k, q_grad, k_grad, dq, dk each (z, h, n, d), then the
+ * positions' (z, n). workspace: tattn_qk_norm_rope_bwd_workspace_bytes bytes, 16-byte aligned. */
+TATTN_API int tattn_qk_norm_rope_bwd(const void* q, const void* k, const void* wq, const void* wk, const void* q_grad,
+                           const void* k_grad, void* dq, void* dk, void* dwq, void* dwk, const float* cos,
+                           const float* sin, const int32_t* positions, void* workspace, const int64_t* strides,
+                           int Z, int H, int Hk, int N, int D, int P, int dtype, int w_dtype, float eps,
+                           int interleaved, void* stream);
+
+/* Bytes of that workspace on the current device, or -1 for an invalid head dim. */
+TATTN_API int64_t tattn_qk_norm_rope_bwd_workspace_bytes(int D);
 
 /* Largest Z*H*N accepted by tattn_bwd_noalloc (its fixed fp32 row buffer: 16 MiB per GPU). */
 #define TATTN_BWD_NOALLOC_MAX_ROWS 4194304

@@ -1671,8 +1671,6 @@ cudaError_t launch_common(Kern kern, int smem, long long grid, const CUtensorMap
   return cudaGetLastError();
 }
 
-int sm_count();
-
 // dQ pass of the split backward, tile variant with BK-row key blocks: 128 (D <= 64; persistent when every
 // tile costs the same, i.e. not causal) or 64 (the ping-pong kernel with alternating blocks).
 template <int D, bool CAUSAL, int BK>
@@ -1686,7 +1684,7 @@ cudaError_t dq_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensor
     if (e != cudaSuccess) return e;
     if (tiles <= 0) return cudaSuccess;
     if (tiles > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-    const unsigned grid = unsigned(tiles < sm_count() ? tiles : sm_count());
+    const unsigned grid = unsigned(tiles < device_sm_count() ? tiles : device_sm_count());
     kern<<<dim3(grid), dim3(kThreads), smem, s>>>(tq, tk, tv, tdo, tdq, a);
     return cudaGetLastError();
   } else if constexpr (BK == 128 && D <= 64) {
@@ -1698,18 +1696,6 @@ cudaError_t dq_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensor
   } else {
     return cudaErrorNotSupported;
   }
-}
-
-// Streaming multiprocessors of the current device (cached per device).
-int sm_count() {
-  static int cache[64] = {0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (cache[dev] == 0) {
-    int n = 0;
-    cache[dev] = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0 ? n : 148;
-  }
-  return cache[dev];
 }
 
 // dK/dV pass of the split backward, tile variant with BQ-row query blocks: 128 (D <= 64; persistent
@@ -1726,7 +1712,7 @@ cudaError_t dkdv_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
     if (e != cudaSuccess) return e;
     if (tiles <= 0) return cudaSuccess;
     if (tiles > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-    const unsigned grid = unsigned(tiles < sm_count() ? tiles : sm_count());
+    const unsigned grid = unsigned(tiles < device_sm_count() ? tiles : device_sm_count());
     kern<<<dim3(grid), dim3(kThreads), smem, s>>>(tq, tk, tv, tdo, tdk, tdv, a);
     return cudaGetLastError();
   } else if constexpr (BQ == 64 || D <= 64) {
@@ -2517,7 +2503,7 @@ cudaError_t fused_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUten
   if (tiles > 0x7fffffffLL || units > 0x7fffffffLL - 1024) return cudaErrorInvalidConfiguration;
   // One CTA per SM at most (shared memory), so a cooperative launch keeps every CTA resident: the grid
   // barrier before the kernel's last phase needs that (its counter is zeroed by the preprocess).
-  const unsigned grid = unsigned(units < sm_count() ? units : sm_count());
+  const unsigned grid = unsigned(units < device_sm_count() ? units : device_sm_count());
   BwdArgs args = a;
   CUtensorMap m[7] = {tq, tk, tv, tdo, tdk, tdv, tdqacc};
   void* params[8] = {&m[0], &m[1], &m[2], &m[3], &m[4], &m[5], &m[6], &args};

@@ -47,6 +47,7 @@ int current_device(int* dev) {
 
 // Once per device (with that device current): check it is sm_100 and resolve the status word address.
 int device_setup(DeviceState** out) {
+  *out = nullptr;
   int dev;
   int rc = current_device(&dev);
   if (rc != TATTN_OK) return rc;
@@ -139,13 +140,32 @@ int encode_f32_dense(CUtensorMap* tm, void* p, int Z, int H, int N, int D, int b
   return r == CUDA_SUCCESS ? TATTN_OK : TATTN_ERR_LAYOUT;
 }
 
+}  // namespace
+
 int cuda_rc(cudaError_t e) {
   if (e == cudaSuccess) return TATTN_OK;
   if (e == cudaErrorNotSupported) return TATTN_ERR_UNSUPPORTED;
   return TATTN_ERR_CUDA;
 }
 
-}  // namespace
+int device_ready(int** status) {
+  DeviceState* st;
+  const int rc = device_setup(&st);
+  *status = st == nullptr ? nullptr : st->status;
+  return rc;
+}
+
+int device_sm_count() {
+  static std::atomic<int> cache[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 148;
+  if (cache[dev].load() == 0) {
+    int n = 0;
+    cache[dev].store(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0 ? n : 148);
+  }
+  return cache[dev].load();
+}
+
 }  // namespace tattn
 
 using namespace tattn;

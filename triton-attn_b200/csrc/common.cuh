@@ -17,6 +17,7 @@ namespace tattn {
 enum : int {
   kStatusWaitTimeout = 1 << 0,  // an mbarrier wait exceeded the launch's wait limit
   kStatusAborted = 1 << 1,      // a CTA unwound because a sibling role timed out
+  kStatusIndexRange = 1 << 2,   // a position or length on the device lies outside its table or cache
 };
 
 constexpr unsigned long long kDefaultWaitLimitNs = 1000ull * 1000ull * 1000ull;  // 1 s

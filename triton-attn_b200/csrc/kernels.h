@@ -70,6 +70,13 @@ struct BwdArgs {
   float* part;       // kMaskWindow, fused backward: partial dV and dK of the split key tiles, or null
 };
 
+// Host helpers of the C-ABI layer (capi.cu). device_ready: the current device is an sm_100 one whose primary
+// context is current on this thread, and *status its status word (a TATTN_* code). device_sm_count: its
+// streaming multiprocessors (cached per device). cuda_rc: a launch's result as a TATTN_* code.
+int device_ready(int** status);
+int device_sm_count();
+int cuda_rc(cudaError_t e);
+
 // `variant` below is a 0-based tile variant of tiles.h (kFwdTiles / kBwdTiles); launchers return
 // cudaErrorNotSupported for a variant that does not fit head dim D.
 // Rows per K/V block of the fp16 forward variant for head dim D: the TMA box height of its K and V
@@ -131,5 +138,34 @@ cudaError_t launch_bwd_dkdv_f32(int D, Mask mask, const BwdArgs& a, cudaStream_t
 // delta = rowsum(dO * O) in fp32 (fp16 or fp32 inputs); also zeroes the rows of a.dq_acc and the
 // counter a.grid_sync when they are set (the fused backward's workspace).
 cudaError_t launch_bwd_preprocess(int D, bool is_f16, const BwdArgs& a, cudaStream_t s);
+
+// Norms and rotation of query and key heads (norm_rope.cu). Strides in elements; the D stride is 1 and rows
+// are 16-byte aligned.
+struct Strides3 {
+  int64_t z, h, n;
+};
+struct RopeTensor {
+  const void* px;   // [Z, H, N, D]
+  const void* pdy;  // backward: the gradient of the result
+  void* py;         // the result or, backward, dx
+  const void* w;    // [D]
+  void* dw;         // backward: [D]
+  Strides3 x, dy, y;
+  int H;
+  int items, blocks;  // work items and CTAs (set by the launcher)
+};
+struct RopeArgs {
+  RopeTensor t[2];            // queries, keys
+  const float *cos, *sin;     // [P, D / 2] dense
+  const int* positions;       // [Z, N], or null: a row's own index n
+  int64_t pos_z, pos_n;
+  float* part;                // backward: a [D] partial of dw for each CTA (kRopeBlocksPerSm * SMs + 2 at most)
+  int Z, N, P;
+  int w_f32;                  // weights (and dw) are fp32, else the tensors' type
+  float eps;
+  int* status;
+};
+constexpr int kRopeBlocksPerSm = 4;
+cudaError_t launch_norm_rope(int D, bool is_f16, bool interleaved, bool backward, RopeArgs a, cudaStream_t s);
 
 }  // namespace tattn

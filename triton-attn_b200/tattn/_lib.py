@@ -17,7 +17,7 @@ TATTN_F16, TATTN_F32 = 0, 1
 OK, ERR_INVALID_ARGUMENT, ERR_LAYOUT, ERR_CUDA, ERR_NO_DEVICE, ERR_DEVICE_STATUS, ERR_UNSUPPORTED = range(7)
 ERR_TOO_LARGE = 7
 BWD_NOALLOC_MAX_ROWS = 4194304  # TATTN_BWD_NOALLOC_MAX_ROWS
-DEV_WAIT_TIMEOUT, DEV_ABORTED = 1, 2  # device status word bits (TATTN_DEV_*)
+DEV_WAIT_TIMEOUT, DEV_ABORTED, DEV_INDEX_RANGE = 1, 2, 4  # device status word bits (TATTN_DEV_*)
 
 # Every symbol include/tattn.h declares, with its ctypes signature.
 _P, _I, _F, _I64P = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.POINTER(ctypes.c_int64)
@@ -33,6 +33,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tattn_window_fwd": (_I, [_P, _P, _P, _P, _P, _I64P, *[_I] * 9, _F, _P]),
     "tattn_window_bwd": (_I, [*[_P] * 11, _I64P, *[_I] * 9, _F, _P]),
     "tattn_window_bwd_workspace_bytes": (ctypes.c_int64, [_I] * 9),
+    "tattn_qk_norm_rope": (_I, [*[_P] * 9, _I64P, *[_I] * 8, _F, _I, _P]),
+    "tattn_qk_norm_rope_bwd": (_I, [*[_P] * 14, _I64P, *[_I] * 8, _F, _I, _P]),
+    "tattn_qk_norm_rope_bwd_workspace_bytes": (ctypes.c_int64, [_I]),
     "tattn_layout_ok": (_I, [_P, _I64P, _I, _I, _I, _I]),
     "tattn_selftest_exp2": (_I, [_P, _P, _P, _P, _I, _P]),
     "tattn_selftest_exp2_poly4": (_I, [_P, _P, _I, _P]),
