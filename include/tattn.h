@@ -157,6 +157,47 @@ TATTN_API int tattn_qk_norm_rope_bwd(const void* q, const void* k, const void* w
 /* Bytes of that workspace on the current device, or -1 for an invalid head dim. */
 TATTN_API int64_t tattn_qk_norm_rope_bwd_workspace_bytes(int D);
 
+/* Attention of one new token of each sequence over a cache (no reference counterpart): the single-token form of
+ * tattn_window_fwd. q, o: [Z, H, 1, D]; k, v: [Z, Hk, C, D], of which sequence z holds the first lengths[z]
+ * tokens (device int32 [Z]), the query's own as the last. The query sees the last `window` of them (window <=
+ * 0: all) and the first `sinks`; nothing held gives zeros. A length outside [0, C] is taken as the nearer
+ * end and sets TATTN_DEV_INDEX_RANGE. Rows past a length are never used, whatever they hold.
+ * strides: 16 int64 = q, k, v, o each (z, h, n, d); rows need unit D stride and 16-byte alignment.
+ * workspace: tattn_decode_workspace_bytes bytes, 16-byte aligned (0 bytes: may be null). */
+TATTN_API int tattn_decode(const void* q, const void* k, const void* v, const int32_t* lengths, void* o, void* workspace,
+                 const int64_t* strides, int Z, int H, int Hk, int C, int D, int dtype, int window, int sinks,
+                 float sm_scale, void* stream);
+
+/* Bytes of the workspace that tattn_decode needs on the current device, or -1 for invalid arguments. It goes
+ * by the sizes alone, so one workspace serves a whole generation on one stream. */
+TATTN_API int64_t tattn_decode_workspace_bytes(int Z, int H, int Hk, int C, int D, int dtype, int window, int sinks);
+
+/* A cache of keys and values held in 4 bits (no reference counterpart), D = 64 or 128. For k and v each: codes
+ * [Z, Hk, C, D / 2] bytes (head dim 2 i in the low half of byte i, 2 i + 1 in the high half) and params [Z, Hk,
+ * C, D / 64, 2] fp16: the scale s and minimum m of each 64 head dims of a row. Code n stands for fp16(s n + m).
+ * All dense and 16-byte aligned.
+ *
+ * Append: rows t < T (t < counts[z] where counts is given) of k, v [Z, Hk, T, D] fp16 are written at positions
+ * start[z] + t (start null: t) with m = min, s = fp16((max - m) / 15), n = round((x - m) / s), ties to even. A
+ * position outside [0, C) is not written and sets TATTN_DEV_INDEX_RANGE. start, counts: device int32 [Z].
+ * strides: 8 int64 = k, v each (z, h, n, d); rows need unit D stride and 16-byte alignment. */
+TATTN_API int tattn_int4_append(const void* k, const void* v, void* k_codes, void* k_params, void* v_codes,
+                      void* v_params, const int32_t* start, const int32_t* counts, const int64_t* strides, int Z,
+                      int Hk, int T, int C, int D, void* stream);
+
+/* Read: the values that positions start[z] + t, t < T, stand for, as dense fp16 k, v [Z, Hk, T, D]. A position
+ * outside [0, C) reads as zeros and sets TATTN_DEV_INDEX_RANGE. */
+TATTN_API int tattn_int4_read(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params,
+                    const int32_t* start, void* k, void* v, int Z, int Hk, int T, int C, int D, void* stream);
+
+/* tattn_decode over that cache; q, o fp16. strides: 8 int64 = q, o each (z, h, n, d). workspace:
+ * tattn_int4_decode_workspace_bytes bytes, 16-byte aligned (0 bytes: may be null). */
+TATTN_API int tattn_int4_decode(const void* q, const void* k_codes, const void* k_params, const void* v_codes,
+                      const void* v_params, const int32_t* lengths, void* o, void* workspace,
+                      const int64_t* strides, int Z, int H, int Hk, int C, int D, int window, int sinks,
+                      float sm_scale, void* stream);
+TATTN_API int64_t tattn_int4_decode_workspace_bytes(int Z, int H, int Hk, int C, int D, int window, int sinks);
+
 /* Largest Z*H*N accepted by tattn_bwd_noalloc (its fixed fp32 row buffer: 16 MiB per GPU). */
 #define TATTN_BWD_NOALLOC_MAX_ROWS 4194304
 

@@ -1,4 +1,5 @@
-// C-ABI boundary (include/tattn.h) of the operators around the attention kernels: head norms with rotation.
+// C-ABI boundary (include/tattn.h) of the operators around the attention kernels: head norms with rotation,
+// the 4-bit cache, and the attention of single tokens over a cache.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -119,4 +120,168 @@ extern "C" int tattn_qk_norm_rope_bwd(const void* q, const void* k, const void* 
 extern "C" int64_t tattn_qk_norm_rope_bwd_workspace_bytes(int D) {
   if (!head_dim_ok(D)) return -1;
   return (int64_t(kRopeBlocksPerSm) * device_sm_count() + 2) * D * 4;
+}
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// The sizes that every single-token call shares; `a` gets them. window <= 0: everything.
+bool decode_dims(DecodeArgs& a, int Z, int H, int Hk, int C, int D, int window, int sinks) {
+  if (Z < 0 || H < 1 || Hk < 1 || H % Hk != 0 || C < 0 || !head_dim_ok(D) || sinks < 0 || int64_t(Z) * H > 0x3fffffff)
+    return false;
+  a.Z = Z;
+  a.H = H;
+  a.Hk = Hk;
+  a.C = C;
+  a.window = window > 0 && window < C ? window : C;
+  a.sinks = sinks < C ? sinks : C;
+  return true;
+}
+
+int64_t decode_workspace(const DecodeArgs& a, int D, int nsplit) {
+  return nsplit == 1 ? 0 : int64_t(a.Z) * a.H * nsplit * (D + 2) * 4;
+}
+
+int decode(DecodeArgs& a, int D, DecodeCache cache, void* workspace, float sm_scale, void* stream) {
+  int rc = device_ready(&a.status);
+  if (rc != TATTN_OK) return rc;
+  a.nsplit = decode_splits(a, D, cache);
+  if (a.nsplit > 1) {
+    if (!workspace) return TATTN_ERR_INVALID_ARGUMENT;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return TATTN_ERR_LAYOUT;
+    a.part = static_cast<float*>(workspace);
+    a.part_ml = a.part + int64_t(a.Z) * a.H * a.nsplit * D;
+  }
+  a.qk_scale = sm_scale * kLog2e;
+  return cuda_rc(launch_decode(D, cache, a, static_cast<cudaStream_t>(stream)));
+}
+
+}  // namespace
+
+extern "C" int tattn_decode(const void* q, const void* k, const void* v, const int32_t* lengths, void* o,
+                            void* workspace, const int64_t* strides, int Z, int H, int Hk, int C, int D, int dtype,
+                            int window, int sinks, float sm_scale, void* stream) {
+  DecodeArgs a{};
+  if (!strides || !decode_dims(a, Z, H, Hk, C, D, window, sinks) || (dtype != TATTN_F16 && dtype != TATTN_F32))
+    return TATTN_ERR_INVALID_ARGUMENT;
+  if (Z == 0) return TATTN_OK;
+  if (!q || !lengths || !o || (C > 0 && (!k || !v))) return TATTN_ERR_INVALID_ARGUMENT;
+  const int64_t *sq = strides, *sk = strides + 4, *sv = strides + 8, *so = strides + 12;
+  const int esz = dtype == TATTN_F16 ? 2 : 4;
+  if (!rows16(q, sq, Z, H, 1, esz) || !rows16(o, so, Z, H, 1, esz) || !rows16(k, sk, Z, Hk, C, esz) ||
+      !rows16(v, sv, Z, Hk, C, esz))
+    return TATTN_ERR_LAYOUT;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.o = o;
+  a.lengths = lengths;
+  a.sq = strides3(sq);
+  a.sk = strides3(sk);
+  a.sv = strides3(sv);
+  a.so = strides3(so);
+  return decode(a, D, dtype == TATTN_F16 ? kCacheF16 : kCacheF32, workspace, sm_scale, stream);
+}
+
+extern "C" int64_t tattn_decode_workspace_bytes(int Z, int H, int Hk, int C, int D, int dtype, int window, int sinks) {
+  DecodeArgs a{};
+  if (!decode_dims(a, Z, H, Hk, C, D, window, sinks) || (dtype != TATTN_F16 && dtype != TATTN_F32)) return -1;
+  return decode_workspace(a, D, decode_splits(a, D, dtype == TATTN_F16 ? kCacheF16 : kCacheF32));
+}
+
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+bool int4_dims(int Z, int Hk, int T, int C, int D) {
+  return Z >= 0 && Hk >= 1 && T >= 0 && C >= 0 && (D == 64 || D == 128);
+}
+
+}  // namespace
+
+extern "C" int tattn_int4_append(const void* k, const void* v, void* k_codes, void* k_params, void* v_codes,
+                                 void* v_params, const int32_t* start, const int32_t* counts, const int64_t* strides,
+                                 int Z, int Hk, int T, int C, int D, void* stream) {
+  if (!strides || !int4_dims(Z, Hk, T, C, D)) return TATTN_ERR_INVALID_ARGUMENT;
+  if (int64_t(Z) * T == 0) return TATTN_OK;
+  if (!k || !v || !k_codes || !k_params || !v_codes || !v_params) return TATTN_ERR_INVALID_ARGUMENT;
+  if (!rows16(k, strides, Z, Hk, T, 2) || !rows16(v, strides + 4, Z, Hk, T, 2) || !aligned16(k_codes) ||
+      !aligned16(k_params) || !aligned16(v_codes) || !aligned16(v_params))
+    return TATTN_ERR_LAYOUT;
+  Int4CacheArgs a{};
+  const int rc = device_ready(&a.status);
+  if (rc != TATTN_OK) return rc;
+  a.k = k;
+  a.v = v;
+  a.sk = strides3(strides);
+  a.sv = strides3(strides + 4);
+  a.k_codes = static_cast<uint8_t*>(k_codes);
+  a.v_codes = static_cast<uint8_t*>(v_codes);
+  a.k_params = k_params;
+  a.v_params = v_params;
+  a.start = start;
+  a.counts = counts;
+  a.Z = Z;
+  a.Hk = Hk;
+  a.T = T;
+  a.C = C;
+  return cuda_rc(launch_int4_append(D, a, static_cast<cudaStream_t>(stream)));
+}
+
+extern "C" int tattn_int4_read(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params,
+                               const int32_t* start, void* k, void* v, int Z, int Hk, int T, int C, int D,
+                               void* stream) {
+  if (!int4_dims(Z, Hk, T, C, D)) return TATTN_ERR_INVALID_ARGUMENT;
+  if (int64_t(Z) * T == 0) return TATTN_OK;
+  if (!k || !v || (C > 0 && (!k_codes || !k_params || !v_codes || !v_params))) return TATTN_ERR_INVALID_ARGUMENT;
+  if (!aligned16(k) || !aligned16(v) || !aligned16(k_codes) || !aligned16(k_params) || !aligned16(v_codes) ||
+      !aligned16(v_params))
+    return TATTN_ERR_LAYOUT;
+  Int4CacheArgs a{};
+  const int rc = device_ready(&a.status);
+  if (rc != TATTN_OK) return rc;
+  a.k_out = k;
+  a.v_out = v;
+  a.k_codes = static_cast<uint8_t*>(const_cast<void*>(k_codes));
+  a.v_codes = static_cast<uint8_t*>(const_cast<void*>(v_codes));
+  a.k_params = const_cast<void*>(k_params);
+  a.v_params = const_cast<void*>(v_params);
+  a.start = start;
+  a.Z = Z;
+  a.Hk = Hk;
+  a.T = T;
+  a.C = C;
+  return cuda_rc(launch_int4_read(D, a, static_cast<cudaStream_t>(stream)));
+}
+
+extern "C" int tattn_int4_decode(const void* q, const void* k_codes, const void* k_params, const void* v_codes,
+                                 const void* v_params, const int32_t* lengths, void* o, void* workspace,
+                                 const int64_t* strides, int Z, int H, int Hk, int C, int D, int window, int sinks,
+                                 float sm_scale, void* stream) {
+  DecodeArgs a{};
+  if (!strides || !decode_dims(a, Z, H, Hk, C, D, window, sinks) || !int4_dims(Z, Hk, 0, C, D))
+    return TATTN_ERR_INVALID_ARGUMENT;
+  if (Z == 0) return TATTN_OK;
+  if (!q || !lengths || !o || (C > 0 && (!k_codes || !k_params || !v_codes || !v_params)))
+    return TATTN_ERR_INVALID_ARGUMENT;
+  if (!rows16(q, strides, Z, H, 1, 2) || !rows16(o, strides + 4, Z, H, 1, 2) || !aligned16(k_codes) ||
+      !aligned16(k_params) || !aligned16(v_codes) || !aligned16(v_params))
+    return TATTN_ERR_LAYOUT;
+  a.q = q;
+  a.o = o;
+  a.k = k_codes;
+  a.v = v_codes;
+  a.k_params = k_params;
+  a.v_params = v_params;
+  a.lengths = lengths;
+  a.sq = strides3(strides);
+  a.so = strides3(strides + 4);
+  return decode(a, D, kCacheInt4, workspace, sm_scale, stream);
+}
+
+extern "C" int64_t tattn_int4_decode_workspace_bytes(int Z, int H, int Hk, int C, int D, int window, int sinks) {
+  DecodeArgs a{};
+  if (!decode_dims(a, Z, H, Hk, C, D, window, sinks) || !int4_dims(Z, Hk, 0, C, D)) return -1;
+  return decode_workspace(a, D, decode_splits(a, D, kCacheInt4));
 }

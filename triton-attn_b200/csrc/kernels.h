@@ -168,4 +168,43 @@ struct RopeArgs {
 constexpr int kRopeBlocksPerSm = 4;
 cudaError_t launch_norm_rope(int D, bool is_f16, bool interleaved, bool backward, RopeArgs a, cudaStream_t s);
 
+// Attention of single tokens over a cache (decode.cu).
+enum DecodeCache : int { kCacheF16, kCacheInt4, kCacheF32 };
+struct DecodeArgs {
+  const void* q;        // [Z, H, D]
+  void* o;              // [Z, H, D]
+  const void *k, *v;    // [Z, Hk, C, D], or the 4-bit cache's codes (Int4CacheArgs)
+  const void *k_params, *v_params;  // 4-bit cache: its scales and minima
+  Strides3 sq, so, sk, sv;
+  const int* lengths;   // [Z]: tokens held, the query's own among them
+  float* part;          // [Z, H, nsplit, D] unnormalised partial rows (nsplit > 1)
+  float* part_ml;       // [Z, H, nsplit, 2] their maxima and sums
+  int Z, H, Hk, C;
+  int window, sinks;    // window >= C: everything
+  int nsplit;
+  float qk_scale;       // sm_scale * log2(e)
+  int* status;
+};
+// CTAs per SM that decode_splits aims at.
+constexpr int kDecodeCtas = 4;
+// Parts that the visible tokens are cut into: by the sizes alone, never by the lengths on the device.
+int decode_splits(const DecodeArgs& a, int D, DecodeCache cache);
+// The 4-bit cache (int4_cache.cu), for k and v each: codes [Z, Hk, C, D / 2] bytes, head dim 2 i in the low half
+// of byte i; params [Z, Hk, C, D / 64, 2] fp16, the scale and minimum of each 64 head dims. All dense.
+struct Int4CacheArgs {
+  const void *k, *v;                // append: [Z, Hk, T, D] fp16 rows
+  Strides3 sk, sv;
+  void *k_out, *v_out;              // read: dense [Z, Hk, T, D] fp16
+  uint8_t *k_codes, *v_codes;
+  void *k_params, *v_params;
+  const int* start;                 // [Z], or null (0): the position of row t = 0
+  const int* counts;                // append, [Z], or null (T): rows t >= counts[z] are not kept
+  int Z, Hk, T, C;
+  int* status;
+};
+cudaError_t launch_int4_append(int D, const Int4CacheArgs& a, cudaStream_t s);
+cudaError_t launch_int4_read(int D, const Int4CacheArgs& a, cudaStream_t s);
+
+cudaError_t launch_decode(int D, DecodeCache cache, const DecodeArgs& a, cudaStream_t s);
+
 }  // namespace tattn

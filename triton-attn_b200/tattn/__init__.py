@@ -2,7 +2,16 @@
 ``tattn`` package (src/tattn/__init__.py:3-5)."""
 
 from tattn.api import attention, cuda_available, triton_available
+from tattn.decode import Int4Cache, decode_attention
 from tattn.norm_rope import qk_norm_rope
 from tattn.window import window_attention
 
-__all__ = ["attention", "cuda_available", "qk_norm_rope", "triton_available", "window_attention"]
+__all__ = [
+    "Int4Cache",
+    "attention",
+    "cuda_available",
+    "decode_attention",
+    "qk_norm_rope",
+    "triton_available",
+    "window_attention",
+]

@@ -36,6 +36,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tattn_qk_norm_rope": (_I, [*[_P] * 9, _I64P, *[_I] * 8, _F, _I, _P]),
     "tattn_qk_norm_rope_bwd": (_I, [*[_P] * 14, _I64P, *[_I] * 8, _F, _I, _P]),
     "tattn_qk_norm_rope_bwd_workspace_bytes": (ctypes.c_int64, [_I]),
+    "tattn_decode": (_I, [*[_P] * 6, _I64P, *[_I] * 8, _F, _P]),
+    "tattn_decode_workspace_bytes": (ctypes.c_int64, [_I] * 8),
+    "tattn_int4_append": (_I, [*[_P] * 8, _I64P, *[_I] * 5, _P]),
+    "tattn_int4_read": (_I, [*[_P] * 7, *[_I] * 5, _P]),
+    "tattn_int4_decode": (_I, [*[_P] * 8, _I64P, *[_I] * 7, _F, _P]),
+    "tattn_int4_decode_workspace_bytes": (ctypes.c_int64, [_I] * 7),
     "tattn_layout_ok": (_I, [_P, _I64P, _I, _I, _I, _I]),
     "tattn_selftest_exp2": (_I, [_P, _P, _P, _P, _I, _P]),
     "tattn_selftest_exp2_poly4": (_I, [_P, _P, _I, _P]),
