@@ -128,7 +128,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // The sizes that every single-token call shares; `a` gets them. window <= 0: everything.
 bool decode_dims(DecodeArgs& a, int Z, int H, int Hk, int C, int D, int window, int sinks) {
-  if (Z < 0 || H < 1 || Hk < 1 || H % Hk != 0 || C < 0 || !head_dim_ok(D) || sinks < 0 || int64_t(Z) * H > 0x3fffffff)
+  if (Z < 0 || H < 1 || Hk < 1 || H % Hk != 0 || C < 0 || C > (1 << 30) || !head_dim_ok(D) || sinks < 0 || int64_t(Z) * H > 0x3fffffff)
     return false;
   a.Z = Z;
   a.H = H;

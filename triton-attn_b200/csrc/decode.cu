@@ -113,15 +113,23 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The same with c = a b.
+__device__ __forceinline__ void mma16816_first(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // A warp's running softmax over its tiles. Lane (g, t) holds columns (query heads) 2t, 2t + 1 of each of the
-// NT 8-head tiles: the maximum m (base-2 scaled scores, the same in all g) and its own rows' share of the
-// sum l. M tiles of 16 output dims: o[mt][nt] as mma16816's c.
+// NT 8-head tiles: off = -m for a maximum m of the base-2 scores (the same in all g; +infinity before the first
+// tile) and its own rows' share of the sum l. M tiles of 16 output dims: o[mt][nt] as mma16816's c.
 template <int D, int NT>
 struct WarpState {
-  float m[NT][2], l[NT][2], o[D / 16][NT][4];
+  float off[NT][2], l[NT][2], o[D / 16][NT][4];
   __device__ __forceinline__ void reset() {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
+    for (int nt = 0; nt < NT; ++nt) off[nt][0] = off[nt][1] = INFINITY, l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
     for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
@@ -131,51 +139,78 @@ struct WarpState {
   }
 };
 
-// Scores x[s][nt] (16-key subtile s; as mma16816's c, in base 2) become p = 2^(x - m) with the maximum taken
-// over all keys so far; alpha is what sums made before are to be multiplied by (if the result, uniform over
-// the warp, is true). The lane's keys are 16 s + row and 16 s + row + 8; those from `left` on do not exist.
-template <int D, int NT, int NS>
-__device__ __forceinline__ bool softmax_tile(WarpState<D, NT>& st, float (*x)[NT][4], int left, int row, float (*alpha)[2]) {
-  bool grown = false;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        if (16 * s + row >= left) x[s][nt][e] = -INFINITY;
-        if (16 * s + row + 8 >= left) x[s][nt][2 + e] = -INFINITY;
-        mx = fmax3(mx, x[s][nt][e], x[s][nt][2 + e]);
-      }
-#pragma unroll
-      for (int o = 4; o < 32; o *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      mx = fmaxf(mx, st.m[nt][e]);
-      grown |= mx > st.m[nt][e];
-      const float use = mx == -INFINITY ? 0.f : mx;
-      alpha[nt][e] = ex2_approx(st.m[nt][e] - use);
-      st.m[nt][e] = mx;
-      float sum = 0.f;
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        x[s][nt][e] = ex2_approx(x[s][nt][e] - use);
-        x[s][nt][2 + e] = ex2_approx(x[s][nt][2 + e] - use);
-        sum += x[s][nt][e] + x[s][nt][2 + e];
-      }
-      st.l[nt][e] = fmaf(st.l[nt][e], alpha[nt][e], sum);
-    }
-  }
-  return __any_sync(0xffffffffu, grown);
+__device__ __forceinline__ float positive_scale(float qk_scale) {
+  // Below 2^-60 scores vanish against 1: a scale of 0 gives the weights that it should and still leaves the
+  // -infinity of a key that does not exist what it is. The sign goes into Q.
+  return fmaxf(fabsf(qk_scale), 0x1p-60f);
 }
-
 template <int D, int NT>
 __device__ __forceinline__ void rescale(WarpState<D, NT>& st, const float (*alpha)[2]) {
 #pragma unroll
-  for (int mt = 0; mt < D / 16; ++mt)
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      st.l[nt][e] *= alpha[nt][e];
+#pragma unroll
+      for (int mt = 0; mt < D / 16; ++mt) {
+        st.o[mt][nt][e] *= alpha[nt][e];
+        st.o[mt][nt][2 + e] *= alpha[nt][e];
+      }
+    }
+}
+
+// Raw scores x[s][nt] (16-key subtile s; as mma16816's c) become p = 2^(scale (x - m)). The lane's keys are
+// 16 s + row and 16 s + row + 8; those from `left` on do not exist. m, a column's maximum over the keys so far,
+// is only raised (and what was summed before rescaled) where some x lies more than 2^kRaise above it in
+// weight: until then p <= 2^kRaise does fp16 no harm, and a tile takes a vote in place of the maximum's
+// shuffles. scale > 0 (positive_scale).
+constexpr float kRaise = 8.f;
+template <int D, int NT, int NS>
+__device__ __forceinline__ void softmax_tile(WarpState<D, NT>& st, float (*x)[NT][4], int left, int row, float scale) {
+  if (left < 16 * NS) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (16 * s + row + e / 2 * 8 >= left) x[s][nt][e] = -INFINITY;
+  }
+  float mx[NT][2];
+  bool raise = false;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      mx[nt][e] = fmaxf(x[0][nt][e], x[0][nt][2 + e]);
+#pragma unroll
+      for (int s = 1; s < NS; ++s) mx[nt][e] = fmax3(mx[nt][e], x[s][nt][e], x[s][nt][2 + e]);
+      raise |= fmaf(mx[nt][e], scale, st.off[nt][e]) > kRaise;
+    }
+  if (__any_sync(0xffffffffu, raise)) {
+    float alpha[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) st.o[mt][nt][e] *= alpha[nt][e % 2];
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 4; o < 32; o *= 2) mx[nt][e] = fmaxf(mx[nt][e], __shfl_xor_sync(0xffffffffu, mx[nt][e], o));
+        const float off = fminf(-scale * mx[nt][e], st.off[nt][e]);
+        alpha[nt][e] = st.off[nt][e] == INFINITY ? 0.f : ex2_approx(off - st.off[nt][e]);
+        st.off[nt][e] = off;
+      }
+    rescale(st, alpha);
+  }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        x[s][nt][e] = ex2_approx(fmaf(x[s][nt][e], scale, st.off[nt][e]));
+        x[s][nt][2 + e] = ex2_approx(fmaf(x[s][nt][2 + e], scale, st.off[nt][e]));
+        st.l[nt][e] += x[s][nt][e] + x[s][nt][2 + e];
+      }
 }
 
 // Joins the warps' results through shared memory (kWarps * 8 NT * (D + 2) floats) and writes the CTA's part:
@@ -195,7 +230,7 @@ __device__ __forceinline__ void finish(const DecodeArgs& a, const Part& p, WarpS
       for (int o = 4; o < 32; o *= 2) l += __shfl_xor_sync(0xffffffffu, l, o);
       const int head = 8 * nt + 2 * t + e;
       if (g == 0) {
-        ml[(warp * HEADS + head) * 2] = st.m[nt][e];
+        ml[(warp * HEADS + head) * 2] = -st.off[nt][e];
         ml[(warp * HEADS + head) * 2 + 1] = l;
       }
 #pragma unroll
@@ -265,26 +300,42 @@ __global__ void __launch_bounds__(kThreads) decode_f16_kernel(const DecodeArgs a
   const __half* kb = static_cast<const __half*>(a.k) + p.z * a.sk.z + p.hk * a.sk.h;
   const __half* vb = static_cast<const __half*>(a.v) + p.z * a.sv.z + p.hk * a.sv.h;
 
-  // Tile i of this warp: tokens from t0 + (i * kWarps + warp) * KT.
-  auto load = [&](int i, int stage) {
-    const int base = p.t0 + (i * kWarps + warp) * C::KT;
-    const uint32_t dst = ring + stage * 2 * C::TILE;
+  // A tile of this warp: tokens from `base` on, into ring slot `to`.
+  auto load = [&](int base, uint32_t to) {
+    constexpr int ROWS = 32 / (D / 8) > 0 ? 32 / (D / 8) : 1;  // rows a step of the warp copies
+    const int row = lane / (D / 8), unit = lane % (D / 8);
+    if (base >= vis.sinks && base + C::KT <= p.t1) {  // rows one after another
+      const __half* k = kb + int64_t(base + vis.jump + row) * a.sk.n + unit * 8;
+      const __half* v = vb + int64_t(base + vis.jump + row) * a.sv.n + unit * 8;
 #pragma unroll
-    for (int j = 0; j < C::KT * (D / 8) / 32; ++j) {
-      const int e = j * 32 + lane, row = e / (D / 8), unit = e % (D / 8);
-      const bool in = base + row < p.t1;
-      const int64_t tok = in ? vis.token(base + row) : 0;  // rows past the end are zeros
-      cp_async16(dst + row_unit<D>(row, unit), kb + tok * a.sk.n + unit * 8, in);
-      cp_async16(dst + C::TILE + row_unit<D>(row, unit), vb + tok * a.sv.n + unit * 8, in);
+      for (int j = 0; j < C::KT / ROWS; ++j) {
+        cp_async16(to + row_unit<D>(j * ROWS + row, unit), k, true);
+        cp_async16(to + C::TILE + row_unit<D>(j * ROWS + row, unit), v, true);
+        k += ROWS * a.sk.n;
+        v += ROWS * a.sv.n;
+      }
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < C::KT / ROWS; ++j) {
+      const int t = base + j * ROWS + row;
+      const bool in = t < p.t1;
+      const int64_t tok = in ? vis.token(t) : 0;  // rows past the end are zeros
+      cp_async16(to + row_unit<D>(j * ROWS + row, unit), kb + tok * a.sk.n + unit * 8, in);
+      cp_async16(to + C::TILE + row_unit<D>(j * ROWS + row, unit), vb + tok * a.sv.n + unit * 8, in);
     }
   };
-  const int tiles = max(0, (p.t1 - p.t0 - warp * C::KT + kWarps * C::KT - 1) / (kWarps * C::KT));
+  // The warp's tiles begin at every kWarps * KT-th token from `base` on; the next load is STAGES - 1 ahead.
+  constexpr int STEP = kWarps * C::KT;
+  int base = p.t0 + warp * C::KT, slot = 0, next = C::STAGES - 1;
 #pragma unroll
   for (int i = 0; i < C::STAGES - 1; ++i) {
-    if (i < tiles) load(i, i);
+    if (base + i * STEP < p.t1) load(base + i * STEP, ring + i * 2 * C::TILE);
     cp_async_commit();
   }
 
+  const float scale = positive_scale(a.qk_scale);
+  const uint32_t sign = a.qk_scale < 0.f ? 0x80008000u : 0u;
   // Q^T as the B operand: column g is head g, rows are dims.
   uint32_t q[D / 16][NT][2];
 #pragma unroll
@@ -295,37 +346,33 @@ __global__ void __launch_bounds__(kThreads) decode_f16_kernel(const DecodeArgs a
     for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        q[kk][nt][e] = head < p.heads ? *reinterpret_cast<const uint32_t*>(qr + kk * 16 + 2 * t + 8 * e) : 0u;
+        q[kk][nt][e] =
+            head < p.heads ? *reinterpret_cast<const uint32_t*>(qr + kk * 16 + 2 * t + 8 * e) ^ sign : 0u;
   }
 
   WarpState<D, NT> st;
   st.reset();
-  for (int i = 0; i < tiles; ++i) {
+  for (; base < p.t1; base += STEP) {
     cp_async_wait<C::STAGES - 2>();
     __syncwarp();
-    const uint32_t kt = ring + (i % C::STAGES) * 2 * C::TILE, vt = kt + C::TILE;
+    const uint32_t kt = ring + slot * 2 * C::TILE, vt = kt + C::TILE;
     float x[C::NS][NT][4];
 #pragma unroll
     for (int s = 0; s < C::NS; ++s) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[s][nt][e] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         uint32_t f[4];  // keys 0-7, 8-15 at 8 dims, then at the next 8
         ldmatrix_x4(f, kt + row_unit<D>(16 * s + lane % 16, 2 * kk + lane / 16));
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16816(x[s][nt], f, q[kk][nt][0], q[kk][nt][1]);
+        for (int nt = 0; nt < NT; ++nt) {
+          if (kk == 0)
+            mma16816_first(x[s][nt], f, q[kk][nt][0], q[kk][nt][1]);
+          else
+            mma16816(x[s][nt], f, q[kk][nt][0], q[kk][nt][1]);
+        }
       }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[s][nt][e] *= a.qk_scale;
     }
-    float alpha[NT][2];
-    const int left = p.t1 - (p.t0 + (i * kWarps + warp) * C::KT);
-    if (softmax_tile<D, NT, C::NS>(st, x, left, g, alpha)) rescale(st, alpha);
+    softmax_tile<D, NT, C::NS>(st, x, p.t1 - base, g, scale);
 #pragma unroll
     for (int s = 0; s < C::NS; ++s) {
       // P is rounded to fp16 for the matrix instruction (2^-12 relative on average per weight, the same as
@@ -344,9 +391,11 @@ __global__ void __launch_bounds__(kThreads) decode_f16_kernel(const DecodeArgs a
         for (int nt = 0; nt < NT; ++nt) mma16816(st.o[mt][nt], f, pt[nt][0], pt[nt][1]);
       }
     }
-    __syncwarp();  // every lane has read the stage that the next load overwrites
-    if (i + C::STAGES - 1 < tiles) load(i + C::STAGES - 1, (i + C::STAGES - 1) % C::STAGES);
+    __syncwarp();  // every lane has read the slot that the next load overwrites
+    if (base + (C::STAGES - 1) * STEP < p.t1) load(base + (C::STAGES - 1) * STEP, ring + next * 2 * C::TILE);
     cp_async_commit();
+    slot = slot + 1 == C::STAGES ? 0 : slot + 1;
+    next = next + 1 == C::STAGES ? 0 : next + 1;
   }
   cp_async_wait<0>();
   __syncthreads();  // the rings become the join's memory
@@ -391,10 +440,13 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
 __device__ __forceinline__ uint32_t as_bits(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
-// The values of the codes in the low (HIGH: high) 4 bits of bytes 0 and 2 of `word`.
+// The values of the codes in the low (HIGH: high) 4 bits of bytes 0 and 2 of `word`. k1024: 1024 twice, in a
+// register (an instruction has room for one constant, the mask; with two the compiler makes two of it).
 template <bool HIGH>
-__device__ __forceinline__ uint32_t code_values(uint32_t word, __half2 s, __half2 m) {
-  const __half2 x = as_half2((word & (HIGH ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u);
+__device__ __forceinline__ uint32_t code_values(uint32_t word, __half2 s, __half2 m, uint32_t k1024) {
+  uint32_t bits;  // (word & mask) | k1024
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(bits) : "r"(word), "n"(HIGH ? 0x00f000f0u : 0x000f000fu), "r"(k1024));
+  const __half2 x = as_half2(bits);
   const __half2 n = HIGH ? __hfma2(x, __float2half2_rn(0.0625f), __float2half2_rn(-64.f))
                          : __hadd2(x, __float2half2_rn(-1024.f));
   return as_bits(__hfma2(s, n, m));
@@ -414,30 +466,45 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeArgs 
   const uint8_t* params[2] = {static_cast<const uint8_t*>(a.k_params) + row0 * (GR * 4),
                               static_cast<const uint8_t*>(a.v_params) + row0 * (GR * 4)};
 
-  auto load = [&](int i, int stage) {
-    const int base = p.t0 + (i * kWarps + warp) * C::KT;
-    const uint32_t dst = ring + stage * C::TILE;
+  // A tile of this warp: tokens from `base` on, into ring slot `to`. Rows one after another are one run of
+  // bytes; the lane's place in the slot is the same for every 32 units of 16 bytes (8 or 16 rows).
+  const uint32_t place = C::at(lane / (D / 32), lane % (D / 32) / 2) + lane % 2 * 16;
+  auto load = [&](int base, uint32_t to) {
+    if (base >= vis.sinks && base + C::KT <= p.t1) {
+      const int64_t tok = base + vis.jump;
 #pragma unroll
-    for (int j = 0; j < C::CODES / 16 / 32; ++j) {
-      const int e = j * 32 + lane, row = e / (D / 32), unit = e % (D / 32);
-      const bool in = base + row < p.t1;
-      const int64_t tok = in ? vis.token(base + row) : 0;  // rows past the end are zeros
-      const uint32_t to = C::at(row, unit / 2) + unit % 2 * 16;
+      for (int x = 0; x < 2; ++x) {
+        const uint8_t* src = codes[x] + tok * (D / 2) + lane * 16;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) cp_async16(dst + x * C::CODES + to, codes[x] + tok * (D / 2) + unit * 16, in);
+        for (int j = 0; j < C::CODES / 512; ++j) cp_async16(to + x * C::CODES + place + j * 512, src + j * 512, true);
+        cp_async_small<GR * 4>(to + 2 * C::CODES + x * C::PARAMS + lane * GR * 4, params[x] + (tok + lane) * (GR * 4), true);
+      }
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < C::CODES / 512; ++j) {
+      const int e = j * 32 + lane, t = base + e / (D / 32), unit = e % (D / 32);
+      const bool in = t < p.t1;
+      const int64_t tok = in ? vis.token(t) : 0;  // rows past the end are zeros
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        cp_async16(to + x * C::CODES + place + j * 512, codes[x] + tok * (D / 2) + unit * 16, in);
     }
     const bool in = base + lane < p.t1;
     const int64_t tok = in ? vis.token(base + lane) : 0;
 #pragma unroll
     for (int x = 0; x < 2; ++x)
-      cp_async_small<GR * 4>(dst + 2 * C::CODES + x * C::PARAMS + lane * GR * 4, params[x] + tok * (GR * 4), in);
+      cp_async_small<GR * 4>(to + 2 * C::CODES + x * C::PARAMS + lane * GR * 4, params[x] + tok * (GR * 4), in);
   };
-  const int tiles = max(0, (p.t1 - p.t0 - warp * C::KT + kWarps * C::KT - 1) / (kWarps * C::KT));
+  constexpr int STEP = kWarps * C::KT;
+  int base = p.t0 + warp * C::KT, slot = 0, next = C::STAGES - 1;
 #pragma unroll
   for (int i = 0; i < C::STAGES - 1; ++i) {
-    if (i < tiles) load(i, i);
+    if (base + i * STEP < p.t1) load(base + i * STEP, ring + i * C::TILE);
     cp_async_commit();
   }
+  const float scale = positive_scale(a.qk_scale);
+  const uint32_t sign = a.qk_scale < 0.f ? 0x80008000u : 0u;
 
   // Q^T as the B operand (column g is head g), its rows in the order in which the codes of K come out of
   // their words: lane t holds 16 dims of each group, step j of 4 takes codes 2 (j % 2), + 4, + 1, + 5 of
@@ -453,7 +520,7 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeArgs 
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const uint4 x = has ? *reinterpret_cast<const uint4*>(qr + gr * kGroupDims + 8 * w) : make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t u[4] = {x.x, x.y, x.z, x.w};  // dims 0,1 | 2,3 | 4,5 | 6,7
+        const uint32_t u[4] = {x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign};  // dims 0,1 | 2,3 | 4,5 | 6,7
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           q[gr][2 * w + j][nt][0] = __byte_perm(u[j], u[j + 2], 0x5410);  // dims 2j, 2j + 4
@@ -466,40 +533,47 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeArgs 
   st.reset();
   // Keys in the order of mma16816's rows lie in the tile's rows (k >> 1) + 4 (k & 1) of each 8.
   const int row = (g >> 1) | ((g & 1) << 2);
-  for (int i = 0; i < tiles; ++i) {
+  // The lane's places in a slot: of rows `row` (K) and t, t + 4 (V), the same in every 8 rows but for 8 ROW.
+  constexpr uint32_t ROW = D / 2;
+  uint32_t at_k[GR], at_v[GR][2];
+#pragma unroll
+  for (int gr = 0; gr < GR; ++gr) {
+    at_k[gr] = C::at(row, gr) + 8 * t;
+    at_v[gr][0] = C::CODES + C::at(t, gr) + 4 * g;
+    at_v[gr][1] = C::CODES + C::at(t + 4, gr) + 4 * g;
+  }
+  uint32_t k1024;
+  asm volatile("mov.b32 %0, 0x64006400;" : "=r"(k1024));
+  const uint32_t at_kp = 2 * C::CODES + row * GR * 4, at_vp = 2 * C::CODES + C::PARAMS + t * GR * 4;
+  for (; base < p.t1; base += STEP) {
     cp_async_wait<C::STAGES - 2>();
     __syncwarp();
-    const uint32_t kt = ring + (i % C::STAGES) * C::TILE, vt = kt + C::CODES, kp = vt + C::CODES, vp = kp + C::PARAMS;
+    const uint32_t tile = ring + slot * C::TILE;
     float x[C::NS][NT][4];
 #pragma unroll
     for (int s = 0; s < C::NS; ++s) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[s][nt][e] = 0.f;
-#pragma unroll
       for (int gr = 0; gr < GR; ++gr) {
-        const uint2 lo = lds64(kt + C::at(16 * s + row, gr) + 8 * t), hi = lds64(kt + C::at(16 * s + 8 + row, gr) + 8 * t);
-        const __half2 pl = as_half2(lds32(kp + ((16 * s + row) * GR + gr) * 4));
-        const __half2 ph = as_half2(lds32(kp + ((16 * s + 8 + row) * GR + gr) * 4));
+        const uint2 lo = lds64(tile + at_k[gr] + 16 * s * ROW), hi = lds64(tile + at_k[gr] + (16 * s + 8) * ROW);
+        const __half2 pl = as_half2(lds32(tile + at_kp + (16 * s * GR + gr) * 4));
+        const __half2 ph = as_half2(lds32(tile + at_kp + ((16 * s + 8) * GR + gr) * 4));
         const __half2 sl = __low2half2(pl), ml = __high2half2(pl), sh = __low2half2(ph), mh = __high2half2(ph);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t wl = (j < 2 ? lo.x : lo.y) >> (j % 2 * 8), wh = (j < 2 ? hi.x : hi.y) >> (j % 2 * 8);
-          const uint32_t f[4] = {code_values<false>(wl, sl, ml), code_values<false>(wh, sh, mh),
-                                 code_values<true>(wl, sl, ml), code_values<true>(wh, sh, mh)};
+          const uint32_t f[4] = {code_values<false>(wl, sl, ml, k1024), code_values<false>(wh, sh, mh, k1024),
+                                 code_values<true>(wl, sl, ml, k1024), code_values<true>(wh, sh, mh, k1024)};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816(x[s][nt], f, q[gr][j][nt][0], q[gr][j][nt][1]);
+          for (int nt = 0; nt < NT; ++nt) {
+            if (gr == 0 && j == 0)
+              mma16816_first(x[s][nt], f, q[gr][j][nt][0], q[gr][j][nt][1]);
+            else
+              mma16816(x[s][nt], f, q[gr][j][nt][0], q[gr][j][nt][1]);
+          }
         }
       }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[s][nt][e] *= a.qk_scale;
     }
-    float alpha[NT][2];
-    const int left = p.t1 - (p.t0 + (i * kWarps + warp) * C::KT);
-    if (softmax_tile<D, NT, C::NS>(st, x, left, row, alpha)) rescale(st, alpha);
+    softmax_tile<D, NT, C::NS>(st, x, p.t1 - base, row, scale);
 #pragma unroll
     for (int s = 0; s < C::NS; ++s) {
       uint32_t pt[NT][2];  // P, rounded as in the fp16 path
@@ -515,8 +589,8 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeArgs 
         uint32_t w[4], par[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          w[r] = lds32(vt + C::at(16 * s + t + 4 * r, gr) + 4 * g);
-          par[r] = lds32(vp + ((16 * s + t + 4 * r) * GR + gr) * 4);
+          w[r] = lds32(tile + at_v[gr][r % 2] + (16 * s + r / 2 * 8) * ROW);
+          par[r] = lds32(tile + at_vp + ((16 * s + 4 * r) * GR + gr) * 4);
         }
         __half2 sv[2], mv[2];
 #pragma unroll
@@ -527,16 +601,18 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeArgs 
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) {
           const uint32_t first = __byte_perm(w[0], w[1], mt | (4 + mt) << 8), second = __byte_perm(w[2], w[3], mt | (4 + mt) << 8);
-          const uint32_t f[4] = {code_values<false>(first, sv[0], mv[0]), code_values<true>(first, sv[0], mv[0]),
-                                 code_values<false>(second, sv[1], mv[1]), code_values<true>(second, sv[1], mv[1])};
+          const uint32_t f[4] = {code_values<false>(first, sv[0], mv[0], k1024), code_values<true>(first, sv[0], mv[0], k1024),
+                                 code_values<false>(second, sv[1], mv[1], k1024), code_values<true>(second, sv[1], mv[1], k1024)};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma16816(st.o[4 * gr + mt][nt], f, pt[nt][0], pt[nt][1]);
         }
       }
     }
-    __syncwarp();  // every lane has read the stage that the next load overwrites
-    if (i + C::STAGES - 1 < tiles) load(i + C::STAGES - 1, (i + C::STAGES - 1) % C::STAGES);
+    __syncwarp();  // every lane has read the slot that the next load overwrites
+    if (base + (C::STAGES - 1) * STEP < p.t1) load(base + (C::STAGES - 1) * STEP, ring + next * C::TILE);
     cp_async_commit();
+    slot = slot + 1 == C::STAGES ? 0 : slot + 1;
+    next = next + 1 == C::STAGES ? 0 : next + 1;
   }
   cp_async_wait<0>();
   __syncthreads();  // the rings become the join's memory
