@@ -15,26 +15,28 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from tattn import _lib
-from tattn.api import _dtype_code, _require_cuda, _stream, _strides, _tma_ready
+from tattn.api import _dtype_code, _require_cuda, _tma_ready
+from tattn.norm_rope import _dense16, _like, _rows16
 
 INT_MAX = 2**31 - 1
 
 
 def _check_heads(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
     """Shapes, devices and dtypes of a call whose keys and values may have fewer heads than its queries."""
-    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+    sq, sk = q.shape, k.shape
+    if len(sq) != 4 or len(sk) != 4 or v.shape != sk:
         raise ValueError(
             "expected q [batch, heads, seq, dim] and k, v of equal shape [batch, kv_heads, kv_seq, dim]; "
-            f"got {q.shape}, {k.shape}, {v.shape}"
+            f"got {sq}, {sk}, {v.shape}"
         )
-    if k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
-        raise ValueError(f"q and k must agree in batch and head dim; got {q.shape}, {k.shape}")
-    if k.shape[1] == 0 or q.shape[1] % k.shape[1] != 0:
-        raise ValueError(f"query heads must be a multiple of key/value heads; got {q.shape[1]} and {k.shape[1]}")
-    if not (q.device == k.device == v.device):
+    if sk[0] != sq[0] or sk[3] != sq[3]:
+        raise ValueError(f"q and k must agree in batch and head dim; got {sq}, {sk}")
+    if sk[1] == 0 or sq[1] % sk[1] != 0:
+        raise ValueError(f"query heads must be a multiple of key/value heads; got {sq[1]} and {sk[1]}")
+    if not (q.get_device() == k.get_device() == v.get_device()):
         raise ValueError(f"q, k, v must be on one device, got {q.device}, {k.device}, {v.device}")
-    if q.shape[3] not in (16, 32, 64, 128):
-        raise ValueError(f"head dim must be 16, 32, 64 or 128, got {q.shape[3]}")
+    if sq[3] not in (16, 32, 64, 128):
+        raise ValueError(f"head dim must be 16, 32, 64 or 128, got {sq[3]}")
     if not (q.dtype == k.dtype == v.dtype) or q.dtype not in (torch.float16, torch.float32):
         raise ValueError(f"q, k, v must share dtype float16 or float32, got {q.dtype}, {k.dtype}, {v.dtype}")
 
@@ -46,32 +48,27 @@ def _check_window(window: int | None, sinks: int) -> None:
         raise ValueError(f"sinks must not be negative, got {sinks}")
 
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """``t`` dense and 16-byte aligned (the rows the delta pass reads)."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
 def _forward(
     q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int, scale: float
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Returns (O, M): O like q, M fp32 [Z, H, Nq] (base-2 log-sum-exp)."""
     _require_cuda(q)
-    lib = _lib.load()
-    z, h, n, d = q.shape
     if q.dtype == torch.float16:
         q, k, v = (_tma_ready(t) for t in (q, k, v))
-    o = torch.empty_like(q)
-    if q.dtype == torch.float16 and not lib.tattn_layout_ok(o.data_ptr(), _lib.strides_array(_strides(o)), z, h, n, d):
+    (z, h, n, d), (_, hk, nk, _) = q.shape, k.shape
+    o = _like(q)
+    if _rows16(o) is not o:
         o = torch.empty((z, h, n, d), device=q.device, dtype=q.dtype)
     m = torch.empty((z, h, n), device=q.device, dtype=torch.float32)
-    with torch.cuda.device(q.device):
-        rc = lib.tattn_window_fwd(
+    at = q.get_device()
+    with _lib.on_device(at):
+        rc = _lib.load().tattn_window_fwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), m.data_ptr(),
-            _lib.strides_array(_strides(q), _strides(k), _strides(v), _strides(o)),
-            z, h, k.shape[1], n, k.shape[2], d, _dtype_code(q), window, sinks, scale, _stream(q),
+            _lib.strides_bytes(q.stride() + k.stride() + v.stride() + o.stride()),
+            z, h, hk, n, nk, d, _dtype_code(q), window, sinks, scale, _lib.raw_stream(at),
         )  # fmt: skip
-    _lib.check("tattn_window_fwd", rc)
+    if rc:
+        _lib.check("tattn_window_fwd", rc)
     return o, m
 
 
@@ -82,25 +79,27 @@ def _backward(
     """Returns contiguous (dq, dk, dv)."""
     _require_cuda(q)
     lib = _lib.load()
-    (z, h, n, d), (hk, nk), code = q.shape, k.shape[1:3], _dtype_code(q)
+    (z, h, n, d), (_, hk, nk, _), code = q.shape, k.shape, _dtype_code(q)
     do = do.to(q.dtype)
     if q.dtype == torch.float16:
         q, k, v, do, o = (_tma_ready(t) for t in (q, k, v, do, o))
     else:
-        do, o = _rows16(do), _rows16(o)
+        do, o = _dense16(do), _dense16(o)
     delta = torch.empty((z, h, n), device=q.device, dtype=torch.float32)
     dq = torch.empty((z, h, n, d), device=q.device, dtype=q.dtype)
-    dk, dv = (torch.empty((z, hk, nk, d), device=q.device, dtype=q.dtype) for _ in range(2))
+    dk, dv = q.new_empty((z, hk, nk, d)), q.new_empty((z, hk, nk, d))
     size = lib.tattn_window_bwd_workspace_bytes(z, h, hk, n, nk, d, code, window, sinks)
     ws = torch.empty(max(size, 0), device=q.device, dtype=torch.uint8)
-    with torch.cuda.device(q.device):
+    at = q.get_device()
+    with _lib.on_device(at):
         rc = lib.tattn_window_bwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(),
             dv.data_ptr(), m.data_ptr(), delta.data_ptr(), ws.data_ptr(),
-            _lib.strides_array(_strides(q), _strides(k), _strides(v), _strides(o), _strides(do)),
-            z, h, hk, n, nk, d, code, window, sinks, scale, _stream(q),
+            _lib.strides_bytes(q.stride() + k.stride() + v.stride() + o.stride() + do.stride()),
+            z, h, hk, n, nk, d, code, window, sinks, scale, _lib.raw_stream(at),
         )  # fmt: skip
-    _lib.check("tattn_window_bwd", rc)
+    if rc:
+        _lib.check("tattn_window_bwd", rc)
     return dq, dk, dv
 
 
@@ -134,5 +133,8 @@ def window_attention(
     if k.shape[2] < q.shape[2]:
         raise ValueError(f"the queries are the last of the keys' sequence; got {q.shape[2]} queries, {k.shape[2]} keys")
     scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(q.shape[3])
-    out: torch.Tensor = _WindowAttention.apply(q, k, v, min(int(window), INT_MAX), min(int(sinks), INT_MAX), scale)
-    return out
+    w, s = min(int(window), INT_MAX), min(int(sinks), INT_MAX)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out: torch.Tensor = _WindowAttention.apply(q, k, v, w, s, scale)
+        return out
+    return _forward(q, k, v, w, s, scale)[0]
