@@ -161,18 +161,30 @@ __device__ __forceinline__ Blocks window_blocks(int row0, int N, const WindowArg
   return b;
 }
 
-// Columns of a key block that a row sees: c < lim and, kMaskWindow, c >= first or c < sink as well.
+// Columns of a key block that a row sees: c < lim; kMaskWindow: those whose bit is set. (One test of a
+// constant bit for a column; written as comparisons, c < lim && (c >= first || c < sink), it compiled to
+// branches, and a block that needed the mask took some 10 us.)
+template <int BN>
 struct Columns {
-  int lim, first, sink;
+  int lim;
+  uint32_t bits[BN / 32];
   template <int MASK>
   __device__ __forceinline__ bool see(int c) const {
-    return MASK == kMaskWindow ? c < lim && (c >= first || c < sink) : c < lim;
+    return MASK == kMaskWindow ? (bits[c / 32] & (1u << (c % 32))) != 0u : c < lim;
   }
+  // The columns in [first, lim) and in [0, min(sink, lim)).
+  __device__ __forceinline__ void set(int lim_, int first, int sink) {
+#pragma unroll
+    for (int w = 0; w < BN / 32; ++w)
+      bits[w] = below(lim_ - 32 * w) & (~below(first - 32 * w) | below(sink - 32 * w));
+  }
+  // The lowest n bits (none for n <= 0, all for n >= 32).
+  static __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : (1u << max(n, 0)) - 1u; }
 };
 
 // Max of one row of raw scores; MASKED ignores the columns that the row does not see.
 template <int BN, bool MASKED, int MASK>
-__device__ __forceinline__ float row_max(const uint32_t* s, const Columns& cols) {
+__device__ __forceinline__ float row_max(const uint32_t* s, const Columns<BN>& cols) {
   float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int c = 0; c < BN; c += 2) {
@@ -189,9 +201,9 @@ __device__ __forceinline__ float row_max(const uint32_t* s, const Columns& cols)
 // One row of P = exp2(S * scale - m) for columns [C0, C1) as fp16 pairs (p[c/2] = columns c, c+1) and
 // its fp32 sum. kEmuPairs of every 8 column pairs use the FMA-pipe exp2, the rest MUFU. MASKED zeroes
 // the columns that the row does not see.
-template <int C0, int C1, bool MASKED, int MASK>
+template <int BN, int C0, int C1, bool MASKED, int MASK>
 __device__ __forceinline__ float exp_cols(const uint32_t* s, uint32_t* p, uint64_t scale2, uint64_t negm2,
-                                          const Columns& cols) {
+                                          const Columns<BN>& cols) {
   uint64_t acc0 = 0, acc1 = 0;
 #pragma unroll
   for (int c = C0; c < C1; c += 2) {
@@ -446,11 +458,11 @@ __global__ void __launch_bounds__(384, 1)
       // kMaskWindow: in every block that the diagonal or the lower edge of some row's window cuts.
       const int col0 = (WINDOW ? list.block(list.entry(i, j)) : j) * BN;
       bool last;
-      Columns cols{};
+      Columns<BN> cols{};
       if (WINDOW) {
         const int pos = row + args.win.off, tile = pos - t;  // positions of this row and of the tile's first
         last = col0 + BN - 1 > tile || (col0 <= tile + C::BM - 1 - args.win.window && col0 + BN > args.win.sinks);
-        cols = Columns{min(args.win.Nk, pos + 1) - col0, pos + 1 - args.win.window - col0, args.win.sinks - col0};
+        if (last) cols.set(min(args.win.Nk, pos + 1) - col0, pos + 1 - args.win.window - col0, args.win.sinks - col0);
       } else {
         last = (col0 + BN > N) || (CAUSAL && col0 + BN - 1 > row - t);
         cols.lim = N - col0;
@@ -485,12 +497,12 @@ __global__ void __launch_bounds__(384, 1)
       uint32_t p[BN / 2];
       const float m_use = WINDOW && m_run == -INFINITY ? 0.f : m_run;  // nothing seen yet: every p is masked to 0
       const uint64_t negm2 = f2(-m_use, -m_use);
-      l_run += last ? exp_cols<0, kSplit, true, MASK>(s, p, scale2, negm2, cols)
-                    : exp_cols<0, kSplit, false, MASK>(s, p, scale2, negm2, cols);
+      l_run += last ? exp_cols<BN, 0, kSplit, true, MASK>(s, p, scale2, negm2, cols)
+                    : exp_cols<BN, 0, kSplit, false, MASK>(s, p, scale2, negm2, cols);
       mbar_arrive(&bar_exp_done[i]);
       if constexpr (kSplit < BN)
-        l_run += last ? exp_cols<kSplit, BN, true, MASK>(s, p, scale2, negm2, cols)
-                      : exp_cols<kSplit, BN, false, MASK>(s, p, scale2, negm2, cols);
+        l_run += last ? exp_cols<BN, kSplit, BN, true, MASK>(s, p, scale2, negm2, cols)
+                      : exp_cols<BN, kSplit, BN, false, MASK>(s, p, scale2, negm2, cols);
 
       // PV(j-1) must have landed before P and O of this tile are touched again (ALIAS_P: it has, since
       // S(j) was issued after it and has completed).
