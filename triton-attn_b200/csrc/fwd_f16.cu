@@ -19,7 +19,11 @@
 // its tile's issuer starts the next QK^T. P then feeds the PV MMA as the A operand straight from
 // TMEM. The two warpgroups ping-pong on the exponent pass (the MUFU-bound part) through a token pair
 // of mbarriers; a warpgroup hands the turn over before its last quarter of columns.
-// A sliding window with sinks (kMaskWindow) is the same kernel on a shorter list of key blocks (Blocks).
+// A sliding window with sinks (kMaskWindow) is the same kernel on a shorter list of key blocks (Blocks). A CTA
+// then lives for a few blocks only, and its start (TMEM, barriers, the first loads), epilogue and
+// replacement, some 5 us of an SM, are a good part of it. So where two CTAs fit an SM (D <= 64) a CTA has
+// one query tile (TILES = 1: 256 threads, 256 TMEM columns, a ring of 2), and while one of the two starts or
+// ends the other computes; their exponent passes take no turns.
 // The running max is rescaled lazily: O (in TMEM) and l are only corrected when a row's max grows by
 // more than kRescaleThreshold (log2 units); P values stay below 2^kRescaleThreshold, exact in fp16.
 #include "common.cuh"
@@ -35,13 +39,17 @@ constexpr float kRescaleThreshold = 8.0f;
 constexpr int kEmuPairs = 2;
 // Register split (setmaxnreg): launch = 384 threads x 168 registers = 64512; softmax warpgroups take
 // 216 and warpgroup 2 keeps 56: 8*32*216 + 4*32*56 = 62464 <= 64512.
-constexpr int kSoftmaxRegs = 216;
-constexpr int kProducerRegs = 56;
+// One tile: launch = 256 x 128 (two CTAs an SM), softmax 208 and producer 48: 128 * 208 + 128 * 48 = 32768.
+template <int TILES>
+constexpr int kSoftmaxRegs = TILES == 2 ? 216 : 208;
+template <int TILES>
+constexpr int kProducerRegs = TILES == 2 ? 56 : 48;
 
-// Geometry of one tile variant (tiles.h, kFwdTiles): head dim D, BN_ keys per block, NS_ ring stages.
-template <int D, int BN_, int NS_>
+// Geometry of one tile variant (tiles.h, kFwdTiles): head dim D, BN_ keys per block, NS_ ring stages; TILES
+// query tiles per CTA.
+template <int D, int BN_, int NS_, int TILES>
 struct FwdCfg {
-  static constexpr int BM = 128;                        // rows per query tile (2 tiles per CTA)
+  static constexpr int BM = 128;                        // rows per query tile
   static constexpr int BN = BN_;                        // keys per block
   static constexpr int NS = NS_;                        // K/V ring depth
   static constexpr int CW = D < 64 ? D : 64;            // columns per swizzle chunk
@@ -53,27 +61,30 @@ struct FwdCfg {
   static constexpr int KCHUNK = BN * SWB;               // one BN-row chunk
   static constexpr int KTILE = KCHUNK * NCH;            // one [BN, D] fp16 key / value block
   static constexpr int OFF_Q = 0;
-  static constexpr int OFF_K = 2 * QTILE;
+  static constexpr int OFF_K = TILES * QTILE;
   static constexpr int OFF_V = OFF_K + NS * KTILE;
   static constexpr int OFF_BAR = OFF_V + NS * KTILE;
-  // q_full, k_full[NS], v_full[NS], kv_empty[2][NS], s_full[2], o_done[2], exp_done[2], fin[2],
-  // s_free[2], p_full[2]
-  static constexpr int NBARS = 1 + 4 * NS + 12;
+  // q_full, k_full[NS], v_full[NS], kv_empty[TILES][NS]; of each tile: s_full, o_done, exp_done, fin, s_free,
+  // p_full
+  static constexpr int NBARS = 1 + 2 * NS + TILES * NS + 6 * TILES;
   static constexpr int OFF_MISC = OFF_BAR + NBARS * 8;  // tmem base (u32), abort flag (int), head index (int)
   static constexpr int SMEM_USED = OFF_MISC + 16;
-  // Request at least ~116 KB so exactly one CTA (which owns all 512 TMEM columns) fits per SM.
-  static constexpr int SMEM_BYTES = (SMEM_USED > 118784 ? SMEM_USED : 118784) + 1024;
+  // Request at least ~116 KB (78 KB) so exactly TILES == 2 ? one CTA : two CTAs, which own all 512 TMEM
+  // columns, fit per SM.
+  static constexpr int SMEM_LEAST = TILES == 2 ? 118784 : 79872;
+  static constexpr int SMEM_BYTES = (SMEM_USED > SMEM_LEAST ? SMEM_USED : SMEM_LEAST) + 1024;
+  static constexpr int TMEM_COLS = 256 * TILES;
   // TMEM: S_i [BN], P_i [BN / 2, fp16 pairs], O_i [D] per tile. Where S, P and O of both tiles do not
   // fit 512 columns (D = 128 with 128-key blocks), P_i is written over the first half of S_i (ALIAS_P):
   // the MMAs of a CTA run in issue order, so S_i(j + 1), issued after PV_i(j), overwrites P_i(j) only
   // once PV_i(j) has read it.
-  static constexpr bool ALIAS_P = 3 * BN + 2 * D > 512;
-  static constexpr uint32_t TM_S = 0;                             // + i * BN
-  static constexpr uint32_t TM_P = ALIAS_P ? TM_S : 2 * BN;       // + i * BN (ALIAS_P) or i * BN / 2
-  static constexpr uint32_t TM_O = ALIAS_P ? 2 * BN : 3 * BN;     // + i * D
-  static constexpr uint32_t P_STRIDE = ALIAS_P ? BN : BN / 2;     // columns between P_0 and P_1
-  static_assert((ALIAS_P ? 2 * BN : 3 * BN) + 2 * D <= 512, "TMEM budget");
-  static_assert(OFF_MISC + 16 + 1024 <= 232448, "shared memory budget");
+  static constexpr bool ALIAS_P = TILES * (BN + BN / 2 + D) > TMEM_COLS;
+  static constexpr uint32_t TM_S = 0;                                              // + i * BN
+  static constexpr uint32_t TM_P = ALIAS_P ? TM_S : TILES * BN;                    // + i * BN (ALIAS_P) or i * BN / 2
+  static constexpr uint32_t TM_O = ALIAS_P ? TILES * BN : TILES * (BN + BN / 2);   // + i * D
+  static constexpr uint32_t P_STRIDE = ALIAS_P ? BN : BN / 2;                      // columns between P_0 and P_1
+  static_assert(TM_O + TILES * D <= TMEM_COLS, "TMEM budget");
+  static_assert((OFF_MISC + 16 + 2048) * (3 - TILES) <= 233472, "shared memory budget");
   static constexpr uint32_t IDESC_S = idesc_f16_f32(128, BN, false);
   static constexpr uint32_t IDESC_PV = idesc_f16_f32(128, D, true);
 };
@@ -126,38 +137,24 @@ __device__ __forceinline__ void issue_pv_stage(int st, uint32_t d_tmem, uint32_t
   issue_pv_st<C, D, ST>(d_tmem, p_tmem, dV, accumulate);
 }
 
-// The key blocks that a CTA's two query tiles go through. Both walk one list, j = 0 .. n1 - 1, through the
-// ring; tile 0 takes its first n0 entries. kMaskWindow: the list is the blocks that hold sinks, then those
-// from the first one in tile 0's window up to the diagonal; tile 1 leaves out the `skip` entries from
-// `from` on, which only tile 0's window reaches.
+// kMaskWindow: the key blocks that a CTA goes through, j = 0 .. n - 1: those that hold sinks, then those from
+// the first one in the window of its first row up to the last one before its last row. Tile 0 of two ends
+// with entry n0 - 1.
 struct Blocks {
-  int n0, n1;        // list entries up to the end of tile 0 / 1 (0: the tile has no rows)
-  int sink, jump;    // entry j >= sink is block j + jump
-  int from, skip;
-
+  int n0, n;
+  int sink, jump;  // entry j >= sink is block j + jump
   __device__ __forceinline__ int block(int j) const { return j < sink ? j : j + jump; }
-  // List entry of tile i's u-th block.
-  __device__ __forceinline__ int entry(int i, int u) const { return i == 1 && u >= from ? u + skip : u; }
-  // Blocks that tile i takes.
-  __device__ __forceinline__ int count(int i) const { return i == 0 ? n0 : n1 > 0 ? n1 - skip : 0; }
 };
-
-// With a ring of 2 (D = 128) tile 1 leaves nothing out: it would run one entry ahead of tile 0, and the
-// entry after that could only be loaded once tile 0 is done with its own.
-template <int BM, int BN, int NS>
+template <int BM, int BN, int TILES>
 __device__ __forceinline__ Blocks window_blocks(int row0, int N, const WindowArgs& w) {
-  const int p0 = row0 + w.off, p1 = p0 + BM;  // positions of the tiles' first rows
-  const int end0 = min(p1 - 1, w.Nk - 1) / BN + 1, end1 = min(p1 + BM - 1, w.Nk - 1) / BN + 1;
-  const int first0 = max(0, p0 - w.window + 1) / BN, first1 = max(0, p1 - w.window + 1) / BN;
-  const int ns = (w.sinks + BN - 1) / BN;
+  const int p0 = row0 + w.off;  // position of the first row
+  const int end0 = min(p0 + BM - 1, w.Nk - 1) / BN + 1, end = min(p0 + TILES * BM - 1, w.Nk - 1) / BN + 1;
+  const int first = max(0, p0 - w.window + 1) / BN;
   Blocks b;
-  b.sink = min(ns, first0);
-  b.jump = first0 - b.sink;
+  b.sink = min((w.sinks + BN - 1) / BN, first);
+  b.jump = first - b.sink;
   b.n0 = end0 - b.jump;
-  b.n1 = row0 + BM < N ? end1 - b.jump : 0;
-  const int keep = max(first0, ns);  // tile 1 needs no block of [keep, first1)
-  b.from = keep - b.jump;
-  b.skip = NS > 2 && b.n1 > 0 ? max(0, first1 - keep) : 0;
+  b.n = end - b.jump;
   return b;
 }
 
@@ -229,12 +226,13 @@ __device__ __forceinline__ float exp_cols(const uint32_t* s, uint32_t* p, uint64
   return t.x + t.y;
 }
 
-template <int D, int MASK, int BN_, int NS_>
-__global__ void __launch_bounds__(384, 1)
+template <int D, int MASK, int BN_, int NS_, int TILES>
+__global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
     fwd_f16_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const FwdArgs args) {
-  using C = FwdCfg<D, BN_, NS_>;
+  using C = FwdCfg<D, BN_, NS_, TILES>;
   constexpr int BN = C::BN;
+  constexpr int kTmaWarp = 4 * TILES, kMmaWarp = kTmaWarp + 1, kAllocWarp = kTmaWarp + 3;  // kMmaWarp + i: tile i
   constexpr bool CAUSAL = MASK == kMaskCausal, WINDOW = MASK == kMaskWindow;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
@@ -245,20 +243,20 @@ __global__ void __launch_bounds__(384, 1)
   uint64_t* bar_q = bars;
   uint64_t* bar_k_full = bars + 1;                   // [NS]
   uint64_t* bar_v_full = bars + 1 + C::NS;           // [NS]
-  uint64_t* bar_kv_empty = bars + 1 + 2 * C::NS;     // [2][NS]: tile i is done with the block in stage s
-  uint64_t* bar_s_full = bars + 1 + 4 * C::NS;       // [2]
-  uint64_t* bar_o_done = bar_s_full + 2;             // [2]
-  uint64_t* bar_exp_done = bar_s_full + 4;           // [2]: warpgroup i finished the exponent pass
-  uint64_t* bar_fin = bar_s_full + 6;                // [2]
-  uint64_t* bar_s_free = bar_s_full + 8;             // [2]: the tile's softmax holds S(j) in registers
-  uint64_t* bar_p_full = bar_s_full + 10;            // [2]: the tile's softmax has stored P(j)
+  uint64_t* bar_kv_empty = bars + 1 + 2 * C::NS;     // [TILES][NS]: tile i is done with the block in stage s
+  uint64_t* bar_s_full = bars + 1 + (2 + TILES) * C::NS;  // [TILES], as all that follow
+  uint64_t* bar_o_done = bar_s_full + TILES;
+  uint64_t* bar_exp_done = bar_s_full + 2 * TILES;   // warpgroup i finished the exponent pass
+  uint64_t* bar_fin = bar_s_full + 3 * TILES;
+  uint64_t* bar_s_free = bar_s_full + 4 * TILES;     // the tile's softmax holds S(j) in registers
+  uint64_t* bar_p_full = bar_s_full + 5 * TILES;     // the tile's softmax has stored P(j)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
   const CtaAbort ab{abort_flag, args.status, args.wait_limit_ns};
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int N = args.N;
-  const int nct = (N + 2 * C::BM - 1) / (2 * C::BM);  // CTAs per (z, h)
+  const int nct = (N + TILES * C::BM - 1) / (TILES * C::BM);  // CTAs per (z, h)
   int bh, cta;
   if (CAUSAL) {  // longest first within groups of heads whose K/V fit in L2 (the highest row blocks see the most keys)
     cta = nct - 1 - causal_cta_rank(nct, args.Z * args.H, N, D, &bh);
@@ -271,22 +269,23 @@ __global__ void __launch_bounds__(384, 1)
   const int NB = (N + BN - 1) / BN;
   // Query tile i of this CTA: rows [row0_i, row0_i + 128), n_i key blocks: [0, n_i) or, kMaskWindow,
   // those of the list.
-  const int row0_0 = 2 * cta * C::BM, row0_1 = row0_0 + C::BM;
+  const int row0_0 = TILES * cta * C::BM, row0_1 = row0_0 + C::BM;
   Blocks list{};
-  if (WINDOW) list = window_blocks<C::BM, BN, C::NS>(row0_0, N, args.win);
-  const int n_0 = WINDOW ? list.count(0) : row0_0 >= N ? 0 : (CAUSAL ? min((row0_0 + C::BM + BN - 1) / BN, NB) : NB);
-  const int n_1 = WINDOW ? list.count(1) : row0_1 >= N ? 0 : (CAUSAL ? min((row0_1 + C::BM + BN - 1) / BN, NB) : NB);
-  const int nmax = WINDOW ? max(list.n0, list.n1) : max(n_0, n_1);
+  if (WINDOW) list = window_blocks<C::BM, BN, TILES>(row0_0, N, args.win);
+  const int n_0 = WINDOW ? list.n0 : row0_0 >= N ? 0 : (CAUSAL ? min((row0_0 + C::BM + BN - 1) / BN, NB) : NB);
+  const int n_1 = TILES == 1 || row0_1 >= N ? 0
+                  : WINDOW                  ? list.n
+                                            : (CAUSAL ? min((row0_1 + C::BM + BN - 1) / BN, NB) : NB);
+  const int nmax = max(n_0, n_1);
 
   if (threadIdx.x == 0) {
     mbar_init(bar_q, 1);
     for (int s = 0; s < C::NS; ++s) {
       mbar_init(&bar_k_full[s], 1);
       mbar_init(&bar_v_full[s], 1);
-      mbar_init(&bar_kv_empty[s], 1);
-      mbar_init(&bar_kv_empty[C::NS + s], 1);
+      for (int i = 0; i < TILES; ++i) mbar_init(&bar_kv_empty[i * C::NS + s], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < TILES; ++i) {
       mbar_init(&bar_s_full[i], 1);
       mbar_init(&bar_o_done[i], 1);
       mbar_init(&bar_exp_done[i], 128);
@@ -298,11 +297,11 @@ __global__ void __launch_bounds__(384, 1)
     *reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8) = bh;  // for the softmax epilogue
     fence_mbar_init();
   }
-  if (warp == 11) {
-    tmem_alloc(tmem_slot, 512);
+  if (warp == kAllocWarp) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
     tmem_relinquish();
   }
-  if (warp == 8 && lane == 0) {
+  if (warp == kTmaWarp && lane == 0) {
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
@@ -314,13 +313,13 @@ __global__ void __launch_bounds__(384, 1)
 
   const uint32_t sQ = base_u32 + C::OFF_Q, sK = base_u32 + C::OFF_K, sV = base_u32 + C::OFF_V;
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
-    if (warp == 8 && lane == 0) {
+  if (warp >= kTmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs<TILES>));
+    if (warp == kTmaWarp && lane == 0) {
       // -------------------------------------------------------------- TMA producer
       const uint32_t qbytes = (n_0 > 0 ? C::QTILE : 0) + (n_1 > 0 ? C::QTILE : 0);
       mbar_arrive_expect_tx(bar_q, qbytes);
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < TILES; ++i) {
         if ((i ? n_1 : n_0) == 0) continue;
         for (int ch = 0; ch < C::NCH; ++ch)
           tma_load_4d(sQ + i * C::QTILE + ch * C::QCHUNK, &tm_q, ch * C::CW, i ? row0_1 : row0_0, hi, zi, bar_q);
@@ -331,8 +330,8 @@ __global__ void __launch_bounds__(384, 1)
         const int st = j % C::NS;
         if (j >= C::NS) {  // both tiles that used the stage's previous block must be done with it
           const int old = j - C::NS;
-          for (int i = 0; i < 2 && ok; ++i)
-            if (old < (WINDOW ? (i ? list.n1 : list.n0) : (i ? n_1 : n_0)) && !mbar_wait(&bar_kv_empty[i * C::NS + st], ((j / C::NS) - 1) & 1, ab))
+          for (int i = 0; i < TILES && ok; ++i)
+            if (old < (i ? n_1 : n_0) && !mbar_wait(&bar_kv_empty[i * C::NS + st], ((j / C::NS) - 1) & 1, ab))
               ok = false;
           if (!ok) break;
         }
@@ -351,51 +350,39 @@ __global__ void __launch_bounds__(384, 1)
         mbar_drain(&bar_k_full[jj % C::NS], (jj / C::NS) & 1, lim);
         mbar_drain(&bar_v_full[jj % C::NS], (jj / C::NS) & 1, lim);
       }
-    } else if (warp == 9 || warp == 10) {
+    } else if (warp >= kMmaWarp && warp < kMmaWarp + TILES) {
       // -------------------------------------------------------------- MMA issuer of tile i
       // Order within a tile = the order its softmax releases inputs: S(j+1) once the softmax holds
       // S(j) in registers (s_free), then PV(j) once it has stored P(j) (p_full). The whole warp runs
       // the loop; elect.sync inside each MMA picks the issuing lane, and every descriptor is a
       // loop-invariant base plus a compile-time constant, so the MMAs go out at tensor-core rate.
-      const int i = warp - 9;
+      const int i = warp - kMmaWarp;
       const int n = i ? n_1 : n_0;
       const uint32_t idesc_s = C::IDESC_S | (args.negate_s ? (1u << 13) : 0u);
       const uint64_t dQ = smem_desc(sQ, 16, 8 * C::SWB, C::LAYOUT);
       const uint64_t dK = smem_desc(sK, 16, 8 * C::SWB, C::LAYOUT);
       const uint64_t dV = smem_desc(sV, C::KCHUNK, 8 * C::SWB, C::LAYOUT);
       const uint32_t tS = tmem + C::TM_S + i * BN, tP = tmem + C::TM_P + i * C::P_STRIDE, tO = tmem + C::TM_O + i * D;
-      // kMaskWindow: releases the list entries [a, b) that this tile leaves out, each once it has landed
-      // (a phase of kv_empty may only complete after the producer has waited for the one before).
-      auto leave_out = [&](int a, int b) -> bool {
-        for (; a < b; ++a) {
-          if (!warp_wait(&bar_k_full[a % C::NS], (a / C::NS) & 1, ab)) return false;
-          mma_commit_elect(&bar_kv_empty[i * C::NS + a % C::NS]);
-        }
-        return true;
-      };
-      int e = WINDOW ? list.entry(i, 0) : 0;  // list entry of block j
-      bool ok = n > 0 && warp_wait(bar_q, 0, ab) && (!WINDOW || leave_out(0, e)) &&
-                warp_wait(&bar_k_full[e % C::NS], (e / C::NS) & 1, ab);
+      bool ok = n > 0 && warp_wait(bar_q, 0, ab) && warp_wait(&bar_k_full[0], 0, ab);
       if (ok) {
         tc_fence_after();
-        issue_qk_stage<C, D>(e % C::NS, i, tS, dQ, dK, idesc_s);
+        issue_qk_stage<C, D>(0, i, tS, dQ, dK, idesc_s);
         mma_commit_elect(&bar_s_full[i]);
       }
       for (int j = 0; ok && j < n; ++j) {
-        e = WINDOW ? list.entry(i, j) : j;
-        const int b = WINDOW ? list.entry(i, j + 1) : j + 1;  // list entry of the next block
         if (C::ALIAS_P) {
           // PV(j) reads P(j) where S(j) was, then S(j + 1) overwrites both (in issue order).
-          if (!warp_wait(&bar_p_full[i], j & 1, ab) || !warp_wait(&bar_v_full[e % C::NS], (e / C::NS) & 1, ab)) {
+          if (!warp_wait(&bar_p_full[i], j & 1, ab) || !warp_wait(&bar_v_full[j % C::NS], (j / C::NS) & 1, ab)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          issue_pv_stage<C, D>(e % C::NS, tO, tP, dV, j > 0 ? 1u : 0u);
+          issue_pv_stage<C, D>(j % C::NS, tO, tP, dV, j > 0 ? 1u : 0u);
           mma_commit_elect(&bar_o_done[i]);
-          mma_commit_elect(&bar_kv_empty[i * C::NS + e % C::NS]);
+          mma_commit_elect(&bar_kv_empty[i * C::NS + j % C::NS]);
           if (j + 1 < n) {
-            if ((WINDOW && !leave_out(e + 1, b)) || !warp_wait(&bar_k_full[b % C::NS], (b / C::NS) & 1, ab)) {
+            const int b = j + 1;
+            if (!warp_wait(&bar_k_full[b % C::NS], (b / C::NS) & 1, ab)) {
               ok = false;
               break;
             }
@@ -406,8 +393,8 @@ __global__ void __launch_bounds__(384, 1)
           continue;
         }
         if (j + 1 < n) {
-          if (!warp_wait(&bar_s_free[i], j & 1, ab) || (WINDOW && !leave_out(e + 1, b)) ||
-              !warp_wait(&bar_k_full[b % C::NS], (b / C::NS) & 1, ab)) {
+          const int b = j + 1;
+          if (!warp_wait(&bar_s_free[i], j & 1, ab) || !warp_wait(&bar_k_full[b % C::NS], (b / C::NS) & 1, ab)) {
             ok = false;
             break;
           }
@@ -415,14 +402,14 @@ __global__ void __launch_bounds__(384, 1)
           issue_qk_stage<C, D>(b % C::NS, i, tS, dQ, dK, idesc_s);
           mma_commit_elect(&bar_s_full[i]);
         }
-        if (!warp_wait(&bar_p_full[i], j & 1, ab) || !warp_wait(&bar_v_full[e % C::NS], (e / C::NS) & 1, ab)) {
+        if (!warp_wait(&bar_p_full[i], j & 1, ab) || !warp_wait(&bar_v_full[j % C::NS], (j / C::NS) & 1, ab)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        issue_pv_stage<C, D>(e % C::NS, tO, tP, dV, j > 0 ? 1u : 0u);
+        issue_pv_stage<C, D>(j % C::NS, tO, tP, dV, j > 0 ? 1u : 0u);
         mma_commit_elect(&bar_o_done[i]);
-        mma_commit_elect(&bar_kv_empty[i * C::NS + e % C::NS]);
+        mma_commit_elect(&bar_kv_empty[i * C::NS + j % C::NS]);
       }
       // Every MMA of this tile must retire before TMEM is released.
       mma_commit_elect(&bar_fin[i]);
@@ -430,7 +417,7 @@ __global__ void __launch_bounds__(384, 1)
     }
   } else {
     // ------------------------------------------------------------------ softmax warpgroups
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs<TILES>));
     const int i = warp / 4;
     const int t = threadIdx.x % 128;
     const int row = (i ? row0_1 : row0_0) + t;
@@ -456,7 +443,7 @@ __global__ void __launch_bounds__(384, 1)
       // Columns past N (ragged tail) only occur in the last block; columns above the diagonal
       // (causal) in every block that reaches past the tile's first row (the last BM / BN blocks).
       // kMaskWindow: in every block that the diagonal or the lower edge of some row's window cuts.
-      const int col0 = (WINDOW ? list.block(list.entry(i, j)) : j) * BN;
+      const int col0 = (WINDOW ? list.block(j) : j) * BN;
       bool last;
       Columns<BN> cols{};
       if (WINDOW) {
@@ -485,7 +472,8 @@ __global__ void __launch_bounds__(384, 1)
       // exponentiates while the other loads S, reduces the max and stores P. Order: tile 0 block j,
       // tile 1 block j, tile 0 block j+1, ...; a turn is only awaited if the other tile has that block.
       const int other_n = i ? n_0 : n_1;
-      if (i == 1 ? (j < other_n) : (j >= 1 && j - 1 < other_n)) {
+      if (TILES == 1) {
+      } else if (i == 1 ? (j < other_n) : (j >= 1 && j - 1 < other_n)) {
         if (!warp_wait(&bar_exp_done[1 - i], (i == 1 ? j : j - 1) & 1, ab)) { ok = false; break; }
       }
       // P = exp2(S * scale - m); the masked variant only runs for blocks that need it, so the column
@@ -493,13 +481,13 @@ __global__ void __launch_bounds__(384, 1)
       // With 128-key blocks the turn is handed over after seven eighths of the columns, so the other
       // tile's pass starts while this one finishes and the exponent unit does not idle across the
       // hand-off (measured at BN = 128: 7/8 best, 3/4 within 1%, 1/2 8% slower; slower at BN = 64).
-      constexpr int kSplit = BN == 128 ? BN * 7 / 8 : BN;
+      constexpr int kSplit = BN == 128 && TILES == 2 ? BN * 7 / 8 : BN;
       uint32_t p[BN / 2];
       const float m_use = WINDOW && m_run == -INFINITY ? 0.f : m_run;  // nothing seen yet: every p is masked to 0
       const uint64_t negm2 = f2(-m_use, -m_use);
       l_run += last ? exp_cols<BN, 0, kSplit, true, MASK>(s, p, scale2, negm2, cols)
                     : exp_cols<BN, 0, kSplit, false, MASK>(s, p, scale2, negm2, cols);
-      mbar_arrive(&bar_exp_done[i]);
+      if (TILES == 2) mbar_arrive(&bar_exp_done[i]);
       if constexpr (kSplit < BN)
         l_run += last ? exp_cols<BN, kSplit, BN, true, MASK>(s, p, scale2, negm2, cols)
                       : exp_cols<BN, kSplit, BN, false, MASK>(s, p, scale2, negm2, cols);
@@ -560,38 +548,40 @@ __global__ void __launch_bounds__(384, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 11) {
+  if (warp == kAllocWarp) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, C::TMEM_COLS);
   }
 }
 
-template <int D, int MASK, int BN, int NS>
+template <int D, int MASK, int BN, int NS, int TILES = 2>
 cudaError_t launch_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FwdArgs& a,
                         cudaStream_t s) {
-  using C = FwdCfg<D, BN, NS>;
-  auto kern = fwd_f16_kernel<D, MASK, BN, NS>;
+  using C = FwdCfg<D, BN, NS, TILES>;
+  auto kern = fwd_f16_kernel<D, MASK, BN, NS, TILES>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
   if (e != cudaSuccess) return e;
-  const int nct = (a.N + 2 * C::BM - 1) / (2 * C::BM);
+  const int nct = (a.N + TILES * C::BM - 1) / (TILES * C::BM);
   const long long grid = (long long)nct * a.Z * a.H;
   if (grid <= 0) return cudaSuccess;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  kern<<<dim3((unsigned)grid), dim3(384), C::SMEM_BYTES, s>>>(tq, tk, tv, a);
+  kern<<<dim3((unsigned)grid), dim3(128 * (TILES + 1)), C::SMEM_BYTES, s>>>(tq, tk, tv, a);
   return cudaGetLastError();
 }
 
 // Variant v (tiles.h, kFwdTiles) for head dim D; variants whose blocks do not fit D's TMEM budget are
-// not instantiated. kMaskWindow has the default variant only.
+// not instantiated. kMaskWindow has the default variant's blocks only.
 template <int D, int MASK>
 cudaError_t launch_variant(int v, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                            const FwdArgs& a, cudaStream_t s) {
   static_assert(kNumFwdTiles == 3, "variant dispatch");
   if constexpr (MASK == kMaskWindow) {
     constexpr TileVariant tile = kFwdTiles[tile_default(0, D, true)];
-    static_assert(tile.block_n == 128, "window_blocks: tile 1 starts at most one block after tile 0");
-    return v == tile_default(0, D, true) ? launch_impl<D, MASK, tile.block_n, tile.stages>(tq, tk, tv, a, s)
-                                         : cudaErrorNotSupported;
+    if (v != tile_default(0, D, true)) return cudaErrorNotSupported;
+    if constexpr (D <= 64)
+      return launch_impl<D, MASK, tile.block_n, 2, 1>(tq, tk, tv, a, s);
+    else
+      return launch_impl<D, MASK, tile.block_n, tile.stages>(tq, tk, tv, a, s);
   } else {
     switch (v) {
       case 0:
