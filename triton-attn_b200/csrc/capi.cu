@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 
@@ -439,7 +440,8 @@ extern "C" int tattn_window_fwd(const void* q, const void* k, const void* v, voi
       !layout_ok(o, so, Z, H, Nq, D))
     return TATTN_ERR_LAYOUT;
   a.so = normalize(so, Z, H, Nq, D);
-  a.qk_scale = (sm_scale < 0.f ? -sm_scale : sm_scale) * kLog2e;
+  // Positive, so that a hidden score stays -infinity; below 2^-60 scores vanish against 1 anyway.
+  a.qk_scale = std::max((sm_scale < 0.f ? -sm_scale : sm_scale) * kLog2e, 0x1p-60f);
   a.negate_s = sm_scale < 0.f ? 1 : 0;
   const int variant = tile_default(0, D, true), kv_rows = fwd_f16_kv_rows(D, variant);
   CUtensorMap tq, tk, tv;

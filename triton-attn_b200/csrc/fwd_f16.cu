@@ -158,37 +158,32 @@ __device__ __forceinline__ Blocks window_blocks(int row0, int N, const WindowArg
   return b;
 }
 
-// Columns of a key block that a row sees: c < lim; kMaskWindow: those whose bit is set. (One test of a
-// constant bit for a column; written as comparisons, c < lim && (c >= first || c < sink), it compiled to
-// branches, and a block that needed the mask took some 10 us.)
+// kMaskWindow: scores of the columns that a row does not see become -infinity: it sees the columns in
+// [first, lim) and in [0, min(sink, lim)). A bit a column, so that each is one test of a constant bit: written
+// as comparisons it compiled to branches, and a block that needed the mask took some 10 us. The pass comes
+// before the row's maximum and exponentials, which are then the same code as for other blocks (a second
+// copy of them for masked blocks had the short-lived CTAs wait for instructions).
 template <int BN>
-struct Columns {
-  int lim;
-  uint32_t bits[BN / 32];
-  template <int MASK>
-  __device__ __forceinline__ bool see(int c) const {
-    return MASK == kMaskWindow ? (bits[c / 32] & (1u << (c % 32))) != 0u : c < lim;
-  }
-  // The columns in [first, lim) and in [0, min(sink, lim)).
-  __device__ __forceinline__ void set(int lim_, int first, int sink) {
+__device__ __forceinline__ void hide_columns(uint32_t* s, int lim, int first, int sink) {
+  auto below = [](int n) { return n >= 32 ? ~0u : (1u << max(n, 0)) - 1u; };  // the lowest n bits
 #pragma unroll
-    for (int w = 0; w < BN / 32; ++w)
-      bits[w] = below(lim_ - 32 * w) & (~below(first - 32 * w) | below(sink - 32 * w));
+  for (int w = 0; w < BN / 32; ++w) {
+    const uint32_t bits = below(lim - 32 * w) & (~below(first - 32 * w) | below(sink - 32 * w));
+#pragma unroll
+    for (int c = 0; c < 32; ++c) s[32 * w + c] = (bits & (1u << c)) != 0u ? s[32 * w + c] : 0xff800000u;
   }
-  // The lowest n bits (none for n <= 0, all for n >= 32).
-  static __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : (1u << max(n, 0)) - 1u; }
-};
+}
 
-// Max of one row of raw scores; MASKED ignores the columns that the row does not see.
-template <int BN, bool MASKED, int MASK>
-__device__ __forceinline__ float row_max(const uint32_t* s, const Columns<BN>& cols) {
+// Max of one row of raw scores; MASK ignores columns >= lim.
+template <int BN, bool MASK>
+__device__ __forceinline__ float row_max(const uint32_t* s, int lim) {
   float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int c = 0; c < BN; c += 2) {
     float a = __uint_as_float(s[c]), b = __uint_as_float(s[c + 1]);
-    if (MASKED) {
-      a = cols.see<MASK>(c) ? a : -INFINITY;
-      b = cols.see<MASK>(c + 1) ? b : -INFINITY;
+    if (MASK) {
+      a = c < lim ? a : -INFINITY;
+      b = c + 1 < lim ? b : -INFINITY;
     }
     m[(c / 2) & 3] = fmax3(m[(c / 2) & 3], a, b);
   }
@@ -196,11 +191,10 @@ __device__ __forceinline__ float row_max(const uint32_t* s, const Columns<BN>& c
 }
 
 // One row of P = exp2(S * scale - m) for columns [C0, C1) as fp16 pairs (p[c/2] = columns c, c+1) and
-// its fp32 sum. kEmuPairs of every 8 column pairs use the FMA-pipe exp2, the rest MUFU. MASKED zeroes
-// the columns that the row does not see.
-template <int BN, int C0, int C1, bool MASKED, int MASK>
-__device__ __forceinline__ float exp_cols(const uint32_t* s, uint32_t* p, uint64_t scale2, uint64_t negm2,
-                                          const Columns<BN>& cols) {
+// its fp32 sum. kEmuPairs of every 8 column pairs use the FMA-pipe exp2, the rest MUFU. MASK zeroes
+// columns >= lim.
+template <int C0, int C1, bool MASK>
+__device__ __forceinline__ float exp_cols(const uint32_t* s, uint32_t* p, uint64_t scale2, uint64_t negm2, int lim) {
   uint64_t acc0 = 0, acc1 = 0;
 #pragma unroll
   for (int c = C0; c < C1; c += 2) {
@@ -212,9 +206,9 @@ __device__ __forceinline__ float exp_cols(const uint32_t* s, uint32_t* p, uint64
       const float2 xv = f2_unpack(x);
       e = make_float2(ex2_approx(xv.x), ex2_approx(xv.y));
     }
-    if (MASKED) {
-      e.x = cols.see<MASK>(c) ? e.x : 0.f;
-      e.y = cols.see<MASK>(c + 1) ? e.y : 0.f;
+    if (MASK) {
+      e.x = c < lim ? e.x : 0.f;
+      e.y = c + 1 < lim ? e.y : 0.f;
     }
     if ((c / 2) & 1)
       acc1 = fadd2(acc1, f2(e.x, e.y));
@@ -442,21 +436,19 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
 
       // Columns past N (ragged tail) only occur in the last block; columns above the diagonal
       // (causal) in every block that reaches past the tile's first row (the last BM / BN blocks).
-      // kMaskWindow: in every block that the diagonal or the lower edge of some row's window cuts.
+      // kMaskWindow: those are hidden beforehand, in every block that the diagonal or the lower edge of some
+      // row's window cuts.
       const int col0 = (WINDOW ? list.block(j) : j) * BN;
-      bool last;
-      Columns<BN> cols{};
       if (WINDOW) {
         const int pos = row + args.win.off, tile = pos - t;  // positions of this row and of the tile's first
-        last = col0 + BN - 1 > tile || (col0 <= tile + C::BM - 1 - args.win.window && col0 + BN > args.win.sinks);
-        if (last) cols.set(min(args.win.Nk, pos + 1) - col0, pos + 1 - args.win.window - col0, args.win.sinks - col0);
-      } else {
-        last = (col0 + BN > N) || (CAUSAL && col0 + BN - 1 > row - t);
-        cols.lim = N - col0;
-        if (CAUSAL) cols.lim = min(cols.lim, row - col0 + 1);
+        if (col0 + BN - 1 > tile || (col0 <= tile + C::BM - 1 - args.win.window && col0 + BN > args.win.sinks))
+          hide_columns<BN>(s, min(args.win.Nk, pos + 1) - col0, pos + 1 - args.win.window - col0,
+                           args.win.sinks - col0);
       }
-      float m_cand = last ? row_max<BN, true, MASK>(s, cols) : row_max<BN, false, MASK>(s, cols);
-      if (!WINDOW || m_cand != -INFINITY) m_cand *= scale;  // (-inf: the row sees none of this block; scale may be 0)
+      const bool last = !WINDOW && ((col0 + BN > N) || (CAUSAL && col0 + BN - 1 > row - t));
+      int lim = N - col0;
+      if (CAUSAL) lim = min(lim, row - col0 + 1);
+      const float m_cand = (last ? row_max<BN, true>(s, lim) : row_max<BN, false>(s, lim)) * scale;
       float alpha = 1.f;
       bool need = false;
       if (j == 0) {
@@ -483,14 +475,13 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
       // hand-off (measured at BN = 128: 7/8 best, 3/4 within 1%, 1/2 8% slower; slower at BN = 64).
       constexpr int kSplit = BN == 128 && TILES == 2 ? BN * 7 / 8 : BN;
       uint32_t p[BN / 2];
-      const float m_use = WINDOW && m_run == -INFINITY ? 0.f : m_run;  // nothing seen yet: every p is masked to 0
+      const float m_use = WINDOW && m_run == -INFINITY ? 0.f : m_run;  // nothing seen yet: every p is 0
       const uint64_t negm2 = f2(-m_use, -m_use);
-      l_run += last ? exp_cols<BN, 0, kSplit, true, MASK>(s, p, scale2, negm2, cols)
-                    : exp_cols<BN, 0, kSplit, false, MASK>(s, p, scale2, negm2, cols);
+      l_run += last ? exp_cols<0, kSplit, true>(s, p, scale2, negm2, lim) : exp_cols<0, kSplit, false>(s, p, scale2, negm2, lim);
       if (TILES == 2) mbar_arrive(&bar_exp_done[i]);
       if constexpr (kSplit < BN)
-        l_run += last ? exp_cols<BN, kSplit, BN, true, MASK>(s, p, scale2, negm2, cols)
-                      : exp_cols<BN, kSplit, BN, false, MASK>(s, p, scale2, negm2, cols);
+        l_run += last ? exp_cols<kSplit, BN, true>(s, p, scale2, negm2, lim)
+                      : exp_cols<kSplit, BN, false>(s, p, scale2, negm2, lim);
 
       // PV(j-1) must have landed before P and O of this tile are touched again (ALIAS_P: it has, since
       // S(j) was issued after it and has completed).
