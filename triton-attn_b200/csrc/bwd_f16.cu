@@ -1948,6 +1948,19 @@ __device__ __forceinline__ void fused_part_epilogue(const BwdArgs& a, int nthrea
   }
 }
 
+// kMaskWindow: S'^T of the queries that do not see a key, those outside columns [lo, hi), becomes -infinity,
+// whose P is 0 (a bit a column, and ahead of the code that all blocks share, as in the forward).
+template <int H>
+__device__ __forceinline__ void hide_queries(uint32_t* s, int lo, int hi) {
+  auto below = [](int n) { return n >= 32 ? ~0u : (1u << max(n, 0)) - 1u; };  // the lowest n bits
+#pragma unroll
+  for (int w = 0; w < H / 32; ++w) {
+    const uint32_t bits = below(hi - 32 * w) & ~below(lo - 32 * w);
+#pragma unroll
+    for (int c = 0; c < 32; ++c) s[32 * w + c] = (bits & (1u << c)) != 0u ? s[32 * w + c] : 0xff800000u;
+  }
+}
+
 // One unit of a CTA's work in the fused backward: key tile kt of key/value head hk, and the query blocks
 // [lo, lo + nb) of each of the query heads h0, h0 + 1, ... : n blocks in all, head by head.
 struct Unit {
@@ -2344,14 +2357,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         mbar_arrive(bar_s_free);  // the tensor core may now write S^T/dP^T of the next block
         const int q0 = at.blk * BQ + w * H;  // first query column of this warpgroup's half
-        bool masked = (q0 + H > N) || (k0 + 128 > Nk) || (CAUSAL && q0 < k0 + 127);
-        int c_lo = CAUSAL ? max(0, key - q0) : 0;  // valid query columns: c_lo <= c < c_hi
-        int c_hi = key < Nk ? N - q0 : 0;
+        const bool masked = !WINDOW && ((q0 + H > N) || (k0 + 128 > Nk) || (CAUSAL && q0 < k0 + 127));
+        const int c_lo = CAUSAL ? max(0, key - q0) : 0;  // valid query columns: c_lo <= c < c_hi
+        const int c_hi = key < Nk ? N - q0 : 0;
         if (WINDOW) {  // a key is seen from its own position on, for one window unless it is a sink
           const int p0 = q0 + args.win.off;
-          masked = masked || p0 < k0 + 127 || (p0 + H - 1 >= k0 + args.win.window && k0 + 128 > args.win.sinks);
-          c_lo = max(0, key - p0);
-          if (key >= args.win.sinks) c_hi = min(c_hi, key + args.win.window - p0);
+          if ((q0 + H > N) || (k0 + 128 > Nk) || p0 < k0 + 127 ||
+              (p0 + H - 1 >= k0 + args.win.window && k0 + 128 > args.win.sinks))
+            hide_queries<H>(s, key - p0, key < args.win.sinks ? c_hi : min(c_hi, key + args.win.window - p0));
         }
         uint32_t pt[H / 2], dst[H / 2];
         if (masked)
