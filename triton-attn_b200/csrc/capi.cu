@@ -198,7 +198,7 @@ extern "C" int tattn_fwd(const void* q, const void* k, const void* v, void* o, f
   a.wait_limit_ns = g_wait_limit_ns.load();
   if (dtype == TATTN_F32) {
     a.qk_scale = sm_scale * kLog2e;
-    return cuda_rc(launch_fwd_f32(D, causal ? kMaskCausal : kMaskNone, q, k, v, sq, sk, sv, a, sm_scale, s));
+    return cuda_rc(launch_fwd_f32(D, causal != 0, q, k, v, sq, sk, sv, a, sm_scale, s));
   }
   if (!layout_ok(q, sq, Z, H, N, D) || !layout_ok(k, sk, Z, H, N, D) || !layout_ok(v, sv, Z, H, N, D) ||
       !layout_ok(o, so, Z, H, N, D))
@@ -287,8 +287,7 @@ int bwd_common(bool dq_pass, const void* q, const void* k, const void* v, const 
   a.wait_limit_ns = g_wait_limit_ns.load();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == TATTN_F32)
-    return cuda_rc(dq_pass ? launch_bwd_dq_f32(D, causal ? kMaskCausal : kMaskNone, a, s)
-                           : launch_bwd_dkdv_f32(D, causal ? kMaskCausal : kMaskNone, a, s));
+    return cuda_rc(dq_pass ? launch_bwd_dq_f32(D, causal != 0, a, s) : launch_bwd_dkdv_f32(D, causal != 0, a, s));
   if (!layout_ok(q, a.sq, Z, H, N, D) || !layout_ok(k, a.sk, Z, H, N, D) || !layout_ok(v, a.sv, Z, H, N, D) ||
       !layout_ok(dout, a.sdo, Z, H, N, D))
     return TATTN_ERR_LAYOUT;
@@ -434,7 +433,7 @@ extern "C" int tattn_window_fwd(const void* q, const void* k, const void* v, voi
   a.win = window_args(H, Hk, Nq, Nk, window, sinks);
   if (dtype == TATTN_F32) {
     a.qk_scale = sm_scale * kLog2e;
-    return cuda_rc(launch_fwd_f32(D, kMaskWindow, q, k, v, sq, sk, sv, a, sm_scale, s));
+    return cuda_rc(launch_window_fwd_f32(D, q, k, v, sq, sk, sv, a, s));
   }
   if (!layout_ok(q, sq, Z, H, Nq, D) || !layout_ok(k, sk, Z, Hk, Nk, D) || !layout_ok(v, sv, Z, Hk, Nk, D) ||
       !layout_ok(o, so, Z, H, Nq, D))
@@ -497,9 +496,7 @@ extern "C" int tattn_window_bwd(const void* q, const void* k, const void* v, con
   a.win = window_args(H, Hk, Nq, Nk, window, sinks);
   if (dtype == TATTN_F32) {
     rc = tattn_bwd_preprocess(o, dout, delta, strides + 12, Z, H, Nq, D, dtype, stream);
-    if (rc == TATTN_OK) rc = cuda_rc(launch_bwd_dkdv_f32(D, kMaskWindow, a, s));
-    if (rc == TATTN_OK) rc = cuda_rc(launch_bwd_dq_f32(D, kMaskWindow, a, s));
-    return rc;
+    return rc != TATTN_OK ? rc : cuda_rc(launch_window_bwd_f32(D, a, s));
   }
   if (!layout_ok(q, a.sq, Z, H, Nq, D) || !layout_ok(k, a.sk, Z, Hk, Nk, D) || !layout_ok(v, a.sv, Z, Hk, Nk, D) ||
       !layout_ok(o, a.so, Z, H, Nq, D) || !layout_ok(dout, a.sdo, Z, H, Nq, D))

@@ -130,10 +130,16 @@ inline int64_t window_bwd_workspace_bytes(int Z, int H, int Hk, int N, int D, co
 }
 
 // SIMT kernels (fp32 inputs; any strides).
-cudaError_t launch_fwd_f32(int D, Mask mask, const void* q, const void* k, const void* v, Strides4 sq,
+cudaError_t launch_fwd_f32(int D, bool causal, const void* q, const void* k, const void* v, Strides4 sq,
                            Strides4 sk, Strides4 sv, const FwdArgs& a, float sm_scale, cudaStream_t s);
-cudaError_t launch_bwd_dq_f32(int D, Mask mask, const BwdArgs& a, cudaStream_t s);
-cudaError_t launch_bwd_dkdv_f32(int D, Mask mask, const BwdArgs& a, cudaStream_t s);
+cudaError_t launch_bwd_dq_f32(int D, bool causal, const BwdArgs& a, cudaStream_t s);
+cudaError_t launch_bwd_dkdv_f32(int D, bool causal, const BwdArgs& a, cudaStream_t s);
+
+// Sliding window with sinks in fp32 (window_f32.cu; any strides). The backward writes dk, dv and dq from
+// a.delta; a.qk_scale and a.sm_scale are signed.
+cudaError_t launch_window_fwd_f32(int D, const void* q, const void* k, const void* v, Strides4 sq, Strides4 sk,
+                                  Strides4 sv, const FwdArgs& a, cudaStream_t s);
+cudaError_t launch_window_bwd_f32(int D, const BwdArgs& a, cudaStream_t s);
 
 // delta = rowsum(dO * O) in fp32 (fp16 or fp32 inputs); also zeroes the rows of a.dq_acc and the
 // counter a.grid_sync when they are set (the fused backward's workspace).

@@ -40,41 +40,22 @@ __device__ __forceinline__ float group_sum(float x) {
 
 __device__ __forceinline__ float ld_f32(const float* p) { return __ldg(p); }
 
-// Does query row `row` see key `col`? N query rows, Nk keys.
-template <int MASK>
-__device__ __forceinline__ bool sees(int row, int col, int N, int Nk, const WindowArgs& w) {
-  if (MASK == kMaskWindow) {
-    const int p = row + w.off;
-    return row < N && col <= p && col < Nk && (col > p - w.window || col < w.sinks);
-  }
-  return row < N && col < Nk && !(MASK == kMaskCausal && col > row);
-}
-
-// The key block after cb for query rows [rb, rb + SB): the next one, but past the sinks straight to the
-// first one that any of the rows' windows reaches.
-template <int MASK, int SB>
-__device__ __forceinline__ int next_key_block(int cb, int rb, const WindowArgs& w) {
-  cb += SB;
-  if (MASK == kMaskWindow && cb >= w.sinks) cb = max(cb, max(0, rb + w.off - w.window + 1) / SB * SB);
-  return cb;
-}
-
-template <int D, int MASK>
+template <int D>
 __global__ void __launch_bounds__(SIMT_THREADS)
     fwd_f32_kernel(const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
-                   Strides4 sq, Strides4 sk, Strides4 sv, FwdArgs a, float qk_scale) {
+                   Strides4 sq, Strides4 sk, Strides4 sv, FwdArgs a, float qk_scale, bool causal) {
   constexpr int SB = Simt<D>::SB, G = Simt<D>::G;
   __shared__ float Qs[SB][D + 1];
   __shared__ float Ks[SB][D + 1];
   __shared__ float Vs[SB][D + 1];
   __shared__ float Ps[SB][SB + 1];
-  const int N = a.N, Nk = MASK == kMaskWindow ? a.win.Nk : N;
-  const int bh = blockIdx.y, zi = bh / a.H, hi = bh % a.H, hk = MASK == kMaskWindow ? hi / a.win.group : hi;
+  const int N = a.N;
+  const int bh = blockIdx.y, zi = bh / a.H, hi = bh % a.H;
   const int rb = blockIdx.x * SB;
   const int tid = threadIdx.x, r = tid / G, g = tid % G;
   const float* qb = q + zi * sq.z + hi * sq.h;
-  const float* kb = k + zi * sk.z + hk * sk.h;
-  const float* vb = v + zi * sv.z + hk * sv.h;
+  const float* kb = k + zi * sk.z + hi * sk.h;
+  const float* vb = v + zi * sv.z + hi * sv.h;
   for (int e = tid; e < SB * D; e += SIMT_THREADS) {
     const int rr = e / D, d = e % D;
     Qs[rr][d] = (rb + rr < N) ? ld_f32(qb + int64_t(rb + rr) * sq.n + d * sq.d) : 0.f;
@@ -84,12 +65,12 @@ __global__ void __launch_bounds__(SIMT_THREADS)
   float acc[D / G];
 #pragma unroll
   for (int dd = 0; dd < D / G; ++dd) acc[dd] = 0.f;
-  const int hi_col = MASK == kMaskNone ? Nk : min(rb + SB + (MASK == kMaskWindow ? a.win.off : 0), Nk);
-  for (int cb = next_key_block<MASK, SB>(-SB, rb, a.win); cb < hi_col; cb = next_key_block<MASK, SB>(cb, rb, a.win)) {
+  const int hi_col = causal ? min(rb + SB, N) : N;
+  for (int cb = 0; cb < hi_col; cb += SB) {
     __syncthreads();
     for (int e = tid; e < SB * D; e += SIMT_THREADS) {
       const int cc = e / D, d = e % D;
-      const bool ok = cb + cc < Nk;
+      const bool ok = cb + cc < N;
       Ks[cc][d] = ok ? ld_f32(kb + int64_t(cb + cc) * sk.n + d * sk.d) : 0.f;
       Vs[cc][d] = ok ? ld_f32(vb + int64_t(cb + cc) * sv.n + d * sv.d) : 0.f;
     }
@@ -103,8 +84,7 @@ __global__ void __launch_bounds__(SIMT_THREADS)
 #pragma unroll 16
       for (int d = 0; d < D; ++d) s = fmaf(Qs[r][d], Ks[c][d], s);
       s *= qk_scale;
-      if (MASK == kMaskWindow ? !sees<MASK>(row, col, N, Nk, a.win) : (col >= N || (MASK == kMaskCausal && col > row)))
-        s = -INFINITY;
+      if (col >= N || (causal && col > row)) s = -INFINITY;
       x[t] = s;
       mx = fmaxf(mx, s);
     }
@@ -142,21 +122,21 @@ __global__ void __launch_bounds__(SIMT_THREADS)
 }
 
 // dQ for one block of SB query rows (reference: _bwd_dq_kernel, kernels.py:242-321).
-template <int D, int MASK>
-__global__ void __launch_bounds__(SIMT_THREADS) bwd_dq_f32_kernel(BwdArgs a) {
+template <int D>
+__global__ void __launch_bounds__(SIMT_THREADS) bwd_dq_f32_kernel(BwdArgs a, bool causal) {
   constexpr int SB = Simt<D>::SB, G = Simt<D>::G;
   __shared__ float Qs[SB][D + 1];
   __shared__ float DOs[SB][D + 1];
   __shared__ float Ks[SB][D + 1];
   __shared__ float Vs[SB][D + 1];
   __shared__ float DSs[SB][SB + 1];
-  const int N = a.N, Nk = MASK == kMaskWindow ? a.win.Nk : N;
-  const int bh = blockIdx.y, zi = bh / a.H, hi = bh % a.H, hk = MASK == kMaskWindow ? hi / a.win.group : hi;
+  const int N = a.N;
+  const int bh = blockIdx.y, zi = bh / a.H, hi = bh % a.H;
   const int rb = blockIdx.x * SB;
   const int tid = threadIdx.x, r = tid / G, g = tid % G;
   const float* q = reinterpret_cast<const float*>(a.q) + zi * a.sq.z + hi * a.sq.h;
-  const float* k = reinterpret_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h;
-  const float* v = reinterpret_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h;
+  const float* k = reinterpret_cast<const float*>(a.k) + zi * a.sk.z + hi * a.sk.h;
+  const float* v = reinterpret_cast<const float*>(a.v) + zi * a.sv.z + hi * a.sv.h;
   const float* dout = reinterpret_cast<const float*>(a.dout) + zi * a.sdo.z + hi * a.sdo.h;
   for (int e = tid; e < SB * D; e += SIMT_THREADS) {
     const int rr = e / D, d = e % D;
@@ -171,12 +151,12 @@ __global__ void __launch_bounds__(SIMT_THREADS) bwd_dq_f32_kernel(BwdArgs a) {
   float acc[D / G];
 #pragma unroll
   for (int dd = 0; dd < D / G; ++dd) acc[dd] = 0.f;
-  const int hi_col = MASK == kMaskNone ? Nk : min(rb + SB + (MASK == kMaskWindow ? a.win.off : 0), Nk);
-  for (int cb = next_key_block<MASK, SB>(-SB, rb, a.win); cb < hi_col; cb = next_key_block<MASK, SB>(cb, rb, a.win)) {
+  const int hi_col = causal ? min(rb + SB, N) : N;
+  for (int cb = 0; cb < hi_col; cb += SB) {
     __syncthreads();
     for (int e = tid; e < SB * D; e += SIMT_THREADS) {
       const int cc = e / D, d = e % D;
-      const bool ok = cb + cc < Nk;
+      const bool ok = cb + cc < N;
       Ks[cc][d] = ok ? ld_f32(k + int64_t(cb + cc) * a.sk.n + d * a.sk.d) : 0.f;
       Vs[cc][d] = ok ? ld_f32(v + int64_t(cb + cc) * a.sv.n + d * a.sv.d) : 0.f;
     }
@@ -190,7 +170,8 @@ __global__ void __launch_bounds__(SIMT_THREADS) bwd_dq_f32_kernel(BwdArgs a) {
         s = fmaf(Qs[r][d], Ks[c][d], s);
         dp = fmaf(DOs[r][d], Vs[c][d], dp);
       }
-      const float p = sees<MASK>(row, col, N, Nk, a.win) ? exp2f(s * qks - m_r) : 0.f;
+      const bool keep = row < N && col < N && !(causal && col > row);
+      const float p = keep ? exp2f(s * qks - m_r) : 0.f;
       DSs[r][c] = p * (dp - d_r);
     }
     __syncwarp();
@@ -210,10 +191,9 @@ __global__ void __launch_bounds__(SIMT_THREADS) bwd_dq_f32_kernel(BwdArgs a) {
   }
 }
 
-// dK, dV for one block of SB keys (reference: _bwd_dkdv_kernel, kernels.py:151-239). kMaskWindow: of one
-// key/value head, summed over the query heads that share it.
-template <int D, int MASK>
-__global__ void __launch_bounds__(SIMT_THREADS) bwd_dkdv_f32_kernel(BwdArgs a) {
+// dK, dV for one block of SB keys (reference: _bwd_dkdv_kernel, kernels.py:151-239).
+template <int D>
+__global__ void __launch_bounds__(SIMT_THREADS) bwd_dkdv_f32_kernel(BwdArgs a, bool causal) {
   constexpr int SB = Simt<D>::SB, G = Simt<D>::G;
   __shared__ float Ks[SB][D + 1];
   __shared__ float Vs[SB][D + 1];
@@ -222,16 +202,17 @@ __global__ void __launch_bounds__(SIMT_THREADS) bwd_dkdv_f32_kernel(BwdArgs a) {
   __shared__ float Pt[SB][SB + 1];
   __shared__ float DSt[SB][SB + 1];
   __shared__ float Ms[SB], Ds[SB];
-  const int N = a.N, Nk = MASK == kMaskWindow ? a.win.Nk : N;
-  const int Hk = MASK == kMaskWindow ? a.win.Hk : a.H, group = MASK == kMaskWindow ? a.win.group : 1;
-  const int bh = blockIdx.y, zi = bh / Hk, hk = bh % Hk;
+  const int N = a.N;
+  const int bh = blockIdx.y, zi = bh / a.H, hi = bh % a.H;
   const int cb = blockIdx.x * SB;
   const int tid = threadIdx.x, c = tid / G, g = tid % G;
-  const float* k = reinterpret_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h;
-  const float* v = reinterpret_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h;
+  const float* q = reinterpret_cast<const float*>(a.q) + zi * a.sq.z + hi * a.sq.h;
+  const float* k = reinterpret_cast<const float*>(a.k) + zi * a.sk.z + hi * a.sk.h;
+  const float* v = reinterpret_cast<const float*>(a.v) + zi * a.sv.z + hi * a.sv.h;
+  const float* dout = reinterpret_cast<const float*>(a.dout) + zi * a.sdo.z + hi * a.sdo.h;
   for (int e = tid; e < SB * D; e += SIMT_THREADS) {
     const int cc = e / D, d = e % D;
-    const bool ok = cb + cc < Nk;
+    const bool ok = cb + cc < N;
     Ks[cc][d] = ok ? ld_f32(k + int64_t(cb + cc) * a.sk.n + d * a.sk.d) : 0.f;
     Vs[cc][d] = ok ? ld_f32(v + int64_t(cb + cc) * a.sv.n + d * a.sv.d) : 0.f;
   }
@@ -240,63 +221,52 @@ __global__ void __launch_bounds__(SIMT_THREADS) bwd_dkdv_f32_kernel(BwdArgs a) {
   float dk[D / G], dv[D / G];
 #pragma unroll
   for (int dd = 0; dd < D / G; ++dd) dk[dd] = dv[dd] = 0.f;
-  // Query rows before this key block never see it; a window's rows end one window after its last key,
-  // unless it holds a sink.
-  int lo = MASK == kMaskCausal ? cb : 0, end = N;
-  if (MASK == kMaskWindow) {
-    lo = max(0, cb - a.win.off);
-    if (cb >= a.win.sinks) end = int(min(int64_t(N), int64_t(cb) + SB - 1 + a.win.window - a.win.off));
-  }
-  for (int hg = 0; hg < group; ++hg) {
-    const int hi = hk * group + hg;
-    const int64_t qh = int64_t(zi) * a.H + hi;
-    const float* q = reinterpret_cast<const float*>(a.q) + zi * a.sq.z + hi * a.sq.h;
-    const float* dout = reinterpret_cast<const float*>(a.dout) + zi * a.sdo.z + hi * a.sdo.h;
-    for (int rb = lo; rb < end; rb += SB) {
-      __syncthreads();
-      for (int e = tid; e < SB * D; e += SIMT_THREADS) {
-        const int rr = e / D, d = e % D;
-        const bool ok = rb + rr < N;
-        Qs[rr][d] = ok ? ld_f32(q + int64_t(rb + rr) * a.sq.n + d * a.sq.d) : 0.f;
-        DOs[rr][d] = ok ? ld_f32(dout + int64_t(rb + rr) * a.sdo.n + d * a.sdo.d) : 0.f;
-      }
-      if (tid < SB) {
-        const bool ok = rb + tid < N;
-        Ms[tid] = ok ? a.m[qh * N + rb + tid] : 0.f;
-        Ds[tid] = ok ? a.delta[qh * N + rb + tid] : 0.f;
-      }
-      __syncthreads();
+  const int lo = causal ? cb : 0;  // query rows before this key block never see it
+  for (int rb = lo; rb < N; rb += SB) {
+    __syncthreads();
+    for (int e = tid; e < SB * D; e += SIMT_THREADS) {
+      const int rr = e / D, d = e % D;
+      const bool ok = rb + rr < N;
+      Qs[rr][d] = ok ? ld_f32(q + int64_t(rb + rr) * a.sq.n + d * a.sq.d) : 0.f;
+      DOs[rr][d] = ok ? ld_f32(dout + int64_t(rb + rr) * a.sdo.n + d * a.sdo.d) : 0.f;
+    }
+    if (tid < SB) {
+      const bool ok = rb + tid < N;
+      Ms[tid] = ok ? a.m[int64_t(bh) * N + rb + tid] : 0.f;
+      Ds[tid] = ok ? a.delta[int64_t(bh) * N + rb + tid] : 0.f;
+    }
+    __syncthreads();
 #pragma unroll
-      for (int t = 0; t < SB / G; ++t) {
-        const int rr = g + G * t, row = rb + rr;
-        float s = 0.f, dp = 0.f;
+    for (int t = 0; t < SB / G; ++t) {
+      const int rr = g + G * t, row = rb + rr;
+      float s = 0.f, dp = 0.f;
 #pragma unroll 16
-        for (int d = 0; d < D; ++d) {
-          s = fmaf(Qs[rr][d], Ks[c][d], s);
-          dp = fmaf(DOs[rr][d], Vs[c][d], dp);
-        }
-        const float p = sees<MASK>(row, col, N, Nk, a.win) ? exp2f(s * qks - Ms[rr]) : 0.f;
-        Pt[c][rr] = p;
-        DSt[c][rr] = p * (dp - Ds[rr]);
+      for (int d = 0; d < D; ++d) {
+        s = fmaf(Qs[rr][d], Ks[c][d], s);
+        dp = fmaf(DOs[rr][d], Vs[c][d], dp);
       }
-      __syncwarp();
+      const bool keep = row < N && col < N && !(causal && col > row);
+      const float p = keep ? exp2f(s * qks - Ms[rr]) : 0.f;
+      Pt[c][rr] = p;
+      DSt[c][rr] = p * (dp - Ds[rr]);
+    }
+    __syncwarp();
 #pragma unroll
-      for (int dd = 0; dd < D / G; ++dd) {
-        const int d = g + G * dd;
-        float x = dv[dd], y = dk[dd];
+    for (int dd = 0; dd < D / G; ++dd) {
+      const int d = g + G * dd;
+      float x = dv[dd], y = dk[dd];
 #pragma unroll 8
-        for (int rr = 0; rr < SB; ++rr) {
-          x = fmaf(Pt[c][rr], DOs[rr][d], x);
-          y = fmaf(DSt[c][rr], Qs[rr][d], y);
-        }
-        dv[dd] = x;
-        dk[dd] = y;
+      for (int rr = 0; rr < SB; ++rr) {
+        x = fmaf(Pt[c][rr], DOs[rr][d], x);
+        y = fmaf(DSt[c][rr], Qs[rr][d], y);
       }
+      dv[dd] = x;
+      dk[dd] = y;
     }
   }
-  if (col < Nk) {
-    float* dkp = reinterpret_cast<float*>(a.dk) + (int64_t(bh) * Nk + col) * D;
-    float* dvp = reinterpret_cast<float*>(a.dv) + (int64_t(bh) * Nk + col) * D;
+  if (col < N) {
+    float* dkp = reinterpret_cast<float*>(a.dk) + (int64_t(bh) * N + col) * D;
+    float* dvp = reinterpret_cast<float*>(a.dv) + (int64_t(bh) * N + col) * D;
 #pragma unroll
     for (int dd = 0; dd < D / G; ++dd) {
       dkp[g + G * dd] = dk[dd] * a.sm_scale;
@@ -355,65 +325,59 @@ __global__ void __launch_bounds__(256) preprocess_kernel(BwdArgs a) {
   if (a.grid_sync != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *a.grid_sync = 0u;  // its grid barrier
 }
 
-template <int D, int MASK>
-cudaError_t fwd_f32_impl(const void* q, const void* k, const void* v, Strides4 sq, Strides4 sk, Strides4 sv,
-                         const FwdArgs& a, float qk_scale, cudaStream_t s) {
+template <int D>
+cudaError_t fwd_f32_impl(bool causal, const void* q, const void* k, const void* v, Strides4 sq, Strides4 sk,
+                         Strides4 sv, const FwdArgs& a, float qk_scale, cudaStream_t s) {
   constexpr int SB = Simt<D>::SB;
   dim3 grid((a.N + SB - 1) / SB, a.Z * a.H);
-  fwd_f32_kernel<D, MASK><<<grid, SIMT_THREADS, 0, s>>>(static_cast<const float*>(q), static_cast<const float*>(k),
-                                                        static_cast<const float*>(v), sq, sk, sv, a, qk_scale);
-  return cudaGetLastError();
-}
-
-template <int D, int MASK>
-cudaError_t bwd_f32_impl(bool dq_pass, const BwdArgs& a, cudaStream_t s) {
-  constexpr int SB = Simt<D>::SB;
-  if (dq_pass) {
-    bwd_dq_f32_kernel<D, MASK><<<dim3((a.N + SB - 1) / SB, a.Z * a.H), SIMT_THREADS, 0, s>>>(a);
-  } else {
-    const int Nk = MASK == kMaskWindow ? a.win.Nk : a.N, Hk = MASK == kMaskWindow ? a.win.Hk : a.H;
-    bwd_dkdv_f32_kernel<D, MASK><<<dim3((Nk + SB - 1) / SB, a.Z * Hk), SIMT_THREADS, 0, s>>>(a);
-  }
+  fwd_f32_kernel<D><<<grid, SIMT_THREADS, 0, s>>>(static_cast<const float*>(q), static_cast<const float*>(k),
+                                                  static_cast<const float*>(v), sq, sk, sv, a, qk_scale, causal);
   return cudaGetLastError();
 }
 
 }  // namespace
 
-// Calls f<D, MASK>(...) for the runtime D and mask.
-#define TATTN_F32_MASKS(f, DD, ...)                                       \
-  case DD:                                                                \
-    return mask == kMaskWindow   ? f<DD, kMaskWindow>(__VA_ARGS__)        \
-           : mask == kMaskCausal ? f<DD, kMaskCausal>(__VA_ARGS__)        \
-                                 : f<DD, kMaskNone>(__VA_ARGS__);
-#define TATTN_F32_DISPATCH(f, ...)                                        \
-  switch (D) {                                                            \
-    TATTN_F32_MASKS(f, 16, __VA_ARGS__)                                   \
-    TATTN_F32_MASKS(f, 32, __VA_ARGS__)                                   \
-    TATTN_F32_MASKS(f, 64, __VA_ARGS__)                                   \
-    TATTN_F32_MASKS(f, 128, __VA_ARGS__)                                  \
-    default: return cudaErrorInvalidValue;                                \
-  }
-
-cudaError_t launch_fwd_f32(int D, Mask mask, const void* q, const void* k, const void* v, Strides4 sq, Strides4 sk,
-                           Strides4 sv, const FwdArgs& a, float sm_scale, cudaStream_t s) {
+cudaError_t launch_fwd_f32(int D, bool causal, const void* q, const void* k, const void* v, Strides4 sq,
+                           Strides4 sk, Strides4 sv, const FwdArgs& a, float sm_scale, cudaStream_t s) {
   const float qk = sm_scale * 1.4426950408889634f;
   if (a.N == 0 || a.Z * a.H == 0) return cudaSuccess;
-  TATTN_F32_DISPATCH(fwd_f32_impl, q, k, v, sq, sk, sv, a, qk, s)
+  switch (D) {
+    case 16: return fwd_f32_impl<16>(causal, q, k, v, sq, sk, sv, a, qk, s);
+    case 32: return fwd_f32_impl<32>(causal, q, k, v, sq, sk, sv, a, qk, s);
+    case 64: return fwd_f32_impl<64>(causal, q, k, v, sq, sk, sv, a, qk, s);
+    case 128: return fwd_f32_impl<128>(causal, q, k, v, sq, sk, sv, a, qk, s);
+    default: return cudaErrorInvalidValue;
+  }
 }
 
-static cudaError_t bwd_f32_dispatch(int D, bool dq_pass, Mask mask, const BwdArgs& a, cudaStream_t s) {
+template <int D>
+cudaError_t bwd_f32_impl(bool dq_pass, bool causal, const BwdArgs& a, cudaStream_t s) {
+  constexpr int SB = Simt<D>::SB;
+  dim3 grid((a.N + SB - 1) / SB, a.Z * a.H);
+  if (dq_pass)
+    bwd_dq_f32_kernel<D><<<grid, SIMT_THREADS, 0, s>>>(a, causal);
+  else
+    bwd_dkdv_f32_kernel<D><<<grid, SIMT_THREADS, 0, s>>>(a, causal);
+  return cudaGetLastError();
+}
+
+static cudaError_t bwd_f32_dispatch(int D, bool dq_pass, bool causal, const BwdArgs& a, cudaStream_t s) {
   if (a.N == 0 || a.Z * a.H == 0) return cudaSuccess;
-  TATTN_F32_DISPATCH(bwd_f32_impl, dq_pass, a, s)
+  switch (D) {
+    case 16: return bwd_f32_impl<16>(dq_pass, causal, a, s);
+    case 32: return bwd_f32_impl<32>(dq_pass, causal, a, s);
+    case 64: return bwd_f32_impl<64>(dq_pass, causal, a, s);
+    case 128: return bwd_f32_impl<128>(dq_pass, causal, a, s);
+    default: return cudaErrorInvalidValue;
+  }
 }
-#undef TATTN_F32_DISPATCH
-#undef TATTN_F32_MASKS
 
-cudaError_t launch_bwd_dq_f32(int D, Mask mask, const BwdArgs& a, cudaStream_t s) {
-  return bwd_f32_dispatch(D, true, mask, a, s);
+cudaError_t launch_bwd_dq_f32(int D, bool causal, const BwdArgs& a, cudaStream_t s) {
+  return bwd_f32_dispatch(D, true, causal, a, s);
 }
 
-cudaError_t launch_bwd_dkdv_f32(int D, Mask mask, const BwdArgs& a, cudaStream_t s) {
-  return bwd_f32_dispatch(D, false, mask, a, s);
+cudaError_t launch_bwd_dkdv_f32(int D, bool causal, const BwdArgs& a, cudaStream_t s) {
+  return bwd_f32_dispatch(D, false, causal, a, s);
 }
 
 cudaError_t launch_bwd_preprocess(int D, bool is_f16, const BwdArgs& a, cudaStream_t s) {

@@ -1,0 +1,328 @@
+// Sliding-window attention with sinks for fp32 on CUDA cores: forward, dK/dV and dQ.
+//
+// The mathematics is the fp16 kernels' (base-2 online softmax, M = m + log2 l, P rebuilt from M in the
+// backward) with every product and sum in fp32: tcgen05 has no fp32 MMA, and fp32 calls are held to fp32
+// accuracy. Two kernels for the backward, dK/dV by key tiles and dQ by query tiles, so that nothing is
+// summed by atomics and results are bitwise reproducible.
+//
+// The bound is the FMA pipe (4 D flop forward and 14 D backward a pair) fed from shared memory: 64 x 64 tiles,
+// 256 threads as 16 x 16, and a thread computes 4 x 4 scores (rows 4 ty + i, columns tx + 16 j) from 16-byte
+// reads along D: 8 reads for 64 FMAs, which a warp's broadcasts turn into 12 shared-memory cycles against
+// 16 of the FMA pipes. Then 4 rows x D / 16 columns of the products with V, K, Q and dO the same way.
+#include <math.h>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace tattn {
+namespace {
+
+constexpr int kThreads = 256, TB = 64;  // threads; rows and columns of a tile
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Row pitch in floats: 16-byte units a row odd in number, so that 16 rows at one unit are in different banks.
+template <int D>
+constexpr int kPitch = D + 4;
+constexpr int kPitchP = TB + 4;
+
+// Rows [r0, r0 + 64) of a [n, D] matrix into shared memory; rows past n are zeros.
+template <int D>
+__device__ __forceinline__ void load_rows(float* dst, const float* src, const Strides4& s, int r0, int n) {
+#pragma unroll 8
+  for (int e = threadIdx.x; e < TB * D; e += kThreads) {
+    const int r = e / D, d = e % D;
+    dst[r * kPitch<D> + d] = r0 + r < n ? __ldg(src + int64_t(r0 + r) * s.n + d * s.d) : 0.f;
+  }
+}
+
+// c[i][j] += a[4 ty + i] . b[tx + 16 j] over D.
+template <int D>
+__device__ __forceinline__ void rows_dot(const float* a, const float* b, int ty, int tx, float (*c)[4]) {
+#pragma unroll 4
+  for (int d = 0; d < D; d += 4) {
+    float4 x[4], y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(a + (4 * ty + i) * kPitch<D> + d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * kPitch<D> + d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        c[i][j] = fmaf(x[i].w, y[j].w, fmaf(x[i].z, y[j].z, fmaf(x[i].y, y[j].y, fmaf(x[i].x, y[j].x, c[i][j]))));
+  }
+}
+
+// acc[i][e] += sum over r of p[4 ty + i][r] b[r][D / 16 tx + e].
+template <int D>
+__device__ __forceinline__ void rows_times(const float* p, const float* b, int ty, int tx, float (*acc)[D / 16]) {
+  constexpr int E = D / 16;
+#pragma unroll 2
+  for (int r = 0; r < TB; r += 4) {
+    float4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(p + (4 * ty + i) * kPitchP + r);
+#pragma unroll
+    for (int rr = 0; rr < 4; ++rr) {
+      float y[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[e] = b[(r + rr) * kPitch<D> + E * tx + e];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float w = rr == 0 ? x[i].x : rr == 1 ? x[i].y : rr == 2 ? x[i].z : x[i].w;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[i][e] = fmaf(w, y[e], acc[i][e]);
+      }
+    }
+  }
+}
+
+// Does query row `row` of N see key `col`?
+__device__ __forceinline__ bool sees(int row, int col, int N, const WindowArgs& w) {
+  const int p = row + w.off;
+  return row < N && col <= p && (col > p - w.window || col < w.sinks);
+}
+
+// Key tiles of query rows [r0, r0 + 64): those with sinks, then those that a window reaches, up to the diagonal.
+__device__ __forceinline__ int next_key_tile(int k0, int r0, const WindowArgs& w) {
+  k0 += TB;
+  return k0 >= w.sinks ? max(k0, max(0, r0 + w.off - w.window + 1) / TB * TB) : k0;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads) window_fwd_f32_kernel(const float* q, const float* k, const float* v,
+                                                                  Strides4 sq, Strides4 sk, Strides4 sv, FwdArgs a) {
+  extern __shared__ __align__(16) float smem[];
+  float *Qs = smem, *Ks = Qs + TB * kPitch<D>, *Vs = Ks + TB * kPitch<D>, *Ps = Vs + TB * kPitch<D>;
+  const int N = a.N, Nk = a.win.Nk, r0 = blockIdx.x * TB;
+  const int zi = blockIdx.y / a.H, hi = blockIdx.y % a.H, hk = hi / a.win.group;
+  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  k += zi * sk.z + hk * sk.h;
+  v += zi * sv.z + hk * sv.h;
+  load_rows<D>(Qs, q + zi * sq.z + hi * sq.h, sq, r0, N);
+  float m[4], l[4], acc[4][D / 16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) acc[i][e] = 0.f;
+  }
+  const int end = min(r0 + TB + a.win.off, Nk);
+  for (int k0 = next_key_tile(-TB, r0, a.win); k0 < end; k0 = next_key_tile(k0, r0, a.win)) {
+    __syncthreads();
+    load_rows<D>(Ks, k, sk, k0, Nk);
+    load_rows<D>(Vs, v, sv, k0, Nk);
+    __syncthreads();
+    float s[4][4] = {};
+    rows_dot<D>(Qs, Ks, ty, tx, s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float mx = m[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = sees(r0 + 4 * ty + i, k0 + tx + 16 * j, N, a.win) ? s[i][j] * a.qk_scale : -INFINITY;
+        mx = fmaxf(mx, s[i][j]);
+      }
+#pragma unroll
+      for (int o = 1; o < 16; o *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float use = mx == -INFINITY ? 0.f : mx, alpha = exp2f(m[i] - use);
+      m[i] = mx;
+      l[i] *= alpha;
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) acc[i][e] *= alpha;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float p = exp2f(s[i][j] - use);
+        l[i] += p;  // this thread's columns
+        Ps[(4 * ty + i) * kPitchP + tx + 16 * j] = p;
+      }
+    }
+    __syncwarp();  // a row of P is written and read by the 16 threads of one half warp
+    rows_times<D>(Ps, Vs, ty, tx, acc);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int o = 1; o < 16; o *= 2) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+    const int row = r0 + 4 * ty + i;
+    if (row >= N) continue;
+    float* o = static_cast<float*>(a.o) + zi * a.so.z + hi * a.so.h + int64_t(row) * a.so.n;
+    const float inv = 1.f / l[i];
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) o[(D / 16 * tx + e) * a.so.d] = acc[i][e] * inv;
+    if (tx == 0) a.m[int64_t(blockIdx.y) * N + row] = m[i] + log2f(l[i]);
+  }
+}
+
+// P and dS of rows 4 ty + i of A (with C) and rows tx + 16 j of B (with E): A, B are queries and keys, or keys
+// and queries (KEYS); C, E their dO and V, or V and dO.
+template <int D, bool KEYS>
+__device__ __forceinline__ void p_ds(const BwdArgs& a, const float* A, const float* B, const float* C, const float* E,
+                                     int ty, int tx, int a0, int b0, const float* Ms, const float* Ds, float (*p)[4],
+                                     float (*ds)[4]) {
+  float s[4][4] = {}, dp[4][4] = {};
+  rows_dot<D>(A, B, ty, tx, s);
+  rows_dot<D>(C, E, ty, tx, dp);
+  const float qks = a.sm_scale * kLog2e;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int ra = 4 * ty + i, rb = tx + 16 * j, row = KEYS ? rb : ra;  // the tile's query row
+      const bool see = KEYS ? sees(b0 + rb, a0 + ra, a.N, a.win) : sees(a0 + ra, b0 + rb, a.N, a.win);
+      p[i][j] = see ? exp2f(s[i][j] * qks - Ms[row]) : 0.f;
+      ds[i][j] = p[i][j] * (dp[i][j] - Ds[row]);
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads) window_dq_f32_kernel(BwdArgs a) {
+  extern __shared__ __align__(16) float smem[];
+  float *Qs = smem, *Os = Qs + TB * kPitch<D>, *Ks = Os + TB * kPitch<D>, *Vs = Ks + TB * kPitch<D>;
+  float *DSs = Vs + TB * kPitch<D>, *Ms = DSs + TB * kPitchP, *Ds = Ms + TB;
+  const int N = a.N, Nk = a.win.Nk, r0 = blockIdx.x * TB;
+  const int zi = blockIdx.y / a.H, hi = blockIdx.y % a.H, hk = hi / a.win.group;
+  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  const float* k = static_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h;
+  const float* v = static_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h;
+  load_rows<D>(Qs, static_cast<const float*>(a.q) + zi * a.sq.z + hi * a.sq.h, a.sq, r0, N);
+  load_rows<D>(Os, static_cast<const float*>(a.dout) + zi * a.sdo.z + hi * a.sdo.h, a.sdo, r0, N);
+  if (threadIdx.x < TB) {
+    const int row = r0 + threadIdx.x;
+    Ms[threadIdx.x] = row < N ? a.m[int64_t(blockIdx.y) * N + row] : 0.f;
+    Ds[threadIdx.x] = row < N ? a.delta[int64_t(blockIdx.y) * N + row] : 0.f;
+  }
+  float acc[4][D / 16] = {};
+  const int end = min(r0 + TB + a.win.off, Nk);
+  for (int k0 = next_key_tile(-TB, r0, a.win); k0 < end; k0 = next_key_tile(k0, r0, a.win)) {
+    __syncthreads();
+    load_rows<D>(Ks, k, a.sk, k0, Nk);
+    load_rows<D>(Vs, v, a.sv, k0, Nk);
+    __syncthreads();
+    float p[4][4], ds[4][4];
+    p_ds<D, false>(a, Qs, Ks, Os, Vs, ty, tx, r0, k0, Ms, Ds, p, ds);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) DSs[(4 * ty + i) * kPitchP + tx + 16 * j] = ds[i][j];
+    __syncwarp();
+    rows_times<D>(DSs, Ks, ty, tx, acc);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = r0 + 4 * ty + i;
+    if (row >= N) continue;
+    float* dq = static_cast<float*>(a.dq) + (int64_t(blockIdx.y) * N + row) * D + D / 16 * tx;
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) dq[e] = acc[i][e] * a.sm_scale;
+  }
+}
+
+// One key tile of one key/value head, summed over the query heads that share it.
+template <int D>
+__global__ void __launch_bounds__(kThreads) window_dkdv_f32_kernel(BwdArgs a) {
+  extern __shared__ __align__(16) float smem[];
+  float *Ks = smem, *Vs = Ks + TB * kPitch<D>, *Qs = Vs + TB * kPitch<D>, *Os = Qs + TB * kPitch<D>;
+  float *Ps = Os + TB * kPitch<D>, *DSs = Ps + TB * kPitchP, *Ms = DSs + TB * kPitchP, *Ds = Ms + TB;
+  const int N = a.N, Nk = a.win.Nk, k0 = blockIdx.x * TB;
+  const int zi = blockIdx.y / a.win.Hk, hk = blockIdx.y % a.win.Hk;
+  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  load_rows<D>(Ks, static_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h, a.sk, k0, Nk);
+  load_rows<D>(Vs, static_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h, a.sv, k0, Nk);
+  float dk[4][D / 16] = {}, dv[4][D / 16] = {};
+  // Rows from the first key's position on; without a sink in the tile, up to one window past its last key.
+  const int first = max(0, k0 - a.win.off);
+  const int end = k0 < a.win.sinks ? N : int(min(int64_t(N), int64_t(k0) + TB - 1 + a.win.window - a.win.off));
+  for (int g = 0; g < a.win.group; ++g) {
+    const int hi = hk * a.win.group + g;
+    const float* q = static_cast<const float*>(a.q) + zi * a.sq.z + hi * a.sq.h;
+    const float* dout = static_cast<const float*>(a.dout) + zi * a.sdo.z + hi * a.sdo.h;
+    const int64_t rows = (int64_t(zi) * a.H + hi) * N;
+    for (int r0 = first; r0 < end; r0 += TB) {
+      __syncthreads();
+      load_rows<D>(Qs, q, a.sq, r0, N);
+      load_rows<D>(Os, dout, a.sdo, r0, N);
+      if (threadIdx.x < TB) {
+        const int row = r0 + threadIdx.x;
+        Ms[threadIdx.x] = row < N ? a.m[rows + row] : 0.f;
+        Ds[threadIdx.x] = row < N ? a.delta[rows + row] : 0.f;
+      }
+      __syncthreads();
+      float p[4][4], ds[4][4];
+      p_ds<D, true>(a, Ks, Qs, Vs, Os, ty, tx, k0, r0, Ms, Ds, p, ds);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          Ps[(4 * ty + i) * kPitchP + tx + 16 * j] = p[i][j];
+          DSs[(4 * ty + i) * kPitchP + tx + 16 * j] = ds[i][j];
+        }
+      __syncwarp();
+      rows_times<D>(Ps, Os, ty, tx, dv);
+      rows_times<D>(DSs, Qs, ty, tx, dk);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int key = k0 + 4 * ty + i;
+    if (key >= Nk) continue;
+    const int64_t at = (int64_t(blockIdx.y) * Nk + key) * D + D / 16 * tx;
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) {
+      static_cast<float*>(a.dk)[at + e] = dk[i][e] * a.sm_scale;
+      static_cast<float*>(a.dv)[at + e] = dv[i][e];
+    }
+  }
+}
+
+template <typename Kernel, typename... Args>
+cudaError_t launch(Kernel kernel, int rows, long long heads, int floats, cudaStream_t s, const Args&... args) {
+  if (heads > 65535) return cudaErrorInvalidConfiguration;
+  const int smem = floats * 4;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  kernel<<<dim3((rows + TB - 1) / TB, unsigned(heads)), kThreads, smem, s>>>(args...);
+  return cudaGetLastError();
+}
+
+template <int D>
+cudaError_t fwd_impl(const float* q, const float* k, const float* v, const Strides4& sq, const Strides4& sk,
+                     const Strides4& sv, const FwdArgs& a, cudaStream_t s) {
+  return launch(window_fwd_f32_kernel<D>, a.N, (long long)a.Z * a.H, TB * (3 * kPitch<D> + kPitchP), s, q, k, v, sq, sk,
+                sv, a);
+}
+
+template <int D>
+cudaError_t bwd_impl(const BwdArgs& a, cudaStream_t s) {
+  const cudaError_t e = launch(window_dkdv_f32_kernel<D>, a.win.Nk, (long long)a.Z * a.win.Hk,
+                               TB * (4 * kPitch<D> + 2 * kPitchP + 2), s, a);
+  if (e != cudaSuccess) return e;
+  return launch(window_dq_f32_kernel<D>, a.N, (long long)a.Z * a.H, TB * (4 * kPitch<D> + kPitchP + 2), s, a);
+}
+
+}  // namespace
+
+cudaError_t launch_window_fwd_f32(int D, const void* q, const void* k, const void* v, Strides4 sq, Strides4 sk,
+                                  Strides4 sv, const FwdArgs& a, cudaStream_t s) {
+  const float *qf = static_cast<const float*>(q), *kf = static_cast<const float*>(k), *vf = static_cast<const float*>(v);
+  switch (D) {
+    case 16: return fwd_impl<16>(qf, kf, vf, sq, sk, sv, a, s);
+    case 32: return fwd_impl<32>(qf, kf, vf, sq, sk, sv, a, s);
+    case 64: return fwd_impl<64>(qf, kf, vf, sq, sk, sv, a, s);
+    case 128: return fwd_impl<128>(qf, kf, vf, sq, sk, sv, a, s);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+cudaError_t launch_window_bwd_f32(int D, const BwdArgs& a, cudaStream_t s) {
+  switch (D) {
+    case 16: return bwd_impl<16>(a, s);
+    case 32: return bwd_impl<32>(a, s);
+    case 64: return bwd_impl<64>(a, s);
+    case 128: return bwd_impl<128>(a, s);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace tattn
