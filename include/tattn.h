@@ -120,7 +120,7 @@ TATTN_API int tattn_window_fwd(const void* q, const void* k, const void* v, void
 
 /* Its backward: delta = rowsum(dO * O), dq [Z, H, Nq, D], and dk, dv [Z, Hk, Nk, D], summed over the query heads
  * that share a head; all dense. strides: 20 int64 = q, k, v, o, dout each (z, h, n, d). delta: fp32 [Z, H,
- * Nq]. workspace: tattn_window_bwd_workspace_bytes bytes, 16-byte aligned (fp32: 0 bytes, may be null). fp16
+ * Nq]. workspace: tattn_window_bwd_workspace_bytes bytes, 16-byte aligned (0 bytes: may be null). fp16
  * sums dq by fp32 additions in the workspace in an order that varies from run to run, as tattn_bwd_fused;
  * dk and dv, and everything in fp32, are bitwise reproducible. */
 TATTN_API int tattn_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, void* dq,

@@ -78,7 +78,9 @@ def test_workspace_size() -> None:
     # 1000 queries are 8 blocks of 128; a window of 100 spans at most ceil(227 / 128) + 1 = 3: 3 chunks.
     assert size(2, 4, 2, 1000, 1000, 64, 0, 100, 4) == 2 * 4 * 1000 * 64 * 4 + 16 + 2 * 2 * 1 * 3 * 2 * 128 * 64 * 4
     assert size(2, 4, 2, 1000, 1000, 64, 0, 1000, 4) == 2 * 4 * 1000 * 64 * 4 + 16  # one chunk: no partials
-    assert size(2, 4, 2, 1000, 1000, 64, 1, 100, 4) == 0  # fp32 needs none
+    # fp32: tiles and blocks of 64, no dQ rows; ceil(163 / 64) + 1 = 4 of 16 blocks: 4 chunks.
+    assert size(2, 4, 2, 1000, 1000, 64, 1, 100, 0) == 0
+    assert size(2, 4, 2, 1000, 1000, 64, 1, 100, 4) == 2 * 2 * 1 * 4 * 2 * 64 * 64 * 4
 
 
 # -------------------------------------------------------------------------------------- on a B200

@@ -495,6 +495,12 @@ extern "C" int tattn_window_bwd(const void* q, const void* k, const void* v, con
   a.wait_limit_ns = g_wait_limit_ns.load();
   a.win = window_args(H, Hk, Nq, Nk, window, sinks);
   if (dtype == TATTN_F32) {
+    a.split = window_split(kWindowF32Tile, kWindowF32Tile, Nq, a.win.window, a.win.sinks);
+    if (a.split.chunks > 1) {
+      if (!workspace) return TATTN_ERR_INVALID_ARGUMENT;
+      if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return TATTN_ERR_LAYOUT;
+      a.part = static_cast<float*>(workspace);
+    }
     rc = tattn_bwd_preprocess(o, dout, delta, strides + 12, Z, H, Nq, D, dtype, stream);
     return rc != TATTN_OK ? rc : cuda_rc(launch_window_bwd_f32(D, a, s));
   }
@@ -507,7 +513,7 @@ extern "C" int tattn_window_bwd(const void* q, const void* k, const void* v, con
   a.dq_acc = static_cast<float*>(workspace);
   char* after = static_cast<char*>(workspace) + int64_t(Z) * H * Nq * D * 4;
   a.grid_sync = reinterpret_cast<unsigned*>(after);
-  a.split = window_split(D, Nq, a.win.window, a.win.sinks);
+  a.split = window_split(128, bwd_fused_query_rows(D), Nq, a.win.window, a.win.sinks);
   a.part = a.split.chunks > 1 ? reinterpret_cast<float*>(after + 16) : nullptr;
   CUtensorMap tq, tk, tv, tdo, tdk, tdv, tdqacc;
   const int q_rows = bwd_fused_query_rows(D), acc_cols = D == 128 ? 32 : D / 2;  // as tattn_bwd_fused
@@ -529,9 +535,12 @@ extern "C" int64_t tattn_window_bwd_workspace_bytes(int Z, int H, int Hk, int Nq
                                                     int sinks) {
   if (!valid_window(Z, H, Hk, Nq, Nk, D, dtype, window, sinks) || double(Z) * H * Nk * (4.0 * D + 4.0) > 4e17)
     return -1;
-  if (dtype == TATTN_F32 || Nq == 0) return 0;
+  if (Nq == 0) return 0;
   const WindowArgs w = window_args(H, Hk, Nq, Nk, window, sinks);
-  return window_bwd_workspace_bytes(Z, H, Hk, Nq, D, window_split(D, Nq, w.window, w.sinks));
+  if (dtype == TATTN_F32)
+    return window_part_bytes(kWindowF32Tile, Z, Hk, D, window_split(kWindowF32Tile, kWindowF32Tile, Nq, w.window, w.sinks));
+  return bwd_fused_workspace_bytes(Z, H, Nq, D) +
+         window_part_bytes(128, Z, Hk, D, window_split(128, bwd_fused_query_rows(D), Nq, w.window, w.sinks));
 }
 
 extern "C" int64_t tattn_bwd_fused_workspace_bytes(int Z, int H, int N, int D) {

@@ -42,7 +42,7 @@ struct FwdArgs {
   WindowArgs win;    // kMaskWindow only
 };
 
-// Fused window backward: the `tiles` first key tiles hold sinks and are seen by every later query, the
+// Window backward: the `tiles` first key tiles hold sinks and are seen by every later query, the
 // others by one window of queries only. Each sink tile's query blocks are cut into `chunks` units of at
 // most `blocks` blocks (tiles = 0, or chunks = 1: no cut).
 struct WindowSplit {
@@ -66,8 +66,8 @@ struct BwdArgs {
   int* status;
   unsigned long long wait_limit_ns;  // bound of every mbarrier wait (tattn_set_wait_limit_ns)
   WindowArgs win;    // kMaskWindow only: dk and dv are then dense [Z, win.Hk, win.Nk, D]
-  WindowSplit split; // kMaskWindow, fused backward only
-  float* part;       // kMaskWindow, fused backward: partial dV and dK of the split key tiles, or null
+  WindowSplit split; // kMaskWindow
+  float* part;       // kMaskWindow: partial dV and dK of the cut key tiles, or null
 };
 
 // Host helpers of the C-ABI layer (capi.cu). device_ready: the current device is an sm_100 one whose primary
@@ -112,21 +112,20 @@ constexpr int kBwdStoreRows = 32;
 __host__ __device__ constexpr int bwd_fused_query_rows(int D) { return D == 128 ? 64 : 128; }
 // Workspace of tattn_bwd_fused: the fp32 dQ rows [Z, H, N, D], then 16 bytes for the grid-barrier counter.
 inline int64_t bwd_fused_workspace_bytes(int Z, int H, int N, int D) { return int64_t(Z) * H * N * D * 4 + 16; }
-// The cut of the sink tiles, so that a unit costs about what a tile with one window of queries does: such
-// a tile sees ceil((window + 127) / BQ) + 1 query blocks at most. At most 32 chunks bound the partials.
-inline WindowSplit window_split(int D, int N, int window, int sinks) {
-  const int bq = bwd_fused_query_rows(D), all = (N + bq - 1) / bq;
-  const int tiles = (sinks + 127) / 128;
+// The cut of the sink tiles (key tiles of `tile` rows, query blocks of bq), so that a unit costs about what a
+// tile with one window of queries does: such a tile sees ceil((window + tile - 1) / bq) + 1 query blocks at
+// most. At most 32 chunks bound the partials.
+inline WindowSplit window_split(int tile, int bq, int N, int window, int sinks) {
+  const int all = (N + bq - 1) / bq, tiles = (sinks + tile - 1) / tile;
   if (tiles == 0 || all == 0) return WindowSplit{0, 1, 0};
-  const int one = int((int64_t(window) + 127 + bq - 1) / bq + 1), least = (all + 31) / 32;
+  const int one = int((int64_t(window) + tile - 1 + bq - 1) / bq + 1), least = (all + 31) / 32;
   const int blocks = one > least ? one : least;
   return WindowSplit{tiles, (all + blocks - 1) / blocks, blocks};
 }
-// Workspace of the fused window backward: the fp32 dQ rows and the barrier counter as above, then, if the
-// sink tiles are cut, fp32 [Z * Hk, tiles, chunks, 2 (dV, dK), 128, D] partials.
-inline int64_t window_bwd_workspace_bytes(int Z, int H, int Hk, int N, int D, const WindowSplit& w) {
-  const int64_t part = w.chunks > 1 ? int64_t(Z) * Hk * w.tiles * w.chunks * 2 * 128 * D * 4 : 0;
-  return bwd_fused_workspace_bytes(Z, H, N, D) + part;
+constexpr int kWindowF32Tile = 64;  // rows of a tile of the fp32 window kernels
+// The partials that a cut writes: fp32 [Z * Hk, tiles, chunks, 2 (dV, dK), tile, D].
+inline int64_t window_part_bytes(int tile, int Z, int Hk, int D, const WindowSplit& w) {
+  return w.chunks > 1 ? int64_t(Z) * Hk * w.tiles * w.chunks * 2 * tile * D * 4 : 0;
 }
 
 // SIMT kernels (fp32 inputs; any strides).
@@ -136,7 +135,7 @@ cudaError_t launch_bwd_dq_f32(int D, bool causal, const BwdArgs& a, cudaStream_t
 cudaError_t launch_bwd_dkdv_f32(int D, bool causal, const BwdArgs& a, cudaStream_t s);
 
 // Sliding window with sinks in fp32 (window_f32.cu; any strides). The backward writes dk, dv and dq from
-// a.delta; a.qk_scale and a.sm_scale are signed.
+// a.delta, cutting its sink tiles as a.split says; a.qk_scale and a.sm_scale are signed.
 cudaError_t launch_window_fwd_f32(int D, const void* q, const void* k, const void* v, Strides4 sq, Strides4 sk,
                                   Strides4 sv, const FwdArgs& a, cudaStream_t s);
 cudaError_t launch_window_bwd_f32(int D, const BwdArgs& a, cudaStream_t s);

@@ -17,7 +17,7 @@
 namespace tattn {
 namespace {
 
-constexpr int kThreads = 256, TB = 64;  // threads; rows and columns of a tile
+constexpr int kThreads = 256, TB = kWindowF32Tile;  // threads; rows and columns of a tile
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Row pitch in floats: 16-byte units a row odd in number, so that 16 rows at one unit are in different banks.
@@ -25,10 +25,21 @@ template <int D>
 constexpr int kPitch = D + 4;
 constexpr int kPitchP = TB + 4;
 
-// Rows [r0, r0 + 64) of a [n, D] matrix into shared memory; rows past n are zeros.
+// Rows [r0, r0 + 64) of a [n, D] matrix into shared memory, 16 bytes at a time where its rows allow; rows past
+// n are zeros.
 template <int D>
 __device__ __forceinline__ void load_rows(float* dst, const float* src, const Strides4& s, int r0, int n) {
-#pragma unroll 8
+  if (s.d == 1 && s.n % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
+#pragma unroll
+    for (int i = 0; i < TB * D / 4 / kThreads; ++i) {
+      const int e = i * kThreads + threadIdx.x, r = e / (D / 4), d = e % (D / 4) * 4;
+      const float4 x = r0 + r < n ? __ldg(reinterpret_cast<const float4*>(src + int64_t(r0 + r) * s.n + d))
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+      *reinterpret_cast<float4*>(dst + r * kPitch<D> + d) = x;
+    }
+    return;
+  }
+#pragma unroll 4
   for (int e = threadIdx.x; e < TB * D; e += kThreads) {
     const int r = e / D, d = e % D;
     dst[r * kPitch<D> + d] = r0 + r < n ? __ldg(src + int64_t(r0 + r) * s.n + d * s.d) : 0.f;
@@ -219,21 +230,28 @@ __global__ void __launch_bounds__(kThreads) window_dq_f32_kernel(BwdArgs a) {
   }
 }
 
-// One key tile of one key/value head, summed over the query heads that share it.
+// One key tile of one key/value head, summed over the query heads that share it; of a tile with sinks, which
+// all later queries see, one chunk of its query rows (WindowSplit) if those are cut, as a partial result.
 template <int D>
 __global__ void __launch_bounds__(kThreads) window_dkdv_f32_kernel(BwdArgs a) {
   extern __shared__ __align__(16) float smem[];
   float *Ks = smem, *Vs = Ks + TB * kPitch<D>, *Qs = Vs + TB * kPitch<D>, *Os = Qs + TB * kPitch<D>;
   float *Ps = Os + TB * kPitch<D>, *DSs = Ps + TB * kPitchP, *Ms = DSs + TB * kPitchP, *Ds = Ms + TB;
-  const int N = a.N, Nk = a.win.Nk, k0 = blockIdx.x * TB;
+  const int cut = a.split.tiles * a.split.chunks, unit = blockIdx.x;
+  const bool sink = unit < cut;
+  const int N = a.N, Nk = a.win.Nk, k0 = TB * (sink ? unit / a.split.chunks : unit - cut + a.split.tiles);
   const int zi = blockIdx.y / a.win.Hk, hk = blockIdx.y % a.win.Hk;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   load_rows<D>(Ks, static_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h, a.sk, k0, Nk);
   load_rows<D>(Vs, static_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h, a.sv, k0, Nk);
   float dk[4][D / 16] = {}, dv[4][D / 16] = {};
   // Rows from the first key's position on; without a sink in the tile, up to one window past its last key.
-  const int first = max(0, k0 - a.win.off);
-  const int end = k0 < a.win.sinks ? N : int(min(int64_t(N), int64_t(k0) + TB - 1 + a.win.window - a.win.off));
+  int first = max(0, k0 - a.win.off);
+  int end = sink ? N : int(min(int64_t(N), int64_t(k0) + TB - 1 + a.win.window - a.win.off));
+  if (sink && a.split.chunks > 1) {
+    first += unit % a.split.chunks * a.split.blocks * TB;
+    end = min(N, first + a.split.blocks * TB);
+  }
   for (int g = 0; g < a.win.group; ++g) {
     const int hi = hk * a.win.group + g;
     const float* q = static_cast<const float*>(a.q) + zi * a.sq.z + hi * a.sq.h;
@@ -267,6 +285,16 @@ __global__ void __launch_bounds__(kThreads) window_dkdv_f32_kernel(BwdArgs a) {
   for (int i = 0; i < 4; ++i) {
     const int key = k0 + 4 * ty + i;
     if (key >= Nk) continue;
+    if (sink && a.split.chunks > 1) {
+      const int64_t slot = int64_t(blockIdx.y) * cut + unit;
+      float* part = a.part + (slot * 2 * TB + 4 * ty + i) * D + D / 16 * tx;
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) {
+        part[e] = dv[i][e];
+        part[TB * D + e] = dk[i][e];
+      }
+      continue;
+    }
     const int64_t at = (int64_t(blockIdx.y) * Nk + key) * D + D / 16 * tx;
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) {
@@ -276,29 +304,49 @@ __global__ void __launch_bounds__(kThreads) window_dkdv_f32_kernel(BwdArgs a) {
   }
 }
 
+// dV and dK of the cut sink tiles: the sums of the chunks' partials, in their order.
+__global__ void __launch_bounds__(kThreads) window_join_f32_kernel(BwdArgs a, int D) {
+  const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x, tile = TB * D;
+  const int which = int(i / tile % 2);  // 0: dV, 1: dK
+  const int64_t t = i / (2 * tile);     // sink tiles of all heads
+  const int key = int(t % a.split.tiles) * TB + int(i % tile / D);
+  if (t >= int64_t(a.Z) * a.win.Hk * a.split.tiles || key >= a.win.Nk) return;
+  const float* p = a.part + t * a.split.chunks * 2 * tile + which * tile + i % tile;
+  float sum = 0.f;
+  for (int c = 0; c < a.split.chunks; ++c) sum += p[c * 2 * tile];
+  float* out = static_cast<float*>(which ? a.dk : a.dv);
+  out[(t / a.split.tiles * a.win.Nk + key) * D + i % D] = which ? sum * a.sm_scale : sum;
+}
+
 template <typename Kernel, typename... Args>
-cudaError_t launch(Kernel kernel, int rows, long long heads, int floats, cudaStream_t s, const Args&... args) {
+cudaError_t launch(Kernel kernel, int tiles, long long heads, int floats, cudaStream_t s, const Args&... args) {
   if (heads > 65535) return cudaErrorInvalidConfiguration;
   const int smem = floats * 4;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kernel<<<dim3((rows + TB - 1) / TB, unsigned(heads)), kThreads, smem, s>>>(args...);
+  kernel<<<dim3(tiles, unsigned(heads)), kThreads, smem, s>>>(args...);
   return cudaGetLastError();
 }
 
 template <int D>
 cudaError_t fwd_impl(const float* q, const float* k, const float* v, const Strides4& sq, const Strides4& sk,
                      const Strides4& sv, const FwdArgs& a, cudaStream_t s) {
-  return launch(window_fwd_f32_kernel<D>, a.N, (long long)a.Z * a.H, TB * (3 * kPitch<D> + kPitchP), s, q, k, v, sq, sk,
+  return launch(window_fwd_f32_kernel<D>, (a.N + TB - 1) / TB, (long long)a.Z * a.H, TB * (3 * kPitch<D> + kPitchP), s, q, k, v, sq, sk,
                 sv, a);
 }
 
 template <int D>
 cudaError_t bwd_impl(const BwdArgs& a, cudaStream_t s) {
-  const cudaError_t e = launch(window_dkdv_f32_kernel<D>, a.win.Nk, (long long)a.Z * a.win.Hk,
-                               TB * (4 * kPitch<D> + 2 * kPitchP + 2), s, a);
+  const int units = (a.win.Nk + TB - 1) / TB + a.split.tiles * (a.split.chunks - 1);
+  cudaError_t e = launch(window_dkdv_f32_kernel<D>, units, (long long)a.Z * a.win.Hk,
+                         TB * (4 * kPitch<D> + 2 * kPitchP + 2), s, a);
   if (e != cudaSuccess) return e;
-  return launch(window_dq_f32_kernel<D>, a.N, (long long)a.Z * a.H, TB * (4 * kPitch<D> + kPitchP + 2), s, a);
+  if (a.split.chunks > 1) {
+    const int64_t values = int64_t(a.Z) * a.win.Hk * a.split.tiles * 2 * TB * D;
+    window_join_f32_kernel<<<unsigned((values + kThreads - 1) / kThreads), kThreads, 0, s>>>(a, D);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  }
+  return launch(window_dq_f32_kernel<D>, (a.N + TB - 1) / TB, (long long)a.Z * a.H, TB * (4 * kPitch<D> + kPitchP + 2), s, a);
 }
 
 }  // namespace
