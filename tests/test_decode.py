@@ -292,7 +292,8 @@ def _quantized(x):
     """Codes, scales and minima of fp16 rows by the format's definition."""
     g = x.double().unflatten(-1, (-1, 64))
     low, high = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
-    s = ((high - low).float() / 15).half().double()
+    span = (high - low).float()
+    s = (span / torch.full_like(span, 15)).half().double()  # (a division; by a number torch multiplies with 1 / 15)
     n = torch.where(s > 0, ((g - low).float() / s.float()).double().round(), 0.0).clamp(0, 15)
     return n.flatten(-2).to(torch.uint8), torch.stack((s.squeeze(-1), low.squeeze(-1)), -1).half()
 
@@ -331,6 +332,24 @@ def test_append_and_read(gpu, t, layout, d) -> None:
             assert torch.equal(y[z], want[z, :, at : at + t])
     whole = cache.read(50)
     assert torch.equal(whole[0][1, :, 7 : 7 + t], values[0][1])
+
+
+@pytest.mark.gpu
+def test_codes_are_the_rounded_quotients(gpu) -> None:
+    """Quotients at and next to the midpoints between codes, at many scales: as torch divides and rounds."""
+    g = torch.Generator().manual_seed(22)
+    rows = 20000
+    s = (2.0 ** (torch.rand(rows, 1, generator=g) * 24 - 14)).half().double()
+    half = torch.randint(0, 31, (rows, 128), generator=g).double() / 2
+    x = (s * half + (torch.rand(rows, 1, generator=g) - 0.5).half().double() * s).half()
+    x[:, 0::64], x[:, 1::64] = (x.amin(-1, keepdim=True), (x.amin(-1, keepdim=True).double() + 15 * s).half())
+    step = torch.randint(-1, 2, x.shape, generator=g, dtype=torch.int16)
+    x = torch.where(torch.isfinite(x) & (x.view(torch.int16).abs() > 2), (x.view(torch.int16) + step).view(torch.float16), x)
+    x = x.cuda().reshape(1, 1, rows, 128)
+    cache = Int4Cache.empty(1, 1, rows, 128)
+    cache.append(x, x)
+    n, p = _quantized(x)
+    assert torch.equal(cache.k_params, p) and torch.equal(_codes(cache)[0], n) and torch.equal(_codes(cache)[1], n)
 
 
 @pytest.mark.gpu

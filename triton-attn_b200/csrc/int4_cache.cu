@@ -5,7 +5,9 @@
 // fp16. Every step but the roundings named is in fp32.
 //
 // The bound is HBM: 2 D bytes in and D / 2 + D / 16 out a row, or the reverse. 8 lanes take a group, each the 16
-// bytes of 8 dims, which are 4 bytes of codes.
+// bytes of 8 dims, which are 4 bytes of codes. A CTA works on one head of one sequence of K or V, and a thread
+// on the same dims of up to kRows rows, all of whose loads it issues first; so the divisions that find the
+// head are done once, for the whole CTA.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -14,136 +16,152 @@
 namespace tattn {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kRows = 4;
 
-// This thread's 8 dims: dims [8 i, 8 i + 8) of row t of head hk of sequence z, and the cache's row for them (or
-// -1: none, the position lies outside the cache). kv: 0 keys, 1 values.
+// This thread's work: dims [8 i, 8 i + 8) of rows t, t + step, ... (kRows of them, below T) of head hk of
+// sequence z. kv: 0 keys, 1 values.
 struct Place {
-  int kv, z, hk, t, i;
-  int64_t row;
+  int kv, z, hk, t, step, i;
+  int64_t head, start;  // the cache's head; the position of row 0
 };
 template <int D>
-__device__ __forceinline__ bool place(const Int4CacheArgs& a, Place* p) {
+__device__ __forceinline__ Place place(const Int4CacheArgs& a) {
   constexpr int L = D / 8;
-  const int64_t id = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-  int64_t r = id / L;
-  p->i = int(id % L);
-  p->t = int(r % a.T);
-  r /= a.T;
-  p->hk = int(r % a.Hk);
-  r /= a.Hk;
-  p->z = int(r % a.Z);
-  p->kv = int(r / a.Z);
-  if (p->kv > 1) return false;
-  const int64_t pos = int64_t(a.start ? a.start[p->z] : 0) + p->t;
-  p->row = pos >= 0 && pos < a.C ? (int64_t(p->z) * a.Hk + p->hk) * a.C + pos : -1;
-  return true;
+  const int rows = int(blockDim.x) / L, chunks = (a.T + kRows * rows - 1) / (kRows * rows);
+  Place p;
+  int head = int(blockIdx.x) / chunks;
+  p.step = rows;
+  p.t = int(blockIdx.x) % chunks * kRows * rows + int(threadIdx.x) / L;
+  p.i = int(threadIdx.x) % L;
+  p.hk = head % a.Hk;
+  head /= a.Hk;
+  p.z = head % a.Z;
+  p.kv = head / a.Z;
+  p.head = int64_t(p.z) * a.Hk + p.hk;
+  p.start = a.start ? a.start[p.z] : 0;
+  return p;
+}
+// The cache's row for row t, or -1: its position lies outside the cache.
+__device__ __forceinline__ int64_t cache_row(const Int4CacheArgs& a, const Place& p, int t) {
+  const int64_t pos = p.start + t;
+  return pos >= 0 && pos < a.C ? p.head * a.C + pos : -1;
 }
 
 template <int D>
 __global__ void __launch_bounds__(kThreads) int4_append_kernel(const Int4CacheArgs a) {
-  Place p;
-  bool any = place<D>(a, &p);
-  if (any && a.counts && p.t >= a.counts[p.z]) any = false;
-  if (any && p.row < 0) {
-    if (p.i == 0) atomicOr(a.status, kStatusIndexRange);
-    any = false;
+  const Place p = place<D>(a);
+  const int T = a.counts ? min(a.T, a.counts[p.z]) : a.T;
+  const Strides3 st = p.kv ? a.sv : a.sk;
+  const __half* src = static_cast<const __half*>(p.kv ? a.v : a.k) + p.z * st.z + p.hk * st.h + 8 * p.i;
+  uint8_t* codes = p.kv ? a.v_codes : a.k_codes;
+  __half2* params = static_cast<__half2*>(p.kv ? a.v_params : a.k_params);
+  uint4 u[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int t = p.t + r * p.step;
+    u[r] = t < T ? *reinterpret_cast<const uint4*>(src + t * st.n) : make_uint4(0u, 0u, 0u, 0u);
   }
-  float x[8];
-  if (any) {
-    const Strides3 s = p.kv ? a.sv : a.sk;
-    const __half* src = static_cast<const __half*>(p.kv ? a.v : a.k) + p.z * s.z + p.hk * s.h + p.t * s.n + 8 * p.i;
-    const uint4 u = *reinterpret_cast<const uint4*>(src);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int t = p.t + r * p.step;
+    const uint32_t w[4] = {u[r].x, u[r].y, u[r].z, u[r].w};
+    float x[8];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
       x[2 * e] = f.x;
       x[2 * e + 1] = f.y;
     }
-  } else {
+    float lo = x[0], hi = x[0];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 0.f;
-  }
-  float lo = x[0], hi = x[0];
+    for (int e = 1; e < 8; ++e) {
+      lo = fminf(lo, x[e]);
+      hi = fmaxf(hi, x[e]);
+    }
 #pragma unroll
-  for (int e = 1; e < 8; ++e) {
-    lo = fminf(lo, x[e]);
-    hi = fmaxf(hi, x[e]);
-  }
+    for (int o = 1; o < 8; o *= 2) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    if (t >= T) continue;
+    const int64_t row = cache_row(a, p, t);
+    if (row < 0) {
+      if (p.i == 0) atomicOr(a.status, kStatusIndexRange);
+      continue;
+    }
+    const __half scale = __float2half_rn((hi - lo) / 15.f);
+    const float s = __half2float(scale);
+    // The quotient (x - lo) / s, correctly rounded, by Markstein's theorem: with inv the correctly rounded 1 /
+    // s and q0 = d inv, the remainder d - q0 s is exact in one FMA and q0 + remainder * inv rounds to the quotient.
+    // (Eight divisions took two thirds of the kernel's time.) Adding 1.5 2^23 rounds it to the nearest integer,
+    // ties to even, in the low bits.
+    const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+    uint32_t code = 0;
 #pragma unroll
-  for (int o = 1; o < 8; o *= 2) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    for (int e = 0; e < 8; ++e) {
+      const float d = x[e] - lo, q0 = d * inv;
+      const float q = fminf(fmaf(fmaf(-q0, s, d), inv, q0), 15.f);
+      code |= (__float_as_uint(q + 12582912.f) & 15u) << (4 * e);
+    }
+    *reinterpret_cast<uint32_t*>(codes + row * (D / 2) + 4 * p.i) = code;
+    if (p.i % 8 == 0) params[row * (D / 64) + p.i / 8] = __halves2half2(scale, __float2half_rn(lo));
   }
-  if (!any) return;
-  const __half scale = __float2half_rn((hi - lo) / 15.f);
-  const float s = __half2float(scale);
-  uint32_t code = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float n = s > 0.f ? fminf(fmaxf(rintf((x[e] - lo) / s), 0.f), 15.f) : 0.f;
-    code |= uint32_t(n) << (4 * e);
-  }
-  *reinterpret_cast<uint32_t*>((p.kv ? a.v_codes : a.k_codes) + p.row * (D / 2) + 4 * p.i) = code;
-  if (p.i % 8 == 0)
-    static_cast<__half2*>(p.kv ? a.v_params : a.k_params)[p.row * (D / 64) + p.i / 8] =
-        __halves2half2(scale, __float2half_rn(lo));
 }
 
 template <int D>
 __global__ void __launch_bounds__(kThreads) int4_read_kernel(const Int4CacheArgs a) {
-  Place p;
-  if (!place<D>(a, &p)) return;
-  uint32_t w[4] = {0u, 0u, 0u, 0u};  // a position outside the cache reads as zeros
-  if (p.row >= 0) {
-    const uint32_t code = *reinterpret_cast<const uint32_t*>((p.kv ? a.v_codes : a.k_codes) + p.row * (D / 2) + 4 * p.i);
-    const __half2 sm = static_cast<const __half2*>(p.kv ? a.v_params : a.k_params)[p.row * (D / 64) + p.i / 8];
-    const __half2 s = __low2half2(sm), m = __high2half2(sm);
+  const Place p = place<D>(a);
+  const uint8_t* codes = p.kv ? a.v_codes : a.k_codes;
+  const __half2* params = static_cast<const __half2*>(p.kv ? a.v_params : a.k_params);
+  __half* out = static_cast<__half*>(p.kv ? a.v_out : a.k_out) + p.head * a.T * D + 8 * p.i;
+  uint32_t code[kRows];
+  __half2 sm[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {  // a position outside the cache reads as zeros
+    const int t = p.t + r * p.step;
+    const int64_t row = t < a.T ? cache_row(a, p, t) : 0;
+    const bool in = t < a.T && row >= 0;
+    code[r] = in ? *reinterpret_cast<const uint32_t*>(codes + row * (D / 2) + 4 * p.i) : 0u;
+    sm[r] = in ? params[row * (D / 64) + p.i / 8] : __float2half2_rn(0.f);
+    if (row < 0 && p.i == 0) atomicOr(a.status, kStatusIndexRange);
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int t = p.t + r * p.step;
+    if (t >= a.T) break;
+    const __half2 s = __low2half2(sm[r]), m = __high2half2(sm[r]);
+    uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const __half2 n = __floats2half2_rn(float((code >> (8 * e)) & 15u), float((code >> (8 * e + 4)) & 15u));
+      const __half2 n = __floats2half2_rn(float((code[r] >> (8 * e)) & 15u), float((code[r] >> (8 * e + 4)) & 15u));
       const __half2 v = __hfma2(s, n, m);  // one rounding
       w[e] = *reinterpret_cast<const uint32_t*>(&v);
     }
-  } else if (p.i == 0) {
-    atomicOr(a.status, kStatusIndexRange);
+    *reinterpret_cast<uint4*>(out + int64_t(t) * D) = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  const int64_t row = (int64_t(p.z) * a.Hk + p.hk) * a.T + p.t;
-  *reinterpret_cast<uint4*>(static_cast<__half*>(p.kv ? a.v_out : a.k_out) + row * D + 8 * p.i) =
-      make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// One thread for each 8 dims of K and V.
-cudaError_t grid_for(int D, const Int4CacheArgs& a, unsigned* grid) {
-  const double blocks = 2.0 * a.Z * a.Hk * a.T * (D / 8) / kThreads + 1.0;
-  if (blocks > 2147483647.0) return cudaErrorInvalidConfiguration;
-  *grid = unsigned((2 * int64_t(a.Z) * a.Hk * a.T * (D / 8) + kThreads - 1) / kThreads);
-  return cudaSuccess;
+template <typename Kernel>
+cudaError_t launch(Kernel kernel, int D, const Int4CacheArgs& a, cudaStream_t s) {
+  // Fewer threads where all the rows of a head need fewer (whole warps).
+  const int64_t need = (int64_t(a.T) * (D / 8) + 31) / 32 * 32;
+  const int threads = need < kThreads ? int(need) : kThreads, rows = threads / (D / 8);
+  const int64_t chunks = (a.T + int64_t(kRows) * rows - 1) / (kRows * rows);
+  if (double(chunks) * 2.0 * a.Z * a.Hk > 2147483647.0) return cudaErrorInvalidConfiguration;
+  const int64_t grid = chunks * 2 * a.Z * a.Hk;
+  if (grid == 0) return cudaSuccess;
+  kernel<<<unsigned(grid), threads, 0, s>>>(a);
+  return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t launch_int4_append(int D, const Int4CacheArgs& a, cudaStream_t s) {
-  unsigned grid;
-  const cudaError_t e = grid_for(D, a, &grid);
-  if (e != cudaSuccess || grid == 0) return e;
-  if (D == 64)
-    int4_append_kernel<64><<<grid, kThreads, 0, s>>>(a);
-  else
-    int4_append_kernel<128><<<grid, kThreads, 0, s>>>(a);
-  return cudaGetLastError();
+  return D == 64 ? launch(int4_append_kernel<64>, D, a, s) : launch(int4_append_kernel<128>, D, a, s);
 }
 
 cudaError_t launch_int4_read(int D, const Int4CacheArgs& a, cudaStream_t s) {
-  unsigned grid;
-  const cudaError_t e = grid_for(D, a, &grid);
-  if (e != cudaSuccess || grid == 0) return e;
-  if (D == 64)
-    int4_read_kernel<64><<<grid, kThreads, 0, s>>>(a);
-  else
-    int4_read_kernel<128><<<grid, kThreads, 0, s>>>(a);
-  return cudaGetLastError();
+  return D == 64 ? launch(int4_read_kernel<64>, D, a, s) : launch(int4_read_kernel<128>, D, a, s);
 }
 
 }  // namespace tattn
