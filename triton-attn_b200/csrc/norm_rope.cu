@@ -12,7 +12,8 @@
 // L = D / (2 VEC) lanes owns a token's row: lane c holds the 16 bytes at c and the 16 bytes half a row
 // further, so a half-split pair lies in one lane, and so does an interleaved one. A work item is one token
 // and HB consecutive heads of one tensor, which share the token's cos and sin and the weight in
-// registers; HB = 4 where there are enough items to fill the GPU with, else 1 (a decoding step's few rows).
+// registers; HB = 4 (backward, with two tensors to hold: 2) where there are enough items to fill the GPU with,
+// else 1 (a decoding step's few rows).
 // dw: every CTA works on one tensor, adds its rows' terms in registers and then shared memory and writes one
 // partial; a second small kernel sums the partials in a fixed order, so dw is bitwise reproducible.
 #include <cuda_fp16.h>
@@ -30,8 +31,7 @@ constexpr int kVec = 16 / int(sizeof(T));
 
 // 16 bytes of T as floats, and back (rounded to nearest).
 template <typename T>
-__device__ __forceinline__ void load16(const T* p, float* x) {
-  const uint4 v = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void unpack16(const uint4& v, float* x) {
   if constexpr (sizeof(T) == 2) {
     const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -46,6 +46,14 @@ __device__ __forceinline__ void load16(const T* p, float* x) {
     x[2] = __uint_as_float(v.z);
     x[3] = __uint_as_float(v.w);
   }
+}
+template <typename T>
+__device__ __forceinline__ uint4 load_raw(const T* p) {
+  return *reinterpret_cast<const uint4*>(p);
+}
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, float* x) {
+  unpack16<T>(load_raw(p), x);
 }
 template <typename T>
 __device__ __forceinline__ void store16(T* p, const float* x) {
@@ -115,7 +123,7 @@ __device__ __forceinline__ Item rope_item(const RopeArgs& a, const RopeTensor& t
 }
 
 template <typename T, int D, bool INTERLEAVED, int HB, bool BACKWARD>
-__global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RopeArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) norm_rope_kernel(const RopeArgs a) {
   constexpr int VEC = kVec<T>, L = D / (2 * VEC), GROUPS = kThreads / L;
   using P = Pairs<VEC, INTERLEAVED>;
   const int which = int(blockIdx.x) < a.t[0].blocks ? 0 : 1;  // the CTA's tensor
@@ -159,57 +167,62 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RopeArgs a) {
       for (int j = 0; j < VEC; ++j) cs[j] = sn[j] = __int_as_float(0x7fffffff);
       if (c == 0) atomicOr(a.status, kStatusIndexRange);
     }
-    // All of the item's loads first: they are what takes time.
-    float x[HB][2 * VEC], dy[BACKWARD ? HB : 1][2 * VEC];
+    // All of the item's loads first, as they come: they are what takes time.
+    uint4 rx[HB][2], rdy[BACKWARD ? HB : 1][2];
 #pragma unroll
     for (int i = 0; i < HB; ++i) {
       const bool row = any && it.h0 + i < t.H;
       const int64_t h = row ? it.h0 + i : 0;
       const T* px = static_cast<const T*>(t.px) + it.z * t.x.z + h * t.x.h + it.n * t.x.n + col;
-      load16(px, x[i]);
-      load16(px + D / 2, x[i] + VEC);
+      rx[i][0] = load_raw(px);
+      rx[i][1] = load_raw(px + D / 2);
       if constexpr (BACKWARD) {
         const T* pd = static_cast<const T*>(t.pdy) + it.z * t.dy.z + h * t.dy.h + it.n * t.dy.n + col;
-        load16(pd, dy[i]);
-        load16(pd + D / 2, dy[i] + VEC);
+        rdy[i][0] = load_raw(pd);
+        rdy[i][1] = load_raw(pd + D / 2);
       }
     }
 #pragma unroll
     for (int i = 0; i < HB; ++i) {
       const bool row = any && it.h0 + i < t.H;
+      float x[2 * VEC];
+      unpack16<T>(rx[i][0], x);
+      unpack16<T>(rx[i][1], x + VEC);
       float sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 2 * VEC; ++e) sum = fmaf(x[i][e], x[i][e], sum);
+      for (int e = 0; e < 2 * VEC; ++e) sum = fmaf(x[e], x[e], sum);
       const float r = rsqrtf(group_sum<L>(sum) * (1.f / D) + a.eps);
       float out[2 * VEC];
       if constexpr (!BACKWARD) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const int f = P::first(j), s = P::second(j);
-          const float zf = x[i][f] * r * w[f], zs = x[i][s] * r * w[s];
+          const float zf = x[f] * r * w[f], zs = x[s] * r * w[s];
           out[f] = zf * cs[j] - zs * sn[j];
           out[s] = zs * cs[j] + zf * sn[j];
         }
       } else {
-        float dot = 0.f;
+        float dy[2 * VEC], dot = 0.f;
+        unpack16<T>(rdy[i][0], dy);
+        unpack16<T>(rdy[i][1], dy + VEC);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const int f = P::first(j), s = P::second(j);
-          const float gf = dy[i][f] * cs[j] + dy[i][s] * sn[j], gs = dy[i][s] * cs[j] - dy[i][f] * sn[j];
-          x[i][f] *= r;
-          x[i][s] *= r;
+          const float gf = dy[f] * cs[j] + dy[s] * sn[j], gs = dy[s] * cs[j] - dy[f] * sn[j];
+          x[f] *= r;
+          x[s] *= r;
           if (row) {
-            dw[f] = fmaf(gf, x[i][f], dw[f]);
-            dw[s] = fmaf(gs, x[i][s], dw[s]);
+            dw[f] = fmaf(gf, x[f], dw[f]);
+            dw[s] = fmaf(gs, x[s], dw[s]);
           }
           out[f] = gf * w[f];
           out[s] = gs * w[s];
-          dot = fmaf(out[f], x[i][f], dot);
-          dot = fmaf(out[s], x[i][s], dot);
+          dot = fmaf(out[f], x[f], dot);
+          dot = fmaf(out[s], x[s], dot);
         }
         const float mean = group_sum<L>(dot) * (1.f / D);
 #pragma unroll
-        for (int e = 0; e < 2 * VEC; ++e) out[e] = r * (out[e] - x[i][e] * mean);
+        for (int e = 0; e < 2 * VEC; ++e) out[e] = r * (out[e] - x[e] * mean);
       }
       if (row) {
         T* py = static_cast<T*>(t.py) + it.z * t.y.z + int64_t(it.h0 + i) * t.y.h + it.n * t.y.n + col;
@@ -233,19 +246,22 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RopeArgs a) {
   }
 }
 
-// dw of both tensors from the CTAs' partials: 16 columns a block, 16 threads a column.
+// dw of both tensors from the CTAs' partials: 8 columns (a 32-byte sector) a block, 32 threads a column.
+constexpr int kDwCols = 8;
 template <typename T>
 __global__ void __launch_bounds__(kThreads) norm_rope_dw_kernel(const RopeArgs a, int D) {
-  __shared__ float part[16][17];
-  const int which = blockIdx.y, col = blockIdx.x * 16 + threadIdx.x % 16, lane = threadIdx.x / 16;
+  __shared__ float part[32][kDwCols + 1];
+  const int which = blockIdx.y, c = threadIdx.x % kDwCols, col = blockIdx.x * kDwCols + c, lane = threadIdx.x / kDwCols;
   const int b0 = which ? a.t[0].blocks : 0, b1 = b0 + a.t[which].blocks;
   float s = 0.f;
-  for (int b = b0 + lane; b < b1; b += 16) s += a.part[int64_t(b) * D + col];
-  part[lane][threadIdx.x % 16] = s;
+#pragma unroll 8
+  for (int b = b0 + lane; b < b1; b += 32) s += a.part[int64_t(b) * D + col];
+  part[lane][c] = s;
   __syncthreads();
   if (lane == 0) {
     s = 0.f;
-    for (int i = 0; i < 16; ++i) s += part[i][threadIdx.x];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += part[i][c];
     if (a.w_f32)
       static_cast<float*>(a.t[which].dw)[col] = s;
     else if constexpr (sizeof(T) == 2)
@@ -259,10 +275,11 @@ template <typename T, int D, bool INTERLEAVED, bool BACKWARD>
 cudaError_t rope_impl(RopeArgs& a, cudaStream_t s) {
   constexpr int GROUPS = kThreads / (D / (2 * kVec<T>));
   const int sms = device_sm_count();
-  // 4 heads an item once that still gives every SM's 2048 threads something to do.
+  // Several heads an item once that still gives every SM's 2048 threads something to do.
+  constexpr int MANY = BACKWARD ? 2 : 4;
   const int64_t rows = int64_t(a.Z) * a.N * (a.t[0].H + a.t[1].H);
-  const bool many = rows * (D / (2 * kVec<T>)) >= int64_t(sms) * 2048 * 4;
-  const int HB = many ? 4 : 1;
+  const bool many = rows * (D / (2 * kVec<T>)) >= int64_t(sms) * 2048 * MANY;
+  const int HB = many ? MANY : 1;
   for (RopeTensor& t : a.t) t.items = a.Z * a.N * ((t.H + HB - 1) / HB);
   const int most = kRopeBlocksPerSm * sms;
   for (int i = 0; i < 2; ++i) {
@@ -275,11 +292,11 @@ cudaError_t rope_impl(RopeArgs& a, cudaStream_t s) {
   const int grid = a.t[0].blocks + a.t[1].blocks;
   if (grid > 0) {
     if (many)
-      norm_rope_kernel<T, D, INTERLEAVED, 4, BACKWARD><<<grid, kThreads, 0, s>>>(a);
+      norm_rope_kernel<T, D, INTERLEAVED, MANY, BACKWARD><<<grid, kThreads, 0, s>>>(a);
     else
       norm_rope_kernel<T, D, INTERLEAVED, 1, BACKWARD><<<grid, kThreads, 0, s>>>(a);
   }
-  if (BACKWARD) norm_rope_dw_kernel<T><<<dim3(D / 16, 2), kThreads, 0, s>>>(a, D);
+  if (BACKWARD) norm_rope_dw_kernel<T><<<dim3(D / kDwCols, 2), kThreads, 0, s>>>(a, D);
   return cudaGetLastError();
 }
 
