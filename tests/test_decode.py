@@ -10,7 +10,10 @@ import torch
 
 import tattn
 from tattn import Int4Cache, _lib, decode_attention, window_attention
+from tests.built import ensure_built
 from tests.plain64 import assert_within
+
+ensure_built()
 
 
 def _decode64(q, k, v, lengths, window, sinks, scale, c, u):

@@ -8,7 +8,10 @@ import torch
 
 import tattn
 from tattn import _lib, qk_norm_rope
+from tests.built import ensure_built
 from tests.plain64 import assert_within
+
+ensure_built()
 
 EPS = 1e-6
 

@@ -11,7 +11,10 @@ import torch
 import tattn
 from tattn import _lib, attention, window_attention
 from tattn.window import _backward, _forward
+from tests.built import ensure_built
 from tests.plain64 import assert_within, window_attention64
+
+ensure_built()
 
 
 def _qkv(b, h, hk, nq, nk, d, dtype, seed, layout="bhnd", device="cuda"):

@@ -2,7 +2,8 @@
 
 Every ``csrc/*.cu`` is compiled for sm_100a only (``-gencode arch=compute_100a,code=sm_100a``) with
 nvcc, then linked into one shared library with a static CUDA runtime. Only the ``tattn_*`` C entry
-points of ``include/tattn.h`` are exported. Objects go to ``triton-attn_b200/_build/``; a file is
+points of ``include/tattn.h`` are exported. ``csrc/torch_binding.cpp``, host code only, is compiled with g++ against
+the installed PyTorch into ``tattn/_torch_ext.so``, which finds the library beside it. Objects go to ``triton-attn_b200/_build/``; a file is
 rebuilt when it or any header is newer than its object. ``-Xptxas -v`` output (registers, spills,
 shared memory per kernel) is kept in ``_build/ptxas.log``.
 
@@ -17,6 +18,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -24,6 +26,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "tattn", "libtattn_b200.so")
+EXT_SRC = os.path.join(CSRC, "torch_binding.cpp")
+EXT = os.path.join(HERE, "tattn", "_torch_ext.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
           "--expt-relaxed-constexpr", "-Xptxas", "-v", "-I", os.path.join(ROOT, "include")]  # fmt: skip
@@ -94,6 +98,28 @@ def build(force: bool = False, jobs: int = 0, verbose: bool = False) -> str:
     return LIB
 
 
+def build_extension(force: bool = False) -> str:
+    """Compile and link tattn/_torch_ext.so (needs build()'s library); returns its path."""
+    import torch
+
+    if not force and not _stale(EXT, [EXT_SRC, os.path.join(ROOT, "include", "tattn.h"), torch.__file__]):
+        return EXT
+    at = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    include = [os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
+               os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]  # fmt: skip
+    libs = ["c10", "c10_cuda", "torch", "torch_cpu", "torch_python"]
+    cmd = [shutil.which("g++") or os.environ.get("CXX", "c++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+           "-DTORCH_EXTENSION_NAME=_torch_ext", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *[x for p in include for x in ("-isystem", p)], EXT_SRC, "-o", EXT, "-L", os.path.join(at, "lib"),
+           *[f"-l{x}" for x in libs], "-L", os.path.dirname(LIB), f"-l:{os.path.basename(LIB)}",
+           "-l:libstdc++.so.6", "-Wl,-rpath,$ORIGIN"]  # (exceptions need PyTorch's own C++ runtime) # fmt: skip
+    p = subprocess.run(cmd, capture_output=True, text=True)
+    if p.returncode != 0:
+        raise RuntimeError(f"g++ failed for {EXT_SRC}:\n{' '.join(cmd)}\n{p.stdout}\n{p.stderr}")
+    return EXT
+
+
 def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("--force", action="store_true")
@@ -102,6 +128,7 @@ def main() -> None:
     args = ap.parse_args()
     try:
         print(build(args.force, args.jobs, args.verbose))
+        print(build_extension(args.force))
     except RuntimeError as e:
         print(e, file=sys.stderr)
         sys.exit(1)

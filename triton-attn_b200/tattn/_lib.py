@@ -6,13 +6,11 @@ loaded the call raises, so a CPU or library substitute can never run silently in
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import importlib
 import os
-import struct
 import threading
-
-import torch
+from types import ModuleType
 
 LIB_NAME = "libtattn_b200.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
@@ -23,8 +21,7 @@ ERR_TOO_LARGE = 7
 BWD_NOALLOC_MAX_ROWS = 4194304  # TATTN_BWD_NOALLOC_MAX_ROWS
 DEV_WAIT_TIMEOUT, DEV_ABORTED, DEV_INDEX_RANGE = 1, 2, 4  # device status word bits (TATTN_DEV_*)
 
-# Every symbol include/tattn.h declares, with its ctypes signature. (An int64 array argument is _I64P where it
-# is built by strides_array, _P where it is built by strides_bytes.)
+# Every symbol include/tattn.h declares, with its ctypes signature.
 _P, _I, _F, _I64P = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.POINTER(ctypes.c_int64)
 _U64 = ctypes.c_uint64
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -35,17 +32,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tattn_bwd_noalloc": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64P, _I, _I, _I, _I, _I, _I, _F, _P]),
     "tattn_bwd_fused": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64P, _I, _I, _I, _I, _I, _I, _F, _P]),
     "tattn_bwd_fused_workspace_bytes": (ctypes.c_int64, [_I, _I, _I, _I]),
-    "tattn_window_fwd": (_I, [*[_P] * 6, *[_I] * 9, _F, _P]),
-    "tattn_window_bwd": (_I, [*[_P] * 12, *[_I] * 9, _F, _P]),
+    "tattn_window_fwd": (_I, [*[_P] * 5, _I64P, *[_I] * 9, _F, _P]),
+    "tattn_window_bwd": (_I, [*[_P] * 11, _I64P, *[_I] * 9, _F, _P]),
     "tattn_window_bwd_workspace_bytes": (ctypes.c_int64, [_I] * 9),
-    "tattn_qk_norm_rope": (_I, [*[_P] * 10, *[_I] * 8, _F, _I, _P]),
-    "tattn_qk_norm_rope_bwd": (_I, [*[_P] * 15, *[_I] * 8, _F, _I, _P]),
+    "tattn_qk_norm_rope": (_I, [*[_P] * 9, _I64P, *[_I] * 8, _F, _I, _P]),
+    "tattn_qk_norm_rope_bwd": (_I, [*[_P] * 14, _I64P, *[_I] * 8, _F, _I, _P]),
     "tattn_qk_norm_rope_bwd_workspace_bytes": (ctypes.c_int64, [_I]),
-    "tattn_decode": (_I, [*[_P] * 7, *[_I] * 8, _F, _P]),
+    "tattn_decode": (_I, [*[_P] * 6, _I64P, *[_I] * 8, _F, _P]),
     "tattn_decode_workspace_bytes": (ctypes.c_int64, [_I] * 8),
-    "tattn_int4_append": (_I, [*[_P] * 9, *[_I] * 5, _P]),
+    "tattn_int4_append": (_I, [*[_P] * 8, _I64P, *[_I] * 5, _P]),
     "tattn_int4_read": (_I, [*[_P] * 7, *[_I] * 5, _P]),
-    "tattn_int4_decode": (_I, [*[_P] * 9, *[_I] * 7, _F, _P]),
+    "tattn_int4_decode": (_I, [*[_P] * 8, _I64P, *[_I] * 7, _F, _P]),
     "tattn_int4_decode_workspace_bytes": (ctypes.c_int64, [_I] * 7),
     "tattn_layout_ok": (_I, [_P, _I64P, _I, _I, _I, _I]),
     "tattn_selftest_exp2": (_I, [_P, _P, _P, _P, _I, _P]),
@@ -65,6 +62,7 @@ ABI_VERSION = 4
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
+_ext: ModuleType | None = None
 
 
 class TattnError(RuntimeError):
@@ -97,6 +95,25 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         return lib
 
 
+def torch_ext() -> ModuleType:
+    """The compiled host side of the operators around attention (csrc/torch_binding.cpp), loaded once. Raises
+    RuntimeError if it or the library is missing."""
+    global _ext
+    if _ext is None:
+        load()
+        try:
+            ext = importlib.import_module("tattn._torch_ext")
+        except ImportError as e:
+            raise RuntimeError(
+                f"tattn._torch_ext cannot be loaded ({e}); build it with `python triton-attn_b200/build.py`. "
+                "There is no fallback."
+            ) from e
+        if ext.abi_version() != ABI_VERSION:
+            raise RuntimeError(f"{ext.__file__}: ABI version {ext.abi_version()} != {ABI_VERSION}")
+        _ext = ext
+    return _ext
+
+
 def status_string(code: int) -> str:
     return load().tattn_status_string(code).decode()
 
@@ -109,29 +126,6 @@ def check(fn: str, code: int) -> None:
 def strides_array(*stride_tuples: tuple[int, ...]) -> ctypes.Array:
     flat = [int(s) for st in stride_tuples for s in st]
     return (ctypes.c_int64 * len(flat))(*flat)
-
-
-_PACK = {n: struct.Struct(f"{n}q") for n in range(0, 40, 2)}
-
-
-def strides_bytes(flat: tuple[int, ...]) -> bytes:
-    """int64 strides for a _P argument. The single-token operators' calls take a few microseconds of device
-    time, so what a call costs on the host counts: this is a quarter of strides_array's cost."""
-    return _PACK[len(flat)].pack(*flat)
-
-
-_HERE = contextlib.nullcontext()
-
-
-def on_device(index: int) -> contextlib.AbstractContextManager[object]:
-    """``torch.cuda.device(index)``, or nothing where that is the current device."""
-    return _HERE if torch.cuda.current_device() == index else torch.cuda.device(index)
-
-
-# The current stream's handle on a device, without building a torch.cuda.Stream around it.
-raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda index: torch.cuda.current_stream(index).cuda_stream
-)
 
 
 def device_status(stream: int = 0, clear: bool = True) -> int:
