@@ -128,7 +128,7 @@ TATTN_API int tattn_window_bwd(const void* q, const void* k, const void* v, cons
                      int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window, int sinks, float sm_scale,
                      void* stream);
 
-/* Bytes of the workspace that tattn_window_bwd needs, or -1 for invalid arguments. */
+/* Bytes of the workspace that tattn_window_bwd needs on the current device, or -1 for invalid arguments. */
 TATTN_API int64_t tattn_window_bwd_workspace_bytes(int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window,
                                          int sinks);
 

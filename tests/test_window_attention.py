@@ -75,15 +75,20 @@ def test_abi_refuses_before_any_device_call() -> None:
 
 
 def test_workspace_size() -> None:
-    """The fp32 dQ rows and 16 bytes, and partial dV and dK of the sink tiles where they are cut."""
+    """The fp32 dQ rows and 16 bytes, and partial dV and dK of the key tiles that are several units' work: units of
+    what a tile without sinks costs or, where that is more, of 8 blocks (a CTA's share is small here)."""
     size = _lib.load().tattn_window_bwd_workspace_bytes
-    assert size(2, 4, 2, 1000, 1000, 64, 0, 100, 0) == 2 * 4 * 1000 * 64 * 4 + 16
-    # 1000 queries are 8 blocks of 128; a window of 100 spans at most ceil(227 / 128) + 1 = 3: 3 chunks.
-    assert size(2, 4, 2, 1000, 1000, 64, 0, 100, 4) == 2 * 4 * 1000 * 64 * 4 + 16 + 2 * 2 * 1 * 3 * 2 * 128 * 64 * 4
-    assert size(2, 4, 2, 1000, 1000, 64, 0, 1000, 4) == 2 * 4 * 1000 * 64 * 4 + 16  # one chunk: no partials
-    # fp32: tiles and blocks of 64, no dQ rows; ceil(163 / 64) + 1 = 4 of 16 blocks: 4 chunks.
+    dq = 2 * 4 * 1000 * 64 * 4 + 16
+    part = 2 * 2 * 2 * 128 * 64 * 4  # of one unit of each of the 2 * 2 key/value heads
+    # A window of 100 meets ceil(227 / 128) + 1 = 3 of the 8 query blocks, of 2 heads: one unit a tile.
+    assert size(2, 4, 2, 1000, 1000, 64, 0, 100, 0) == dq
+    # The sink tile meets all 8, of 2 heads: 3 units of 6.
+    assert size(2, 4, 2, 1000, 1000, 64, 0, 100, 4) == dq + 3 * part
+    # A window of everything: 2 units for each of the 8 tiles.
+    assert size(2, 4, 2, 1000, 1000, 64, 0, 1000, 4) == dq + 16 * part
+    # fp32: tiles and blocks of 64, no dQ rows; 4 and 16 blocks of 2 heads.
     assert size(2, 4, 2, 1000, 1000, 64, 1, 100, 0) == 0
-    assert size(2, 4, 2, 1000, 1000, 64, 1, 100, 4) == 2 * 2 * 1 * 4 * 2 * 64 * 64 * 4
+    assert size(2, 4, 2, 1000, 1000, 64, 1, 100, 4) == 2 * 2 * 4 * 2 * 64 * 64 * 4
 
 
 # -------------------------------------------------------------------------------------- on a B200

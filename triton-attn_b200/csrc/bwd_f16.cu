@@ -1743,10 +1743,10 @@ cudaError_t dkdv_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
 //     accumulated in TMEM by its own MMAs; the compute warps read it one block later, right after
 //     handing over the next block's P^T/dS^T (the dQ MMAs of that block wait for the read: dq_read),
 //     and add it into a dense fp32 workspace through TMA tensor reduce-adds (one 32 x 32 box per warp).
-//   * kMaskWindow: a unit is a key tile of one key/value head with the query blocks that see it, once for
-//     every query head that shares the head, so dK and dV are summed over those heads in TMEM. The tiles
-//     with sinks, which all later queries see, are cut into units of about a window's length (WindowSplit);
-//     each writes fp32 partial dV and dK, which the last phase sums in a fixed order.
+//   * kMaskWindow: a unit is a key tile of one key/value head with (a part of) the query blocks that see it, once
+//     for every query head that shares the head, so dK and dV are summed over those heads in TMEM. Tiles with
+//     sinks, which all later queries see, and tiles of a wide group are several units (WindowSplit), each of
+//     which writes fp32 partial dV and dK for the last phase to sum in a fixed order.
 //   * After its last tile every CTA (a cooperative launch of at most one CTA per SM) waits at a grid
 //     barrier for all reduce-adds, then its compute warps scale a share of the workspace by sm_scale
 //     into the fp16 dQ.
@@ -1920,31 +1920,54 @@ __device__ __forceinline__ void fused_dq_epilogue(const BwdArgs& a, int nthreads
   }
 }
 
-// Last phase of a window backward whose sink tiles were cut: dV and dK of those tiles, 8 elements a
-// thread, as the sum of the chunks' partials in their order (dK times sm_scale).
+// A unit's partial: for dV and dK each, boxes of one warp's 32 key rows x PW columns, [2 column halves][HW / PW]
+// [4 warps][32 rows][PW], the 16-byte units of a row in the order u ^ (row mod the units of a row): as a warp
+// stages a box without bank conflicts and copies it out in one piece.
 template <int D>
-__device__ __forceinline__ void fused_part_epilogue(const BwdArgs& a, int nthreads) {
+struct PartBox {
+  static constexpr int HW = D / 2, PW = HW < 32 ? HW : 32, UNITS = PW / 4, BYTES = 32 * PW * 4;
+  static __device__ __forceinline__ int64_t box(int which, int half, int pass, int warp) {
+    return (((which * 2 + half) * (HW / PW) + pass) * 4 + warp) * int64_t(32 * PW);
+  }
+  static __device__ __forceinline__ int unit(int row, int u) { return row * PW + ((u ^ (row & (UNITS - 1))) * 4); }
+};
+
+// Last phase of a window backward with tiles of several units: their dV and dK, 8 elements a thread, as the sum
+// of the units' partials in their order (dK times sm_scale). A CTA takes one tile's dV or dK at a time.
+template <int D>
+__device__ __forceinline__ void fused_part_epilogue(const BwdArgs& a) {
+  using B = PartBox<D>;
   unsigned t, cta;
   asm volatile("mov.u32 %0, %%tid.x;" : "=r"(t));
   asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(cta));
-  constexpr int kRow = D / 8, kTile = 128 * kRow;  // groups of 8 elements
-  const int64_t n8 = int64_t(a.Z) * a.win.Hk * a.split.tiles * 2 * kTile;
-  for (int64_t i = int64_t(cta) * nthreads + t; i < n8; i += int64_t(gridDim.x) * nthreads) {
-    const int e = int(i % kTile), which = int(i / kTile % 2);  // 0: dV, 1: dK
-    const int64_t tile = i / (2 * kTile);                      // head-major
-    const int key = int(tile % a.split.tiles) * 128 + e / kRow;
-    if (key >= a.win.Nk) continue;
-    const float4* p = reinterpret_cast<const float4*>(a.part) + 2 * ((tile * a.split.chunks * 2 + which) * kTile + e);
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-    for (int c = 0; c < a.split.chunks; ++c, p += 4 * kTile) {
-      const float4 u = __ldcg(p), v = __ldcg(p + 1);
-      x = make_float4(x.x + u.x, x.y + u.y, x.z + u.z, x.w + u.w);
-      y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
-    }
+  constexpr int kRow = D / 8;  // groups of 8 elements in a row
+  const int key_tiles = (a.win.Nk + 127) / 128, slots = a.split.slots(key_tiles);
+  const int tiles = a.split.units > 1 ? key_tiles : a.split.tiles;  // of a head, those that may have several
+  const int jobs = a.Z * a.win.Hk * tiles * 2;
+  for (int job = int(cta); job < jobs; job += int(gridDim.x)) {
+    const int which = job % 2, kt = job / 2 % tiles, bh = job / 2 / tiles;  // which: 0 dV, 1 dK
+    const bool sink = kt < a.split.tiles;
+    const int count = sink ? a.split.sink_units : a.split.units;
+    if (count == 1) continue;
+    const int first = sink ? kt * count : a.split.tiles * a.split.sink_units + (kt - a.split.tiles) * count;
+    const float* part = a.part + int64_t(bh * slots + first) * 2 * 128 * D;
+    uint4* out = static_cast<uint4*>(which ? a.dk : a.dv) + (int64_t(bh) * a.win.Nk + kt * 128) * kRow;
     const float sc = which ? a.sm_scale : 1.f;
-    uint4* out = static_cast<uint4*>(which ? a.dk : a.dv) + ((tile / a.split.tiles) * a.win.Nk + key) * kRow + e % kRow;
-    *out = make_uint4(pack_half2(x.x * sc, x.y * sc), pack_half2(x.z * sc, x.w * sc), pack_half2(y.x * sc, y.y * sc),
-                      pack_half2(y.z * sc, y.w * sc));
+    for (int e = int(t); e < 128 * kRow; e += 256) {
+      const int row = e / kRow, col = e % kRow * 8, colh = col % B::HW;
+      if (kt * 128 + row >= a.win.Nk) break;
+      const float* p = part + B::box(which, col / B::HW, colh / B::PW, row / 32);
+      const int u = colh % B::PW / 4, at0 = B::unit(row % 32, u), at1 = B::unit(row % 32, u + 1);
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+#pragma unroll 4
+      for (int c = 0; c < count; ++c, p += 2 * 128 * D) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(p + at0)), w = __ldcg(reinterpret_cast<const float4*>(p + at1));
+        x = make_float4(x.x + v.x, x.y + v.y, x.z + v.z, x.w + v.w);
+        y = make_float4(y.x + w.x, y.y + w.y, y.z + w.z, y.w + w.w);
+      }
+      out[e] = make_uint4(pack_half2(x.x * sc, x.y * sc), pack_half2(x.z * sc, x.w * sc),
+                          pack_half2(y.x * sc, y.y * sc), pack_half2(y.z * sc, y.w * sc));
+    }
   }
 }
 
@@ -1961,17 +1984,18 @@ __device__ __forceinline__ void hide_queries(uint32_t* s, int lo, int hi) {
   }
 }
 
-// One unit of a CTA's work in the fused backward: key tile kt of key/value head hk, and the query blocks
-// [lo, lo + nb) of each of the query heads h0, h0 + 1, ... : n blocks in all, head by head.
+// One unit of a CTA's work in the fused backward: key tile kt of key/value head hk and n (query head, query
+// block) pairs, from (h0, blk0) on: blocks [lo, lo + nb) of one head after another. Not kMaskWindow: one
+// head's blocks from lo on.
 struct Unit {
-  int zi, hk, h0, kt, lo, nb, n;
-  int chunk;  // kMaskWindow: of a cut sink tile, else -1
+  int zi, hk, kt, n;
+  int h0, blk0, lo, nb;
+  int slot;  // kMaskWindow: of its partial, else -1
 };
-// The (query head, query block) pairs of a unit in order. Not kMaskWindow: one head, blocks ascending.
 template <bool WINDOW>
 struct UnitWalk {
   int h, blk;
-  __device__ __forceinline__ explicit UnitWalk(const Unit& u) : h(u.h0), blk(u.lo) {}
+  __device__ __forceinline__ explicit UnitWalk(const Unit& u) : h(u.h0), blk(u.blk0) {}
   __device__ __forceinline__ void next(const Unit& u) {
     ++blk;
     if (WINDOW && blk == u.lo + u.nb) {
@@ -2032,7 +2056,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // unit first. Equal units balance the CTAs, and the tiles running at any time belong to a few
   // neighbouring heads, so their fp32 dQ workspace rows and Q/dO blocks are shared in L2 (ordering the
   // tiles longest-first across all heads instead spreads 148 CTAs over ~148 heads, whose workspaces miss
-  // L2: ~10x the algorithmic DRAM traffic at N = 8192 with 1,024 heads). kMaskWindow: window_unit below.
+  // L2: ~10x the algorithmic DRAM traffic at N = 8192 with 1,024 heads). kMaskWindow: next_window_unit.
   const int n_units = CAUSAL ? zh * ((nct + 1) / 2) : ntiles;
   auto next_tile = [&](int2& seq, int* bh, int* kt) -> bool {  // seq = (unit, second tile of the unit)
     if (seq.x >= n_units) return false;
@@ -2053,44 +2077,39 @@ __global__ void __launch_bounds__(kThreads, 1)
     return true;
   };
 
-  // kMaskWindow: of each key/value head, the chunks of the sink tiles, then the other tiles; these units
-  // cost about the same and are taken round-robin. A tile may have no query blocks (n = 0) where the
-  // queries begin after its window, and a chunk none where its tile's queries begin later.
-  auto window_unit = [&](int2& seq, Unit* u) -> bool {
-    const int cut = args.split.tiles * args.split.chunks, per_head = cut + nct - args.split.tiles;
+  // kMaskWindow: the units of each key/value head (window_unit), those of the sink tiles first; they cost about
+  // the same and are taken round-robin.
+  auto next_window_unit = [&](int2& seq, Unit* u) -> bool {
+    const int per_head = args.split.per_head(nct);
     if (seq.x >= zh * per_head) return false;
-    const int bh = seq.x / per_head, p = seq.x % per_head;
+    const int bh = seq.x / per_head;
+    const WindowUnit w = window_unit<128, BQ>(args.split, args.win, N, seq.x % per_head);
     seq.x += int(gridDim.x);
     u->zi = bh / args.win.Hk;
     u->hk = bh % args.win.Hk;
+    u->kt = w.kt;
+    u->n = w.n;
+    u->lo = w.lo;
+    u->nb = w.nb;
     u->h0 = u->hk * args.win.group;
-    const bool sink = p < cut;
-    u->kt = sink ? p / args.split.chunks : p - cut + args.split.tiles;
-    const int k0 = 128 * u->kt, first = max(0, k0 - args.win.off) / BQ;  // first block with a query at k0 or later
-    // The last query that sees key k0 + 127 is at position k0 + 127 + window - 1.
-    const int last = k0 + 126 + args.win.window - args.win.off;
-    int end = sink ? NBq : last < 0 ? 0 : min(NBq, last / BQ + 1);
-    u->lo = first;
-    u->chunk = -1;
-    if (sink && args.split.chunks > 1) {
-      u->chunk = p % args.split.chunks;
-      u->lo = first + u->chunk * args.split.blocks;
-      end = min(NBq, u->lo + args.split.blocks);
+    u->blk0 = w.lo;
+    if (w.start > 0 && w.nb > 0) {
+      u->h0 += w.start / w.nb;
+      u->blk0 += w.start % w.nb;
     }
-    u->nb = max(0, end - u->lo);
-    u->n = u->nb * args.win.group;
+    u->slot = w.slot < 0 ? -1 : bh * args.split.slots(nct) + w.slot;
     return true;
   };
   auto next_unit = [&](int2& seq, Unit* u) -> bool {
-    if (WINDOW) return window_unit(seq, u);
+    if (WINDOW) return next_window_unit(seq, u);
     int bh, kt;
     if (!next_tile(seq, &bh, &kt)) return false;
     u->zi = bh / args.H;
     u->hk = u->h0 = bh % args.H;
     u->kt = kt;
-    u->lo = tile_lo(kt);
+    u->lo = u->blk0 = tile_lo(kt);
     u->n = u->nb = NBq - u->lo;
-    u->chunk = -1;
+    u->slot = -1;
     return true;
   };
 
@@ -2427,11 +2446,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         if (any) fused_dqt_out(oq, stg, &tm_dqacc, 32 * q4, prev_blk * BQ + 32 * w, prev_h, zi, lane);
       }
-      float* part = nullptr;  // kMaskWindow: this thread's row of the chunk's partial
-      if (WINDOW && u.chunk >= 0) {
-        const int64_t slot = ((int64_t(zi) * args.win.Hk + u.hk) * args.split.tiles + u.kt) * args.split.chunks + u.chunk;
-        part = args.part + ((slot * 2 + w) * 128 + r) * D;
-      }
+      float* part = nullptr;  // kMaskWindow: the unit's partial
+      if (WINDOW && u.slot >= 0) part = args.part + int64_t(u.slot) * 2 * 128 * D;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {  // columns [half * HW, half * HW + HW)
         if constexpr (C::DQT) {
@@ -2448,11 +2464,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int c = 0; c < OR; ++c) o[c] = 0u;
         }
         if (WINDOW && part != nullptr) {
+          using B = PartBox<D>;
 #pragma unroll
-          for (int c = 0; c < C::HW; c += 4)
-            *reinterpret_cast<uint4*>(part + half * C::HW + c) =
-                make_uint4(o[(C::DQT ? 0 : half * C::HW) + c], o[(C::DQT ? 0 : half * C::HW) + c + 1],
-                           o[(C::DQT ? 0 : half * C::HW) + c + 2], o[(C::DQT ? 0 : half * C::HW) + c + 3]);
+          for (int pass = 0; pass < B::HW / B::PW; ++pass) {
+            if (lane == 0) tma_store_wait_read_all();
+            __syncwarp();
+#pragma unroll
+            for (int v = 0; v < B::UNITS; ++v) {
+              const int cc = (C::DQT ? 0 : half * C::HW) + pass * B::PW + 4 * v;
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stg + B::unit(lane, v) * 4), "r"(o[cc]),
+                           "r"(o[cc + 1]), "r"(o[cc + 2]), "r"(o[cc + 3]) : "memory");
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              bulk_store(part + B::box(w, half, pass, q4), stg, B::BYTES);
+              tma_store_commit();
+            }
+          }
           continue;
         }
         if (lane == 0) tma_store_wait_read_all();  // this warp's previous store has left the staging area
@@ -2485,7 +2514,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // warps of all CTAs (named barrier 1 over their 256 threads).
     if (grid_barrier(args.grid_sync, gridDim.x, ab, 1, 256, threadIdx.x == 0)) {
       fused_dq_epilogue<D>(args, 256);
-      if (WINDOW && args.part != nullptr) fused_part_epilogue<D>(args, 256);
+      if (WINDOW && args.part != nullptr) fused_part_epilogue<D>(args);
     }
   }
 
@@ -2510,7 +2539,7 @@ cudaError_t fused_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUten
   const long long tiles = nct * a.Z * (WINDOW ? a.win.Hk : a.H);
   if (tiles <= 0) return cudaSuccess;
   // The kernel's units (next_unit).
-  const long long units = WINDOW ? (nct + (long long)a.split.tiles * (a.split.chunks - 1)) * a.Z * a.win.Hk
+  const long long units = WINDOW ? (long long)a.split.per_head(int(nct)) * a.Z * a.win.Hk
                           : MASK == kMaskCausal ? (nct + 1) / 2 * a.Z * a.H
                                                 : tiles;
   if (tiles > 0x7fffffffLL || units > 0x7fffffffLL - 1024) return cudaErrorInvalidConfiguration;

@@ -398,8 +398,13 @@ extern "C" int tattn_bwd_fused(const void* q, const void* k, const void* v, cons
 namespace {
 
 bool valid_window(int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window, int sinks) {
-  return valid_dims(Z, H, Nq, D) && Hk >= 1 && H % Hk == 0 && Nk >= Nq && window >= 1 && sinks >= 0 &&
+  return valid_dims(Z, H, Nq, D) && Hk >= 1 && H % Hk == 0 && Nk >= Nq && Nk <= (1 << 29) && window >= 1 && sinks >= 0 &&
          (dtype == TATTN_F16 || dtype == TATTN_F32);
+}
+
+// The fp32 kernel has two CTAs an SM.
+WindowSplit window_f32_split(int Z, const WindowArgs& w, int Nq) {
+  return window_split(kWindowF32Tile, kWindowF32Tile, Z, w, Nq, 2 * device_sm_count());
 }
 
 // Windows and sinks longer than the keys say no more than the keys themselves.
@@ -495,8 +500,8 @@ extern "C" int tattn_window_bwd(const void* q, const void* k, const void* v, con
   a.wait_limit_ns = g_wait_limit_ns.load();
   a.win = window_args(H, Hk, Nq, Nk, window, sinks);
   if (dtype == TATTN_F32) {
-    a.split = window_split(kWindowF32Tile, kWindowF32Tile, Nq, a.win.window, a.win.sinks);
-    if (a.split.chunks > 1) {
+    a.split = window_f32_split(Z, a.win, Nq);
+    if (window_part_bytes(kWindowF32Tile, Z, a.win, D, a.split) > 0) {
       if (!workspace) return TATTN_ERR_INVALID_ARGUMENT;
       if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return TATTN_ERR_LAYOUT;
       a.part = static_cast<float*>(workspace);
@@ -513,8 +518,8 @@ extern "C" int tattn_window_bwd(const void* q, const void* k, const void* v, con
   a.dq_acc = static_cast<float*>(workspace);
   char* after = static_cast<char*>(workspace) + int64_t(Z) * H * Nq * D * 4;
   a.grid_sync = reinterpret_cast<unsigned*>(after);
-  a.split = window_split(128, bwd_fused_query_rows(D), Nq, a.win.window, a.win.sinks);
-  a.part = a.split.chunks > 1 ? reinterpret_cast<float*>(after + 16) : nullptr;
+  a.split = window_split(128, bwd_fused_query_rows(D), Z, a.win, Nq, device_sm_count());
+  a.part = window_part_bytes(128, Z, a.win, D, a.split) > 0 ? reinterpret_cast<float*>(after + 16) : nullptr;
   CUtensorMap tq, tk, tv, tdo, tdk, tdv, tdqacc;
   const int q_rows = bwd_fused_query_rows(D), acc_cols = D == 128 ? 32 : D / 2;  // as tattn_bwd_fused
   if ((rc = encode_f16(&tq, q, a.sq, Z, H, Nq, D, q_rows)) != TATTN_OK) return rc;
@@ -538,9 +543,9 @@ extern "C" int64_t tattn_window_bwd_workspace_bytes(int Z, int H, int Hk, int Nq
   if (Nq == 0) return 0;
   const WindowArgs w = window_args(H, Hk, Nq, Nk, window, sinks);
   if (dtype == TATTN_F32)
-    return window_part_bytes(kWindowF32Tile, Z, Hk, D, window_split(kWindowF32Tile, kWindowF32Tile, Nq, w.window, w.sinks));
+    return window_part_bytes(kWindowF32Tile, Z, w, D, window_f32_split(Z, w, Nq));
   return bwd_fused_workspace_bytes(Z, H, Nq, D) +
-         window_part_bytes(128, Z, Hk, D, window_split(128, bwd_fused_query_rows(D), Nq, w.window, w.sinks));
+         window_part_bytes(128, Z, w, D, window_split(128, bwd_fused_query_rows(D), Z, w, Nq, device_sm_count()));
 }
 
 extern "C" int64_t tattn_bwd_fused_workspace_bytes(int Z, int H, int N, int D) {

@@ -42,12 +42,46 @@ struct FwdArgs {
   WindowArgs win;    // kMaskWindow only
 };
 
-// Window backward: the `tiles` first key tiles hold sinks and are seen by every later query, the
-// others by one window of queries only. Each sink tile's query blocks are cut into `chunks` units of at
-// most `blocks` blocks (tiles = 0, or chunks = 1: no cut).
+// Window backward: its units of work. A key tile of a key/value head meets the query blocks that see it, once
+// for each query head of the group: a run of (head, block) pairs, head by head, which is cut into units of at
+// most `len` pairs. The `tiles` first key tiles hold sinks, which all later queries see: sink_units units each;
+// the others are seen by one window of queries: `units` each. A tile of several units is the sum of fp32
+// partials, added up in the units' order.
 struct WindowSplit {
-  int tiles, chunks, blocks;
+  int len;
+  int tiles, sink_units, units;
+  __host__ __device__ int per_head(int key_tiles) const { return tiles * sink_units + (key_tiles - tiles) * units; }
+  // Partials of a head: of every unit, of those of the sink tiles, or none.
+  __host__ __device__ int slots(int key_tiles) const {
+    return units > 1 ? per_head(key_tiles) : sink_units > 1 ? tiles * sink_units : 0;
+  }
 };
+
+// Unit p of a key/value head (key tiles of TILE rows, query blocks of BQ): pairs [start, start + n) of key tile
+// kt's run over the blocks [lo, lo + nb) of each head. n may be 0: the queries begin after the tile's window,
+// or the tile's run is shorter than others'.
+struct WindowUnit {
+  int kt, lo, nb, start, n;
+  int slot;  // its partial in the head, or -1: it is the whole tile
+};
+template <int TILE, int BQ>
+__host__ __device__ inline WindowUnit window_unit(const WindowSplit& s, const WindowArgs& w, int N, int p) {
+  const bool sink = p < s.tiles * s.sink_units;
+  const int rest = p - s.tiles * s.sink_units, count = sink ? s.sink_units : s.units;
+  const int piece = sink ? p % s.sink_units : rest % s.units;
+  WindowUnit u;
+  u.kt = sink ? p / s.sink_units : s.tiles + rest / s.units;
+  const int k0 = TILE * u.kt, blocks = (N + BQ - 1) / BQ;
+  const int last = k0 + TILE - 2 + w.window - w.off;  // the last query that sees the tile's last key
+  const int end = sink ? blocks : last < 0 ? 0 : (last / BQ + 1 < blocks ? last / BQ + 1 : blocks);
+  u.lo = (k0 > w.off ? k0 - w.off : 0) / BQ;
+  u.nb = end > u.lo ? end - u.lo : 0;
+  u.start = piece * s.len;
+  const int left = u.nb * w.group - u.start;
+  u.n = left < 0 ? 0 : left < s.len ? left : s.len;
+  u.slot = count > 1 ? p : -1;
+  return u;
+}
 
 struct BwdArgs {
   // inputs
@@ -67,7 +101,7 @@ struct BwdArgs {
   unsigned long long wait_limit_ns;  // bound of every mbarrier wait (tattn_set_wait_limit_ns)
   WindowArgs win;    // kMaskWindow only: dk and dv are then dense [Z, win.Hk, win.Nk, D]
   WindowSplit split; // kMaskWindow
-  float* part;       // kMaskWindow: partial dV and dK of the cut key tiles, or null
+  float* part;       // kMaskWindow: partial dV and dK of the tiles of several units, or null
 };
 
 // Host helpers of the C-ABI layer (capi.cu). device_ready: the current device is an sm_100 one whose primary
@@ -112,20 +146,28 @@ constexpr int kBwdStoreRows = 32;
 __host__ __device__ constexpr int bwd_fused_query_rows(int D) { return D == 128 ? 64 : 128; }
 // Workspace of tattn_bwd_fused: the fp32 dQ rows [Z, H, N, D], then 16 bytes for the grid-barrier counter.
 inline int64_t bwd_fused_workspace_bytes(int Z, int H, int N, int D) { return int64_t(Z) * H * N * D * 4 + 16; }
-// The cut of the sink tiles (key tiles of `tile` rows, query blocks of bq), so that a unit costs about what a
-// tile with one window of queries does: such a tile sees ceil((window + tile - 1) / bq) + 1 query blocks at
-// most. At most 32 chunks bound the partials.
-inline WindowSplit window_split(int tile, int bq, int N, int window, int sinks) {
-  const int all = (N + bq - 1) / bq, tiles = (sinks + tile - 1) / tile;
-  if (tiles == 0 || all == 0) return WindowSplit{0, 1, 0};
-  const int one = int((int64_t(window) + tile - 1 + bq - 1) / bq + 1), least = (all + 31) / 32;
-  const int blocks = one > least ? one : least;
-  return WindowSplit{tiles, (all + blocks - 1) / blocks, blocks};
+// Units of about one size for `workers` CTAs that take them in turn: what a tile without sinks costs (one
+// window's blocks for the group) or, where that leaves a CTA fewer than 4 units, a quarter of its share,
+// but 8 blocks at least, since a unit starts and ends at the cost of a few, and partials are memory traffic
+// (at most 64 a tile).
+inline WindowSplit window_split(int tile, int bq, int Z, const WindowArgs& w, int N, int workers) {
+  const int64_t blocks = (N + bq - 1) / bq, key_tiles = (w.Nk + tile - 1) / tile, tiles = (w.sinks + tile - 1) / tile;
+  const int64_t span = (int64_t(w.window) + tile - 1 + bq - 1) / bq + 1, one = span < blocks ? span : blocks;
+  const int64_t all = int64_t(Z) * w.Hk * w.group * (tiles * blocks + (key_tiles - tiles) * one);
+  const int64_t quarter = all / (4 * int64_t(workers)) + 1;
+  int64_t len = w.group * one < quarter ? w.group * one : quarter;
+  const int64_t least = (w.group * blocks + 63) / 64;
+  len = len < 8 ? 8 : len;
+  len = len < least ? least : len;
+  const int64_t cut = (w.group * one + len - 1) / len;  // equal parts of a tile without sinks
+  if (cut > 0) len = (w.group * one + cut - 1) / cut > least ? (w.group * one + cut - 1) / cut : least;
+  auto units = [&](int64_t pairs) { return int((pairs + len - 1) / len > 0 ? (pairs + len - 1) / len : 1); };
+  return WindowSplit{int(len), int(tiles), units(w.group * blocks), units(w.group * one)};
 }
 constexpr int kWindowF32Tile = 64;  // rows of a tile of the fp32 window kernels
-// The partials that a cut writes: fp32 [Z * Hk, tiles, chunks, 2 (dV, dK), tile, D].
-inline int64_t window_part_bytes(int tile, int Z, int Hk, int D, const WindowSplit& w) {
-  return w.chunks > 1 ? int64_t(Z) * Hk * w.tiles * w.chunks * 2 * tile * D * 4 : 0;
+// The partials: fp32 [Z * Hk, slots, 2 (dV, dK), tile, D].
+inline int64_t window_part_bytes(int tile, int Z, const WindowArgs& w, int D, const WindowSplit& s) {
+  return int64_t(Z) * w.Hk * s.slots((w.Nk + tile - 1) / tile) * 2 * tile * D * 4;
 }
 
 // SIMT kernels (fp32 inputs; any strides).
@@ -135,7 +177,7 @@ cudaError_t launch_bwd_dq_f32(int D, bool causal, const BwdArgs& a, cudaStream_t
 cudaError_t launch_bwd_dkdv_f32(int D, bool causal, const BwdArgs& a, cudaStream_t s);
 
 // Sliding window with sinks in fp32 (window_f32.cu; any strides). The backward writes dk, dv and dq from
-// a.delta, cutting its sink tiles as a.split says; a.qk_scale and a.sm_scale are signed.
+// a.delta in the units of a.split; a.qk_scale and a.sm_scale are signed.
 cudaError_t launch_window_fwd_f32(int D, const void* q, const void* k, const void* v, Strides4 sq, Strides4 sk,
                                   Strides4 sv, const FwdArgs& a, cudaStream_t s);
 cudaError_t launch_window_bwd_f32(int D, const BwdArgs& a, cudaStream_t s);

@@ -230,63 +230,54 @@ __global__ void __launch_bounds__(kThreads) window_dq_f32_kernel(BwdArgs a) {
   }
 }
 
-// One key tile of one key/value head, summed over the query heads that share it; of a tile with sinks, which
-// all later queries see, one chunk of its query rows (WindowSplit) if those are cut, as a partial result.
+// One unit of a key/value head (window_unit): a key tile, summed over the query heads that share it, or a part of
+// that sum.
 template <int D>
 __global__ void __launch_bounds__(kThreads) window_dkdv_f32_kernel(BwdArgs a) {
   extern __shared__ __align__(16) float smem[];
   float *Ks = smem, *Vs = Ks + TB * kPitch<D>, *Qs = Vs + TB * kPitch<D>, *Os = Qs + TB * kPitch<D>;
   float *Ps = Os + TB * kPitch<D>, *DSs = Ps + TB * kPitchP, *Ms = DSs + TB * kPitchP, *Ds = Ms + TB;
-  const int cut = a.split.tiles * a.split.chunks, unit = blockIdx.x;
-  const bool sink = unit < cut;
-  const int N = a.N, Nk = a.win.Nk, k0 = TB * (sink ? unit / a.split.chunks : unit - cut + a.split.tiles);
+  const int N = a.N, Nk = a.win.Nk;
+  const WindowUnit u = window_unit<TB, TB>(a.split, a.win, N, blockIdx.x);
+  const int k0 = TB * u.kt;
   const int zi = blockIdx.y / a.win.Hk, hk = blockIdx.y % a.win.Hk;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   load_rows<D>(Ks, static_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h, a.sk, k0, Nk);
   load_rows<D>(Vs, static_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h, a.sv, k0, Nk);
   float dk[4][D / 16] = {}, dv[4][D / 16] = {};
-  // Rows from the first key's position on; without a sink in the tile, up to one window past its last key.
-  int first = max(0, k0 - a.win.off);
-  int end = sink ? N : int(min(int64_t(N), int64_t(k0) + TB - 1 + a.win.window - a.win.off));
-  if (sink && a.split.chunks > 1) {
-    first += unit % a.split.chunks * a.split.blocks * TB;
-    end = min(N, first + a.split.blocks * TB);
-  }
-  for (int g = 0; g < a.win.group; ++g) {
-    const int hi = hk * a.win.group + g;
+  for (int i = u.start; i < u.start + u.n; ++i) {
+    const int hi = hk * a.win.group + i / u.nb, r0 = (u.lo + i % u.nb) * TB;
     const float* q = static_cast<const float*>(a.q) + zi * a.sq.z + hi * a.sq.h;
     const float* dout = static_cast<const float*>(a.dout) + zi * a.sdo.z + hi * a.sdo.h;
     const int64_t rows = (int64_t(zi) * a.H + hi) * N;
-    for (int r0 = first; r0 < end; r0 += TB) {
-      __syncthreads();
-      load_rows<D>(Qs, q, a.sq, r0, N);
-      load_rows<D>(Os, dout, a.sdo, r0, N);
-      if (threadIdx.x < TB) {
-        const int row = r0 + threadIdx.x;
-        Ms[threadIdx.x] = row < N ? a.m[rows + row] : 0.f;
-        Ds[threadIdx.x] = row < N ? a.delta[rows + row] : 0.f;
-      }
-      __syncthreads();
-      float p[4][4], ds[4][4];
-      p_ds<D, true>(a, Ks, Qs, Vs, Os, ty, tx, k0, r0, Ms, Ds, p, ds);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          Ps[(4 * ty + i) * kPitchP + tx + 16 * j] = p[i][j];
-          DSs[(4 * ty + i) * kPitchP + tx + 16 * j] = ds[i][j];
-        }
-      __syncwarp();
-      rows_times<D>(Ps, Os, ty, tx, dv);
-      rows_times<D>(DSs, Qs, ty, tx, dk);
+    __syncthreads();
+    load_rows<D>(Qs, q, a.sq, r0, N);
+    load_rows<D>(Os, dout, a.sdo, r0, N);
+    if (threadIdx.x < TB) {
+      const int row = r0 + threadIdx.x;
+      Ms[threadIdx.x] = row < N ? a.m[rows + row] : 0.f;
+      Ds[threadIdx.x] = row < N ? a.delta[rows + row] : 0.f;
     }
+    __syncthreads();
+    float p[4][4], ds[4][4];
+    p_ds<D, true>(a, Ks, Qs, Vs, Os, ty, tx, k0, r0, Ms, Ds, p, ds);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        Ps[(4 * ty + i) * kPitchP + tx + 16 * j] = p[i][j];
+        DSs[(4 * ty + i) * kPitchP + tx + 16 * j] = ds[i][j];
+      }
+    __syncwarp();
+    rows_times<D>(Ps, Os, ty, tx, dv);
+    rows_times<D>(DSs, Qs, ty, tx, dk);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int key = k0 + 4 * ty + i;
     if (key >= Nk) continue;
-    if (sink && a.split.chunks > 1) {
-      const int64_t slot = int64_t(blockIdx.y) * cut + unit;
+    if (u.slot >= 0) {
+      const int64_t slot = int64_t(blockIdx.y) * a.split.slots((Nk + TB - 1) / TB) + u.slot;
       float* part = a.part + (slot * 2 * TB + 4 * ty + i) * D + D / 16 * tx;
 #pragma unroll
       for (int e = 0; e < D / 16; ++e) {
@@ -304,18 +295,22 @@ __global__ void __launch_bounds__(kThreads) window_dkdv_f32_kernel(BwdArgs a) {
   }
 }
 
-// dV and dK of the cut sink tiles: the sums of the chunks' partials, in their order.
+// dV and dK of the tiles of several units: the sums of the units' partials, in their order.
 __global__ void __launch_bounds__(kThreads) window_join_f32_kernel(BwdArgs a, int D) {
+  const int key_tiles = (a.win.Nk + TB - 1) / TB, tiles = a.split.units > 1 ? key_tiles : a.split.tiles;
   const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x, tile = TB * D;
   const int which = int(i / tile % 2);  // 0: dV, 1: dK
-  const int64_t t = i / (2 * tile);     // sink tiles of all heads
-  const int key = int(t % a.split.tiles) * TB + int(i % tile / D);
-  if (t >= int64_t(a.Z) * a.win.Hk * a.split.tiles || key >= a.win.Nk) return;
-  const float* p = a.part + t * a.split.chunks * 2 * tile + which * tile + i % tile;
+  const int64_t t = i / (2 * tile), head = t / tiles;
+  const int kt = int(t % tiles), key = kt * TB + int(i % tile / D);
+  const bool sink = kt < a.split.tiles;
+  const int count = sink ? a.split.sink_units : a.split.units;
+  if (head >= int64_t(a.Z) * a.win.Hk || count == 1 || key >= a.win.Nk) return;
+  const int first = sink ? kt * count : a.split.tiles * a.split.sink_units + (kt - a.split.tiles) * count;
+  const float* p = a.part + ((head * a.split.slots(key_tiles) + first) * 2 + which) * tile + i % tile;
   float sum = 0.f;
-  for (int c = 0; c < a.split.chunks; ++c) sum += p[c * 2 * tile];
+  for (int c = 0; c < count; ++c) sum += p[c * 2 * tile];
   float* out = static_cast<float*>(which ? a.dk : a.dv);
-  out[(t / a.split.tiles * a.win.Nk + key) * D + i % D] = which ? sum * a.sm_scale : sum;
+  out[(head * a.win.Nk + key) * D + i % D] = which ? sum * a.sm_scale : sum;
 }
 
 template <typename Kernel, typename... Args>
@@ -337,12 +332,12 @@ cudaError_t fwd_impl(const float* q, const float* k, const float* v, const Strid
 
 template <int D>
 cudaError_t bwd_impl(const BwdArgs& a, cudaStream_t s) {
-  const int units = (a.win.Nk + TB - 1) / TB + a.split.tiles * (a.split.chunks - 1);
-  cudaError_t e = launch(window_dkdv_f32_kernel<D>, units, (long long)a.Z * a.win.Hk,
+  const int key_tiles = (a.win.Nk + TB - 1) / TB;
+  cudaError_t e = launch(window_dkdv_f32_kernel<D>, a.split.per_head(key_tiles), (long long)a.Z * a.win.Hk,
                          TB * (4 * kPitch<D> + 2 * kPitchP + 2), s, a);
   if (e != cudaSuccess) return e;
-  if (a.split.chunks > 1) {
-    const int64_t values = int64_t(a.Z) * a.win.Hk * a.split.tiles * 2 * TB * D;
+  if (a.split.slots(key_tiles) > 0) {
+    const int64_t values = int64_t(a.Z) * a.win.Hk * (a.split.units > 1 ? key_tiles : a.split.tiles) * 2 * TB * D;
     window_join_f32_kernel<<<unsigned((values + kThreads - 1) / kThreads), kThreads, 0, s>>>(a, D);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
