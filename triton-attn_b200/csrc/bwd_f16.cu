@@ -1953,20 +1953,41 @@ __device__ __forceinline__ void fused_part_epilogue(const BwdArgs& a) {
     const float* part = a.part + int64_t(bh * slots + first) * 2 * 128 * D;
     uint4* out = static_cast<uint4*>(which ? a.dk : a.dv) + (int64_t(bh) * a.win.Nk + kt * 128) * kRow;
     const float sc = which ? a.sm_scale : 1.f;
-    for (int e = int(t); e < 128 * kRow; e += 256) {
-      const int row = e / kRow, col = e % kRow * 8, colh = col % B::HW;
-      if (kt * 128 + row >= a.win.Nk) break;
-      const float* p = part + B::box(which, col / B::HW, colh / B::PW, row / 32);
-      const int u = colh % B::PW / 4, at0 = B::unit(row % 32, u), at1 = B::unit(row % 32, u + 1);
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-#pragma unroll 4
-      for (int c = 0; c < count; ++c, p += 2 * 128 * D) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(p + at0)), w = __ldcg(reinterpret_cast<const float4*>(p + at1));
-        x = make_float4(x.x + v.x, x.y + v.y, x.z + v.z, x.w + v.w);
-        y = make_float4(y.x + w.x, y.y + w.y, y.z + w.z, y.w + w.w);
+    // G groups of a thread at once: their loads of one unit's partial are in flight together.
+    constexpr int G = 128 * kRow / 256 < 4 ? 128 * kRow / 256 : 4;
+    for (int e0 = int(t); e0 < 128 * kRow; e0 += 256 * G) {
+      const float *p0[G], *p1[G];
+      float4 x[G], y[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const int e = e0 + 256 * g, row = e / kRow, col = e % kRow * 8, colh = col % B::HW, u = colh % B::PW / 4;
+        const float* box = part + B::box(which, col / B::HW, colh / B::PW, row / 32);
+        p0[g] = box + B::unit(row % 32, u);
+        p1[g] = box + B::unit(row % 32, u + 1);
+        x[g] = y[g] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
-      out[e] = make_uint4(pack_half2(x.x * sc, x.y * sc), pack_half2(x.z * sc, x.w * sc),
-                          pack_half2(y.x * sc, y.y * sc), pack_half2(y.z * sc, y.w * sc));
+#pragma unroll 2
+      for (int c = 0; c < count; ++c) {
+        const int64_t slot = int64_t(c) * 2 * 128 * D;
+        float4 v[G], w[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          v[g] = __ldcg(reinterpret_cast<const float4*>(p0[g] + slot));
+          w[g] = __ldcg(reinterpret_cast<const float4*>(p1[g] + slot));
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          x[g] = make_float4(x[g].x + v[g].x, x[g].y + v[g].y, x[g].z + v[g].z, x[g].w + v[g].w);
+          y[g] = make_float4(y[g].x + w[g].x, y[g].y + w[g].y, y[g].z + w[g].z, y[g].w + w[g].w);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const int e = e0 + 256 * g;
+        if (kt * 128 + e / kRow < a.win.Nk)
+          out[e] = make_uint4(pack_half2(x[g].x * sc, x[g].y * sc), pack_half2(x[g].z * sc, x[g].w * sc),
+                              pack_half2(y[g].x * sc, y[g].y * sc), pack_half2(y[g].z * sc, y[g].w * sc));
+      }
     }
   }
 }
