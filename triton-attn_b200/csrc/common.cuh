@@ -321,16 +321,19 @@ __device__ __forceinline__ void tmem_store_cols(uint32_t taddr, const uint32_t* 
 // group's K and V (2 * N * D fp16 each) take at most ~48 MiB, and the order is longest first within a
 // group, one group after another. Returns the CTA's position in its head's longest-first order (0 = the
 // longest tile) and sets *bh.
-__device__ __forceinline__ int causal_cta_rank(int nct, int zh, int N, int D, int* bh) {
-  const long long per_head = 4ll * N * D;
+// (per_head: its K and V in bytes; index: the CTA's place among zh heads of nct tiles each.)
+__device__ __forceinline__ int grouped_cta_rank(int index, int nct, int zh, long long per_head, int* bh) {
   const int hg = int(per_head <= 0 ? zh : max(1ll, min((long long)zh, (48ll << 20) / per_head)));
   const int per_group = hg * nct;
-  const int grp = int(blockIdx.x) / per_group;
+  const int grp = index / per_group;
   const int h0 = grp * hg;
   const int gh = min(hg, zh - h0);             // heads in this group (the last one may be short)
-  const int r = int(blockIdx.x) - grp * per_group;  // < gh * nct
+  const int r = index - grp * per_group;       // < gh * nct
   *bh = h0 + r % gh;
   return r / gh;
+}
+__device__ __forceinline__ int causal_cta_rank(int nct, int zh, int N, int D, int* bh) {
+  return grouped_cta_rank(int(blockIdx.x), nct, zh, 4ll * N * D, bh);
 }
 
 // ----------------------------------------------------------------------------------------------

@@ -254,6 +254,19 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
   int bh, cta;
   if (CAUSAL) {  // longest first within groups of heads whose K/V fit in L2 (the highest row blocks see the most keys)
     cta = nct - 1 - causal_cta_rank(nct, args.Z * args.H, N, D, &bh);
+  } else if (WINDOW) {
+    // As below, but the row blocks whose windows the sequence's beginning cuts short come after all others, the
+    // longest first as in a causal grid: they fill the end of the grid (130 us against 124 at B4 H16 N4096 D64,
+    // window 1024).
+    const int zh = args.Z * args.H, cut = args.win.window - args.win.off;
+    const int brief = min(nct, max(0, cut) / (TILES * C::BM)), whole = nct - brief;
+    const int rest = int(blockIdx.x) - zh * whole;
+    if (rest < 0) {
+      bh = int(blockIdx.x) / whole;
+      cta = brief + int(blockIdx.x) % whole;
+    } else {
+      cta = brief - 1 - grouped_cta_rank(rest, brief, zh, 4ll * args.win.Nk * D / args.win.group, &bh);
+    }
   } else {  // row blocks of one head adjacent: K/V of a head stay hot in L2
     bh = blockIdx.x / nct;
     cta = blockIdx.x % nct;
