@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
   } else if (WINDOW) {
     // As below, but the row blocks whose windows the sequence's beginning cuts short come after all others, the
     // longest first as in a causal grid: they fill the end of the grid (130 us against 124 at B4 H16 N4096 D64,
-    // window 1024).
+    // window 1024; with half as many heads a group, as in a causal grid, 128).
     const int zh = args.Z * args.H, cut = args.win.window - args.win.off;
     const int brief = min(nct, max(0, cut) / (TILES * C::BM)), whole = nct - brief;
     const int rest = int(blockIdx.x) - zh * whole;
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
       bh = int(blockIdx.x) / whole;
       cta = brief + int(blockIdx.x) % whole;
     } else {
-      cta = brief - 1 - grouped_cta_rank(rest, brief, zh, 4ll * args.win.Nk * D / args.win.group, &bh);
+      cta = brief - 1 - grouped_cta_rank(rest, brief, zh, 2ll * args.win.Nk * D / args.win.group, &bh);
     }
   } else {  // row blocks of one head adjacent: K/V of a head stay hot in L2
     bh = blockIdx.x / nct;
