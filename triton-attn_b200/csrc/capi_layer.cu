@@ -139,15 +139,16 @@ bool decode_dims(DecodeArgs& a, int Z, int H, int Hk, int C, int D, int window, 
   return true;
 }
 
-int64_t decode_workspace(const DecodeArgs& a, int D, int nsplit) {
-  return nsplit == 1 ? 0 : int64_t(a.Z) * a.H * nsplit * (D + 2) * 4;
+int64_t decode_workspace(const DecodeArgs& a, int D, DecodeCache cache) {
+  const int nsplit = decode_splits(a, D, cache);
+  return decode_joins(nsplit, cache) ? int64_t(a.Z) * a.H * nsplit * (D + 2) * 4 : 0;
 }
 
 int decode(DecodeArgs& a, int D, DecodeCache cache, void* workspace, float sm_scale, void* stream) {
   int rc = device_ready(&a.status);
   if (rc != TATTN_OK) return rc;
   a.nsplit = decode_splits(a, D, cache);
-  if (a.nsplit > 1) {
+  if (decode_joins(a.nsplit, cache)) {
     if (!workspace) return TATTN_ERR_INVALID_ARGUMENT;
     if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return TATTN_ERR_LAYOUT;
     a.part = static_cast<float*>(workspace);
@@ -187,7 +188,7 @@ extern "C" int tattn_decode(const void* q, const void* k, const void* v, const i
 extern "C" int64_t tattn_decode_workspace_bytes(int Z, int H, int Hk, int C, int D, int dtype, int window, int sinks) {
   DecodeArgs a{};
   if (!decode_dims(a, Z, H, Hk, C, D, window, sinks) || (dtype != TATTN_F16 && dtype != TATTN_F32)) return -1;
-  return decode_workspace(a, D, decode_splits(a, D, dtype == TATTN_F16 ? kCacheF16 : kCacheF32));
+  return decode_workspace(a, D, dtype == TATTN_F16 ? kCacheF16 : kCacheF32);
 }
 
 namespace {
@@ -283,5 +284,5 @@ extern "C" int tattn_int4_decode(const void* q, const void* k_codes, const void*
 extern "C" int64_t tattn_int4_decode_workspace_bytes(int Z, int H, int Hk, int C, int D, int window, int sinks) {
   DecodeArgs a{};
   if (!decode_dims(a, Z, H, Hk, C, D, window, sinks) || !int4_dims(Z, Hk, 0, C, D)) return -1;
-  return decode_workspace(a, D, decode_splits(a, D, kCacheInt4));
+  return decode_workspace(a, D, kCacheInt4);
 }

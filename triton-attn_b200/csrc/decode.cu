@@ -8,7 +8,8 @@
 // takes one key/value head, up to 8 NT of its query heads and one of nsplit equal parts of the visible
 // tokens; its warps take 16- or 32-key tiles in turn through rings of their own (cp.async, no barrier
 // between warps) and keep their own running maximum and sum, which are joined at the end: within the CTA
-// through shared memory, over the parts by a second small kernel. With few heads a matrix instruction of 8
+// through shared memory, over the parts, where they are at most kClusterParts, by the cluster that they form,
+// through each other's shared memory, else by a second small kernel. With few heads a matrix instruction of 8
 // columns is enough: S^T = K Q^T and O^T += V^T P^T as mma.m16n8k16 with keys (then dims) as the 16 rows
 // and query heads as the 8 columns, so nothing is computed for rows that do not exist, and the S^T
 // accumulators become the P^T operand by one 8 x 8 transposition in registers. (tcgen05 has 64 rows at
@@ -213,14 +214,48 @@ __device__ __forceinline__ void softmax_tile(WarpState<D, NT>& st, float (*x)[NT
       }
 }
 
-// Joins the warps' results through shared memory (kWarps * 8 NT * (D + 2) floats) and writes the CTA's part:
-// the finished row if there is only one part, else the unnormalised row with its maximum and sum.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// The address in the cluster's CTA `rank` of what lies at `addr` in this one's shared memory, and loads from it.
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 load_cluster4(uint32_t addr) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(addr) : "memory");
+  return x;
+}
+__device__ __forceinline__ float2 load_cluster2(uint32_t addr) {
+  float2 x;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(addr) : "memory");
+  return x;
+}
+
+template <int D>
+__device__ __forceinline__ void write_row4(const DecodeArgs& a, int z, int h, int d, const float4& o, float l) {
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // NaN stays NaN
+  *reinterpret_cast<uint2*>(static_cast<__half*>(a.o) + z * a.so.z + h * a.so.h + d) =
+      make_uint2(pack_half2(o.x * inv, o.y * inv), pack_half2(o.z * inv, o.w * inv));
+}
+
+// Floats of shared memory that finish() needs: every warp's rows with their maxima and sums, and their join.
+template <int D>
+constexpr int finish_floats(int NT) {
+  return (kWarps + 1) * 8 * NT * (D + 2);
+}
+
+// Joins the warps' results through shared memory, then the parts': writes finished rows if there is only one
+// part or the parts are a cluster, else the part's unnormalised rows with their maxima and sums.
 // dim(mt, half): the head dim of this lane's row g + 8 half of M tile mt.
 template <int D, int NT, typename Dim>
 __device__ __forceinline__ void finish(const DecodeArgs& a, const Part& p, WarpState<D, NT>& st, float* smem, Dim dim) {
   constexpr int HEADS = 8 * NT;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-  float* ml = smem + kWarps * HEADS * D;  // [warp][head][2]
+  float* ml = smem + kWarps * HEADS * D;            // [warp][head][2]
+  float* mine = smem + kWarps * HEADS * (D + 2);    // the CTA's [head][D], then [head][2]
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -256,15 +291,44 @@ __device__ __forceinline__ void finish(const DecodeArgs& a, const Part& p, WarpS
     }
     const int h = p.h0 + head;
     if (a.nsplit == 1) {
-      const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // NaN stays NaN
-      *reinterpret_cast<uint2*>(static_cast<__half*>(a.o) + p.z * a.so.z + h * a.so.h + d) =
-          make_uint2(pack_half2(o.x * inv, o.y * inv), pack_half2(o.z * inv, o.w * inv));
+      write_row4<D>(a, p.z, h, d, o, l);
+    } else if (a.nsplit <= kClusterParts) {
+      *reinterpret_cast<float4*>(mine + head * D + d) = o;
+      if (d == 0) *reinterpret_cast<float2*>(mine + HEADS * D + head * 2) = make_float2(m, l);
     } else {
       const int64_t row = (int64_t(p.z) * a.H + h) * a.nsplit + p.split;
       *reinterpret_cast<float4*>(a.part + row * D + d) = o;
       if (d == 0) *reinterpret_cast<float2*>(a.part_ml + row * 2) = make_float2(m, l);
     }
   }
+  if (a.nsplit == 1 || a.nsplit > kClusterParts) return;
+  // The cluster's CTAs are the parts in order; each finishes a share of the rows.
+  cluster_sync();
+  const uint32_t rows = smem_u32(mine);
+  for (int i = p.split * kThreads + threadIdx.x; i < p.heads * (D / 4); i += a.nsplit * kThreads) {
+    const int head = i / (D / 4), d = i % (D / 4) * 4;
+    float2 ml_of[kClusterParts];
+    float4 x[kClusterParts];
+    float m = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kClusterParts; ++c) {
+      if (c >= a.nsplit) break;
+      ml_of[c] = load_cluster2(in_cta(rows + (HEADS * D + head * 2) * 4, c));
+      x[c] = load_cluster4(in_cta(rows + (head * D + d) * 4, c));
+      m = fmaxf(m, ml_of[c].x);
+    }
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+#pragma unroll
+    for (int c = 0; c < kClusterParts; ++c) {
+      if (c >= a.nsplit) break;
+      const float f = m == -INFINITY ? 0.f : ex2_approx(ml_of[c].x - m);
+      l = fmaf(f, ml_of[c].y, l);
+      o = make_float4(fmaf(f, x[c].x, o.x), fmaf(f, x[c].y, o.y), fmaf(f, x[c].z, o.z), fmaf(f, x[c].w, o.w));
+    }
+    write_row4<D>(a, p.z, p.h0 + head, d, o, l);
+  }
+  cluster_sync();  // no CTA leaves while another reads its rows
 }
 
 // ------------------------------------------------------------------------------------- fp16 cache
@@ -284,7 +348,7 @@ struct F16Cfg {
   static constexpr int TILE = KT * D * 2;  // bytes of a K or V tile
   static constexpr int RING = kWarps * STAGES * 2 * TILE;
   static constexpr int smem(int NT) {
-    const int join = kWarps * 8 * NT * (D + 2) * 4;
+    const int join = finish_floats<D>(NT) * 4;
     return RING > join ? RING : join;
   }
 };
@@ -417,7 +481,7 @@ struct Int4Cfg {
   static constexpr int TILE = 2 * (CODES + PARAMS);               // K codes, V codes, K params, V params
   static constexpr int RING = kWarps * STAGES * TILE;
   static constexpr int smem(int NT) {
-    const int join = kWarps * 8 * NT * (D + 2) * 4;
+    const int join = finish_floats<D>(NT) * 4;
     return RING > join ? RING : join;
   }
   // Where a group's 32 bytes lie in a tile: so that the four rows a quarter of the lanes reads at a time, 0, 4,
@@ -705,43 +769,70 @@ __global__ void __launch_bounds__(kThreads) decode_f32_kernel(const DecodeArgs a
   }
 }
 
-// Joins the parts of each query head: one warp a head.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeArgs a, int D) {
-  const int row = blockIdx.x * kWarps + threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (row >= a.Z * a.H) return;
+// Joins the parts of each query head: one CTA a head, whose threads take 4 dims of every so many-th part.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeArgs a) {
+  constexpr int V = D / 4, LANES = kThreads / V;  // threads of a row, rows in flight
+  __shared__ float4 so[LANES][V];
+  __shared__ float sl[LANES];
+  const int row = blockIdx.x, t = threadIdx.x % V, p = threadIdx.x / V;
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + int64_t(row) * a.nsplit;
   float m = -INFINITY;
-  for (int s = lane; s < a.nsplit; s += 32) m = fmaxf(m, ml[s].x);
+  for (int s = threadIdx.x % 32; s < a.nsplit; s += 32) m = fmaxf(m, ml[s].x);
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float use = m == -INFINITY ? 0.f : m;
-  float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};  // dims lane, lane + 32, ...
-  const float* o = a.part + int64_t(row) * a.nsplit * D;
+  float l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4* o = reinterpret_cast<const float4*>(a.part) + int64_t(row) * a.nsplit * V + t;
 #pragma unroll 4
-  for (int s = 0; s < a.nsplit; ++s) {
+  for (int s = p; s < a.nsplit; s += LANES) {
     const float2 x = ml[s];
+    const float4 v = o[int64_t(s) * V];
     const float f = exp2f(x.x - use);
     l = fmaf(f, x.y, l);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (lane + 32 * e < D) acc[e] = fmaf(f, o[int64_t(s) * D + lane + 32 * e], acc[e]);
+    acc = make_float4(fmaf(f, v.x, acc.x), fmaf(f, v.y, acc.y), fmaf(f, v.z, acc.z), fmaf(f, v.w, acc.w));
   }
-  T* out = static_cast<T*>(a.o) + row / a.H * a.so.z + row % a.H * a.so.h;
+  so[p][t] = acc;
+  if (t == 0) sl[p] = l;
+  __syncthreads();
+  if (p > 0) return;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (lane + 32 * e < D) out[lane + 32 * e] = T(l == 0.f ? 0.f : acc[e] / l);
+  for (int q = 1; q < LANES; ++q) {
+    const float4 v = so[q][t];
+    acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
+    l += sl[q];
+  }
+  const int z = row / a.H, h = row % a.H;
+  if constexpr (sizeof(T) == 2) {
+    write_row4<D>(a, z, h, 4 * t, acc, l);
+  } else {
+    float* out = static_cast<float*>(a.o) + z * a.so.z + h * a.so.h + 4 * t;
+    const float den = l == 0.f ? 1.f : l;  // (then acc is 0)
+    *reinterpret_cast<float4*>(out) = make_float4(acc.x / den, acc.y / den, acc.z / den, acc.w / den);
+  }
 }
 
+// `cluster`: the parts of a unit, which are neighbours in the grid, as one cluster.
 template <typename K>
-cudaError_t launch(K kernel, int smem, long long grid, const DecodeArgs& a, cudaStream_t s) {
-  if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+cudaError_t launch(K kernel, int smem, long long units, bool cluster, const DecodeArgs& a, cudaStream_t s) {
+  if (units * a.nsplit > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
   }
-  kernel<<<unsigned(grid), kThreads, smem, s>>>(a);
-  return cudaGetLastError();
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(unsigned(units * a.nsplit));
+  c.blockDim = dim3(kThreads);
+  c.dynamicSmemBytes = size_t(smem);
+  c.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = unsigned(a.nsplit);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  c.attrs = &attr;
+  c.numAttrs = cluster ? 1 : 0;
+  return cudaLaunchKernelEx(&c, kernel, a);
 }
 
 // CTAs before splitting: sequences, key/value heads and chunks of their query heads.
@@ -751,20 +842,26 @@ long long decode_units(const DecodeArgs& a, int heads_per_cta) {
 }
 
 template <int D>
-cudaError_t f16_impl(const DecodeArgs& a, cudaStream_t s) {
-  return a.H / a.Hk <= 8 ? launch(decode_f16_kernel<D, 1>, F16Cfg<D>::smem(1), decode_units(a, 8) * a.nsplit, a, s)
-                         : launch(decode_f16_kernel<D, 2>, F16Cfg<D>::smem(2), decode_units(a, 16) * a.nsplit, a, s);
-}
-
-template <int D>
-cudaError_t int4_impl(const DecodeArgs& a, cudaStream_t s) {
-  return a.H / a.Hk <= 8 ? launch(decode_int4_kernel<D, 1>, Int4Cfg<D>::smem(1), decode_units(a, 8) * a.nsplit, a, s)
-                         : launch(decode_int4_kernel<D, 2>, Int4Cfg<D>::smem(2), decode_units(a, 16) * a.nsplit, a, s);
-}
-
-template <int D>
-cudaError_t f32_impl(const DecodeArgs& a, cudaStream_t s) {
-  return launch(decode_f32_kernel<D>, 0, decode_units(a, 1) * a.nsplit, a, s);
+cudaError_t decode_impl(DecodeCache cache, const DecodeArgs& a, cudaStream_t s) {
+  const bool join = decode_joins(a.nsplit, cache), cluster = a.nsplit > 1 && !join, wide = a.H / a.Hk > 8;
+  cudaError_t e;
+  if (cache == kCacheF32) {
+    e = launch(decode_f32_kernel<D>, 0, decode_units(a, 1), false, a, s);
+  } else if (cache == kCacheF16) {
+    e = wide ? launch(decode_f16_kernel<D, 2>, F16Cfg<D>::smem(2), decode_units(a, 16), cluster, a, s)
+             : launch(decode_f16_kernel<D, 1>, F16Cfg<D>::smem(1), decode_units(a, 8), cluster, a, s);
+  } else if constexpr (D % kGroupDims == 0) {
+    e = wide ? launch(decode_int4_kernel<D, 2>, Int4Cfg<D>::smem(2), decode_units(a, 16), cluster, a, s)
+             : launch(decode_int4_kernel<D, 1>, Int4Cfg<D>::smem(1), decode_units(a, 8), cluster, a, s);
+  } else {
+    e = cudaErrorNotSupported;
+  }
+  if (e != cudaSuccess || !join) return e;
+  if (cache == kCacheF32)
+    decode_join_kernel<float, D><<<unsigned(a.Z * a.H), kThreads, 0, s>>>(a);
+  else
+    decode_join_kernel<__half, D><<<unsigned(a.Z * a.H), kThreads, 0, s>>>(a);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -776,26 +873,21 @@ int decode_splits(const DecodeArgs& a, int D, DecodeCache cache) {
   const long long most = a.window < a.C ? std::min<long long>(a.C, (long long)a.window + a.sinks) : a.C;
   // Enough CTAs to fill the GPU several times over, none with less than a tile for each warp.
   const int tile = kWarps * (cache == kCacheF32 ? 4 : cache == kCacheF16 && D == 128 ? 16 : 32);
-  const long long want = (kDecodeCtas * (long long)device_sm_count() + units - 1) / units;
-  return int(std::max<long long>(1, std::min<long long>(want, (most + tile - 1) / tile)));
+  const long long want = (decode_ctas(cache) * (long long)device_sm_count() + units - 1) / units;
+  const long long n = std::max<long long>(1, std::min<long long>(want, (most + tile - 1) / tile));
+  // A few parts more than a cluster has are not worth a second kernel where parts are short.
+  return int(decode_joins(int(n), cache) && n <= 2 * kClusterParts && most <= kClusterParts * 2048 && cache != kCacheF32 ? kClusterParts : n);
 }
 
 cudaError_t launch_decode(int D, DecodeCache cache, const DecodeArgs& a, cudaStream_t s) {
   if (a.Z * a.H == 0) return cudaSuccess;
-  cudaError_t e = cudaErrorInvalidValue;
   switch (D) {
-    case 16: e = cache == kCacheF16 ? f16_impl<16>(a, s) : f32_impl<16>(a, s); break;
-    case 32: e = cache == kCacheF16 ? f16_impl<32>(a, s) : f32_impl<32>(a, s); break;
-    case 64: e = cache == kCacheF16 ? f16_impl<64>(a, s) : cache == kCacheInt4 ? int4_impl<64>(a, s) : f32_impl<64>(a, s); break;
-    case 128: e = cache == kCacheF16 ? f16_impl<128>(a, s) : cache == kCacheInt4 ? int4_impl<128>(a, s) : f32_impl<128>(a, s); break;
+    case 16: return decode_impl<16>(cache, a, s);
+    case 32: return decode_impl<32>(cache, a, s);
+    case 64: return decode_impl<64>(cache, a, s);
+    case 128: return decode_impl<128>(cache, a, s);
+    default: return cudaErrorInvalidValue;
   }
-  if (e != cudaSuccess || a.nsplit == 1) return e;
-  const unsigned grid = unsigned((a.Z * a.H + kWarps - 1) / kWarps);
-  if (cache == kCacheF32)
-    decode_join_kernel<float><<<grid, kThreads, 0, s>>>(a, D);
-  else
-    decode_join_kernel<__half><<<grid, kThreads, 0, s>>>(a, D);
-  return cudaGetLastError();
 }
 
 }  // namespace tattn

@@ -236,8 +236,16 @@ struct DecodeArgs {
   float qk_scale;       // sm_scale * log2(e)
   int* status;
 };
-// CTAs per SM that decode_splits aims at.
-constexpr int kDecodeCtas = 4;
+// CTAs per SM that decode_splits aims at: as many as an SM holds. (fp16, 64 sequences of 4096 visible tokens, 4
+// heads of 128: 2 parts each 82 us, 3 parts 86, 4 parts 90. 4 bits, 16 sequences of up to 65536 tokens: 10
+// parts 112 us, 14 to 37 parts 110 to 106, but 2 such sequences: 27 us with 4 CTAs an SM, 32 with 8.)
+constexpr int decode_ctas(DecodeCache cache) { return cache == kCacheF16 ? 2 : 4; }
+// Up to so many parts are one cluster (the most that any GPU takes) and join through its shared memory; more, and
+// the fp32 kernel's, are joined by a second kernel through the workspace.
+constexpr int kClusterParts = 8;
+inline bool decode_joins(int nsplit, DecodeCache cache) {
+  return nsplit > (cache == kCacheF32 ? 1 : kClusterParts);
+}
 // Parts that the visible tokens are cut into: by the sizes alone, never by the lengths on the device.
 int decode_splits(const DecodeArgs& a, int D, DecodeCache cache);
 // The 4-bit cache (int4_cache.cu), for k and v each: codes [Z, Hk, C, D / 2] bytes, head dim 2 i in the low half
