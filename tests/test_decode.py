@@ -266,6 +266,36 @@ def test_layouts(gpu) -> None:
 
 
 @pytest.mark.gpu
+def test_nothing_to_attend_with(gpu) -> None:
+    q, k, v = _inputs(2, 0, 1, 50, 64, torch.float16, 4)
+    assert decode_attention(q, k, v, _lens(3, 4)).shape == q.shape
+    q, k, v = _inputs(0, 2, 1, 50, 64, torch.float16, 4)
+    assert decode_attention(q, k, v, _lens()).shape == q.shape
+    q, k, v = _inputs(2, 2, 1, 0, 64, torch.float16, 4)
+    assert not bool(decode_attention(q, k, v, _lens(0, 0)).any())
+    cache = Int4Cache.empty(2, 1, 0, 64)
+    assert not bool(cache.attend(q, _lens(0, 0)).any())
+    cache.append(k, v)
+    assert cache.read(0)[0].shape == (2, 1, 0, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [1000, 4000, 40000])
+def test_every_way_of_joining_parts(gpu, cap) -> None:
+    """One sequence of few heads is cut into as many parts as its capacity allows: a cluster or a second kernel;
+    with parts that hold nothing (a short length) in both."""
+    for d, h in ((64, 1), (128, 12)):
+        q, k, v = _inputs(2, h, 1, cap, d, torch.float16, 23)
+        cache = Int4Cache.empty(2, 1, cap, d)
+        cache.append(k, v)
+        for lengths in ((cap, cap - 1), (1, 40), (0, 700)):
+            o = decode_attention(q, k, v, _lens(*lengths))
+            assert_within(o, *_decode64(q, k, v, lengths, None, 0, d**-0.5, 1e-3, 2.0**-11), "o")
+            o = cache.attend(q, _lens(*lengths))
+            assert_within(o, *_decode64(q, *_exact_values(cache), lengths, None, 0, d**-0.5, 2e-3, 2.0**-11), "4 bits")
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits(gpu) -> None:
     """The last sequence's rows begin past 2^32 elements of a cache and 2^32 bytes of codes."""
     b, cap, d = 3, 1 << 24, 128

@@ -264,6 +264,33 @@ def test_no_queries(gpu) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["f16", "f32"])
+def test_nothing_to_attend_with(gpu, dtype) -> None:
+    """No batch, or no query heads: empty results, and zeros for keys and values that no query sees."""
+    for b, h in ((0, 2), (3, 0)):
+        q, k, v, do = _qkv(b, h, 2, 5, 9, 32, dtype, 16)
+        for t in (q, k, v):
+            t.requires_grad_()
+        o = window_attention(q, k, v, 4, 1)
+        grads = torch.autograd.grad(o, (q, k, v), do)
+        assert o.shape == q.shape and all(g.shape == t.shape for g, t in zip(grads, (q, k, v), strict=True))
+        assert not bool(grads[1].any()) and not bool(grads[2].any())
+
+
+@pytest.mark.gpu
+def test_more_heads_than_a_grid_dimension(gpu) -> None:
+    for dtype in (torch.float16, torch.float32):
+        q, k, v, do = _qkv(66000, 1, 1, 3, 5, 16, dtype, 17)
+        for t in (q, k, v):
+            t.requires_grad_()
+        o = window_attention(q, k, v, 2, 1)
+        got = (o, *torch.autograd.grad(o, (q, k, v), do))
+        want, bounds = window_attention64(q, k, v, do, 2, 1, 0.25)
+        for g, w, e, name in zip(got, want, bounds, ("o", "dq", "dk", "dv"), strict=True):
+            assert_within(g, w, e, name)
+
+
+@pytest.mark.gpu
 def test_side_stream_and_once_differentiable(gpu) -> None:
     q, k, v, do = _qkv(1, 4, 2, 500, 500, 64, torch.float16, 15)
     want = window_attention(q, k, v, 100, 4)
@@ -275,8 +302,13 @@ def test_side_stream_and_once_differentiable(gpu) -> None:
     assert torch.equal(got, want)
     args = [t.clone().requires_grad_() for t in (q, k, v)]
     (g,) = torch.autograd.grad(window_attention(*args, 100, 4), args[:1], do.requires_grad_(), create_graph=True)
-    with pytest.raises(RuntimeError):
+    with pytest.raises(RuntimeError, match="once_differentiable"):
         g.sum().backward()
+    # ... and where the gradient is only a part of what is differentiated.
+    args = [t.clone().requires_grad_() for t in (q, k, v)]
+    (g,) = torch.autograd.grad(window_attention(*args, 100, 4), args[:1], do, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        (g.sum() + args[0].sum()).backward()
 
 
 def test_public_name() -> None:

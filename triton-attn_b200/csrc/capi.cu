@@ -460,13 +460,13 @@ extern "C" int tattn_window_bwd(const void* q, const void* k, const void* v, con
                                 const int64_t* strides, int Z, int H, int Hk, int Nq, int Nk, int D, int dtype,
                                 int window, int sinks, float sm_scale, void* stream) {
   if (!strides || !valid_window(Z, H, Hk, Nq, Nk, D, dtype, window, sinks)) return TATTN_ERR_INVALID_ARGUMENT;
-  if (int64_t(Z) * H * Nk == 0) return TATTN_OK;
+  if (int64_t(Z) * Hk * Nk == 0) return TATTN_OK;
   if (!dk || !dv) return TATTN_ERR_INVALID_ARGUMENT;
   DeviceState* st;
   int rc = device_setup(&st);
   if (rc != TATTN_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (Nq == 0) {  // keys that no query sees
+  if (Nq == 0 || H == 0) {  // keys that no query sees
     const size_t bytes = size_t(Z) * Hk * Nk * D * (dtype == TATTN_F16 ? 2 : 4);
     for (void* p : {dk, dv})
       if (cudaMemsetAsync(p, 0, bytes, s) != cudaSuccess) return TATTN_ERR_CUDA;
@@ -540,7 +540,7 @@ extern "C" int64_t tattn_window_bwd_workspace_bytes(int Z, int H, int Hk, int Nq
                                                     int sinks) {
   if (!valid_window(Z, H, Hk, Nq, Nk, D, dtype, window, sinks) || double(Z) * H * Nk * (4.0 * D + 4.0) > 4e17)
     return -1;
-  if (Nq == 0) return 0;
+  if (Nq == 0 || H == 0) return 0;
   const WindowArgs w = window_args(H, Hk, Nq, Nk, window, sinks);
   if (dtype == TATTN_F32)
     return window_part_bytes(kWindowF32Tile, Z, w, D, window_f32_split(Z, w, Nq));

@@ -356,6 +356,7 @@ Tensor decode_attention(const Tensor& q0, const Tensor& k, const Tensor& v, cons
                     "k and v need contiguous, 16-byte aligned rows: a cache is read in place, never copied");
   const Tensor q = rows16(q0), lengths = lengths0.contiguous();
   Tensor o = like(q);
+  if (o.numel() == 0) return o;
   const int z = dim(q, 0), h = dim(q, 1), hk = dim(k, 1), cap = dim(k, 2), d = dim(q, 3);
   const int w = clamp_int(window.value_or(0)), s = clamp_int(sinks);
   Strides st;
@@ -448,6 +449,7 @@ Tensor int4_attend(const Tensor& kc, const Tensor& kp, const Tensor& vc, const T
   require_cuda(q0);
   const Tensor q = rows16(q0), lengths = lengths0.contiguous();
   Tensor o = like(q);
+  if (o.numel() == 0) return o;
   const int z = dim(q, 0), h = dim(q, 1), hk = dim(kc, 1), cap = dim(kc, 2);
   const int w = clamp_int(window.value_or(0)), s = clamp_int(sinks);
   Strides st;

@@ -88,6 +88,9 @@ __device__ __forceinline__ void rows_times(const float* p, const float* b, int t
   }
 }
 
+// The CTA's head among Z * H: the grid's second and third dimension, as one is limited to 65535.
+__device__ __forceinline__ int64_t cta_head() { return int64_t(blockIdx.z) * gridDim.y + blockIdx.y; }
+
 // Does query row `row` of N see key `col`?
 __device__ __forceinline__ bool sees(int row, int col, int N, const WindowArgs& w) {
   const int p = row + w.off;
@@ -106,7 +109,9 @@ __global__ void __launch_bounds__(kThreads) window_fwd_f32_kernel(const float* q
   extern __shared__ __align__(16) float smem[];
   float *Qs = smem, *Ks = Qs + TB * kPitch<D>, *Vs = Ks + TB * kPitch<D>, *Ps = Vs + TB * kPitch<D>;
   const int N = a.N, Nk = a.win.Nk, r0 = blockIdx.x * TB;
-  const int zi = blockIdx.y / a.H, hi = blockIdx.y % a.H, hk = hi / a.win.group;
+  const int64_t head = cta_head();
+  if (head >= int64_t(a.Z) * a.H) return;
+  const int zi = int(head / a.H), hi = int(head % a.H), hk = hi / a.win.group;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   k += zi * sk.z + hk * sk.h;
   v += zi * sv.z + hk * sv.h;
@@ -162,7 +167,7 @@ __global__ void __launch_bounds__(kThreads) window_fwd_f32_kernel(const float* q
     const float inv = 1.f / l[i];
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) o[(D / 16 * tx + e) * a.so.d] = acc[i][e] * inv;
-    if (tx == 0) a.m[int64_t(blockIdx.y) * N + row] = m[i] + log2f(l[i]);
+    if (tx == 0) a.m[head * N + row] = m[i] + log2f(l[i]);
   }
 }
 
@@ -193,7 +198,9 @@ __global__ void __launch_bounds__(kThreads) window_dq_f32_kernel(BwdArgs a) {
   float *Qs = smem, *Os = Qs + TB * kPitch<D>, *Ks = Os + TB * kPitch<D>, *Vs = Ks + TB * kPitch<D>;
   float *DSs = Vs + TB * kPitch<D>, *Ms = DSs + TB * kPitchP, *Ds = Ms + TB;
   const int N = a.N, Nk = a.win.Nk, r0 = blockIdx.x * TB;
-  const int zi = blockIdx.y / a.H, hi = blockIdx.y % a.H, hk = hi / a.win.group;
+  const int64_t head = cta_head();
+  if (head >= int64_t(a.Z) * a.H) return;
+  const int zi = int(head / a.H), hi = int(head % a.H), hk = hi / a.win.group;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const float* k = static_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h;
   const float* v = static_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h;
@@ -201,8 +208,8 @@ __global__ void __launch_bounds__(kThreads) window_dq_f32_kernel(BwdArgs a) {
   load_rows<D>(Os, static_cast<const float*>(a.dout) + zi * a.sdo.z + hi * a.sdo.h, a.sdo, r0, N);
   if (threadIdx.x < TB) {
     const int row = r0 + threadIdx.x;
-    Ms[threadIdx.x] = row < N ? a.m[int64_t(blockIdx.y) * N + row] : 0.f;
-    Ds[threadIdx.x] = row < N ? a.delta[int64_t(blockIdx.y) * N + row] : 0.f;
+    Ms[threadIdx.x] = row < N ? a.m[head * N + row] : 0.f;
+    Ds[threadIdx.x] = row < N ? a.delta[head * N + row] : 0.f;
   }
   float acc[4][D / 16] = {};
   const int end = min(r0 + TB + a.win.off, Nk);
@@ -224,7 +231,7 @@ __global__ void __launch_bounds__(kThreads) window_dq_f32_kernel(BwdArgs a) {
   for (int i = 0; i < 4; ++i) {
     const int row = r0 + 4 * ty + i;
     if (row >= N) continue;
-    float* dq = static_cast<float*>(a.dq) + (int64_t(blockIdx.y) * N + row) * D + D / 16 * tx;
+    float* dq = static_cast<float*>(a.dq) + (head * N + row) * D + D / 16 * tx;
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) dq[e] = acc[i][e] * a.sm_scale;
   }
@@ -240,7 +247,9 @@ __global__ void __launch_bounds__(kThreads) window_dkdv_f32_kernel(BwdArgs a) {
   const int N = a.N, Nk = a.win.Nk;
   const WindowUnit u = window_unit<TB, TB>(a.split, a.win, N, blockIdx.x);
   const int k0 = TB * u.kt;
-  const int zi = blockIdx.y / a.win.Hk, hk = blockIdx.y % a.win.Hk;
+  const int64_t head = cta_head();
+  if (head >= int64_t(a.Z) * a.win.Hk) return;
+  const int zi = int(head / a.win.Hk), hk = int(head % a.win.Hk);
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   load_rows<D>(Ks, static_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h, a.sk, k0, Nk);
   load_rows<D>(Vs, static_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h, a.sv, k0, Nk);
@@ -277,7 +286,7 @@ __global__ void __launch_bounds__(kThreads) window_dkdv_f32_kernel(BwdArgs a) {
     const int key = k0 + 4 * ty + i;
     if (key >= Nk) continue;
     if (u.slot >= 0) {
-      const int64_t slot = int64_t(blockIdx.y) * a.split.slots((Nk + TB - 1) / TB) + u.slot;
+      const int64_t slot = head * a.split.slots((Nk + TB - 1) / TB) + u.slot;
       float* part = a.part + (slot * 2 * TB + 4 * ty + i) * D + D / 16 * tx;
 #pragma unroll
       for (int e = 0; e < D / 16; ++e) {
@@ -286,7 +295,7 @@ __global__ void __launch_bounds__(kThreads) window_dkdv_f32_kernel(BwdArgs a) {
       }
       continue;
     }
-    const int64_t at = (int64_t(blockIdx.y) * Nk + key) * D + D / 16 * tx;
+    const int64_t at = (head * Nk + key) * D + D / 16 * tx;
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) {
       static_cast<float*>(a.dk)[at + e] = dk[i][e] * a.sm_scale;
@@ -315,11 +324,12 @@ __global__ void __launch_bounds__(kThreads) window_join_f32_kernel(BwdArgs a, in
 
 template <typename Kernel, typename... Args>
 cudaError_t launch(Kernel kernel, int tiles, long long heads, int floats, cudaStream_t s, const Args&... args) {
-  if (heads > 65535) return cudaErrorInvalidConfiguration;
+  const long long y = heads < 65535 ? heads : 65535, z = (heads + y - 1) / y;
+  if (z > 65535) return cudaErrorInvalidConfiguration;
   const int smem = floats * 4;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kernel<<<dim3(tiles, unsigned(heads)), kThreads, smem, s>>>(args...);
+  kernel<<<dim3(tiles, unsigned(y), unsigned(z)), kThreads, smem, s>>>(args...);
   return cudaGetLastError();
 }
 
