@@ -2098,27 +2098,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     return true;
   };
 
-  // kMaskWindow: the units of each key/value head (window_unit), those of the sink tiles first; they cost about
-  // the same and are taken round-robin.
-  auto next_window_unit = [&](int2& seq, Unit* u) -> bool {
-    const int per_head = args.split.per_head(nct);
-    if (seq.x >= zh * per_head) return false;
-    const int bh = seq.x / per_head;
-    const WindowUnit w = window_unit<128, BQ>(args.split, args.win, N, seq.x % per_head);
-    seq.x += int(gridDim.x);
-    u->zi = bh / args.win.Hk;
-    u->hk = bh % args.win.Hk;
+  // kMaskWindow: the units in their order (window_unit), from the longest to the shortest, taken round-robin there
+  // and back.
+  auto next_window_unit = [&](int2& seq, Unit* u) -> bool {  // seq = (CTA, first unit of the round)
+    const int p = seq.y + seq.x;
+    if (p >= zh * args.split.per_head(nct)) return false;
+    const WindowUnit w = window_unit<128, BQ>(args.split, args.win, args.Z, N, p);
+    seq = make_int2(int(gridDim.x) - 1 - seq.x, seq.y + int(gridDim.x));
+    u->zi = int(unsigned(w.head) / unsigned(args.win.Hk));
+    u->hk = w.head - u->zi * args.win.Hk;
     u->kt = w.kt;
     u->n = w.n;
     u->lo = w.lo;
     u->nb = w.nb;
     u->h0 = u->hk * args.win.group;
     u->blk0 = w.lo;
-    if (w.start > 0 && w.nb > 0) {
-      u->h0 += w.start / w.nb;
-      u->blk0 += w.start % w.nb;
+    if (w.start > 0) {
+      const int heads = int(unsigned(w.start) / unsigned(w.nb));
+      u->h0 += heads;
+      u->blk0 += w.start - heads * w.nb;
     }
-    u->slot = w.slot < 0 ? -1 : bh * args.split.slots(nct) + w.slot;
+    u->slot = w.slot < 0 ? -1 : w.head * args.split.slots(nct) + w.slot;
     return true;
   };
   auto next_unit = [&](int2& seq, Unit* u) -> bool {
@@ -2380,7 +2380,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int g = 0, it = 0;
     bool ok = true;
     int2 seq = make_int2(int(blockIdx.x), 0);
-    for (Unit u; ok && next_unit(seq, &u); ++it) {
+    Unit u, following;
+    for (bool more = next_unit(seq, &u); ok && more; ++it, u = following) {
       const int zi = u.zi, k0 = 128 * u.kt, n = u.n;
       const int key = k0 + r;
       UnitWalk<WINDOW> at(u);
@@ -2446,6 +2447,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         prev_h = at.h;
         prev_blk = at.blk;
       }
+      more = next_unit(seq, &following);  // worked out while the unit's last MMAs run
       if (!ok || !warp_wait(bar_acc_done, it & 1, ab)) { ok = false; break; }
       // ---- epilogue: the last block's dQ part, then dV (warpgroup 0) or dK * sm_scale (warpgroup 1)
       tc_fence_after();

@@ -403,8 +403,8 @@ bool valid_window(int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int wi
 }
 
 // The fp32 kernel has two CTAs an SM.
-WindowSplit window_f32_split(int Z, const WindowArgs& w, int Nq) {
-  return window_split(kWindowF32Tile, kWindowF32Tile, Z, w, Nq, 2 * device_sm_count());
+WindowSplit window_f32_split(int Z, const WindowArgs& w, int Nq, int D) {
+  return window_split(kWindowF32Tile, kWindowF32Tile, Z, w, Nq, D, 2 * device_sm_count());
 }
 
 // Windows and sinks longer than the keys say no more than the keys themselves.
@@ -500,7 +500,7 @@ extern "C" int tattn_window_bwd(const void* q, const void* k, const void* v, con
   a.wait_limit_ns = g_wait_limit_ns.load();
   a.win = window_args(H, Hk, Nq, Nk, window, sinks);
   if (dtype == TATTN_F32) {
-    a.split = window_f32_split(Z, a.win, Nq);
+    a.split = window_f32_split(Z, a.win, Nq, D);
     if (window_part_bytes(kWindowF32Tile, Z, a.win, D, a.split) > 0) {
       if (!workspace) return TATTN_ERR_INVALID_ARGUMENT;
       if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return TATTN_ERR_LAYOUT;
@@ -518,7 +518,7 @@ extern "C" int tattn_window_bwd(const void* q, const void* k, const void* v, con
   a.dq_acc = static_cast<float*>(workspace);
   char* after = static_cast<char*>(workspace) + int64_t(Z) * H * Nq * D * 4;
   a.grid_sync = reinterpret_cast<unsigned*>(after);
-  a.split = window_split(128, bwd_fused_query_rows(D), Z, a.win, Nq, device_sm_count());
+  a.split = window_split(128, bwd_fused_query_rows(D), Z, a.win, Nq, D, device_sm_count());
   a.part = window_part_bytes(128, Z, a.win, D, a.split) > 0 ? reinterpret_cast<float*>(after + 16) : nullptr;
   CUtensorMap tq, tk, tv, tdo, tdk, tdv, tdqacc;
   const int q_rows = bwd_fused_query_rows(D), acc_cols = D == 128 ? 32 : D / 2;  // as tattn_bwd_fused
@@ -543,9 +543,9 @@ extern "C" int64_t tattn_window_bwd_workspace_bytes(int Z, int H, int Hk, int Nq
   if (Nq == 0 || H == 0) return 0;
   const WindowArgs w = window_args(H, Hk, Nq, Nk, window, sinks);
   if (dtype == TATTN_F32)
-    return window_part_bytes(kWindowF32Tile, Z, w, D, window_f32_split(Z, w, Nq));
+    return window_part_bytes(kWindowF32Tile, Z, w, D, window_f32_split(Z, w, Nq, D));
   return bwd_fused_workspace_bytes(Z, H, Nq, D) +
-         window_part_bytes(128, Z, w, D, window_split(128, bwd_fused_query_rows(D), Z, w, Nq, device_sm_count()));
+         window_part_bytes(128, Z, w, D, window_split(128, bwd_fused_query_rows(D), Z, w, Nq, D, device_sm_count()));
 }
 
 extern "C" int64_t tattn_bwd_fused_workspace_bytes(int Z, int H, int N, int D) {

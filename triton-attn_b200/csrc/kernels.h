@@ -43,13 +43,17 @@ struct FwdArgs {
 };
 
 // Window backward: its units of work. A key tile of a key/value head meets the query blocks that see it, once
-// for each query head of the group: a run of (head, block) pairs, head by head, which is cut into units of at
-// most `len` pairs. The `tiles` first key tiles hold sinks, which all later queries see: sink_units units each;
-// the others are seen by one window of queries: `units` each. A tile of several units is the sum of fp32
-// partials, added up in the units' order.
+// for each query head of the group: a run of (head, block) pairs, head by head, which is cut into equal units.
+// The `tiles` first key tiles hold sinks, which all later queries see: sink_units units each; the others are seen
+// by one window of queries: `units` each. A tile of several units is the sum of fp32 partials, added up in the
+// units' order.
+//
+// The units' order: `heads` heads at a time, first each head's tiles that meet a whole window of queries (those
+// of the sinks first), then the tiles whose window the first query (`before` of them) or the last one cuts short
+// (from tile `last` on), for all heads at once from the longest to the shortest.
 struct WindowSplit {
-  int len;
   int tiles, sink_units, units;
+  int before, last, heads;
   __host__ __device__ int per_head(int key_tiles) const { return tiles * sink_units + (key_tiles - tiles) * units; }
   // Partials of a head: of every unit, of those of the sink tiles, or none.
   __host__ __device__ int slots(int key_tiles) const {
@@ -57,29 +61,52 @@ struct WindowSplit {
   }
 };
 
-// Unit p of a key/value head (key tiles of TILE rows, query blocks of BQ): pairs [start, start + n) of key tile
-// kt's run over the blocks [lo, lo + nb) of each head. n may be 0: the queries begin after the tile's window,
-// or the tile's run is shorter than others'.
+// Unit p of all heads: part `piece` of key tile kt (of TILE rows) of key/value head `head`, which is pairs
+// [start, start + n) of the tile's run over the query blocks (of BQ) [lo, lo + nb) of each query head.
 struct WindowUnit {
-  int kt, lo, nb, start, n;
-  int slot;  // its partial in the head, or -1: it is the whole tile
+  int head;
+  int kt, lo, nb;
+  int start, n;  // n may be 0: the queries begin after the tile's window
+  int slot;      // its partial in the head, or -1: it is the whole tile
 };
 template <int TILE, int BQ>
-__host__ __device__ inline WindowUnit window_unit(const WindowSplit& s, const WindowArgs& w, int N, int p) {
-  const bool sink = p < s.tiles * s.sink_units;
-  const int rest = p - s.tiles * s.sink_units, count = sink ? s.sink_units : s.units;
-  const int piece = sink ? p % s.sink_units : rest % s.units;
+__host__ __device__ inline WindowUnit window_unit(const WindowSplit& s, const WindowArgs& w, int Z, int N, unsigned p) {
+  using u32 = unsigned;  // unsigned 32-bit divisions: they stand between one unit and the next
+  const u32 key_tiles = u32(w.Nk + TILE - 1) / TILE, sink_part = s.tiles * s.sink_units;
+  const u32 set = p / (s.per_head(key_tiles) * s.heads), rest = p - set * s.per_head(key_tiles) * s.heads;
+  const u32 first = set * s.heads, left = u32(Z) * w.Hk - first, heads = left < u32(s.heads) ? left : s.heads;
+  const u32 whole = sink_part + (s.last - s.before - s.tiles) * s.units;
+  u32 head, kt, piece;
+  if (rest < heads * whole) {
+    head = rest / whole;
+    const u32 i = rest - head * whole;
+    const bool sink = i < sink_part;
+    const u32 j = sink ? i : i - sink_part, count = sink ? s.sink_units : s.units;
+    kt = j / count;
+    piece = j - kt * count;
+    if (!sink) kt += s.tiles + s.before;
+  } else {
+    const u32 tail = rest - heads * whole, rank = tail / (heads * s.units), i = tail - rank * heads * s.units;
+    head = i / s.units;
+    piece = i - head * s.units;
+    const u32 after = key_tiles - s.last, both = 2 * (after < u32(s.before) ? after : s.before);
+    const bool late = rank < both ? rank % 2 == 0 : after > u32(s.before);  // the two ends' tiles in turn
+    const u32 j = rank < both ? rank / 2 : rank - both / 2;
+    kt = late ? s.last + j : s.tiles + s.before - 1 - j;
+  }
   WindowUnit u;
-  u.kt = sink ? p / s.sink_units : s.tiles + rest / s.units;
-  const int k0 = TILE * u.kt, blocks = (N + BQ - 1) / BQ;
+  u.head = first + head;
+  u.kt = kt;
+  const bool sink = u.kt < s.tiles;
+  const int k0 = TILE * u.kt, blocks = int(u32(N + BQ - 1) / BQ), count = sink ? s.sink_units : s.units;
   const int last = k0 + TILE - 2 + w.window - w.off;  // the last query that sees the tile's last key
   const int end = sink ? blocks : last < 0 ? 0 : (last / BQ + 1 < blocks ? last / BQ + 1 : blocks);
   u.lo = (k0 > w.off ? k0 - w.off : 0) / BQ;
   u.nb = end > u.lo ? end - u.lo : 0;
-  u.start = piece * s.len;
-  const int left = u.nb * w.group - u.start;
-  u.n = left < 0 ? 0 : left < s.len ? left : s.len;
-  u.slot = count > 1 ? p : -1;
+  const u32 pairs = u32(u.nb) * w.group, each = pairs / count, more = pairs - each * count;
+  u.start = each * piece + (piece < more ? piece : more);
+  u.n = each + (piece < more ? 1 : 0);
+  u.slot = count > 1 ? (sink ? 0 : s.tiles * (s.sink_units - s.units)) + u.kt * count + int(piece) : -1;
   return u;
 }
 
@@ -152,7 +179,7 @@ inline int64_t bwd_fused_workspace_bytes(int Z, int H, int N, int D) { return in
 // written and read again. Backward with B4 H16 Hk4 N4096 D64, window 1024: 286 us in whole tiles of 40 blocks,
 // 333 in halves; B1 H16 Hk4, 4096 queries of 16384 tokens, window 4096: 490 us in whole tiles of 132, 430 in
 // quarters; B2 H16 Hk4 N2500 D128, window 777: within 5 % from 16 blocks to whole tiles.)
-inline WindowSplit window_split(int tile, int bq, int Z, const WindowArgs& w, int N, int workers) {
+inline WindowSplit window_split(int tile, int bq, int Z, const WindowArgs& w, int N, int D, int workers) {
   const int64_t blocks = (N + bq - 1) / bq, key_tiles = (w.Nk + tile - 1) / tile, tiles = (w.sinks + tile - 1) / tile;
   const int64_t span = (int64_t(w.window) + tile - 1 + bq - 1) / bq + 1, one = span < blocks ? span : blocks;
   const int64_t unseen = (w.off > w.window ? w.off - w.window : 0) / tile;  // tiles before every query's window
@@ -166,7 +193,16 @@ inline WindowSplit window_split(int tile, int bq, int Z, const WindowArgs& w, in
   const int64_t cut = (w.group * one + len - 1) / len;  // equal parts of a tile without sinks
   if (cut > 0) len = (w.group * one + cut - 1) / cut > least ? (w.group * one + cut - 1) / cut : least;
   auto units = [&](int64_t pairs) { return int((pairs + len - 1) / len > 0 ? (pairs + len - 1) / len : 1); };
-  return WindowSplit{int(len), int(tiles), units(w.group * blocks), units(w.group * one)};
+  // Tiles [tiles, tiles + before) begin before the first query; the window of those from `last` on ends behind
+  // the last one.
+  const int64_t cut_low = w.off > 0 ? (w.off + tile - 1) / tile - tiles : 0, before = cut_low > 0 ? cut_low : 0;
+  const int64_t room = int64_t(w.Nk) - w.window - tile + 2, high = room > 0 ? (room + tile - 1) / tile : 0;
+  const int64_t last = high < tiles + before ? tiles + before : high < key_tiles ? high : key_tiles;
+  // Heads whose short tiles run together share L2 with their Q and dO rows and (fp16) their dQ sums: 64 MB of
+  // them at most.
+  const int64_t rows = N < w.window ? N : w.window, bytes = rows * w.group * D * 8, fit = (int64_t(64) << 20) / (bytes > 0 ? bytes : 1);
+  const int64_t zh = int64_t(Z) * w.Hk < 65536 ? int64_t(Z) * w.Hk : 65536, heads = fit < 1 ? 1 : fit < zh ? fit : zh;
+  return WindowSplit{int(tiles), units(w.group * blocks), units(w.group * one), int(before), int(last), int(heads > 0 ? heads : 1)};
 }
 constexpr int kWindowF32Tile = 64;  // rows of a tile of the fp32 window kernels
 // The partials: fp32 [Z * Hk, slots, 2 (dV, dK), tile, D].

@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kThreads) window_dq_f32_kernel(BwdArgs a) {
   }
 }
 
-// One unit of a key/value head (window_unit): a key tile, summed over the query heads that share it, or a part of
+// One unit (window_unit): a key tile of a key/value head, summed over the query heads that share it, or a part of
 // that sum.
 template <int D>
 __global__ void __launch_bounds__(kThreads) window_dkdv_f32_kernel(BwdArgs a) {
@@ -245,10 +245,10 @@ __global__ void __launch_bounds__(kThreads) window_dkdv_f32_kernel(BwdArgs a) {
   float *Ks = smem, *Vs = Ks + TB * kPitch<D>, *Qs = Vs + TB * kPitch<D>, *Os = Qs + TB * kPitch<D>;
   float *Ps = Os + TB * kPitch<D>, *DSs = Ps + TB * kPitchP, *Ms = DSs + TB * kPitchP, *Ds = Ms + TB;
   const int N = a.N, Nk = a.win.Nk;
-  const WindowUnit u = window_unit<TB, TB>(a.split, a.win, N, blockIdx.x);
+  if (cta_head() >= int64_t(a.Z) * a.win.Hk) return;
+  const WindowUnit u = window_unit<TB, TB>(a.split, a.win, a.Z, N, unsigned(cta_head() * gridDim.x + blockIdx.x));
   const int k0 = TB * u.kt;
-  const int64_t head = cta_head();
-  if (head >= int64_t(a.Z) * a.win.Hk) return;
+  const int64_t head = u.head;
   const int zi = int(head / a.win.Hk), hk = int(head % a.win.Hk);
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   load_rows<D>(Ks, static_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h, a.sk, k0, Nk);
