@@ -113,20 +113,22 @@ TATTN_API int64_t tattn_bwd_fused_workspace_bytes(int Z, int H, int N, int D);
  * + i of a sequence of Nk >= Nq tokens and sees the keys j <= p that are among the last `window` ones (j >
  * p - window, window >= 1) or the first `sinks` (j < sinks, sinks >= 0); every query sees its own key. K and V
  * have Hk heads, each shared by H / Hk consecutive query heads (Hk divides H).
- * strides: 16 int64 = q, k, v, o each (z, h, n, d). m: dense fp32 [Z, H, Nq]. */
-TATTN_API int tattn_window_fwd(const void* q, const void* k, const void* v, void* o, float* m, const int64_t* strides,
-                     int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window, int sinks, float sm_scale,
-                     void* stream);
+ * strides: 16 int64 = q, k, v, o each (z, h, n, d). m: dense fp32 [Z, H, Nq]. o_rest: null, or for a backward pass
+ * in fp16 Z * H * Nq * D bytes, 16-byte aligned, that hold for it what rounding o to fp16 took off (fp32: unused). */
+TATTN_API int tattn_window_fwd(const void* q, const void* k, const void* v, void* o, float* m, void* o_rest,
+                     const int64_t* strides, int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window,
+                     int sinks, float sm_scale, void* stream);
 
-/* Its backward: delta = rowsum(dO * O), dq [Z, H, Nq, D], and dk, dv [Z, Hk, Nk, D], summed over the query heads
+/* Its backward: delta = rowsum(dO * O) (with o_rest, the forward's, of O before its rounding: where a query sees few
+ * keys, that rounding would be most of the gradients' error), dq [Z, H, Nq, D], and dk, dv [Z, Hk, Nk, D], summed over the query heads
  * that share a head; all dense. strides: 20 int64 = q, k, v, o, dout each (z, h, n, d). delta: fp32 [Z, H,
  * Nq]. workspace: tattn_window_bwd_workspace_bytes bytes, 16-byte aligned (0 bytes: may be null). fp16
  * sums dq by fp32 additions in the workspace in an order that varies from run to run, as tattn_bwd_fused;
  * dk and dv, and everything in fp32, are bitwise reproducible. */
 TATTN_API int tattn_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, void* dq,
-                     void* dk, void* dv, const float* m, float* delta, void* workspace, const int64_t* strides,
-                     int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window, int sinks, float sm_scale,
-                     void* stream);
+                     void* dk, void* dv, const float* m, const void* o_rest, float* delta, void* workspace,
+                     const int64_t* strides, int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window,
+                     int sinks, float sm_scale, void* stream);
 
 /* Bytes of the workspace that tattn_window_bwd needs on the current device, or -1 for invalid arguments. */
 TATTN_API int64_t tattn_window_bwd_workspace_bytes(int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window,

@@ -414,9 +414,9 @@ WindowArgs window_args(int H, int Hk, int Nq, int Nk, int window, int sinks) {
 
 }  // namespace
 
-extern "C" int tattn_window_fwd(const void* q, const void* k, const void* v, void* o, float* m, const int64_t* strides,
-                                int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window, int sinks,
-                                float sm_scale, void* stream) {
+extern "C" int tattn_window_fwd(const void* q, const void* k, const void* v, void* o, float* m, void* o_rest,
+                                const int64_t* strides, int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int window,
+                                int sinks, float sm_scale, void* stream) {
   if (!strides || !valid_window(Z, H, Hk, Nq, Nk, D, dtype, window, sinks)) return TATTN_ERR_INVALID_ARGUMENT;
   if (int64_t(Z) * H * Nq == 0) return TATTN_OK;
   if (!q || !k || !v || !o || !m) return TATTN_ERR_INVALID_ARGUMENT;
@@ -441,8 +441,9 @@ extern "C" int tattn_window_fwd(const void* q, const void* k, const void* v, voi
     return cuda_rc(launch_window_fwd_f32(D, q, k, v, sq, sk, sv, a, s));
   }
   if (!layout_ok(q, sq, Z, H, Nq, D) || !layout_ok(k, sk, Z, Hk, Nk, D) || !layout_ok(v, sv, Z, Hk, Nk, D) ||
-      !layout_ok(o, so, Z, H, Nq, D))
+      !layout_ok(o, so, Z, H, Nq, D) || (reinterpret_cast<uintptr_t>(o_rest) & 15u) != 0)
     return TATTN_ERR_LAYOUT;
+  a.o_rest = static_cast<uint8_t*>(o_rest);
   a.so = normalize(so, Z, H, Nq, D);
   // Positive, so that a hidden score stays -infinity; below 2^-60 scores vanish against 1 anyway.
   a.qk_scale = std::max((sm_scale < 0.f ? -sm_scale : sm_scale) * kLog2e, 0x1p-60f);
@@ -456,9 +457,9 @@ extern "C" int tattn_window_fwd(const void* q, const void* k, const void* v, voi
 }
 
 extern "C" int tattn_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
-                                void* dq, void* dk, void* dv, const float* m, float* delta, void* workspace,
-                                const int64_t* strides, int Z, int H, int Hk, int Nq, int Nk, int D, int dtype,
-                                int window, int sinks, float sm_scale, void* stream) {
+                                void* dq, void* dk, void* dv, const float* m, const void* o_rest, float* delta,
+                                void* workspace, const int64_t* strides, int Z, int H, int Hk, int Nq, int Nk, int D,
+                                int dtype, int window, int sinks, float sm_scale, void* stream) {
   if (!strides || !valid_window(Z, H, Hk, Nq, Nk, D, dtype, window, sinks)) return TATTN_ERR_INVALID_ARGUMENT;
   if (int64_t(Z) * Hk * Nk == 0) return TATTN_OK;
   if (!dk || !dv) return TATTN_ERR_INVALID_ARGUMENT;
@@ -513,8 +514,9 @@ extern "C" int tattn_window_bwd(const void* q, const void* k, const void* v, con
       !layout_ok(o, a.so, Z, H, Nq, D) || !layout_ok(dout, a.sdo, Z, H, Nq, D))
     return TATTN_ERR_LAYOUT;
   for (const void* p : {static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv),
-                        static_cast<const void*>(workspace)})
+                        static_cast<const void*>(workspace), o_rest})
     if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0) return TATTN_ERR_LAYOUT;
+  a.o_rest = static_cast<const uint8_t*>(o_rest);
   a.dq_acc = static_cast<float*>(workspace);
   char* after = static_cast<char*>(workspace) + int64_t(Z) * H * Nq * D * 4;
   a.grid_sync = reinterpret_cast<unsigned*>(after);

@@ -26,6 +26,9 @@
 // ends the other computes; their exponent passes take no turns.
 // The running max is rescaled lazily: O (in TMEM) and l are only corrected when a row's max grows by
 // more than kRescaleThreshold (log2 units); P values stay below 2^kRescaleThreshold, exact in fp16.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "tiles.h"
@@ -218,6 +221,14 @@ __device__ __forceinline__ float exp_cols(const uint32_t* s, uint32_t* p, uint64
   }
   const float2 t = f2_unpack(fadd2(acc0, acc1));
   return t.x + t.y;
+}
+
+// The rests (kRestScale) of two values of O, o[0] and o[1] times inv_l, which were rounded to `h`.
+__device__ __forceinline__ uint32_t rest_of(const uint32_t* o, uint32_t h, float inv_l) {
+  const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return __nv_cvt_float2_to_fp8x2(make_float2((__uint_as_float(o[0]) * inv_l - r.x) * kRestScale,
+                                              (__uint_as_float(o[1]) * inv_l - r.y) * kRestScale),
+                                  __NV_SATFINITE, __NV_E5M2);
 }
 
 template <int D, int MASK, int BN_, int NS_, int TILES>
@@ -544,6 +555,16 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
           uint4* dst = reinterpret_cast<uint4*>(orow + c0);
 #pragma unroll
           for (int v = 0; v < W / 8; ++v) dst[v] = make_uint4(h[4 * v], h[4 * v + 1], h[4 * v + 2], h[4 * v + 3]);
+        }
+        if (WINDOW && args.o_rest != nullptr && row < N) {
+          uint32_t rest[W / 4];
+#pragma unroll
+          for (int c = 0; c < W; c += 4)
+            rest[c / 4] = rest_of(o + c, h[c / 2], inv_l) | (rest_of(o + c + 2, h[c / 2 + 1], inv_l) << 16);
+          uint4* dst = reinterpret_cast<uint4*>(args.o_rest + (int64_t(bh_e) * N + row) * D + c0);
+#pragma unroll
+          for (int v = 0; v < W / 16; ++v)
+            dst[v] = make_uint4(rest[4 * v], rest[4 * v + 1], rest[4 * v + 2], rest[4 * v + 3]);
         }
       }
       if (row < N) args.m[int64_t(bh_e) * N + row] = m_run + log2f(l_run);

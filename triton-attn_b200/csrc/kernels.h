@@ -30,6 +30,11 @@ struct WindowArgs {
   int sinks;      // 0 <= sinks <= Nk
 };
 
+// What rounding the window forward's O to fp16 took off, times kRestScale, as 8-bit floats of 5 exponent bits (the
+// upper byte of an fp16): a rest is half a unit in O's last place at most, so the scale keeps the rests of all
+// finite O, the subnormal ones included, in range, and 2 mantissa bits leave an eighth of it.
+constexpr float kRestScale = 2048.f;
+
 struct FwdArgs {
   void* o;           // [Z, H, N, D], strides `so`
   float* m;          // [Z, H, N] dense fp32: rowmax + log2(rowsum), base-2 units
@@ -40,6 +45,7 @@ struct FwdArgs {
   int* status;       // device status word
   unsigned long long wait_limit_ns;  // bound of every mbarrier wait (tattn_set_wait_limit_ns)
   WindowArgs win;    // kMaskWindow only
+  uint8_t* o_rest;   // kMaskWindow in fp16: what rounding O took off (kRestScale), dense [Z, H, N, D], or null
 };
 
 // Window backward: its units of work. A key tile of a key/value head meets the query blocks that see it, once
@@ -126,6 +132,7 @@ struct BwdArgs {
   int negate_s;
   int* status;
   unsigned long long wait_limit_ns;  // bound of every mbarrier wait (tattn_set_wait_limit_ns)
+  const uint8_t* o_rest;  // kMaskWindow in fp16: the forward's, or null
   WindowArgs win;    // kMaskWindow only: dk and dv are then dense [Z, win.Hk, win.Nk, D]
   WindowSplit split; // kMaskWindow
   float* part;       // kMaskWindow: partial dV and dK of the tiles of several units, or null

@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) bwd_dkdv_f32_kernel(BwdArgs a, b
 
 // delta[bh, i] = sum_d O[i, d] * dO[i, d] in fp32 (reference: _bwd_preprocess, kernels.py:324-337).
 // L lanes cooperate on one row with 16-byte loads; rows need a unit D stride and 16-byte alignment.
-// With a.dq_acc set (fused backward) the row's fp32 dQ workspace is zeroed as well.
+// With a.o_rest set, O is the fp16 values plus the rests. With a.dq_acc set (fused backward) the row's fp32 dQ workspace is zeroed as well.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) preprocess_kernel(BwdArgs a) {
   constexpr int VEC = 16 / sizeof(T);  // elements per 16-byte load
@@ -306,6 +306,18 @@ __global__ void __launch_bounds__(256) preprocess_kernel(BwdArgs a) {
         const float2 of = __half22float2(oh[e]), gf = __half22float2(gh[e]);
         acc = fmaf(of.x, gf.x, acc);
         acc = fmaf(of.y, gf.y, acc);
+      }
+      if (a.o_rest != nullptr) {  // 8 rests, each the upper byte of an fp16
+        const uint2 rv = __ldg(reinterpret_cast<const uint2*>(a.o_rest + row_g * D) + sub);
+        float rest = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t two = __byte_perm(e < 2 ? rv.x : rv.y, 0u, e % 2 ? 0x3424 : 0x1404);
+          const float2 rf = __half22float2(*reinterpret_cast<const __half2*>(&two)), gf = __half22float2(gh[e]);
+          rest = fmaf(rf.x, gf.x, rest);
+          rest = fmaf(rf.y, gf.y, rest);
+        }
+        acc = fmaf(rest, 1.f / kRestScale, acc);
       }
     } else {
       const float* of = reinterpret_cast<const float*>(&ov);

@@ -255,12 +255,14 @@ double scale_of(const std::optional<double>& sm_scale, const Tensor& q) {
   return sm_scale.has_value() ? *sm_scale : 1.0 / std::sqrt(double(q.size(3)));
 }
 
-// (O like q, M fp32 [Z, H, Nq]) of checked tensors.
-std::tuple<Tensor, Tensor> window_forward(const Tensor& q0, const Tensor& k0, const Tensor& v0, int64_t window, int64_t sinks,
-                                          double scale) {
+// (O like q, M fp32 [Z, H, Nq]) of checked tensors and, in fp16 with `rest`, what rounding took off O, for a
+// backward pass (else an undefined tensor).
+std::tuple<Tensor, Tensor, Tensor> window_forward_rest(const Tensor& q0, const Tensor& k0, const Tensor& v0, int64_t window,
+                                                       int64_t sinks, double scale, bool rest) {
   const bool half = q0.scalar_type() == at::kHalf;
   const Tensor q = half ? tma_ready(q0) : q0, k = half ? tma_ready(k0) : k0, v = half ? tma_ready(v0) : v0;
-  Tensor o = like(q), m = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+  Tensor o = like(q), m = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat)), o_rest;
+  if (rest && half) o_rest = at::empty(q.sizes(), q.options().dtype(at::kByte), at::MemoryFormat::Contiguous);
   Strides st;
   st.add(q);
   st.add(k);
@@ -268,16 +270,22 @@ std::tuple<Tensor, Tensor> window_forward(const Tensor& q0, const Tensor& k0, co
   st.add(o);
   const c10::cuda::CUDAGuard guard(q.device());
   check_status("tattn_window_fwd",
-               tattn_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), m.data_ptr<float>(), st.s, dim(q, 0),
-                                dim(q, 1), dim(k, 1), dim(q, 2), dim(k, 2), dim(q, 3), code(q), clamp_int(window),
+               tattn_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), m.data_ptr<float>(),
+                                o_rest.defined() ? o_rest.data_ptr() : nullptr, st.s, dim(q, 0), dim(q, 1), dim(k, 1),
+                                dim(q, 2), dim(k, 2), dim(q, 3), code(q), clamp_int(window),
                                 clamp_int(sinks), float(scale), stream_of(q)));
+  return {o, m, o_rest};
+}
+std::tuple<Tensor, Tensor> window_forward(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks,
+                                          double scale) {
+  const auto [o, m, rest] = window_forward_rest(q, k, v, window, sinks, scale, false);
   return {o, m};
 }
 
-// Dense (dq, dk, dv).
-std::tuple<Tensor, Tensor, Tensor> window_backward(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& o0,
-                                                   const Tensor& m, const Tensor& do0, int64_t window, int64_t sinks,
-                                                   double scale) {
+// Dense (dq, dk, dv); rest: the forward's, or undefined.
+std::tuple<Tensor, Tensor, Tensor> window_backward_rest(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& o0,
+                                                        const Tensor& m, const Tensor& rest, const Tensor& do0,
+                                                        int64_t window, int64_t sinks, double scale) {
   const bool half = q0.scalar_type() == at::kHalf;
   const Tensor dout = do0.to(q0.scalar_type());
   const Tensor q = half ? tma_ready(q0) : q0, k = half ? tma_ready(k0) : k0, v = half ? tma_ready(v0) : v0;
@@ -297,17 +305,22 @@ std::tuple<Tensor, Tensor, Tensor> window_backward(const Tensor& q0, const Tenso
   const Tensor ws = bytes(std::max<int64_t>(0, tattn_window_bwd_workspace_bytes(z, h, hk, n, nk, d, code(q), w, s)), q);
   check_status("tattn_window_bwd",
                tattn_window_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), g.data_ptr(), dq.data_ptr(),
-                                dk.data_ptr(), dv.data_ptr(), m.data_ptr<float>(), delta.data_ptr<float>(), ws.data_ptr(), st.s,
-                                z, h, hk, n, nk, d, code(q), w, s, float(scale), stream_of(q)));
+                                dk.data_ptr(), dv.data_ptr(), m.data_ptr<float>(), rest.defined() ? rest.data_ptr() : nullptr,
+                                delta.data_ptr<float>(), ws.data_ptr(), st.s, z, h, hk, n, nk, d, code(q), w, s, float(scale), stream_of(q)));
   return {dq, dk, dv};
+}
+std::tuple<Tensor, Tensor, Tensor> window_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o,
+                                                   const Tensor& m, const Tensor& dout, int64_t window, int64_t sinks,
+                                                   double scale) {
+  return window_backward_rest(q, k, v, o, m, Tensor(), dout, window, sinks, scale);
 }
 
 struct WindowAttention : torch::autograd::Function<WindowAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks,
                         double scale) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [o, m] = window_forward(q, k, v, window, sinks, scale);
-    ctx->save_for_backward({q, k, v, o, m});
+    auto [o, m, rest] = window_forward_rest(q, k, v, window, sinks, scale, true);
+    ctx->save_for_backward({q, k, v, o, m, rest});
     ctx->saved_data["window"] = window;
     ctx->saved_data["sinks"] = sinks;
     ctx->saved_data["scale"] = scale;
@@ -319,7 +332,7 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
       at::AutoDispatchBelowADInplaceOrView below;
       const variable_list s = ctx->get_saved_variables();
       std::tie(out[0], out[1], out[2]) =
-          window_backward(s[0], s[1], s[2], s[3], s[4], grads[0], ctx->saved_data["window"].toInt(),
+          window_backward_rest(s[0], s[1], s[2], s[3], s[4], s[5], grads[0], ctx->saved_data["window"].toInt(),
                           ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble());
     }
     return once(std::move(out));

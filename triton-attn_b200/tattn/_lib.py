@@ -32,8 +32,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tattn_bwd_noalloc": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64P, _I, _I, _I, _I, _I, _I, _F, _P]),
     "tattn_bwd_fused": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64P, _I, _I, _I, _I, _I, _I, _F, _P]),
     "tattn_bwd_fused_workspace_bytes": (ctypes.c_int64, [_I, _I, _I, _I]),
-    "tattn_window_fwd": (_I, [*[_P] * 5, _I64P, *[_I] * 9, _F, _P]),
-    "tattn_window_bwd": (_I, [*[_P] * 11, _I64P, *[_I] * 9, _F, _P]),
+    "tattn_window_fwd": (_I, [*[_P] * 6, _I64P, *[_I] * 9, _F, _P]),
+    "tattn_window_bwd": (_I, [*[_P] * 12, _I64P, *[_I] * 9, _F, _P]),
     "tattn_window_bwd_workspace_bytes": (ctypes.c_int64, [_I] * 9),
     "tattn_qk_norm_rope": (_I, [*[_P] * 9, _I64P, *[_I] * 8, _F, _I, _P]),
     "tattn_qk_norm_rope_bwd": (_I, [*[_P] * 14, _I64P, *[_I] * 8, _F, _I, _P]),
