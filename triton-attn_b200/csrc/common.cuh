@@ -351,6 +351,12 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
+// ---- 16 bytes of global memory (zeros where not `valid`: src is then not read) into shared memory, asynchronously
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // ---- packed fp32 pairs (sm_100 f32x2 instructions: one issue slot for two lanes' worth of math)
 __device__ __forceinline__ uint64_t f2(float lo, float hi) {
   uint64_t r;

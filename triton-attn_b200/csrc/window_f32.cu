@@ -5,10 +5,16 @@
 // accuracy. Two kernels for the backward, dK/dV by key tiles and dQ by query tiles, so that nothing is
 // summed by atomics and results are bitwise reproducible.
 //
-// The bound is the FMA pipe (4 D flop forward and 14 D backward a pair) fed from shared memory: 64 x 64 tiles,
-// 256 threads as 16 x 16, and a thread computes 4 x 4 scores (rows 4 ty + i, columns tx + 16 j) from 16-byte
-// reads along D: 8 reads for 64 FMAs, which a warp's broadcasts turn into 12 shared-memory cycles against
-// 16 of the FMA pipes. Then 4 rows x D / 16 columns of the products with V, K, Q and dO the same way.
+// The bound is the FMA pipe (4 D flop forward and 14 D backward a pair) fed from shared memory: 64 x 64 tiles, and a
+// thread computes R x 4 scores (rows R ty + i, columns tx + 16 j) from 16-byte reads along D, then R rows x D / 16
+// columns of the products with V, K, Q and dO the same way. A read that 16 threads share costs 1 to 2 cycles of shared
+// memory and one of 16 different units 4: with R = 4 (256 threads) they outweigh the FMAs (72 % of the cycles against
+// 53 %, dK/dV at B4 H16 N2048 D64, window 512), with R = 8 (128 threads, up to 255 registers) they do not: 580 -> 514 us
+// forward and 1820 -> 1632 backward there; D = 32: 251 -> 220 and 642 -> 549 (B2 H8 N2000, causal). D = 16 has too little
+// to do for 8 rows (13 -> 17 us forward, B2 H8 N500), D = 128 too few registers. The tiles of the next step are on
+// their way while this one's are computed with (cp.async); at 8 to 16 warps an SM what is left is latency: 40 of the
+// FMA pipes' 74 TFLOP/s at the size above, and at B3 H5 N1000, window 200, where 240 tiles make 1.6 CTAs an SM, 17
+// (60 us forward, 175 backward).
 #include <math.h>
 
 #include "common.cuh"
@@ -17,7 +23,11 @@
 namespace tattn {
 namespace {
 
-constexpr int kThreads = 256, TB = kWindowF32Tile;  // threads; rows and columns of a tile
+constexpr int TB = kWindowF32Tile;  // rows and columns of a tile
+template <int D>
+constexpr int kRows = D == 32 || D == 64 ? 8 : 4;  // of a tile, a thread's
+template <int D>
+constexpr int kThreads = 16 * TB / kRows<D>;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Row pitch in floats: 16-byte units a row odd in number, so that 16 rows at one unit are in different banks.
@@ -25,64 +35,75 @@ template <int D>
 constexpr int kPitch = D + 4;
 constexpr int kPitchP = TB + 4;
 
-// Rows [r0, r0 + 64) of a [n, D] matrix into shared memory, 16 bytes at a time where its rows allow; rows past
-// n are zeros.
+// Rows [r0, r0 + 64) of a [n, D] matrix into shared memory, 16 bytes at a time and asynchronously (cp_async_wait) where
+// its rows allow; rows past n are zeros.
 template <int D>
 __device__ __forceinline__ void load_rows(float* dst, const float* src, const Strides4& s, int r0, int n) {
   if (s.d == 1 && s.n % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
 #pragma unroll
-    for (int i = 0; i < TB * D / 4 / kThreads; ++i) {
-      const int e = i * kThreads + threadIdx.x, r = e / (D / 4), d = e % (D / 4) * 4;
-      const float4 x = r0 + r < n ? __ldg(reinterpret_cast<const float4*>(src + int64_t(r0 + r) * s.n + d))
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
-      *reinterpret_cast<float4*>(dst + r * kPitch<D> + d) = x;
+    for (int i = 0; i < TB * D / 4 / kThreads<D>; ++i) {
+      const int e = i * kThreads<D> + threadIdx.x, r = e / (D / 4), d = e % (D / 4) * 4;
+      cp_async16(smem_u32(dst + r * kPitch<D> + d), src + int64_t(min(r0 + r, n - 1)) * s.n + d, r0 + r < n);
     }
     return;
   }
 #pragma unroll 4
-  for (int e = threadIdx.x; e < TB * D; e += kThreads) {
+  for (int e = threadIdx.x; e < TB * D; e += kThreads<D>) {
     const int r = e / D, d = e % D;
     dst[r * kPitch<D> + d] = r0 + r < n ? __ldg(src + int64_t(r0 + r) * s.n + d * s.d) : 0.f;
   }
 }
 
-// c[i][j] += a[4 ty + i] . b[tx + 16 j] over D.
+// c[i][j] = a[R ty + i] . b[tx + 16 j] over D.
 template <int D>
 __device__ __forceinline__ void rows_dot(const float* a, const float* b, int ty, int tx, float (*c)[4]) {
-#pragma unroll 4
-  for (int d = 0; d < D; d += 4) {
-    float4 x[4], y[4];
+  constexpr int R = kRows<D>;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(a + (4 * ty + i) * kPitch<D> + d);
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[i][j] = 0.f;
+#pragma unroll 2
+  for (int d = 0; d < D; d += 4) {
+    float4 x[R], y[4];
+#pragma unroll
+    for (int i = 0; i < R; ++i) x[i] = *reinterpret_cast<const float4*>(a + (R * ty + i) * kPitch<D> + d);
 #pragma unroll
     for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * kPitch<D> + d);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         c[i][j] = fmaf(x[i].w, y[j].w, fmaf(x[i].z, y[j].z, fmaf(x[i].y, y[j].y, fmaf(x[i].x, y[j].x, c[i][j]))));
   }
 }
 
-// acc[i][e] += sum over r of p[4 ty + i][r] b[r][D / 16 tx + e].
+// acc[i][e] += sum over r of p[R ty + i][r] b[r][D / 16 tx + e], two e in a packed FMA.
 template <int D>
 __device__ __forceinline__ void rows_times(const float* p, const float* b, int ty, int tx, float (*acc)[D / 16]) {
-  constexpr int E = D / 16;
+  constexpr int E = D / 16, R = kRows<D>;
 #pragma unroll 2
   for (int r = 0; r < TB; r += 4) {
-    float4 x[4];
+    float4 x[R];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(p + (4 * ty + i) * kPitchP + r);
+    for (int i = 0; i < R; ++i) x[i] = *reinterpret_cast<const float4*>(p + (R * ty + i) * kPitchP + r);
 #pragma unroll
     for (int rr = 0; rr < 4; ++rr) {
       float y[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) y[e] = b[(r + rr) * kPitch<D> + E * tx + e];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < R; ++i) {
         const float w = rr == 0 ? x[i].x : rr == 1 ? x[i].y : rr == 2 ? x[i].z : x[i].w;
+        if constexpr (E == 1) {
+          acc[i][0] = fmaf(w, y[0], acc[i][0]);
+        } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[i][e] = fmaf(w, y[e], acc[i][e]);
+          for (int e = 0; e < E; e += 2) {
+            const float2 f = f2_unpack(ffma2(f2(w, w), f2(y[e], y[e + 1]), f2(acc[i][e], acc[i][e + 1])));
+            acc[i][e] = f.x;
+            acc[i][e + 1] = f.y;
+          }
+        }
       }
     }
   }
@@ -104,8 +125,9 @@ __device__ __forceinline__ int next_key_tile(int k0, int r0, const WindowArgs& w
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads) window_fwd_f32_kernel(const float* q, const float* k, const float* v,
+__global__ void __launch_bounds__(kThreads<D>) window_fwd_f32_kernel(const float* q, const float* k, const float* v,
                                                                   Strides4 sq, Strides4 sk, Strides4 sv, FwdArgs a) {
+  constexpr int R = kRows<D>;
   extern __shared__ __align__(16) float smem[];
   float *Qs = smem, *Ks = Qs + TB * kPitch<D>, *Vs = Ks + TB * kPitch<D>, *Ps = Vs + TB * kPitch<D>;
   const int N = a.N, Nk = a.win.Nk, r0 = blockIdx.x * TB;
@@ -115,29 +137,30 @@ __global__ void __launch_bounds__(kThreads) window_fwd_f32_kernel(const float* q
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   k += zi * sk.z + hk * sk.h;
   v += zi * sv.z + hk * sv.h;
+  int k0 = next_key_tile(-TB, r0, a.win);
   load_rows<D>(Qs, q + zi * sq.z + hi * sq.h, sq, r0, N);
-  float m[4], l[4], acc[4][D / 16];
+  load_rows<D>(Ks, k, sk, k0, Nk);
+  float m[R], l[R], acc[R][D / 16];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < R; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) acc[i][e] = 0.f;
   }
   const int end = min(r0 + TB + a.win.off, Nk);
-  for (int k0 = next_key_tile(-TB, r0, a.win); k0 < end; k0 = next_key_tile(k0, r0, a.win)) {
-    __syncthreads();
-    load_rows<D>(Ks, k, sk, k0, Nk);
+  for (int next; k0 < end; k0 = next) {
+    cp_async_wait_all();
+    __syncthreads();  // K is here, and V's last tile has been read
     load_rows<D>(Vs, v, sv, k0, Nk);
-    __syncthreads();
-    float s[4][4] = {};
+    float s[R][4];
     rows_dot<D>(Qs, Ks, ty, tx, s);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < R; ++i) {
       float mx = m[i];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        s[i][j] = sees(r0 + 4 * ty + i, k0 + tx + 16 * j, N, a.win) ? s[i][j] * a.qk_scale : -INFINITY;
+        s[i][j] = sees(r0 + R * ty + i, k0 + tx + 16 * j, N, a.win) ? s[i][j] * a.qk_scale : -INFINITY;
         mx = fmaxf(mx, s[i][j]);
       }
 #pragma unroll
@@ -151,17 +174,20 @@ __global__ void __launch_bounds__(kThreads) window_fwd_f32_kernel(const float* q
       for (int j = 0; j < 4; ++j) {
         const float p = exp2f(s[i][j] - use);
         l[i] += p;  // this thread's columns
-        Ps[(4 * ty + i) * kPitchP + tx + 16 * j] = p;
+        Ps[(R * ty + i) * kPitchP + tx + 16 * j] = p;
       }
     }
-    __syncwarp();  // a row of P is written and read by the 16 threads of one half warp
+    cp_async_wait_all();
+    __syncthreads();  // V is here, and K has been read
+    next = next_key_tile(k0, r0, a.win);
+    if (next < end) load_rows<D>(Ks, k, sk, next, Nk);
     rows_times<D>(Ps, Vs, ty, tx, acc);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < R; ++i) {
 #pragma unroll
     for (int o = 1; o < 16; o *= 2) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
-    const int row = r0 + 4 * ty + i;
+    const int row = r0 + R * ty + i;
     if (row >= N) continue;
     float* o = static_cast<float*>(a.o) + zi * a.so.z + hi * a.so.h + int64_t(row) * a.so.n;
     const float inv = 1.f / l[i];
@@ -171,21 +197,22 @@ __global__ void __launch_bounds__(kThreads) window_fwd_f32_kernel(const float* q
   }
 }
 
-// P and dS of rows 4 ty + i of A (with C) and rows tx + 16 j of B (with E): A, B are queries and keys, or keys
+// P and dS of rows R ty + i of A (with C) and rows tx + 16 j of B (with E): A, B are queries and keys, or keys
 // and queries (KEYS); C, E their dO and V, or V and dO.
 template <int D, bool KEYS>
 __device__ __forceinline__ void p_ds(const BwdArgs& a, const float* A, const float* B, const float* C, const float* E,
                                      int ty, int tx, int a0, int b0, const float* Ms, const float* Ds, float (*p)[4],
                                      float (*ds)[4]) {
-  float s[4][4] = {}, dp[4][4] = {};
+  constexpr int R = kRows<D>;
+  float s[R][4], dp[R][4];
   rows_dot<D>(A, B, ty, tx, s);
   rows_dot<D>(C, E, ty, tx, dp);
   const float qks = a.sm_scale * kLog2e;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int ra = 4 * ty + i, rb = tx + 16 * j, row = KEYS ? rb : ra;  // the tile's query row
+      const int ra = R * ty + i, rb = tx + 16 * j, row = KEYS ? rb : ra;  // the tile's query row
       const bool see = KEYS ? sees(b0 + rb, a0 + ra, a.N, a.win) : sees(a0 + ra, b0 + rb, a.N, a.win);
       p[i][j] = see ? exp2f(s[i][j] * qks - Ms[row]) : 0.f;
       ds[i][j] = p[i][j] * (dp[i][j] - Ds[row]);
@@ -193,10 +220,12 @@ __device__ __forceinline__ void p_ds(const BwdArgs& a, const float* A, const flo
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads) window_dq_f32_kernel(BwdArgs a) {
+__global__ void __launch_bounds__(kThreads<D>) window_dq_f32_kernel(BwdArgs a) {
+  constexpr int R = kRows<D>;
   extern __shared__ __align__(16) float smem[];
-  float *Qs = smem, *Os = Qs + TB * kPitch<D>, *Ks = Os + TB * kPitch<D>, *Vs = Ks + TB * kPitch<D>;
-  float *DSs = Vs + TB * kPitch<D>, *Ms = DSs + TB * kPitchP, *Ds = Ms + TB;
+  float *Qs = smem, *Os = Qs + TB * kPitch<D>, *Vs = Os + TB * kPitch<D>;
+  float *Ks = Vs + TB * kPitch<D>, *Kn = Ks + TB * kPitch<D>;  // K's tile and the next one
+  float *DSs = Kn + TB * kPitch<D>, *Ms = DSs + TB * kPitchP, *Ds = Ms + TB;
   const int N = a.N, Nk = a.win.Nk, r0 = blockIdx.x * TB;
   const int64_t head = cta_head();
   if (head >= int64_t(a.Z) * a.H) return;
@@ -206,30 +235,37 @@ __global__ void __launch_bounds__(kThreads) window_dq_f32_kernel(BwdArgs a) {
   const float* v = static_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h;
   load_rows<D>(Qs, static_cast<const float*>(a.q) + zi * a.sq.z + hi * a.sq.h, a.sq, r0, N);
   load_rows<D>(Os, static_cast<const float*>(a.dout) + zi * a.sdo.z + hi * a.sdo.h, a.sdo, r0, N);
+  int k0 = next_key_tile(-TB, r0, a.win);
+  load_rows<D>(Ks, k, a.sk, k0, Nk);
+  load_rows<D>(Vs, v, a.sv, k0, Nk);
   if (threadIdx.x < TB) {
     const int row = r0 + threadIdx.x;
     Ms[threadIdx.x] = row < N ? a.m[head * N + row] : 0.f;
     Ds[threadIdx.x] = row < N ? a.delta[head * N + row] : 0.f;
   }
-  float acc[4][D / 16] = {};
+  float acc[R][D / 16] = {};
   const int end = min(r0 + TB + a.win.off, Nk);
-  for (int k0 = next_key_tile(-TB, r0, a.win); k0 < end; k0 = next_key_tile(k0, r0, a.win)) {
-    __syncthreads();
-    load_rows<D>(Ks, k, a.sk, k0, Nk);
-    load_rows<D>(Vs, v, a.sv, k0, Nk);
-    __syncthreads();
-    float p[4][4], ds[4][4];
+  for (int next; k0 < end; k0 = next) {
+    cp_async_wait_all();
+    __syncthreads();  // K and V are here, and K's last tile has been read
+    next = next_key_tile(k0, r0, a.win);
+    if (next < end) load_rows<D>(Kn, k, a.sk, next, Nk);
+    float p[R][4], ds[R][4];
     p_ds<D, false>(a, Qs, Ks, Os, Vs, ty, tx, r0, k0, Ms, Ds, p, ds);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < R; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) DSs[(4 * ty + i) * kPitchP + tx + 16 * j] = ds[i][j];
-    __syncwarp();
+      for (int j = 0; j < 4; ++j) DSs[(R * ty + i) * kPitchP + tx + 16 * j] = ds[i][j];
+    __syncthreads();  // V has been read
+    if (next < end) load_rows<D>(Vs, v, a.sv, next, Nk);
     rows_times<D>(DSs, Ks, ty, tx, acc);
+    float* t = Ks;
+    Ks = Kn;
+    Kn = t;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = r0 + 4 * ty + i;
+  for (int i = 0; i < R; ++i) {
+    const int row = r0 + R * ty + i;
     if (row >= N) continue;
     float* dq = static_cast<float*>(a.dq) + (head * N + row) * D + D / 16 * tx;
 #pragma unroll
@@ -240,10 +276,12 @@ __global__ void __launch_bounds__(kThreads) window_dq_f32_kernel(BwdArgs a) {
 // One unit (window_unit): a key tile of a key/value head, summed over the query heads that share it, or a part of
 // that sum.
 template <int D>
-__global__ void __launch_bounds__(kThreads) window_dkdv_f32_kernel(BwdArgs a) {
+__global__ void __launch_bounds__(kThreads<D>) window_dkdv_f32_kernel(BwdArgs a) {
+  constexpr int R = kRows<D>;
   extern __shared__ __align__(16) float smem[];
-  float *Ks = smem, *Vs = Ks + TB * kPitch<D>, *Qs = Vs + TB * kPitch<D>, *Os = Qs + TB * kPitch<D>;
-  float *Ps = Os + TB * kPitch<D>, *DSs = Ps + TB * kPitchP, *Ms = DSs + TB * kPitchP, *Ds = Ms + TB;
+  float *Ks = smem, *Vs = Ks + TB * kPitch<D>, *Os = Vs + TB * kPitch<D>;
+  float *Qs = Os + TB * kPitch<D>, *Qn = Qs + TB * kPitch<D>;  // Q's tile and the next one
+  float *Ps = Qn + TB * kPitch<D>, *Ms = Ps + TB * kPitchP, *Mn = Ms + 2 * TB;  // M and delta of them
   const int N = a.N, Nk = a.win.Nk;
   if (cta_head() >= int64_t(a.Z) * a.win.Hk) return;
   const WindowUnit u = window_unit<TB, TB>(a.split, a.win, a.Z, N, unsigned(cta_head() * gridDim.x + blockIdx.x));
@@ -253,41 +291,60 @@ __global__ void __launch_bounds__(kThreads) window_dkdv_f32_kernel(BwdArgs a) {
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   load_rows<D>(Ks, static_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h, a.sk, k0, Nk);
   load_rows<D>(Vs, static_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h, a.sv, k0, Nk);
-  float dk[4][D / 16] = {}, dv[4][D / 16] = {};
-  for (int i = u.start; i < u.start + u.n; ++i) {
+  float dk[R][D / 16] = {}, dv[R][D / 16] = {};
+  auto rows_of = [&](const void* x, const Strides4& st, int i, float* to) {  // the tile of pair i
     const int hi = hk * a.win.group + i / u.nb, r0 = (u.lo + i % u.nb) * TB;
-    const float* q = static_cast<const float*>(a.q) + zi * a.sq.z + hi * a.sq.h;
-    const float* dout = static_cast<const float*>(a.dout) + zi * a.sdo.z + hi * a.sdo.h;
-    const int64_t rows = (int64_t(zi) * a.H + hi) * N;
-    __syncthreads();
-    load_rows<D>(Qs, q, a.sq, r0, N);
-    load_rows<D>(Os, dout, a.sdo, r0, N);
+    load_rows<D>(to, static_cast<const float*>(x) + zi * st.z + hi * st.h, st, r0, N);
+  };
+  auto load_q = [&](int i, float* to, float* md) {
+    rows_of(a.q, a.sq, i, to);
     if (threadIdx.x < TB) {
-      const int row = r0 + threadIdx.x;
-      Ms[threadIdx.x] = row < N ? a.m[rows + row] : 0.f;
-      Ds[threadIdx.x] = row < N ? a.delta[rows + row] : 0.f;
+      const int hi = hk * a.win.group + i / u.nb, row = (u.lo + i % u.nb) * TB + threadIdx.x;
+      const int64_t at = (int64_t(zi) * a.H + hi) * N + row;
+      md[threadIdx.x] = row < N ? a.m[at] : 0.f;
+      md[TB + threadIdx.x] = row < N ? a.delta[at] : 0.f;
     }
-    __syncthreads();
-    float p[4][4], ds[4][4];
-    p_ds<D, true>(a, Ks, Qs, Vs, Os, ty, tx, k0, r0, Ms, Ds, p, ds);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        Ps[(4 * ty + i) * kPitchP + tx + 16 * j] = p[i][j];
-        DSs[(4 * ty + i) * kPitchP + tx + 16 * j] = ds[i][j];
-      }
-    __syncwarp();
-    rows_times<D>(Ps, Os, ty, tx, dv);
-    rows_times<D>(DSs, Qs, ty, tx, dk);
+  };
+  const int end = u.start + u.n;
+  if (u.n > 0) {
+    load_q(u.start, Qs, Ms);
+    rows_of(a.dout, a.sdo, u.start, Os);
   }
+  for (int i = u.start; i < end; ++i) {
+    const int r0 = (u.lo + i % u.nb) * TB;
+    cp_async_wait_all();
+    __syncthreads();  // Q and dO are here, and Q's last tile has been read
+    if (i + 1 < end) load_q(i + 1, Qn, Mn);
+    float p[R][4], ds[R][4];
+    p_ds<D, true>(a, Ks, Qs, Vs, Os, ty, tx, k0, r0, Ms, Ms + TB, p, ds);
+    auto put = [&](const float(*x)[4]) {  // a row is written and read by the 16 threads of one half warp
+      __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int key = k0 + 4 * ty + i;
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) Ps[(R * ty + i) * kPitchP + tx + 16 * j] = x[i][j];
+      __syncwarp();
+    };
+    put(p);
+    rows_times<D>(Ps, Os, ty, tx, dv);
+    __syncthreads();  // dO has been read
+    if (i + 1 < end) rows_of(a.dout, a.sdo, i + 1, Os);
+    put(ds);
+    rows_times<D>(Ps, Qs, ty, tx, dk);
+    float *q = Qs, *md = Ms;
+    Qs = Qn;
+    Qn = q;
+    Ms = Mn;
+    Mn = md;
+  }
+  cp_async_wait_all();  // K and V, where no query sees the tile
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int key = k0 + R * ty + i;
     if (key >= Nk) continue;
     if (u.slot >= 0) {
       const int64_t slot = head * a.split.slots((Nk + TB - 1) / TB) + u.slot;
-      float* part = a.part + (slot * 2 * TB + 4 * ty + i) * D + D / 16 * tx;
+      float* part = a.part + (slot * 2 * TB + R * ty + i) * D + D / 16 * tx;
 #pragma unroll
       for (int e = 0; e < D / 16; ++e) {
         part[e] = dv[i][e];
@@ -304,10 +361,12 @@ __global__ void __launch_bounds__(kThreads) window_dkdv_f32_kernel(BwdArgs a) {
   }
 }
 
+constexpr int kJoinThreads = 256;
+
 // dV and dK of the tiles of several units: the sums of the units' partials, in their order.
-__global__ void __launch_bounds__(kThreads) window_join_f32_kernel(BwdArgs a, int D) {
+__global__ void __launch_bounds__(kJoinThreads) window_join_f32_kernel(BwdArgs a, int D) {
   const int key_tiles = (a.win.Nk + TB - 1) / TB, tiles = a.split.units > 1 ? key_tiles : a.split.tiles;
-  const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x, tile = TB * D;
+  const int64_t i = int64_t(blockIdx.x) * kJoinThreads + threadIdx.x, tile = TB * D;
   const int which = int(i / tile % 2);  // 0: dV, 1: dK
   const int64_t t = i / (2 * tile), head = t / tiles;
   const int kt = int(t % tiles), key = kt * TB + int(i % tile / D);
@@ -322,36 +381,36 @@ __global__ void __launch_bounds__(kThreads) window_join_f32_kernel(BwdArgs a, in
   out[(head * a.win.Nk + key) * D + i % D] = which ? sum * a.sm_scale : sum;
 }
 
-template <typename Kernel, typename... Args>
+template <int D, typename Kernel, typename... Args>
 cudaError_t launch(Kernel kernel, int tiles, long long heads, int floats, cudaStream_t s, const Args&... args) {
   const long long y = heads < 65535 ? heads : 65535, z = (heads + y - 1) / y;
   if (z > 65535) return cudaErrorInvalidConfiguration;
   const int smem = floats * 4;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kernel<<<dim3(tiles, unsigned(y), unsigned(z)), kThreads, smem, s>>>(args...);
+  kernel<<<dim3(tiles, unsigned(y), unsigned(z)), kThreads<D>, smem, s>>>(args...);
   return cudaGetLastError();
 }
 
 template <int D>
 cudaError_t fwd_impl(const float* q, const float* k, const float* v, const Strides4& sq, const Strides4& sk,
                      const Strides4& sv, const FwdArgs& a, cudaStream_t s) {
-  return launch(window_fwd_f32_kernel<D>, (a.N + TB - 1) / TB, (long long)a.Z * a.H, TB * (3 * kPitch<D> + kPitchP), s, q, k, v, sq, sk,
+  return launch<D>(window_fwd_f32_kernel<D>, (a.N + TB - 1) / TB, (long long)a.Z * a.H, TB * (3 * kPitch<D> + kPitchP), s, q, k, v, sq, sk,
                 sv, a);
 }
 
 template <int D>
 cudaError_t bwd_impl(const BwdArgs& a, cudaStream_t s) {
   const int key_tiles = (a.win.Nk + TB - 1) / TB;
-  cudaError_t e = launch(window_dkdv_f32_kernel<D>, a.split.per_head(key_tiles), (long long)a.Z * a.win.Hk,
-                         TB * (4 * kPitch<D> + 2 * kPitchP + 2), s, a);
+  cudaError_t e = launch<D>(window_dkdv_f32_kernel<D>, a.split.per_head(key_tiles), (long long)a.Z * a.win.Hk,
+                         TB * (5 * kPitch<D> + kPitchP + 4), s, a);
   if (e != cudaSuccess) return e;
   if (a.split.slots(key_tiles) > 0) {
     const int64_t values = int64_t(a.Z) * a.win.Hk * (a.split.units > 1 ? key_tiles : a.split.tiles) * 2 * TB * D;
-    window_join_f32_kernel<<<unsigned((values + kThreads - 1) / kThreads), kThreads, 0, s>>>(a, D);
+    window_join_f32_kernel<<<unsigned((values + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, s>>>(a, D);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
-  return launch(window_dq_f32_kernel<D>, (a.N + TB - 1) / TB, (long long)a.Z * a.H, TB * (4 * kPitch<D> + kPitchP + 2), s, a);
+  return launch<D>(window_dq_f32_kernel<D>, (a.N + TB - 1) / TB, (long long)a.Z * a.H, TB * (5 * kPitch<D> + kPitchP + 2), s, a);
 }
 
 }  // namespace
