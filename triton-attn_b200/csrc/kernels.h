@@ -181,19 +181,18 @@ __host__ __device__ constexpr int bwd_fused_query_rows(int D) { return D == 128 
 // Workspace of tattn_bwd_fused: the fp32 dQ rows [Z, H, N, D], then 16 bytes for the grid-barrier counter.
 inline int64_t bwd_fused_workspace_bytes(int Z, int H, int N, int D) { return int64_t(Z) * H * N * D * 4 + 16; }
 // Units of about one size for `workers` CTAs that take them in turn: what a tile without sinks costs (one
-// window's blocks for the group) or, where that leaves a CTA fewer than 3 units, a third of its share; 8 blocks at
-// least and at most 64 units a tile. (A unit starts and ends at the cost of about 3 blocks, and partials are
-// written and read again. Backward with B4 H16 Hk4 N4096 D64, window 1024: 286 us in whole tiles of 40 blocks,
-// 333 in halves; B1 H16 Hk4, 4096 queries of 16384 tokens, window 4096: 490 us in whole tiles of 132, 430 in
-// quarters; B2 H16 Hk4 N2500 D128, window 777: within 5 % from 16 blocks to whole tiles.)
+// window's blocks for the group) or, where that is less, a CTA's share; 8 blocks at least and at most 64 units a
+// tile. (A unit starts and ends at the cost of about 2 blocks, and partials are written and read again. Share, half
+// and third of it: B2 H16 Hk4 N2500 D128, window 777, 130 sinks: 214, 205, 222 us; B1 H16 Hk4, 4096 queries of
+// 16384 tokens, D64, window 4096: 236, 255, 250; B1 H32 Hk8 N1000 D128, causal: 71, 79, 98.)
 inline WindowSplit window_split(int tile, int bq, int Z, const WindowArgs& w, int N, int D, int workers) {
   const int64_t blocks = (N + bq - 1) / bq, key_tiles = (w.Nk + tile - 1) / tile, tiles = (w.sinks + tile - 1) / tile;
   const int64_t span = (int64_t(w.window) + tile - 1 + bq - 1) / bq + 1, one = span < blocks ? span : blocks;
   const int64_t unseen = (w.off > w.window ? w.off - w.window : 0) / tile;  // tiles before every query's window
   const int64_t seen = key_tiles - (unseen > tiles ? unseen : tiles);
   const int64_t all = int64_t(Z) * w.Hk * w.group * (tiles * blocks + seen * one);
-  const int64_t third = all / (3 * int64_t(workers)) + 1;
-  int64_t len = w.group * one < third ? w.group * one : third;
+  const int64_t share = all / workers + 1;
+  int64_t len = w.group * one < share ? w.group * one : share;
   const int64_t least = (w.group * blocks + 63) / 64;
   len = len < 8 ? 8 : len;
   len = len < least ? least : len;
