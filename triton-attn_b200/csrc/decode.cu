@@ -15,6 +15,12 @@
 // accumulators become the P^T operand by one 8 x 8 transposition in registers. (tcgen05 has 64 rows at
 // least and takes its operands from shared memory in its own layout; unpacked 4-bit codes would have to be
 // written there first.)
+//
+// Measured (B200): fp16, 64 sequences of 4,096 visible tokens, 4 key/value heads of 128 for 16 query heads: 538 MB in 82
+// us, 6.5 TB/s, a copy's rate. 4 bits, 16 sequences of 35,536 to 65,536 tokens, the same heads: 471 MB in 112 us, 4.2
+// TB/s: there the issue slots bound it, about 340 instructions for a warp's 16 keys, most of them to make fp16
+// values of codes (the fp16 pipes are busy 49 % of the time and the integer ones 45 %). One sequence of 512 or 1,000
+// tokens: 4.5 and 5 us, of which the launch, the loads' latency and the join are each 1 to 2.
 #include <cuda_fp16.h>
 #include <math.h>
 

