@@ -86,9 +86,9 @@ def test_workspace_size() -> None:
     assert size(2, 4, 2, 1000, 1000, 64, 0, 100, 4) == dq + 3 * part
     # A window of everything: 2 units for each of the 8 tiles.
     assert size(2, 4, 2, 1000, 1000, 64, 0, 1000, 4) == dq + 16 * part
-    # fp32: tiles and blocks of 64, no dQ rows; 4 and 16 blocks of 2 heads.
+    # fp32: tiles of 32 here and blocks of 64, no dQ rows; 4 and 16 blocks of 2 heads.
     assert size(2, 4, 2, 1000, 1000, 64, 1, 100, 0) == 0
-    assert size(2, 4, 2, 1000, 1000, 64, 1, 100, 4) == 2 * 2 * 4 * 2 * 64 * 64 * 4
+    assert size(2, 4, 2, 1000, 1000, 64, 1, 100, 4) == 2 * 2 * 4 * 2 * 32 * 64 * 4
 
 
 # -------------------------------------------------------------------------------------- on a B200
@@ -148,6 +148,21 @@ def test_against_the_definition(gpu, shape, d, dtype) -> None:
 def test_longer_sequences(gpu, window, sinks, d) -> None:
     _check(1, 4, 2, 2500, 2500, d, window, sinks, torch.float16)
     _check(1, 4, 2, 1100, 2500, d, window, sinks, torch.float16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("hk", [12, 4])
+def test_many_tiles_in_fp32(gpu, hk, d) -> None:
+    """96 query heads of 8 tiles of 64 rows fill the GPU five times: tiles of 64 rows, for 12 key heads also of keys."""
+    _check(8, 12, hk, 500, 510, d, 90, 70, torch.float32)
+
+
+@pytest.mark.gpu
+def test_heads_in_sets(gpu) -> None:
+    """fp16: 66 heads of 1,100 tokens, of which 59 with their tiles cut short by the ends are taken at once."""
+    _check(6, 11, 11, 1100, 1100, 128, 1100, 4, torch.float16)
+    _check(6, 11, 11, 1100, 1300, 128, 1200, 0, torch.float16)
 
 
 @pytest.mark.gpu

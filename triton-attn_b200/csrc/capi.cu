@@ -405,7 +405,7 @@ bool valid_window(int Z, int H, int Hk, int Nq, int Nk, int D, int dtype, int wi
 // The fp32 kernel has two CTAs an SM, which take units as they come: half of their share (B2 H8 N2000 D32, causal:
 // 550 us, the whole share 584).
 WindowSplit window_f32_split(int Z, const WindowArgs& w, int Nq, int D) {
-  return window_split(kWindowF32Tile, kWindowF32Tile, Z, w, Nq, D, 4 * device_sm_count());
+  return window_split(window_f32_tile(D, (long long)Z * w.Hk, w.Nk), kWindowF32Block, Z, w, Nq, D, 4 * device_sm_count());
 }
 
 // Windows and sinks longer than the keys say no more than the keys themselves.
@@ -503,7 +503,7 @@ extern "C" int tattn_window_bwd(const void* q, const void* k, const void* v, con
   a.win = window_args(H, Hk, Nq, Nk, window, sinks);
   if (dtype == TATTN_F32) {
     a.split = window_f32_split(Z, a.win, Nq, D);
-    if (window_part_bytes(kWindowF32Tile, Z, a.win, D, a.split) > 0) {
+    if (window_part_bytes(window_f32_tile(D, (long long)Z * Hk, Nk), Z, a.win, D, a.split) > 0) {
       if (!workspace) return TATTN_ERR_INVALID_ARGUMENT;
       if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return TATTN_ERR_LAYOUT;
       a.part = static_cast<float*>(workspace);
@@ -546,7 +546,7 @@ extern "C" int64_t tattn_window_bwd_workspace_bytes(int Z, int H, int Hk, int Nq
   if (Nq == 0 || H == 0) return 0;
   const WindowArgs w = window_args(H, Hk, Nq, Nk, window, sinks);
   if (dtype == TATTN_F32)
-    return window_part_bytes(kWindowF32Tile, Z, w, D, window_f32_split(Z, w, Nq, D));
+    return window_part_bytes(window_f32_tile(D, (long long)Z * Hk, Nk), Z, w, D, window_f32_split(Z, w, Nq, D));
   return bwd_fused_workspace_bytes(Z, H, Nq, D) +
          window_part_bytes(128, Z, w, D, window_split(128, bwd_fused_query_rows(D), Z, w, Nq, D, device_sm_count()));
 }

@@ -210,7 +210,9 @@ inline WindowSplit window_split(int tile, int bq, int Z, const WindowArgs& w, in
   const int64_t zh = int64_t(Z) * w.Hk < 65536 ? int64_t(Z) * w.Hk : 65536, heads = fit < 1 ? 1 : fit < zh ? fit : zh;
   return WindowSplit{int(tiles), units(w.group * blocks), units(w.group * one), int(before), int(last), int(heads > 0 ? heads : 1)};
 }
-constexpr int kWindowF32Tile = 64;  // rows of a tile of the fp32 window kernels
+constexpr int kWindowF32Block = 64;  // rows that the fp32 window kernels load at a time
+// Rows of their tiles: queries or keys of `heads` heads.
+int window_f32_tile(int D, long long heads, int rows);
 // The partials: fp32 [Z * Hk, slots, 2 (dV, dK), tile, D].
 inline int64_t window_part_bytes(int tile, int Z, const WindowArgs& w, int D, const WindowSplit& s) {
   return int64_t(Z) * w.Hk * s.slots((w.Nk + tile - 1) / tile) * 2 * tile * D * 4;

@@ -5,16 +5,20 @@
 // accuracy. Two kernels for the backward, dK/dV by key tiles and dQ by query tiles, so that nothing is
 // summed by atomics and results are bitwise reproducible.
 //
-// The bound is the FMA pipe (4 D flop forward and 14 D backward a pair) fed from shared memory: 64 x 64 tiles, and a
+// The bound is the FMA pipe (4 D flop forward and 14 D backward a pair) fed from shared memory: tiles of T x 64, and a
 // thread computes R x 4 scores (rows R ty + i, columns tx + 16 j) from 16-byte reads along D, then R rows x D / 16
 // columns of the products with V, K, Q and dO the same way. A read that 16 threads share costs 1 to 2 cycles of shared
-// memory and one of 16 different units 4: with R = 4 (256 threads) they outweigh the FMAs (72 % of the cycles against
-// 53 %, dK/dV at B4 H16 N2048 D64, window 512), with R = 8 (128 threads, up to 255 registers) they do not: 580 -> 514 us
-// forward and 1820 -> 1632 backward there; D = 32: 251 -> 220 and 642 -> 549 (B2 H8 N2000, causal). D = 16 has too little
-// to do for 8 rows (13 -> 17 us forward, B2 H8 N500), D = 128 too few registers. The tiles of the next step are on
-// their way while this one's are computed with (cp.async); at 8 to 16 warps an SM what is left is latency: 40 of the
-// FMA pipes' 74 TFLOP/s at the size above, and at B3 H5 N1000, window 200, where 240 tiles make 1.6 CTAs an SM, 17
-// (60 us forward, 175 backward).
+// memory and one of 16 different units 4: with R = 4 they outweigh the FMAs (72 % of the cycles against 53 %, dK/dV at
+// B4 H16 N2048 D64, window 512), with R = 8 they do not. The next block's rows are on their way while this one's are
+// computed with (cp.async).
+//
+// T = 64 (R = 8; 4 at D = 128, for the registers): 580 -> 515 us forward and 1822 -> 1635 backward there against R = 4.
+// With fewer tiles than 5 an SM, T = 32 (R = 4): more CTAs to spread and fewer masked pairs (B1 H4 N700 D64, causal:
+// 72 -> 42 forward, 153 -> 106 backward; B2 H8 N1500 D128, window 300: 195 -> 185 and 660 -> 630; with 14 tiles an SM 527
+// and 1850 for the 515 and 1635 above), and for D = 16, whose 64 rows take more threads than they give work (B4 H16 N2048,
+// window 512: 248 -> 220 and 704 -> 640). Rates: 40 of the FMA pipes' 74 TFLOP/s at the first size; 19 at B3 H5 N1000 D64,
+// window 200, 4 sinks (56 us forward, 172 backward), where the 480 tiles differ in length and the busiest SM has 1.55
+// times the mean.
 #include <math.h>
 
 #include "common.cuh"
@@ -23,11 +27,11 @@
 namespace tattn {
 namespace {
 
-constexpr int TB = kWindowF32Tile;  // rows and columns of a tile
-template <int D>
-constexpr int kRows = D == 32 || D == 64 ? 8 : 4;  // of a tile, a thread's
-template <int D>
-constexpr int kThreads = 16 * TB / kRows<D>;
+constexpr int TB = kWindowF32Block;  // columns of a tile: the rows that are loaded one block after another
+template <int D, int T>              // T: rows of a tile, 64 or 32
+constexpr int kRows = T == 64 && (D == 32 || D == 64) ? 8 : 4;  // a thread's
+template <int D, int T>
+constexpr int kThreads = 16 * T / kRows<D, T>;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Row pitch in floats: 16-byte units a row odd in number, so that 16 rows at one unit are in different banks.
@@ -35,29 +39,28 @@ template <int D>
 constexpr int kPitch = D + 4;
 constexpr int kPitchP = TB + 4;
 
-// Rows [r0, r0 + 64) of a [n, D] matrix into shared memory, 16 bytes at a time and asynchronously (cp_async_wait) where
+// Rows [r0, r0 + ROWS) of a [n, D] matrix into shared memory, 16 bytes at a time and asynchronously (cp_async_wait) where
 // its rows allow; rows past n are zeros.
-template <int D>
+template <int D, int ROWS, int THREADS>
 __device__ __forceinline__ void load_rows(float* dst, const float* src, const Strides4& s, int r0, int n) {
   if (s.d == 1 && s.n % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
 #pragma unroll
-    for (int i = 0; i < TB * D / 4 / kThreads<D>; ++i) {
-      const int e = i * kThreads<D> + threadIdx.x, r = e / (D / 4), d = e % (D / 4) * 4;
+    for (int i = 0; i < ROWS * D / 4 / THREADS; ++i) {
+      const int e = i * THREADS + threadIdx.x, r = e / (D / 4), d = e % (D / 4) * 4;
       cp_async16(smem_u32(dst + r * kPitch<D> + d), src + int64_t(min(r0 + r, n - 1)) * s.n + d, r0 + r < n);
     }
     return;
   }
 #pragma unroll 4
-  for (int e = threadIdx.x; e < TB * D; e += kThreads<D>) {
+  for (int e = threadIdx.x; e < ROWS * D; e += THREADS) {
     const int r = e / D, d = e % D;
     dst[r * kPitch<D> + d] = r0 + r < n ? __ldg(src + int64_t(r0 + r) * s.n + d * s.d) : 0.f;
   }
 }
 
 // c[i][j] = a[R ty + i] . b[tx + 16 j] over D.
-template <int D>
+template <int D, int R>
 __device__ __forceinline__ void rows_dot(const float* a, const float* b, int ty, int tx, float (*c)[4]) {
-  constexpr int R = kRows<D>;
 #pragma unroll
   for (int i = 0; i < R; ++i)
 #pragma unroll
@@ -78,9 +81,9 @@ __device__ __forceinline__ void rows_dot(const float* a, const float* b, int ty,
 }
 
 // acc[i][e] += sum over r of p[R ty + i][r] b[r][D / 16 tx + e], two e in a packed FMA.
-template <int D>
+template <int D, int R>
 __device__ __forceinline__ void rows_times(const float* p, const float* b, int ty, int tx, float (*acc)[D / 16]) {
-  constexpr int E = D / 16, R = kRows<D>;
+  constexpr int E = D / 16;
 #pragma unroll 2
   for (int r = 0; r < TB; r += 4) {
     float4 x[R];
@@ -118,28 +121,28 @@ __device__ __forceinline__ bool sees(int row, int col, int N, const WindowArgs& 
   return row < N && col <= p && (col > p - w.window || col < w.sinks);
 }
 
-// Key tiles of query rows [r0, r0 + 64): those with sinks, then those that a window reaches, up to the diagonal.
-__device__ __forceinline__ int next_key_tile(int k0, int r0, const WindowArgs& w) {
+// Blocks of keys of the query rows from r0 on: those with sinks, then those that a window reaches, up to the diagonal.
+__device__ __forceinline__ int next_keys(int k0, int r0, const WindowArgs& w) {
   k0 += TB;
   return k0 >= w.sinks ? max(k0, max(0, r0 + w.off - w.window + 1) / TB * TB) : k0;
 }
 
-template <int D>
-__global__ void __launch_bounds__(kThreads<D>) window_fwd_f32_kernel(const float* q, const float* k, const float* v,
+template <int D, int T>
+__global__ void __launch_bounds__(kThreads<D, T>) window_fwd_f32_kernel(const float* q, const float* k, const float* v,
                                                                   Strides4 sq, Strides4 sk, Strides4 sv, FwdArgs a) {
-  constexpr int R = kRows<D>;
+  constexpr int R = kRows<D, T>, TH = kThreads<D, T>;
   extern __shared__ __align__(16) float smem[];
-  float *Qs = smem, *Ks = Qs + TB * kPitch<D>, *Vs = Ks + TB * kPitch<D>, *Ps = Vs + TB * kPitch<D>;
-  const int N = a.N, Nk = a.win.Nk, r0 = blockIdx.x * TB;
+  float *Qs = smem, *Ks = Qs + T * kPitch<D>, *Vs = Ks + TB * kPitch<D>, *Ps = Vs + TB * kPitch<D>;
+  const int N = a.N, Nk = a.win.Nk, r0 = blockIdx.x * T;
   const int64_t head = cta_head();
   if (head >= int64_t(a.Z) * a.H) return;
   const int zi = int(head / a.H), hi = int(head % a.H), hk = hi / a.win.group;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   k += zi * sk.z + hk * sk.h;
   v += zi * sv.z + hk * sv.h;
-  int k0 = next_key_tile(-TB, r0, a.win);
-  load_rows<D>(Qs, q + zi * sq.z + hi * sq.h, sq, r0, N);
-  load_rows<D>(Ks, k, sk, k0, Nk);
+  int k0 = next_keys(-TB, r0, a.win);
+  load_rows<D, T, TH>(Qs, q + zi * sq.z + hi * sq.h, sq, r0, N);
+  load_rows<D, TB, TH>(Ks, k, sk, k0, Nk);
   float m[R], l[R], acc[R][D / 16];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -148,13 +151,13 @@ __global__ void __launch_bounds__(kThreads<D>) window_fwd_f32_kernel(const float
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) acc[i][e] = 0.f;
   }
-  const int end = min(r0 + TB + a.win.off, Nk);
+  const int end = min(r0 + T + a.win.off, Nk);
   for (int next; k0 < end; k0 = next) {
     cp_async_wait_all();
     __syncthreads();  // K is here, and V's last tile has been read
-    load_rows<D>(Vs, v, sv, k0, Nk);
+    load_rows<D, TB, TH>(Vs, v, sv, k0, Nk);
     float s[R][4];
-    rows_dot<D>(Qs, Ks, ty, tx, s);
+    rows_dot<D, R>(Qs, Ks, ty, tx, s);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       float mx = m[i];
@@ -179,9 +182,9 @@ __global__ void __launch_bounds__(kThreads<D>) window_fwd_f32_kernel(const float
     }
     cp_async_wait_all();
     __syncthreads();  // V is here, and K has been read
-    next = next_key_tile(k0, r0, a.win);
-    if (next < end) load_rows<D>(Ks, k, sk, next, Nk);
-    rows_times<D>(Ps, Vs, ty, tx, acc);
+    next = next_keys(k0, r0, a.win);
+    if (next < end) load_rows<D, TB, TH>(Ks, k, sk, next, Nk);
+    rows_times<D, R>(Ps, Vs, ty, tx, acc);
   }
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -199,14 +202,13 @@ __global__ void __launch_bounds__(kThreads<D>) window_fwd_f32_kernel(const float
 
 // P and dS of rows R ty + i of A (with C) and rows tx + 16 j of B (with E): A, B are queries and keys, or keys
 // and queries (KEYS); C, E their dO and V, or V and dO.
-template <int D, bool KEYS>
+template <int D, int R, bool KEYS>
 __device__ __forceinline__ void p_ds(const BwdArgs& a, const float* A, const float* B, const float* C, const float* E,
                                      int ty, int tx, int a0, int b0, const float* Ms, const float* Ds, float (*p)[4],
                                      float (*ds)[4]) {
-  constexpr int R = kRows<D>;
   float s[R][4], dp[R][4];
-  rows_dot<D>(A, B, ty, tx, s);
-  rows_dot<D>(C, E, ty, tx, dp);
+  rows_dot<D, R>(A, B, ty, tx, s);
+  rows_dot<D, R>(C, E, ty, tx, dp);
   const float qks = a.sm_scale * kLog2e;
 #pragma unroll
   for (int i = 0; i < R; ++i)
@@ -219,46 +221,46 @@ __device__ __forceinline__ void p_ds(const BwdArgs& a, const float* A, const flo
     }
 }
 
-template <int D>
-__global__ void __launch_bounds__(kThreads<D>) window_dq_f32_kernel(BwdArgs a) {
-  constexpr int R = kRows<D>;
+template <int D, int T>
+__global__ void __launch_bounds__(kThreads<D, T>) window_dq_f32_kernel(BwdArgs a) {
+  constexpr int R = kRows<D, T>, TH = kThreads<D, T>;
   extern __shared__ __align__(16) float smem[];
-  float *Qs = smem, *Os = Qs + TB * kPitch<D>, *Vs = Os + TB * kPitch<D>;
+  float *Qs = smem, *Os = Qs + T * kPitch<D>, *Vs = Os + T * kPitch<D>;
   float *Ks = Vs + TB * kPitch<D>, *Kn = Ks + TB * kPitch<D>;  // K's tile and the next one
-  float *DSs = Kn + TB * kPitch<D>, *Ms = DSs + TB * kPitchP, *Ds = Ms + TB;
-  const int N = a.N, Nk = a.win.Nk, r0 = blockIdx.x * TB;
+  float *DSs = Kn + TB * kPitch<D>, *Ms = DSs + T * kPitchP, *Ds = Ms + T;
+  const int N = a.N, Nk = a.win.Nk, r0 = blockIdx.x * T;
   const int64_t head = cta_head();
   if (head >= int64_t(a.Z) * a.H) return;
   const int zi = int(head / a.H), hi = int(head % a.H), hk = hi / a.win.group;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const float* k = static_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h;
   const float* v = static_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h;
-  load_rows<D>(Qs, static_cast<const float*>(a.q) + zi * a.sq.z + hi * a.sq.h, a.sq, r0, N);
-  load_rows<D>(Os, static_cast<const float*>(a.dout) + zi * a.sdo.z + hi * a.sdo.h, a.sdo, r0, N);
-  int k0 = next_key_tile(-TB, r0, a.win);
-  load_rows<D>(Ks, k, a.sk, k0, Nk);
-  load_rows<D>(Vs, v, a.sv, k0, Nk);
-  if (threadIdx.x < TB) {
+  load_rows<D, T, TH>(Qs, static_cast<const float*>(a.q) + zi * a.sq.z + hi * a.sq.h, a.sq, r0, N);
+  load_rows<D, T, TH>(Os, static_cast<const float*>(a.dout) + zi * a.sdo.z + hi * a.sdo.h, a.sdo, r0, N);
+  int k0 = next_keys(-TB, r0, a.win);
+  load_rows<D, TB, TH>(Ks, k, a.sk, k0, Nk);
+  load_rows<D, TB, TH>(Vs, v, a.sv, k0, Nk);
+  if (threadIdx.x < T) {
     const int row = r0 + threadIdx.x;
     Ms[threadIdx.x] = row < N ? a.m[head * N + row] : 0.f;
     Ds[threadIdx.x] = row < N ? a.delta[head * N + row] : 0.f;
   }
   float acc[R][D / 16] = {};
-  const int end = min(r0 + TB + a.win.off, Nk);
+  const int end = min(r0 + T + a.win.off, Nk);
   for (int next; k0 < end; k0 = next) {
     cp_async_wait_all();
     __syncthreads();  // K and V are here, and K's last tile has been read
-    next = next_key_tile(k0, r0, a.win);
-    if (next < end) load_rows<D>(Kn, k, a.sk, next, Nk);
+    next = next_keys(k0, r0, a.win);
+    if (next < end) load_rows<D, TB, TH>(Kn, k, a.sk, next, Nk);
     float p[R][4], ds[R][4];
-    p_ds<D, false>(a, Qs, Ks, Os, Vs, ty, tx, r0, k0, Ms, Ds, p, ds);
+    p_ds<D, R, false>(a, Qs, Ks, Os, Vs, ty, tx, r0, k0, Ms, Ds, p, ds);
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) DSs[(R * ty + i) * kPitchP + tx + 16 * j] = ds[i][j];
     __syncthreads();  // V has been read
-    if (next < end) load_rows<D>(Vs, v, a.sv, next, Nk);
-    rows_times<D>(DSs, Ks, ty, tx, acc);
+    if (next < end) load_rows<D, TB, TH>(Vs, v, a.sv, next, Nk);
+    rows_times<D, R>(DSs, Ks, ty, tx, acc);
     float* t = Ks;
     Ks = Kn;
     Kn = t;
@@ -275,26 +277,26 @@ __global__ void __launch_bounds__(kThreads<D>) window_dq_f32_kernel(BwdArgs a) {
 
 // One unit (window_unit): a key tile of a key/value head, summed over the query heads that share it, or a part of
 // that sum.
-template <int D>
-__global__ void __launch_bounds__(kThreads<D>) window_dkdv_f32_kernel(BwdArgs a) {
-  constexpr int R = kRows<D>;
+template <int D, int T>
+__global__ void __launch_bounds__(kThreads<D, T>) window_dkdv_f32_kernel(BwdArgs a) {
+  constexpr int R = kRows<D, T>, TH = kThreads<D, T>;
   extern __shared__ __align__(16) float smem[];
-  float *Ks = smem, *Vs = Ks + TB * kPitch<D>, *Os = Vs + TB * kPitch<D>;
+  float *Ks = smem, *Vs = Ks + T * kPitch<D>, *Os = Vs + T * kPitch<D>;
   float *Qs = Os + TB * kPitch<D>, *Qn = Qs + TB * kPitch<D>;  // Q's tile and the next one
-  float *Ps = Qn + TB * kPitch<D>, *Ms = Ps + TB * kPitchP, *Mn = Ms + 2 * TB;  // M and delta of them
+  float *Ps = Qn + TB * kPitch<D>, *Ms = Ps + T * kPitchP, *Mn = Ms + 2 * TB;  // M and delta of them
   const int N = a.N, Nk = a.win.Nk;
   if (cta_head() >= int64_t(a.Z) * a.win.Hk) return;
-  const WindowUnit u = window_unit<TB, TB>(a.split, a.win, a.Z, N, unsigned(cta_head() * gridDim.x + blockIdx.x));
-  const int k0 = TB * u.kt;
+  const WindowUnit u = window_unit<T, TB>(a.split, a.win, a.Z, N, unsigned(cta_head() * gridDim.x + blockIdx.x));
+  const int k0 = T * u.kt;
   const int64_t head = u.head;
   const int zi = int(head / a.win.Hk), hk = int(head % a.win.Hk);
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  load_rows<D>(Ks, static_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h, a.sk, k0, Nk);
-  load_rows<D>(Vs, static_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h, a.sv, k0, Nk);
+  load_rows<D, T, TH>(Ks, static_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h, a.sk, k0, Nk);
+  load_rows<D, T, TH>(Vs, static_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h, a.sv, k0, Nk);
   float dk[R][D / 16] = {}, dv[R][D / 16] = {};
   auto rows_of = [&](const void* x, const Strides4& st, int i, float* to) {  // the tile of pair i
     const int hi = hk * a.win.group + i / u.nb, r0 = (u.lo + i % u.nb) * TB;
-    load_rows<D>(to, static_cast<const float*>(x) + zi * st.z + hi * st.h, st, r0, N);
+    load_rows<D, TB, TH>(to, static_cast<const float*>(x) + zi * st.z + hi * st.h, st, r0, N);
   };
   auto load_q = [&](int i, float* to, float* md) {
     rows_of(a.q, a.sq, i, to);
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(kThreads<D>) window_dkdv_f32_kernel(BwdArgs a)
     __syncthreads();  // Q and dO are here, and Q's last tile has been read
     if (i + 1 < end) load_q(i + 1, Qn, Mn);
     float p[R][4], ds[R][4];
-    p_ds<D, true>(a, Ks, Qs, Vs, Os, ty, tx, k0, r0, Ms, Ms + TB, p, ds);
+    p_ds<D, R, true>(a, Ks, Qs, Vs, Os, ty, tx, k0, r0, Ms, Ms + TB, p, ds);
     auto put = [&](const float(*x)[4]) {  // a row is written and read by the 16 threads of one half warp
       __syncwarp();
 #pragma unroll
@@ -326,11 +328,11 @@ __global__ void __launch_bounds__(kThreads<D>) window_dkdv_f32_kernel(BwdArgs a)
       __syncwarp();
     };
     put(p);
-    rows_times<D>(Ps, Os, ty, tx, dv);
+    rows_times<D, R>(Ps, Os, ty, tx, dv);
     __syncthreads();  // dO has been read
     if (i + 1 < end) rows_of(a.dout, a.sdo, i + 1, Os);
     put(ds);
-    rows_times<D>(Ps, Qs, ty, tx, dk);
+    rows_times<D, R>(Ps, Qs, ty, tx, dk);
     float *q = Qs, *md = Ms;
     Qs = Qn;
     Qn = q;
@@ -343,12 +345,12 @@ __global__ void __launch_bounds__(kThreads<D>) window_dkdv_f32_kernel(BwdArgs a)
     const int key = k0 + R * ty + i;
     if (key >= Nk) continue;
     if (u.slot >= 0) {
-      const int64_t slot = head * a.split.slots((Nk + TB - 1) / TB) + u.slot;
-      float* part = a.part + (slot * 2 * TB + R * ty + i) * D + D / 16 * tx;
+      const int64_t slot = head * a.split.slots((Nk + T - 1) / T) + u.slot;
+      float* part = a.part + (slot * 2 * T + R * ty + i) * D + D / 16 * tx;
 #pragma unroll
       for (int e = 0; e < D / 16; ++e) {
         part[e] = dv[i][e];
-        part[TB * D + e] = dk[i][e];
+        part[T * D + e] = dk[i][e];
       }
       continue;
     }
@@ -364,12 +366,12 @@ __global__ void __launch_bounds__(kThreads<D>) window_dkdv_f32_kernel(BwdArgs a)
 constexpr int kJoinThreads = 256;
 
 // dV and dK of the tiles of several units: the sums of the units' partials, in their order.
-__global__ void __launch_bounds__(kJoinThreads) window_join_f32_kernel(BwdArgs a, int D) {
-  const int key_tiles = (a.win.Nk + TB - 1) / TB, tiles = a.split.units > 1 ? key_tiles : a.split.tiles;
-  const int64_t i = int64_t(blockIdx.x) * kJoinThreads + threadIdx.x, tile = TB * D;
+__global__ void __launch_bounds__(kJoinThreads) window_join_f32_kernel(BwdArgs a, int T, int D) {
+  const int key_tiles = (a.win.Nk + T - 1) / T, tiles = a.split.units > 1 ? key_tiles : a.split.tiles;
+  const int64_t i = int64_t(blockIdx.x) * kJoinThreads + threadIdx.x, tile = T * D;
   const int which = int(i / tile % 2);  // 0: dV, 1: dK
   const int64_t t = i / (2 * tile), head = t / tiles;
-  const int kt = int(t % tiles), key = kt * TB + int(i % tile / D);
+  const int kt = int(t % tiles), key = kt * T + int(i % tile / D);
   const bool sink = kt < a.split.tiles;
   const int count = sink ? a.split.sink_units : a.split.units;
   if (head >= int64_t(a.Z) * a.win.Hk || count == 1 || key >= a.win.Nk) return;
@@ -381,58 +383,83 @@ __global__ void __launch_bounds__(kJoinThreads) window_join_f32_kernel(BwdArgs a
   out[(head * a.win.Nk + key) * D + i % D] = which ? sum * a.sm_scale : sum;
 }
 
-template <int D, typename Kernel, typename... Args>
-cudaError_t launch(Kernel kernel, int tiles, long long heads, int floats, cudaStream_t s, const Args&... args) {
+template <typename Kernel, typename... Args>
+cudaError_t launch(Kernel kernel, int tiles, long long heads, int threads, int floats, cudaStream_t s, const Args&... args) {
   const long long y = heads < 65535 ? heads : 65535, z = (heads + y - 1) / y;
   if (z > 65535) return cudaErrorInvalidConfiguration;
   const int smem = floats * 4;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kernel<<<dim3(tiles, unsigned(y), unsigned(z)), kThreads<D>, smem, s>>>(args...);
+  kernel<<<dim3(tiles, unsigned(y), unsigned(z)), threads, smem, s>>>(args...);
   return cudaGetLastError();
 }
 
-template <int D>
+template <int D, int T>
 cudaError_t fwd_impl(const float* q, const float* k, const float* v, const Strides4& sq, const Strides4& sk,
                      const Strides4& sv, const FwdArgs& a, cudaStream_t s) {
-  return launch<D>(window_fwd_f32_kernel<D>, (a.N + TB - 1) / TB, (long long)a.Z * a.H, TB * (3 * kPitch<D> + kPitchP), s, q, k, v, sq, sk,
-                sv, a);
+  return launch(window_fwd_f32_kernel<D, T>, (a.N + T - 1) / T, (long long)a.Z * a.H, kThreads<D, T>,
+                (T + 2 * TB) * kPitch<D> + T * kPitchP, s, q, k, v, sq, sk, sv, a);
+}
+
+template <int D, int T>
+cudaError_t dkdv_impl(const BwdArgs& a, cudaStream_t s) {
+  const int key_tiles = (a.win.Nk + T - 1) / T;
+  const cudaError_t e = launch(window_dkdv_f32_kernel<D, T>, a.split.per_head(key_tiles), (long long)a.Z * a.win.Hk, kThreads<D, T>,
+                               (2 * T + 3 * TB) * kPitch<D> + T * kPitchP + 4 * TB, s, a);
+  if (e != cudaSuccess || a.split.slots(key_tiles) == 0) return e;
+  const int64_t values = int64_t(a.Z) * a.win.Hk * (a.split.units > 1 ? key_tiles : a.split.tiles) * 2 * T * D;
+  window_join_f32_kernel<<<unsigned((values + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, s>>>(a, T, D);
+  return cudaGetLastError();
+}
+template <int D, int T>
+cudaError_t dq_impl(const BwdArgs& a, cudaStream_t s) {
+  return launch(window_dq_f32_kernel<D, T>, (a.N + T - 1) / T, (long long)a.Z * a.H, kThreads<D, T>,
+                (2 * T + 3 * TB) * kPitch<D> + T * kPitchP + 2 * T, s, a);
 }
 
 template <int D>
-cudaError_t bwd_impl(const BwdArgs& a, cudaStream_t s) {
-  const int key_tiles = (a.win.Nk + TB - 1) / TB;
-  cudaError_t e = launch<D>(window_dkdv_f32_kernel<D>, a.split.per_head(key_tiles), (long long)a.Z * a.win.Hk,
-                         TB * (5 * kPitch<D> + kPitchP + 4), s, a);
-  if (e != cudaSuccess) return e;
-  if (a.split.slots(key_tiles) > 0) {
-    const int64_t values = int64_t(a.Z) * a.win.Hk * (a.split.units > 1 ? key_tiles : a.split.tiles) * 2 * TB * D;
-    window_join_f32_kernel<<<unsigned((values + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, s>>>(a, D);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+cudaError_t fwd_tiles(const float* q, const float* k, const float* v, const Strides4& sq, const Strides4& sk,
+                      const Strides4& sv, const FwdArgs& a, cudaStream_t s) {
+  if constexpr (D > 16)
+    if (window_f32_tile(D, (long long)a.Z * a.H, a.N) == 64) return fwd_impl<D, 64>(q, k, v, sq, sk, sv, a, s);
+  return fwd_impl<D, 32>(q, k, v, sq, sk, sv, a, s);
+}
+template <int D>
+cudaError_t bwd_tiles(const BwdArgs& a, cudaStream_t s) {
+  auto of_keys = dkdv_impl<D, 32>;
+  auto of_queries = dq_impl<D, 32>;
+  if constexpr (D > 16) {
+    if (window_f32_tile(D, (long long)a.Z * a.win.Hk, a.win.Nk) == 64) of_keys = dkdv_impl<D, 64>;
+    if (window_f32_tile(D, (long long)a.Z * a.H, a.N) == 64) of_queries = dq_impl<D, 64>;
   }
-  return launch<D>(window_dq_f32_kernel<D>, (a.N + TB - 1) / TB, (long long)a.Z * a.H, TB * (5 * kPitch<D> + kPitchP + 2), s, a);
+  const cudaError_t e = of_keys(a, s);
+  return e != cudaSuccess ? e : of_queries(a, s);
 }
 
 }  // namespace
+
+int window_f32_tile(int D, long long heads, int rows) {
+  return D == 16 || heads * ((rows + 63) / 64) < 5LL * device_sm_count() ? 32 : 64;
+}
 
 cudaError_t launch_window_fwd_f32(int D, const void* q, const void* k, const void* v, Strides4 sq, Strides4 sk,
                                   Strides4 sv, const FwdArgs& a, cudaStream_t s) {
   const float *qf = static_cast<const float*>(q), *kf = static_cast<const float*>(k), *vf = static_cast<const float*>(v);
   switch (D) {
-    case 16: return fwd_impl<16>(qf, kf, vf, sq, sk, sv, a, s);
-    case 32: return fwd_impl<32>(qf, kf, vf, sq, sk, sv, a, s);
-    case 64: return fwd_impl<64>(qf, kf, vf, sq, sk, sv, a, s);
-    case 128: return fwd_impl<128>(qf, kf, vf, sq, sk, sv, a, s);
+    case 16: return fwd_tiles<16>(qf, kf, vf, sq, sk, sv, a, s);
+    case 32: return fwd_tiles<32>(qf, kf, vf, sq, sk, sv, a, s);
+    case 64: return fwd_tiles<64>(qf, kf, vf, sq, sk, sv, a, s);
+    case 128: return fwd_tiles<128>(qf, kf, vf, sq, sk, sv, a, s);
     default: return cudaErrorInvalidValue;
   }
 }
 
 cudaError_t launch_window_bwd_f32(int D, const BwdArgs& a, cudaStream_t s) {
   switch (D) {
-    case 16: return bwd_impl<16>(a, s);
-    case 32: return bwd_impl<32>(a, s);
-    case 64: return bwd_impl<64>(a, s);
-    case 128: return bwd_impl<128>(a, s);
+    case 16: return bwd_tiles<16>(a, s);
+    case 32: return bwd_tiles<32>(a, s);
+    case 64: return bwd_tiles<64>(a, s);
+    case 128: return bwd_tiles<128>(a, s);
     default: return cudaErrorInvalidValue;
   }
 }
