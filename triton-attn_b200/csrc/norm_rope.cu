@@ -12,14 +12,14 @@
 // L = D / (2 VEC) lanes owns a token's row: lane c holds the 16 bytes at c and the 16 bytes half a row
 // further, so a half-split pair lies in one lane, and so does an interleaved one. A work item is one token
 // and HB consecutive heads of one tensor, which share the token's cos and sin and the weight in
-// registers; HB = 4 (backward, with two tensors to hold: 2) where there are enough items to fill the GPU with,
-// else 1 (a decoding step's few rows).
+// registers; HB = kMany where there are enough items to fill the GPU with, else 1 (a decoding step's few rows).
 // dw: every CTA works on one tensor, adds its rows' terms in registers and then shared memory and writes one
 // partial; a second small kernel sums the partials in a fixed order, so dw is bitwise reproducible.
 //
-// Measured (B200, fp16): B4 N4096, 16 query and 4 key heads of 64, forward and backward 57 us on the device for
-// 170 MB, which is 3.0 TB/s with the tensors partly in L2 (D 64: 4 lanes a row, so a warp's 8 rows of one head are
-// runs of 64 bytes), and one token of 8 sequences, 16 and 4 heads of 128: 2.8 us, the launch.
+// Measured (B200, B4 N4096, passes over three sets of tensors): fp16, 16 query and 4 key heads of 64: forward 16 us, 5.1
+// TB/s, backward 38 us, 3.3 TB/s (dw's second kernel, 3 us, among them; issue slots bound it: 16 values of x, dy, w, dw
+// and the result are held in fp32 by each lane); fp32, 16 and 16 heads of 64: 42 us, 6.4 TB/s, and 67 us, 6.0 TB/s. One
+// token of 8 sequences, 16 and 4 heads of 128 in fp16: 2.5 us, the launch.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -29,6 +29,11 @@ namespace tattn {
 namespace {
 
 constexpr int kThreads = 256;
+// Heads of a work item. fp16 lanes hold twice the values, in 128 registers: fewer CTAs with more loads each. (Backward in
+// fp16 with one head and 4 CTAs an SM 46 us for the 38 above, with 8-byte loads 45 to 53; fp32 with 2 CTAs an SM and 4
+// and 2 heads 46 and 78 us for 42 and 67.)
+template <typename T, bool BACKWARD>
+constexpr int kMany = sizeof(T) == 4 ? (BACKWARD ? 1 : 2) : (BACKWARD ? 2 : 4);
 
 template <typename T>
 constexpr int kVec = 16 / int(sizeof(T));
@@ -127,7 +132,7 @@ __device__ __forceinline__ Item rope_item(const RopeArgs& a, const RopeTensor& t
 }
 
 template <typename T, int D, bool INTERLEAVED, int HB, bool BACKWARD>
-__global__ void __launch_bounds__(kThreads, 2) norm_rope_kernel(const RopeArgs a) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 2) norm_rope_kernel(const RopeArgs a) {
   constexpr int VEC = kVec<T>, L = D / (2 * VEC), GROUPS = kThreads / L;
   using P = Pairs<VEC, INTERLEAVED>;
   const int which = int(blockIdx.x) < a.t[0].blocks ? 0 : 1;  // the CTA's tensor
@@ -279,8 +284,8 @@ template <typename T, int D, bool INTERLEAVED, bool BACKWARD>
 cudaError_t rope_impl(RopeArgs& a, cudaStream_t s) {
   constexpr int GROUPS = kThreads / (D / (2 * kVec<T>));
   const int sms = device_sm_count();
-  // Several heads an item once that still gives every SM's 2048 threads something to do.
-  constexpr int MANY = BACKWARD ? 2 : 4;
+  // Several heads an item (fp32 backward: one at all sizes) once that still gives every SM's 2048 threads something to do.
+  constexpr int MANY = kMany<T, BACKWARD>;
   const int64_t rows = int64_t(a.Z) * a.N * (a.t[0].H + a.t[1].H);
   const bool many = rows * (D / (2 * kVec<T>)) >= int64_t(sms) * 2048 * MANY;
   const int HB = many ? MANY : 1;
