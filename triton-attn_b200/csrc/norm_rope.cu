@@ -17,8 +17,9 @@
 // partial; a second small kernel sums the partials in a fixed order, so dw is bitwise reproducible.
 //
 // Measured (B200, B4 N4096, passes over three sets of tensors): fp16, 16 query and 4 key heads of 64: forward 16 us, 5.1
-// TB/s, backward 38 us, 3.3 TB/s (dw's second kernel, 3 us, among them; issue slots bound it: 16 values of x, dy, w, dw
-// and the result are held in fp32 by each lane); fp32, 16 and 16 heads of 64: 42 us, 6.4 TB/s, and 67 us, 6.0 TB/s. One
+// TB/s, backward 38 us, 3.3 TB/s (dw's second kernel, 3 us, among them; a lane holds 16 values each of x, dy, w, dw and
+// the result in fp32, so two CTAs fit an SM, and 16 warps that load, compute and store in turn leave HBM idle between:
+// issue slots 50 % busy); fp32, 16 and 16 heads of 64: 42 us, 6.4 TB/s, and 67 us, 6.0 TB/s. One
 // token of 8 sequences, 16 and 4 heads of 128 in fp16: 2.5 us, the launch.
 #include <cuda_fp16.h>
 
