@@ -512,3 +512,32 @@ def test_a_captured_step(gpu) -> None:
         v.copy_(vs[:, :, i : i + 1])
         graph.replay()
         assert torch.equal(out, other.attend(q, _lens(i + 1, i + 1), 8, 2)), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_append_shows_what_is_not_a_number(gpu, d) -> None:
+    """A group of 64 dims with a NaN or an infinity among them reads as NaN, wherever it lies and whatever else the
+    group holds; every other group is as it would be alone. Attention shows it too."""
+    _, k, v = _inputs(2, 1, 2, 80, d, torch.float16, 24)
+    clean = Int4Cache.empty(2, 2, 80, d)
+    clean.append(k, v)
+    hit = [torch.zeros(2, 2, 80, d // 64, dtype=torch.bool, device="cuda") for _ in range(2)]
+    kinds = (math.nan, math.inf, -math.inf)
+    for i in range(64):  # every place of a group, in different rows
+        for x, h, n in ((k, hit[0], i), (v, hit[1], 3 * i)):
+            x[i % 2, 0, n % 80, 64 * (i % (d // 64)) + i] = kinds[i % 3]
+            h[i % 2, 0, n % 80, i % (d // 64)] = True
+    k[0, 0, 79, :2], k[1, 0, 79, :2] = torch.tensor([math.nan, math.inf]), torch.tensor([math.inf, -math.inf])
+    hit[0][:, 0, 79, 0] = True
+    cache = Int4Cache.empty(2, 2, 80, d)
+    cache.append(k, v)
+    for got, want, h in zip(cache.read(80), clean.read(80), hit, strict=True):
+        h = h.repeat_interleave(64, -1)
+        assert bool(got[h].isnan().all()) and torch.equal(got[~h], want[~h])
+    q, _, _ = _inputs(2, 2, 1, 1, d, torch.float16, 25)
+    o, want = cache.attend(q, _lens(80, 80)), clean.attend(q, _lens(80, 80))
+    assert bool(o[:, 0].isnan().all()) and torch.equal(o[:, 1], want[:, 1])
+    only_v = Int4Cache(clean.k_codes, clean.k_params, cache.v_codes, cache.v_params)
+    o, h = only_v.attend(q, _lens(80, 80)), hit[1].any(2).repeat_interleave(64, -1)[:, :, None]
+    assert bool(o[h].isnan().all()) and torch.equal(o[~h], want[~h])

@@ -2,7 +2,8 @@
 //
 // A group of 64 head dims of a row x: m = min(x), s = fp16((max(x) - m) / 15), code n = round((x - m) / s) in
 // [0, 15] (ties to even; 0 where s = 0); it stands for fp16(s n + m). m is one of the inputs, hence exact in
-// fp16. Every step but the roundings named is in fp32.
+// fp16. Every step but the roundings named is in fp32. A group with a NaN or an infinity has no range: its scale is
+// NaN, and all of it reads as NaN.
 //
 // The bound is HBM: 2 D bytes in and D / 2 + D / 16 out a row, or the reverse. 8 lanes take a group, each the 16
 // bytes of 8 dims, which are 4 bytes of codes. A CTA works on one head of one sequence of K or V, and a thread
@@ -12,6 +13,7 @@
 // Measured (B200): 4 sequences of 4,096 tokens, 4 heads of 128, K and V (67 MB in fp16, 19 MB in 4 bits): append 16.5
 // us, 5.2 TB/s; read 10.5 us, 8.2 TB/s, as the cache is then in L2.
 #include <cuda_fp16.h>
+#include <math.h>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -20,6 +22,18 @@ namespace tattn {
 namespace {
 
 constexpr int kThreads = 256, kRows = 4;
+
+// A NaN on either side is the result (fminf and fmaxf give the other side).
+__device__ __forceinline__ float min_or_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 // This thread's work: dims [8 i, 8 i + 8) of rows t, t + step, ... (kRows of them, below T) of head hk of
 // sequence z. kv: 0 keys, 1 values.
@@ -78,13 +92,13 @@ __global__ void __launch_bounds__(kThreads) int4_append_kernel(const Int4CacheAr
     float lo = x[0], hi = x[0];
 #pragma unroll
     for (int e = 1; e < 8; ++e) {
-      lo = fminf(lo, x[e]);
-      hi = fmaxf(hi, x[e]);
+      lo = min_or_nan(lo, x[e]);
+      hi = max_or_nan(hi, x[e]);
     }
 #pragma unroll
     for (int o = 1; o < 8; o *= 2) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      lo = min_or_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = max_or_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
     if (t >= T) continue;
     const int64_t row = cache_row(a, p, t);
@@ -92,7 +106,8 @@ __global__ void __launch_bounds__(kThreads) int4_append_kernel(const Int4CacheAr
       if (p.i == 0) atomicOr(a.status, kStatusIndexRange);
       continue;
     }
-    const __half scale = __float2half_rn((hi - lo) / 15.f);
+    const float range = hi - lo;  // infinite or NaN where a value is
+    const __half scale = __float2half_rn(range < INFINITY ? range / 15.f : NAN);
     const float s = __half2float(scale);
     // The quotient (x - lo) / s, correctly rounded, by Markstein's theorem: with inv the correctly rounded 1 /
     // s and q0 = d inv, the remainder d - q0 s is exact in one FMA and q0 + remainder * inv rounds to the quotient.

@@ -35,10 +35,11 @@ class Int4Cache:
 
     A group of 64 head dims of a token's head is held as a scale s and a minimum m (fp16) and codes n in 0..15,
     which stand for fp16(s n + m); appending rounds to the nearest code. Of normal heads that is within a
-    thirtieth of the group's range. For keys and values each there are the tensors
-    ``*_codes`` uint8 [batch, kv_heads, capacity, dim / 2] (head dim 2 i in the low half of byte i) and
-    ``*_params`` float16 [batch, kv_heads, capacity, dim / 64, 2] (s, m); ``Int4Cache.empty`` makes them. The
-    cache holds no lengths: the caller says where rows go and how many there are. Head dims 64 and 128.
+    thirtieth of the group's range; a group with a NaN or an infinity in it reads as NaN throughout. For keys and
+    values each there are the tensors ``*_codes`` uint8 [batch, kv_heads, capacity, dim / 2] (head dim 2 i in the
+    low half of byte i) and ``*_params`` float16 [batch, kv_heads, capacity, dim / 64, 2] (s, m);
+    ``Int4Cache.empty`` makes them. The cache holds no lengths: the caller says where rows go and how many there
+    are. Head dims 64 and 128.
     """
 
     def __init__(
