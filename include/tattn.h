@@ -180,10 +180,10 @@ TATTN_API int64_t tattn_decode_workspace_bytes(int Z, int H, int Hk, int C, int 
  * All dense and 16-byte aligned.
  *
  * Append: rows t < T (t < counts[z] where counts is given) of k, v [Z, Hk, T, D] fp16 are written at positions
- * start[z] + t (start null: t) with m = min, s = fp16((max - m) / 15), n = round((x - m) / s), ties to even; 64 head
- * dims with a NaN or an infinity among them get s = NaN, so all of them read as NaN. A position outside [0, C) is
- * not written and sets TATTN_DEV_INDEX_RANGE. start, counts: device int32 [Z]. strides: 8 int64 = k, v each (z, h,
- * n, d); rows need unit D stride and 16-byte alignment. */
+ * start[z] + t (start null: t) with m = min, s = fp16((max - m) / 15), n = round((x - m) / s), ties to even. Where
+ * fp16(15 s + m) would be infinite, s is rounded down. 64 head dims with a NaN or an infinity among them get s = NaN,
+ * so all of them read as NaN. A position outside [0, C) is not written and sets TATTN_DEV_INDEX_RANGE. start, counts:
+ * device int32 [Z]. strides: 8 int64 = k, v each (z, h, n, d); rows need unit D stride and 16-byte alignment. */
 TATTN_API int tattn_int4_append(const void* k, const void* v, void* k_codes, void* k_params, void* v_codes,
                       void* v_params, const int32_t* start, const int32_t* counts, const int64_t* strides, int Z,
                       int Hk, int T, int C, int D, void* stream);

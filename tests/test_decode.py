@@ -541,3 +541,23 @@ def test_append_shows_what_is_not_a_number(gpu, d) -> None:
     only_v = Int4Cache(clean.k_codes, clean.k_params, cache.v_codes, cache.v_params)
     o, h = only_v.attend(q, _lens(80, 80)), hit[1].any(2).repeat_interleave(64, -1)[:, :, None]
     assert bool(o[h].isnan().all()) and torch.equal(o[~h], want[~h])
+
+
+@pytest.mark.gpu
+def test_the_whole_range_of_fp16_reads_back_finite(gpu) -> None:
+    """Groups that reach 65504, with minima from there down to -65504: each value is within half a step of its own, or
+    at the top within what 15 steps of a scale rounded down fall short (15 units in its last place: 120 at most),
+    and rounded to fp16 (16 there)."""
+    g = torch.Generator().manual_seed(26)
+    top = 65504.0
+    low = torch.cat((torch.tensor([-top, 0.0, -1.0, 1.0, 600.0, 65000.0, top]), (torch.rand(993, generator=g) * 2 - 1) * top))
+    x = (low[:, None] + torch.rand(1000, 64, generator=g) * (top - low[:, None])).half().clamp(-top, top)
+    x[:, 0], x[:, 1] = low.half(), top
+    x = torch.cat((x, -x), 1).cuda().reshape(1, 1, 1000, 128)  # and the same below zero
+    cache = Int4Cache.empty(1, 1, 1000, 128)
+    cache.append(x, x)
+    for y, p in zip(cache.read(1000), (cache.k_params, cache.v_params), strict=True):
+        s = p[..., 0].double().repeat_interleave(64, -1)
+        assert_within(y, x.double(), (s / 2).clamp(min=120) + 16, "values")
+    q = torch.full((1, 1, 1, 128), 1e-4, device="cuda", dtype=torch.float16)
+    assert bool(torch.isfinite(cache.attend(q, _lens(1000))).all())

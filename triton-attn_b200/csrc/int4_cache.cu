@@ -2,7 +2,8 @@
 //
 // A group of 64 head dims of a row x: m = min(x), s = fp16((max(x) - m) / 15), code n = round((x - m) / s) in
 // [0, 15] (ties to even; 0 where s = 0); it stands for fp16(s n + m). m is one of the inputs, hence exact in
-// fp16. Every step but the roundings named is in fp32. A group with a NaN or an infinity has no range: its scale is
+// fp16. Where s rounded up would make 15 s + m infinite, s is rounded down. Every step but the roundings named is in
+// fp32. A group with a NaN or an infinity has no range: its scale is
 // NaN, and all of it reads as NaN.
 //
 // The bound is HBM: 2 D bytes in and D / 2 + D / 16 out a row, or the reverse. 8 lanes take a group, each the 16
@@ -107,7 +108,10 @@ __global__ void __launch_bounds__(kThreads) int4_append_kernel(const Int4CacheAr
       continue;
     }
     const float range = hi - lo;  // infinite or NaN where a value is
-    const __half scale = __float2half_rn(range < INFINITY ? range / 15.f : NAN);
+    const float step = range < INFINITY ? range / 15.f : NAN;
+    __half scale = __float2half_rn(step);
+    // A step rounded up may take the largest code's value past fp16 (65520 rounds to infinity); rounded down it cannot.
+    if (fmaf(15.f, __half2float(scale), lo) >= 65520.f) scale = __float2half_rd(step);
     const float s = __half2float(scale);
     // The quotient (x - lo) / s, correctly rounded, by Markstein's theorem: with inv the correctly rounded 1 /
     // s and q0 = d inv, the remainder d - q0 s is exact in one FMA and q0 + remainder * inv rounds to the quotient.
