@@ -343,3 +343,29 @@ def test_side_stream_and_once_differentiable(gpu) -> None:
 
 def test_public_name() -> None:
     assert tattn.window_attention is window_attention and "window_attention" in tattn.__all__
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["f16", "f32"])
+@pytest.mark.parametrize("d", [16, 64, 128])
+@pytest.mark.parametrize("how", ["window", "causal", "full"])
+def test_a_key_that_is_not_a_number_shows(gpu, how, d, dtype) -> None:
+    """Head i has a NaN in key i, i + 100 or 299 - i: the queries that see it give NaN and every other one what it
+    gives without, wherever in a block the key lies."""
+    n, heads = 300, 48
+    q, k, v, _ = _qkv(1, heads, heads, n, n, d, dtype, 31)
+
+    def call(k):
+        return window_attention(q, k, v, 70, 9) if how == "window" else attention(q, k, v, causal=how == "causal")
+
+    clean = call(k)
+    p, j = torch.arange(n, device="cuda")[:, None], torch.arange(n, device="cuda")
+    see = {"window": (j <= p) & ((j > p - 70) | (j < 9)), "causal": j <= p, "full": (j >= 0).expand(n, n)}[how]
+    for at in (lambda i: i, lambda i: i + 100, lambda i: 299 - i):
+        bad, keys = k.clone(), torch.tensor([at(i) for i in range(heads)], device="cuda")
+        bad[0, torch.arange(heads, device="cuda"), keys, 5] = math.nan
+        o, shows = call(bad), see[:, keys].T  # [heads, n]
+        assert bool(o[0][shows].isnan().all()) and torch.equal(o[0][~shows], clean[0][~shows])
+    if how == "window":
+        m, clean_m = _forward(q, bad, v, 70, 9, 0.1)[1][0], _forward(q, k, v, 70, 9, 0.1)[1][0]
+        assert bool(m[shows].isnan().all()) and torch.equal(m[~shows], clean_m[~shows])

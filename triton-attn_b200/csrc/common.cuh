@@ -389,6 +389,13 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return r;
 }
 
+// The same where a NaN is the result if one of them is (max.f32 gives the largest of the others).
+__device__ __forceinline__ float fmax3_or_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // 2^x for a pair on the FMA/ALU pipes, leaving MUFU free for the other exponentials of a row.
 // Method: Cody-Waite style reduction x = j + f with j = round-to-nearest(x) obtained by adding the
 // shifter 1.5*2^23 (j lands in the low mantissa bits of t = x + shifter), f = x - j in [-0.5, 0.5];

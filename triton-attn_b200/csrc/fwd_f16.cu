@@ -29,8 +29,11 @@
 // us, 0.6 PFLOP/s. What bounds it then is each tile's chain of S, exponentials and P V.
 // The running max is rescaled lazily: O (in TMEM) and l are only corrected when a row's max grows by
 // more than kRescaleThreshold (log2 units); P values stay below 2^kRescaleThreshold, exact in fp16.
+// A NaN among a row's visible scores makes its maximum NaN, and with it M and O. (The exponentials on the FMA pipe
+// clamp, which makes a weight of 0 of a NaN: whether it showed depended on the key's place in its block.)
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
+#include <math.h>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -180,7 +183,7 @@ __device__ __forceinline__ void hide_columns(uint32_t* s, int lim, int first, in
   }
 }
 
-// Max of one row of raw scores; MASK ignores columns >= lim.
+// Max of one row of raw scores, NaN if one of them is; MASK ignores columns >= lim.
 template <int BN, bool MASK>
 __device__ __forceinline__ float row_max(const uint32_t* s, int lim) {
   float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -191,9 +194,9 @@ __device__ __forceinline__ float row_max(const uint32_t* s, int lim) {
       a = c < lim ? a : -INFINITY;
       b = c + 1 < lim ? b : -INFINITY;
     }
-    m[(c / 2) & 3] = fmax3(m[(c / 2) & 3], a, b);
+    m[(c / 2) & 3] = fmax3_or_nan(m[(c / 2) & 3], a, b);
   }
-  return fmax3(fmaxf(m[0], m[1]), m[2], m[3]);
+  return fmax3_or_nan(fmax3_or_nan(m[0], m[1], m[1]), m[2], m[3]);
 }
 
 // One row of P = exp2(S * scale - m) for columns [C0, C1) as fp16 pairs (p[c/2] = columns c, c+1) and
@@ -480,7 +483,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
       bool need = false;
       if (j == 0) {
         m_run = m_cand;
-      } else if (m_cand > m_run + kRescaleThreshold) {
+      } else if (!(m_cand <= m_run + kRescaleThreshold)) {
         alpha = ex2_approx(m_run - m_cand);
         m_run = m_cand;
         l_run *= alpha;
@@ -537,7 +540,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
 
     if (ok && n > 0 && warp_wait(&bar_o_done[i], (n - 1) & 1, ab)) {
       tc_fence_after();
-      const float inv_l = 1.f / l_run;
+      const float inv_l = m_run == m_run ? 1.f / l_run : NAN;  // (l itself misses a NaN on the FMA pipe)
       // The head index from shared memory rather than a register held through the block loop (one
       // spilled register fewer).
       const int bh_e = *reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
