@@ -369,3 +369,29 @@ def test_a_key_that_is_not_a_number_shows(gpu, how, d, dtype) -> None:
     if how == "window":
         m, clean_m = _forward(q, bad, v, 70, 9, 0.1)[1][0], _forward(q, k, v, 70, 9, 0.1)[1][0]
         assert bool(m[shows].isnan().all()) and torch.equal(m[~shows], clean_m[~shows])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["f16", "f32"])
+@pytest.mark.parametrize("d", [16, 64, 128])
+@pytest.mark.parametrize("how", ["window", "causal", "full"])
+def test_a_query_that_is_not_a_number_shows_in_the_gradients(gpu, how, d, dtype) -> None:
+    """Head i has a NaN in query i, i + 100 or 299 - i: its weights are NaN, so dV and dK of the keys that it sees are no
+    numbers, nor is its own dQ. In each of another head's gradients all is finite."""
+    n, heads = 300, 48
+    q, k, v, do = _qkv(1, heads, heads, n, n, d, dtype, 32)
+    p, j = torch.arange(n, device="cuda")[:, None], torch.arange(n, device="cuda")
+    see = {"window": (j <= p) & ((j > p - 70) | (j < 9)), "causal": j <= p, "full": (j >= 0).expand(n, n)}[how]
+    for at in (lambda i: i, lambda i: i + 100, lambda i: 299 - i):
+        bad, rows = q.clone(), torch.tensor([at(i) for i in range(heads)], device="cuda")
+        every = torch.arange(0, heads, 2, device="cuda")  # the even heads
+        bad[0, every, rows[every], 5] = math.nan
+        args = [t.clone().requires_grad_() for t in (bad, k, v)]
+        o = window_attention(*args, 70, 9) if how == "window" else attention(*args, causal=how == "causal")
+        dq, dk, dv = torch.autograd.grad(o, args, do)
+        shows = see[rows[every]]  # [heads, keys]
+        assert not bool(torch.isfinite(dq[0, every, rows[every]]).any())
+        for g in (dk, dv):
+            assert not bool(torch.isfinite(g[0, every][shows]).any())
+        for g in (dq, dk, dv):
+            assert bool(torch.isfinite(g[0, 1::2]).all())

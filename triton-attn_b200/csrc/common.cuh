@@ -390,6 +390,11 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
 }
 
 // The same where a NaN is the result if one of them is (max.f32 gives the largest of the others).
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float fmax3_or_nan(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -420,11 +425,12 @@ __device__ __forceinline__ uint64_t exp2_poly_x2(uint64_t x2) {
 }
 
 // The same with a degree-4 polynomial (max relative error 2.7e-6, one more packed FMA): accurate enough
-// that a gradient summed over thousands of query rows stays within the fp16 bound (the backward).
+// that a gradient summed over thousands of query rows stays within the fp16 bound (the backward). A NaN (a query whose
+// M is one) comes out as a NaN or, by the addition to the exponent, as the largest float, infinite in the fp16 P.
 __device__ __forceinline__ uint64_t exp2_poly4_x2(uint64_t x2) {
   float2 x = f2_unpack(x2);
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
+  x.x = max_or_nan(x.x, -126.f);
+  x.y = max_or_nan(x.y, -126.f);
   const uint64_t xc = f2(x.x, x.y);
   const uint64_t shifter = f2(12582912.f, 12582912.f);
   const uint64_t t = fadd2(xc, shifter);

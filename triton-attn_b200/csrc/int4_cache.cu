@@ -24,15 +24,10 @@ namespace {
 
 constexpr int kThreads = 256, kRows = 4;
 
-// A NaN on either side is the result (fminf and fmaxf give the other side).
+// A NaN on either side is the result (fminf gives the other side), as of max_or_nan.
 __device__ __forceinline__ float min_or_nan(float a, float b) {
   float r;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float max_or_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
