@@ -561,3 +561,30 @@ def test_the_whole_range_of_fp16_reads_back_finite(gpu) -> None:
         assert_within(y, x.double(), (s / 2).clamp(min=120) + 16, "values")
     q = torch.full((1, 1, 1, 128), 1e-4, device="cuda", dtype=torch.float16)
     assert bool(torch.isfinite(cache.attend(q, _lens(1000))).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["f16", "f32"])
+@pytest.mark.parametrize("sm_scale", [0.125, -0.125])
+def test_scores_of_minus_infinity(gpu, sm_scale, dtype) -> None:
+    """Keys with an infinity that makes their scores -infinity weigh nothing, also where they fill whole tiles, ahead
+    of all others or behind them; where all that is seen is such keys there is no result."""
+    q, k, v = _inputs(3, 4, 2, 700, 64, dtype, 27)
+    q[..., 3] = 1.0
+    lengths = (700, 300, 90)
+    for first, last in ((0, 60), (0, 690), (300, 700), (100, 130)):
+        bad = k.clone()
+        bad[:, :, first:last, 3] = math.copysign(math.inf, -sm_scale)
+        o = decode_attention(q, bad, v, _lens(*lengths), sm_scale=sm_scale)
+        for z, n in enumerate(lengths):
+            at = [j for j in range(n) if not first <= j < last]
+            if not at:
+                assert bool(o[z].isnan().all())
+                continue
+            want, bound = _decode64(
+                q[z : z + 1], k[z : z + 1, :, at], v[z : z + 1, :, at], (len(at),), None, 0, sm_scale, *_c(dtype, n)
+            )
+            assert_within(o[z : z + 1], want, bound, f"{first} to {last}, length {n}")
+    cut = decode_attention(q, bad, v, _lens(700, 110, 101), 10, 0, sm_scale)  # the window hides or shows them
+    assert bool(torch.isfinite(cut[0]).all()) and bool(cut[1].isnan().all()) and bool(torch.isfinite(cut[2]).all())
+    assert not bool(decode_attention(q, bad, v, _lens(0, 0, 0), sm_scale=sm_scale).any())

@@ -22,6 +22,7 @@
 // values of codes (the fp16 pipes are busy 49 % of the time and the integer ones 45 %). One sequence of 512 or 1,000
 // tokens: 4.5 and 5 us, of which the launch, the loads' latency and the join are each 1 to 2.
 #include <cuda_fp16.h>
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -126,14 +127,15 @@ __device__ __forceinline__ void mma16816_first(float* c, const uint32_t* a, uint
 }
 
 // A warp's running softmax over its tiles. Lane (g, t) holds columns (query heads) 2t, 2t + 1 of each of the
-// NT 8-head tiles: off = -m for a maximum m of the base-2 scores (the same in all g; +infinity before the first
-// tile) and its own rows' share of the sum l. M tiles of 16 output dims: o[mt][nt] as mma16816's c.
+// NT 8-head tiles: off = -m for a maximum m of the base-2 scores (the same in all g; the largest float before the
+// first score above -infinity, infinity if the warp has no tile) and its own rows' share of the sum l. M tiles of
+// 16 output dims: o[mt][nt] as mma16816's c.
 template <int D, int NT>
 struct WarpState {
   float off[NT][2], l[NT][2], o[D / 16][NT][4];
-  __device__ __forceinline__ void reset() {
+  __device__ __forceinline__ void reset(bool has_tile) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) off[nt][0] = off[nt][1] = INFINITY, l[nt][0] = l[nt][1] = 0.f;
+    for (int nt = 0; nt < NT; ++nt) off[nt][0] = off[nt][1] = has_tile ? FLT_MAX : INFINITY, l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
     for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
@@ -200,7 +202,7 @@ __device__ __forceinline__ void softmax_tile(WarpState<D, NT>& st, float (*x)[NT
 #pragma unroll
         for (int o = 4; o < 32; o *= 2) mx[nt][e] = fmaxf(mx[nt][e], __shfl_xor_sync(0xffffffffu, mx[nt][e], o));
         const float off = fminf(-scale * mx[nt][e], st.off[nt][e]);
-        alpha[nt][e] = st.off[nt][e] == INFINITY ? 0.f : ex2_approx(off - st.off[nt][e]);
+        alpha[nt][e] = ex2_approx(off - st.off[nt][e]);  // (nothing summed yet: of zeros)
         st.off[nt][e] = off;
       }
     rescale(st, alpha);
@@ -237,9 +239,11 @@ __device__ __forceinline__ float2 load_cluster2(uint32_t addr) {
   return x;
 }
 
+// o is divided by l, the sum beside the maximum m. m = -infinity: no token is seen, and the row is zeros. l = 0
+// otherwise: every score is -infinity, and the row 0 / 0.
 template <int D>
-__device__ __forceinline__ void write_row4(const DecodeArgs& a, int z, int h, int d, const float4& o, float l) {
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // NaN stays NaN
+__device__ __forceinline__ void write_row4(const DecodeArgs& a, int z, int h, int d, const float4& o, float m, float l) {
+  const float inv = m == -INFINITY ? 0.f : 1.f / l;
   *reinterpret_cast<uint2*>(static_cast<__half*>(a.o) + z * a.so.z + h * a.so.h + d) =
       make_uint2(pack_half2(o.x * inv, o.y * inv), pack_half2(o.z * inv, o.w * inv));
 }
@@ -294,7 +298,7 @@ __device__ __forceinline__ void finish(const DecodeArgs& a, const Part& p, WarpS
     }
     const int h = p.h0 + head;
     if (a.nsplit == 1) {
-      write_row4<D>(a, p.z, h, d, o, l);
+      write_row4<D>(a, p.z, h, d, o, m, l);
     } else if (a.nsplit <= kClusterParts) {
       *reinterpret_cast<float4*>(mine + head * D + d) = o;
       if (d == 0) *reinterpret_cast<float2*>(mine + HEADS * D + head * 2) = make_float2(m, l);
@@ -329,7 +333,7 @@ __device__ __forceinline__ void finish(const DecodeArgs& a, const Part& p, WarpS
       l = fmaf(f, ml_of[c].y, l);
       o = make_float4(fmaf(f, x[c].x, o.x), fmaf(f, x[c].y, o.y), fmaf(f, x[c].z, o.z), fmaf(f, x[c].w, o.w));
     }
-    write_row4<D>(a, p.z, p.h0 + head, d, o, l);
+    write_row4<D>(a, p.z, p.h0 + head, d, o, m, l);
   }
   cluster_sync();  // no CTA leaves while another reads its rows
 }
@@ -418,7 +422,7 @@ __global__ void __launch_bounds__(kThreads) decode_f16_kernel(const DecodeArgs a
   }
 
   WarpState<D, NT> st;
-  st.reset();
+  st.reset(base < p.t1);
   for (; base < p.t1; base += STEP) {
     cp_async_wait<C::STAGES - 2>();
     __syncwarp();
@@ -597,7 +601,7 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeArgs 
   }
 
   WarpState<D, NT> st;
-  st.reset();
+  st.reset(base < p.t1);
   // Keys in the order of mma16816's rows lie in the tile's rows (k >> 1) + 4 (k & 1) of each 8.
   const int row = (g >> 1) | ((g & 1) << 2);
   // The lane's places in a slot: of rows `row` (K) and t, t + 4 (V), the same in every 8 rows but for 8 ROW.
@@ -702,7 +706,7 @@ __global__ void __launch_bounds__(kThreads) decode_f32_kernel(const DecodeArgs a
   const float* q = static_cast<const float*>(a.q) + p.z * a.sq.z + p.h0 * a.sq.h + d;
   const float* kb = static_cast<const float*>(a.k) + p.z * a.sk.z + p.hk * a.sk.h + d;
   const float* vb = static_cast<const float*>(a.v) + p.z * a.sv.z + p.hk * a.sv.h + d;
-  float qv[E], o[E], m = -INFINITY, l = 0.f;
+  float qv[E], o[E], m = p.t0 + warp * U < p.t1 ? -FLT_MAX : -INFINITY, l = 0.f;  // as WarpState's -off
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     qv[e] = has ? q[e] * a.qk_scale : 0.f;
@@ -729,14 +733,14 @@ __global__ void __launch_bounds__(kThreads) decode_f32_kernel(const DecodeArgs a
       if (t + u >= p.t1) x[u] = -INFINITY;
       mx = fmaxf(mx, x[u]);
     }
-    const float use = mx == -INFINITY ? 0.f : mx, alpha = exp2f(m - use);
+    const float alpha = exp2f(m - mx);
     m = mx;
     l *= alpha;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] *= alpha;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const float w = exp2f(x[u] - use);
+      const float w = exp2f(x[u] - m);
       l += w;
 #pragma unroll
       for (int e = 0; e < E; ++e) o[e] = fmaf(w, v[u][e], o[e]);
@@ -763,7 +767,7 @@ __global__ void __launch_bounds__(kThreads) decode_f32_kernel(const DecodeArgs a
       acc = fmaf(f, so[w][c], acc);
     }
     if (a.nsplit == 1) {
-      static_cast<float*>(a.o)[p.z * a.so.z + p.h0 * a.so.h + c] = l == 0.f ? 0.f : acc / l;
+      static_cast<float*>(a.o)[p.z * a.so.z + p.h0 * a.so.h + c] = m == -INFINITY ? 0.f : acc / l;
     } else {
       const int64_t row = (int64_t(p.z) * a.H + p.h0) * a.nsplit + p.split;
       a.part[row * D + c] = acc;
@@ -808,10 +812,10 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeArgs 
   }
   const int z = row / a.H, h = row % a.H;
   if constexpr (sizeof(T) == 2) {
-    write_row4<D>(a, z, h, 4 * t, acc, l);
+    write_row4<D>(a, z, h, 4 * t, acc, m, l);
   } else {
     float* out = static_cast<float*>(a.o) + z * a.so.z + h * a.so.h + 4 * t;
-    const float den = l == 0.f ? 1.f : l;  // (then acc is 0)
+    const float den = m == -INFINITY ? 1.f : l;  // (acc is 0 then)
     *reinterpret_cast<float4*>(out) = make_float4(acc.x / den, acc.y / den, acc.z / den, acc.w / den);
   }
 }
