@@ -395,3 +395,28 @@ def test_a_query_that_is_not_a_number_shows_in_the_gradients(gpu, how, d, dtype)
             assert not bool(torch.isfinite(g[0, every][shows]).any())
         for g in (dq, dk, dv):
             assert bool(torch.isfinite(g[0, 1::2]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["f16", "f32"])
+@pytest.mark.parametrize("d", [16, 64, 128])
+def test_scores_of_minus_infinity(gpu, d, dtype) -> None:
+    """Keys with an infinity that makes their scores -infinity weigh nothing; a query that sees no others has no result
+    and a log-sum-exp of -infinity."""
+    n = 300
+    q, k, v, _ = _qkv(1, 4, 2, n, n, d, dtype, 33)
+    q[..., 3] = 1.0
+    for first, last in ((0, 150), (0, 290), (130, 300)):
+        bad = k.clone()
+        bad[:, :, first:last, 3] = -math.inf
+        o, m = _forward(q, bad, v, 70, 0, 0.2)
+        p, j = torch.arange(n, device="cuda")[:, None], torch.arange(n, device="cuda")
+        see = (j <= p) & (j > p - 70) & ((j < first) | (j >= last))
+        none = ~see.any(1)
+        assert bool(o[:, :, none].isnan().all()) and bool((m[:, :, none] == -math.inf).all())
+        x = (q.double() @ k.repeat_interleave(2, 1).double().transpose(-1, -2) * 0.2).masked_fill(~see, -math.inf)
+        w = torch.softmax(x, -1)[:, :, ~none]
+        vx = v.repeat_interleave(2, 1).double()
+        # As plain64: each weight is off by c of it, the result by its rounding.
+        c, u = (1e-3, 2.0**-11) if dtype == torch.float16 else ((n + d) * 2.0**-23 + 1e-6, 2.0**-24)
+        assert_within(o[:, :, ~none], w @ vx, c * (w @ vx.abs()) + 2 * u * (w @ vx).abs() + 2.0**-24, "o")

@@ -540,7 +540,8 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
 
     if (ok && n > 0 && warp_wait(&bar_o_done[i], (n - 1) & 1, ab)) {
       tc_fence_after();
-      const float inv_l = m_run == m_run ? 1.f / l_run : NAN;  // (l itself misses a NaN on the FMA pipe)
+      // No result where the largest score is NaN, or infinite of either sign (l itself misses some of that).
+      const float inv_l = m_run - m_run == 0.f ? 1.f / l_run : NAN;
       // The head index from shared memory rather than a register held through the block loop (one
       // spilled register fewer).
       const int bh_e = *reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
