@@ -588,3 +588,14 @@ def test_scores_of_minus_infinity(gpu, sm_scale, dtype) -> None:
     cut = decode_attention(q, bad, v, _lens(700, 110, 101), 10, 0, sm_scale)  # the window hides or shows them
     assert bool(torch.isfinite(cut[0]).all()) and bool(cut[1].isnan().all()) and bool(torch.isfinite(cut[2]).all())
     assert not bool(decode_attention(q, bad, v, _lens(0, 0, 0), sm_scale=sm_scale).any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sm_scale", [math.nan, math.inf, -math.inf])
+def test_a_scale_that_is_no_number_shows(gpu, sm_scale) -> None:
+    for dtype in (torch.float16, torch.float32):
+        q, k, v = _inputs(2, 4, 2, 90, 64, dtype, 28)
+        assert bool(decode_attention(q, k, v, _lens(90, 50), sm_scale=sm_scale).isnan().all())
+        assert bool(window_attention(q, k, v, 40, sm_scale=sm_scale).isnan().all())
+        assert not bool(decode_attention(q, k, v, _lens(0, 0), sm_scale=sm_scale).any())
+    assert bool(_filled(2, 2, 90, 64, 29).attend(q.half(), _lens(90, 50), sm_scale=sm_scale).isnan().all())

@@ -148,7 +148,7 @@ struct WarpState {
 __device__ __forceinline__ float positive_scale(float qk_scale) {
   // Below 2^-60 scores vanish against 1: a scale of 0 gives the weights that it should and still leaves the
   // -infinity of a key that does not exist what it is. The sign goes into Q.
-  return fmaxf(fabsf(qk_scale), 0x1p-60f);
+  return fabsf(qk_scale) < 0x1p-60f ? 0x1p-60f : fabsf(qk_scale);  // (NaN stays)
 }
 template <int D, int NT>
 __device__ __forceinline__ void rescale(WarpState<D, NT>& st, const float (*alpha)[2]) {
