@@ -599,3 +599,16 @@ def test_a_scale_that_is_no_number_shows(gpu, sm_scale) -> None:
         assert bool(window_attention(q, k, v, 40, sm_scale=sm_scale).isnan().all())
         assert not bool(decode_attention(q, k, v, _lens(0, 0), sm_scale=sm_scale).any())
     assert bool(_filled(2, 2, 90, 64, 29).attend(q.half(), _lens(90, 50), sm_scale=sm_scale).isnan().all())
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_forward_mode_derivatives_are_refused(which) -> None:
+    """Without a GPU: before the device check."""
+    with torch.autograd.forward_ad.dual_level():
+        args = [_cpu(2, 4, 1, 64), _cpu(2, 2, 8, 64), _cpu(2, 2, 8, 64)]
+        args[which] = torch.autograd.forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        for take in (torch.enable_grad, torch.no_grad):
+            with take(), pytest.raises(NotImplementedError, match="forward-mode"):
+                decode_attention(*args, _len(2))
+            with take(), pytest.raises(NotImplementedError, match="forward-mode"):
+                _cache().append(*args[1:]) if which else _cache().attend(args[0], _len(2))

@@ -281,3 +281,14 @@ def test_reproducible_empty_and_streams(gpu) -> None:
     outs = qk_norm_rope(*none, *args[2:], cos, sin)
     grads = torch.autograd.grad(outs, (*none, *args[2:]), outs)
     assert outs[0].shape == none[0].shape and not bool(grads[2].any()) and not bool(grads[3].any())
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_forward_mode_derivatives_are_refused(which) -> None:
+    """For each tensor that could carry a tangent. (Without a GPU: before the device check.)"""
+    with torch.autograd.forward_ad.dual_level():
+        args = [torch.zeros(1, 2, 8, 16), torch.zeros(1, 1, 8, 16), *[torch.ones(16)] * 2, *[torch.ones(8, 8)] * 2]
+        args[which] = torch.autograd.forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        for take in (torch.enable_grad, torch.no_grad):
+            with take(), pytest.raises(NotImplementedError, match="forward-mode"):
+                qk_norm_rope(*args)

@@ -420,3 +420,14 @@ def test_scores_of_minus_infinity(gpu, d, dtype) -> None:
         # As plain64: each weight is off by c of it, the result by its rounding.
         c, u = (1e-3, 2.0**-11) if dtype == torch.float16 else ((n + d) * 2.0**-23 + 1e-6, 2.0**-24)
         assert_within(o[:, :, ~none], w @ vx, c * (w @ vx.abs()) + 2 * u * (w @ vx).abs() + 2.0**-24, "o")
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_forward_mode_derivatives_are_refused(which) -> None:
+    """As tattn.attention refuses them: not a result without a tangent. (Without a GPU: before the device check.)"""
+    with torch.autograd.forward_ad.dual_level():
+        args = [_cpu(1, 2, 8, 16) for _ in range(3)]
+        args[which] = torch.autograd.forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        for take in (torch.enable_grad, torch.no_grad):
+            with take(), pytest.raises(NotImplementedError, match="forward-mode"):
+                window_attention(*args, 4)

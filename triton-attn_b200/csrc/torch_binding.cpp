@@ -101,6 +101,11 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (t->requires_grad()) return true;
   return false;
 }
+// None of the operators carries forward-mode derivatives: a result without a tangent would say that it is zero.
+void refuse_forward_mode(const char* fn, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), fn, " has no forward-mode derivatives");
+}
 // A backward that can be differentiated once: its results raise when differentiated again.
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -146,6 +151,7 @@ void check_norm_rope(const Tensor& q, const Tensor& k, const Tensor& wq, const T
     CHECK_VALUE(cos.size(0) > 0 || b * n == 0, "the tables hold no positions");
     CHECK_VALUE(p.device() == q.device(), "all tensors must be on one device, got ", q.device(), " and ", p.device());
   }
+  refuse_forward_mode("qk_norm_rope", {&q, &k, &wq, &wk, &cos, &sin});
   for (const Tensor* t : {&k, &wq, &wk, &cos, &sin})
     CHECK_VALUE(t->device() == q.device(), "all tensors must be on one device, got ", q.device(), " and ", t->device());
   require_cuda(q);
@@ -345,6 +351,7 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
   check_window(window, sinks);
   CHECK_VALUE(k.size(2) >= q.size(2), "the queries are the last of the keys' sequence; got ", q.size(2), " queries, ",
                     k.size(2), " keys");
+  refuse_forward_mode("window_attention", {&q, &k, &v});
   require_cuda(q);
   if (!wants_grad({&q, &k, &v})) return std::get<0>(window_forward(q, k, v, window, sinks, scale_of(sm_scale, q)));
   return WindowAttention::apply(q, k, v, window, sinks, scale_of(sm_scale, q));
@@ -364,6 +371,7 @@ Tensor decode_attention(const Tensor& q0, const Tensor& k, const Tensor& v, cons
                         const std::optional<int64_t>& window, int64_t sinks, const std::optional<double>& sm_scale) {
   check_heads(q0, k, v);
   check_token(q0, lengths0, window, sinks);
+  refuse_forward_mode("decode_attention", {&q0, &k, &v});
   require_cuda(q0);
   CHECK_VALUE(rows16_ok(k) && rows16_ok(v),
                     "k and v need contiguous, 16-byte aligned rows: a cache is read in place, never copied");
@@ -422,6 +430,7 @@ void int4_append(const Tensor& kc, const Tensor& kp, const Tensor& vc, const Ten
   CHECK_VALUE(k0.device() == kc.device() && v0.device() == kc.device(), "k, v and the cache must be on one device, got ",
                     k0.device(), ", ", v0.device());
   const std::optional<Tensor> start = check_index("start", start0, kc), counts = check_index("counts", counts0, kc);
+  refuse_forward_mode("Int4Cache.append", {&k0, &v0});
   require_cuda(k0);
   const Tensor k = rows16(k0), v = rows16(v0);
   Strides st;
@@ -459,6 +468,7 @@ Tensor int4_attend(const Tensor& kc, const Tensor& kp, const Tensor& vc, const T
   CHECK_VALUE(q0.scalar_type() == at::kHalf, "q must be float16, got ", q0.scalar_type());
   CHECK_VALUE(q0.device() == kc.device(), "q and the cache must be on one device, got ", q0.device(), ", ", kc.device());
   check_token(q0, lengths0, window, sinks);
+  refuse_forward_mode("Int4Cache.attend", {&q0});
   require_cuda(q0);
   const Tensor q = rows16(q0), lengths = lengths0.contiguous();
   Tensor o = like(q);

@@ -35,7 +35,8 @@ def window_attention(
 
     q is [batch, heads, seq, dim]; k and v are [batch, kv_heads, kv_seq, dim] with kv_heads dividing heads and
     kv_seq >= seq. Query i stands at position p = kv_seq - seq + i and sees the keys j <= p with j > p - window
-    or j < sinks. Returns a tensor like q; gradients reach q, k and v. As in any masked product, a NaN or an
-    infinity in v reaches queries near its token that do not see it.
+    or j < sinks. Returns a tensor like q; gradients reach q, k and v, once and in reverse mode (forward-mode
+    tensors are refused). As in any masked product, a NaN or an infinity in v reaches queries near its token that
+    do not see it.
     """
     return _lib.torch_ext().window_attention(q, k, v, window, sinks, sm_scale)
