@@ -612,3 +612,18 @@ def test_forward_mode_derivatives_are_refused(which) -> None:
                 decode_attention(*args, _len(2))
             with take(), pytest.raises(NotImplementedError, match="forward-mode"):
                 _cache().append(*args[1:]) if which else _cache().attend(args[0], _len(2))
+
+
+@pytest.mark.parametrize("which", [1, 2])
+def test_keys_and_values_that_need_gradients_are_refused(which) -> None:
+    """Of each tensor alone; without gradients being recorded they are taken (as far as the device check)."""
+    args = [_cpu(2, 4, 1, 64), _cpu(2, 2, 8, 64), _cpu(2, 2, 8, 64)]
+    args[which].requires_grad_()
+    with pytest.raises(RuntimeError, match="no backward"):
+        decode_attention(*args, _len(2))
+    with pytest.raises(RuntimeError, match="no gradients"):
+        _cache().append(*args[1:])
+    with torch.no_grad():
+        for call in (lambda: decode_attention(*args, _len(2)), lambda: _cache().append(*args[1:])):
+            with pytest.raises(RuntimeError, match="no CPU path"):
+                call()

@@ -358,19 +358,22 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
 }
 
 // ------------------------------------------------------------------------- single tokens over a cache
-void check_token(const Tensor& q, const Tensor& lengths, const std::optional<int64_t>& window, int64_t sinks) {
+// inputs: q, and the keys and values that may need gradients.
+void check_token(std::initializer_list<const Tensor*> inputs, const Tensor& lengths, const std::optional<int64_t>& window,
+                 int64_t sinks) {
+  const Tensor& q = **inputs.begin();
   CHECK_VALUE(q.size(2) == 1, "q holds one token of each sequence; got ", q.sizes());
   CHECK_VALUE(lengths.scalar_type() == at::kInt && lengths.dim() == 1 && lengths.size(0) == q.size(0),
                     "lengths must be int32 [", q.size(0), "]; got ", lengths.scalar_type(), " ", lengths.sizes());
   CHECK_VALUE(lengths.device() == q.device(), "lengths must be on q's device, got ", lengths.device());
-  TORCH_CHECK(!wants_grad({&q}), "attention over a cache has no backward pass; use window_attention, or torch.no_grad()");
+  TORCH_CHECK(!wants_grad(inputs), "attention over a cache has no backward pass; use window_attention, or torch.no_grad()");
   check_window(window, sinks);
 }
 
 Tensor decode_attention(const Tensor& q0, const Tensor& k, const Tensor& v, const Tensor& lengths0,
                         const std::optional<int64_t>& window, int64_t sinks, const std::optional<double>& sm_scale) {
   check_heads(q0, k, v);
-  check_token(q0, lengths0, window, sinks);
+  check_token({&q0, &k, &v}, lengths0, window, sinks);
   refuse_forward_mode("decode_attention", {&q0, &k, &v});
   require_cuda(q0);
   CHECK_VALUE(rows16_ok(k) && rows16_ok(v),
@@ -430,6 +433,7 @@ void int4_append(const Tensor& kc, const Tensor& kp, const Tensor& vc, const Ten
   CHECK_VALUE(k0.device() == kc.device() && v0.device() == kc.device(), "k, v and the cache must be on one device, got ",
                     k0.device(), ", ", v0.device());
   const std::optional<Tensor> start = check_index("start", start0, kc), counts = check_index("counts", counts0, kc);
+  TORCH_CHECK(!wants_grad({&k0, &v0}), "the cache carries no gradients; detach k and v, or use torch.no_grad()");
   refuse_forward_mode("Int4Cache.append", {&k0, &v0});
   require_cuda(k0);
   const Tensor k = rows16(k0), v = rows16(v0);
@@ -467,7 +471,7 @@ Tensor int4_attend(const Tensor& kc, const Tensor& kp, const Tensor& vc, const T
                     "query heads must be a multiple of key/value heads; got ", q0.size(1), " and ", kc.size(1));
   CHECK_VALUE(q0.scalar_type() == at::kHalf, "q must be float16, got ", q0.scalar_type());
   CHECK_VALUE(q0.device() == kc.device(), "q and the cache must be on one device, got ", q0.device(), ", ", kc.device());
-  check_token(q0, lengths0, window, sinks);
+  check_token({&q0}, lengths0, window, sinks);
   refuse_forward_mode("Int4Cache.attend", {&q0});
   require_cuda(q0);
   const Tensor q = rows16(q0), lengths = lengths0.contiguous();

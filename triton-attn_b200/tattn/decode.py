@@ -1,8 +1,9 @@
 """Attention of one new token of each sequence over a cache: ``decode_attention`` over keys and values in the
 queries' dtype, ``Int4Cache`` holding them in 4 bits.
 
-The single-token form of ``tattn.window_attention``, for generation: no gradients, nothing read from the device
-(the lengths stay there), so a step can be captured in a CUDA graph.
+The single-token form of ``tattn.window_attention``, for generation: no gradients (tensors that need them are refused
+where gradients are recorded), nothing read from the device (the lengths stay there), so a step can be captured in a
+CUDA graph.
 """
 
 from __future__ import annotations
@@ -86,7 +87,8 @@ class Int4Cache:
     ) -> None:
         """Hold the rows of k and v, fp16 [batch, kv_heads, seq, dim], from position start[b] of sequence b on (None:
         0); with ``counts`` only the first counts[b] of them. Both are int32 [batch], on the device. A row past
-        the capacity is not held and sets DEV_INDEX_RANGE in the device status word."""
+        the capacity is not held and sets DEV_INDEX_RANGE in the device status word. k and v that need gradients are
+        refused: the cache carries none."""
         _lib.torch_ext().int4_append(self.k_codes, self.k_params, self.v_codes, self.v_params, k, v, start, counts)
 
     def read(self, count: int, start: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
