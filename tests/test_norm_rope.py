@@ -292,3 +292,14 @@ def test_forward_mode_derivatives_are_refused(which) -> None:
         for take in (torch.enable_grad, torch.no_grad):
             with take(), pytest.raises(NotImplementedError, match="forward-mode"):
                 qk_norm_rope(*args)
+
+
+@pytest.mark.parametrize("which", [4, 5])
+def test_tables_that_need_gradients_are_refused(which) -> None:
+    """Gradients reach q, k and the weights; a table would get none. (Without a GPU: before the device check.)"""
+    args = [torch.zeros(1, 2, 8, 16), torch.zeros(1, 1, 8, 16), *[torch.ones(16)] * 2, *[torch.ones(8, 8)] * 2]
+    args[which] = args[which].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        qk_norm_rope(*args)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+        qk_norm_rope(*args)

@@ -151,6 +151,7 @@ void check_norm_rope(const Tensor& q, const Tensor& k, const Tensor& wq, const T
     CHECK_VALUE(cos.size(0) > 0 || b * n == 0, "the tables hold no positions");
     CHECK_VALUE(p.device() == q.device(), "all tensors must be on one device, got ", q.device(), " and ", p.device());
   }
+  TORCH_CHECK(!wants_grad({&cos, &sin}), "cos and sin get no gradients; detach them");
   refuse_forward_mode("qk_norm_rope", {&q, &k, &wq, &wk, &cos, &sin});
   for (const Tensor* t : {&k, &wq, &wk, &cos, &sin})
     CHECK_VALUE(t->device() == q.device(), "all tensors must be on one device, got ", q.device(), " and ", t->device());

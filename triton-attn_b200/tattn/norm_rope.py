@@ -24,6 +24,7 @@ def qk_norm_rope(
     are (j, j + dim / 2) or, interleaved, (2 j, 2 j + 1). Token n of a sequence stands at p = n, or where
     ``positions`` (int32 [seq] or [batch, seq]) says; a position outside the tables gives NaN rows and
     sets DEV_INDEX_RANGE in the device status word. Weights are [dim], of q's dtype or float32; gradients
-    reach q, k and the weights, once and in reverse mode (forward-mode tensors are refused).
+    reach q, k and the weights, once and in reverse mode (forward-mode tensors, and tables that need gradients, are
+    refused).
     """
     return _lib.torch_ext().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
