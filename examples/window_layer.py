@@ -33,9 +33,11 @@ class WindowLayer(nn.Module):
         self.qkv = nn.Linear(width, (heads + 2 * kv_heads) * dim, bias=False)
         self.out = nn.Linear(heads * dim, width, bias=False)
         self.q_norm, self.k_norm = nn.Parameter(torch.ones(dim)), nn.Parameter(torch.ones(dim))
-        angle = torch.arange(positions)[:, None] * 10000.0 ** (-torch.arange(0, dim, 2) / dim)
-        self.register_buffer("cos", angle.cos(), persistent=False)
-        self.register_buffer("sin", angle.sin(), persistent=False)
+        # Angles in 64 bits (one of thousands in 32 is off by 2^-12), their cosines and sines in 32.
+        inverse = 10000.0 ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+        angle = torch.arange(positions, dtype=torch.float64)[:, None] * inverse
+        self.register_buffer("cos", angle.cos().float(), persistent=False)
+        self.register_buffer("sin", angle.sin().float(), persistent=False)
 
     def _project(
         self, x: torch.Tensor, positions: torch.Tensor | None
@@ -64,6 +66,14 @@ class WindowLayer(nn.Module):
         cache.append(k, v, held)
         held.add_(1)
         return self._merge(cache.attend(q, held, self.window, self.sinks))
+
+
+def make_layer(width: int, device: str) -> WindowLayer:
+    """The projections in fp16; the norms' weights and the tables stay in fp32."""
+    layer = WindowLayer(width, heads=8, kv_heads=2, dim=64, window=64, sinks=4)
+    layer.qkv.half()
+    layer.out.half()
+    return layer.to(device)
 
 
 def train(layer: WindowLayer, steps: int, batch: int, seq: int, width: int) -> list[float]:
@@ -114,9 +124,7 @@ def generate(layer: WindowLayer, batch: int, prompt: int, tokens: int, width: in
 def main() -> tuple[list[float], float]:
     torch.manual_seed(0)
     width = 256
-    layer = WindowLayer(width, heads=8, kv_heads=2, dim=64, window=64, sinks=4).cuda().half()
-    layer.q_norm.data, layer.k_norm.data = layer.q_norm.data.float(), layer.k_norm.data.float()
-    layer.cos, layer.sin = layer.cos.float(), layer.sin.float()
+    layer = make_layer(width, "cuda")
     losses = train(layer, 60, batch=4, seq=500, width=width)
     print(f"training loss {losses[0]:.3f} -> {losses[-1]:.3f}")
     steps, whole = generate(layer, batch=3, prompt=150, tokens=40, width=width)
