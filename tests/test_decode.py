@@ -627,3 +627,77 @@ def test_keys_and_values_that_need_gradients_are_refused(which) -> None:
         for call in (lambda: decode_attention(*args, _len(2)), lambda: _cache().append(*args[1:])):
             with pytest.raises(RuntimeError, match="no CPU path"):
                 call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_attend_against_the_values_that_codes_stand_for(gpu, case, d) -> None:
+    """The format's values are fp16(s n + m), which read gives (checked bit for bit above); over them a 4-bit cache is
+    held to what an fp16 cache is."""
+    h, hk, cap, lengths, window, sinks = case
+    cache = _filled(len(lengths), hk, cap, d, 30)
+    q, _, _ = _inputs(len(lengths), h, 1, 1, d, torch.float16, 31)
+    o = cache.attend(q, _lens(*lengths), window, sinks)
+    k, v = cache.read(cap)
+    assert_within(o, *_decode64(q, k, v, lengths, window, sinks, 1 / math.sqrt(d), *_c(torch.float16, cap)), "o")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_takes_the_rounded_values(gpu, d) -> None:
+    """Keys around 8 in a range of a quarter: fp16(s n + m) is up to 2^-8 from s n + m, which under queries of 16 moves a
+    score by some 0.04 and the weights of five tokens by as much. c: 1e-3 as above, and twice what fp32 sums of d
+    products (d 2^-24 of the sum of their sizes) leave in the exponent."""
+    _, k, v = _inputs(8, 1, 2, 5, d, torch.float16, 32)
+    q, _, _ = _inputs(8, 8, 1, 1, d, torch.float16, 33)
+    q, k = 16 * q, (8 + 0.05 * k.float()).half()
+    cache = Int4Cache.empty(8, 2, 5, d)
+    cache.append(k, v)
+    o = cache.attend(q, _lens(*[5] * 8))
+    k, v = cache.read(5)
+    scale = d**-0.5
+    size = float((q.double().abs().sum(-1) * 8.2).max()) * scale
+    c = 1e-3 + 2 * d * 2.0**-24 * size
+    want, bound = _decode64(q, k, v, [5] * 8, None, 0, scale, c, 2.0**-11)
+    assert_within(o, want, bound, "o")
+    unrounded = []
+    for codes, params in zip(_codes(cache), (cache.k_params, cache.v_params), strict=True):
+        p = params.double()
+        unrounded.append((p[..., :1] * codes.double().unflatten(-1, (-1, 64)) + p[..., 1:]).flatten(-2))
+    other, _ = _decode64(q, *unrounded, [5] * 8, None, 0, scale, c, 2.0**-11)
+    assert int(((other - want).abs() > bound).sum()) > 100  # the test tells the two apart
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [2e-4, 1000.0])
+def test_attend_small_and_large_values_as_read(gpu, size) -> None:
+    """Scales near fp16's subnormals, and scores of some thousands: fp32 sums of 128 products (128 2^-24 of the sum of
+    their sizes) are twice in c."""
+    cache = _filled(2, 2, 200, 128, 34, size)
+    q, _, _ = _inputs(2, 4, 1, 1, 128, torch.float16, 35)
+    k, v = cache.read(200)
+    terms = float((q[:, :, 0].double().abs().unflatten(1, (2, 2)) @ k.double().abs().transpose(-1, -2)).max()) * 128**-0.5
+    c = 1e-3 + 2 * 128 * 2.0**-24 * terms
+    o = cache.attend(q, _lens(200, 150))
+    assert_within(o, *_decode64(q, k, v, (200, 150), None, 0, 128**-0.5, c, 2.0**-11), "o")
+
+
+@pytest.mark.gpu
+def test_attend_with_very_unequal_tokens_as_read(gpu) -> None:
+    """Values of neighbouring tokens a thousand times apart, either kind first, the small ones with nearly all of the
+    weight: nothing is lost beyond each product's own rounding. A weight below 2^-14 of the largest one is rounded to
+    2^-25 of that, in fp16's subnormals."""
+    for first in (1.0, 1e-3):
+        _, k, v = _inputs(1, 1, 1, 300, 64, torch.float16, 36)
+        sizes = torch.where(torch.arange(300, device="cuda") % 150 < 75, first, 1e-3 / first).half()
+        q, _, _ = _inputs(1, 2, 1, 1, 64, torch.float16, 37)
+        k[0, 0, :, 0] = torch.where(sizes < 0.5, 2.0, -2.0).half()
+        q[..., 0] = 20
+        cache = Int4Cache.empty(1, 1, 300, 64)
+        cache.append(k, v * sizes[None, None, :, None])
+        o = cache.attend(q, _lens(300))
+        kx, vx = cache.read(300)
+        want, bound = _decode64(q, kx, vx, (300,), None, 0, 0.125, 1e-3, 2.0**-11)
+        most = torch.softmax(kx[0, 0].double() @ q[0, :, 0].double().T * 0.125, 0).max()
+        assert_within(o, want, bound + 2.0**-25 * most * vx.double().abs().sum(2, keepdim=True), "o")
