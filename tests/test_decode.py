@@ -701,3 +701,31 @@ def test_attend_with_very_unequal_tokens_as_read(gpu) -> None:
         want, bound = _decode64(q, kx, vx, (300,), None, 0, 0.125, 1e-3, 2.0**-11)
         most = torch.softmax(kx[0, 0].double() @ q[0, :, 0].double().T * 0.125, 0).max()
         assert_within(o, want, bound + 2.0**-25 * most * vx.double().abs().sum(2, keepdim=True), "o")
+
+
+@pytest.mark.gpu
+def test_caches_on_side_streams(gpu) -> None:
+    """Two streams append to caches of their own and attend over them at the same time (parts joined by a second kernel,
+    through a workspace): each gets what it gets alone."""
+    cap, lengths = 40000, _lens(40000)
+
+    def work(i):
+        q, k, v = rows[i]
+        cache = Int4Cache.empty(1, 1, cap, 64)
+        cache.append(k, v)
+        return cache.attend(q, lengths), decode_attention(q, k, v, lengths)
+
+    rows = [_inputs(1, 2, 1, cap, 64, torch.float16, 38 + i) for i in range(2)]
+    want = [work(i) for i in range(2)]
+    torch.cuda.synchronize()
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(8):
+        for i, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                got[i].append(work(i))
+    for side in sides:
+        side.synchronize()
+    for results, first in zip(got, want, strict=True):
+        for result in results:
+            assert all(torch.equal(a, b) for a, b in zip(result, first, strict=True))

@@ -303,3 +303,31 @@ def test_tables_that_need_gradients_are_refused(which) -> None:
         qk_norm_rope(*args)
     with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
         qk_norm_rope(*args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["f16", "f32"])
+def test_forward_and_backward_on_side_streams(gpu, dtype) -> None:
+    """Two streams work on different inputs at the same time, forward and backward: each gets what its inputs give alone
+    (the results are bitwise reproducible)."""
+    cos, sin = _tables(1000, 64)
+    inputs = [_inputs(2, 16, 4, 1000, 64, dtype, 50 + i) for i in range(2)]
+    args = [[t.clone().requires_grad_() for t in x[:4]] for x in inputs]
+
+    def both(i):
+        outs = qk_norm_rope(*args[i], cos, sin)
+        return (*outs, *torch.autograd.grad(outs, args[i], inputs[i][4:]))
+
+    want = [both(i) for i in range(2)]
+    torch.cuda.synchronize()
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(8):
+        for i, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                got[i].append(both(i))
+    for side in sides:
+        side.synchronize()
+    for results, first in zip(got, want, strict=True):
+        for result in results:
+            assert all(torch.equal(a, b) for a, b in zip(result, first, strict=True))

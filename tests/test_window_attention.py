@@ -431,3 +431,30 @@ def test_forward_mode_derivatives_are_refused(which) -> None:
         for take in (torch.enable_grad, torch.no_grad):
             with take(), pytest.raises(NotImplementedError, match="forward-mode"):
                 window_attention(*args, 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["f16", "f32"])
+def test_forward_and_backward_on_side_streams(gpu, dtype) -> None:
+    """Two streams work on different inputs at the same time, forward and backward (whose kernel has its workspace and a
+    barrier over its few CTAs): each gets its own inputs' results."""
+    b, h, hk, n, d, window, sinks = 1, 4, 2, 500, 64, 100, 130
+    inputs = [_qkv(b, h, hk, n, n, d, dtype, 40 + i) for i in range(2)]
+    want = [window_attention64(*x, window, sinks, d**-0.5) for x in inputs]
+    args = [[t.detach().clone().requires_grad_() for t in x[:3]] for x in inputs]
+    torch.cuda.synchronize()
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(8):
+        for i, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                o = window_attention(*args[i], window, sinks)
+                got[i].append((o, *torch.autograd.grad(o, args[i], inputs[i][3])))
+    for side in sides:
+        side.synchronize()
+    for results, (outs, bounds) in zip(got, want, strict=True):
+        for result in results:
+            for g, w, e, name in zip(result, outs, bounds, ("o", "dq", "dk", "dv"), strict=True):
+                assert_within(g, w, e, name)
+                if dtype == torch.float32 or name != "dq":  # (its sums vary in order in fp16)
+                    assert torch.equal(g, results[0][("o", "dq", "dk", "dv").index(name)])
