@@ -18,9 +18,10 @@
 //
 // Measured (B200): fp16, 64 sequences of 4,096 visible tokens, 4 key/value heads of 128 for 16 query heads: 538 MB in 82
 // us, 6.5 TB/s, a copy's rate. 4 bits, 16 sequences of 35,536 to 65,536 tokens, the same heads: 471 MB in 112 us, 4.2
-// TB/s: there the issue slots bound it, about 340 instructions for a warp's 16 keys, most of them to make fp16
-// values of codes (the fp16 pipes are busy 49 % of the time and the integer ones 45 %). One sequence of 512 or 1,000
-// tokens: 4.5 and 5 us, of which the launch, the loads' latency and the join are each 1 to 2.
+// TB/s: there it is the making of fp16 values from codes, most of about 340 instructions for a warp's 16 keys (the fp16
+// pipes are busy 49 % of the time and the integer ones 45 %). Issue slots are at 65 %: the rest is the latency of each
+// subtile's shared-memory reads and conversions, which an SM's 16 warps do not cover. One sequence of 512 or 1,000
+// tokens: 4.5 and 5 us, of which the launch, the loads' latency and the join are each 1 to 2. fp32: beside its kernel.
 #include <cuda_fp16.h>
 #include <float.h>
 #include <math.h>
@@ -476,10 +477,10 @@ __global__ void __launch_bounds__(kThreads) decode_f16_kernel(const DecodeArgs a
 // ------------------------------------------------------------------------------------ 4-bit cache
 // A group of 64 head dims of a row is 32 bytes of codes n (0 .. 15) with a scale s and a minimum m; it stands
 // for the fp16 values s n + m, which are what the matrix instructions take. Four bits become fp16 without a
-// conversion: in the low (high) half of a byte's 8 bits, under the exponent of 1024, they are 1024 + n
-// (1024 + 16 n), from which one subtraction (one fused multiply-add by 1/16) leaves n exactly and another
-// fused multiply-add s n + m, rounded once. Two codes an instruction: with its 5 (K) to 6 (V) integer
-// instructions for 8 codes, the kernel has about as many instructions to issue as HBM gives it time for.
+// conversion: in the low (high) half of a byte's 8 bits, under the exponent of 1024, where an fp16's last place is 1,
+// they are 1024 + n (1024 + 16 n; a published technique: Kim, Henry, Fahim, Awadalla 2022), from which one subtraction (one fused multiply-add by 1/16) leaves n exactly and another
+// fused multiply-add s n + m, rounded once. Two codes an instruction, and 5 (K) to 6 (V) integer instructions for 8
+// codes.
 template <int D>
 struct Int4Cfg {
   static constexpr int KT = 32, NS = KT / 16, GR = D / kGroupDims;
@@ -692,8 +693,11 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeArgs 
 }
 
 // ------------------------------------------------------------------------------------- fp32 cache
-// Exact fp32 on CUDA cores (a correctness path, as the other fp32 kernels): a CTA takes one query head, a
-// warp every kWarps-th token, its lanes the head dims.
+// fp32 throughout, on CUDA cores: a CTA takes one query head, a warp every kWarps-th group of U tokens, its lanes the
+// head dims. K and V of a head that query heads share are read once for each of them, from L2 where they fit it.
+// Measured (B200, 16 sequences of 8,192 tokens, D 128): 16 key/value heads for 16 query heads, 2.1 GB in 358 us, 6.0
+// TB/s; 4 for 16, 0.54 GB in 324 us, 1.7 TB/s of those bytes and 6.6 of those asked for: the fourfold reading bounds it.
+// One sequence of 1,000 tokens, 16 heads of 64: 7.3 us.
 template <int D>
 __global__ void __launch_bounds__(kThreads) decode_f32_kernel(const DecodeArgs a) {
   constexpr int E = D >= 32 ? D / 32 : 1, U = 4;  // dims a lane, tokens at a time

@@ -16,8 +16,9 @@
 // With fewer tiles than 5 an SM, T = 32 (R = 4): more CTAs to spread and fewer masked pairs (B1 H4 N700 D64, causal:
 // 72 -> 42 forward, 153 -> 106 backward; B2 H8 N1500 D128, window 300: 195 -> 185 and 660 -> 630; with 14 tiles an SM 527
 // and 1850 for the 515 and 1635 above), and for D = 16, whose 64 rows take more threads than they give work (B4 H16 N2048,
-// window 512: 248 -> 220 and 704 -> 640). Rates: 40 of the FMA pipes' 74 TFLOP/s at the first size; 19 at B3 H5 N1000 D64,
-// window 200, 4 sinks (56 us forward, 172 backward), where the 480 tiles differ in length and the busiest SM has 1.55
+// window 512: 248 -> 220 and 704 -> 640). Rates by visible pairs, of the FMA pipes' 74 TFLOP/s: 29 forward and 32 backward
+// at the first size (40 with the masked pairs of its tiles), 13 to 14 at B3 H5 N1000 D64, window 200, 4 sinks (56 us
+// forward, 172 backward; 19 with the masked ones), where the 480 tiles differ in length and the busiest SM has 1.55
 // times the mean.
 #include <math.h>
 

@@ -37,6 +37,6 @@ def window_attention(
     kv_seq >= seq. Query i stands at position p = kv_seq - seq + i and sees the keys j <= p with j > p - window
     or j < sinks. Returns a tensor like q; gradients reach q, k and v, once and in reverse mode (forward-mode
     tensors are refused). As in any masked product, a NaN or an infinity in v reaches queries near its token that
-    do not see it.
+    do not see it, and in the gradients one in any input reaches tokens near its own.
     """
     return _lib.torch_ext().window_attention(q, k, v, window, sinks, sm_scale)
