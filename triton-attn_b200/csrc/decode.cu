@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(kThreads) decode_f16_kernel(const DecodeArgs a
 #pragma unroll
     for (int s = 0; s < C::NS; ++s) {
       // P is rounded to fp16 for the matrix instruction (2^-12 relative on average per weight, the same as
-      // the output's own rounding); its sum l is not.
+      // the output's own rounding, and 2^-25 of the largest weight for those below 2^-14 of it); its sum l is not.
       uint32_t pt[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
