@@ -389,7 +389,7 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return r;
 }
 
-// The same where a NaN is the result if one of them is (max.f32 gives the largest of the others).
+// Maxima that are NaN if one of the values is (max.f32 gives the largest of the others).
 __device__ __forceinline__ float max_or_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));

@@ -29,8 +29,8 @@
 // us, 0.6 PFLOP/s. What bounds it then is each tile's chain of S, exponentials and P V.
 // The running max is rescaled lazily: O (in TMEM) and l are only corrected when a row's max grows by
 // more than kRescaleThreshold (log2 units); P values stay below 2^kRescaleThreshold, exact in fp16.
-// A NaN among a row's visible scores makes its maximum NaN, and with it M and O. (The exponentials on the FMA pipe
-// clamp, which makes a weight of 0 of a NaN: whether it showed depended on the key's place in its block.)
+// A NaN among a row's visible scores makes its maximum NaN, and with it M and O (the exponentials on the FMA pipe clamp,
+// which makes a weight of 0 of a NaN).
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <math.h>
