@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define TATTN_ABI_VERSION 4
+#define TATTN_ABI_VERSION 5
 
 #if defined(__GNUC__)
 #define TATTN_API __attribute__((visibility("default")))
@@ -159,6 +159,24 @@ TATTN_API int tattn_qk_norm_rope_bwd(const void* q, const void* k, const void* w
 /* Bytes of that workspace on the current device, or -1 for an invalid head dim. */
 TATTN_API int64_t tattn_qk_norm_rope_bwd_workspace_bytes(int D);
 
+/* The rotation by positions on A axes (1 to 4; no reference counterpart): as tattn_qk_norm_rope, but pair j of token
+ * (z, n) turns by row positions[axes[j], z, n] of the tables. positions: device int32 [A, Z, N]; axes: host int32
+ * [D / 2], each in [0, A). A position outside [0, P) on any axis makes the token's rows NaN and sets
+ * TATTN_DEV_INDEX_RANGE. wq, wk both null: the rotation alone (eps and w_dtype then say nothing; w_dtype must still be
+ * `dtype` or TATTN_F32). strides: 19 int64 = q, k, q_out, k_out each (z, h, n, d), then the positions' (axis, z, n). */
+TATTN_API int tattn_qk_rope_axes(const void* q, const void* k, const void* wq, const void* wk, void* q_out, void* k_out,
+                       const float* cos, const float* sin, const int32_t* positions, const int32_t* axes,
+                       const int64_t* strides, int Z, int H, int Hk, int N, int D, int P, int A, int dtype,
+                       int w_dtype, float eps, int interleaved, void* stream);
+
+/* Its gradients, as tattn_qk_norm_rope_bwd with its workspace. Without weights q, k, dwq, dwk and workspace are not
+ * used and may be null. strides: 27 int64 = q, k, q_grad, k_grad, dq, dk each (z, h, n, d), then the positions'. */
+TATTN_API int tattn_qk_rope_axes_bwd(const void* q, const void* k, const void* wq, const void* wk, const void* q_grad,
+                           const void* k_grad, void* dq, void* dk, void* dwq, void* dwk, const float* cos,
+                           const float* sin, const int32_t* positions, const int32_t* axes, void* workspace,
+                           const int64_t* strides, int Z, int H, int Hk, int N, int D, int P, int A, int dtype,
+                           int w_dtype, float eps, int interleaved, void* stream);
+
 /* Attention of one new token of each sequence over a cache (no reference counterpart): the single-token form of
  * tattn_window_fwd. q, o: [Z, H, 1, D]; k, v: [Z, Hk, C, D], of which sequence z holds the first lengths[z]
  * tokens (device int32 [Z]), the query's own as the last. The query sees the last `window` of them (window <=
@@ -200,6 +218,44 @@ TATTN_API int tattn_int4_decode(const void* q, const void* k_codes, const void* 
                       const int64_t* strides, int Z, int H, int Hk, int C, int D, int window, int sinks,
                       float sm_scale, void* stream);
 TATTN_API int64_t tattn_int4_decode_workspace_bytes(int Z, int H, int Hk, int C, int D, int window, int sinks);
+
+/* Attention to keys of another length than the queries' (cross attention to an encoder's states; no reference
+ * counterpart): every query of sequence z sees its first lengths[z] keys (device int32 [Z]; null: all Nk). q, o: [Z, H,
+ * Nq, D]; k, v: [Z, Hk, Nk, D], query head h reading head h / (H / Hk). No keys: zeros. A length outside [0, Nk] is taken
+ * as the nearer end and sets TATTN_DEV_INDEX_RANGE. Rows of k and v past a length are never used, whatever they hold.
+ * m: fp32 [Z, H, Nq], rowmax + log2(rowsum) in base-2 units (-infinity: no keys), and o_rest (fp16: what rounding O took
+ * off, dense [Z, H, Nq, D] bytes, as tattn_window_fwd's) are for the backward; either may be null. strides: 16 int64 =
+ * q, k, v, o each (z, h, n, d); rows need unit D stride and 16-byte alignment (TATTN_ERR_LAYOUT). workspace:
+ * tattn_cross_fwd_workspace_bytes bytes, 16-byte aligned (0 bytes: may be null). */
+TATTN_API int tattn_cross_fwd(const void* q, const void* k, const void* v, const int32_t* lengths, void* o, float* m,
+                    void* o_rest, void* workspace, const int64_t* strides, int Z, int H, int Hk, int Nq, int Nk, int D,
+                    int dtype, float sm_scale, void* stream);
+/* Bytes of that workspace on the current device, or -1 for invalid arguments. It goes by the sizes alone. */
+TATTN_API int64_t tattn_cross_fwd_workspace_bytes(int Z, int H, int Hk, int Nq, int Nk, int D, int dtype);
+
+/* Its backward: dq [Z, H, Nq, D] and dk, dv [Z, Hk, Nk, D], all dense, zeros in the rows past a length; m, o_rest (or
+ * null) and o as the forward wrote them. strides: 20 int64 = q, k, v, o, dout each (z, h, n, d). delta: fp32 [Z, H, Nq].
+ * workspace: tattn_cross_bwd_workspace_bytes bytes, 16-byte aligned (0 bytes: may be null). As tattn_window_bwd, fp16
+ * sums dq in an order that varies from run to run. */
+TATTN_API int tattn_cross_bwd(const void* q, const void* k, const void* v, const int32_t* lengths, const void* o,
+                    const void* dout, void* dq, void* dk, void* dv, const float* m, const void* o_rest, float* delta,
+                    void* workspace, const int64_t* strides, int Z, int H, int Hk, int Nq, int Nk, int D, int dtype,
+                    float sm_scale, void* stream);
+TATTN_API int64_t tattn_cross_bwd_workspace_bytes(int Z, int H, int Hk, int Nq, int Nk, int D, int dtype);
+
+/* One new token of each of prompts * samples sequences, where the `samples` consecutive sequences of a prompt share its
+ * keys and values (no reference counterpart). q, o: [prompts * samples, H, 1, D]; prefix_k, prefix_v: [prompts, Hk, P, D],
+ * of which prompt p holds the first prefix_lengths[p] tokens (device int32 [prompts]; null: all P); k, v: [prompts *
+ * samples, Hk, C, D], the sequences' own tokens behind it, of which sequence b holds lengths[b] (device int32). The query
+ * sees all of both; nothing held gives zeros. Lengths outside their range, and rows past a length, as in tattn_decode.
+ * strides: 24 int64 = q, prefix_k, prefix_v, k, v, o each (z, h, n, d); rows need unit D stride and 16-byte alignment.
+ * workspace: tattn_prefix_decode_workspace_bytes bytes, 16-byte aligned. */
+TATTN_API int tattn_prefix_decode(const void* q, const void* prefix_k, const void* prefix_v, const int32_t* prefix_lengths,
+                        const void* k, const void* v, const int32_t* lengths, void* o, void* workspace,
+                        const int64_t* strides, int prompts, int samples, int H, int Hk, int P, int C, int D, int dtype,
+                        float sm_scale, void* stream);
+TATTN_API int64_t tattn_prefix_decode_workspace_bytes(int prompts, int samples, int H, int Hk, int P, int C, int D,
+                                            int dtype);
 
 /* Largest Z*H*N accepted by tattn_bwd_noalloc (its fixed fp32 row buffer: 16 MiB per GPU). */
 #define TATTN_BWD_NOALLOC_MAX_ROWS 4194304

@@ -37,6 +37,8 @@
 // commits for it (S/dP and accumulation) have landed.
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "tiles.h"
@@ -1751,6 +1753,10 @@ cudaError_t dkdv_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
 //     128 x 128 block, as the other masks, and 5,500 a unit (its first scores, the accumulators' way out); the delta
 //     pass with the workspace's zeros 25, dQ's scaling and the partials 33, the last CTAs' lead the rest. B2 H16 Hk4
 //     N2500 D128, window 777, 130 sinks: 215 us.
+//   * kMaskRows: a window that hides nothing, over the first lengths[z] keys of a sequence. What lies behind them (an
+//     infinity, a NaN) must not meet a weight of 0 in a product: the compute warps make those rows of S'^T -infinity, of
+//     dP'^T zeros, and of the K tile in shared memory zeros before the dQ MMAs read it. Key tiles behind them do no
+//     work but write their zeros.
 //   * After its last tile every CTA (a cooperative launch of at most one CTA per SM) waits at a grid
 //     barrier for all reduce-adds, then its compute warps scale a share of the workspace by sm_scale
 //     into the fp16 dQ.
@@ -2009,6 +2015,18 @@ __device__ __forceinline__ void hide_queries(uint32_t* s, int lo, int hi) {
   }
 }
 
+// kMaskRows: row r of the key tile at `tile` becomes zeros.
+template <int D>
+__device__ __forceinline__ void clear_key_row(uint32_t tile, int r) {
+  using G = Geo<D>;
+#pragma unroll
+  for (int ch = 0; ch < G::NCH; ++ch)
+#pragma unroll
+    for (int u = 0; u < G::SWB / 16; ++u)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + ch * G::chunk(128) + r * G::SWB + u * 16), "r"(0u)
+                   : "memory");
+}
+
 // One unit of a CTA's work in the fused backward: key tile kt of key/value head hk and n (query head, query
 // block) pairs, from (h0, blk0) on: blocks [lo, lo + nb) of one head after another. Not kMaskWindow: one
 // head's blocks from lo on.
@@ -2016,6 +2034,7 @@ struct Unit {
   int zi, hk, kt, n;
   int h0, blk0, lo, nb;
   int slot;  // kMaskWindow: of its partial, else -1
+  int len;   // kMaskRows: keys of the tile that are the sequence's (128 or more: all)
 };
 template <bool WINDOW>
 struct UnitWalk {
@@ -2030,16 +2049,19 @@ struct UnitWalk {
   }
 };
 
+template <int MASK>
+using FusedArgs = std::conditional_t<MASK == kMaskRows, RowsBwdArgs, BwdArgs>;
+
 template <int D, int MASK>
 __global__ void __launch_bounds__(kThreads, 1)
     bwd_fused_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
                      const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv,
-                     const __grid_constant__ CUtensorMap tm_dqacc, const BwdArgs args) {
+                     const __grid_constant__ CUtensorMap tm_dqacc, const FusedArgs<MASK> args) {
   using C = FusedCfg<D>;
   using G = Geo<D>;
   constexpr int H = C::H, BQ = C::BQ, NS = C::NS;
-  constexpr bool CAUSAL = MASK == kMaskCausal, WINDOW = MASK == kMaskWindow;
+  constexpr bool CAUSAL = MASK == kMaskCausal, ROWS = MASK == kMaskRows, WINDOW = MASK == kMaskWindow || ROWS;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
   const uint32_t base_u32 = (raw_u32 + 1023u) & ~1023u;
@@ -2123,6 +2145,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       u->blk0 += w.start - heads * w.nb;
     }
     u->slot = w.slot < 0 ? -1 : w.head * args.split.slots(nct) + w.slot;
+    if constexpr (ROWS) {
+      bool outside;  // (the forward has reported it)
+      u->len = held_keys(args.lengths, u->zi, Nk, &outside) - 128 * w.kt;
+      if (u->len <= 0) u->n = 0;
+    }
     return true;
   };
   auto next_unit = [&](int2& seq, Unit* u) -> bool {
@@ -2405,7 +2432,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool masked = !WINDOW && ((q0 + H > N) || (k0 + 128 > Nk) || (CAUSAL && q0 < k0 + 127));
         const int c_lo = CAUSAL ? max(0, key - q0) : 0;  // valid query columns: c_lo <= c < c_hi
         const int c_hi = key < Nk ? N - q0 : 0;
-        if (WINDOW) {  // a key is seen from its own position on, for one window unless it is a sink
+        if constexpr (ROWS) {
+          if (q0 + H > N || u.len < 128) hide_queries<H>(s, 0, r < u.len ? N - q0 : 0);
+          if (u.len < 128) {
+#pragma unroll
+            for (int x = 0; x < H; ++x) dp[x] = r < u.len ? dp[x] : 0u;
+            if (c == 0 && w == 0 && r >= u.len) clear_key_row<D>(sK + (it & 1) * C::T_KEY, r);  // (fenced below)
+          }
+        } else if (WINDOW) {  // a key is seen from its own position on, for one window unless it is a sink
           const int p0 = q0 + args.win.off;
           if ((q0 + H > N) || (k0 + 128 > Nk) || p0 < k0 + 127 ||
               (p0 + H - 1 >= k0 + args.win.window && k0 + 128 > args.win.sinks))
@@ -2486,7 +2520,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_arrive(bar_acc_read);
           }
         }
-        if (WINDOW && !any) {
+        bool none = WINDOW && !any;
+        if constexpr (ROWS) none = none || r >= u.len;
+        if (none) {
 #pragma unroll
           for (int c = 0; c < OR; ++c) o[c] = 0u;
         }
@@ -2555,13 +2591,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <int D, int MASK>
 cudaError_t fused_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
-                       const CUtensorMap& tdk, const CUtensorMap& tdv, const CUtensorMap& tdqacc, const BwdArgs& a,
+                       const CUtensorMap& tdk, const CUtensorMap& tdv, const CUtensorMap& tdqacc, const FusedArgs<MASK>& a,
                        cudaStream_t s) {
   auto kern = bwd_fused_kernel<D, MASK>;
   constexpr int smem = FusedCfg<D>::SMEM_BYTES;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  constexpr bool WINDOW = MASK == kMaskWindow;
+  constexpr bool WINDOW = MASK == kMaskWindow || MASK == kMaskRows;
   const long long nct = ((WINDOW ? a.win.Nk : a.N) + 127) / 128;
   const long long tiles = nct * a.Z * (WINDOW ? a.win.Hk : a.H);
   if (tiles <= 0) return cudaSuccess;
@@ -2573,7 +2609,7 @@ cudaError_t fused_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUten
   // One CTA per SM at most (shared memory), so a cooperative launch keeps every CTA resident: the grid
   // barrier before the kernel's last phase needs that (its counter is zeroed by the preprocess).
   const unsigned grid = unsigned(units < device_sm_count() ? units : device_sm_count());
-  BwdArgs args = a;
+  FusedArgs<MASK> args = a;
   CUtensorMap m[7] = {tq, tk, tv, tdo, tdk, tdv, tdqacc};
   void* params[8] = {&m[0], &m[1], &m[2], &m[3], &m[4], &m[5], &m[6], &args};
   e = cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(kern), dim3(grid), dim3(kThreads), params, smem, s);
@@ -2663,5 +2699,16 @@ cudaError_t launch_bwd_fused_f16(int D, Mask mask, const CUtensorMap& tq, const 
   }
 }
 
+cudaError_t launch_bwd_rows_f16(int D, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                                const CUtensorMap& tdo, const CUtensorMap& tdk, const CUtensorMap& tdv,
+                                const CUtensorMap& tdqacc, const RowsBwdArgs& a, cudaStream_t s) {
+  switch (D) {
+    case 16: return fused_impl<16, kMaskRows>(tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s);
+    case 32: return fused_impl<32, kMaskRows>(tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s);
+    case 64: return fused_impl<64, kMaskRows>(tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s);
+    case 128: return fused_impl<128, kMaskRows>(tq, tk, tv, tdo, tdk, tdv, tdqacc, a, s);
+    default: return cudaErrorNotSupported;
+  }
+}
 
 }  // namespace tattn

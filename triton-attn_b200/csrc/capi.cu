@@ -82,6 +82,8 @@ bool valid_dims(int Z, int H, int N, int D) {
   return Z >= 0 && H >= 0 && N >= 0 && (D == 16 || D == 32 || D == 64 || D == 128);
 }
 
+}  // namespace
+
 Strides4 load_strides(const int64_t* s) { return Strides4{s[0], s[1], s[2], s[3]}; }
 
 // Strides of extent-1 dimensions never move an address; replace them by the dense value so the TMA
@@ -106,7 +108,7 @@ bool layout_ok(const void* p, Strides4 s, int Z, int H, int N, int D) {
 
 // [Z, H, N, D] fp16 tensor as a 4-D TMA map {D, N, H, Z}; box = {box_cols columns (default min(D, 64)),
 // box_rows rows} with the swizzle that matches one box row (16 bytes: none; 32/64/128 bytes).
-int encode_f16(CUtensorMap* tm, const void* p, Strides4 s, int Z, int H, int N, int D, int box_rows, int box_cols = 0) {
+int encode_f16(CUtensorMap* tm, const void* p, Strides4 s, int Z, int H, int N, int D, int box_rows, int box_cols) {
   s = normalize(s, Z, H, N, D);
   const int cw = box_cols > 0 ? box_cols : (D < 64 ? D : 64);
   cuuint64_t dims[4] = {cuuint64_t(D), cuuint64_t(N), cuuint64_t(H), cuuint64_t(Z)};
@@ -141,7 +143,7 @@ int encode_f32_dense(CUtensorMap* tm, void* p, int Z, int H, int N, int D, int b
   return r == CUDA_SUCCESS ? TATTN_OK : TATTN_ERR_LAYOUT;
 }
 
-}  // namespace
+unsigned long long wait_limit_ns() { return g_wait_limit_ns.load(); }
 
 int cuda_rc(cudaError_t e) {
   if (e == cudaSuccess) return TATTN_OK;

@@ -24,12 +24,12 @@ bool rows16(const void* p, const int64_t* s, int Z, int H, int N, int esz) {
 
 Strides3 strides3(const int64_t* s) { return Strides3{s[0], s[1], s[2]}; }
 
-int norm_rope(RopeArgs& a, bool backward, const int64_t* strides, int Z, int H, int Hk, int N, int D, int P, int dtype,
-              int w_dtype, int interleaved, void* stream) {
+// strides: of q, k, q_out, k_out (backward: of q, k, q_grad, k_grad, dq, dk); positions (axis, z, n strides).
+int norm_rope(RopeArgs& a, RopeForm form, bool backward, const int64_t* strides, const int64_t* pos, int Z, int H, int Hk,
+              int N, int D, int P, int dtype, int w_dtype, int interleaved, void* stream) {
   const int esz = dtype == TATTN_F16 ? 2 : 4, heads[2] = {H, Hk};
   for (int i = 0; i < 2; ++i) {
     RopeTensor& t = a.t[i];
-    // forward: q, k, q_out, k_out; backward: q, k, q_grad, k_grad, dq, dk
     const int64_t *sx = strides + 4 * i, *sdy = strides + 8 + 4 * i, *sy = strides + (backward ? 16 : 8) + 4 * i;
     if (!rows16(t.px, sx, Z, heads[i], N, esz) || (backward && !rows16(t.pdy, sdy, Z, heads[i], N, esz)) ||
         !rows16(t.py, sy, Z, heads[i], N, esz) || (reinterpret_cast<uintptr_t>(t.w) & 15u) != 0)
@@ -40,16 +40,16 @@ int norm_rope(RopeArgs& a, bool backward, const int64_t* strides, int Z, int H, 
     t.H = heads[i];
   }
   if (((reinterpret_cast<uintptr_t>(a.cos) | reinterpret_cast<uintptr_t>(a.sin)) & 15u) != 0) return TATTN_ERR_LAYOUT;
-  const int64_t* pos = strides + (backward ? 24 : 16);
-  a.pos_z = pos[0];
-  a.pos_n = pos[1];
+  a.pos_a = pos[0];
+  a.pos_z = pos[1];
+  a.pos_n = pos[2];
   a.Z = Z;
   a.N = N;
   a.P = P;
   a.w_f32 = w_dtype == TATTN_F32;
   const int rc = device_ready(&a.status);
   if (rc != TATTN_OK) return rc;
-  return cuda_rc(launch_norm_rope(D, dtype == TATTN_F16, interleaved != 0, backward, a, static_cast<cudaStream_t>(stream)));
+  return cuda_rc(launch_norm_rope(D, dtype == TATTN_F16, form, interleaved != 0, backward, a, static_cast<cudaStream_t>(stream)));
 }
 
 int norm_rope_dims(int Z, int H, int Hk, int N, int D, int P, int dtype, int w_dtype) {
@@ -84,7 +84,8 @@ extern "C" int tattn_qk_norm_rope(const void* q, const void* k, const void* wq, 
   a.sin = sin;
   a.positions = positions;
   a.eps = eps;
-  return norm_rope(a, false, strides, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved, stream);
+  const int64_t pos[3] = {0, strides[16], strides[17]};
+  return norm_rope(a, kOnePosition, false, strides, pos, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved, stream);
 }
 
 extern "C" int tattn_qk_norm_rope_bwd(const void* q, const void* k, const void* wq, const void* wk, const void* q_grad,
@@ -114,12 +115,92 @@ extern "C" int tattn_qk_norm_rope_bwd(const void* q, const void* k, const void* 
   a.positions = positions;
   a.eps = eps;
   a.part = static_cast<float*>(workspace);
-  return norm_rope(a, true, strides, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved, stream);
+  const int64_t pos[3] = {0, strides[24], strides[25]};
+  return norm_rope(a, kOnePosition, true, strides, pos, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved, stream);
 }
 
 extern "C" int64_t tattn_qk_norm_rope_bwd_workspace_bytes(int D) {
   if (!head_dim_ok(D)) return -1;
   return (int64_t(kRopeBlocksPerSm) * device_sm_count() + 2) * D * 4;
+}
+
+namespace {
+
+// The axis of each pair into a.axes; false where one is outside [0, A).
+bool rope_axes(RopeArgs& a, const int32_t* axes, int A, int D) {
+  if (!axes || A < 1 || A > kRopeAxes) return false;
+  a.A = A;
+  for (int j = 0; j < D / 2; ++j) {
+    if (axes[j] < 0 || axes[j] >= A) return false;
+    a.axes[j / 16] |= uint32_t(axes[j]) << (2 * (j % 16));
+  }
+  return true;
+}
+
+}  // namespace
+
+extern "C" int tattn_qk_rope_axes(const void* q, const void* k, const void* wq, const void* wk, void* q_out, void* k_out,
+                                  const float* cos, const float* sin, const int32_t* positions, const int32_t* axes,
+                                  const int64_t* strides, int Z, int H, int Hk, int N, int D, int P, int A, int dtype,
+                                  int w_dtype, float eps, int interleaved, void* stream) {
+  if (!strides) return TATTN_ERR_INVALID_ARGUMENT;
+  const int rc = norm_rope_dims(Z, H, Hk, N, D, P, dtype, w_dtype);
+  if (rc != TATTN_OK) return rc;
+  RopeArgs a{};
+  if (!rope_axes(a, axes, A, D) || (wq == nullptr) != (wk == nullptr)) return TATTN_ERR_INVALID_ARGUMENT;
+  if (int64_t(Z) * N == 0) return TATTN_OK;
+  if (!q || !k || !q_out || !k_out || !cos || !sin || !positions) return TATTN_ERR_INVALID_ARGUMENT;
+  a.t[0].px = q;
+  a.t[1].px = k;
+  a.t[0].py = q_out;
+  a.t[1].py = k_out;
+  a.t[0].w = wq;
+  a.t[1].w = wk;
+  a.cos = cos;
+  a.sin = sin;
+  a.positions = positions;
+  a.eps = eps;
+  return norm_rope(a, wq ? kAxesNorm : kAxes, false, strides, strides + 16, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved,
+                   stream);
+}
+
+extern "C" int tattn_qk_rope_axes_bwd(const void* q, const void* k, const void* wq, const void* wk, const void* q_grad,
+                                      const void* k_grad, void* dq, void* dk, void* dwq, void* dwk, const float* cos,
+                                      const float* sin, const int32_t* positions, const int32_t* axes, void* workspace,
+                                      const int64_t* strides, int Z, int H, int Hk, int N, int D, int P, int A, int dtype,
+                                      int w_dtype, float eps, int interleaved, void* stream) {
+  if (!strides) return TATTN_ERR_INVALID_ARGUMENT;
+  const int rc = norm_rope_dims(Z, H, Hk, N, D, P, dtype, w_dtype);
+  if (rc != TATTN_OK) return rc;
+  RopeArgs a{};
+  const bool norm = wq != nullptr, any = int64_t(Z) * N > 0;
+  if (!rope_axes(a, axes, A, D) || norm != (wk != nullptr) || (norm && (!dwq || !dwk || !workspace)))
+    return TATTN_ERR_INVALID_ARGUMENT;
+  if (any && (!q_grad || !k_grad || !dq || !dk || !cos || !sin || !positions || (norm && (!q || !k))))
+    return TATTN_ERR_INVALID_ARGUMENT;
+  a.cos = cos;
+  a.sin = sin;
+  a.positions = positions;
+  a.t[0].py = dq;
+  a.t[1].py = dk;
+  if (!norm) {  // the gradients turned back
+    if (!any) return TATTN_OK;
+    a.t[0].px = q_grad;
+    a.t[1].px = k_grad;
+    a.back = 1;
+    return norm_rope(a, kAxes, false, strides + 8, strides + 24, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved, stream);
+  }
+  a.t[0].px = q;
+  a.t[1].px = k;
+  a.t[0].pdy = q_grad;
+  a.t[1].pdy = k_grad;
+  a.t[0].w = wq;
+  a.t[1].w = wk;
+  a.t[0].dw = dwq;
+  a.t[1].dw = dwk;
+  a.eps = eps;
+  a.part = static_cast<float*>(workspace);
+  return norm_rope(a, kAxesNorm, true, strides, strides + 24, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved, stream);
 }
 
 namespace {

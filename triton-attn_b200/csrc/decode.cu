@@ -43,7 +43,7 @@ struct Visible {
   __device__ __forceinline__ int token(int t) const { return t < sinks ? t : t + jump; }
 };
 __device__ __forceinline__ Visible visible_tokens(const DecodeArgs& a, int z, bool report) {
-  int len = a.lengths[z];
+  int len = a.lengths ? a.lengths[z] : a.C;
   if (len < 0 || len > a.C) {
     if (report) atomicOr(a.status, kStatusIndexRange);
     len = len < 0 ? 0 : a.C;
@@ -298,9 +298,9 @@ __device__ __forceinline__ void finish(const DecodeArgs& a, const Part& p, WarpS
       o = make_float4(fmaf(f, x.x, o.x), fmaf(f, x.y, o.y), fmaf(f, x.z, o.z), fmaf(f, x.w, o.w));
     }
     const int h = p.h0 + head;
-    if (a.nsplit == 1) {
+    if (a.nsplit == 1 && !a.parts_only) {
       write_row4<D>(a, p.z, h, d, o, m, l);
-    } else if (a.nsplit <= kClusterParts) {
+    } else if (a.nsplit <= kClusterParts && !a.parts_only) {
       *reinterpret_cast<float4*>(mine + head * D + d) = o;
       if (d == 0) *reinterpret_cast<float2*>(mine + HEADS * D + head * 2) = make_float2(m, l);
     } else {
@@ -309,7 +309,7 @@ __device__ __forceinline__ void finish(const DecodeArgs& a, const Part& p, WarpS
       if (d == 0) *reinterpret_cast<float2*>(a.part_ml + row * 2) = make_float2(m, l);
     }
   }
-  if (a.nsplit == 1 || a.nsplit > kClusterParts) return;
+  if (a.nsplit == 1 || a.nsplit > kClusterParts || a.parts_only) return;
   // The cluster's CTAs are the parts in order; each finishes a share of the rows.
   cluster_sync();
   const uint32_t rows = smem_u32(mine);
@@ -770,7 +770,7 @@ __global__ void __launch_bounds__(kThreads) decode_f32_kernel(const DecodeArgs a
       l = fmaf(f, sml[w][1], l);
       acc = fmaf(f, so[w][c], acc);
     }
-    if (a.nsplit == 1) {
+    if (a.nsplit == 1 && !a.parts_only) {
       static_cast<float*>(a.o)[p.z * a.so.z + p.h0 * a.so.h + c] = m == -INFINITY ? 0.f : acc / l;
     } else {
       const int64_t row = (int64_t(p.z) * a.H + p.h0) * a.nsplit + p.split;
@@ -854,7 +854,8 @@ long long decode_units(const DecodeArgs& a, int heads_per_cta) {
 
 template <int D>
 cudaError_t decode_impl(DecodeCache cache, const DecodeArgs& a, cudaStream_t s) {
-  const bool join = decode_joins(a.nsplit, cache), cluster = a.nsplit > 1 && !join, wide = a.H / a.Hk > 8;
+  const bool join = decode_joins(a.nsplit, cache) && !a.parts_only, wide = a.H / a.Hk > 8;
+  const bool cluster = a.nsplit > 1 && !decode_joins(a.nsplit, cache) && !a.parts_only;
   cudaError_t e;
   if (cache == kCacheF32) {
     e = launch(decode_f32_kernel<D>, 0, decode_units(a, 1), false, a, s);

@@ -33,7 +33,10 @@
 // which makes a weight of 0 of a NaN).
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
+#include <float.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -151,7 +154,7 @@ __device__ __forceinline__ void issue_pv_stage(int st, uint32_t d_tmem, uint32_t
 // with entry n0 - 1.
 struct Blocks {
   int n0, n;
-  int sink, jump;  // entry j >= sink is block j + jump
+  int sink, jump;  // entry j >= sink is block j + jump (kMaskRows: entry j is block j + jump)
   __device__ __forceinline__ int block(int j) const { return j < sink ? j : j + jump; }
 };
 template <int BM, int BN, int TILES>
@@ -165,6 +168,39 @@ __device__ __forceinline__ Blocks window_blocks(int row0, int N, const WindowArg
   b.n0 = end0 - b.jump;
   b.n = end - b.jump;
   return b;
+}
+
+// kMaskRows: rows [row0, row0 + 128) of the head's matrix into a query tile's shared memory, by the 128 threads of a
+// warpgroup (t: the thread's index in it); rows past N are zeros.
+template <typename C, int D>
+__device__ __forceinline__ void load_row_tile(const RowsFwdArgs& a, uint32_t dst, int zi, int hi, int row0, int t) {
+  constexpr int U = D / 8, CU = C::SWB / 16;  // 16-byte units of a row, of its part in a chunk
+  const __half* q = static_cast<const __half*>(a.rows.q);
+#pragma unroll 1
+  for (int i = 0; i < U; ++i) {
+    const int e = i * 128 + t, row = e / U, unit = e % U, r = row0 + row;
+    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+    if (r < a.N)
+      x = __ldg(reinterpret_cast<const uint4*>(row_of(q, a.rows.sq, a.rows.inner, zi, hi, r)) + unit);
+    const uint32_t at = dst + unit / CU * C::QCHUNK + swizzle_offset<C::SWB>(uint32_t(row * C::SWB + unit % CU * 16));
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+  }
+  fence_proxy_async_smem();
+}
+
+// kMaskRows: rows [from, BN) of the value block at `block` become zeros: their weights are 0, but behind a sequence's
+// last key there may lie anything, an infinity or a NaN too.
+template <typename C>
+__device__ __forceinline__ void clear_value_rows(uint32_t block, int from, int t) {
+  if (t >= from && t < C::BN) {
+#pragma unroll
+    for (int ch = 0; ch < C::NCH; ++ch)
+#pragma unroll
+      for (int u = 0; u < C::SWB / 16; ++u)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(block + ch * C::KCHUNK + t * C::SWB + u * 16), "r"(0u)
+                     : "memory");
+  }
+  fence_proxy_async_smem();
 }
 
 // kMaskWindow: scores of the columns that a row does not see become -infinity: it sees the columns in
@@ -237,14 +273,58 @@ __device__ __forceinline__ uint32_t rest_of(const uint32_t* o, uint32_t h, float
                                   __NV_SATFINITE, __NV_E5M2);
 }
 
+// kMaskRows: a row whose part has no keys. Not to be joined: zeros, and M = -infinity.
+template <int D>
+__device__ __forceinline__ void no_keys(const RowsFwdArgs& a, int bh, int row, int nct) {
+  const int64_t at = int64_t(bh) * a.N + row;
+  if (a.rows.part != nullptr) {
+    const int split = int(blockIdx.x) / nct - bh * a.rows.nsplit;
+    reinterpret_cast<float2*>(a.rows.part_ml)[at * a.rows.nsplit + split] = make_float2(-INFINITY, 0.f);
+    return;
+  }
+  __half* o = row_of(static_cast<__half*>(a.o), a.rows.so, a.rows.inner, bh / a.H, bh % a.H, row);
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+  for (int u = 0; u < D / 8; ++u) reinterpret_cast<uint4*>(o)[u] = zero;
+  if (a.o_rest != nullptr)
+#pragma unroll
+    for (int u = 0; u < D / 16; ++u) reinterpret_cast<uint4*>(a.o_rest + at * D)[u] = zero;
+  if (a.m != nullptr) a.m[at] = -INFINITY;
+}
+
+// kMaskRows: a row's part as it is.
+template <typename C, int D>
+__device__ __forceinline__ void store_part(const RowsFwdArgs& a, int bh, int row, int nct, uint32_t tO, float m, float l) {
+  const int64_t at = (int64_t(bh) * a.N + row) * a.rows.nsplit + (int(blockIdx.x) / nct - bh * a.rows.nsplit);
+#pragma unroll
+  for (int c0 = 0; c0 < D; c0 += 32) {
+    constexpr int W = D < 32 ? D : 32;
+    uint32_t o[W];
+    tmem_load_cols<W>(tO + c0, o);
+    tmem_wait_ld();
+    reg_fence<W>(o);
+    if (row < a.N) {
+      uint4* dst = reinterpret_cast<uint4*>(a.rows.part + at * D + c0);
+#pragma unroll
+      for (int v = 0; v < W / 4; ++v) dst[v] = make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+    }
+  }
+  // All scores -infinity: the largest float below 0 and no weight (the FMA pipe's exponentials left 2^-126 each); -infinity
+  // would say that the part has no keys.
+  if (row < a.N) reinterpret_cast<float2*>(a.rows.part_ml)[at] = m == -INFINITY ? make_float2(-FLT_MAX, 0.f) : make_float2(m, l);
+}
+
+template <int MASK>
+using Args = std::conditional_t<MASK == kMaskRows, RowsFwdArgs, FwdArgs>;
+
 template <int D, int MASK, int BN_, int NS_, int TILES>
 __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
     fwd_f16_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                   const __grid_constant__ CUtensorMap tm_v, const FwdArgs args) {
+                   const __grid_constant__ CUtensorMap tm_v, const Args<MASK> args) {
   using C = FwdCfg<D, BN_, NS_, TILES>;
   constexpr int BN = C::BN;
   constexpr int kTmaWarp = 4 * TILES, kMmaWarp = kTmaWarp + 1, kAllocWarp = kTmaWarp + 3;  // kMmaWarp + i: tile i
-  constexpr bool CAUSAL = MASK == kMaskCausal, WINDOW = MASK == kMaskWindow;
+  constexpr bool CAUSAL = MASK == kMaskCausal, WINDOW = MASK == kMaskWindow, ROWS = MASK == kMaskRows;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
   const uint32_t base_u32 = (raw_u32 + 1023u) & ~1023u;
@@ -284,6 +364,10 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
     } else {
       cta = brief - 1 - grouped_cta_rank(rest, brief, zh, 2ll * args.win.Nk * D / args.win.group, &bh);
     }
+  } else if constexpr (ROWS) {  // the row blocks that go through the same keys adjacent
+    const int part = int(blockIdx.x) / nct;
+    cta = int(blockIdx.x) - part * nct;
+    bh = part / args.rows.nsplit;
   } else {  // row blocks of one head adjacent: K/V of a head stay hot in L2
     bh = blockIdx.x / nct;
     cta = blockIdx.x % nct;
@@ -296,14 +380,25 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
   const int row0_0 = TILES * cta * C::BM, row0_1 = row0_0 + C::BM;
   Blocks list{};
   if (WINDOW) list = window_blocks<C::BM, BN, TILES>(row0_0, N, args.win);
-  const int n_0 = WINDOW ? list.n0 : row0_0 >= N ? 0 : (CAUSAL ? min((row0_0 + C::BM + BN - 1) / BN, NB) : NB);
+  int len = 0;  // kMaskRows: keys that the rows see
+  if constexpr (ROWS) {
+    bool outside;
+    len = held_keys(args.rows.lengths, zi, args.rows.Nk, &outside);
+    if (outside && threadIdx.x == 0) atomicOr(args.status, kStatusIndexRange);
+    const int split = int(blockIdx.x) / nct - bh * args.rows.nsplit;
+    const int64_t blocks = (len + BN - 1) / BN;
+    list.jump = int(blocks * split / args.rows.nsplit);
+    list.n = int(blocks * (split + 1) / args.rows.nsplit) - list.jump;
+    list.n0 = list.n;
+  }
+  const int n_0 = WINDOW || ROWS ? list.n0 : row0_0 >= N ? 0 : (CAUSAL ? min((row0_0 + C::BM + BN - 1) / BN, NB) : NB);
   const int n_1 = TILES == 1 || row0_1 >= N ? 0
-                  : WINDOW                  ? list.n
+                  : WINDOW || ROWS          ? list.n
                                             : (CAUSAL ? min((row0_1 + C::BM + BN - 1) / BN, NB) : NB);
   const int nmax = max(n_0, n_1);
 
   if (threadIdx.x == 0) {
-    mbar_init(bar_q, 1);
+    mbar_init(bar_q, ROWS ? 128 * TILES : 1);
     for (int s = 0; s < C::NS; ++s) {
       mbar_init(&bar_k_full[s], 1);
       mbar_init(&bar_v_full[s], 1);
@@ -326,7 +421,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
     tmem_relinquish();
   }
   if (warp == kTmaWarp && lane == 0) {
-    tma_prefetch_desc(&tm_q);
+    if (!ROWS) tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
@@ -341,12 +436,14 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs<TILES>));
     if (warp == kTmaWarp && lane == 0) {
       // -------------------------------------------------------------- TMA producer
-      const uint32_t qbytes = (n_0 > 0 ? C::QTILE : 0) + (n_1 > 0 ? C::QTILE : 0);
-      mbar_arrive_expect_tx(bar_q, qbytes);
-      for (int i = 0; i < TILES; ++i) {
-        if ((i ? n_1 : n_0) == 0) continue;
-        for (int ch = 0; ch < C::NCH; ++ch)
-          tma_load_4d(sQ + i * C::QTILE + ch * C::QCHUNK, &tm_q, ch * C::CW, i ? row0_1 : row0_0, hi, zi, bar_q);
+      if (!ROWS) {
+        const uint32_t qbytes = (n_0 > 0 ? C::QTILE : 0) + (n_1 > 0 ? C::QTILE : 0);
+        mbar_arrive_expect_tx(bar_q, qbytes);
+        for (int i = 0; i < TILES; ++i) {
+          if ((i ? n_1 : n_0) == 0) continue;
+          for (int ch = 0; ch < C::NCH; ++ch)
+            tma_load_4d(sQ + i * C::QTILE + ch * C::QCHUNK, &tm_q, ch * C::CW, i ? row0_1 : row0_0, hi, zi, bar_q);
+        }
       }
       int j = 0;
       bool ok = true;
@@ -359,7 +456,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
               ok = false;
           if (!ok) break;
         }
-        const int key0 = (WINDOW ? list.block(j) : j) * BN;
+        const int key0 = (WINDOW ? list.block(j) : ROWS ? j + list.jump : j) * BN;
         mbar_arrive_expect_tx(&bar_k_full[st], C::KTILE);
         for (int ch = 0; ch < C::NCH; ++ch)
           tma_load_4d(sK + st * C::KTILE + ch * C::KCHUNK, &tm_k, ch * C::CW, key0, hk, zi, &bar_k_full[st]);
@@ -369,7 +466,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
       }
       // Every copy this CTA issued must land before the CTA exits (instant on the normal path).
       const unsigned long long lim = 100ull * 1000ull * 1000ull;
-      mbar_drain(bar_q, 0, lim);
+      if (!ROWS) mbar_drain(bar_q, 0, lim);
       for (int jj = max(0, j - C::NS); jj < j; ++jj) {
         mbar_drain(&bar_k_full[jj % C::NS], (jj / C::NS) & 1, lim);
         mbar_drain(&bar_v_full[jj % C::NS], (jj / C::NS) & 1, lim);
@@ -454,6 +551,10 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
     const uint64_t scale2 = f2(scale, scale);
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
+    if constexpr (ROWS) {
+      if (n > 0) load_row_tile<C, D>(args, sQ + i * C::QTILE, zi, hi, row - t, t);
+      mbar_arrive(bar_q);
+    }
     for (int j = 0; j < n; ++j) {
       if (!warp_wait(&bar_s_full[i], j & 1, ab)) { ok = false; break; }
       tc_fence_after();
@@ -468,14 +569,16 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
       // (causal) in every block that reaches past the tile's first row (the last BM / BN blocks).
       // kMaskWindow: those are hidden beforehand, in every block that the diagonal or the lower edge of some
       // row's window cuts.
-      const int col0 = (WINDOW ? list.block(j) : j) * BN;
+      // kMaskRows: those past the sequence's keys, in its last block.
+      const int col0 = (WINDOW ? list.block(j) : ROWS ? j + list.jump : j) * BN;
+      if (ROWS && col0 + BN > len) hide_columns<BN>(s, len - col0, 0, 0);
       if (WINDOW) {
         const int pos = row + args.win.off, tile = pos - t;  // positions of this row and of the tile's first
         if (col0 + BN - 1 > tile || (col0 <= tile + C::BM - 1 - args.win.window && col0 + BN > args.win.sinks))
           hide_columns<BN>(s, min(args.win.Nk, pos + 1) - col0, pos + 1 - args.win.window - col0,
                            args.win.sinks - col0);
       }
-      const bool last = !WINDOW && ((col0 + BN > N) || (CAUSAL && col0 + BN - 1 > row - t));
+      const bool last = !WINDOW && !ROWS && ((col0 + BN > N) || (CAUSAL && col0 + BN - 1 > row - t));
       int lim = N - col0;
       if (CAUSAL) lim = min(lim, row - col0 + 1);
       const float m_cand = (last ? row_max<BN, true>(s, lim) : row_max<BN, false>(s, lim)) * scale;
@@ -505,7 +608,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
       // hand-off (measured at BN = 128: 7/8 best, 3/4 within 1%, 1/2 8% slower; slower at BN = 64).
       constexpr int kSplit = BN == 128 && TILES == 2 ? BN * 7 / 8 : BN;
       uint32_t p[BN / 2];
-      const float m_use = WINDOW && m_run == -INFINITY ? 0.f : m_run;  // nothing seen yet: every p is 0
+      const float m_use = (WINDOW || ROWS) && m_run == -INFINITY ? 0.f : m_run;  // nothing seen yet: every p is 0
       const uint64_t negm2 = f2(-m_use, -m_use);
       l_run += last ? exp_cols<0, kSplit, true>(s, p, scale2, negm2, lim) : exp_cols<0, kSplit, false>(s, p, scale2, negm2, lim);
       if (TILES == 2) mbar_arrive(&bar_exp_done[i]);
@@ -533,6 +636,11 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
         }
       }
       tmem_store_cols<BN / 2>(tP, p);
+      if (ROWS && col0 + BN > len) {
+        const int st = j % C::NS;
+        if (!warp_wait(&bar_v_full[st], (j / C::NS) & 1, ab)) { ok = false; break; }
+        clear_value_rows<C>(sV + st * C::KTILE, len - col0, t);
+      }
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&bar_p_full[i]);
@@ -546,36 +654,48 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
       // spilled register fewer).
       const int bh_e = *reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
       const int zi_e = bh_e / args.H, hi_e = bh_e % args.H;
-      __half* orow = reinterpret_cast<__half*>(args.o) + zi_e * args.so.z + hi_e * args.so.h + int64_t(row) * args.so.n;
+      bool whole = true;
+      if constexpr (ROWS) whole = args.rows.part == nullptr;
+      if (!whole) {
+        if constexpr (ROWS) store_part<C, D>(args, bh_e, row, nct, tO, m_run, l_run);
+      } else {
+        __half* orow;
+        if constexpr (ROWS)
+          orow = row_of(static_cast<__half*>(args.o), args.rows.so, args.rows.inner, zi_e, hi_e, row);
+        else
+          orow = reinterpret_cast<__half*>(args.o) + zi_e * args.so.z + hi_e * args.so.h + int64_t(row) * args.so.n;
 #pragma unroll
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        constexpr int W = D < 32 ? D : 32;
-        uint32_t o[W];
-        tmem_load_cols<W>(tO + c0, o);
-        tmem_wait_ld();
-        reg_fence<W>(o);
-        uint32_t h[W / 2];
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          constexpr int W = D < 32 ? D : 32;
+          uint32_t o[W];
+          tmem_load_cols<W>(tO + c0, o);
+          tmem_wait_ld();
+          reg_fence<W>(o);
+          uint32_t h[W / 2];
 #pragma unroll
-        for (int c = 0; c < W; c += 2)
-          h[c / 2] = pack_half2(__uint_as_float(o[c]) * inv_l, __uint_as_float(o[c + 1]) * inv_l);
-        if (row < N) {
-          uint4* dst = reinterpret_cast<uint4*>(orow + c0);
+          for (int c = 0; c < W; c += 2)
+            h[c / 2] = pack_half2(__uint_as_float(o[c]) * inv_l, __uint_as_float(o[c + 1]) * inv_l);
+          if (row < N) {
+            uint4* dst = reinterpret_cast<uint4*>(orow + c0);
 #pragma unroll
-          for (int v = 0; v < W / 8; ++v) dst[v] = make_uint4(h[4 * v], h[4 * v + 1], h[4 * v + 2], h[4 * v + 3]);
+            for (int v = 0; v < W / 8; ++v) dst[v] = make_uint4(h[4 * v], h[4 * v + 1], h[4 * v + 2], h[4 * v + 3]);
+          }
+          if ((WINDOW || ROWS) && args.o_rest != nullptr && row < N) {
+            uint32_t rest[W / 4];
+#pragma unroll
+            for (int c = 0; c < W; c += 4)
+              rest[c / 4] = rest_of(o + c, h[c / 2], inv_l) | (rest_of(o + c + 2, h[c / 2 + 1], inv_l) << 16);
+            uint4* dst = reinterpret_cast<uint4*>(args.o_rest + (int64_t(bh_e) * N + row) * D + c0);
+#pragma unroll
+            for (int v = 0; v < W / 16; ++v)
+              dst[v] = make_uint4(rest[4 * v], rest[4 * v + 1], rest[4 * v + 2], rest[4 * v + 3]);
+          }
         }
-        if (WINDOW && args.o_rest != nullptr && row < N) {
-          uint32_t rest[W / 4];
-#pragma unroll
-          for (int c = 0; c < W; c += 4)
-            rest[c / 4] = rest_of(o + c, h[c / 2], inv_l) | (rest_of(o + c + 2, h[c / 2 + 1], inv_l) << 16);
-          uint4* dst = reinterpret_cast<uint4*>(args.o_rest + (int64_t(bh_e) * N + row) * D + c0);
-#pragma unroll
-          for (int v = 0; v < W / 16; ++v)
-            dst[v] = make_uint4(rest[4 * v], rest[4 * v + 1], rest[4 * v + 2], rest[4 * v + 3]);
-        }
+        if (row < N && (!ROWS || args.m != nullptr)) args.m[int64_t(bh_e) * N + row] = m_run + log2f(l_run);
       }
-      if (row < N) args.m[int64_t(bh_e) * N + row] = m_run + log2f(l_run);
     }
+    if constexpr (ROWS)
+      if (n == 0 && row < N) no_keys<D>(args, *reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8), row, nct);
   }
 
   tc_fence_before();
@@ -587,14 +707,15 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
 }
 
 template <int D, int MASK, int BN, int NS, int TILES = 2>
-cudaError_t launch_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FwdArgs& a,
+cudaError_t launch_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const Args<MASK>& a,
                         cudaStream_t s) {
   using C = FwdCfg<D, BN, NS, TILES>;
   auto kern = fwd_f16_kernel<D, MASK, BN, NS, TILES>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
   if (e != cudaSuccess) return e;
   const int nct = (a.N + TILES * C::BM - 1) / (TILES * C::BM);
-  const long long grid = (long long)nct * a.Z * a.H;
+  long long grid = (long long)nct * a.Z * a.H;
+  if constexpr (MASK == kMaskRows) grid *= a.rows.nsplit;
   if (grid <= 0) return cudaSuccess;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   kern<<<dim3((unsigned)grid), dim3(128 * (TILES + 1)), C::SMEM_BYTES, s>>>(tq, tk, tv, a);
@@ -630,7 +751,23 @@ cudaError_t launch_variant(int v, const CUtensorMap& tq, const CUtensorMap& tk, 
   }
 }
 
+template <int D>
+cudaError_t launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const RowsFwdArgs& a, cudaStream_t s) {
+  if (rows_f16_tiles(D, a.N) == 1) return launch_impl<D, kMaskRows, rows_f16_block(D, 1), 2, 1>(tk, tk, tv, a, s);
+  return launch_impl<D, kMaskRows, rows_f16_block(D, 2), kFwdTiles[tile_default(0, D, false)].stages>(tk, tk, tv, a, s);
+}
+
 }  // namespace
+
+cudaError_t launch_rows_f16(int D, const CUtensorMap& tk, const CUtensorMap& tv, const RowsFwdArgs& a, cudaStream_t s) {
+  switch (D) {
+    case 16: return launch_rows<16>(tk, tv, a, s);
+    case 32: return launch_rows<32>(tk, tv, a, s);
+    case 64: return launch_rows<64>(tk, tv, a, s);
+    case 128: return launch_rows<128>(tk, tv, a, s);
+    default: return cudaErrorInvalidValue;
+  }
+}
 
 int fwd_f16_kv_rows(int D, int variant) {
   return tile_supported(0, variant, D) ? kFwdTiles[variant].block_n : 0;

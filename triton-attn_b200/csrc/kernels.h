@@ -18,6 +18,7 @@ enum Mask : int {
   kMaskNone = 0,    // all
   kMaskCausal = 1,  // key <= query
   kMaskWindow = 2,  // a sliding window and the first tokens (WindowArgs)
+  kMaskRows = 3,    // the first lengths[z] of them (RowsArgs)
 };
 
 // kMaskWindow: query row i stands at position i + off of its sequence and sees the keys j <= i + off with
@@ -35,6 +36,47 @@ struct WindowArgs {
 // finite O, the subnormal ones included, in range, and 2 mantissa bits leave an eighth of it.
 constexpr float kRestScale = 2048.f;
 
+// kMaskRows: `N` query rows against each of Z * H key/value heads, all of which see the head's first lengths[z] keys.
+// Row r lies at element r / inner * outer + r % inner * in behind the head's first: rows of several query heads, tokens
+// or sequences that share the keys are one matrix.
+struct RowMap {
+  int64_t z, h;      // of sequence z's and key/value head h's first row
+  int64_t outer, in;
+};
+constexpr int kMaxRowSplits = 128;
+template <typename T>
+__device__ __forceinline__ T* row_of(T* p, const RowMap& s, int inner, int z, int h, int row) {
+  const int o = row / inner;
+  return p + z * s.z + h * s.h + o * s.outer + (row - o * inner) * s.in;
+}
+struct RowsArgs {
+  const void* q;
+  RowMap sq, so;
+  int inner;
+  int Nk;               // rows of K and V
+  const int* lengths;   // [Z], or null: all Nk
+  // The blocks of keys are cut into nsplit equal parts, a CTA each. part not null: their unnormalised rows [Z * H, N,
+  // nsplit, D] and their maxima and sums [Z * H, N, nsplit, 2] (decode.cu's convention) are written, to be joined; else
+  // nsplit is 1.
+  int nsplit;
+  float* part;
+  float* part_ml;
+};
+// Parts that the `blocks` key blocks of `tiles` row tiles are cut into, of which `slots` run at a time: the number with
+// the shortest time, in blocks, when a CTA takes `start` to begin and to end and the parts' join `join`.
+inline int rows_splits(long long tiles, long long blocks, long long slots, int start, int join) {
+  int best = 1;
+  long long least = 0;
+  for (int n = 1; n <= blocks && n <= kMaxRowSplits; ++n) {
+    const long long cost = (tiles * n + slots - 1) / slots * ((blocks + n - 1) / n + start) + (n > 1 ? join : 0);
+    if (n == 1 || cost < least) {
+      least = cost;
+      best = n;
+    }
+  }
+  return best;
+}
+
 struct FwdArgs {
   void* o;           // [Z, H, N, D], strides `so`
   float* m;          // [Z, H, N] dense fp32: rowmax + log2(rowsum), base-2 units
@@ -45,8 +87,20 @@ struct FwdArgs {
   int* status;       // device status word
   unsigned long long wait_limit_ns;  // bound of every mbarrier wait (tattn_set_wait_limit_ns)
   WindowArgs win;    // kMaskWindow only
-  uint8_t* o_rest;   // kMaskWindow in fp16: what rounding O took off (kRestScale), dense [Z, H, N, D], or null
+  uint8_t* o_rest;   // kMaskWindow, kMaskRows in fp16: what rounding O took off (kRestScale), dense [Z, H, N, D], or null
 };
+// kMaskRows (apart from the others' arguments, whose kernels' registers a longer list costs); `so` is rows.so, and m
+// may be null.
+struct RowsFwdArgs : FwdArgs {
+  RowsArgs rows;
+};
+
+// Keys of sequence z that its queries see; a length outside [0, Nk] counts as the nearer end.
+__device__ __forceinline__ int held_keys(const int* lengths, int z, int Nk, bool* outside) {
+  const int len = lengths ? lengths[z] : Nk;
+  *outside = len < 0 || len > Nk;
+  return len < 0 ? 0 : len > Nk ? Nk : len;
+}
 
 // Window backward: its units of work. A key tile of a key/value head meets the query blocks that see it, once
 // for each query head of the group: a run of (head, block) pairs, head by head, which is cut into equal units.
@@ -116,6 +170,19 @@ __host__ __device__ inline WindowUnit window_unit(const WindowSplit& s, const Wi
   return u;
 }
 
+// Parts of rows that are to be joined: of every row up to two lists of unnormalised parts with their maxima and sums.
+struct JoinArgs {
+  const float *part[2], *part_ml[2];  // [rows, n, D] and [rows, n, 2]
+  int n[2];
+  RowMap other;        // where a row (as RowsArgs counts them) lies in the second list, in rows
+  void* o;
+  RowMap so;
+  int inner;
+  int Z, H, N;
+  float* m;            // as FwdArgs; null: not wanted
+  uint8_t* o_rest;     // as FwdArgs, or null
+};
+
 struct BwdArgs {
   // inputs
   const void* q; const void* k; const void* v; const void* o; const void* dout;
@@ -137,11 +204,25 @@ struct BwdArgs {
   WindowSplit split; // kMaskWindow
   float* part;       // kMaskWindow: partial dV and dK of the tiles of several units, or null
 };
+// kMaskRows: a window (`win`, `split`) that shows every query every key, of which sequence z has the first lengths[z].
+struct RowsBwdArgs : BwdArgs {
+  const int* lengths;  // [Z], or null: all
+};
+// The window that hides nothing.
+inline WindowArgs whole_window(int H, int Hk, int Nq, int Nk) { return WindowArgs{Hk, H / Hk, Nk, Nk, Nk + Nq, 0}; }
 
 // Host helpers of the C-ABI layer (capi.cu). device_ready: the current device is an sm_100 one whose primary
 // context is current on this thread, and *status its status word (a TATTN_* code). device_sm_count: its
 // streaming multiprocessors (cached per device). cuda_rc: a launch's result as a TATTN_* code.
 int device_ready(int** status);
+unsigned long long wait_limit_ns();
+// fp16 tensors for TMA (capi.cu): normalize replaces the strides of extent-1 dimensions, layout_ok says whether TMA can
+// address a tensor, encode_* make the maps (TATTN_* codes).
+Strides4 load_strides(const int64_t* s);
+Strides4 normalize(Strides4 s, int Z, int H, int N, int D);
+bool layout_ok(const void* p, Strides4 s, int Z, int H, int N, int D);
+int encode_f16(CUtensorMap* tm, const void* p, Strides4 s, int Z, int H, int N, int D, int box_rows, int box_cols = 0);
+int encode_f32_dense(CUtensorMap* tm, void* p, int Z, int H, int N, int D, int box_rows, int box_cols);
 int device_sm_count();
 int cuda_rc(cudaError_t e);
 
@@ -150,6 +231,11 @@ int cuda_rc(cudaError_t e);
 // Rows per K/V block of the fp16 forward variant for head dim D: the TMA box height of its K and V
 // tensor maps (the Q map always uses 128-row boxes); 0 if the variant does not fit D.
 int fwd_f16_kv_rows(int D, int variant);
+// kMaskRows: K and V in boxes of rows_f16_block keys.
+cudaError_t launch_rows_f16(int D, const CUtensorMap& tk, const CUtensorMap& tv, const RowsFwdArgs& a, cudaStream_t s);
+// kMaskRows: query tiles of a CTA, and keys of a block by that number. One tile (two CTAs an SM) where it holds all rows.
+constexpr int rows_f16_tiles(int D, int rows) { return rows <= 128 ? 1 : 2; }
+constexpr int rows_f16_block(int D, int tiles) { return D == 128 && tiles == 1 ? 64 : 128; }
 // TMA box heights of the fp16 split-backward kernels' Q/dO and K/V tensor maps for head dim D, dQ pass
 // or dK/dV pass, and tile variant.
 void bwd_f16_box_rows(int D, bool dq_pass, int variant, int* q_rows, int* kv_rows);
@@ -174,6 +260,9 @@ cudaError_t launch_bwd_dkdv_f16(int D, bool causal, int variant, const CUtensorM
 cudaError_t launch_bwd_fused_f16(int D, Mask mask, const CUtensorMap& tq, const CUtensorMap& tk,
                                  const CUtensorMap& tv, const CUtensorMap& tdo, const CUtensorMap& tdk,
                                  const CUtensorMap& tdv, const CUtensorMap& tdqacc, const BwdArgs& a, cudaStream_t s);
+cudaError_t launch_bwd_rows_f16(int D, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                                const CUtensorMap& tdo, const CUtensorMap& tdk, const CUtensorMap& tdv,
+                                const CUtensorMap& tdqacc, const RowsBwdArgs& a, cudaStream_t s);
 // Box height of the backward's output store maps (one warp's 32 TMEM lanes).
 constexpr int kBwdStoreRows = 32;
 // Query rows per block of the fused backward (its Q / dO box height): 128, or 64 at D = 128.
@@ -229,6 +318,10 @@ cudaError_t launch_bwd_dkdv_f32(int D, bool causal, const BwdArgs& a, cudaStream
 cudaError_t launch_window_fwd_f32(int D, const void* q, const void* k, const void* v, Strides4 sq, Strides4 sk,
                                   Strides4 sv, const FwdArgs& a, cudaStream_t s);
 cudaError_t launch_window_bwd_f32(int D, const BwdArgs& a, cudaStream_t s);
+// The same of rows against a sequence's first keys (kMaskRows; any strides but a unit one along D).
+cudaError_t launch_rows_f32(int D, const void* k, const void* v, Strides4 sk, Strides4 sv, const RowsFwdArgs& a, cudaStream_t s);
+cudaError_t launch_rows_bwd_f32(int D, const RowsBwdArgs& a, cudaStream_t s);
+cudaError_t launch_rows_join(int D, bool is_f16, const JoinArgs& a, cudaStream_t s);
 
 // delta = rowsum(dO * O) in fp32 (fp16 or fp32 inputs); also zeroes the rows of a.dq_acc and the
 // counter a.grid_sync when they are set (the fused backward's workspace).
@@ -259,9 +352,16 @@ struct RopeArgs {
   int w_f32;                  // weights (and dw) are fp32, else the tensors' type
   float eps;
   int* status;
+  // kAxesNorm, kAxes: positions is [A, Z, N], with axis stride pos_a
+  int64_t pos_a;
+  int A;                      // 1 to kRopeAxes
+  int back;                   // kAxes: turn by the negative angles
+  uint32_t axes[4];           // the axis of each of the D / 2 pairs, 2 bits a pair
 };
-constexpr int kRopeBlocksPerSm = 4;
-cudaError_t launch_norm_rope(int D, bool is_f16, bool interleaved, bool backward, RopeArgs a, cudaStream_t s);
+constexpr int kRopeBlocksPerSm = 4, kRopeAxes = 4;
+// One position a token, with the norms; positions on several axes, with the norms; those without (forward only).
+enum RopeForm : int { kOnePosition, kAxesNorm, kAxes };
+cudaError_t launch_norm_rope(int D, bool is_f16, RopeForm form, bool interleaved, bool backward, RopeArgs a, cudaStream_t s);
 
 // Attention of single tokens over a cache (decode.cu).
 enum DecodeCache : int { kCacheF16, kCacheInt4, kCacheF32 };
@@ -271,7 +371,7 @@ struct DecodeArgs {
   const void *k, *v;    // [Z, Hk, C, D], or the 4-bit cache's codes (Int4CacheArgs)
   const void *k_params, *v_params;  // 4-bit cache: its scales and minima
   Strides3 sq, so, sk, sv;
-  const int* lengths;   // [Z]: tokens held, the query's own among them
+  const int* lengths;   // [Z]: tokens held, the query's own among them; null: all C
   float* part;          // [Z, H, nsplit, D] unnormalised partial rows (nsplit > 1)
   float* part_ml;       // [Z, H, nsplit, 2] their maxima and sums
   int Z, H, Hk, C;
@@ -279,6 +379,7 @@ struct DecodeArgs {
   int nsplit;
   float qk_scale;       // sm_scale * log2(e)
   int* status;
+  bool parts_only;      // write the parts, also one alone, and do not join them
 };
 // CTAs per SM that decode_splits aims at: as many as an SM holds. (fp16, 64 sequences of 4096 visible tokens, 4
 // heads of 128: 2 parts each 82 us, 3 parts 86, 4 parts 90. 4 bits, 16 sequences of up to 65536 tokens: 10

@@ -1,4 +1,5 @@
-// Norms of query and key heads with the position rotation in the same pass, and the gradients.
+// Norms of query and key heads with the position rotation in the same pass, and the gradients; the rotation by
+// positions on several axes, with the norms or alone.
 //
 // A row x (one head of one token, D values) at position p, with the tensor's weight w and the tables
 // cos[p], sin[p] (D / 2 values each):
@@ -6,6 +7,8 @@
 //   y_i = z_i cos_j - z_i' sin_j,  y_i' = z_i' cos_j + z_i sin_j
 // for pair j = (i, i') = (j, j + D / 2), or (2 j, 2 j + 1) where `interleaved`. Backward, from dy:
 //   g = R^T dy,  dw = sum over rows of g x r,  h = g w,  dx = r (h - x r mean(h x r)).
+// On several axes (kAxesNorm, kAxes) a token has a position on each, and pair j is rotated by the tables' row at its
+// position on axis axes[j]. kAxes has no norm: y = R x and dx = R^T dy, the same kernel turning the other way.
 // Everything between the loads and the stores is fp32; results are rounded once.
 //
 // The bound is HBM: x is read and y written once (backward: x, dy, dx), about 3 (7) FMAs a value. A group of
@@ -132,9 +135,36 @@ __device__ __forceinline__ Item rope_item(const RopeArgs& a, const RopeTensor& t
   return it;
 }
 
-template <typename T, int D, bool INTERLEAVED, int HB, bool BACKWARD>
+// The cosines (or sines) of the lane's VEC pairs, from a row of their table.
+template <int D, int VEC, bool INTERLEAVED>
+__device__ __forceinline__ void load_angles(const float* row, int col, float* x) {
+  if constexpr (INTERLEAVED) {
+    load_floats<VEC / 2>(row + col / 2, x);
+    load_floats<VEC / 2>(row + D / 4 + col / 2, x + VEC / 2);
+  } else {
+    load_floats<VEC>(row + col, x);
+  }
+}
+
+// Which axis each of the lane's VEC pairs turns by (2 bits a pair from bit 0 on), and the set of those axes (from
+// bit 16 on).
+template <int D, int VEC, bool INTERLEAVED>
+__device__ __forceinline__ uint32_t lane_axes(const RopeArgs& a, int col) {
+  uint32_t x = 0;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    const int pair = !INTERLEAVED ? col + j : j < VEC / 2 ? col / 2 + j : D / 4 + col / 2 + j - VEC / 2;
+    const uint32_t axis = (a.axes[pair / 16] >> (2 * (pair % 16))) & 3u;
+    x |= axis << (2 * j) | 0x10000u << axis;
+  }
+  return x;
+}
+
+template <typename T, int D, bool INTERLEAVED, int HB, bool BACKWARD, RopeForm FORM>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 2) norm_rope_kernel(const RopeArgs a) {
   constexpr int VEC = kVec<T>, L = D / (2 * VEC), GROUPS = kThreads / L;
+  constexpr bool NORM = FORM != kAxes;
+  static_assert(NORM || !BACKWARD, "a rotation alone is turned back by the forward kernel");
   using P = Pairs<VEC, INTERLEAVED>;
   const int which = int(blockIdx.x) < a.t[0].blocks ? 0 : 1;  // the CTA's tensor
   const RopeTensor& t = a.t[which];
@@ -142,13 +172,17 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 2) norm_rope_ke
   const int c = threadIdx.x % L;
   const int col = c * VEC;  // and D / 2 + col
   float w[2 * VEC];
-  if (a.w_f32) {
-    load_floats<VEC>(static_cast<const float*>(t.w) + col, w);
-    load_floats<VEC>(static_cast<const float*>(t.w) + D / 2 + col, w + VEC);
-  } else {
-    load16(static_cast<const T*>(t.w) + col, w);
-    load16(static_cast<const T*>(t.w) + D / 2 + col, w + VEC);
+  if constexpr (NORM) {
+    if (a.w_f32) {
+      load_floats<VEC>(static_cast<const float*>(t.w) + col, w);
+      load_floats<VEC>(static_cast<const float*>(t.w) + D / 2 + col, w + VEC);
+    } else {
+      load16(static_cast<const T*>(t.w) + col, w);
+      load16(static_cast<const T*>(t.w) + D / 2 + col, w + VEC);
+    }
   }
+  uint32_t axes = 0;
+  if constexpr (FORM != kOnePosition) axes = lane_axes<D, VEC, INTERLEAVED>(a, col);
   float dw[2 * VEC];
 #pragma unroll
   for (int e = 0; e < 2 * VEC; ++e) dw[e] = 0.f;
@@ -158,19 +192,42 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 2) norm_rope_ke
     const int item = base + int(threadIdx.x) / L;
     const bool any = item < t.items;
     const Item it = rope_item(a, t, HB, any ? item : 0);
-    const int pos = a.positions ? a.positions[it.z * a.pos_z + it.n * a.pos_n] : it.n;
-    const bool in_table = pos >= 0 && pos < a.P;
     float cs[VEC], sn[VEC];
-    const float* ct = a.cos + int64_t(in_table ? pos : 0) * (D / 2);
-    const float* st = a.sin + int64_t(in_table ? pos : 0) * (D / 2);
-    if constexpr (INTERLEAVED) {
-      load_floats<VEC / 2>(ct + col / 2, cs);
-      load_floats<VEC / 2>(ct + D / 4 + col / 2, cs + VEC / 2);
-      load_floats<VEC / 2>(st + col / 2, sn);
-      load_floats<VEC / 2>(st + D / 4 + col / 2, sn + VEC / 2);
+    bool in_table = true;
+    if constexpr (FORM == kOnePosition) {
+      const int pos = a.positions ? a.positions[it.z * a.pos_z + it.n * a.pos_n] : it.n;
+      in_table = pos >= 0 && pos < a.P;
+      const int64_t at = int64_t(in_table ? pos : 0) * (D / 2);
+      load_angles<D, VEC, INTERLEAVED>(a.cos + at, col, cs);
+      load_angles<D, VEC, INTERLEAVED>(a.sin + at, col, sn);
     } else {
-      load_floats<VEC>(ct + col, cs);
-      load_floats<VEC>(st + col, sn);
+      int pos[kRopeAxes];
+#pragma unroll
+      for (int x = 0; x < kRopeAxes; ++x) {  // all of them, whichever axes the lane's pairs use: a row is NaN as a whole
+        pos[x] = x < a.A ? a.positions[x * a.pos_a + it.z * a.pos_z + it.n * a.pos_n] : 0;
+        in_table = in_table && pos[x] >= 0 && pos[x] < a.P;
+      }
+      // A row of each axis that some pair of the lane uses, 16 bytes at a time, and of it what those pairs need.
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) cs[j] = sn[j] = 0.f;
+#pragma unroll
+      for (int x = 0; x < kRopeAxes; ++x) {
+        if ((axes & (0x10000u << x)) == 0u) continue;
+        const int64_t at = int64_t(in_table ? pos[x] : 0) * (D / 2);
+        float c4[VEC], s4[VEC];
+        load_angles<D, VEC, INTERLEAVED>(a.cos + at, col, c4);
+        load_angles<D, VEC, INTERLEAVED>(a.sin + at, col, s4);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const bool mine = ((axes >> (2 * j)) & 3u) == uint32_t(x);
+          cs[j] = mine ? c4[j] : cs[j];
+          sn[j] = mine ? s4[j] : sn[j];
+        }
+      }
+      if (FORM == kAxes && a.back) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sn[j] = -sn[j];
+      }
     }
     if (!in_table && any) {  // no rotation exists: the rows become NaN, and the status word says why
 #pragma unroll
@@ -198,16 +255,19 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 2) norm_rope_ke
       float x[2 * VEC];
       unpack16<T>(rx[i][0], x);
       unpack16<T>(rx[i][1], x + VEC);
-      float sum = 0.f;
+      float r = 1.f;
+      if constexpr (NORM) {
+        float sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 2 * VEC; ++e) sum = fmaf(x[e], x[e], sum);
-      const float r = rsqrtf(group_sum<L>(sum) * (1.f / D) + a.eps);
+        for (int e = 0; e < 2 * VEC; ++e) sum = fmaf(x[e], x[e], sum);
+        r = rsqrtf(group_sum<L>(sum) * (1.f / D) + a.eps);
+      }
       float out[2 * VEC];
       if constexpr (!BACKWARD) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const int f = P::first(j), s = P::second(j);
-          const float zf = x[f] * r * w[f], zs = x[s] * r * w[s];
+          const float zf = NORM ? x[f] * r * w[f] : x[f], zs = NORM ? x[s] * r * w[s] : x[s];
           out[f] = zf * cs[j] - zs * sn[j];
           out[s] = zs * cs[j] + zf * sn[j];
         }
@@ -281,7 +341,7 @@ __global__ void __launch_bounds__(kThreads) norm_rope_dw_kernel(const RopeArgs a
   }
 }
 
-template <typename T, int D, bool INTERLEAVED, bool BACKWARD>
+template <typename T, int D, bool INTERLEAVED, bool BACKWARD, RopeForm FORM>
 cudaError_t rope_impl(RopeArgs& a, cudaStream_t s) {
   constexpr int GROUPS = kThreads / (D / (2 * kVec<T>));
   const int sms = device_sm_count();
@@ -302,30 +362,47 @@ cudaError_t rope_impl(RopeArgs& a, cudaStream_t s) {
   const int grid = a.t[0].blocks + a.t[1].blocks;
   if (grid > 0) {
     if (many)
-      norm_rope_kernel<T, D, INTERLEAVED, MANY, BACKWARD><<<grid, kThreads, 0, s>>>(a);
+      norm_rope_kernel<T, D, INTERLEAVED, MANY, BACKWARD, FORM><<<grid, kThreads, 0, s>>>(a);
     else
-      norm_rope_kernel<T, D, INTERLEAVED, 1, BACKWARD><<<grid, kThreads, 0, s>>>(a);
+      norm_rope_kernel<T, D, INTERLEAVED, 1, BACKWARD, FORM><<<grid, kThreads, 0, s>>>(a);
   }
   if (BACKWARD) norm_rope_dw_kernel<T><<<dim3(D / kDwCols, 2), kThreads, 0, s>>>(a, D);
   return cudaGetLastError();
 }
 
-template <typename T, bool BACKWARD>
+template <typename T, bool BACKWARD, RopeForm FORM>
 cudaError_t rope_dispatch(int D, bool interleaved, RopeArgs& a, cudaStream_t s) {
+#define TATTN_ROPE_CASE(DD) \
+  case DD: return interleaved ? rope_impl<T, DD, true, BACKWARD, FORM>(a, s) : rope_impl<T, DD, false, BACKWARD, FORM>(a, s);
   switch (D) {
-    case 16: return interleaved ? rope_impl<T, 16, true, BACKWARD>(a, s) : rope_impl<T, 16, false, BACKWARD>(a, s);
-    case 32: return interleaved ? rope_impl<T, 32, true, BACKWARD>(a, s) : rope_impl<T, 32, false, BACKWARD>(a, s);
-    case 64: return interleaved ? rope_impl<T, 64, true, BACKWARD>(a, s) : rope_impl<T, 64, false, BACKWARD>(a, s);
-    case 128: return interleaved ? rope_impl<T, 128, true, BACKWARD>(a, s) : rope_impl<T, 128, false, BACKWARD>(a, s);
+    TATTN_ROPE_CASE(16)
+    TATTN_ROPE_CASE(32)
+    TATTN_ROPE_CASE(64)
+    TATTN_ROPE_CASE(128)
     default: return cudaErrorInvalidValue;
+  }
+#undef TATTN_ROPE_CASE
+}
+
+template <typename T>
+cudaError_t rope_form(int D, RopeForm form, bool interleaved, bool backward, RopeArgs& a, cudaStream_t s) {
+  switch (form) {
+    case kOnePosition:
+      return backward ? rope_dispatch<T, true, kOnePosition>(D, interleaved, a, s)
+                      : rope_dispatch<T, false, kOnePosition>(D, interleaved, a, s);
+    case kAxesNorm:
+      return backward ? rope_dispatch<T, true, kAxesNorm>(D, interleaved, a, s)
+                      : rope_dispatch<T, false, kAxesNorm>(D, interleaved, a, s);
+    default:
+      return rope_dispatch<T, false, kAxes>(D, interleaved, a, s);
   }
 }
 
 }  // namespace
 
-cudaError_t launch_norm_rope(int D, bool is_f16, bool interleaved, bool backward, RopeArgs a, cudaStream_t s) {
-  if (is_f16) return backward ? rope_dispatch<__half, true>(D, interleaved, a, s) : rope_dispatch<__half, false>(D, interleaved, a, s);
-  return backward ? rope_dispatch<float, true>(D, interleaved, a, s) : rope_dispatch<float, false>(D, interleaved, a, s);
+cudaError_t launch_norm_rope(int D, bool is_f16, RopeForm form, bool interleaved, bool backward, RopeArgs a, cudaStream_t s) {
+  return is_f16 ? rope_form<__half>(D, form, interleaved, backward, a, s)
+                : rope_form<float>(D, form, interleaved, backward, a, s);
 }
 
 }  // namespace tattn

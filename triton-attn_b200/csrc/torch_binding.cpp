@@ -69,10 +69,11 @@ Tensor dense16(const Tensor& t) {
   return aligned16(c) ? c : c.clone();
 }
 Tensor rows16(const Tensor& t) { return rows16_ok(t) ? t : dense16(t); }
-// In place if the fp16 kernels' TMA can address it, else a dense copy.
-Tensor tma_ready(const Tensor& t) {
-  return tattn_layout_ok(t.data_ptr(), t.strides().data(), dim(t, 0), dim(t, 1), dim(t, 2), dim(t, 3)) ? t : dense16(t);
+bool tma_ok(const Tensor& t) {
+  return tattn_layout_ok(t.data_ptr(), t.strides().data(), dim(t, 0), dim(t, 1), dim(t, 2), dim(t, 3));
 }
+// In place if the fp16 kernels' TMA can address it, else a dense copy.
+Tensor tma_ready(const Tensor& t) { return tma_ok(t) ? t : dense16(t); }
 // A tensor for results, dense in the order of t's dimensions where that leaves 16-byte rows.
 Tensor like(const Tensor& t) {
   Tensor out = at::empty_like(t);
@@ -238,6 +239,158 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const 
   return {out[0], out[1]};
 }
 
+// ------------------------------------------------------------- rotation by positions on several axes
+constexpr int64_t kMaxAxes = 4;
+
+std::vector<int32_t> check_rope_axes(const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin, const Tensor& positions,
+                                     const std::vector<int64_t>& axes, const std::optional<Tensor>& wq,
+                                     const std::optional<Tensor>& wk) {
+  CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) && q.size(2) == k.size(2) && q.size(3) == k.size(3),
+                    "expected q [batch, heads, seq, dim] and k [batch, kv_heads, seq, dim]; got ", q.sizes(), ", ", k.sizes());
+  const int64_t b = q.size(0), n = q.size(2), d = q.size(3);
+  CHECK_VALUE(q.size(1) > 0 && k.size(1) > 0, "q and k need at least one head; got ", q.sizes(), ", ", k.sizes());
+  CHECK_VALUE(head_dim_ok(d), "head dim must be 16, 32, 64 or 128, got ", d);
+  CHECK_VALUE(k.scalar_type() == q.scalar_type() && dtype_ok(q), "q, k must share dtype float16 or float32, got ",
+                    q.scalar_type(), ", ", k.scalar_type());
+  CHECK_VALUE(wq.has_value() == wk.has_value(), "weights must be given for both q and k, or for neither");
+  if (wq.has_value()) {
+    CHECK_VALUE(wq->dim() == 1 && wk->dim() == 1 && wq->size(0) == d && wk->size(0) == d, "weights must have shape [", d,
+                      "]; got ", wq->sizes(), ", ", wk->sizes());
+    CHECK_VALUE(wk->scalar_type() == wq->scalar_type() && (wq->scalar_type() == q.scalar_type() || wq->scalar_type() == at::kFloat),
+                      "weights must share q's dtype or float32; got ", wq->scalar_type(), ", ", wk->scalar_type());
+  }
+  CHECK_VALUE(cos.dim() == 2 && cos.size(1) == d / 2 && sin.sizes() == cos.sizes(),
+                    "cos and sin must have shape [positions, ", d / 2, "]; got ", cos.sizes(), ", ", sin.sizes());
+  CHECK_VALUE(cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat, "cos and sin must be float32; got ",
+                    cos.scalar_type(), ", ", sin.scalar_type());
+  const Tensor& p = positions;
+  const int64_t a = p.dim() > 0 ? p.size(0) : 0;
+  const bool shape = (p.dim() == 2 && p.size(1) == n) || (p.dim() == 3 && p.size(1) == b && p.size(2) == n);
+  CHECK_VALUE(p.scalar_type() == at::kInt && shape && a >= 1 && a <= kMaxAxes, "positions must be int32 [axes, ", n, "] or [axes, ",
+                    b, ", ", n, "] with 1 to ", kMaxAxes, " axes; got ", p.scalar_type(), " ", p.sizes());
+  CHECK_VALUE(cos.size(0) > 0 || b * n == 0, "the tables hold no positions");
+  CHECK_VALUE(int64_t(axes.size()) == d / 2, "axes must name one axis for each of the ", d / 2, " pairs; got ", axes.size());
+  std::vector<int32_t> of_pairs(axes.size());
+  for (size_t j = 0; j < axes.size(); ++j) {
+    CHECK_VALUE(axes[j] >= 0 && axes[j] < a, "axes must lie in [0, ", a, "), got ", axes[j]);
+    of_pairs[j] = int32_t(axes[j]);
+  }
+  TORCH_CHECK(!wants_grad({&cos, &sin}), "cos and sin get no gradients; detach them");
+  refuse_forward_mode("qk_rope_axes", {&q, &k, &cos, &sin});
+  if (wq.has_value()) refuse_forward_mode("qk_rope_axes", {&*wq, &*wk});
+  auto same_device = [&](const Tensor& t) {
+    CHECK_VALUE(t.device() == q.device(), "all tensors must be on one device, got ", q.device(), " and ", t.device());
+  };
+  for (const Tensor* t : {&k, &cos, &sin, &positions}) same_device(*t);
+  if (wq.has_value()) {
+    same_device(*wq);
+    same_device(*wk);
+  }
+  require_cuda(q);
+  return of_pairs;
+}
+
+struct AxesArgs {
+  Tensor cos, sin, positions;
+  std::vector<int32_t> axes;
+  double eps;
+  bool interleaved;
+  void add_positions(Strides& st) const {
+    st.s[st.n++] = positions.stride(0);
+    positions.dim() == 2 ? st.add(0, positions.stride(1)) : st.add(positions.stride(1), positions.stride(2));
+  }
+};
+
+std::tuple<Tensor, Tensor> rope_axes_forward(const Tensor& q, const Tensor& k, const std::optional<Tensor>& wq,
+                                             const std::optional<Tensor>& wk, const AxesArgs& a) {
+  Tensor q_out = like(q), k_out = like(k);
+  Strides st;
+  st.add(q);
+  st.add(k);
+  st.add(q_out);
+  st.add(k_out);
+  a.add_positions(st);
+  const c10::cuda::CUDAGuard guard(q.device());
+  check_status("tattn_qk_rope_axes",
+               tattn_qk_rope_axes(q.data_ptr(), k.data_ptr(), ptr(wq), ptr(wk), q_out.data_ptr(), k_out.data_ptr(),
+                                  a.cos.data_ptr<float>(), a.sin.data_ptr<float>(), a.positions.data_ptr<int32_t>(), a.axes.data(),
+                                  st.s, dim(q, 0), dim(q, 1), dim(k, 1), dim(q, 2), dim(q, 3), dim(a.cos, 0),
+                                  dim(a.positions, 0), code(q), wq.has_value() ? code(*wq) : code(q), float(a.eps),
+                                  a.interleaved, stream_of(q)));
+  return {q_out, k_out};
+}
+
+struct QkRopeAxes : torch::autograd::Function<QkRopeAxes> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const std::optional<Tensor>& wq,
+                               const std::optional<Tensor>& wk, const Tensor& cos, const Tensor& sin, const Tensor& positions,
+                               const std::vector<int64_t>& axes, double eps, bool interleaved) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    // The rotation alone is turned back without q and k.
+    const bool norm = wq.has_value();
+    ctx->save_for_backward({norm ? q : Tensor(), norm ? k : Tensor(), norm ? *wq : Tensor(), norm ? *wk : Tensor(), cos, sin, positions});
+    ctx->saved_data["axes"] = axes;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    auto [q_out, k_out] = rope_axes_forward(q, k, wq, wk, AxesArgs{cos, sin, positions, {axes.begin(), axes.end()}, eps, interleaved});
+    return {q_out, k_out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(10);
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const variable_list saved = ctx->get_saved_variables();
+      const Tensor &wq = saved[2], &wk = saved[3];
+      const std::vector<int64_t> axes = ctx->saved_data["axes"].toIntVector();
+      const AxesArgs a{saved[4], saved[5], saved[6], {axes.begin(), axes.end()}, ctx->saved_data["eps"].toDouble(),
+                       ctx->saved_data["interleaved"].toBool()};
+      const bool norm = wq.defined();
+      const Tensor gq = rows16(grads[0]), gk = rows16(grads[1]);  // (zeros where a result was not used)
+      const Tensor &q = norm ? saved[0] : gq, &k = norm ? saved[1] : gk;
+      Tensor dq = like(q), dk = like(k), dwq, dwk, ws;
+      const c10::cuda::CUDAGuard guard(q.device());
+      if (norm) {
+        dwq = at::empty_like(wq);
+        dwk = at::empty_like(wk);
+        ws = bytes(tattn_qk_norm_rope_bwd_workspace_bytes(dim(q, 3)), q);
+      }
+      Strides st;
+      st.add(q);
+      st.add(k);
+      st.add(gq);
+      st.add(gk);
+      st.add(dq);
+      st.add(dk);
+      a.add_positions(st);
+      auto at = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+      check_status("tattn_qk_rope_axes_bwd",
+                   tattn_qk_rope_axes_bwd(q.data_ptr(), k.data_ptr(), at(wq), at(wk), gq.data_ptr(), gk.data_ptr(), dq.data_ptr(),
+                                          dk.data_ptr(), at(dwq), at(dwk), a.cos.data_ptr<float>(), a.sin.data_ptr<float>(),
+                                          a.positions.data_ptr<int32_t>(), a.axes.data(), at(ws), st.s, dim(q, 0), dim(q, 1),
+                                          dim(k, 1), dim(q, 2), dim(q, 3), dim(a.cos, 0), dim(a.positions, 0), code(q),
+                                          norm ? code(wq) : code(q), float(a.eps), a.interleaved, stream_of(q)));
+      out[0] = dq;
+      out[1] = dk;
+      out[2] = dwq;
+      out[3] = dwk;
+    }
+    return once(std::move(out));
+  }
+};
+
+std::tuple<Tensor, Tensor> qk_rope_axes(const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin, const Tensor& positions,
+                                        const std::vector<int64_t>& axes, const std::optional<Tensor>& wq,
+                                        const std::optional<Tensor>& wk, double eps, bool interleaved) {
+  std::vector<int32_t> of_pairs = check_rope_axes(q, k, cos, sin, positions, axes, wq, wk);
+  const bool norm = wq.has_value();
+  const Tensor q_ = rows16(q), k_ = rows16(k), cos_ = dense16(cos), sin_ = dense16(sin);
+  const std::optional<Tensor> wq_ = norm ? std::optional<Tensor>(dense16(*wq)) : std::nullopt;
+  const std::optional<Tensor> wk_ = norm ? std::optional<Tensor>(dense16(*wk)) : std::nullopt;
+  if (!wants_grad({&q, &k}) && !(norm && wants_grad({&*wq, &*wk})))
+    return rope_axes_forward(q_, k_, wq_, wk_, AxesArgs{cos_, sin_, positions, std::move(of_pairs), eps, interleaved});
+  variable_list out = QkRopeAxes::apply(q_, k_, wq_, wk_, cos_, sin_, positions, axes, eps, interleaved);
+  return {out[0], out[1]};
+}
+
 // --------------------------------------------------------------------------------- window attention
 void check_heads(const Tensor& q, const Tensor& k, const Tensor& v) {
   CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes(),
@@ -399,6 +552,139 @@ Tensor decode_attention(const Tensor& q0, const Tensor& k, const Tensor& v, cons
   return o;
 }
 
+// ------------------------------------------------------------------------------- cross attention
+// int32 [count] on q's device, or none.
+std::optional<Tensor> check_lengths(const char* name, const std::optional<Tensor>& t, const Tensor& q, int64_t count) {
+  if (!t.has_value()) return std::nullopt;
+  CHECK_VALUE(t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == count, name, " must be int32 [", count, "]; got ",
+                    t->scalar_type(), " ", t->sizes());
+  CHECK_VALUE(t->device() == q.device(), name, " must be on q's device, got ", t->device());
+  return t->contiguous();
+}
+
+// A tensor that the kernels read in place, or its dense copy: 16-byte rows, and in fp16 what TMA can address.
+Tensor rows_ready(const Tensor& t) {
+  const Tensor r = rows16(t);
+  return t.scalar_type() == at::kHalf ? tma_ready(r) : r;
+}
+
+// (O like q, M fp32 [Z, H, Nq], what rounding took off an fp16 O) of checked tensors that rows_ready gave; the last two
+// for a backward pass only.
+std::tuple<Tensor, Tensor, Tensor> cross_forward(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                 const std::optional<Tensor>& lengths, double scale, bool backward) {
+  Tensor o = like(q), m, rest;
+  if (backward) {
+    m = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+    if (q.scalar_type() == at::kHalf) rest = at::empty(q.sizes(), q.options().dtype(at::kByte), at::MemoryFormat::Contiguous);
+  }
+  const int z = dim(q, 0), h = dim(q, 1), hk = dim(k, 1), n = dim(q, 2), nk = dim(k, 2), d = dim(q, 3);
+  Strides st;
+  st.add(q);
+  st.add(k);
+  st.add(v);
+  st.add(o);
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int64_t size = tattn_cross_fwd_workspace_bytes(z, h, hk, n, nk, d, code(q));
+  const Tensor ws = size > 0 ? bytes(size, q) : Tensor();
+  check_status("tattn_cross_fwd",
+               tattn_cross_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), static_cast<const int32_t*>(ptr(lengths)), o.data_ptr(),
+                               backward ? m.data_ptr<float>() : nullptr, rest.defined() ? rest.data_ptr() : nullptr,
+                               size > 0 ? ws.data_ptr() : nullptr, st.s, z, h, hk, n, nk, d, code(q), float(scale), stream_of(q)));
+  return {o, m, rest};
+}
+
+struct CrossAttention : torch::autograd::Function<CrossAttention> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                        const std::optional<Tensor>& lengths, double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [o, m, rest] = cross_forward(q, k, v, lengths, scale, true);
+    ctx->save_for_backward({q, k, v, lengths.has_value() ? *lengths : Tensor(), o, m, rest});
+    ctx->saved_data["scale"] = scale;
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(5);
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const variable_list s = ctx->get_saved_variables();
+      const Tensor &q = s[0], &k = s[1], &v = s[2], &lengths = s[3], &m = s[5], &rest = s[6];
+      const Tensor o = rows_ready(s[4]), g = rows_ready(grads[0]);
+      const int z = dim(q, 0), h = dim(q, 1), hk = dim(k, 1), n = dim(q, 2), nk = dim(k, 2), d = dim(q, 3);
+      Tensor delta = at::empty({z, h, n}, q.options().dtype(at::kFloat));
+      Tensor dq = at::empty({z, h, n, d}, q.options()), dk = at::empty({z, hk, nk, d}, q.options());
+      Tensor dv = at::empty({z, hk, nk, d}, q.options());
+      Strides st;
+      st.add(q);
+      st.add(k);
+      st.add(v);
+      st.add(o);
+      st.add(g);
+      const c10::cuda::CUDAGuard guard(q.device());
+      const int64_t size = std::max<int64_t>(0, tattn_cross_bwd_workspace_bytes(z, h, hk, n, nk, d, code(q)));
+      const Tensor ws = size > 0 ? bytes(size, q) : Tensor();
+      check_status("tattn_cross_bwd",
+                   tattn_cross_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), lengths.defined() ? lengths.data_ptr<int32_t>() : nullptr,
+                                   o.data_ptr(), g.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), m.data_ptr<float>(),
+                                   rest.defined() ? rest.data_ptr() : nullptr, delta.data_ptr<float>(),
+                                   size > 0 ? ws.data_ptr() : nullptr, st.s, z, h, hk, n, nk, d, code(q),
+                                   float(ctx->saved_data["scale"].toDouble()), stream_of(q)));
+      out[0] = dq;
+      out[1] = dk;
+      out[2] = dv;
+    }
+    return once(std::move(out));
+  }
+};
+
+Tensor cross_attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, const std::optional<Tensor>& lengths0,
+                       const std::optional<double>& sm_scale) {
+  check_heads(q0, k0, v0);
+  const std::optional<Tensor> lengths = check_lengths("lengths", lengths0, q0, q0.size(0));
+  refuse_forward_mode("cross_attention", {&q0, &k0, &v0});
+  require_cuda(q0);
+  const Tensor q = rows_ready(q0), k = rows_ready(k0), v = rows_ready(v0);
+  const double scale = scale_of(sm_scale, q);
+  if (!wants_grad({&q0, &k0, &v0})) return std::get<0>(cross_forward(q, k, v, lengths, scale, false));
+  return CrossAttention::apply(q, k, v, lengths, scale);
+}
+
+// ------------------------------------------------------------- single tokens over a shared prefix
+Tensor prefix_decode_attention(const Tensor& q0, const Tensor& pk, const Tensor& pv, const Tensor& k, const Tensor& v,
+                               const Tensor& lengths0, const std::optional<Tensor>& prefix_lengths0,
+                               const std::optional<double>& sm_scale) {
+  check_heads(q0, k, v);
+  CHECK_VALUE(pk.dim() == 4 && pv.sizes() == pk.sizes() && pk.size(1) == k.size(1) && pk.size(3) == k.size(3),
+                    "expected prefix_k, prefix_v [prompts, ", k.size(1), ", prefix capacity, ", k.size(3), "]; got ", pk.sizes(),
+                    ", ", pv.sizes());
+  CHECK_VALUE(pk.scalar_type() == q0.scalar_type() && pv.scalar_type() == q0.scalar_type(), "the prefix must have q's dtype ",
+                    q0.scalar_type(), ", got ", pk.scalar_type(), ", ", pv.scalar_type());
+  CHECK_VALUE(pk.device() == q0.device() && pv.device() == q0.device(), "the prefix must be on q's device, got ", pk.device(),
+                    ", ", pv.device());
+  const int64_t prompts = pk.size(0), batch = q0.size(0);
+  CHECK_VALUE(prompts > 0 ? batch % prompts == 0 : batch == 0, "the batch must be a multiple of the prompts; got ", batch, " and ",
+                    prompts);
+  check_token({&q0, &k, &v, &pk, &pv}, lengths0, std::nullopt, 0);
+  const std::optional<Tensor> prefix_lengths = check_lengths("prefix_lengths", prefix_lengths0, q0, prompts);
+  refuse_forward_mode("prefix_decode_attention", {&q0, &k, &v, &pk, &pv});
+  require_cuda(q0);
+  for (const Tensor* t : {&k, &v, &pk, &pv})
+    CHECK_VALUE(rows16_ok(*t) && (t->scalar_type() != at::kHalf || t == &k || t == &v || tma_ok(*t)),
+                      "k, v and the prefix need contiguous, 16-byte aligned rows: a cache is read in place, never copied");
+  const Tensor q = rows16(q0), lengths = lengths0.contiguous();
+  Tensor o = like(q);
+  if (o.numel() == 0) return o;
+  const int samples = int(batch / prompts), h = dim(q, 1), hk = dim(k, 1), p = dim(pk, 2), cap = dim(k, 2), d = dim(q, 3);
+  Strides st;
+  for (const Tensor* t : std::initializer_list<const Tensor*>{&q, &pk, &pv, &k, &v, &o}) st.add(*t);
+  const c10::cuda::CUDAGuard guard(q.device());
+  const Tensor ws = bytes(std::max<int64_t>(0, tattn_prefix_decode_workspace_bytes(dim(pk, 0), samples, h, hk, p, cap, d, code(q))), q);
+  check_status("tattn_prefix_decode",
+               tattn_prefix_decode(q.data_ptr(), pk.data_ptr(), pv.data_ptr(), static_cast<const int32_t*>(ptr(prefix_lengths)),
+                                   k.data_ptr(), v.data_ptr(), lengths.data_ptr<int>(), o.data_ptr(), ws.data_ptr(), st.s,
+                                   dim(pk, 0), samples, h, hk, p, cap, d, code(q), float(scale_of(sm_scale, q)), stream_of(q)));
+  return o;
+}
+
 // ------------------------------------------------------------------------------------- 4-bit cache
 // The cache's tensors, as tattn.Int4Cache holds them.
 void int4_check(const Tensor& kc, const Tensor& kp, const Tensor& vc, const Tensor& vp) {
@@ -498,10 +784,13 @@ Tensor int4_attend(const Tensor& kc, const Tensor& kp, const Tensor& vc, const T
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("abi_version", &tattn_abi_version);
   m.def("qk_norm_rope", &qk_norm_rope);
+  m.def("qk_rope_axes", &qk_rope_axes);
   m.def("window_attention", &window_attention);
   m.def("window_forward", &window_forward);
   m.def("window_backward", &window_backward);
   m.def("decode_attention", &decode_attention);
+  m.def("cross_attention", &cross_attention);
+  m.def("prefix_decode_attention", &prefix_decode_attention);
   m.def("int4_check", &int4_check);
   m.def("int4_append", &int4_append);
   m.def("int4_read", &int4_read);

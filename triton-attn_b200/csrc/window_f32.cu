@@ -1,4 +1,5 @@
-// Sliding-window attention with sinks for fp32 on CUDA cores: forward, dK/dV and dQ.
+// Sliding-window attention with sinks for fp32 on CUDA cores: forward, dK/dV and dQ. The same kernels with ROWS are
+// attention to the first lengths[z] keys of a sequence (kMaskRows), whose forward may take a part of the keys.
 //
 // The mathematics is the fp16 kernels' (base-2 online softmax, M = m + log2 l, P rebuilt from M in the
 // backward) with every product and sum in fp32: tcgen05 has no fp32 MMA, and fp32 calls are held to fp32
@@ -20,7 +21,10 @@
 // at the first size (40 with the masked pairs of its tiles), 13 to 14 at B3 H5 N1000 D64, window 200, 4 sinks (56 us
 // forward, 172 backward; 19 with the masked ones), where the 480 tiles differ in length and the busiest SM has 1.55
 // times the mean.
+#include <float.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -56,6 +60,18 @@ __device__ __forceinline__ void load_rows(float* dst, const float* src, const St
   for (int e = threadIdx.x; e < ROWS * D; e += THREADS) {
     const int r = e / D, d = e % D;
     dst[r * kPitch<D> + d] = r0 + r < n ? __ldg(src + int64_t(r0 + r) * s.n + d * s.d) : 0.f;
+  }
+}
+
+// ROWS: rows [r0, r0 + T) of the head's matrix (RowMap).
+template <int D, int T, int THREADS>
+__device__ __forceinline__ void load_mapped_rows(float* dst, const RowsFwdArgs& a, int z, int h, int r0) {
+#pragma unroll 2
+  for (int i = 0; i < T * D / 4 / THREADS; ++i) {
+    const int e = i * THREADS + threadIdx.x, r = e / (D / 4), d = e % (D / 4) * 4;
+    const bool in = r0 + r < a.N;
+    cp_async16(smem_u32(dst + r * kPitch<D> + d),
+               row_of(static_cast<const float*>(a.rows.q), a.rows.sq, a.rows.inner, z, h, in ? r0 + r : 0) + d, in);
   }
 }
 
@@ -121,6 +137,15 @@ __device__ __forceinline__ bool sees(int row, int col, int N, const WindowArgs& 
   const int p = row + w.off;
   return row < N && col <= p && (col > p - w.window || col < w.sinks);
 }
+// ROWS: of `len` keys all, as the window of `w` hides none.
+template <bool ROWS>
+__device__ __forceinline__ bool sees(int row, int col, int N, int len, const WindowArgs& w) {
+  return ROWS ? row < N && col < len : sees(row, col, N, w);
+}
+template <bool ROWS>
+using Fwd = std::conditional_t<ROWS, RowsFwdArgs, FwdArgs>;
+template <bool ROWS>
+using Bwd = std::conditional_t<ROWS, RowsBwdArgs, BwdArgs>;
 
 // Blocks of keys of the query rows from r0 on: those with sinks, then those that a window reaches, up to the diagonal.
 __device__ __forceinline__ int next_keys(int k0, int r0, const WindowArgs& w) {
@@ -128,22 +153,36 @@ __device__ __forceinline__ int next_keys(int k0, int r0, const WindowArgs& w) {
   return k0 >= w.sinks ? max(k0, max(0, r0 + w.off - w.window + 1) / TB * TB) : k0;
 }
 
-template <int D, int T>
+template <int D, int T, bool ROWS>
 __global__ void __launch_bounds__(kThreads<D, T>) window_fwd_f32_kernel(const float* q, const float* k, const float* v,
-                                                                  Strides4 sq, Strides4 sk, Strides4 sv, FwdArgs a) {
+                                                                  Strides4 sq, Strides4 sk, Strides4 sv, Fwd<ROWS> a) {
   constexpr int R = kRows<D, T>, TH = kThreads<D, T>;
   extern __shared__ __align__(16) float smem[];
   float *Qs = smem, *Ks = Qs + T * kPitch<D>, *Vs = Ks + TB * kPitch<D>, *Ps = Vs + TB * kPitch<D>;
-  const int N = a.N, Nk = a.win.Nk, r0 = blockIdx.x * T;
+  const int N = a.N, tiles = (N + T - 1) / T, split = ROWS ? blockIdx.x / tiles : 0, r0 = (blockIdx.x - split * tiles) * T;
   const int64_t head = cta_head();
   if (head >= int64_t(a.Z) * a.H) return;
-  const int zi = int(head / a.H), hi = int(head % a.H), hk = hi / a.win.group;
+  const int zi = int(head / a.H), hi = int(head % a.H), hk = ROWS ? hi : hi / a.win.group;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   k += zi * sk.z + hk * sk.h;
   v += zi * sv.z + hk * sv.h;
-  int k0 = next_keys(-TB, r0, a.win);
-  load_rows<D, T, TH>(Qs, q + zi * sq.z + hi * sq.h, sq, r0, N);
-  load_rows<D, TB, TH>(Ks, k, sk, k0, Nk);
+  int Nk, k0, end;  // keys; the first and behind the last one that this CTA goes through
+  auto after = [&](int k0) { return ROWS ? k0 + TB : next_keys(k0, r0, a.win); };
+  if constexpr (ROWS) {
+    bool outside;
+    Nk = held_keys(a.rows.lengths, zi, a.rows.Nk, &outside);
+    if (outside && threadIdx.x == 0) atomicOr(a.status, kStatusIndexRange);
+    const int64_t blocks = (Nk + TB - 1) / TB;
+    k0 = int(blocks * split / a.rows.nsplit) * TB;
+    end = min(int(blocks * (split + 1) / a.rows.nsplit) * TB, Nk);
+    load_mapped_rows<D, T, TH>(Qs, a, zi, hi, r0);
+  } else {
+    Nk = a.win.Nk;
+    k0 = next_keys(-TB, r0, a.win);
+    end = min(r0 + T + a.win.off, Nk);
+    load_rows<D, T, TH>(Qs, q + zi * sq.z + hi * sq.h, sq, r0, N);
+  }
+  if (!ROWS || k0 < end) load_rows<D, TB, TH>(Ks, k, sk, k0, Nk);
   float m[R], l[R], acc[R][D / 16];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -152,7 +191,7 @@ __global__ void __launch_bounds__(kThreads<D, T>) window_fwd_f32_kernel(const fl
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) acc[i][e] = 0.f;
   }
-  const int end = min(r0 + T + a.win.off, Nk);
+  const bool any = k0 < end;
   for (int next; k0 < end; k0 = next) {
     cp_async_wait_all();
     __syncthreads();  // K is here, and V's last tile has been read
@@ -164,7 +203,7 @@ __global__ void __launch_bounds__(kThreads<D, T>) window_fwd_f32_kernel(const fl
       float mx = m[i];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        s[i][j] = sees(r0 + R * ty + i, k0 + tx + 16 * j, N, a.win) ? s[i][j] * a.qk_scale : -INFINITY;
+        s[i][j] = sees<ROWS>(r0 + R * ty + i, k0 + tx + 16 * j, N, Nk, a.win) ? s[i][j] * a.qk_scale : -INFINITY;
         mx = fmaxf(mx, s[i][j]);
       }
 #pragma unroll
@@ -183,16 +222,34 @@ __global__ void __launch_bounds__(kThreads<D, T>) window_fwd_f32_kernel(const fl
     }
     cp_async_wait_all();
     __syncthreads();  // V is here, and K has been read
-    next = next_keys(k0, r0, a.win);
+    next = after(k0);
     if (next < end) load_rows<D, TB, TH>(Ks, k, sk, next, Nk);
     rows_times<D, R>(Ps, Vs, ty, tx, acc);
   }
+  if (ROWS) cp_async_wait_all();  // the rows, where there are no keys
 #pragma unroll
   for (int i = 0; i < R; ++i) {
 #pragma unroll
     for (int o = 1; o < 16; o *= 2) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
     const int row = r0 + R * ty + i;
     if (row >= N) continue;
+    if constexpr (ROWS) {
+      if (a.rows.part != nullptr) {
+        const int64_t at = (head * N + row) * a.rows.nsplit + split;
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) a.rows.part[at * D + D / 16 * tx + e] = acc[i][e];
+        if (tx == 0)
+          reinterpret_cast<float2*>(a.rows.part_ml)[at] =
+              make_float2(any && m[i] == -INFINITY ? -FLT_MAX : m[i], l[i]);  // (-infinity: no keys)
+      } else {
+        float* o = row_of(static_cast<float*>(a.o), a.rows.so, a.rows.inner, zi, hi, row) + D / 16 * tx;
+        const float inv = any ? 1.f / l[i] : 0.f;
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) o[e] = acc[i][e] * inv;
+        if (a.m != nullptr && tx == 0) a.m[head * N + row] = any ? m[i] + log2f(l[i]) : -INFINITY;
+      }
+      continue;
+    }
     float* o = static_cast<float*>(a.o) + zi * a.so.z + hi * a.so.h + int64_t(row) * a.so.n;
     const float inv = 1.f / l[i];
 #pragma unroll
@@ -203,9 +260,9 @@ __global__ void __launch_bounds__(kThreads<D, T>) window_fwd_f32_kernel(const fl
 
 // P and dS of rows R ty + i of A (with C) and rows tx + 16 j of B (with E): A, B are queries and keys, or keys
 // and queries (KEYS); C, E their dO and V, or V and dO.
-template <int D, int R, bool KEYS>
-__device__ __forceinline__ void p_ds(const BwdArgs& a, const float* A, const float* B, const float* C, const float* E,
-                                     int ty, int tx, int a0, int b0, const float* Ms, const float* Ds, float (*p)[4],
+template <int D, int R, bool KEYS, bool ROWS>
+__device__ __forceinline__ void p_ds(const Bwd<ROWS>& a, const float* A, const float* B, const float* C, const float* E,
+                                     int ty, int tx, int a0, int b0, int len, const float* Ms, const float* Ds, float (*p)[4],
                                      float (*ds)[4]) {
   float s[R][4], dp[R][4];
   rows_dot<D, R>(A, B, ty, tx, s);
@@ -216,45 +273,50 @@ __device__ __forceinline__ void p_ds(const BwdArgs& a, const float* A, const flo
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int ra = R * ty + i, rb = tx + 16 * j, row = KEYS ? rb : ra;  // the tile's query row
-      const bool see = KEYS ? sees(b0 + rb, a0 + ra, a.N, a.win) : sees(a0 + ra, b0 + rb, a.N, a.win);
+      const bool see = KEYS ? sees<ROWS>(b0 + rb, a0 + ra, a.N, len, a.win) : sees<ROWS>(a0 + ra, b0 + rb, a.N, len, a.win);
       p[i][j] = see ? exp2f(s[i][j] * qks - Ms[row]) : 0.f;
-      ds[i][j] = p[i][j] * (dp[i][j] - Ds[row]);
+      ds[i][j] = ROWS && !see ? 0.f : p[i][j] * (dp[i][j] - Ds[row]);
     }
 }
 
-template <int D, int T>
-__global__ void __launch_bounds__(kThreads<D, T>) window_dq_f32_kernel(BwdArgs a) {
+template <int D, int T, bool ROWS>
+__global__ void __launch_bounds__(kThreads<D, T>) window_dq_f32_kernel(Bwd<ROWS> a) {
   constexpr int R = kRows<D, T>, TH = kThreads<D, T>;
   extern __shared__ __align__(16) float smem[];
   float *Qs = smem, *Os = Qs + T * kPitch<D>, *Vs = Os + T * kPitch<D>;
   float *Ks = Vs + TB * kPitch<D>, *Kn = Ks + TB * kPitch<D>;  // K's tile and the next one
   float *DSs = Kn + TB * kPitch<D>, *Ms = DSs + T * kPitchP, *Ds = Ms + T;
-  const int N = a.N, Nk = a.win.Nk, r0 = blockIdx.x * T;
+  const int N = a.N, r0 = blockIdx.x * T;
   const int64_t head = cta_head();
   if (head >= int64_t(a.Z) * a.H) return;
   const int zi = int(head / a.H), hi = int(head % a.H), hk = hi / a.win.group;
+  int Nk = a.win.Nk;
+  bool outside;
+  if constexpr (ROWS) Nk = held_keys(a.lengths, zi, Nk, &outside);
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const float* k = static_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h;
   const float* v = static_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h;
   load_rows<D, T, TH>(Qs, static_cast<const float*>(a.q) + zi * a.sq.z + hi * a.sq.h, a.sq, r0, N);
   load_rows<D, T, TH>(Os, static_cast<const float*>(a.dout) + zi * a.sdo.z + hi * a.sdo.h, a.sdo, r0, N);
-  int k0 = next_keys(-TB, r0, a.win);
-  load_rows<D, TB, TH>(Ks, k, a.sk, k0, Nk);
-  load_rows<D, TB, TH>(Vs, v, a.sv, k0, Nk);
+  int k0 = ROWS ? 0 : next_keys(-TB, r0, a.win);
+  if (!ROWS || Nk > 0) {
+    load_rows<D, TB, TH>(Ks, k, a.sk, k0, Nk);
+    load_rows<D, TB, TH>(Vs, v, a.sv, k0, Nk);
+  }
   if (threadIdx.x < T) {
     const int row = r0 + threadIdx.x;
     Ms[threadIdx.x] = row < N ? a.m[head * N + row] : 0.f;
     Ds[threadIdx.x] = row < N ? a.delta[head * N + row] : 0.f;
   }
   float acc[R][D / 16] = {};
-  const int end = min(r0 + T + a.win.off, Nk);
+  const int end = ROWS ? Nk : min(r0 + T + a.win.off, Nk);
   for (int next; k0 < end; k0 = next) {
     cp_async_wait_all();
     __syncthreads();  // K and V are here, and K's last tile has been read
-    next = next_keys(k0, r0, a.win);
+    next = ROWS ? k0 + TB : next_keys(k0, r0, a.win);
     if (next < end) load_rows<D, TB, TH>(Kn, k, a.sk, next, Nk);
     float p[R][4], ds[R][4];
-    p_ds<D, R, false>(a, Qs, Ks, Os, Vs, ty, tx, r0, k0, Ms, Ds, p, ds);
+    p_ds<D, R, false, ROWS>(a, Qs, Ks, Os, Vs, ty, tx, r0, k0, Nk, Ms, Ds, p, ds);
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
@@ -266,6 +328,7 @@ __global__ void __launch_bounds__(kThreads<D, T>) window_dq_f32_kernel(BwdArgs a
     Ks = Kn;
     Kn = t;
   }
+  if (ROWS) cp_async_wait_all();  // Q and dO, where there are no keys
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int row = r0 + R * ty + i;
@@ -278,8 +341,8 @@ __global__ void __launch_bounds__(kThreads<D, T>) window_dq_f32_kernel(BwdArgs a
 
 // One unit (window_unit): a key tile of a key/value head, summed over the query heads that share it, or a part of
 // that sum.
-template <int D, int T>
-__global__ void __launch_bounds__(kThreads<D, T>) window_dkdv_f32_kernel(BwdArgs a) {
+template <int D, int T, bool ROWS>
+__global__ void __launch_bounds__(kThreads<D, T>) window_dkdv_f32_kernel(Bwd<ROWS> a) {
   constexpr int R = kRows<D, T>, TH = kThreads<D, T>;
   extern __shared__ __align__(16) float smem[];
   float *Ks = smem, *Vs = Ks + T * kPitch<D>, *Os = Vs + T * kPitch<D>;
@@ -287,13 +350,21 @@ __global__ void __launch_bounds__(kThreads<D, T>) window_dkdv_f32_kernel(BwdArgs
   float *Ps = Qn + TB * kPitch<D>, *Ms = Ps + T * kPitchP, *Mn = Ms + 2 * TB;  // M and delta of them
   const int N = a.N, Nk = a.win.Nk;
   if (cta_head() >= int64_t(a.Z) * a.win.Hk) return;
-  const WindowUnit u = window_unit<T, TB>(a.split, a.win, a.Z, N, unsigned(cta_head() * gridDim.x + blockIdx.x));
+  WindowUnit u = window_unit<T, TB>(a.split, a.win, a.Z, N, unsigned(cta_head() * gridDim.x + blockIdx.x));
   const int k0 = T * u.kt;
   const int64_t head = u.head;
   const int zi = int(head / a.win.Hk), hk = int(head % a.win.Hk);
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  load_rows<D, T, TH>(Ks, static_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h, a.sk, k0, Nk);
-  load_rows<D, T, TH>(Vs, static_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h, a.sv, k0, Nk);
+  int len = Nk;
+  bool outside;
+  if constexpr (ROWS) {
+    len = held_keys(a.lengths, zi, Nk, &outside);
+    if (k0 >= len) u.n = 0;
+  }
+  if (!ROWS || u.n > 0) {
+    load_rows<D, T, TH>(Ks, static_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h, a.sk, k0, len);
+    load_rows<D, T, TH>(Vs, static_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h, a.sv, k0, len);
+  }
   float dk[R][D / 16] = {}, dv[R][D / 16] = {};
   auto rows_of = [&](const void* x, const Strides4& st, int i, float* to) {  // the tile of pair i
     const int hi = hk * a.win.group + i / u.nb, r0 = (u.lo + i % u.nb) * TB;
@@ -319,7 +390,7 @@ __global__ void __launch_bounds__(kThreads<D, T>) window_dkdv_f32_kernel(BwdArgs
     __syncthreads();  // Q and dO are here, and Q's last tile has been read
     if (i + 1 < end) load_q(i + 1, Qn, Mn);
     float p[R][4], ds[R][4];
-    p_ds<D, R, true>(a, Ks, Qs, Vs, Os, ty, tx, k0, r0, Ms, Ms + TB, p, ds);
+    p_ds<D, R, true, ROWS>(a, Ks, Qs, Vs, Os, ty, tx, k0, r0, len, Ms, Ms + TB, p, ds);
     auto put = [&](const float(*x)[4]) {  // a row is written and read by the 16 threads of one half warp
       __syncwarp();
 #pragma unroll
@@ -345,6 +416,10 @@ __global__ void __launch_bounds__(kThreads<D, T>) window_dkdv_f32_kernel(BwdArgs
   for (int i = 0; i < R; ++i) {
     const int key = k0 + R * ty + i;
     if (key >= Nk) continue;
+    if (ROWS && key >= len) {  // zeros, whatever dO and Q hold
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) dk[i][e] = dv[i][e] = 0.f;
+    }
     if (u.slot >= 0) {
       const int64_t slot = head * a.split.slots((Nk + T - 1) / T) + u.slot;
       float* part = a.part + (slot * 2 * T + R * ty + i) * D + D / 16 * tx;
@@ -398,23 +473,24 @@ cudaError_t launch(Kernel kernel, int tiles, long long heads, int threads, int f
 template <int D, int T>
 cudaError_t fwd_impl(const float* q, const float* k, const float* v, const Strides4& sq, const Strides4& sk,
                      const Strides4& sv, const FwdArgs& a, cudaStream_t s) {
-  return launch(window_fwd_f32_kernel<D, T>, (a.N + T - 1) / T, (long long)a.Z * a.H, kThreads<D, T>,
+  return launch(window_fwd_f32_kernel<D, T, false>, (a.N + T - 1) / T, (long long)a.Z * a.H, kThreads<D, T>,
                 (T + 2 * TB) * kPitch<D> + T * kPitchP, s, q, k, v, sq, sk, sv, a);
 }
 
-template <int D, int T>
-cudaError_t dkdv_impl(const BwdArgs& a, cudaStream_t s) {
+template <int D, int T, bool ROWS>
+cudaError_t dkdv_impl(const Bwd<ROWS>& a, cudaStream_t s) {
   const int key_tiles = (a.win.Nk + T - 1) / T;
-  const cudaError_t e = launch(window_dkdv_f32_kernel<D, T>, a.split.per_head(key_tiles), (long long)a.Z * a.win.Hk, kThreads<D, T>,
+  const cudaError_t e = launch(window_dkdv_f32_kernel<D, T, ROWS>, a.split.per_head(key_tiles), (long long)a.Z * a.win.Hk, kThreads<D, T>,
                                (2 * T + 3 * TB) * kPitch<D> + T * kPitchP + 4 * TB, s, a);
   if (e != cudaSuccess || a.split.slots(key_tiles) == 0) return e;
   const int64_t values = int64_t(a.Z) * a.win.Hk * (a.split.units > 1 ? key_tiles : a.split.tiles) * 2 * T * D;
-  window_join_f32_kernel<<<unsigned((values + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, s>>>(a, T, D);
+  const BwdArgs& join = a;
+  window_join_f32_kernel<<<unsigned((values + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, s>>>(join, T, D);
   return cudaGetLastError();
 }
-template <int D, int T>
-cudaError_t dq_impl(const BwdArgs& a, cudaStream_t s) {
-  return launch(window_dq_f32_kernel<D, T>, (a.N + T - 1) / T, (long long)a.Z * a.H, kThreads<D, T>,
+template <int D, int T, bool ROWS>
+cudaError_t dq_impl(const Bwd<ROWS>& a, cudaStream_t s) {
+  return launch(window_dq_f32_kernel<D, T, ROWS>, (a.N + T - 1) / T, (long long)a.Z * a.H, kThreads<D, T>,
                 (2 * T + 3 * TB) * kPitch<D> + T * kPitchP + 2 * T, s, a);
 }
 
@@ -425,13 +501,24 @@ cudaError_t fwd_tiles(const float* q, const float* k, const float* v, const Stri
     if (window_f32_tile(D, (long long)a.Z * a.H, a.N) == 64) return fwd_impl<D, 64>(q, k, v, sq, sk, sv, a, s);
   return fwd_impl<D, 32>(q, k, v, sq, sk, sv, a, s);
 }
+template <int D, int T>
+cudaError_t rows_impl(const float* k, const float* v, const Strides4& sk, const Strides4& sv, const RowsFwdArgs& a, cudaStream_t s) {
+  return launch(window_fwd_f32_kernel<D, T, true>, (a.N + T - 1) / T * a.rows.nsplit, (long long)a.Z * a.H, kThreads<D, T>,
+                (T + 2 * TB) * kPitch<D> + T * kPitchP, s, static_cast<const float*>(nullptr), k, v, Strides4{}, sk, sv, a);
+}
 template <int D>
-cudaError_t bwd_tiles(const BwdArgs& a, cudaStream_t s) {
-  auto of_keys = dkdv_impl<D, 32>;
-  auto of_queries = dq_impl<D, 32>;
+cudaError_t rows_tiles(const float* k, const float* v, const Strides4& sk, const Strides4& sv, const RowsFwdArgs& a, cudaStream_t s) {
+  if constexpr (D > 16)
+    if (window_f32_tile(D, (long long)a.Z * a.H, a.N) == 64) return rows_impl<D, 64>(k, v, sk, sv, a, s);
+  return rows_impl<D, 32>(k, v, sk, sv, a, s);
+}
+template <int D, bool ROWS>
+cudaError_t bwd_tiles(const Bwd<ROWS>& a, cudaStream_t s) {
+  auto of_keys = dkdv_impl<D, 32, ROWS>;
+  auto of_queries = dq_impl<D, 32, ROWS>;
   if constexpr (D > 16) {
-    if (window_f32_tile(D, (long long)a.Z * a.win.Hk, a.win.Nk) == 64) of_keys = dkdv_impl<D, 64>;
-    if (window_f32_tile(D, (long long)a.Z * a.H, a.N) == 64) of_queries = dq_impl<D, 64>;
+    if (window_f32_tile(D, (long long)a.Z * a.win.Hk, a.win.Nk) == 64) of_keys = dkdv_impl<D, 64, ROWS>;
+    if (window_f32_tile(D, (long long)a.Z * a.H, a.N) == 64) of_queries = dq_impl<D, 64, ROWS>;
   }
   const cudaError_t e = of_keys(a, s);
   return e != cudaSuccess ? e : of_queries(a, s);
@@ -457,10 +544,31 @@ cudaError_t launch_window_fwd_f32(int D, const void* q, const void* k, const voi
 
 cudaError_t launch_window_bwd_f32(int D, const BwdArgs& a, cudaStream_t s) {
   switch (D) {
-    case 16: return bwd_tiles<16>(a, s);
-    case 32: return bwd_tiles<32>(a, s);
-    case 64: return bwd_tiles<64>(a, s);
-    case 128: return bwd_tiles<128>(a, s);
+    case 16: return bwd_tiles<16, false>(a, s);
+    case 32: return bwd_tiles<32, false>(a, s);
+    case 64: return bwd_tiles<64, false>(a, s);
+    case 128: return bwd_tiles<128, false>(a, s);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+cudaError_t launch_rows_f32(int D, const void* k, const void* v, Strides4 sk, Strides4 sv, const RowsFwdArgs& a, cudaStream_t s) {
+  const float *kf = static_cast<const float*>(k), *vf = static_cast<const float*>(v);
+  switch (D) {
+    case 16: return rows_tiles<16>(kf, vf, sk, sv, a, s);
+    case 32: return rows_tiles<32>(kf, vf, sk, sv, a, s);
+    case 64: return rows_tiles<64>(kf, vf, sk, sv, a, s);
+    case 128: return rows_tiles<128>(kf, vf, sk, sv, a, s);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+cudaError_t launch_rows_bwd_f32(int D, const RowsBwdArgs& a, cudaStream_t s) {
+  switch (D) {
+    case 16: return bwd_tiles<16, true>(a, s);
+    case 32: return bwd_tiles<32, true>(a, s);
+    case 64: return bwd_tiles<64, true>(a, s);
+    case 128: return bwd_tiles<128, true>(a, s);
     default: return cudaErrorInvalidValue;
   }
 }

@@ -1,5 +1,6 @@
 """Attention of one new token of each sequence over a cache: ``decode_attention`` over keys and values in the
-queries' dtype, ``Int4Cache`` holding them in 4 bits.
+queries' dtype, ``prefix_decode_attention`` where several sequences share a prompt's, ``Int4Cache`` holding them in 4
+bits.
 
 The single-token form of ``tattn.window_attention``, for generation: no gradients (tensors that need them are refused
 where gradients are recorded), nothing read from the device (the lengths stay there), so a step can be captured in a
@@ -29,6 +30,22 @@ def decode_attention(
     their rows must be contiguous and 16-byte aligned.
     """
     return _lib.torch_ext().decode_attention(q, k, v, lengths, window, sinks, sm_scale)
+
+
+def prefix_decode_attention(
+    q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+    lengths: torch.Tensor, prefix_lengths: torch.Tensor | None = None, sm_scale: float | None = None,
+) -> torch.Tensor:  # fmt: skip
+    """``decode_attention`` for several samples of each prompt, which share the prompt's keys and values.
+
+    prefix_k and prefix_v are [prompts, kv_heads, prefix capacity, dim], held once for each prompt: the first
+    prefix_lengths[p] tokens of prompt p (int32 [prompts], on the device; None: all). q is [batch, heads, 1, dim] and k, v
+    are [batch, kv_heads, capacity, dim] for a batch of prompts * samples sequences, those of a prompt one after another;
+    of sequence b's own tokens, which stand behind its prompt, the first lengths[b] are held (int32 [batch], the query's
+    own as the last). The query sees the whole prompt and all of its sequence's tokens; where none are held the result is
+    zeros. Lengths outside their ranges, rows past a length and the caches' layout are as for ``decode_attention``.
+    """
+    return _lib.torch_ext().prefix_decode_attention(q, prefix_k, prefix_v, k, v, lengths, prefix_lengths, sm_scale)
 
 
 class Int4Cache:
