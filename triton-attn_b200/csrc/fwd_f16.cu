@@ -203,6 +203,15 @@ __device__ __forceinline__ void clear_value_rows(uint32_t block, int from, int t
   fence_proxy_async_smem();
 }
 
+// The same for entry j of the CTA's list, the one whose first *lim rows are the sequence's.
+template <typename C>
+__device__ __forceinline__ bool clear_behind(int j, uint32_t sV, int t, uint64_t* bar_v_full, volatile int* lim, const CtaAbort& ab) {
+  const int st = j % C::NS;
+  if (!warp_wait(&bar_v_full[st], (j / C::NS) & 1, ab)) return false;
+  clear_value_rows<C>(sV + st * C::KTILE, *lim, t);
+  return true;
+}
+
 // kMaskWindow: scores of the columns that a row does not see become -infinity: it sees the columns in
 // [first, lim) and in [0, min(sink, lim)). A bit a column, so that each is one test of a constant bit: written
 // as comparisons it compiled to branches, and a block that needed the mask took some 10 us. The pass comes
@@ -390,6 +399,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
     list.jump = int(blocks * split / args.rows.nsplit);
     list.n = int(blocks * (split + 1) / args.rows.nsplit) - list.jump;
     list.n0 = list.n;
+    if (threadIdx.x == 0) *reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 12) = len - (list.jump + list.n - 1) * BN;
   }
   const int n_0 = WINDOW || ROWS ? list.n0 : row0_0 >= N ? 0 : (CAUSAL ? min((row0_0 + C::BM + BN - 1) / BN, NB) : NB);
   const int n_1 = TILES == 1 || row0_1 >= N ? 0
@@ -551,11 +561,32 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
     const uint64_t scale2 = f2(scale, scale);
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
+    // kMaskRows: the block that the sequence's keys fill in part, if one of this CTA's is; how far stands in shared
+    // memory (two registers fewer through the loop).
+    const int partial = ROWS && n > 0 && (n + list.jump) * BN > len ? n - 1 : n;
+    volatile int* lim_slot = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 12);
     if constexpr (ROWS) {
       if (n > 0) load_row_tile<C, D>(args, sQ + i * C::QTILE, zi, hi, row - t, t);
       mbar_arrive(bar_q);
     }
-    for (int j = 0; j < n; ++j) {
+    // kMaskRows: a warp without rows computes nothing (what stands in its TMEM lanes reaches no other rows), but
+    // takes part in the barriers. It arrives for a block only once the last block's P V is done, as the others do, so
+    // that its arrivals count for their own phase. (A loop of its own: a branch in the others' costs them 4 %.)
+    int start = 0;
+    if (ROWS && row - lane >= N) {
+      for (; start < n; ++start) {
+        if (start == partial && !clear_behind<C>(start, sV, t, bar_v_full, lim_slot, ab)) { ok = false; break; }
+        if (!warp_wait(&bar_s_full[i], start & 1, ab)) { ok = false; break; }
+        if (!C::ALIAS_P) mbar_arrive(&bar_s_free[i]);
+        if (start > 0 && !warp_wait(&bar_o_done[i], (start - 1) & 1, ab)) { ok = false; break; }
+        if (TILES == 2) mbar_arrive(&bar_exp_done[i]);
+        mbar_arrive(&bar_p_full[i]);
+      }
+      if (!ok) start = n;
+    }
+    for (int j = start; j < n; ++j) {
+      // (behind the wait for S the registers are full)
+      if (ROWS && j == partial && !clear_behind<C>(j, sV, t, bar_v_full, lim_slot, ab)) { ok = false; break; }
       if (!warp_wait(&bar_s_full[i], j & 1, ab)) { ok = false; break; }
       tc_fence_after();
       uint32_t s[BN];
@@ -569,17 +600,19 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
       // (causal) in every block that reaches past the tile's first row (the last BM / BN blocks).
       // kMaskWindow: those are hidden beforehand, in every block that the diagonal or the lower edge of some
       // row's window cuts.
-      // kMaskRows: those past the sequence's keys, in its last block.
-      const int col0 = (WINDOW ? list.block(j) : ROWS ? j + list.jump : j) * BN;
-      if (ROWS && col0 + BN > len) hide_columns<BN>(s, len - col0, 0, 0);
+      // kMaskRows: those past the sequence's keys, in its last block (beforehand, too, in CTAs of one tile).
+      const int col0 = (WINDOW ? list.block(j) : j) * BN;
+      if (ROWS && TILES == 1 && j == partial) hide_columns<BN>(s, *lim_slot, 0, 0);
       if (WINDOW) {
         const int pos = row + args.win.off, tile = pos - t;  // positions of this row and of the tile's first
         if (col0 + BN - 1 > tile || (col0 <= tile + C::BM - 1 - args.win.window && col0 + BN > args.win.sinks))
           hide_columns<BN>(s, min(args.win.Nk, pos + 1) - col0, pos + 1 - args.win.window - col0,
                            args.win.sinks - col0);
       }
-      const bool last = !WINDOW && !ROWS && ((col0 + BN > N) || (CAUSAL && col0 + BN - 1 > row - t));
+      const bool last = ROWS ? TILES == 2 && j == partial
+                             : !WINDOW && ((col0 + BN > N) || (CAUSAL && col0 + BN - 1 > row - t));
       int lim = N - col0;
+      if (ROWS && last) lim = *lim_slot;
       if (CAUSAL) lim = min(lim, row - col0 + 1);
       const float m_cand = (last ? row_max<BN, true>(s, lim) : row_max<BN, false>(s, lim)) * scale;
       float alpha = 1.f;
@@ -636,11 +669,6 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
         }
       }
       tmem_store_cols<BN / 2>(tP, p);
-      if (ROWS && col0 + BN > len) {
-        const int st = j % C::NS;
-        if (!warp_wait(&bar_v_full[st], (j / C::NS) & 1, ab)) { ok = false; break; }
-        clear_value_rows<C>(sV + st * C::KTILE, len - col0, t);
-      }
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&bar_p_full[i]);
@@ -753,8 +781,10 @@ cudaError_t launch_variant(int v, const CUtensorMap& tq, const CUtensorMap& tk, 
 
 template <int D>
 cudaError_t launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const RowsFwdArgs& a, cudaStream_t s) {
-  if (rows_f16_tiles(D, a.N) == 1) return launch_impl<D, kMaskRows, rows_f16_block(D, 1), 2, 1>(tk, tk, tv, a, s);
-  return launch_impl<D, kMaskRows, rows_f16_block(D, 2), kFwdTiles[tile_default(0, D, false)].stages>(tk, tk, tv, a, s);
+  if constexpr (rows_f16_tiles(D, 129) == 2)
+    if (rows_f16_tiles(D, a.N) == 2)
+      return launch_impl<D, kMaskRows, rows_f16_block(D, 2), kFwdTiles[tile_default(0, D, false)].stages>(tk, tk, tv, a, s);
+  return launch_impl<D, kMaskRows, rows_f16_block(D, 1), 2, 1>(tk, tk, tv, a, s);
 }
 
 }  // namespace
