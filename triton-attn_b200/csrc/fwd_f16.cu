@@ -175,15 +175,24 @@ __device__ __forceinline__ Blocks window_blocks(int row0, int N, const WindowArg
 template <typename C, int D>
 __device__ __forceinline__ void load_row_tile(const RowsFwdArgs& a, uint32_t dst, int zi, int hi, int row0, int t) {
   constexpr int U = D / 8, CU = C::SWB / 16;  // 16-byte units of a row, of its part in a chunk
+  constexpr int G = U < 8 ? U : 8;  // loads in flight
   const __half* q = static_cast<const __half*>(a.rows.q);
 #pragma unroll 1
-  for (int i = 0; i < U; ++i) {
-    const int e = i * 128 + t, row = e / U, unit = e % U, r = row0 + row;
-    uint4 x = make_uint4(0u, 0u, 0u, 0u);
-    if (r < a.N)
-      x = __ldg(reinterpret_cast<const uint4*>(row_of(q, a.rows.sq, a.rows.inner, zi, hi, r)) + unit);
-    const uint32_t at = dst + unit / CU * C::QCHUNK + swizzle_offset<C::SWB>(uint32_t(row * C::SWB + unit % CU * 16));
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+  for (int i0 = 0; i0 < U; i0 += G) {
+    uint4 x[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int e = (i0 + i) * 128 + t, r = row0 + e / U;
+      x[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < a.N) x[i] = __ldg(reinterpret_cast<const uint4*>(row_of(q, a.rows.sq, a.rows.inner, zi, hi, r)) + e % U);
+    }
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int e = (i0 + i) * 128 + t, row = e / U, unit = e % U;
+      const uint32_t at = dst + unit / CU * C::QCHUNK + swizzle_offset<C::SWB>(uint32_t(row * C::SWB + unit % CU * 16));
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[i].x), "r"(x[i].y), "r"(x[i].z), "r"(x[i].w)
+                   : "memory");
+    }
   }
   fence_proxy_async_smem();
 }
