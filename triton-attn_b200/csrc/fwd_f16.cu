@@ -171,8 +171,8 @@ __device__ __forceinline__ Blocks window_blocks(int row0, int N, const WindowArg
 }
 
 // kMaskRows: rows [row0, row0 + 128) of the head's matrix into a query tile's shared memory, by the 128 threads of a
-// warpgroup (t: the thread's index in it); rows past N are zeros.
-template <typename C, int D>
+// warpgroup (t: the thread's index in it); rows past N are zeros. COPIES: the first 128 / COPIES of them so many times.
+template <typename C, int D, int COPIES>
 __device__ __forceinline__ void load_row_tile(const RowsFwdArgs& a, uint32_t dst, int zi, int hi, int row0, int t) {
   constexpr int U = D / 8, CU = C::SWB / 16;  // 16-byte units of a row, of its part in a chunk
   constexpr int G = U < 8 ? U : 8;  // loads in flight
@@ -182,7 +182,7 @@ __device__ __forceinline__ void load_row_tile(const RowsFwdArgs& a, uint32_t dst
     uint4 x[G];
 #pragma unroll
     for (int i = 0; i < G; ++i) {
-      const int e = (i0 + i) * 128 + t, r = row0 + e / U;
+      const int e = (i0 + i) * 128 + t, r = row0 + e / U % (128 / COPIES);
       x[i] = make_uint4(0u, 0u, 0u, 0u);
       if (r < a.N) x[i] = __ldg(reinterpret_cast<const uint4*>(row_of(q, a.rows.sq, a.rows.inner, zi, hi, r)) + e % U);
     }
@@ -332,15 +332,83 @@ __device__ __forceinline__ void store_part(const RowsFwdArgs& a, int bh, int row
   if (row < a.N) reinterpret_cast<float2*>(a.rows.part_ml)[at] = m == -INFINITY ? make_float2(-FLT_MAX, 0.f) : make_float2(m, l);
 }
 
+// kMaskRows with COPIES: joins the copies of each row, which took a share of every block's keys each, through shared
+// memory, and finishes the row, or its part. Called by the warpgroup's 128 threads (t), whether their waits ran out or not.
+template <typename C, int D, int COPIES>
+__device__ __forceinline__ void finish_copies(const RowsFwdArgs& a, float* smem, int bh, int nct, int t, uint32_t tO, float m,
+                                              float l) {
+  constexpr int ROWS = 128 / COPIES, PITCH = D + 4;
+  static_assert((128 * PITCH + 256) * 4 <= C::OFF_BAR, "the tiles' memory holds the rows");
+  const int row = t % ROWS, copy = t / ROWS;
+  float2* ml = reinterpret_cast<float2*>(smem + 128 * PITCH);
+  ml[t] = make_float2(m, l);
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int c = 0; c < COPIES; ++c) top = max_or_nan(top, ml[c * ROWS + row].x);
+  const float use = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int c = 0; c < COPIES; ++c) {
+    const float2 x = ml[c * ROWS + row];
+    if (x.x != -INFINITY) sum = fmaf(ex2_approx(x.x - use), x.y, sum);
+  }
+  const float f = m == -INFINITY ? 0.f : ex2_approx(m - use);
+#pragma unroll
+  for (int c0 = 0; c0 < D; c0 += 32) {
+    constexpr int W = D < 32 ? D : 32;
+    uint32_t o[W];
+    tmem_load_cols<W>(tO + c0, o);
+    tmem_wait_ld();
+    reg_fence<W>(o);
+#pragma unroll
+    for (int c = 0; c < W; c += 4)
+      *reinterpret_cast<float4*>(smem + t * PITCH + c0 + c) =
+          make_float4(__uint_as_float(o[c]) * f, __uint_as_float(o[c + 1]) * f, __uint_as_float(o[c + 2]) * f,
+                      __uint_as_float(o[c + 3]) * f);
+  }
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  if (row >= a.N) return;
+  const int64_t index = int64_t(bh) * a.N + row;
+  const int64_t part = index * a.rows.nsplit + (int(blockIdx.x) / nct - bh * a.rows.nsplit);
+  __half* out = a.rows.part ? nullptr : row_of(static_cast<__half*>(a.o), a.rows.so, a.rows.inner, bh / a.H, bh % a.H, row);
+  const float inv_l = top - top == 0.f ? 1.f / sum : NAN;
+#pragma unroll
+  for (int c = 0; c < D / COPIES; c += 4) {
+    const int col = copy * (D / COPIES) + c;
+    float4 x = *reinterpret_cast<const float4*>(smem + row * PITCH + col);
+#pragma unroll
+    for (int i = 1; i < COPIES; ++i) {
+      const float4 y = *reinterpret_cast<const float4*>(smem + (i * ROWS + row) * PITCH + col);
+      x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+    }
+    if (a.rows.part) {
+      *reinterpret_cast<float4*>(a.rows.part + part * D + col) = x;
+      continue;
+    }
+    const uint32_t o[4] = {__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(x.z), __float_as_uint(x.w)};
+    const uint2 h = make_uint2(pack_half2(x.x * inv_l, x.y * inv_l), pack_half2(x.z * inv_l, x.w * inv_l));
+    *reinterpret_cast<uint2*>(out + col) = h;
+    if (a.o_rest != nullptr)
+      *reinterpret_cast<uint32_t*>(a.o_rest + index * D + col) = rest_of(o, h.x, inv_l) | (rest_of(o + 2, h.y, inv_l) << 16);
+  }
+  if (copy > 0) return;
+  if (a.rows.part)  // (as store_part)
+    reinterpret_cast<float2*>(a.rows.part_ml)[part] = top == -INFINITY ? make_float2(-FLT_MAX, 0.f) : make_float2(top, sum);
+  else if (a.m != nullptr)
+    a.m[index] = top + log2f(sum);
+}
+
 template <int MASK>
 using Args = std::conditional_t<MASK == kMaskRows, RowsFwdArgs, FwdArgs>;
 
-template <int D, int MASK, int BN_, int NS_, int TILES>
+template <int D, int MASK, int BN_, int NS_, int TILES, int COPIES>
 __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
     fwd_f16_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const Args<MASK> args) {
   using C = FwdCfg<D, BN_, NS_, TILES>;
   constexpr int BN = C::BN;
+  constexpr int BC = BN / COPIES;  // columns of S that a softmax thread takes
+  static_assert(COPIES == 1 || (MASK == kMaskRows && TILES == 1 && !C::ALIAS_P && BC >= 32), "copies of rows");
   constexpr int kTmaWarp = 4 * TILES, kMmaWarp = kTmaWarp + 1, kAllocWarp = kTmaWarp + 3;  // kMmaWarp + i: tile i
   constexpr bool CAUSAL = MASK == kMaskCausal, WINDOW = MASK == kMaskWindow, ROWS = MASK == kMaskRows;
   extern __shared__ uint8_t smem_raw[];
@@ -560,8 +628,9 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs<TILES>));
     const int i = warp / 4;
     const int t = threadIdx.x % 128;
-    const int row = (i ? row0_1 : row0_0) + t;
+    const int row = (i ? row0_1 : row0_0) + (COPIES > 1 ? t % (128 / COPIES) : t);
     const int n = i ? n_1 : n_0;
+    const int col = COPIES > 1 ? t / (128 / COPIES) * BC : 0;  // the thread's first column of a block
     const uint32_t lane_off = uint32_t((warp % 4) * 32) << 16;
     const uint32_t tS = tmem + lane_off + C::TM_S + i * BN;
     const uint32_t tP = tmem + lane_off + C::TM_P + i * C::P_STRIDE;
@@ -575,33 +644,24 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
     const int partial = ROWS && n > 0 && (n + list.jump) * BN > len ? n - 1 : n;
     volatile int* lim_slot = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 12);
     if constexpr (ROWS) {
-      if (n > 0) load_row_tile<C, D>(args, sQ + i * C::QTILE, zi, hi, row - t, t);
+      if (n > 0) load_row_tile<C, D, COPIES>(args, sQ + i * C::QTILE, zi, hi, COPIES > 1 ? 0 : row - t, t);
       mbar_arrive(bar_q);
-    }
-    // kMaskRows: a warp without rows computes nothing (what stands in its TMEM lanes reaches no other rows), but
-    // takes part in the barriers. It arrives for a block only once the last block's P V is done, as the others do, so
-    // that its arrivals count for their own phase. (A loop of its own: a branch in the others' costs them 4 %.)
-    int start = 0;
-    if (ROWS && row - lane >= N) {
-      for (; start < n; ++start) {
-        if (start == partial && !clear_behind<C>(start, sV, t, bar_v_full, lim_slot, ab)) { ok = false; break; }
-        if (!warp_wait(&bar_s_full[i], start & 1, ab)) { ok = false; break; }
-        if (!C::ALIAS_P) mbar_arrive(&bar_s_free[i]);
-        if (start > 0 && !warp_wait(&bar_o_done[i], (start - 1) & 1, ab)) { ok = false; break; }
-        if (TILES == 2) mbar_arrive(&bar_exp_done[i]);
-        mbar_arrive(&bar_p_full[i]);
+      if (COPIES > 1 && n > 0) {  // the other copies' columns of P are zeros throughout
+        uint32_t zero[BN / 2];
+#pragma unroll
+        for (int c = 0; c < BN / 2; ++c) zero[c] = 0u;
+        tmem_store_cols<BN / 2>(tP, zero);
       }
-      if (!ok) start = n;
     }
-    for (int j = start; j < n; ++j) {
+    for (int j = 0; j < n; ++j) {
       // (behind the wait for S the registers are full)
       if (ROWS && j == partial && !clear_behind<C>(j, sV, t, bar_v_full, lim_slot, ab)) { ok = false; break; }
       if (!warp_wait(&bar_s_full[i], j & 1, ab)) { ok = false; break; }
       tc_fence_after();
-      uint32_t s[BN];
-      tmem_load_cols<BN>(tS, s);
+      uint32_t s[BC];
+      tmem_load_cols<BC>(tS + col, s);
       tmem_wait_ld();
-      reg_fence<BN>(s);
+      reg_fence<BC>(s);
       tc_fence_before();
       if (!C::ALIAS_P) mbar_arrive(&bar_s_free[i]);  // the tensor core may now write S(j+1) of this tile
 
@@ -611,7 +671,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
       // row's window cuts.
       // kMaskRows: those past the sequence's keys, in its last block (beforehand, too, in CTAs of one tile).
       const int col0 = (WINDOW ? list.block(j) : j) * BN;
-      if (ROWS && TILES == 1 && j == partial) hide_columns<BN>(s, *lim_slot, 0, 0);
+      if (ROWS && TILES == 1 && j == partial) hide_columns<BC>(s, *lim_slot - col, 0, 0);
       if (WINDOW) {
         const int pos = row + args.win.off, tile = pos - t;  // positions of this row and of the tile's first
         if (col0 + BN - 1 > tile || (col0 <= tile + C::BM - 1 - args.win.window && col0 + BN > args.win.sinks))
@@ -623,7 +683,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
       int lim = N - col0;
       if (ROWS && last) lim = *lim_slot;
       if (CAUSAL) lim = min(lim, row - col0 + 1);
-      const float m_cand = (last ? row_max<BN, true>(s, lim) : row_max<BN, false>(s, lim)) * scale;
+      const float m_cand = (last ? row_max<BC, true>(s, lim) : row_max<BC, false>(s, lim)) * scale;
       float alpha = 1.f;
       bool need = false;
       if (j == 0) {
@@ -648,15 +708,15 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
       // With 128-key blocks the turn is handed over after seven eighths of the columns, so the other
       // tile's pass starts while this one finishes and the exponent unit does not idle across the
       // hand-off (measured at BN = 128: 7/8 best, 3/4 within 1%, 1/2 8% slower; slower at BN = 64).
-      constexpr int kSplit = BN == 128 && TILES == 2 ? BN * 7 / 8 : BN;
-      uint32_t p[BN / 2];
+      constexpr int kSplit = BN == 128 && TILES == 2 ? BN * 7 / 8 : BC;
+      uint32_t p[BC / 2];
       const float m_use = (WINDOW || ROWS) && m_run == -INFINITY ? 0.f : m_run;  // nothing seen yet: every p is 0
       const uint64_t negm2 = f2(-m_use, -m_use);
       l_run += last ? exp_cols<0, kSplit, true>(s, p, scale2, negm2, lim) : exp_cols<0, kSplit, false>(s, p, scale2, negm2, lim);
       if (TILES == 2) mbar_arrive(&bar_exp_done[i]);
-      if constexpr (kSplit < BN)
-        l_run += last ? exp_cols<kSplit, BN, true>(s, p, scale2, negm2, lim)
-                      : exp_cols<kSplit, BN, false>(s, p, scale2, negm2, lim);
+      if constexpr (kSplit < BC)
+        l_run += last ? exp_cols<kSplit, BC, true>(s, p, scale2, negm2, lim)
+                      : exp_cols<kSplit, BC, false>(s, p, scale2, negm2, lim);
 
       // PV(j-1) must have landed before P and O of this tile are touched again (ALIAS_P: it has, since
       // S(j) was issued after it and has completed).
@@ -677,13 +737,20 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
           tmem_store_cols<W>(tO + c0, o);
         }
       }
-      tmem_store_cols<BN / 2>(tP, p);
+      tmem_store_cols<BC / 2>(tP + col / 2, p);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&bar_p_full[i]);
     }
 
-    if (ok && n > 0 && warp_wait(&bar_o_done[i], (n - 1) & 1, ab)) {
+    if constexpr (COPIES > 1) {
+      if (n > 0) {
+        if (ok) warp_wait(&bar_o_done[i], (n - 1) & 1, ab);
+        tc_fence_after();
+        finish_copies<C, D, COPIES>(args, reinterpret_cast<float*>(smem), *reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8),
+                                    nct, t, tO, m_run, l_run);
+      }
+    } else if (ok && n > 0 && warp_wait(&bar_o_done[i], (n - 1) & 1, ab)) {
       tc_fence_after();
       // No result where the largest score is NaN, or infinite of either sign (l itself misses some of that).
       const float inv_l = m_run - m_run == 0.f ? 1.f / l_run : NAN;
@@ -732,7 +799,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
       }
     }
     if constexpr (ROWS)
-      if (n == 0 && row < N) no_keys<D>(args, *reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8), row, nct);
+      if (n == 0 && row < N && col == 0) no_keys<D>(args, *reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8), row, nct);
   }
 
   tc_fence_before();
@@ -743,11 +810,11 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
   }
 }
 
-template <int D, int MASK, int BN, int NS, int TILES = 2>
+template <int D, int MASK, int BN, int NS, int TILES = 2, int COPIES = 1>
 cudaError_t launch_impl(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const Args<MASK>& a,
                         cudaStream_t s) {
   using C = FwdCfg<D, BN, NS, TILES>;
-  auto kern = fwd_f16_kernel<D, MASK, BN, NS, TILES>;
+  auto kern = fwd_f16_kernel<D, MASK, BN, NS, TILES, COPIES>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
   if (e != cudaSuccess) return e;
   const int nct = (a.N + TILES * C::BM - 1) / (TILES * C::BM);
@@ -793,7 +860,12 @@ cudaError_t launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const Rows
   if constexpr (rows_f16_tiles(D, 129) == 2)
     if (rows_f16_tiles(D, a.N) == 2)
       return launch_impl<D, kMaskRows, rows_f16_block(D, 2), kFwdTiles[tile_default(0, D, false)].stages>(tk, tk, tv, a, s);
-  return launch_impl<D, kMaskRows, rows_f16_block(D, 1), 2, 1>(tk, tk, tv, a, s);
+  // Copies of few rows share a block's exponentials, the longest part of its way, among the tile's threads.
+  constexpr int BN = rows_f16_block(D, 1);
+  if constexpr (BN >= 128)
+    if (a.N <= 32) return launch_impl<D, kMaskRows, BN, 2, 1, 4>(tk, tk, tv, a, s);
+  if (a.N <= 64) return launch_impl<D, kMaskRows, BN, 2, 1, 2>(tk, tk, tv, a, s);
+  return launch_impl<D, kMaskRows, BN, 2, 1>(tk, tk, tv, a, s);
 }
 
 }  // namespace
