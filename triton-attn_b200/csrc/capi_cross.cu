@@ -50,7 +50,7 @@ int row_parts(int D, int dtype, int64_t heads, int rows, int Nk) {
     const int tile = window_f32_tile(D, heads, rows);
     return rows_splits(heads * ((rows + tile - 1) / tile), (int64_t(Nk) + kWindowF32Block - 1) / kWindowF32Block, 4 * sms, 1, 2);
   }
-  const int tiles = rows_f16_tiles(D, rows), block = rows_f16_block(D, tiles);
+  const int tiles = rows_f16_tiles(D, rows), block = rows_f16_block(D, rows);
   return rows_splits(heads * ((rows + 128 * tiles - 1) / (128 * tiles)), (int64_t(Nk) + block - 1) / block,
                      int64_t(sms) * (tiles == 1 ? 2 : 1), 4, 4);
 }
@@ -71,7 +71,7 @@ int run_rows(int D, int dtype, const void* k, const void* v, const int64_t* sk, 
   a.qk_scale = positive(sm_scale);
   a.negate_s = sm_scale < 0.f ? 1 : 0;
   if (!layout_ok(k, tk, a.Z, a.H, Nk, D) || !layout_ok(v, tv, a.Z, a.H, Nk, D)) return TATTN_ERR_LAYOUT;
-  const int block = rows_f16_block(D, rows_f16_tiles(D, a.N));
+  const int block = rows_f16_block(D, a.N);
   CUtensorMap mk, mv;
   if ((rc = encode_f16(&mk, k, tk, a.Z, a.H, Nk, D, block)) != TATTN_OK) return rc;
   if ((rc = encode_f16(&mv, v, tv, a.Z, a.H, Nk, D, block)) != TATTN_OK) return rc;

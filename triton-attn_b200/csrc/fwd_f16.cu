@@ -230,10 +230,10 @@ template <int BN>
 __device__ __forceinline__ void hide_columns(uint32_t* s, int lim, int first, int sink) {
   auto below = [](int n) { return n >= 32 ? ~0u : (1u << max(n, 0)) - 1u; };  // the lowest n bits
 #pragma unroll
-  for (int w = 0; w < BN / 32; ++w) {
+  for (int w = 0; w < (BN + 31) / 32; ++w) {
     const uint32_t bits = below(lim - 32 * w) & (~below(first - 32 * w) | below(sink - 32 * w));
 #pragma unroll
-    for (int c = 0; c < 32; ++c) s[32 * w + c] = (bits & (1u << c)) != 0u ? s[32 * w + c] : 0xff800000u;
+    for (int c = 0; c < 32 && 32 * w + c < BN; ++c) s[32 * w + c] = (bits & (1u << c)) != 0u ? s[32 * w + c] : 0xff800000u;
   }
 }
 
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
   using C = FwdCfg<D, BN_, NS_, TILES>;
   constexpr int BN = C::BN;
   constexpr int BC = BN / COPIES;  // columns of S that a softmax thread takes
-  static_assert(COPIES == 1 || (MASK == kMaskRows && TILES == 1 && !C::ALIAS_P && BC >= 32), "copies of rows");
+  static_assert(COPIES == 1 || (MASK == kMaskRows && TILES == 1 && !C::ALIAS_P), "copies of rows");
   constexpr int kTmaWarp = 4 * TILES, kMmaWarp = kTmaWarp + 1, kAllocWarp = kTmaWarp + 3;  // kMmaWarp + i: tile i
   constexpr bool CAUSAL = MASK == kMaskCausal, WINDOW = MASK == kMaskWindow, ROWS = MASK == kMaskRows;
   extern __shared__ uint8_t smem_raw[];
@@ -859,13 +859,13 @@ template <int D>
 cudaError_t launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const RowsFwdArgs& a, cudaStream_t s) {
   if constexpr (rows_f16_tiles(D, 129) == 2)
     if (rows_f16_tiles(D, a.N) == 2)
-      return launch_impl<D, kMaskRows, rows_f16_block(D, 2), kFwdTiles[tile_default(0, D, false)].stages>(tk, tk, tv, a, s);
-  // Copies of few rows share a block's exponentials, the longest part of its way, among the tile's threads.
-  constexpr int BN = rows_f16_block(D, 1);
-  if constexpr (BN >= 128)
-    if (a.N <= 32) return launch_impl<D, kMaskRows, BN, 2, 1, 4>(tk, tk, tv, a, s);
-  if (a.N <= 64) return launch_impl<D, kMaskRows, BN, 2, 1, 2>(tk, tk, tv, a, s);
-  return launch_impl<D, kMaskRows, BN, 2, 1>(tk, tk, tv, a, s);
+      return launch_impl<D, kMaskRows, rows_f16_block(D, 129), kFwdTiles[tile_default(0, D, false)].stages>(tk, tk, tv, a, s);
+  // Copies of few rows share a block's exponentials among the tile's threads. Such calls wait for HBM: smaller blocks,
+  // more of them on their way.
+  constexpr int FEW = rows_f16_block(D, 64), STAGES = D == 128 ? 2 : D == 64 ? 5 : 8;
+  if (a.N <= 32) return launch_impl<D, kMaskRows, FEW, STAGES, 1, 4>(tk, tk, tv, a, s);
+  if (a.N <= 64) return launch_impl<D, kMaskRows, FEW, STAGES, 1, 2>(tk, tk, tv, a, s);
+  return launch_impl<D, kMaskRows, rows_f16_block(D, 128), 2, 1>(tk, tk, tv, a, s);
 }
 
 }  // namespace

@@ -233,10 +233,10 @@ int cuda_rc(cudaError_t e);
 int fwd_f16_kv_rows(int D, int variant);
 // kMaskRows: K and V in boxes of rows_f16_block keys.
 cudaError_t launch_rows_f16(int D, const CUtensorMap& tk, const CUtensorMap& tv, const RowsFwdArgs& a, cudaStream_t s);
-// kMaskRows: query tiles of a CTA, and keys of a block by that number. One tile (two CTAs an SM) at D <= 64 (B2 H16 N4096
+// kMaskRows: query tiles of a CTA, and keys of a block, by the number of rows. One tile (two CTAs an SM) at D <= 64 (B2 H16 N4096
 // D64: 265 us with two, 220 with one), and at D = 128 where it holds all rows.
 constexpr int rows_f16_tiles(int D, int rows) { return rows <= 128 || D <= 64 ? 1 : 2; }
-constexpr int rows_f16_block(int D, int tiles) { return D == 128 && tiles == 1 ? 64 : 128; }
+constexpr int rows_f16_block(int D, int rows) { return rows <= 64 || (D == 128 && rows <= 128) ? 64 : 128; }
 // TMA box heights of the fp16 split-backward kernels' Q/dO and K/V tensor maps for head dim D, dQ pass
 // or dK/dV pass, and tile variant.
 void bwd_f16_box_rows(int D, bool dq_pass, int variant, int* q_rows, int* kv_rows);
