@@ -382,14 +382,15 @@ extern "C" int tattn_prefix_decode(const void* q, const void* prefix_k, const vo
   d.sk = Strides3{sk[0], sk[1], sk[2]};
   d.sv = Strides3{sv[0], sv[1], sv[2]};
   d.qk_scale = sm_scale * kLog2e;
-  JoinArgs j{};
   if (P > 0) {
     if ((rc = run_rows(D, dtype, prefix_k, prefix_v, spk, spv, a, sm_scale, s)) != TATTN_OK) return rc;
-    j.n[0] = a.rows.nsplit;
+    d.overlap = true;
   }
   if ((rc = cuda_rc(launch_decode(D, cache_of(dtype), d, s))) != TATTN_OK) return rc;
+  JoinArgs j{};
   j.part[0] = a.rows.part;
   j.part_ml[0] = a.rows.part_ml;
+  j.n[0] = P > 0 ? a.rows.nsplit : 0;
   j.part[1] = d.part;
   j.part_ml[1] = d.part_ml;
   j.n[1] = d.nsplit;

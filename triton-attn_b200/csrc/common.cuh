@@ -351,6 +351,11 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
+// ---- two kernels of a stream that overlap (programmatic dependent launch): the first lets the second start once all its
+// CTAs run, and what the second does up to its wait does not read the first's results; behind the wait the first has ended.
+__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_last_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- 16 bytes of global memory (zeros where not `valid`: src is then not read) into shared memory, asynchronously
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");

@@ -258,7 +258,7 @@ constexpr int finish_floats(int NT) {
 // Joins the warps' results through shared memory, then the parts': writes finished rows if there is only one
 // part or the parts are a cluster, else the part's unnormalised rows with their maxima and sums.
 // dim(mt, half): the head dim of this lane's row g + 8 half of M tile mt.
-template <int D, int NT, typename Dim>
+template <int D, int NT, bool OVERLAP, typename Dim>
 __device__ __forceinline__ void finish(const DecodeArgs& a, const Part& p, WarpState<D, NT>& st, float* smem, Dim dim) {
   constexpr int HEADS = 8 * NT;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
@@ -283,6 +283,7 @@ __device__ __forceinline__ void finish(const DecodeArgs& a, const Part& p, WarpS
       }
     }
   __syncthreads();
+  if (OVERLAP) wait_for_last_kernel();
   for (int i = threadIdx.x; i < p.heads * (D / 4); i += kThreads) {
     const int head = i / (D / 4), d = i % (D / 4) * 4;
     float m = -INFINITY;
@@ -361,7 +362,8 @@ struct F16Cfg {
   }
 };
 
-template <int D, int NT>
+// OVERLAP: the kernel runs beside the stream's last one, of which it reads nothing, and ends after it.
+template <int D, int NT, bool OVERLAP>
 __global__ void __launch_bounds__(kThreads) decode_f16_kernel(const DecodeArgs a) {
   using C = F16Cfg<D>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -471,7 +473,7 @@ __global__ void __launch_bounds__(kThreads) decode_f16_kernel(const DecodeArgs a
   }
   cp_async_wait<0>();
   __syncthreads();  // the rings become the join's memory
-  finish<D, NT>(a, p, st, reinterpret_cast<float*>(smem), [&](int mt, int half) { return 16 * mt + 8 * half + g; });
+  finish<D, NT, OVERLAP>(a, p, st, reinterpret_cast<float*>(smem), [&](int mt, int half) { return 16 * mt + 8 * half + g; });
 }
 
 // ------------------------------------------------------------------------------------ 4-bit cache
@@ -688,7 +690,7 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeArgs 
   }
   cp_async_wait<0>();
   __syncthreads();  // the rings become the join's memory
-  finish<D, NT>(a, p, st, reinterpret_cast<float*>(smem),
+  finish<D, NT, false>(a, p, st, reinterpret_cast<float*>(smem),
                 [&](int mt, int half) { return mt / 4 * kGroupDims + 8 * g + 2 * (mt % 4) + half; });
 }
 
@@ -698,7 +700,7 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeArgs 
 // Measured (B200, 16 sequences of 8,192 tokens, D 128): 16 key/value heads for 16 query heads, 2.1 GB in 358 us, 6.0
 // TB/s; 4 for 16, 0.54 GB in 324 us, 1.7 TB/s of those bytes and 6.6 of those asked for: the fourfold reading bounds it.
 // One sequence of 1,000 tokens, 16 heads of 64: 7.3 us.
-template <int D>
+template <int D, bool OVERLAP>
 __global__ void __launch_bounds__(kThreads) decode_f32_kernel(const DecodeArgs a) {
   constexpr int E = D >= 32 ? D / 32 : 1, U = 4;  // dims a lane, tokens at a time
   __shared__ float so[kWarps][D], sml[kWarps][2];
@@ -758,6 +760,7 @@ __global__ void __launch_bounds__(kThreads) decode_f32_kernel(const DecodeArgs a
     sml[warp][1] = l;
   }
   __syncthreads();
+  if (OVERLAP) wait_for_last_kernel();
   for (int c = threadIdx.x; c < D; c += kThreads) {
     m = -INFINITY;
 #pragma unroll
@@ -826,7 +829,7 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeArgs 
 
 // `cluster`: the parts of a unit, which are neighbours in the grid, as one cluster.
 template <typename K>
-cudaError_t launch(K kernel, int smem, long long units, bool cluster, const DecodeArgs& a, cudaStream_t s) {
+cudaError_t launch(K kernel, int smem, long long units, bool cluster, const DecodeArgs& a, cudaStream_t s, bool overlap = false) {
   if (units * a.nsplit > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -837,12 +840,15 @@ cudaError_t launch(K kernel, int smem, long long units, bool cluster, const Deco
   c.blockDim = dim3(kThreads);
   c.dynamicSmemBytes = size_t(smem);
   c.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = unsigned(a.nsplit);
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  c.attrs = &attr;
-  c.numAttrs = cluster ? 1 : 0;
+  cudaLaunchAttribute attr[2] = {};
+  if (cluster) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(a.nsplit);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  }
+  if (overlap) attr[cluster ? 1 : 0] = overlapping_launch();
+  c.attrs = attr;
+  c.numAttrs = unsigned(cluster) + unsigned(overlap);
   return cudaLaunchKernelEx(&c, kernel, a);
 }
 
@@ -858,10 +864,14 @@ cudaError_t decode_impl(DecodeCache cache, const DecodeArgs& a, cudaStream_t s) 
   const bool cluster = a.nsplit > 1 && !decode_joins(a.nsplit, cache) && !a.parts_only;
   cudaError_t e;
   if (cache == kCacheF32) {
-    e = launch(decode_f32_kernel<D>, 0, decode_units(a, 1), false, a, s);
+    e = a.overlap ? launch(decode_f32_kernel<D, true>, 0, decode_units(a, 1), false, a, s, true)
+                    : launch(decode_f32_kernel<D, false>, 0, decode_units(a, 1), false, a, s);
+  } else if (cache == kCacheF16 && a.overlap) {
+    e = wide ? launch(decode_f16_kernel<D, 2, true>, F16Cfg<D>::smem(2), decode_units(a, 16), cluster, a, s, true)
+             : launch(decode_f16_kernel<D, 1, true>, F16Cfg<D>::smem(1), decode_units(a, 8), cluster, a, s, true);
   } else if (cache == kCacheF16) {
-    e = wide ? launch(decode_f16_kernel<D, 2>, F16Cfg<D>::smem(2), decode_units(a, 16), cluster, a, s)
-             : launch(decode_f16_kernel<D, 1>, F16Cfg<D>::smem(1), decode_units(a, 8), cluster, a, s);
+    e = wide ? launch(decode_f16_kernel<D, 2, false>, F16Cfg<D>::smem(2), decode_units(a, 16), cluster, a, s)
+             : launch(decode_f16_kernel<D, 1, false>, F16Cfg<D>::smem(1), decode_units(a, 8), cluster, a, s);
   } else if constexpr (D % kGroupDims == 0) {
     e = wide ? launch(decode_int4_kernel<D, 2>, Int4Cfg<D>::smem(2), decode_units(a, 16), cluster, a, s)
              : launch(decode_int4_kernel<D, 1>, Int4Cfg<D>::smem(1), decode_units(a, 8), cluster, a, s);

@@ -170,22 +170,24 @@ __device__ __forceinline__ Blocks window_blocks(int row0, int N, const WindowArg
   return b;
 }
 
-// kMaskRows: rows [row0, row0 + 128) of the head's matrix into a query tile's shared memory, by the 128 threads of a
+// kMaskRows: rows [row0, row0 + 128) of the head's matrix for a query tile's shared memory, by the 128 threads of a
 // warpgroup (t: the thread's index in it); rows past N are zeros. COPIES: the first 128 / COPIES of them so many times.
+// Steps of up to 8 units a thread: load(i0), then store(i0).
 template <typename C, int D, int COPIES>
-__device__ __forceinline__ void load_row_tile(const RowsFwdArgs& a, uint32_t dst, int zi, int hi, int row0, int t) {
-  constexpr int U = D / 8, CU = C::SWB / 16;  // 16-byte units of a row, of its part in a chunk
-  constexpr int G = U < 8 ? U : 8;  // loads in flight
-  const __half* q = static_cast<const __half*>(a.rows.q);
-#pragma unroll 1
-  for (int i0 = 0; i0 < U; i0 += G) {
-    uint4 x[G];
+struct RowTile {
+  static constexpr int U = D / 8, CU = C::SWB / 16;  // 16-byte units of a row, of its part in a chunk
+  static constexpr int G = U < 8 ? U : 8;
+  uint4 x[G];
+  __device__ __forceinline__ void load(const RowsFwdArgs& a, int zi, int hi, int row0, int t, int i0) {
+    const __half* q = static_cast<const __half*>(a.rows.q);
 #pragma unroll
     for (int i = 0; i < G; ++i) {
       const int e = (i0 + i) * 128 + t, r = row0 + e / U % (128 / COPIES);
       x[i] = make_uint4(0u, 0u, 0u, 0u);
       if (r < a.N) x[i] = __ldg(reinterpret_cast<const uint4*>(row_of(q, a.rows.sq, a.rows.inner, zi, hi, r)) + e % U);
     }
+  }
+  __device__ __forceinline__ void store(uint32_t dst, int t, int i0) const {
 #pragma unroll
     for (int i = 0; i < G; ++i) {
       const int e = (i0 + i) * 128 + t, row = e / U, unit = e % U;
@@ -194,8 +196,7 @@ __device__ __forceinline__ void load_row_tile(const RowsFwdArgs& a, uint32_t dst
                    : "memory");
     }
   }
-  fence_proxy_async_smem();
-}
+};
 
 // kMaskRows: rows [from, BN) of the value block at `block` become zeros: their weights are 0, but behind a sequence's
 // last key there may lie anything, an infinity or a NaN too.
@@ -484,6 +485,11 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
                                             : (CAUSAL ? min((row0_1 + C::BM + BN - 1) / BN, NB) : NB);
   const int nmax = max(n_0, n_1);
 
+  // kMaskRows: the first of the rows' units on their way before all else.
+  RowTile<C, D, COPIES> tile;
+  if constexpr (ROWS)
+    if (warp < 4 * TILES) tile.load(args, zi, hi, warp / 4 ? row0_1 : row0_0, threadIdx.x % 128, 0);
+
   if (threadIdx.x == 0) {
     mbar_init(bar_q, ROWS ? 128 * TILES : 1);
     for (int s = 0; s < C::NS; ++s) {
@@ -644,8 +650,16 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
     const int partial = ROWS && n > 0 && (n + list.jump) * BN > len ? n - 1 : n;
     volatile int* lim_slot = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 12);
     if constexpr (ROWS) {
-      if (n > 0) load_row_tile<C, D, COPIES>(args, sQ + i * C::QTILE, zi, hi, COPIES > 1 ? 0 : row - t, t);
+      using T = RowTile<C, D, COPIES>;
+      tile.store(sQ + i * C::QTILE, t, 0);
+#pragma unroll 1
+      for (int i0 = T::G; i0 < T::U; i0 += T::G) {
+        tile.load(args, zi, hi, i ? row0_1 : row0_0, t, i0);
+        tile.store(sQ + i * C::QTILE, t, i0);
+      }
+      fence_proxy_async_smem();
       mbar_arrive(bar_q);
+      let_next_kernel_start();
       if (COPIES > 1 && n > 0) {  // the other copies' columns of P are zeros throughout
         uint32_t zero[BN / 2];
 #pragma unroll

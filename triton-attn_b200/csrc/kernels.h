@@ -170,7 +170,7 @@ __host__ __device__ inline WindowUnit window_unit(const WindowSplit& s, const Wi
   return u;
 }
 
-// Parts of rows that are to be joined: of every row up to two lists of unnormalised parts with their maxima and sums.
+// Launched to overlap with the kernel that writes the parts (overlapping_launch). Parts of rows that are to be joined: of every row up to two lists of unnormalised parts with their maxima and sums.
 struct JoinArgs {
   const float *part[2], *part_ml[2];  // [rows, n, D] and [rows, n, 2]
   int n[2];
@@ -225,6 +225,13 @@ int encode_f16(CUtensorMap* tm, const void* p, Strides4 s, int Z, int H, int N, 
 int encode_f32_dense(CUtensorMap* tm, void* p, int Z, int H, int N, int D, int box_rows, int box_cols);
 int device_sm_count();
 int cuda_rc(cudaError_t e);
+// A launch that may start before the stream's last kernel has ended, which it then waits for itself (common.cuh).
+inline cudaLaunchAttribute overlapping_launch() {
+  cudaLaunchAttribute a{};
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  return a;
+}
 
 // `variant` below is a 0-based tile variant of tiles.h (kFwdTiles / kBwdTiles); launchers return
 // cudaErrorNotSupported for a variant that does not fit head dim D.
@@ -381,6 +388,7 @@ struct DecodeArgs {
   float qk_scale;       // sm_scale * log2(e)
   int* status;
   bool parts_only;      // write the parts, also one alone, and do not join them
+  bool overlap;         // run beside the stream's last kernel (fp16, fp32)
 };
 // CTAs per SM that decode_splits aims at: as many as an SM holds. (fp16, 64 sequences of 4096 visible tokens, 4
 // heads of 128: 2 parts each 82 us, 3 parts 86, 4 parts 90. 4 bits, 16 sequences of up to 65536 tokens: 10

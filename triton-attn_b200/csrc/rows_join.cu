@@ -24,6 +24,7 @@ __global__ void __launch_bounds__(kThreads) rows_join_kernel(const JoinArgs a) {
   const int outer = row / a.inner, in = row - outer * a.inner;
   const int64_t rows[2] = {index, z * a.other.z + h * a.other.h + outer * a.other.outer + in * a.other.in};
   const int t = threadIdx.x % V, p = threadIdx.x / V;
+  wait_for_last_kernel();
   float m = -INFINITY;
 #pragma unroll
   for (int x = 0; x < 2; ++x)
@@ -81,11 +82,14 @@ cudaError_t join_impl(bool is_f16, const JoinArgs& a, cudaStream_t s) {
   const int64_t rows = int64_t(a.Z) * a.H * a.N;
   if (rows == 0) return cudaSuccess;
   if (rows > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  if (is_f16)
-    rows_join_kernel<__half, D><<<unsigned(rows), kThreads, 0, s>>>(a);
-  else
-    rows_join_kernel<float, D><<<unsigned(rows), kThreads, 0, s>>>(a);
-  return cudaGetLastError();
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(unsigned(rows));
+  c.blockDim = dim3(kThreads);
+  c.stream = s;
+  cudaLaunchAttribute attr = overlapping_launch();
+  c.attrs = &attr;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, is_f16 ? rows_join_kernel<__half, D> : rows_join_kernel<float, D>, a);
 }
 
 }  // namespace
