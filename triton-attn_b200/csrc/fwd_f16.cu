@@ -170,33 +170,55 @@ __device__ __forceinline__ Blocks window_blocks(int row0, int N, const WindowArg
   return b;
 }
 
-// kMaskRows: rows [row0, row0 + 128) of the head's matrix for a query tile's shared memory, by the 128 threads of a
-// warpgroup (t: the thread's index in it); rows past N are zeros. COPIES: the first 128 / COPIES of them so many times.
-// Steps of up to 8 units a thread: load(i0), then store(i0).
+// kMaskRows: rows [row0, row0 + 128) of the head's matrix into a query tile's shared memory, asynchronously, by the 128
+// threads of a warpgroup (t: the thread's index in it); rows past N are zeros. COPIES: the first 128 / COPIES of them so
+// many times. (Rolled: a kernel of a few microseconds waits for its instructions.)
 template <typename C, int D, int COPIES>
-struct RowTile {
-  static constexpr int U = D / 8, CU = C::SWB / 16;  // 16-byte units of a row, of its part in a chunk
-  static constexpr int G = U < 8 ? U : 8;
-  uint4 x[G];
-  __device__ __forceinline__ void load(const RowsFwdArgs& a, int zi, int hi, int row0, int t, int i0) {
-    const __half* q = static_cast<const __half*>(a.rows.q);
+__device__ __forceinline__ void load_row_tile(const RowsFwdArgs& a, uint32_t dst, int zi, int hi, int row0, int t) {
+  constexpr int U = D / 8, CU = C::SWB / 16;  // 16-byte units of a row, of its part in a chunk
+  constexpr int STEP = 128 / U, ROWS = 128 / COPIES;
+  const RowMap& s = a.rows.sq;
+  const int inner = a.rows.inner, unit = t % U, q0 = STEP / inner, r0 = STEP - q0 * inner;
+  int outer = (row0 + t / U) / inner, in = row0 + t / U - outer * inner;  // (stepped: divisions are long)
+  const __half* q = static_cast<const __half*>(a.rows.q) + zi * s.z + hi * s.h + unit * 8;
+#pragma unroll 1
+  for (int row = t / U; row < ROWS; row += STEP) {
+    const bool valid = row0 + row < a.N;
+    const __half* src = q + (valid ? outer * s.outer + in * s.in : 0);
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
-      const int e = (i0 + i) * 128 + t, r = row0 + e / U % (128 / COPIES);
-      x[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < a.N) x[i] = __ldg(reinterpret_cast<const uint4*>(row_of(q, a.rows.sq, a.rows.inner, zi, hi, r)) + e % U);
+    for (int c = 0; c < COPIES; ++c)
+      cp_async16(dst + unit / CU * C::QCHUNK + swizzle_offset<C::SWB>(uint32_t((row + c * ROWS) * C::SWB + unit % CU * 16)), src, valid);
+    outer += q0;
+    in += r0;
+    if (in >= inner) {
+      in -= inner;
+      ++outer;
     }
   }
-  __device__ __forceinline__ void store(uint32_t dst, int t, int i0) const {
-#pragma unroll
-    for (int i = 0; i < G; ++i) {
-      const int e = (i0 + i) * 128 + t, row = e / U, unit = e % U;
-      const uint32_t at = dst + unit / CU * C::QCHUNK + swizzle_offset<C::SWB>(uint32_t(row * C::SWB + unit % CU * 16));
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[i].x), "r"(x[i].y), "r"(x[i].z), "r"(x[i].w)
-                   : "memory");
-    }
+}
+
+// kMaskRows: 16-byte units of a warp's 32 rows, U a row, by way of its part of the query tile's shared memory (which no
+// MMA reads any more), so that a row leaves as one run: written by the rows' threads, read U lanes a row.
+template <int U>
+__device__ __forceinline__ uint32_t staged(uint32_t base, int row, int unit) {
+  return base + (row * U + (unit ^ (row & (U - 1)))) * 16;
+}
+__device__ __forceinline__ void stage_put(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// to(row): where row `row` of the warp's goes; rows from `rows` on go nowhere.
+template <int U, typename To>
+__device__ __forceinline__ void stage_out(uint32_t base, int rows, int lane, To to) {
+  __syncwarp();
+#pragma unroll 4
+  for (int i = 0; i < U; ++i) {
+    const int row = (i * 32 + lane) / U, unit = (i * 32 + lane) % U;
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(staged<U>(base, row, unit)) : "memory");
+    if (row < rows) *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(to(row)) + unit * 16) = x;
   }
-};
+  __syncwarp();
+}
 
 // kMaskRows: rows [from, BN) of the value block at `block` become zeros: their weights are 0, but behind a sequence's
 // last key there may lie anything, an infinity or a NaN too.
@@ -311,26 +333,32 @@ __device__ __forceinline__ void no_keys(const RowsFwdArgs& a, int bh, int row, i
   if (a.m != nullptr) a.m[at] = -INFINITY;
 }
 
-// kMaskRows: a row's part as it is.
-template <typename C, int D>
-__device__ __forceinline__ void store_part(const RowsFwdArgs& a, int bh, int row, int nct, uint32_t tO, float m, float l) {
-  const int64_t at = (int64_t(bh) * a.N + row) * a.rows.nsplit + (int(blockIdx.x) / nct - bh * a.rows.nsplit);
+// kMaskRows: the parts of a warp's rows (row: the thread's) as they are. stage: 64 D bytes of shared memory. (Stored by the
+// rows' own threads, a part of D = 128 took 6 us. Finished rows, of half the bytes, are no faster this way.)
+template <int D>
+__device__ __forceinline__ void store_parts(const RowsFwdArgs& a, uint32_t stage, int bh, int row, int nct, uint32_t tO, float m,
+                                            float l) {
+  constexpr int HALF = D / 2, U = HALF / 4, V = HALF < 32 ? HALF : 32;
+  const int lane = threadIdx.x % 32, rows = a.N - (row - lane);
+  const int64_t part0 = (int64_t(bh) * a.N + row - lane) * a.rows.nsplit + (int(blockIdx.x) / nct - bh * a.rows.nsplit);
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h) {
 #pragma unroll
-  for (int c0 = 0; c0 < D; c0 += 32) {
-    constexpr int W = D < 32 ? D : 32;
-    uint32_t o[W];
-    tmem_load_cols<W>(tO + c0, o);
-    tmem_wait_ld();
-    reg_fence<W>(o);
-    if (row < a.N) {
-      uint4* dst = reinterpret_cast<uint4*>(a.rows.part + at * D + c0);
+    for (int c0 = 0; c0 < HALF; c0 += V) {
+      uint32_t o[V];
+      tmem_load_cols<V>(tO + h * HALF + c0, o);
+      tmem_wait_ld();
+      reg_fence<V>(o);
 #pragma unroll
-      for (int v = 0; v < W / 4; ++v) dst[v] = make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+      for (int c = 0; c < V; c += 4) stage_put(staged<U>(stage, lane, (c0 + c) / 4), o[c], o[c + 1], o[c + 2], o[c + 3]);
     }
+    stage_out<U>(stage, rows, lane, [&](int r) { return a.rows.part + (part0 + int64_t(r) * a.rows.nsplit) * D + h * HALF; });
   }
-  // All scores -infinity: the largest float below 0 and no weight (the FMA pipe's exponentials left 2^-126 each); -infinity
-  // would say that the part has no keys.
-  if (row < a.N) reinterpret_cast<float2*>(a.rows.part_ml)[at] = m == -INFINITY ? make_float2(-FLT_MAX, 0.f) : make_float2(m, l);
+  // All scores -infinity: the largest float below 0 and no weight (the FMA pipe's exponentials left 2^-126 each);
+  // -infinity would say that the part has no keys.
+  if (lane < rows)
+    reinterpret_cast<float2*>(a.rows.part_ml)[part0 + int64_t(lane) * a.rows.nsplit] =
+        m == -INFINITY ? make_float2(-FLT_MAX, 0.f) : make_float2(m, l);
 }
 
 // kMaskRows with COPIES: joins the copies of each row, which took a share of every block's keys each, through shared
@@ -393,7 +421,7 @@ __device__ __forceinline__ void finish_copies(const RowsFwdArgs& a, float* smem,
       *reinterpret_cast<uint32_t*>(a.o_rest + index * D + col) = rest_of(o, h.x, inv_l) | (rest_of(o + 2, h.y, inv_l) << 16);
   }
   if (copy > 0) return;
-  if (a.rows.part)  // (as store_part)
+  if (a.rows.part)  // (as store_parts)
     reinterpret_cast<float2*>(a.rows.part_ml)[part] = top == -INFINITY ? make_float2(-FLT_MAX, 0.f) : make_float2(top, sum);
   else if (a.m != nullptr)
     a.m[index] = top + log2f(sum);
@@ -485,10 +513,10 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
                                             : (CAUSAL ? min((row0_1 + C::BM + BN - 1) / BN, NB) : NB);
   const int nmax = max(n_0, n_1);
 
-  // kMaskRows: the first of the rows' units on their way before all else.
-  RowTile<C, D, COPIES> tile;
-  if constexpr (ROWS)
-    if (warp < 4 * TILES) tile.load(args, zi, hi, warp / 4 ? row0_1 : row0_0, threadIdx.x % 128, 0);
+  const uint32_t sQ = base_u32 + C::OFF_Q, sK = base_u32 + C::OFF_K, sV = base_u32 + C::OFF_V;
+  if constexpr (ROWS)  // on their way before all else
+    if (warp < 4 * TILES)
+      load_row_tile<C, D, COPIES>(args, sQ + warp / 4 * C::QTILE, zi, hi, warp / 4 ? row0_1 : row0_0, threadIdx.x % 128);
 
   if (threadIdx.x == 0) {
     mbar_init(bar_q, ROWS ? 128 * TILES : 1);
@@ -523,7 +551,6 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  const uint32_t sQ = base_u32 + C::OFF_Q, sK = base_u32 + C::OFF_K, sV = base_u32 + C::OFF_V;
 
   if (warp >= kTmaWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs<TILES>));
@@ -650,13 +677,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
     const int partial = ROWS && n > 0 && (n + list.jump) * BN > len ? n - 1 : n;
     volatile int* lim_slot = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 12);
     if constexpr (ROWS) {
-      using T = RowTile<C, D, COPIES>;
-      tile.store(sQ + i * C::QTILE, t, 0);
-#pragma unroll 1
-      for (int i0 = T::G; i0 < T::U; i0 += T::G) {
-        tile.load(args, zi, hi, i ? row0_1 : row0_0, t, i0);
-        tile.store(sQ + i * C::QTILE, t, i0);
-      }
+      cp_async_wait_all();
       fence_proxy_async_smem();
       mbar_arrive(bar_q);
       let_next_kernel_start();
@@ -766,17 +787,18 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
       }
     } else if (ok && n > 0 && warp_wait(&bar_o_done[i], (n - 1) & 1, ab)) {
       tc_fence_after();
-      // No result where the largest score is NaN, or infinite of either sign (l itself misses some of that).
-      const float inv_l = m_run - m_run == 0.f ? 1.f / l_run : NAN;
       // The head index from shared memory rather than a register held through the block loop (one
       // spilled register fewer).
       const int bh_e = *reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
-      const int zi_e = bh_e / args.H, hi_e = bh_e % args.H;
       bool whole = true;
       if constexpr (ROWS) whole = args.rows.part == nullptr;
       if (!whole) {
-        if constexpr (ROWS) store_part<C, D>(args, bh_e, row, nct, tO, m_run, l_run);
+        if constexpr (ROWS)
+          store_parts<D>(args, sQ + i * C::QTILE + warp % 4 * (C::QTILE / 4), bh_e, row, nct, tO, m_run, l_run);
       } else {
+        // No result where the largest score is NaN, or infinite of either sign (l itself misses some of that).
+        const float inv_l = m_run - m_run == 0.f ? 1.f / l_run : NAN;
+        const int zi_e = bh_e / args.H, hi_e = bh_e % args.H;
         __half* orow;
         if constexpr (ROWS)
           orow = row_of(static_cast<__half*>(args.o), args.rows.so, args.rows.inner, zi_e, hi_e, row);

@@ -64,17 +64,21 @@ struct RowsArgs {
 };
 // Parts that the `blocks` key blocks of `tiles` row tiles are cut into, of which `slots` run at a time: the number with
 // the shortest time, in blocks, when a CTA takes `start` to begin and to end and the parts' join `join`.
+// (Of the numbers that take equally many rounds, the largest.)
 inline int rows_splits(long long tiles, long long blocks, long long slots, int start, int join) {
-  int best = 1;
-  long long least = 0;
-  for (int n = 1; n <= blocks && n <= kMaxRowSplits; ++n) {
-    const long long cost = (tiles * n + slots - 1) / slots * ((blocks + n - 1) / n + start) + (n > 1 ? join : 0);
-    if (n == 1 || cost < least) {
+  long long best = 1, least = (tiles + slots - 1) / slots * (blocks + start);
+  for (long long rounds = 1; rounds <= 4; ++rounds) {
+    long long n = rounds * slots / tiles;
+    n = n < blocks ? n : blocks;
+    n = n < kMaxRowSplits ? n : kMaxRowSplits;
+    if (n <= 1) continue;
+    const long long cost = (tiles * n + slots - 1) / slots * ((blocks + n - 1) / n + start) + join;
+    if (cost < least) {
       least = cost;
       best = n;
     }
   }
-  return best;
+  return int(best);
 }
 
 struct FwdArgs {
