@@ -93,6 +93,14 @@ DecodeArgs token_args(int Z, int H, int Hk, int Nq, int Nk) {
   return a;
 }
 DecodeCache cache_of(int dtype) { return dtype == TATTN_F16 ? kCacheF16 : kCacheF32; }
+// Parts of a sequence's keys: as for a cache, but no more than run at a time. (8 sequences of up to 1500 keys, 16 heads of
+// 64: 14.3 us with the cache's 3 parts, 2 of which an SM holds, 10.6 with 2.)
+int token_parts(const DecodeArgs& a, int D, int dtype) {
+  const int n = decode_splits(a, D, cache_of(dtype)), heads = dtype == TATTN_F32 ? 1 : a.H / a.Hk <= 8 ? 8 : 16;
+  const int64_t units = int64_t(a.Z) * a.Hk * ((a.H / a.Hk + heads - 1) / heads);
+  const int64_t most = int64_t(decode_ctas(cache_of(dtype))) * device_sm_count() / std::max<int64_t>(units, 1);
+  return int(std::max<int64_t>(1, std::min<int64_t>(n, most)));
+}
 
 }  // namespace
 
@@ -103,7 +111,7 @@ extern "C" int64_t tattn_cross_fwd_workspace_bytes(int Z, int H, int Hk, int Nq,
   const int parts = row_parts(D, dtype, int64_t(Z) * Hk, H / Hk * Nq, Nk);
   int64_t bytes = parts > 1 ? part_bytes(D, rows, parts) : 0;
   if (few_rows(H, Hk, Nq, dtype)) {
-    const int n = decode_splits(token_args(Z, H, Hk, Nq, Nk), D, cache_of(dtype));
+    const int n = token_parts(token_args(Z, H, Hk, Nq, Nk), D, dtype);
     if (decode_joins(n, cache_of(dtype))) bytes = std::max(bytes, part_bytes(D, rows, n));
   }
   return bytes;
@@ -127,7 +135,7 @@ extern "C" int tattn_cross_fwd(const void* q, const void* k, const void* v, cons
     DecodeArgs a = token_args(Z, H, Hk, Nq, Nk);
     const int rc = device_ready(&a.status);
     if (rc != TATTN_OK) return rc;
-    a.nsplit = decode_splits(a, D, cache_of(dtype));
+    a.nsplit = token_parts(a, D, dtype);
     if (decode_joins(a.nsplit, cache_of(dtype))) {
       if (!workspace) return TATTN_ERR_INVALID_ARGUMENT;
       a.part = static_cast<float*>(workspace);
@@ -326,6 +334,11 @@ bool prefix_fits(int prompts, int samples, int H, int Hk, int P) {
   return double(prompts) * samples * H < 5e8 && double(prompts) * Hk * (P / 128 + 1) < 1e7;
 }
 DecodeArgs own_args(int prompts, int samples, int H, int Hk, int C) { return token_args(prompts * samples, H, Hk, 1, C); }
+// Parts of the sequences' own tokens: as for a cache, but of 256 tokens at least, as the prefix's parts are joined anyhow
+// (16 samples of up to 256 tokens: 11.4 us with 2 parts, 10.6 with one).
+int own_parts(const DecodeArgs& a, int D, int dtype) {
+  return std::min(decode_splits(a, D, cache_of(dtype)), std::max(1, a.C / 256));
+}
 
 }  // namespace
 
@@ -334,7 +347,7 @@ extern "C" int64_t tattn_prefix_decode_workspace_bytes(int prompts, int samples,
   const int64_t rows = int64_t(prompts) * samples * H;
   if (rows == 0) return 0;
   return part_bytes(D, rows, row_parts(D, dtype, int64_t(prompts) * Hk, samples * (H / Hk), P)) +
-         part_bytes(D, rows, decode_splits(own_args(prompts, samples, H, Hk, C), D, cache_of(dtype)));
+         part_bytes(D, rows, own_parts(own_args(prompts, samples, H, Hk, C), D, dtype));
 }
 
 extern "C" int tattn_prefix_decode(const void* q, const void* prefix_k, const void* prefix_v, const int32_t* prefix_lengths,
@@ -370,7 +383,7 @@ extern "C" int tattn_prefix_decode(const void* q, const void* prefix_k, const vo
   DecodeArgs d = own_args(prompts, samples, H, Hk, C);
   int rc = device_ready(&d.status);
   if (rc != TATTN_OK) return rc;
-  d.nsplit = decode_splits(d, D, cache_of(dtype));
+  d.nsplit = own_parts(d, D, dtype);
   d.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_bytes(D, rows, a.rows.nsplit));
   d.part_ml = d.part + rows * d.nsplit * D;
   d.parts_only = true;

@@ -192,6 +192,25 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 2) norm_rope_ke
     const int item = base + int(threadIdx.x) / L;
     const bool any = item < t.items;
     const Item it = rope_item(a, t, HB, any ? item : 0);
+    // All of the item's loads first, as they come: they are what takes time. (On several axes also before the
+    // positions, which the tables' loads wait for.)
+    uint4 rx[HB][2], rdy[BACKWARD ? HB : 1][2];
+    auto load_rows = [&] {
+#pragma unroll
+      for (int i = 0; i < HB; ++i) {
+        const bool row = any && it.h0 + i < t.H;
+        const int64_t h = row ? it.h0 + i : 0;
+        const T* px = static_cast<const T*>(t.px) + it.z * t.x.z + h * t.x.h + it.n * t.x.n + col;
+        rx[i][0] = load_raw(px);
+        rx[i][1] = load_raw(px + D / 2);
+        if constexpr (BACKWARD) {
+          const T* pd = static_cast<const T*>(t.pdy) + it.z * t.dy.z + h * t.dy.h + it.n * t.dy.n + col;
+          rdy[i][0] = load_raw(pd);
+          rdy[i][1] = load_raw(pd + D / 2);
+        }
+      }
+    };
+    if (FORM != kOnePosition) load_rows();
     float cs[VEC], sn[VEC];
     bool in_table = true;
     if constexpr (FORM == kOnePosition) {
@@ -234,21 +253,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 2) norm_rope_ke
       for (int j = 0; j < VEC; ++j) cs[j] = sn[j] = __int_as_float(0x7fffffff);
       if (c == 0) atomicOr(a.status, kStatusIndexRange);
     }
-    // All of the item's loads first, as they come: they are what takes time.
-    uint4 rx[HB][2], rdy[BACKWARD ? HB : 1][2];
-#pragma unroll
-    for (int i = 0; i < HB; ++i) {
-      const bool row = any && it.h0 + i < t.H;
-      const int64_t h = row ? it.h0 + i : 0;
-      const T* px = static_cast<const T*>(t.px) + it.z * t.x.z + h * t.x.h + it.n * t.x.n + col;
-      rx[i][0] = load_raw(px);
-      rx[i][1] = load_raw(px + D / 2);
-      if constexpr (BACKWARD) {
-        const T* pd = static_cast<const T*>(t.pdy) + it.z * t.dy.z + h * t.dy.h + it.n * t.dy.n + col;
-        rdy[i][0] = load_raw(pd);
-        rdy[i][1] = load_raw(pd + D / 2);
-      }
-    }
+    if (FORM == kOnePosition) load_rows();
 #pragma unroll
     for (int i = 0; i < HB; ++i) {
       const bool row = any && it.h0 + i < t.H;
