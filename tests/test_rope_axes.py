@@ -213,7 +213,8 @@ def test_one_axis_and_equal_axes_are_qk_norm_rope(gpu, interleaved, dtype) -> No
     want = qk_norm_rope(q, k, wq, wk, cos, sin, at[0], interleaved=interleaved)
     for count, mixed in ((1, False), (3, False), (4, True)):
         got = qk_rope_axes(q, k, cos, sin, at.expand(count, 2, 70), _pair_axes(64, count, mixed), wq, wk, interleaved=interleaved)
-        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        for g, w in zip(got, want, strict=True):  # the same sums in another order: 16-bit results a rounding apart
+            torch.testing.assert_close(g, w, atol=2e-6, rtol=2.0**-10 if dtype == torch.float16 else 2e-6)
 
 
 @pytest.mark.gpu

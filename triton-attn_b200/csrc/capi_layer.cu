@@ -24,9 +24,9 @@ bool rows16(const void* p, const int64_t* s, int Z, int H, int N, int esz) {
 
 Strides3 strides3(const int64_t* s) { return Strides3{s[0], s[1], s[2]}; }
 
-// strides: of q, k, q_out, k_out (backward: of q, k, q_grad, k_grad, dq, dk); positions (axis, z, n strides).
-int norm_rope(RopeArgs& a, RopeForm form, bool backward, const int64_t* strides, const int64_t* pos, int Z, int H, int Hk,
-              int N, int D, int P, int dtype, int w_dtype, int interleaved, void* stream) {
+// The arguments of both rotations but for the positions' strides. strides: of q, k, q_out, k_out (backward: of q, k,
+// q_grad, k_grad, dq, dk).
+int rope_args(RopeArgs& a, bool backward, const int64_t* strides, int Z, int H, int Hk, int N, int P, int dtype, int w_dtype) {
   const int esz = dtype == TATTN_F16 ? 2 : 4, heads[2] = {H, Hk};
   for (int i = 0; i < 2; ++i) {
     RopeTensor& t = a.t[i];
@@ -40,16 +40,31 @@ int norm_rope(RopeArgs& a, RopeForm form, bool backward, const int64_t* strides,
     t.H = heads[i];
   }
   if (((reinterpret_cast<uintptr_t>(a.cos) | reinterpret_cast<uintptr_t>(a.sin)) & 15u) != 0) return TATTN_ERR_LAYOUT;
-  a.pos_a = pos[0];
-  a.pos_z = pos[1];
-  a.pos_n = pos[2];
   a.Z = Z;
   a.N = N;
   a.P = P;
   a.w_f32 = w_dtype == TATTN_F32;
-  const int rc = device_ready(&a.status);
+  return device_ready(&a.status);
+}
+
+int norm_rope(RopeArgs& a, bool backward, const int64_t* strides, int Z, int H, int Hk, int N, int D, int P, int dtype,
+              int w_dtype, int interleaved, void* stream) {
+  const int rc = rope_args(a, backward, strides, Z, H, Hk, N, P, dtype, w_dtype);
   if (rc != TATTN_OK) return rc;
-  return cuda_rc(launch_norm_rope(D, dtype == TATTN_F16, form, interleaved != 0, backward, a, static_cast<cudaStream_t>(stream)));
+  const int64_t* pos = strides + (backward ? 24 : 16);
+  a.pos_z = pos[0];
+  a.pos_n = pos[1];
+  return cuda_rc(launch_norm_rope(D, dtype == TATTN_F16, interleaved != 0, backward, a, static_cast<cudaStream_t>(stream)));
+}
+
+int rope_axes(RopeAxesArgs& a, bool norm, bool backward, const int64_t* strides, const int64_t* pos, int Z, int H, int Hk, int N,
+              int D, int P, int dtype, int w_dtype, int interleaved, void* stream) {
+  const int rc = rope_args(a, backward, strides, Z, H, Hk, N, P, dtype, w_dtype);
+  if (rc != TATTN_OK) return rc;
+  a.pos_a = pos[0];
+  a.pos_z = pos[1];
+  a.pos_n = pos[2];
+  return cuda_rc(launch_rope_axes(D, dtype == TATTN_F16, norm, interleaved != 0, backward, a, static_cast<cudaStream_t>(stream)));
 }
 
 int norm_rope_dims(int Z, int H, int Hk, int N, int D, int P, int dtype, int w_dtype) {
@@ -84,8 +99,7 @@ extern "C" int tattn_qk_norm_rope(const void* q, const void* k, const void* wq, 
   a.sin = sin;
   a.positions = positions;
   a.eps = eps;
-  const int64_t pos[3] = {0, strides[16], strides[17]};
-  return norm_rope(a, kOnePosition, false, strides, pos, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved, stream);
+  return norm_rope(a, false, strides, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved, stream);
 }
 
 extern "C" int tattn_qk_norm_rope_bwd(const void* q, const void* k, const void* wq, const void* wk, const void* q_grad,
@@ -115,8 +129,7 @@ extern "C" int tattn_qk_norm_rope_bwd(const void* q, const void* k, const void* 
   a.positions = positions;
   a.eps = eps;
   a.part = static_cast<float*>(workspace);
-  const int64_t pos[3] = {0, strides[24], strides[25]};
-  return norm_rope(a, kOnePosition, true, strides, pos, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved, stream);
+  return norm_rope(a, true, strides, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved, stream);
 }
 
 extern "C" int64_t tattn_qk_norm_rope_bwd_workspace_bytes(int D) {
@@ -127,7 +140,7 @@ extern "C" int64_t tattn_qk_norm_rope_bwd_workspace_bytes(int D) {
 namespace {
 
 // The axis of each pair into a.axes; false where one is outside [0, A).
-bool rope_axes(RopeArgs& a, const int32_t* axes, int A, int D) {
+bool pair_axes(RopeAxesArgs& a, const int32_t* axes, int A, int D) {
   if (!axes || A < 1 || A > kRopeAxes) return false;
   a.A = A;
   for (int j = 0; j < D / 2; ++j) {
@@ -146,8 +159,8 @@ extern "C" int tattn_qk_rope_axes(const void* q, const void* k, const void* wq, 
   if (!strides) return TATTN_ERR_INVALID_ARGUMENT;
   const int rc = norm_rope_dims(Z, H, Hk, N, D, P, dtype, w_dtype);
   if (rc != TATTN_OK) return rc;
-  RopeArgs a{};
-  if (!rope_axes(a, axes, A, D) || (wq == nullptr) != (wk == nullptr)) return TATTN_ERR_INVALID_ARGUMENT;
+  RopeAxesArgs a{};
+  if (!pair_axes(a, axes, A, D) || (wq == nullptr) != (wk == nullptr)) return TATTN_ERR_INVALID_ARGUMENT;
   if (int64_t(Z) * N == 0) return TATTN_OK;
   if (!q || !k || !q_out || !k_out || !cos || !sin || !positions) return TATTN_ERR_INVALID_ARGUMENT;
   a.t[0].px = q;
@@ -160,8 +173,7 @@ extern "C" int tattn_qk_rope_axes(const void* q, const void* k, const void* wq, 
   a.sin = sin;
   a.positions = positions;
   a.eps = eps;
-  return norm_rope(a, wq ? kAxesNorm : kAxes, false, strides, strides + 16, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved,
-                   stream);
+  return rope_axes(a, wq != nullptr, false, strides, strides + 16, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved, stream);
 }
 
 extern "C" int tattn_qk_rope_axes_bwd(const void* q, const void* k, const void* wq, const void* wk, const void* q_grad,
@@ -172,9 +184,9 @@ extern "C" int tattn_qk_rope_axes_bwd(const void* q, const void* k, const void* 
   if (!strides) return TATTN_ERR_INVALID_ARGUMENT;
   const int rc = norm_rope_dims(Z, H, Hk, N, D, P, dtype, w_dtype);
   if (rc != TATTN_OK) return rc;
-  RopeArgs a{};
+  RopeAxesArgs a{};
   const bool norm = wq != nullptr, any = int64_t(Z) * N > 0;
-  if (!rope_axes(a, axes, A, D) || norm != (wk != nullptr) || (norm && (!dwq || !dwk || !workspace)))
+  if (!pair_axes(a, axes, A, D) || norm != (wk != nullptr) || (norm && (!dwq || !dwk || !workspace)))
     return TATTN_ERR_INVALID_ARGUMENT;
   if (any && (!q_grad || !k_grad || !dq || !dk || !cos || !sin || !positions || (norm && (!q || !k))))
     return TATTN_ERR_INVALID_ARGUMENT;
@@ -188,7 +200,7 @@ extern "C" int tattn_qk_rope_axes_bwd(const void* q, const void* k, const void* 
     a.t[0].px = q_grad;
     a.t[1].px = k_grad;
     a.back = 1;
-    return norm_rope(a, kAxes, false, strides + 8, strides + 24, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved, stream);
+    return rope_axes(a, false, false, strides + 8, strides + 24, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved, stream);
   }
   a.t[0].px = q;
   a.t[1].px = k;
@@ -200,7 +212,7 @@ extern "C" int tattn_qk_rope_axes_bwd(const void* q, const void* k, const void* 
   a.t[1].dw = dwk;
   a.eps = eps;
   a.part = static_cast<float*>(workspace);
-  return norm_rope(a, kAxesNorm, true, strides, strides + 24, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved, stream);
+  return rope_axes(a, true, true, strides, strides + 24, Z, H, Hk, N, D, P, dtype, w_dtype, interleaved, stream);
 }
 
 namespace {

@@ -364,16 +364,36 @@ struct RopeArgs {
   int w_f32;                  // weights (and dw) are fp32, else the tensors' type
   float eps;
   int* status;
-  // kAxesNorm, kAxes: positions is [A, Z, N], with axis stride pos_a
-  int64_t pos_a;
-  int A;                      // 1 to kRopeAxes
-  int back;                   // kAxes: turn by the negative angles
-  uint32_t axes[4];           // the axis of each of the D / 2 pairs, 2 bits a pair
 };
-constexpr int kRopeBlocksPerSm = 4, kRopeAxes = 4;
-// One position a token, with the norms; positions on several axes, with the norms; those without (forward only).
-enum RopeForm : int { kOnePosition, kAxesNorm, kAxes };
-cudaError_t launch_norm_rope(int D, bool is_f16, RopeForm form, bool interleaved, bool backward, RopeArgs a, cudaStream_t s);
+constexpr int kRopeBlocksPerSm = 4;
+cudaError_t launch_norm_rope(int D, bool is_f16, bool interleaved, bool backward, RopeArgs a, cudaStream_t s);
+// The weights' gradients from the CTAs' partials (a.part, of a.t[0].blocks CTAs, then a.t[1].blocks).
+cudaError_t launch_norm_rope_dw(bool is_f16, int D, const RopeArgs& a, cudaStream_t s);
+
+// A division by d of numbers below 2^31: of the high half of a product (Granlund and Montgomery, 1994). With l =
+// ceil(log2 d) and m = ceil(2^(31 + l) / d) < 2^32 it is exact, as m d - 2^(31 + l) < d <= 2^l.
+struct ByMultiple {
+  uint32_t d, m;
+  int shift;  // l - 1; -1: d is 1
+  __device__ __forceinline__ uint32_t quotient(uint32_t x) const { return shift < 0 ? x : __umulhi(x, m) >> shift; }
+};
+inline ByMultiple by_multiple(int d) {
+  int l = 0;
+  while ((int64_t(1) << l) < d) ++l;
+  return d <= 1 ? ByMultiple{1, 0, -1} : ByMultiple{uint32_t(d), uint32_t(((uint64_t(1) << (31 + l)) + d - 1) / d), l - 1};
+}
+
+// Rotation by positions on several axes (rope_axes.cu): positions is [A, Z, N].
+constexpr int kRopeAxes = 4;
+struct RopeAxesArgs : RopeArgs {
+  int64_t pos_a;       // the axes' stride
+  int A;               // 1 to kRopeAxes
+  int back;            // without norms: turn by the negative angles
+  uint32_t axes[4];    // the axis of each of the D / 2 pairs, 2 bits a pair
+  ByMultiple chunks[2], tokens;  // divisions by a tensor's chunks of heads and by N (set by the launcher)
+};
+// Without the norms only forward (`back` for the gradients).
+cudaError_t launch_rope_axes(int D, bool is_f16, bool norm, bool interleaved, bool backward, RopeAxesArgs a, cudaStream_t s);
 
 // Attention of single tokens over a cache (decode.cu).
 enum DecodeCache : int { kCacheF16, kCacheInt4, kCacheF32 };

@@ -1,5 +1,4 @@
-// Norms of query and key heads with the position rotation in the same pass, and the gradients; the rotation by
-// positions on several axes, with the norms or alone.
+// Norms of query and key heads with the position rotation in the same pass, and the gradients.
 //
 // A row x (one head of one token, D values) at position p, with the tensor's weight w and the tables
 // cos[p], sin[p] (D / 2 values each):
@@ -7,8 +6,6 @@
 //   y_i = z_i cos_j - z_i' sin_j,  y_i' = z_i' cos_j + z_i sin_j
 // for pair j = (i, i') = (j, j + D / 2), or (2 j, 2 j + 1) where `interleaved`. Backward, from dy:
 //   g = R^T dy,  dw = sum over rows of g x r,  h = g w,  dx = r (h - x r mean(h x r)).
-// On several axes (kAxesNorm, kAxes) a token has a position on each, and pair j is rotated by the tables' row at its
-// position on axis axes[j]. kAxes has no norm: y = R x and dx = R^T dy, the same kernel turning the other way.
 // Everything between the loads and the stores is fp32; results are rounded once.
 //
 // The bound is HBM: x is read and y written once (backward: x, dy, dx), about 3 (7) FMAs a value. A group of
@@ -28,6 +25,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "rope.cuh"
 
 namespace tattn {
 namespace {
@@ -38,80 +36,6 @@ constexpr int kThreads = 256;
 // and 2 heads 46 and 78 us for 42 and 67.)
 template <typename T, bool BACKWARD>
 constexpr int kMany = sizeof(T) == 4 ? (BACKWARD ? 1 : 2) : (BACKWARD ? 2 : 4);
-
-template <typename T>
-constexpr int kVec = 16 / int(sizeof(T));
-
-// 16 bytes of T as floats, and back (rounded to nearest).
-template <typename T>
-__device__ __forceinline__ void unpack16(const uint4& v, float* x) {
-  if constexpr (sizeof(T) == 2) {
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-  } else {
-    x[0] = __uint_as_float(v.x);
-    x[1] = __uint_as_float(v.y);
-    x[2] = __uint_as_float(v.z);
-    x[3] = __uint_as_float(v.w);
-  }
-}
-template <typename T>
-__device__ __forceinline__ uint4 load_raw(const T* p) {
-  return *reinterpret_cast<const uint4*>(p);
-}
-template <typename T>
-__device__ __forceinline__ void load16(const T* p, float* x) {
-  unpack16<T>(load_raw(p), x);
-}
-template <typename T>
-__device__ __forceinline__ void store16(T* p, const float* x) {
-  if constexpr (sizeof(T) == 2)
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]),
-                                              pack_half2(x[6], x[7]));
-  else
-    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-}
-
-// N consecutive floats (N = 2, 4 or 8; aligned to their size, at most 16 bytes).
-template <int N>
-__device__ __forceinline__ void load_floats(const float* p, float* x) {
-  if constexpr (N == 2) {
-    const float2 v = *reinterpret_cast<const float2*>(p);
-    x[0] = v.x;
-    x[1] = v.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(p + i);
-      x[i] = v.x;
-      x[i + 1] = v.y;
-      x[i + 2] = v.z;
-      x[i + 3] = v.w;
-    }
-  }
-}
-
-// Sum over the L lanes of a group (L a power of two, groups aligned in the warp).
-template <int L>
-__device__ __forceinline__ float group_sum(float x) {
-#pragma unroll
-  for (int o = L / 2; o > 0; o /= 2) x += __shfl_xor_sync(0xffffffffu, x, o);
-  return x;
-}
-
-// The lane's 2 VEC values of a row as VEC pairs: value e of the first 16 bytes pairs with value e of the
-// second (half-split), or neighbours pair, those of the second 16 bytes after those of the first
-// (interleaved). first(j), second(j): where pair j's two values are.
-template <int VEC, bool INTERLEAVED>
-struct Pairs {
-  static __device__ __forceinline__ constexpr int first(int j) { return INTERLEAVED ? 2 * j : j; }
-  static __device__ __forceinline__ constexpr int second(int j) { return INTERLEAVED ? 2 * j + 1 : VEC + j; }
-};
 
 // One tensor's items: tokens x chunks of HB heads, in memory order (heads first where a token's heads lie
 // next to each other).
@@ -135,36 +59,9 @@ __device__ __forceinline__ Item rope_item(const RopeArgs& a, const RopeTensor& t
   return it;
 }
 
-// The cosines (or sines) of the lane's VEC pairs, from a row of their table.
-template <int D, int VEC, bool INTERLEAVED>
-__device__ __forceinline__ void load_angles(const float* row, int col, float* x) {
-  if constexpr (INTERLEAVED) {
-    load_floats<VEC / 2>(row + col / 2, x);
-    load_floats<VEC / 2>(row + D / 4 + col / 2, x + VEC / 2);
-  } else {
-    load_floats<VEC>(row + col, x);
-  }
-}
-
-// Which axis each of the lane's VEC pairs turns by (2 bits a pair from bit 0 on), and the set of those axes (from
-// bit 16 on).
-template <int D, int VEC, bool INTERLEAVED>
-__device__ __forceinline__ uint32_t lane_axes(const RopeArgs& a, int col) {
-  uint32_t x = 0;
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) {
-    const int pair = !INTERLEAVED ? col + j : j < VEC / 2 ? col / 2 + j : D / 4 + col / 2 + j - VEC / 2;
-    const uint32_t axis = (a.axes[pair / 16] >> (2 * (pair % 16))) & 3u;
-    x |= axis << (2 * j) | 0x10000u << axis;
-  }
-  return x;
-}
-
-template <typename T, int D, bool INTERLEAVED, int HB, bool BACKWARD, RopeForm FORM>
+template <typename T, int D, bool INTERLEAVED, int HB, bool BACKWARD>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 2) norm_rope_kernel(const RopeArgs a) {
   constexpr int VEC = kVec<T>, L = D / (2 * VEC), GROUPS = kThreads / L;
-  constexpr bool NORM = FORM != kAxes;
-  static_assert(NORM || !BACKWARD, "a rotation alone is turned back by the forward kernel");
   using P = Pairs<VEC, INTERLEAVED>;
   const int which = int(blockIdx.x) < a.t[0].blocks ? 0 : 1;  // the CTA's tensor
   const RopeTensor& t = a.t[which];
@@ -172,17 +69,13 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 2) norm_rope_ke
   const int c = threadIdx.x % L;
   const int col = c * VEC;  // and D / 2 + col
   float w[2 * VEC];
-  if constexpr (NORM) {
-    if (a.w_f32) {
-      load_floats<VEC>(static_cast<const float*>(t.w) + col, w);
-      load_floats<VEC>(static_cast<const float*>(t.w) + D / 2 + col, w + VEC);
-    } else {
-      load16(static_cast<const T*>(t.w) + col, w);
-      load16(static_cast<const T*>(t.w) + D / 2 + col, w + VEC);
-    }
+  if (a.w_f32) {
+    load_floats<VEC>(static_cast<const float*>(t.w) + col, w);
+    load_floats<VEC>(static_cast<const float*>(t.w) + D / 2 + col, w + VEC);
+  } else {
+    load16(static_cast<const T*>(t.w) + col, w);
+    load16(static_cast<const T*>(t.w) + D / 2 + col, w + VEC);
   }
-  uint32_t axes = 0;
-  if constexpr (FORM != kOnePosition) axes = lane_axes<D, VEC, INTERLEAVED>(a, col);
   float dw[2 * VEC];
 #pragma unroll
   for (int e = 0; e < 2 * VEC; ++e) dw[e] = 0.f;
@@ -192,87 +85,56 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 2) norm_rope_ke
     const int item = base + int(threadIdx.x) / L;
     const bool any = item < t.items;
     const Item it = rope_item(a, t, HB, any ? item : 0);
-    // All of the item's loads first, as they come: they are what takes time. (On several axes also before the
-    // positions, which the tables' loads wait for.)
-    uint4 rx[HB][2], rdy[BACKWARD ? HB : 1][2];
-    auto load_rows = [&] {
-#pragma unroll
-      for (int i = 0; i < HB; ++i) {
-        const bool row = any && it.h0 + i < t.H;
-        const int64_t h = row ? it.h0 + i : 0;
-        const T* px = static_cast<const T*>(t.px) + it.z * t.x.z + h * t.x.h + it.n * t.x.n + col;
-        rx[i][0] = load_raw(px);
-        rx[i][1] = load_raw(px + D / 2);
-        if constexpr (BACKWARD) {
-          const T* pd = static_cast<const T*>(t.pdy) + it.z * t.dy.z + h * t.dy.h + it.n * t.dy.n + col;
-          rdy[i][0] = load_raw(pd);
-          rdy[i][1] = load_raw(pd + D / 2);
-        }
-      }
-    };
-    if (FORM != kOnePosition) load_rows();
+    const int pos = a.positions ? a.positions[it.z * a.pos_z + it.n * a.pos_n] : it.n;
+    const bool in_table = pos >= 0 && pos < a.P;
     float cs[VEC], sn[VEC];
-    bool in_table = true;
-    if constexpr (FORM == kOnePosition) {
-      const int pos = a.positions ? a.positions[it.z * a.pos_z + it.n * a.pos_n] : it.n;
-      in_table = pos >= 0 && pos < a.P;
-      const int64_t at = int64_t(in_table ? pos : 0) * (D / 2);
-      load_angles<D, VEC, INTERLEAVED>(a.cos + at, col, cs);
-      load_angles<D, VEC, INTERLEAVED>(a.sin + at, col, sn);
+    const float* ct = a.cos + int64_t(in_table ? pos : 0) * (D / 2);
+    const float* st = a.sin + int64_t(in_table ? pos : 0) * (D / 2);
+    if constexpr (INTERLEAVED) {
+      load_floats<VEC / 2>(ct + col / 2, cs);
+      load_floats<VEC / 2>(ct + D / 4 + col / 2, cs + VEC / 2);
+      load_floats<VEC / 2>(st + col / 2, sn);
+      load_floats<VEC / 2>(st + D / 4 + col / 2, sn + VEC / 2);
     } else {
-      int pos[kRopeAxes];
-#pragma unroll
-      for (int x = 0; x < kRopeAxes; ++x) {  // all of them, whichever axes the lane's pairs use: a row is NaN as a whole
-        pos[x] = x < a.A ? a.positions[x * a.pos_a + it.z * a.pos_z + it.n * a.pos_n] : 0;
-        in_table = in_table && pos[x] >= 0 && pos[x] < a.P;
-      }
-      // A row of each axis that some pair of the lane uses, 16 bytes at a time, and of it what those pairs need.
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) cs[j] = sn[j] = 0.f;
-#pragma unroll
-      for (int x = 0; x < kRopeAxes; ++x) {
-        if ((axes & (0x10000u << x)) == 0u) continue;
-        const int64_t at = int64_t(in_table ? pos[x] : 0) * (D / 2);
-        float c4[VEC], s4[VEC];
-        load_angles<D, VEC, INTERLEAVED>(a.cos + at, col, c4);
-        load_angles<D, VEC, INTERLEAVED>(a.sin + at, col, s4);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const bool mine = ((axes >> (2 * j)) & 3u) == uint32_t(x);
-          cs[j] = mine ? c4[j] : cs[j];
-          sn[j] = mine ? s4[j] : sn[j];
-        }
-      }
-      if (FORM == kAxes && a.back) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) sn[j] = -sn[j];
-      }
+      load_floats<VEC>(ct + col, cs);
+      load_floats<VEC>(st + col, sn);
     }
     if (!in_table && any) {  // no rotation exists: the rows become NaN, and the status word says why
 #pragma unroll
       for (int j = 0; j < VEC; ++j) cs[j] = sn[j] = __int_as_float(0x7fffffff);
       if (c == 0) atomicOr(a.status, kStatusIndexRange);
     }
-    if (FORM == kOnePosition) load_rows();
+    // All of the item's loads first, as they come: they are what takes time.
+    uint4 rx[HB][2], rdy[BACKWARD ? HB : 1][2];
+#pragma unroll
+    for (int i = 0; i < HB; ++i) {
+      const bool row = any && it.h0 + i < t.H;
+      const int64_t h = row ? it.h0 + i : 0;
+      const T* px = static_cast<const T*>(t.px) + it.z * t.x.z + h * t.x.h + it.n * t.x.n + col;
+      rx[i][0] = load_raw(px);
+      rx[i][1] = load_raw(px + D / 2);
+      if constexpr (BACKWARD) {
+        const T* pd = static_cast<const T*>(t.pdy) + it.z * t.dy.z + h * t.dy.h + it.n * t.dy.n + col;
+        rdy[i][0] = load_raw(pd);
+        rdy[i][1] = load_raw(pd + D / 2);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < HB; ++i) {
       const bool row = any && it.h0 + i < t.H;
       float x[2 * VEC];
       unpack16<T>(rx[i][0], x);
       unpack16<T>(rx[i][1], x + VEC);
-      float r = 1.f;
-      if constexpr (NORM) {
-        float sum = 0.f;
+      float sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < 2 * VEC; ++e) sum = fmaf(x[e], x[e], sum);
-        r = rsqrtf(group_sum<L>(sum) * (1.f / D) + a.eps);
-      }
+      for (int e = 0; e < 2 * VEC; ++e) sum = fmaf(x[e], x[e], sum);
+      const float r = rsqrtf(group_sum<L>(sum) * (1.f / D) + a.eps);
       float out[2 * VEC];
       if constexpr (!BACKWARD) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const int f = P::first(j), s = P::second(j);
-          const float zf = NORM ? x[f] * r * w[f] : x[f], zs = NORM ? x[s] * r * w[s] : x[s];
+          const float zf = x[f] * r * w[f], zs = x[s] * r * w[s];
           out[f] = zf * cs[j] - zs * sn[j];
           out[s] = zs * cs[j] + zf * sn[j];
         }
@@ -346,7 +208,7 @@ __global__ void __launch_bounds__(kThreads) norm_rope_dw_kernel(const RopeArgs a
   }
 }
 
-template <typename T, int D, bool INTERLEAVED, bool BACKWARD, RopeForm FORM>
+template <typename T, int D, bool INTERLEAVED, bool BACKWARD>
 cudaError_t rope_impl(RopeArgs& a, cudaStream_t s) {
   constexpr int GROUPS = kThreads / (D / (2 * kVec<T>));
   const int sms = device_sm_count();
@@ -367,47 +229,38 @@ cudaError_t rope_impl(RopeArgs& a, cudaStream_t s) {
   const int grid = a.t[0].blocks + a.t[1].blocks;
   if (grid > 0) {
     if (many)
-      norm_rope_kernel<T, D, INTERLEAVED, MANY, BACKWARD, FORM><<<grid, kThreads, 0, s>>>(a);
+      norm_rope_kernel<T, D, INTERLEAVED, MANY, BACKWARD><<<grid, kThreads, 0, s>>>(a);
     else
-      norm_rope_kernel<T, D, INTERLEAVED, 1, BACKWARD, FORM><<<grid, kThreads, 0, s>>>(a);
+      norm_rope_kernel<T, D, INTERLEAVED, 1, BACKWARD><<<grid, kThreads, 0, s>>>(a);
   }
   if (BACKWARD) norm_rope_dw_kernel<T><<<dim3(D / kDwCols, 2), kThreads, 0, s>>>(a, D);
   return cudaGetLastError();
 }
 
-template <typename T, bool BACKWARD, RopeForm FORM>
+template <typename T, bool BACKWARD>
 cudaError_t rope_dispatch(int D, bool interleaved, RopeArgs& a, cudaStream_t s) {
-#define TATTN_ROPE_CASE(DD) \
-  case DD: return interleaved ? rope_impl<T, DD, true, BACKWARD, FORM>(a, s) : rope_impl<T, DD, false, BACKWARD, FORM>(a, s);
   switch (D) {
-    TATTN_ROPE_CASE(16)
-    TATTN_ROPE_CASE(32)
-    TATTN_ROPE_CASE(64)
-    TATTN_ROPE_CASE(128)
+    case 16: return interleaved ? rope_impl<T, 16, true, BACKWARD>(a, s) : rope_impl<T, 16, false, BACKWARD>(a, s);
+    case 32: return interleaved ? rope_impl<T, 32, true, BACKWARD>(a, s) : rope_impl<T, 32, false, BACKWARD>(a, s);
+    case 64: return interleaved ? rope_impl<T, 64, true, BACKWARD>(a, s) : rope_impl<T, 64, false, BACKWARD>(a, s);
+    case 128: return interleaved ? rope_impl<T, 128, true, BACKWARD>(a, s) : rope_impl<T, 128, false, BACKWARD>(a, s);
     default: return cudaErrorInvalidValue;
-  }
-#undef TATTN_ROPE_CASE
-}
-
-template <typename T>
-cudaError_t rope_form(int D, RopeForm form, bool interleaved, bool backward, RopeArgs& a, cudaStream_t s) {
-  switch (form) {
-    case kOnePosition:
-      return backward ? rope_dispatch<T, true, kOnePosition>(D, interleaved, a, s)
-                      : rope_dispatch<T, false, kOnePosition>(D, interleaved, a, s);
-    case kAxesNorm:
-      return backward ? rope_dispatch<T, true, kAxesNorm>(D, interleaved, a, s)
-                      : rope_dispatch<T, false, kAxesNorm>(D, interleaved, a, s);
-    default:
-      return rope_dispatch<T, false, kAxes>(D, interleaved, a, s);
   }
 }
 
 }  // namespace
 
-cudaError_t launch_norm_rope(int D, bool is_f16, RopeForm form, bool interleaved, bool backward, RopeArgs a, cudaStream_t s) {
-  return is_f16 ? rope_form<__half>(D, form, interleaved, backward, a, s)
-                : rope_form<float>(D, form, interleaved, backward, a, s);
+cudaError_t launch_norm_rope(int D, bool is_f16, bool interleaved, bool backward, RopeArgs a, cudaStream_t s) {
+  if (is_f16) return backward ? rope_dispatch<__half, true>(D, interleaved, a, s) : rope_dispatch<__half, false>(D, interleaved, a, s);
+  return backward ? rope_dispatch<float, true>(D, interleaved, a, s) : rope_dispatch<float, false>(D, interleaved, a, s);
+}
+
+cudaError_t launch_norm_rope_dw(bool is_f16, int D, const RopeArgs& a, cudaStream_t s) {
+  if (is_f16)
+    norm_rope_dw_kernel<__half><<<dim3(D / kDwCols, 2), kThreads, 0, s>>>(a, D);
+  else
+    norm_rope_dw_kernel<float><<<dim3(D / kDwCols, 2), kThreads, 0, s>>>(a, D);
+  return cudaGetLastError();
 }
 
 }  // namespace tattn
