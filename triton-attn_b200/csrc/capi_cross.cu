@@ -212,6 +212,17 @@ int64_t cross_part_bytes(int Z, int H, int Hk, int Nq, int Nk, int D, int dtype)
                            cross_split(Z, H, Hk, Nq, Nk, D, dtype));
 }
 
+// fp32: parts of the keys for dq, and where their sums stand behind the tiles' partials.
+int dq_parts(int Z, int H, int Nq, int Nk, int D) {
+  const int tile = window_f32_tile(D, (long long)Z * H, Nq);
+  return rows_splits(int64_t(Z) * H * ((Nq + tile - 1) / tile), (int64_t(Nk) + kWindowF32Block - 1) / kWindowF32Block,
+                     2 * device_sm_count(), 1, 1);
+}
+int64_t dq_part_bytes(int Z, int H, int Nq, int Nk, int D) {
+  const int parts = dq_parts(Z, H, Nq, Nk, D);
+  return parts > 1 ? int64_t(parts) * Z * H * Nq * D * 4 : 0;
+}
+
 }  // namespace
 
 extern "C" int64_t tattn_cross_bwd_workspace_bytes(int Z, int H, int Hk, int Nq, int Nk, int D, int dtype) {
@@ -219,10 +230,13 @@ extern "C" int64_t tattn_cross_bwd_workspace_bytes(int Z, int H, int Hk, int Nq,
   if (int64_t(Z) * H * Nq == 0) return 0;
   const int64_t dq = dtype == TATTN_F16 ? bwd_fused_workspace_bytes(Z, H, Nq, D) : 0;
   if (Nk == 0) return dq;
-  int64_t part = cross_part_bytes(Z, H, Hk, Nq, Nk, D, dtype);
+  auto parts = [&] {
+    return cross_part_bytes(Z, H, Hk, Nq, Nk, D, dtype) + (dtype == TATTN_F32 ? dq_part_bytes(Z, H, Nq, Nk, D) : 0);
+  };
+  int64_t part = parts();
   if (folds(H, Hk, Nq)) {
     fold(H, Hk, Nq);
-    part = std::max(part, cross_part_bytes(Z, H, Hk, Nq, Nk, D, dtype));
+    part = std::max(part, parts());
   }
   return dq + part;
 }
@@ -293,9 +307,11 @@ extern "C" int tattn_cross_bwd(const void* q, const void* k, const void* v, cons
   a.lengths = lengths;
   const int64_t parts = cross_part_bytes(Z, H, Hk, Nq, Nk, D, dtype);
   if (!half) {
-    if (parts > 0) {
+    a.dq_split = dq_parts(Z, H, Nq, Nk, D);
+    if (parts > 0 || a.dq_split > 1) {
       if (!workspace) return TATTN_ERR_INVALID_ARGUMENT;
-      a.part = static_cast<float*>(workspace);
+      a.part = static_cast<float*>(workspace);  // (a multiple of 16 bytes, then dq's)
+      a.dq_part = a.part + parts / 4;
     }
     rc = cuda_rc(launch_bwd_preprocess(D, false, a, s));
     return rc != TATTN_OK ? rc : cuda_rc(launch_rows_bwd_f32(D, a, s));

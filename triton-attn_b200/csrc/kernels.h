@@ -211,6 +211,10 @@ struct BwdArgs {
 // kMaskRows: a window (`win`, `split`) that shows every query every key, of which sequence z has the first lengths[z].
 struct RowsBwdArgs : BwdArgs {
   const int* lengths;  // [Z], or null: all
+  // fp32: the keys that dq sums over are cut into dq_split parts; more than one: their sums [dq_split, Z, H, N, D], to be
+  // added up.
+  int dq_split;
+  float* dq_part;
 };
 // The window that hides nothing.
 inline WindowArgs whole_window(int H, int Hk, int Nq, int Nk) { return WindowArgs{Hk, H / Hk, Nk, Nk, Nk + Nq, 0}; }

@@ -287,20 +287,27 @@ __global__ void __launch_bounds__(kThreads<D, T>) window_dq_f32_kernel(Bwd<ROWS>
   float *Qs = smem, *Os = Qs + T * kPitch<D>, *Vs = Os + T * kPitch<D>;
   float *Ks = Vs + TB * kPitch<D>, *Kn = Ks + TB * kPitch<D>;  // K's tile and the next one
   float *DSs = Kn + TB * kPitch<D>, *Ms = DSs + T * kPitchP, *Ds = Ms + T;
-  const int N = a.N, r0 = blockIdx.x * T;
+  const int N = a.N, tiles = (N + T - 1) / T, split = ROWS ? blockIdx.x / tiles : 0, r0 = (blockIdx.x - split * tiles) * T;
   const int64_t head = cta_head();
   if (head >= int64_t(a.Z) * a.H) return;
   const int zi = int(head / a.H), hi = int(head % a.H), hk = hi / a.win.group;
-  int Nk = a.win.Nk;
-  bool outside;
-  if constexpr (ROWS) Nk = held_keys(a.lengths, zi, Nk, &outside);
+  int Nk = a.win.Nk, k0, end;
+  if constexpr (ROWS) {
+    bool outside;
+    Nk = held_keys(a.lengths, zi, Nk, &outside);
+    const int64_t blocks = (Nk + TB - 1) / TB;
+    k0 = int(blocks * split / a.dq_split) * TB;
+    end = min(int(blocks * (split + 1) / a.dq_split) * TB, Nk);
+  } else {
+    k0 = next_keys(-TB, r0, a.win);
+    end = min(r0 + T + a.win.off, Nk);
+  }
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const float* k = static_cast<const float*>(a.k) + zi * a.sk.z + hk * a.sk.h;
   const float* v = static_cast<const float*>(a.v) + zi * a.sv.z + hk * a.sv.h;
   load_rows<D, T, TH>(Qs, static_cast<const float*>(a.q) + zi * a.sq.z + hi * a.sq.h, a.sq, r0, N);
   load_rows<D, T, TH>(Os, static_cast<const float*>(a.dout) + zi * a.sdo.z + hi * a.sdo.h, a.sdo, r0, N);
-  int k0 = ROWS ? 0 : next_keys(-TB, r0, a.win);
-  if (!ROWS || Nk > 0) {
+  if (!ROWS || k0 < end) {
     load_rows<D, TB, TH>(Ks, k, a.sk, k0, Nk);
     load_rows<D, TB, TH>(Vs, v, a.sv, k0, Nk);
   }
@@ -310,7 +317,6 @@ __global__ void __launch_bounds__(kThreads<D, T>) window_dq_f32_kernel(Bwd<ROWS>
     Ds[threadIdx.x] = row < N ? a.delta[head * N + row] : 0.f;
   }
   float acc[R][D / 16] = {};
-  const int end = ROWS ? Nk : min(r0 + T + a.win.off, Nk);
   for (int next; k0 < end; k0 = next) {
     cp_async_wait_all();
     __syncthreads();  // K and V are here, and K's last tile has been read
@@ -335,6 +341,8 @@ __global__ void __launch_bounds__(kThreads<D, T>) window_dq_f32_kernel(Bwd<ROWS>
     const int row = r0 + R * ty + i;
     if (row >= N) continue;
     float* dq = static_cast<float*>(a.dq) + (head * N + row) * D + D / 16 * tx;
+    if constexpr (ROWS)
+      if (a.dq_split > 1) dq = a.dq_part + ((int64_t(split) * a.Z * a.H + head) * N + row) * D + D / 16 * tx;
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) dq[e] = acc[i][e] * a.sm_scale;
   }
@@ -460,6 +468,18 @@ __global__ void __launch_bounds__(kJoinThreads) window_join_f32_kernel(BwdArgs a
   out[(head * a.win.Nk + key) * D + i % D] = which ? sum * a.sm_scale : sum;
 }
 
+// dq of rows whose keys were cut into parts: the parts' sums, in their order.
+__global__ void __launch_bounds__(kJoinThreads) rows_dq_join_f32_kernel(const float4* part, float4* dq, int64_t units, int split) {
+  const int64_t i = int64_t(blockIdx.x) * kJoinThreads + threadIdx.x;
+  if (i >= units) return;
+  float4 sum = part[i];
+  for (int s = 1; s < split; ++s) {
+    const float4 x = part[s * units + i];
+    sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
+  }
+  dq[i] = sum;
+}
+
 template <typename Kernel, typename... Args>
 cudaError_t launch(Kernel kernel, int tiles, long long heads, int threads, int floats, cudaStream_t s, const Args&... args) {
   const long long y = heads < 65535 ? heads : 65535, z = (heads + y - 1) / y;
@@ -491,8 +511,18 @@ cudaError_t dkdv_impl(const Bwd<ROWS>& a, cudaStream_t s) {
 }
 template <int D, int T, bool ROWS>
 cudaError_t dq_impl(const Bwd<ROWS>& a, cudaStream_t s) {
-  return launch(window_dq_f32_kernel<D, T, ROWS>, (a.N + T - 1) / T, (long long)a.Z * a.H, kThreads<D, T>,
-                (2 * T + 3 * TB) * kPitch<D> + T * kPitchP + 2 * T, s, a);
+  int split = 1;
+  if constexpr (ROWS) split = a.dq_split;
+  const cudaError_t e = launch(window_dq_f32_kernel<D, T, ROWS>, (a.N + T - 1) / T * split, (long long)a.Z * a.H, kThreads<D, T>,
+                               (2 * T + 3 * TB) * kPitch<D> + T * kPitchP + 2 * T, s, a);
+  if constexpr (ROWS) {
+    if (e != cudaSuccess || split == 1) return e;
+    const int64_t units = int64_t(a.Z) * a.H * a.N * D / 4;
+    rows_dq_join_f32_kernel<<<unsigned((units + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, s>>>(
+        reinterpret_cast<const float4*>(a.dq_part), static_cast<float4*>(a.dq), units, split);
+    return cudaGetLastError();
+  }
+  return e;
 }
 
 template <int D>
