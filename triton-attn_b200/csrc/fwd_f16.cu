@@ -680,7 +680,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
       cp_async_wait_all();
       fence_proxy_async_smem();
       mbar_arrive(bar_q);
-      let_next_kernel_start();
+      if (args.rows.part != nullptr) let_next_kernel_start();  // the one that joins the parts, or comes before that
       if (COPIES > 1 && n > 0) {  // the other copies' columns of P are zeros throughout
         uint32_t zero[BN / 2];
 #pragma unroll

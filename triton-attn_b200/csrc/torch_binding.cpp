@@ -642,9 +642,12 @@ Tensor cross_attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, con
   const std::optional<Tensor> lengths = check_lengths("lengths", lengths0, q0, q0.size(0));
   refuse_forward_mode("cross_attention", {&q0, &k0, &v0});
   require_cuda(q0);
+  const double scale = scale_of(sm_scale, q0);
+  const bool grad = wants_grad({&q0, &k0, &v0});
+  if (!grad && q0.size(2) == 1)  // single tokens need no TMA, so an expanded batch of states is read as it is
+    return std::get<0>(cross_forward(rows16(q0), rows16(k0), rows16(v0), lengths, scale, false));
   const Tensor q = rows_ready(q0), k = rows_ready(k0), v = rows_ready(v0);
-  const double scale = scale_of(sm_scale, q);
-  if (!wants_grad({&q0, &k0, &v0})) return std::get<0>(cross_forward(q, k, v, lengths, scale, false));
+  if (!grad) return std::get<0>(cross_forward(q, k, v, lengths, scale, false));
   return CrossAttention::apply(q, k, v, lengths, scale);
 }
 

@@ -192,7 +192,8 @@ __global__ void __launch_bounds__(kThreads<D, T>) window_fwd_f32_kernel(const fl
     for (int e = 0; e < D / 16; ++e) acc[i][e] = 0.f;
   }
   const bool any = k0 < end;
-  if (ROWS) let_next_kernel_start();
+  if constexpr (ROWS)
+    if (a.rows.part != nullptr) let_next_kernel_start();  // the one that joins the parts, or comes before that
   for (int next; k0 < end; k0 = next) {
     cp_async_wait_all();
     __syncthreads();  // K is here, and V's last tile has been read
