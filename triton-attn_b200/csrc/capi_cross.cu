@@ -350,10 +350,11 @@ bool prefix_fits(int prompts, int samples, int H, int Hk, int P) {
   return double(prompts) * samples * H < 5e8 && double(prompts) * Hk * (P / 128 + 1) < 1e7;
 }
 DecodeArgs own_args(int prompts, int samples, int H, int Hk, int C) { return token_args(prompts * samples, H, Hk, 1, C); }
-// Parts of the sequences' own tokens: as for a cache, but of 256 tokens at least, as the prefix's parts are joined anyhow
-// (16 samples of up to 256 tokens: 11.4 us with 2 parts, 10.6 with one).
+// Parts of the sequences' own tokens: as for a cache, but in fp16 of 256 tokens at least, as the prefix's parts are joined
+// anyhow (16 samples of up to 256 tokens: 11.4 us with 2 parts, 10.6 with one).
 int own_parts(const DecodeArgs& a, int D, int dtype) {
-  return std::min(decode_splits(a, D, cache_of(dtype)), std::max(1, a.C / 256));
+  const int n = decode_splits(a, D, cache_of(dtype));
+  return dtype == TATTN_F32 ? n : std::min(n, std::max(1, a.C / 256));
 }
 
 }  // namespace
