@@ -23,31 +23,51 @@ __global__ void __launch_bounds__(kThreads) rows_join_kernel(const JoinArgs a) {
   const int head = int(index / a.N), row = int(index % a.N), z = head / a.H, h = head % a.H;
   const int outer = row / a.inner, in = row - outer * a.inner;
   const int64_t rows[2] = {index, z * a.other.z + h * a.other.h + outer * a.other.outer + in * a.other.in};
-  const int t = threadIdx.x % V, p = threadIdx.x / V;
+  const int t = threadIdx.x % V, p = threadIdx.x / V, total = a.n[0] + a.n[1];
+  // Part s of both lists: its maximum and sum, and this thread's dims.
+  auto part_ml = [&](int s) {
+    const bool second = s >= a.n[0];
+    const int64_t at = second ? rows[1] * a.n[1] + s - a.n[0] : rows[0] * a.n[0] + s;
+    return __ldcg(reinterpret_cast<const float2*>(a.part_ml[second]) + at);
+  };
+  auto part_row = [&](int s) {
+    const bool second = s >= a.n[0];
+    const int64_t at = second ? rows[1] * a.n[1] + s - a.n[0] : rows[0] * a.n[0] + s;
+    return __ldcg(reinterpret_cast<const float4*>(a.part[second]) + at * V + t);
+  };
   wait_for_last_kernel();
-  float m = -INFINITY;
+  // The thread's first parts on their way before the maximum is known. (What stands in the row of a part without keys is
+  // read and not used.)
+  constexpr int AHEAD = 4;
+  float2 c[AHEAD];
+  float4 v[AHEAD];
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
-    for (int s = threadIdx.x % 32; s < a.n[x]; s += 32) m = max_or_nan(m, a.part_ml[x][(rows[x] * a.n[x] + s) * 2]);
+  for (int i = 0; i < AHEAD; ++i) {
+    const int s = p + i * LANES;
+    c[i] = make_float2(-INFINITY, 0.f);
+    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (s < total) {
+      c[i] = part_ml(s);
+      v[i] = part_row(s);
+    }
+  }
+  float m = -INFINITY;
+  for (int s = threadIdx.x % 32; s < total; s += 32) m = max_or_nan(m, part_ml(s).x);
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) m = max_or_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float use = m == -INFINITY ? 0.f : m;
   float l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](const float2& c, const float4& v) {
+    if (c.x == -INFINITY) return;
+    const float f = exp2f(c.x - use);
+    l = fmaf(f, c.y, l);
+    acc = make_float4(fmaf(f, v.x, acc.x), fmaf(f, v.y, acc.y), fmaf(f, v.z, acc.z), fmaf(f, v.w, acc.w));
+  };
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const float2* ml = reinterpret_cast<const float2*>(a.part_ml[x]) + rows[x] * a.n[x];
-    const float4* o = reinterpret_cast<const float4*>(a.part[x]) + rows[x] * a.n[x] * V + t;
+  for (int i = 0; i < AHEAD; ++i) add(c[i], v[i]);
 #pragma unroll 4
-    for (int s = p; s < a.n[x]; s += LANES) {
-      const float2 c = ml[s];
-      if (c.x == -INFINITY) continue;  // a part without keys has written no row
-      const float4 v = o[int64_t(s) * V];
-      const float f = exp2f(c.x - use);
-      l = fmaf(f, c.y, l);
-      acc = make_float4(fmaf(f, v.x, acc.x), fmaf(f, v.y, acc.y), fmaf(f, v.z, acc.z), fmaf(f, v.w, acc.w));
-    }
-  }
+  for (int s = p + AHEAD * LANES; s < total; s += LANES) add(part_ml(s), part_row(s));
   so[p][t] = acc;
   if (t == 0) sl[p] = l;
   __syncthreads();
