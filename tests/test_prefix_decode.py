@@ -186,6 +186,8 @@ def test_long_ones_are_decode_attention_over_the_joined_cache(gpu, d, dtype) -> 
 def test_without_a_prefix_or_own_tokens(gpu, dtype) -> None:
     _check(2, 3, 4, 2, 0, 40, 64, dtype)
     _check(2, 3, 4, 2, 40, 0, 64, dtype)
+    _check(2, 3, 3, 1, 0, 40, 64, dtype)
+    _check(1, 3, 3, 1, 40, 0, 64, dtype)
     q, pk, pv, k, v = _inputs(2, 3, 4, 2, 0, 0, 64, dtype)
     assert not bool(prefix_decode_attention(q, pk, pv, k, v, _int([0] * 6)).any())
     q, pk, pv, k, v = (t[:0] for t in _inputs(2, 3, 4, 2, 7, 5, 64, dtype))
