@@ -176,6 +176,17 @@ def test_many_tiles(gpu, d) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d", [32, 128])
+@pytest.mark.parametrize("b, h, hk, nq, nk", [(1, 1, 1, 2000, 100), (2, 8, 2, 300, 1300), (70, 2, 1, 130, 400), (40, 4, 4, 260, 250)])
+def test_tiles_cut_between_ctas(gpu, b, h, hk, nq, nk, d) -> None:
+    """fp16 backward: a last round of few key tiles is cut into runs of pairs; batches of more than 32 sequences, with and
+    without lengths (every third none)."""
+    inputs = _qkv(b, h, hk, nq, nk, d, torch.float16, 2)
+    _compare(*inputs, None)
+    _compare(*inputs, _int(*[(i * 53) % (nk + 1) if i % 3 else 0 for i in range(1, b + 1)]))
+
+
+@pytest.mark.gpu
 @F16_F32
 @pytest.mark.parametrize("nq", [1, 4, 300])
 @pytest.mark.parametrize("scale", [0.3, -0.2, 0.0])
