@@ -568,15 +568,17 @@ Tensor rows_ready(const Tensor& t) {
   return t.scalar_type() == at::kHalf ? tma_ready(r) : r;
 }
 
-// (O like q, M fp32 [Z, H, Nq], what rounding took off an fp16 O) of checked tensors that rows_ready gave; the last two
-// for a backward pass only.
-std::tuple<Tensor, Tensor, Tensor> cross_forward(const Tensor& q, const Tensor& k, const Tensor& v,
-                                                 const std::optional<Tensor>& lengths, double scale, bool backward) {
-  Tensor o = like(q), m, rest;
-  if (backward) {
-    m = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
-    if (q.scalar_type() == at::kHalf) rest = at::empty(q.sizes(), q.options().dtype(at::kByte), at::MemoryFormat::Contiguous);
-  }
+// fp32 values for each of q's rows (M, or delta), in bytes that leave what stands behind them aligned.
+int64_t row_bytes(const Tensor& q) { return (q.size(0) * q.size(1) * q.size(2) * 4 + 15) / 16 * 16; }
+
+// O like q of checked tensors that rows_ready gave and, for a backward pass, M (fp32 [Z, H, Nq]) with, behind it, what
+// rounding took off an fp16 O (else an undefined tensor).
+std::tuple<Tensor, Tensor> cross_forward(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& lengths,
+                                         double scale, bool backward) {
+  const bool half = q.scalar_type() == at::kHalf;
+  Tensor o = like(q), kept;
+  if (backward) kept = bytes(row_bytes(q) + (half ? q.numel() : 0), q);
+  uint8_t* m = backward ? kept.data_ptr<uint8_t>() : nullptr;
   const int z = dim(q, 0), h = dim(q, 1), hk = dim(k, 1), n = dim(q, 2), nk = dim(k, 2), d = dim(q, 3);
   Strides st;
   st.add(q);
@@ -588,17 +590,17 @@ std::tuple<Tensor, Tensor, Tensor> cross_forward(const Tensor& q, const Tensor& 
   const Tensor ws = size > 0 ? bytes(size, q) : Tensor();
   check_status("tattn_cross_fwd",
                tattn_cross_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), static_cast<const int32_t*>(ptr(lengths)), o.data_ptr(),
-                               backward ? m.data_ptr<float>() : nullptr, rest.defined() ? rest.data_ptr() : nullptr,
+                               reinterpret_cast<float*>(m), backward && half ? m + row_bytes(q) : nullptr,
                                size > 0 ? ws.data_ptr() : nullptr, st.s, z, h, hk, n, nk, d, code(q), float(scale), stream_of(q)));
-  return {o, m, rest};
+  return {o, kept};
 }
 
 struct CrossAttention : torch::autograd::Function<CrossAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
                         const std::optional<Tensor>& lengths, double scale) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [o, m, rest] = cross_forward(q, k, v, lengths, scale, true);
-    ctx->save_for_backward({q, k, v, lengths.has_value() ? *lengths : Tensor(), o, m, rest});
+    auto [o, kept] = cross_forward(q, k, v, lengths, scale, true);
+    ctx->save_for_backward({q, k, v, lengths.has_value() ? *lengths : Tensor(), o, kept});
     ctx->saved_data["scale"] = scale;
     return o;
   }
@@ -607,10 +609,10 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const variable_list s = ctx->get_saved_variables();
-      const Tensor &q = s[0], &k = s[1], &v = s[2], &lengths = s[3], &m = s[5], &rest = s[6];
+      const Tensor &q = s[0], &k = s[1], &v = s[2], &lengths = s[3], &kept = s[5];
+      const bool half = q.scalar_type() == at::kHalf;
       const Tensor o = rows_ready(s[4]), g = rows_ready(grads[0]);
       const int z = dim(q, 0), h = dim(q, 1), hk = dim(k, 1), n = dim(q, 2), nk = dim(k, 2), d = dim(q, 3);
-      Tensor delta = at::empty({z, h, n}, q.options().dtype(at::kFloat));
       Tensor dq = at::empty({z, h, n, d}, q.options()), dk = at::empty({z, hk, nk, d}, q.options());
       Tensor dv = at::empty({z, hk, nk, d}, q.options());
       Strides st;
@@ -621,13 +623,13 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
       st.add(g);
       const c10::cuda::CUDAGuard guard(q.device());
       const int64_t size = std::max<int64_t>(0, tattn_cross_bwd_workspace_bytes(z, h, hk, n, nk, d, code(q)));
-      const Tensor ws = size > 0 ? bytes(size, q) : Tensor();
+      const Tensor ws = bytes(row_bytes(q) + size, q);  // delta, then the workspace
+      uint8_t *m = kept.data_ptr<uint8_t>(), *delta = ws.data_ptr<uint8_t>();
       check_status("tattn_cross_bwd",
                    tattn_cross_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), lengths.defined() ? lengths.data_ptr<int32_t>() : nullptr,
-                                   o.data_ptr(), g.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), m.data_ptr<float>(),
-                                   rest.defined() ? rest.data_ptr() : nullptr, delta.data_ptr<float>(),
-                                   size > 0 ? ws.data_ptr() : nullptr, st.s, z, h, hk, n, nk, d, code(q),
-                                   float(ctx->saved_data["scale"].toDouble()), stream_of(q)));
+                                   o.data_ptr(), g.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), reinterpret_cast<float*>(m),
+                                   half ? m + row_bytes(q) : nullptr, reinterpret_cast<float*>(delta), delta + row_bytes(q), st.s, z,
+                                   h, hk, n, nk, d, code(q), float(ctx->saved_data["scale"].toDouble()), stream_of(q)));
       out[0] = dq;
       out[1] = dk;
       out[2] = dv;
