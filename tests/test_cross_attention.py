@@ -303,6 +303,21 @@ def test_layouts_that_need_a_copy(gpu, nq, dtype) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("nq, nk", [(1, 1), (200, 1), (300, 129), (40, 2000)])
+def test_one_key_has_no_gradient_through_its_score(gpu, nq, nk, d, dtype) -> None:
+    """Its weight is 1 whatever its score: exact zeros for Q and K."""
+    q, k, v, do = _qkv(3, 4, 2, nq, nk, d, dtype, seed=nq)
+    lengths = torch.tensor([1, nk, 1], dtype=torch.int32, device="cuda")
+    out = cross_attention(q.requires_grad_(), k.requires_grad_(), v.requires_grad_(), lengths)
+    out.backward(do)
+    for z in (0, 2):
+        assert not q.grad[z].any() and not k.grad[z].any()
+    assert bool(q.grad[1].any()) == (nk > 1)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("d", [64, 128])
 def test_equal_lengths_are_attention(gpu, d) -> None:
     """fp16: the same mathematics in another kernel; both are within the bound of the definition."""

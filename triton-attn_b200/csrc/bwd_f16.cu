@@ -2508,6 +2508,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int x = 0; x < H; ++x) dp[x] = r < u.len ? dp[x] : 0u;
             if (c == 0 && w == 0 && r >= u.len) clear_key_row<D>(sK + (it & 1) * C::T_KEY, r);  // (fenced below)
+            if (u.len == 1 && u.kt == 0) {  // one key weighs 1 whatever its score: dP - delta is 0, but for rounding
+#pragma unroll
+              for (int x = 0; x < H; ++x) dp[x] = __float_as_uint(0.f * __uint_as_float(dp[x]));
+            }
           }
         } else if (WINDOW) {  // a key is seen from its own position on, for one window unless it is a sink
           const int p0 = q0 + args.win.off;

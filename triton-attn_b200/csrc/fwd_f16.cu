@@ -27,6 +27,13 @@
 // CTA 201 us, one 165; 131 with hidden scores made -infinity ahead of the code that all blocks share, and 124 with
 // the row blocks of short windows last (0.5 PFLOP/s). H16 Hk4 D64, 4096 queries of 16384 tokens, window 4096: 115
 // us, 0.6 PFLOP/s. What bounds it then is each tile's chain of S, exponentials and P V.
+// kMaskRows is attention to a sequence's first keys, lengths on the device, of query rows that need not be one tensor's
+// tokens: the queries of all heads that share a key/value head, or of all samples that share a prompt, are one matrix
+// (RowMap), so that a key block is read once for 128 or 256 of them. Calls with few rows cut the keys into parts, a CTA
+// each, whose unnormalised rows rows_join.cu joins. B2 H16 Hk4, 2,000 queries of 6,404 keys, D128: 222 us, 0.89 PFLOP/s,
+// 256 CTAs for 148 SMs; B2 H16 N4096 D64: 197 us, 0.70 (the same as `attention`: 219): the softmax warps. 64 queries of 16,384
+// keys, H16 D64 (67 MB): 24.4 us, of which the keys' way at 5.8 TB/s takes 11.5, the first loads and the epilogue 3 each, the
+// join 4; there BN is 64 and each row has two (four) copies in the tile whose threads share a block's exponentials.
 // The running max is rescaled lazily: O (in TMEM) and l are only corrected when a row's max grows by
 // more than kRescaleThreshold (log2 units); P values stay below 2^kRescaleThreshold, exact in fp16.
 // A NaN among a row's visible scores makes its maximum NaN, and with it M and O (the exponentials on the FMA pipe clamp,

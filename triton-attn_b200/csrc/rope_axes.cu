@@ -12,6 +12,10 @@
 // all of one axis as 16-byte loads, else pair by pair (whole rows of every axis with a choice among them took 1.5 times the
 // instructions). What is left is instructions: arithmetic on pairs of floats (fma.rn.f32x2), the forward's weight times
 // the angle once for an item's heads, divisions by multiplication.
+// Measured (B200, B4 N4096, passes over three sets of tensors, axes in turn over the pairs, with norms): fp16, 16 and 4 heads
+// of 128: forward 40 us, 4.2 TB/s, backward 62 us, 4.1 TB/s (dw's second kernel, 5 us, among them); issue slots are 50 % busy
+// with 16 warps an SM, the rest is loads that they wait for (with 2 heads an item and 3 CTAs an SM 47 us; backward with one
+// head and 3 CTAs 69). fp32, 16 and 16 heads of 64: 47 us, 5.7 TB/s, and 74 us, 5.5 TB/s. The rotation alone: 37 us (fp16).
 // dw: each CTA adds its rows' terms in registers and writes one partial; norm_rope.cu's second kernel sums them in order.
 #include <cuda_fp16.h>
 

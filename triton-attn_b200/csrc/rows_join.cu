@@ -1,7 +1,9 @@
 // Joins the parts of query rows whose keys were cut into several (RowsArgs): O = sum of 2^(m_i - m) O_i over sum of
 // 2^(m_i - m) l_i, m the largest of the parts' maxima.
 //
-// A CTA takes one row, its threads 4 dims of every so many-th part. The parts were just written, so they come from L2.
+// A CTA takes one row, its threads 4 dims of every so many-th part. The parts were just written, so they come from L2; what
+// bounds it is its launch and the loads' latency, so it is launched while the last parts are made, and a thread's first
+// loads do not wait for the maximum (B200, 1,024 rows: 18 parts of 64 dims 4 us, 39 parts of 128 9 us in a call).
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <math.h>
