@@ -174,7 +174,8 @@ __host__ __device__ inline WindowUnit window_unit(const WindowSplit& s, const Wi
   return u;
 }
 
-// Launched to overlap with the kernel that writes the parts (overlapping_launch). Parts of rows that are to be joined: of every row up to two lists of unnormalised parts with their maxima and sums.
+// Parts of rows that are to be joined: of every row up to two lists of unnormalised parts with their maxima and sums.
+// The join is launched to overlap with the kernel that writes them (overlapping_launch).
 struct JoinArgs {
   const float *part[2], *part_ml[2];  // [rows, n, D] and [rows, n, 2]
   int n[2];

@@ -81,7 +81,7 @@ Tensor like(const Tensor& t) {
 }
 
 struct Strides {
-  int64_t s[26];
+  int64_t s[27];  // the longest list, of tattn_qk_rope_axes_bwd
   int n = 0;
   void add(const Tensor& t) {
     for (int64_t x : t.strides()) s[n++] = x;
