@@ -1,7 +1,9 @@
 // Sliding-window attention with sinks for fp32 on CUDA cores: forward, dK/dV and dQ. The same kernels with ROWS are
 // attention to the first lengths[z] keys of a sequence (kMaskRows); their forward and dQ may take a part of the keys, so that
 // few rows still give every SM something to do (B3 H5, 200 queries of up to 777 keys, D64: dQ 62 -> 40 us; 40 queries of
-// 5,000 keys, H4: the backward 399 -> 69). 16 rows of 4,000 keys, 16 heads of 64: 20 us, shared memory at 60 %.
+// 5,000 keys, H4: the backward 399 -> 69). Up to 16 rows, a sampled prompt's, take T = 16 (R = 2: half the products
+// and less of shared memory; R = 4 with half the threads is between): 16 rows of 4,000 keys, B4 Hk4: D32 15.5 -> 12.6 us, D64
+// 25.4 -> 19.6, D128 54.6 -> 49.3 with the join; 16 rows of 500 keys, B32 H16: 71 -> 56 at D64, 165 -> 141 at D128.
 //
 // The mathematics is the fp16 kernels' (base-2 online softmax, M = m + log2 l, P rebuilt from M in the
 // backward) with every product and sum in fp32: tcgen05 has no fp32 MMA, and fp32 calls are held to fp32
@@ -35,8 +37,8 @@ namespace tattn {
 namespace {
 
 constexpr int TB = kWindowF32Block;  // columns of a tile: the rows that are loaded one block after another
-template <int D, int T>              // T: rows of a tile, 64 or 32
-constexpr int kRows = T == 64 && (D == 32 || D == 64) ? 8 : 4;  // a thread's
+template <int D, int T>              // T: rows of a tile, 64, 32 or 16
+constexpr int kRows = T == 16 ? 2 : T == 64 && (D == 32 || D == 64) ? 8 : 4;  // a thread's
 template <int D, int T>
 constexpr int kThreads = 16 * T / kRows<D, T>;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -544,8 +546,10 @@ cudaError_t rows_impl(const float* k, const float* v, const Strides4& sk, const 
 }
 template <int D>
 cudaError_t rows_tiles(const float* k, const float* v, const Strides4& sk, const Strides4& sv, const RowsFwdArgs& a, cudaStream_t s) {
-  if constexpr (D > 16)
+  if constexpr (D > 16) {
     if (window_f32_tile(D, (long long)a.Z * a.H, a.N) == 64) return rows_impl<D, 64>(k, v, sk, sv, a, s);
+    if (a.N <= 16) return rows_impl<D, 16>(k, v, sk, sv, a, s);
+  }
   return rows_impl<D, 32>(k, v, sk, sv, a, s);
 }
 template <int D, bool ROWS>
