@@ -212,11 +212,14 @@ int64_t cross_part_bytes(int Z, int H, int Hk, int Nq, int Nk, int D, int dtype)
                            cross_split(Z, H, Hk, Nq, Nk, D, dtype));
 }
 
-// fp32: parts of the keys for dq, and where their sums stand behind the tiles' partials.
+// fp32: parts of the keys for dq, and where their sums stand behind the tiles' partials. As many CTAs as shared memory lets
+// run at a time; a part's beginning counts for nothing, as lengths may differ and smaller parts even them out (B3 H5, 200
+// queries of up to 777 keys: the backward 88 -> 79 us at D64, 70 -> 64 at D32, nothing lost with equal lengths; one block
+// for it: 88. Twice the CTAs at D64: 79, but 40 queries of 5,000 keys 71 -> 82).
 int dq_parts(int Z, int H, int Nq, int Nk, int D) {
   const int tile = window_f32_tile(D, (long long)Z * H, Nq);
   return rows_splits(int64_t(Z) * H * ((Nq + tile - 1) / tile), (int64_t(Nk) + kWindowF32Block - 1) / kWindowF32Block,
-                     2 * device_sm_count(), 1, 1);
+                     (D <= 32 ? 4 : 2) * device_sm_count(), 0, 1);
 }
 int64_t dq_part_bytes(int Z, int H, int Nq, int Nk, int D) {
   const int parts = dq_parts(Z, H, Nq, Nk, D);

@@ -1,6 +1,6 @@
 // Sliding-window attention with sinks for fp32 on CUDA cores: forward, dK/dV and dQ. The same kernels with ROWS are
 // attention to the first lengths[z] keys of a sequence (kMaskRows); their forward and dQ may take a part of the keys, so that
-// few rows still give every SM something to do (B3 H5, 200 queries of up to 777 keys, D64: dQ 62 -> 40 us; 40 queries of
+// few rows still give every SM something to do (B3 H5, 200 queries of up to 777 keys, D64: dQ 62 -> 27 us; 40 queries of
 // 5,000 keys, H4: the backward 399 -> 69). Up to 16 rows, a sampled prompt's, take T = 16 (R = 2: half the products
 // and less of shared memory; R = 4 with half the threads is between): 16 rows of 4,000 keys, B4 Hk4: D32 15.5 -> 12.6 us, D64
 // 25.4 -> 19.6, D128 54.6 -> 49.3 with the join; 16 rows of 500 keys, B32 H16: 71 -> 56 at D64, 165 -> 141 at D128.
