@@ -206,6 +206,20 @@ __device__ __forceinline__ void mma_f16_ts_elect(uint32_t d_tmem, uint32_t a_tme
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// The same for lanes [LANE0, LANE0 + LANES) of D alone (multiples of 32): the others keep what they hold.
+template <int LANE0, int LANES>
+__device__ __forceinline__ void mma_f16_ts_lanes_elect(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                                       uint32_t accumulate) {
+  static_assert(LANE0 % 32 == 0 && LANES % 32 == 0 && LANE0 + LANES <= 128, "whole warps' lanes");
+  constexpr auto off = [](int w) { return 32 * w >= LANE0 && 32 * w < LANE0 + LANES ? 0u : ~0u; };
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 rx;\n\t"
+      "elect.sync rx|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(off(0)), "r"(off(1)), "r"(off(2)), "r"(off(3))
+      : "memory");
+}
 __device__ __forceinline__ void mma_commit_elect(uint64_t* bar) {
   asm volatile(
       "{\n\t.reg .pred e;\n\t.reg .b32 rx;\n\t"

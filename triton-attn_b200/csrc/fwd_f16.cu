@@ -33,7 +33,8 @@
 // each, whose unnormalised rows rows_join.cu joins. B2 H16 Hk4, 2,000 queries of 6,404 keys, D128: 222 us, 0.89 PFLOP/s,
 // 256 CTAs for 148 SMs; B2 H16 N4096 D64: 197 us, 0.70 (the same as `attention`: 219): the softmax warps. 64 queries of 16,384
 // keys, H16 D64 (67 MB): 24.4 us, of which the keys' way at 5.8 TB/s takes 11.5, the first loads and the epilogue 3 each, the
-// join 4; there BN is 64 and each row has two (four) copies in the tile whose threads share a block's exponentials.
+// join 4; there BN is 64 and each row has two (four) copies in the tile whose threads share a block's exponentials: a copy
+// takes a share of the block's columns, and its lanes of O only the products of those (issue_pv_st).
 // The running max is rescaled lazily: O (in TMEM) and l are only corrected when a row's max grows by
 // more than kRescaleThreshold (log2 units); P values stay below 2^kRescaleThreshold, exact in fp16.
 // A NaN among a row's visible scores makes its maximum NaN, and with it M and O (the exponentials on the FMA pipe clamp,
@@ -135,25 +136,33 @@ __device__ __forceinline__ void issue_qk_stage(int st, int i, uint32_t d_tmem, u
   issue_qk_st<C, D, ST>(i, d_tmem, dQ, dK, idesc);
 }
 
-// O_i += P_i V for the V block in ring stage ST: BN/16 MMAs with P (fp16) read from TMEM.
-template <typename C, int D, int ST>
+// O_i += P_i V for the V block in ring stage ST: BN/16 MMAs with P (fp16) read from TMEM. COPIES: each adds to the lanes of
+// the copy whose columns it reads, and to no others. (Their weights are none of this copy's: even a P of zeros there would
+// make a NaN of an infinity in V.)
+template <typename C, int D, int COPIES, int ST, int KK = 0>
 __device__ __forceinline__ void issue_pv_st(uint32_t d_tmem, uint32_t p_tmem, uint64_t dV, uint32_t accumulate) {
-  asm volatile("" : "+l"(dV));
-#pragma unroll
-  for (int kk = 0; kk < C::BN / 16; ++kk)
-    mma_f16_ts_elect(d_tmem, p_tmem + kk * 8, dV + uint64_t((ST * C::KTILE + kk * 16 * C::SWB) >> 4), C::IDESC_PV,
-                     kk > 0 ? 1u : accumulate);
+  if constexpr (KK == 0) asm volatile("" : "+l"(dV));
+  if constexpr (KK < C::BN / 16) {
+    constexpr int STEPS = C::BN / 16 / COPIES;  // of a copy
+    const uint64_t dv = dV + uint64_t((ST * C::KTILE + KK * 16 * C::SWB) >> 4);
+    const uint32_t add = KK % STEPS > 0 ? 1u : accumulate;
+    if constexpr (COPIES == 1)
+      mma_f16_ts_elect(d_tmem, p_tmem + KK * 8, dv, C::IDESC_PV, add);
+    else
+      mma_f16_ts_lanes_elect<KK / STEPS * (128 / COPIES), 128 / COPIES>(d_tmem, p_tmem + KK * 8, dv, C::IDESC_PV, add);
+    issue_pv_st<C, D, COPIES, ST, KK + 1>(d_tmem, p_tmem, dV, accumulate);
+  }
 }
-template <typename C, int D, int ST = 0>
+template <typename C, int D, int COPIES, int ST = 0>
 __device__ __forceinline__ void issue_pv_stage(int st, uint32_t d_tmem, uint32_t p_tmem, uint64_t dV,
                                                uint32_t accumulate) {
   if constexpr (ST + 1 < C::NS) {
     if (st != ST) {
-      issue_pv_stage<C, D, ST + 1>(st, d_tmem, p_tmem, dV, accumulate);
+      issue_pv_stage<C, D, COPIES, ST + 1>(st, d_tmem, p_tmem, dV, accumulate);
       return;
     }
   }
-  issue_pv_st<C, D, ST>(d_tmem, p_tmem, dV, accumulate);
+  issue_pv_st<C, D, COPIES, ST>(d_tmem, p_tmem, dV, accumulate);
 }
 
 // kMaskWindow: the key blocks that a CTA goes through, j = 0 .. n - 1: those that hold sinks, then those from
@@ -625,7 +634,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
             break;
           }
           tc_fence_after();
-          issue_pv_stage<C, D>(j % C::NS, tO, tP, dV, j > 0 ? 1u : 0u);
+          issue_pv_stage<C, D, COPIES>(j % C::NS, tO, tP, dV, j > 0 ? 1u : 0u);
           mma_commit_elect(&bar_o_done[i]);
           mma_commit_elect(&bar_kv_empty[i * C::NS + j % C::NS]);
           if (j + 1 < n) {
@@ -655,7 +664,7 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
           break;
         }
         tc_fence_after();
-        issue_pv_stage<C, D>(j % C::NS, tO, tP, dV, j > 0 ? 1u : 0u);
+        issue_pv_stage<C, D, COPIES>(j % C::NS, tO, tP, dV, j > 0 ? 1u : 0u);
         mma_commit_elect(&bar_o_done[i]);
         mma_commit_elect(&bar_kv_empty[i * C::NS + j % C::NS]);
       }
@@ -688,12 +697,6 @@ __global__ void __launch_bounds__(128 * (TILES + 1), 3 - TILES)
       fence_proxy_async_smem();
       mbar_arrive(bar_q);
       if (args.rows.part != nullptr) let_next_kernel_start();  // the one that joins the parts, or comes before that
-      if (COPIES > 1 && n > 0) {  // the other copies' columns of P are zeros throughout
-        uint32_t zero[BN / 2];
-#pragma unroll
-        for (int c = 0; c < BN / 2; ++c) zero[c] = 0u;
-        tmem_store_cols<BN / 2>(tP, zero);
-      }
     }
     for (int j = 0; j < n; ++j) {
       // (behind the wait for S the registers are full)

@@ -21,7 +21,8 @@ def cross_attention(
     With ``lengths`` (int32 [batch], on the device) the queries of sequence b see the first lengths[b] keys only; where
     there are none the result is zeros. A length outside [0, kv_seq] counts as the nearer end and sets DEV_INDEX_RANGE in
     the device status word. Rows of k and v past a length are never used, whatever they hold, and their gradients are
-    zeros. Returns a tensor like q; gradients reach q, k and v, once and in reverse mode (forward-mode tensors are
+    zeros. An infinity in a row of v that is seen is one in the result, where its weight is above 0 (fp16: above 2^-25 of
+    the largest). Returns a tensor like q; gradients reach q, k and v, once and in reverse mode (forward-mode tensors are
     refused).
     """
     return _lib.torch_ext().cross_attention(q, k, v, lengths, sm_scale)
