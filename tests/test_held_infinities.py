@@ -70,6 +70,32 @@ def test_cross_attention(gpu, nq, nk, held, d, dtype) -> None:
 @pytest.mark.gpu
 @F16_F32
 @pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("where", ["v", "do"])
+@pytest.mark.parametrize("nq, nk, held", [(1, 300, 289), (20, 3000, 2900), (33, 300, 289), (129, 300, 289), (300, 1300, 1200)])
+def test_cross_attention_gradients(gpu, nq, nk, held, where, d, dtype) -> None:
+    """dV does not read V, and a dim of it reads that dim of dO alone; the other heads and sequences have finite gradients
+    throughout."""
+    q, do = _rows(2, 4, nq, d, dtype=dtype, seed=1), _rows(2, 4, nq, d, dtype=dtype, seed=2)
+    k, v = _rows(2, 2, nk, d, dtype=dtype, seed=3), _rows(2, 2, nk, d, dtype=dtype, seed=4)
+    if where == "v":
+        _plant(v, 70, held - 1)
+    else:  # (of a query head of the second key/value head)
+        do[0, 3, nq // 2, 2], do[0, 3, nq // 2, 3] = math.inf, -math.inf
+    lengths = torch.tensor([held, nk], dtype=torch.int32, device="cuda")
+    want, bounds = cross_attention64(q, k, v, do, lengths, d**-0.5)
+    args = [t.detach().requires_grad_() for t in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(cross_attention(*args, lengths), args, do)
+    seen = torch.arange(nk, device="cuda") < lengths[:, None]
+    want_dv = torch.where(seen[:, None, :, None], want[3], torch.zeros_like(want[3]))  # (0 x infinity in the definition's sum)
+    _same(dv, want_dv, bounds[3], "dv")
+    for got, i, heads in ((dq, 1, 2), (dk, 2, 1)):
+        assert_within(got[0, :heads], want[i][0, :heads], bounds[i][0, :heads], "dq, dk of the other heads")
+        assert_within(got[1], want[i][1], bounds[i][1], "dq, dk of the other sequence")
+
+
+@pytest.mark.gpu
+@F16_F32
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
 @pytest.mark.parametrize("where", ["prefix", "own"])
 @pytest.mark.parametrize("samples", [1, 3, 16, 20, 32, 33, 70])
 def test_prefix_decode_attention(gpu, samples, where, d, dtype) -> None:

@@ -1791,14 +1791,17 @@ struct FusedCfg {
   // -M/qk_scale and -delta of each query of a ring slot, each as an exact sum of three bf16 parts, as
   // the B operand [128 queries x 16 K] (no swizzle; K columns 0-2 = the -M parts, 3-5 = the -delta
   // parts, 6-7 zero) of one extra K = 16 step of the S^T and dP^T MMAs. Only 8 K columns are stored: the
-  // step's upper 8 read the same bytes (LBO = 0), against zeros in the A operand.
+  // step's upper 8 read the same bytes (LBO = 0), against zeros in the A operand. kMaskRows: the -delta parts stand apart,
+  // in K columns 0-2 of a slot of their own, so that an infinite delta meets no zero beside S^T.
   static constexpr int MD_SLOT = BQ * 16;
   static constexpr int OFF_MD = OFF_STG + 8 * STG;        // NS x MD_SLOT
   // The A operands of that step, [128 keys x 16 K] bf16 (no swizzle): ones in K columns 0-2 (S^T) or
-  // 3-5 (dP^T), zeros elsewhere, so the step adds -M/qk_scale to S^T and -delta to dP^T.
+  // 3-5 (dP^T), zeros elsewhere, so the step adds -M/qk_scale to S^T and -delta to dP^T. kMaskRows: the first one alone,
+  // and the -delta parts' slots in the second one's place.
   static constexpr int ONES_TILE = 128 * 32;
-  static constexpr int OFF_ONES = OFF_MD + NS * MD_SLOT;  // 2 x ONES_TILE
-  static constexpr int OFF_BAR = OFF_ONES + 2 * ONES_TILE;
+  static constexpr int OFF_ONES = OFF_MD + NS * MD_SLOT;  // ONES_TILE, then ONES_TILE or NS x MD_SLOT
+  static constexpr int OFF_DELTA = OFF_ONES + ONES_TILE;
+  static constexpr int OFF_BAR = OFF_DELTA + (ONES_TILE > NS * MD_SLOT ? ONES_TILE : NS * MD_SLOT);
   // k_full[2], k_empty[2], q_full[NS], md_full[NS], q_empty[NS], s_full, s_free, p_full, acc_free,
   // acc_done, acc_read, fin[3], dq_read, v_full, v_empty
   static constexpr int NBARS = 4 + 3 * NS + 12;
@@ -2270,7 +2273,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   // The constant A operands of the folded -M / -delta step (bf16 1.0 = 0x3F80): in every 8-row group,
   // bytes [0, 128) hold K columns 0-7 of the 8 rows (16 bytes a row), bytes [128, 256) columns 8-15.
-  for (int idx = threadIdx.x; idx < 2 * C::ONES_TILE / 16; idx += blockDim.x) {
+  for (int idx = threadIdx.x; idx < (ROWS ? 1 : 2) * C::ONES_TILE / 16; idx += blockDim.x) {
     const int t = idx / (C::ONES_TILE / 16), byte = (idx % (C::ONES_TILE / 16)) * 16;
     const bool low_k = (byte % 256) < 128;
     const uint4 row = t == 0 ? make_uint4(0x3F803F80u, 0x00003F80u, 0u, 0u)   // K 0-2: the -M parts
@@ -2326,8 +2329,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t hm[3], hd[3];
             split_bf16x3(q < N ? -mrow[q] * inv_scale : 0.f, hm);
             split_bf16x3(q < N ? -drow[q] : 0.f, hd);
-            *reinterpret_cast<uint4*>(slot + j * 16) =
-                make_uint4(hm[0] | (hm[1] << 16), hm[2] | (hd[0] << 16), hd[1] | (hd[2] << 16), 0u);
+            if constexpr (ROWS) {
+              *reinterpret_cast<uint4*>(slot + j * 16) = make_uint4(hm[0] | (hm[1] << 16), hm[2], 0u, 0u);
+              *reinterpret_cast<uint4*>(smem + C::OFF_DELTA + st * C::MD_SLOT + j * 16) = make_uint4(hd[0] | (hd[1] << 16), hd[2], 0u, 0u);
+            } else {
+              *reinterpret_cast<uint4*>(slot + j * 16) =
+                  make_uint4(hm[0] | (hm[1] << 16), hm[2] | (hd[0] << 16), hd[1] | (hd[2] << 16), 0u);
+            }
           }
           fence_proxy_async_smem();  // read by the S^T / dP^T MMAs through the async proxy
           mbar_arrive(&bar_md_full[st]);
@@ -2349,8 +2357,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       // 8-row groups 256), B = the slot's parts (no swizzle: 8-query groups 128 bytes apart, the upper
       // K core matrix the same bytes).
       const uint64_t dOnesM = smem_desc(base_u32 + C::OFF_ONES, 128, 256, 0u);
-      const uint64_t dOnesD = smem_desc(base_u32 + C::OFF_ONES + C::ONES_TILE, 128, 256, 0u);
+      const uint64_t dOnesD = ROWS ? dOnesM : smem_desc(base_u32 + C::OFF_ONES + C::ONES_TILE, 128, 256, 0u);
       const uint64_t dMD = smem_desc(base_u32 + C::OFF_MD, 0, 128, 0u);
+      const uint64_t dDelta = ROWS ? smem_desc(base_u32 + C::OFF_DELTA, 0, 128, 0u) : dMD;
       int g = 0, it = 0;
       bool ok = true;
       int2 seq = make_int2(int(blockIdx.x), 0);
@@ -2375,7 +2384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           mma_kmajor<D, G::chunk(128), G::chunk(BQ)>(tmem + C::T_ST, dK + ko, dQ + so, idesc_s);
           mma_f16_ss_elect(tmem + C::T_ST, dOnesM, dMD + mo, C::IDESC_MD, 1u);
           mma_kmajor<D, G::chunk(128), G::chunk(BQ)>(tmem + C::T_DPT, dV, dDO + so, C::IDESC_S);
-          mma_f16_ss_elect(tmem + C::T_DPT, dOnesD, dMD + mo, C::IDESC_MD, 1u);
+          mma_f16_ss_elect(tmem + C::T_DPT, dOnesD, dDelta + mo, C::IDESC_MD, 1u);
           mma_commit_elect(bar_s_full);
           mma_commit_elect(&bar_q_empty[g % NS]);
         }
