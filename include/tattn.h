@@ -52,7 +52,7 @@ enum tattn_status {
   TATTN_ERR_NO_DEVICE = 4,        /* current device is not sm_100 or the TMA encoder is missing */
   TATTN_ERR_DEVICE_STATUS = 5,    /* a kernel recorded a failure in the device status word */
   TATTN_ERR_UNSUPPORTED = 6,      /* valid request this build does not implement */
-  TATTN_ERR_TOO_LARGE = 7         /* problem exceeds a fixed-size library buffer (tattn_bwd_noalloc) */
+  TATTN_ERR_TOO_LARGE = 7         /* sizes above the limit that the call states */
 };
 
 /* Device status word bits (tattn_device_status). */
@@ -226,7 +226,8 @@ TATTN_API int64_t tattn_int4_decode_workspace_bytes(int Z, int H, int Hk, int C,
  * m: fp32 [Z, H, Nq], rowmax + log2(rowsum) in base-2 units (-infinity: no keys), and o_rest (fp16: what rounding O took
  * off, dense [Z, H, Nq, D] bytes, as tattn_window_fwd's) are for the backward; either may be null. strides: 16 int64 =
  * q, k, v, o each (z, h, n, d); rows need unit D stride and 16-byte alignment (TATTN_ERR_LAYOUT). workspace:
- * tattn_cross_fwd_workspace_bytes bytes, 16-byte aligned (0 bytes: may be null). */
+ * tattn_cross_fwd_workspace_bytes bytes, 16-byte aligned (0 bytes: may be null). Nk and Nq * H / Hk up to 2^29; Z * H *
+ * Nq < 10^9 and Z * Hk * (Nk / 128 + 1) < 10^7 (TATTN_ERR_TOO_LARGE), forward and backward. */
 TATTN_API int tattn_cross_fwd(const void* q, const void* k, const void* v, const int32_t* lengths, void* o, float* m,
                     void* o_rest, void* workspace, const int64_t* strides, int Z, int H, int Hk, int Nq, int Nk, int D,
                     int dtype, float sm_scale, void* stream);
@@ -249,7 +250,8 @@ TATTN_API int64_t tattn_cross_bwd_workspace_bytes(int Z, int H, int Hk, int Nq, 
  * samples, Hk, C, D], the sequences' own tokens behind it, of which sequence b holds lengths[b] (device int32). The query
  * sees all of both; nothing held gives zeros. Lengths outside their range, and rows past a length, as in tattn_decode.
  * strides: 24 int64 = q, prefix_k, prefix_v, k, v, o each (z, h, n, d); rows need unit D stride and 16-byte alignment.
- * workspace: tattn_prefix_decode_workspace_bytes bytes, 16-byte aligned. */
+ * workspace: tattn_prefix_decode_workspace_bytes bytes, 16-byte aligned. P up to 2^29, C up to 2^30; prompts * samples * H
+ * < 5 * 10^8 and prompts * Hk * (P / 128 + 1) < 10^7 (TATTN_ERR_TOO_LARGE). */
 TATTN_API int tattn_prefix_decode(const void* q, const void* prefix_k, const void* prefix_v, const int32_t* prefix_lengths,
                         const void* k, const void* v, const int32_t* lengths, void* o, void* workspace,
                         const int64_t* strides, int prompts, int samples, int H, int Hk, int P, int C, int D, int dtype,

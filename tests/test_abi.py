@@ -120,3 +120,15 @@ def test_fused_workspace_size(lib: ctypes.CDLL) -> None:
     assert lib.tattn_bwd_fused_workspace_bytes(1, 1, 8, 48) == -1
     assert lib.tattn_bwd_fused_workspace_bytes(-1, 1, 8, 64) == -1
     assert lib.tattn_bwd_fused_workspace_bytes(1 << 30, 1 << 30, 1 << 30, 64) == -1
+
+
+def test_a_size_above_a_limit_is_named_as_such(lib: ctypes.CDLL) -> None:
+    """Several calls have one, so the text is not about the buffer of one of them alone, and the header states each."""
+    strides = _lib.strides_array(*[(8 * 16, 8 * 16, 16, 1)] * 6)
+    large = 1 << 20, 2, 2, 1 << 10, 9, 16, 0
+    assert lib.tattn_cross_fwd(*[16] * 8, strides, *large, 0.1, None) == _lib.ERR_TOO_LARGE
+    assert lib.tattn_prefix_decode(*[16] * 9, strides, 1 << 15, 1 << 15, 2, 2, 8, 8, 16, 0, 0.1, None) == _lib.ERR_TOO_LARGE
+    assert _lib.status_string(_lib.ERR_TOO_LARGE).startswith("sizes above the call's limit in tattn.h")
+    calls = re.split(r"(?=/\*)", open(HEADER).read())
+    for name in ("tattn_qk_norm_rope", "tattn_cross_fwd", "tattn_prefix_decode", "tattn_bwd_noalloc"):
+        assert any(f" {name}(" in c and "TATTN_ERR_TOO_LARGE" in c for c in calls), name
