@@ -988,7 +988,8 @@ __device__ __forceinline__ void split_bf16x3(float v, uint32_t* h) {
 
 // P^T and dS^T for H query columns of one key row of the fused backward, whose S^T and dP^T already hold
 // S^T - M/qk_scale and dP^T - delta (folded into the MMAs): P = exp2(S'^T * qk_scale), dS = P * dP'^T.
-// MASK keeps only columns c_lo <= c < c_hi.
+// MASK keeps only columns c_lo <= c < c_hi. Both are rounded to fp16 for the MMAs, whose operands are 16 bits wide: up to
+// 2^-11 relative, and up to 2^-25 below 2^-14.
 template <int H, bool MASK>
 __device__ __forceinline__ void pds_row_folded(const uint32_t* s, const uint32_t* dp, uint32_t* pt, uint32_t* dst,
                                                uint64_t scale2, int c_lo, int c_hi) {

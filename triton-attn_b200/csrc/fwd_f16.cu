@@ -33,10 +33,10 @@
 // each, whose unnormalised rows rows_join.cu joins. B2 H16 Hk4, 2,000 queries of 6,404 keys, D128: 222 us, 0.89 PFLOP/s,
 // 256 CTAs for 148 SMs; B2 H16 N4096 D64: 197 us, 0.70 (the same as `attention`: 219): the softmax warps. 64 queries of 16,384
 // keys, H16 D64 (67 MB): 24.4 us, of which the keys' way at 5.8 TB/s takes 11.5, the first loads and the epilogue 3 each, the
-// join 4; there BN is 64 and each row has two (four) copies in the tile whose threads share a block's exponentials: a copy
+// join 3; there BN is 64 and each row has two (four) copies in the tile whose threads share a block's exponentials: a copy
 // takes a share of the block's columns, and its lanes of O only the products of those (issue_pv_st).
 // The running max is rescaled lazily: O (in TMEM) and l are only corrected when a row's max grows by
-// more than kRescaleThreshold (log2 units); P values stay below 2^kRescaleThreshold, exact in fp16.
+// more than kRescaleThreshold (log2 units); P values stay below 2^kRescaleThreshold, in fp16's range.
 // A NaN among a row's visible scores makes its maximum NaN, and with it M and O (the exponentials on the FMA pipe clamp,
 // which makes a weight of 0 of a NaN).
 #include <cuda_fp16.h>
@@ -293,7 +293,8 @@ __device__ __forceinline__ float row_max(const uint32_t* s, int lim) {
 }
 
 // One row of P = exp2(S * scale - m) for columns [C0, C1) as fp16 pairs (p[c/2] = columns c, c+1) and
-// its fp32 sum. kEmuPairs of every 8 column pairs use the FMA-pipe exp2, the rest MUFU. MASK zeroes
+// its fp32 sum. P is rounded to fp16 for the MMA, whose operands are 16 bits wide: up to 2^-11 relative a weight, as the
+// output's own rounding, and up to 2^-25 for one below 2^-14; the sum takes the weights as they were. kEmuPairs of every 8 column pairs use the FMA-pipe exp2, the rest MUFU. MASK zeroes
 // columns >= lim.
 template <int C0, int C1, bool MASK>
 __device__ __forceinline__ float exp_cols(const uint32_t* s, uint32_t* p, uint64_t scale2, uint64_t negm2, int lim) {

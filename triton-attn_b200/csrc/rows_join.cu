@@ -3,7 +3,8 @@
 //
 // A CTA takes one row, its threads 4 dims of every so many-th part. The parts were just written, so they come from L2; what
 // bounds it is its launch and the loads' latency, so it is launched while the last parts are made, and a thread's first
-// loads do not wait for the maximum (B200, 1,024 rows: 18 parts of 64 dims 4 us, 39 parts of 128 9 us in a call).
+// loads do not wait for the maximum. What it adds to a call (B200, 1,024 rows, the calls with and without it): 18 parts of 64
+// dims 3.2 us, 39 parts of 128 9.0 us.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <math.h>

@@ -1,9 +1,10 @@
 // Sliding-window attention with sinks for fp32 on CUDA cores: forward, dK/dV and dQ. The same kernels with ROWS are
 // attention to the first lengths[z] keys of a sequence (kMaskRows); their forward and dQ may take a part of the keys, so that
 // few rows still give every SM something to do (B3 H5, 200 queries of up to 777 keys, D64: dQ 62 -> 27 us; 40 queries of
-// 5,000 keys, H4: the backward 399 -> 69). Up to 16 rows, a sampled prompt's, take T = 16 (R = 2: half the products
-// and less of shared memory; R = 4 with half the threads is between): 16 rows of 4,000 keys, B4 Hk4: D32 15.5 -> 12.6 us, D64
-// 25.4 -> 19.6, D128 54.6 -> 49.3 with the join; 16 rows of 500 keys, B32 H16: 71 -> 56 at D64, 165 -> 141 at D128.
+// 5,000 keys, H4: the backward 399 -> 69). Up to 16 rows, a sampled prompt's, of heads too few for T = 64 (window_f32_tile)
+// take T = 16 (R = 2: half the products and less of shared memory; R = 4 with half the threads is between): 16 rows of
+// 4,000 keys, B4 Hk4: D32 15.5 -> 12.6 us, D64 25.4 -> 19.6, D128 54.6 -> 49.3 with the join; 16 rows of 500 keys, B32 H16: 71 ->
+// 56 at D64, 165 -> 141 at D128.
 //
 // The mathematics is the fp16 kernels' (base-2 online softmax, M = m + log2 l, P rebuilt from M in the
 // backward) with every product and sum in fp32: tcgen05 has no fp32 MMA, and fp32 calls are held to fp32

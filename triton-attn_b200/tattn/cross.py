@@ -23,6 +23,7 @@ def cross_attention(
     the device status word. Rows of k and v past a length are never used, whatever they hold, and their gradients are
     zeros. An infinity in a row of v that is seen is one in the result, where its weight is above 0 (fp16: above 2^-25 of
     the largest). Returns a tensor like q; gradients reach q, k and v, once and in reverse mode (forward-mode tensors are
-    refused).
+    refused), and all three are computed where any is needed. Tensors that the kernels cannot address in place are copied
+    in each call: rows not contiguous or not 16-byte aligned and, in fp16, expanded ones (but k and v of single tokens).
     """
     return _lib.torch_ext().cross_attention(q, k, v, lengths, sm_scale)
