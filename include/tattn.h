@@ -225,9 +225,10 @@ TATTN_API int64_t tattn_int4_decode_workspace_bytes(int Z, int H, int Hk, int C,
  * as the nearer end and sets TATTN_DEV_INDEX_RANGE. Rows of k and v past a length are never used, whatever they hold.
  * m: fp32 [Z, H, Nq], rowmax + log2(rowsum) in base-2 units (-infinity: no keys), and o_rest (fp16: what rounding O took
  * off, dense [Z, H, Nq, D] bytes, as tattn_window_fwd's) are for the backward; either may be null. strides: 16 int64 =
- * q, k, v, o each (z, h, n, d); rows need unit D stride and 16-byte alignment (TATTN_ERR_LAYOUT). workspace:
- * tattn_cross_fwd_workspace_bytes bytes, 16-byte aligned (0 bytes: may be null). Nk and Nq * H / Hk up to 2^29; Z * H *
- * Nq < 10^9 and Z * Hk * (Nk / 128 + 1) < 10^7 (TATTN_ERR_TOO_LARGE), forward and backward. */
+ * q, k, v, o each (z, h, n, d); rows need unit D stride and 16-byte alignment and, in fp16 with m or with Nq > 1, k and v
+ * what tattn_layout_ok asks for, so no stride of 0 (TATTN_ERR_LAYOUT). workspace: tattn_cross_fwd_workspace_bytes bytes,
+ * 16-byte aligned (0 bytes: may be null). Nk and Nq * H / Hk up to 2^29; Z * H * Nq < 10^9 and Z * Hk * (Nk / 128 + 1) <
+ * 10^7 (TATTN_ERR_TOO_LARGE), forward and backward. */
 TATTN_API int tattn_cross_fwd(const void* q, const void* k, const void* v, const int32_t* lengths, void* o, float* m,
                     void* o_rest, void* workspace, const int64_t* strides, int Z, int H, int Hk, int Nq, int Nk, int D,
                     int dtype, float sm_scale, void* stream);
@@ -236,7 +237,8 @@ TATTN_API int64_t tattn_cross_fwd_workspace_bytes(int Z, int H, int Hk, int Nq, 
 
 /* Its backward: dq [Z, H, Nq, D] and dk, dv [Z, Hk, Nk, D], all dense, zeros in the rows past a length; m, o_rest (or
  * null) and o as the forward wrote them. strides: 20 int64 = q, k, v, o, dout each (z, h, n, d). delta: fp32 [Z, H, Nq].
- * workspace: tattn_cross_bwd_workspace_bytes bytes, 16-byte aligned (0 bytes: may be null). As tattn_window_bwd, fp16
+ * fp16: all five as tattn_layout_ok asks. workspace: tattn_cross_bwd_workspace_bytes bytes, 16-byte aligned (0 bytes: may be
+ * null). As tattn_window_bwd, fp16
  * sums dq in an order that varies from run to run. */
 TATTN_API int tattn_cross_bwd(const void* q, const void* k, const void* v, const int32_t* lengths, const void* o,
                     const void* dout, void* dq, void* dk, void* dv, const float* m, const void* o_rest, float* delta,
@@ -249,9 +251,10 @@ TATTN_API int64_t tattn_cross_bwd_workspace_bytes(int Z, int H, int Hk, int Nq, 
  * of which prompt p holds the first prefix_lengths[p] tokens (device int32 [prompts]; null: all P); k, v: [prompts *
  * samples, Hk, C, D], the sequences' own tokens behind it, of which sequence b holds lengths[b] (device int32). The query
  * sees all of both; nothing held gives zeros. Lengths outside their range, and rows past a length, as in tattn_decode.
- * strides: 24 int64 = q, prefix_k, prefix_v, k, v, o each (z, h, n, d); rows need unit D stride and 16-byte alignment.
- * workspace: tattn_prefix_decode_workspace_bytes bytes, 16-byte aligned. P up to 2^29, C up to 2^30; prompts * samples * H
- * < 5 * 10^8 and prompts * Hk * (P / 128 + 1) < 10^7 (TATTN_ERR_TOO_LARGE). */
+ * strides: 24 int64 = q, prefix_k, prefix_v, k, v, o each (z, h, n, d); rows need unit D stride and 16-byte alignment,
+ * an fp16 prefix what tattn_layout_ok asks for. workspace: tattn_prefix_decode_workspace_bytes bytes, 16-byte aligned.
+ * P up to 2^29, C up to 2^30; prompts * samples * H < 5 * 10^8 and prompts * Hk * (P / 128 + 1) < 10^7
+ * (TATTN_ERR_TOO_LARGE). */
 TATTN_API int tattn_prefix_decode(const void* q, const void* prefix_k, const void* prefix_v, const int32_t* prefix_lengths,
                         const void* k, const void* v, const int32_t* lengths, void* o, void* workspace,
                         const int64_t* strides, int prompts, int samples, int H, int Hk, int P, int C, int D, int dtype,

@@ -291,3 +291,21 @@ def test_captured_steps_with_lengths_that_change_and_two_streams(gpu, dtype) -> 
                 got.append(prefix_decode_attention(*call))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
+
+
+@pytest.mark.gpu
+@F16_F32
+@pytest.mark.parametrize("dim", [0, 1])
+def test_an_expanded_prefix(gpu, dim, dtype) -> None:
+    """Over prompts or heads: fp32 reads it in place; fp16 refuses it, and says why (its own tokens may be expanded)."""
+    q, pk, pv, k, v = _inputs(2, 3, 4, 2, 100, 30, 64, dtype)
+    pk, pv, k, v = (t.narrow(dim, 0, 1).expand_as(t) for t in (pk, pv, k, v))
+    lengths = _int([30, 1, 0, 7, 30, 5])
+    want = prefix_decode_attention(q, *(t.contiguous() for t in (pk, pv, k, v)), lengths)
+    assert torch.equal(prefix_decode_attention(q, pk.contiguous(), pv.contiguous(), k, v, lengths), want)
+    if dtype == torch.float32:
+        assert torch.equal(prefix_decode_attention(q, pk, pv, k, v, lengths), want)
+        return
+    for args in ((pk, pv.contiguous()), (pk.contiguous(), pv)):
+        with pytest.raises(ValueError, match="a prefix in float16 cannot be expanded"):
+            prefix_decode_attention(q, *args, k, v, lengths)

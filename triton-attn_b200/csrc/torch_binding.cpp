@@ -673,8 +673,11 @@ Tensor prefix_decode_attention(const Tensor& q0, const Tensor& pk, const Tensor&
   refuse_forward_mode("prefix_decode_attention", {&q0, &k, &v, &pk, &pv});
   require_cuda(q0);
   for (const Tensor* t : {&k, &v, &pk, &pv})
-    CHECK_VALUE(t->numel() == 0 || (rows16_ok(*t) && (t->scalar_type() != at::kHalf || t == &k || t == &v || tma_ok(*t))),
+    CHECK_VALUE(t->numel() == 0 || rows16_ok(*t),
                       "k, v and the prefix need contiguous, 16-byte aligned rows: a cache is read in place, never copied");
+  for (const Tensor* t : {&pk, &pv})  // (TMA takes no stride of 0)
+    CHECK_VALUE(t->numel() == 0 || t->scalar_type() != at::kHalf || tma_ok(*t),
+                      "a prefix in float16 cannot be expanded: it is read in place, never copied; got strides ", t->strides());
   const Tensor q = rows16(q0), lengths = lengths0.contiguous();
   Tensor o = like(q);
   if (o.numel() == 0) return o;

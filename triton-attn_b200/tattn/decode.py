@@ -43,8 +43,8 @@ def prefix_decode_attention(
     are [batch, kv_heads, capacity, dim] for a batch of prompts * samples sequences, those of a prompt one after another;
     of sequence b's own tokens, which stand behind its prompt, the first lengths[b] are held (int32 [batch], the query's
     own as the last). The query sees the whole prompt and all of its sequence's tokens; where none are held the result is
-    zeros. Lengths outside their ranges, rows past a length and the caches' layout are as for ``decode_attention``. An
-    infinity among the values is one in the result, as for ``cross_attention``.
+    zeros. Lengths outside their ranges, rows past a length and the caches' layout are as for ``decode_attention``, but
+    that a float16 prefix must not be expanded. An infinity among the values is one in the result, as for ``cross_attention``.
     """
     return _lib.torch_ext().prefix_decode_attention(q, prefix_k, prefix_v, k, v, lengths, prefix_lengths, sm_scale)
 
