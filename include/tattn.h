@@ -237,9 +237,8 @@ TATTN_API int64_t tattn_cross_fwd_workspace_bytes(int Z, int H, int Hk, int Nq, 
 
 /* Its backward: dq [Z, H, Nq, D] and dk, dv [Z, Hk, Nk, D], all dense, zeros in the rows past a length; m, o_rest (or
  * null) and o as the forward wrote them. strides: 20 int64 = q, k, v, o, dout each (z, h, n, d). delta: fp32 [Z, H, Nq].
- * fp16: all five as tattn_layout_ok asks. workspace: tattn_cross_bwd_workspace_bytes bytes, 16-byte aligned (0 bytes: may be
- * null). As tattn_window_bwd, fp16
- * sums dq in an order that varies from run to run. */
+ * fp16: all five as tattn_layout_ok asks. workspace: tattn_cross_bwd_workspace_bytes bytes, 16-byte aligned (0 bytes: may
+ * be null). As tattn_window_bwd, fp16 sums dq in an order that varies from run to run. */
 TATTN_API int tattn_cross_bwd(const void* q, const void* k, const void* v, const int32_t* lengths, const void* o,
                     const void* dout, void* dq, void* dk, void* dv, const float* m, const void* o_rest, float* delta,
                     void* workspace, const int64_t* strides, int Z, int H, int Hk, int Nq, int Nk, int D, int dtype,

@@ -1,5 +1,5 @@
 """What lies past a length at every head dim of ``tattn.cross_attention`` and ``tattn.prefix_decode_attention``, rows without
-a softmax beside rows that have one, and sizes past 65,535 heads and 2^32 bytes."""
+a softmax beside rows that have one, and sizes past 65,535 heads and 2^32 bytes (``tattn.qk_rope_axes`` too)."""
 
 from __future__ import annotations
 
@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from tattn import _lib, cross_attention, prefix_decode_attention
+from tattn import _lib, cross_attention, prefix_decode_attention, qk_rope_axes
 from tests.built import ensure_built
 from tests.plain64 import assert_within, cross_attention64
 
@@ -163,3 +163,38 @@ def test_gradients_past_32_bits(gpu, dtype) -> None:
         assert not bool(grads[1][-1, -1, held:].any()) and not bool(grads[2][-1, -1, held:].any())
         del q, k, v, do, o, grads, args, last, got
         torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@F16_F32
+@pytest.mark.parametrize("norm", [True, False], ids=["norm", "alone"])
+@pytest.mark.parametrize("layout", ["bhnd", "bnhd"])
+def test_rotation_past_32_bits(gpu, layout, norm, dtype) -> None:
+    """Bitwise the results of the last tokens by themselves: of more than 2^31 values, fp16, and 2^32 bytes, fp32."""
+    n, h, d = (1 << 17) + 5, 136 if dtype == torch.float16 else 68, 128
+    g = torch.Generator(device="cuda").manual_seed(1)
+
+    def make():
+        shape = (1, h, n, d) if layout == "bhnd" else (1, n, h, d)
+        t = torch.empty(shape, device="cuda", dtype=dtype).normal_(generator=g)
+        return t if layout == "bhnd" else t.transpose(1, 2)
+
+    q, dq = make(), make()
+    k, dk = (t[:, -1:].clone() for t in (q, dq))
+    angle = torch.rand((64, d // 2), generator=g, device="cuda") * 6
+    positions = torch.randint(0, 64, (3, n), generator=g, device="cuda", dtype=torch.int32)
+    weights = [1 + 0.1 * torch.randn(d, generator=g, device="cuda") for _ in range(2)] if norm else []
+    axes = [j % 3 for j in range(d // 2)]
+
+    def run(x, y, gx, gy, at):
+        x, y = (t.detach().requires_grad_() for t in (x, y))
+        outs = qk_rope_axes(x, y, angle.cos(), angle.sin(), at, axes, *weights)
+        return (*(o.detach() for o in outs), *torch.autograd.grad(outs, (x, y), (gx, gy)))
+
+    whole = run(q, k, dq, dk, positions)
+    last = slice(n - 300, n)
+    part = run(*(t[:, :, last] for t in (q, k, dq, dk)), positions[:, last])
+    for a, b, name in zip(whole, part, ("q", "k", "dq", "dk"), strict=True):
+        assert torch.equal(a[:, :, last], b), name
+    if not norm:  # the key head is the last query head
+        assert torch.equal(whole[0][:, -1], whole[1][:, 0])
